@@ -13,7 +13,7 @@ pool of pages in the cache's byte layout:
   value = s * (1 + code / 16) + o
 
 For a group of 32 channels with least and largest value lo, hi (each clamped
-to +-30000): s = f16((hi - lo) * 16/15), o = f16(lo - s) and
+to +-20000): s = f16((hi - lo) * 16/15), o = f16(lo - s) and
 code = clamp(round((x - o) * (16 / s) - 16), 0, 15).
 """
 
@@ -26,7 +26,7 @@ import torch
 own = False
 
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
-LIMIT = 30000.0
+LIMIT = 20000.0
 DEV = "cuda"
 
 
