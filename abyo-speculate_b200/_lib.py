@@ -97,6 +97,27 @@ class ModelDesc(ctypes.Structure):
                 ("damp_e4", ctypes.c_int), ("reserved", ctypes.c_int * 4)]
 
 
+class KV4Desc(ctypes.Structure):
+    """spec_kv4_desc (include/spec_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("device", "n_layers", "n_heads", "n_kv_heads", "head_dim", "page_tokens",
+                                            "n_pages", "rope_half")] + [("reserved", ctypes.c_int * 8)]
+
+
+class KV4Step(ctypes.Structure):
+    """spec_kv4_step (include/spec_b200.h)."""
+
+    _fields_ = [("n_seqs", ctypes.c_int), ("table_stride", ctypes.c_int)] + [
+        (n, ctypes.c_void_p) for n in ("kv_len", "n_rows", "page_table", "positions", "masks", "src_rows")]
+
+
+class KV4Rows(ctypes.Structure):
+    """spec_kv4_rows (include/spec_b200.h)."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("n_rows", ctypes.c_int64), ("dtype", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
 # (name, restype, argtypes) of every function declared in include/spec_b200.h
 SIGNATURES = [
     ("spec_load_gguf", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(LoadOpts), ctypes.POINTER(ctypes.c_void_p)]),
@@ -185,6 +206,18 @@ SIGNATURES = [
     ("spec_tp_size", ctypes.c_int, [ctypes.c_void_p]),
     ("spec_qmatmul_noalloc", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+    ("spec_kv4_pool_bytes", ctypes.c_int64, [ctypes.POINTER(KV4Desc)]),
+    ("spec_kv4_create", ctypes.c_int,
+     [ctypes.POINTER(KV4Desc), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+      ctypes.POINTER(ctypes.c_void_p)]),
+    ("spec_kv4_free", None, [ctypes.c_void_p]),
+    ("spec_kv4_batch_create", ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]),
+    ("spec_kv4_batch_free", None, [ctypes.c_void_p]),
+    ("spec_kv4_plan", ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(KV4Step), ctypes.c_void_p]),
+    ("spec_kv4_append", ctypes.c_int, [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 7),
+    ("spec_kv4_attend", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p]),
+    ("spec_kv4_status", ctypes.c_int, [ctypes.c_void_p]),
 ]
 
 _lib: Optional[ctypes.CDLL] = None

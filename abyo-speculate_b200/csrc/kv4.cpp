@@ -1,0 +1,484 @@
+// 4-bit paged KV cache: handles, the per-step plan, and the checks of every
+// argument that the kernels rely on.  A plan is validated on the host and kept
+// in device memory of the library's own, so the kernels need no bounds checks
+// on pages and slots.
+#include <limits.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "../../include/spec_b200.h"
+#include "kv4.h"
+#include "model.h"
+
+using namespace specb200;
+using namespace specb200::kv4;
+
+namespace {
+
+// What a cache handle and its batches share.
+struct Cache {
+  spec_kv4_desc d{};
+  uint8_t* pool = nullptr;
+  const float *cos = nullptr, *sin = nullptr;
+  int n_positions = 0;
+  int64_t layer_bytes() const {
+    return (int64_t)d.n_pages * d.n_kv_heads * block_bytes(d.page_tokens, d.head_dim);
+  }
+};
+
+int fail(int rc, const char* msg) {
+  set_thread_error(msg);
+  return rc;
+}
+template <class... A>
+int fail(int rc, const char* fmt, A... a) {
+  char msg[256];
+  snprintf(msg, sizeof msg, fmt, a...);
+  set_thread_error(msg);
+  return rc;
+}
+int fail_cuda(cudaError_t e, const char* what) {
+  return fail(e == cudaErrorMemoryAllocation ? SPEC_ERR_OOM : SPEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+int check_desc(const spec_kv4_desc* d) {
+  if (!d) return fail(SPEC_ERR_INVALID, "spec_kv4: null description");
+  if (d->head_dim != 64 && d->head_dim != 128)
+    return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4: head_dim %d (64 or 128 are built)", d->head_dim);
+  if (d->page_tokens != 16 && d->page_tokens != 32 && d->page_tokens != 64 && d->page_tokens != 128)
+    return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4: page_tokens %d (16, 32, 64 or 128 are built)", d->page_tokens);
+  if (d->n_layers < 1 || d->n_pages < 1 || d->n_kv_heads < 1 || d->n_kv_heads > 1024 || d->n_heads < d->n_kv_heads ||
+      d->n_heads > 4096 || d->n_heads % d->n_kv_heads)
+    return fail(SPEC_ERR_INVALID,
+                "spec_kv4: n_layers %d, n_pages %d, n_heads %d, n_kv_heads %d: positive counts, n_heads a multiple of "
+                "n_kv_heads, at most 4096 and 1024",
+                d->n_layers, d->n_pages, d->n_heads, d->n_kv_heads);
+  if (d->device < 0) return fail(SPEC_ERR_INVALID, "spec_kv4: device %d", d->device);
+  const int64_t block = block_bytes(d->page_tokens, d->head_dim);
+  if ((int64_t)d->n_pages * d->n_kv_heads > INT64_MAX / 2 / block / d->n_layers)
+    return fail(SPEC_ERR_INVALID, "spec_kv4: the pool's size passes 63 bits");
+  return SPEC_OK;
+}
+
+}  // namespace
+
+struct spec_kv4 {
+  std::shared_ptr<Cache> c;
+};
+
+struct spec_kv4_batch {
+  std::shared_ptr<Cache> c;
+  // The plan: one device allocation, written from one pinned one.
+  uint8_t *dev = nullptr, *host = nullptr;
+  size_t cap = 0;
+  unsigned* err = nullptr;
+  cudaEvent_t tail = nullptr, copied = nullptr;
+  unsigned long long last = 0;  // id of the stream of the previous call
+  bool planned = false, used = false;
+  int n_seqs = 0, n_rows = 0, max_src = -1;
+  int min_pos = 0, max_pos = -1;
+  bool has_src = false, has_masks = false;
+  const SeqDev* seqs = nullptr;
+  const RowDev* rows = nullptr;
+  const int *row_seq = nullptr, *table = nullptr;
+  const unsigned long long* masks = nullptr;
+  std::vector<uint8_t> seen;  // per page: 1 = read, 2 = written; zero between plans
+};
+
+namespace {
+
+bool capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+
+// Orders a call on `s` after the batch's previous call.
+cudaError_t enter(spec_kv4_batch* b, cudaStream_t s) {
+  if (!b->used || capturing(s)) return cudaSuccess;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetId(s, &id);
+  if (e != cudaSuccess || id == b->last) return e;
+  return cudaStreamWaitEvent(s, b->tail, 0);
+}
+cudaError_t leave(spec_kv4_batch* b, cudaStream_t s) {
+  if (capturing(s)) return cudaSuccess;
+  const cudaError_t e = cudaStreamGetId(s, &b->last);
+  if (e != cudaSuccess) return e;
+  b->used = true;
+  return cudaEventRecord(b->tail, s);
+}
+
+void release(spec_kv4_batch* b) {
+  if (b->used) cudaEventSynchronize(b->tail);
+  if (b->dev) cudaFree(b->dev);
+  if (b->host) cudaFreeHost(b->host);
+  if (b->err) cudaFree(b->err);
+  if (b->tail) cudaEventDestroy(b->tail);
+  if (b->copied) cudaEventDestroy(b->copied);
+}
+
+int check_rows(const char* what, const spec_kv4_rows* r, int64_t need, int heads, int D, bool written) {
+  if (!r->ptr) return fail(SPEC_ERR_INVALID, "spec_kv4: %s has no data", what);
+  if (r->dtype < T_BF16 || r->dtype > T_F32) return fail(SPEC_ERR_INVALID, "spec_kv4: %s has type %d", what, r->dtype);
+  if (r->n_rows < need)
+    return fail(SPEC_ERR_INVALID, "spec_kv4: %s has %lld rows, the plan needs %lld", what, (long long)r->n_rows,
+                (long long)need);
+  const int64_t lim = INT64_C(1) << 40;
+  if (r->row_stride < 0 || r->head_stride < 0 || r->row_stride > lim || r->head_stride > lim)
+    return fail(SPEC_ERR_INVALID, "spec_kv4: %s has a stride outside [0, 2^40]", what);
+  if (reinterpret_cast<uintptr_t>(r->ptr) % (r->dtype == T_F32 ? 4 : 2))
+    return fail(SPEC_ERR_INVALID, "spec_kv4: %s is not aligned to its element size", what);
+  // Outputs must not overlap themselves.
+  if (written && heads > 1 && r->head_stride < D)
+    return fail(SPEC_ERR_INVALID, "spec_kv4: heads of %s overlap (stride %lld)", what, (long long)r->head_stride);
+  if (written && need > 1 && r->row_stride < D)
+    return fail(SPEC_ERR_INVALID, "spec_kv4: rows of %s overlap (stride %lld)", what, (long long)r->row_stride);
+  return SPEC_OK;
+}
+
+Rows to_rows(const spec_kv4_rows* r) {
+  Rows o;
+  if (r) {
+    o.ptr = r->ptr;
+    o.row_stride = r->row_stride;
+    o.head_stride = r->head_stride;
+    o.dtype = r->dtype;
+  }
+  return o;
+}
+
+// Whether 8 consecutive channels are one (f32: two) aligned 16-byte access.
+bool wide(const spec_kv4_rows* r) {
+  if (!r) return true;
+  const int64_t sz = r->dtype == T_F32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(r->ptr) % 16 == 0 && r->row_stride * sz % 16 == 0 && r->head_stride * sz % 16 == 0;
+}
+
+int make_current(int device) {
+  int cur = -1;
+  if (cudaGetDevice(&cur) != cudaSuccess || cur != device) return fail(SPEC_ERR_CUDA, "spec_kv4: cudaSetDevice failed");
+  return SPEC_OK;
+}
+
+size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
+  const Cache& c = *b->c;
+  const int P = c.d.page_tokens;
+  if (s->n_seqs < 0 || (s->n_seqs > 0 && (!s->kv_len || !s->n_rows || !s->page_table || s->table_stride < 1)))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_plan: null array or negative count");
+  // Lengths.
+  int64_t rows = 0, pages = 0;
+  for (int i = 0; i < s->n_seqs; ++i) {
+    const int64_t n = s->kv_len[i], m = s->n_rows[i];
+    if (n < 0 || m < 0 || n + m > (int64_t)s->table_stride * P || n + m > INT_MAX - 1024)
+      return fail(SPEC_ERR_INVALID, "spec_kv4_plan: sequence %d: %lld tokens and %lld rows do not fit %d pages of %d", i,
+                  (long long)n, (long long)m, s->table_stride, P);
+    if (s->masks && m > 64)
+      return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4_plan: sequence %d: masks cover at most 64 rows, got %lld", i,
+                  (long long)m);
+    rows += m;
+    pages += (n + m + P - 1) / P;
+  }
+  if (rows > (1 << 24)) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: %lld rows (at most 2^24)", (long long)rows);
+  if (pages > (INT64_C(1) << 28)) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: page tables of %lld entries", (long long)pages);
+  // Pages: inside the pool, and a page that is written is listed once.
+  b->seen.resize(c.d.n_pages, 0);
+  int rc = SPEC_OK, done = 0;
+  for (; done < s->n_seqs && rc == SPEC_OK; ++done) {
+    const int32_t* t = s->page_table + (int64_t)done * s->table_stride;
+    const int n = s->kv_len[done], m = s->n_rows[done], np = (n + m + P - 1) / P, w0 = m ? n / P : np;
+    for (int i = 0; i < np; ++i) {
+      if (t[i] < 0 || t[i] >= c.d.n_pages) {
+        rc = fail(SPEC_ERR_INVALID, "spec_kv4_plan: sequence %d lists page %d of a pool of %d", done, t[i], c.d.n_pages);
+        break;
+      }
+      uint8_t& f = b->seen[t[i]];
+      if (i >= w0 ? f != 0 : f == 2) {
+        rc = fail(SPEC_ERR_INVALID, "spec_kv4_plan: page %d is written by one sequence and listed again", t[i]);
+        break;
+      }
+      f = i >= w0 ? 2 : 1;
+    }
+  }
+  for (int q = 0; q < done; ++q) {
+    const int32_t* t = s->page_table + (int64_t)q * s->table_stride;
+    const int np = (s->kv_len[q] + s->n_rows[q] + P - 1) / P;
+    for (int i = 0; i < np; ++i)
+      if (t[i] >= 0 && t[i] < c.d.n_pages) b->seen[t[i]] = 0;
+  }
+  if (rc != SPEC_OK) return rc;
+  int min_pos = INT_MAX, max_pos = -1, max_src = -1;
+  for (int64_t r = 0; r < rows; ++r) {
+    if (s->src_rows) {
+      if (s->src_rows[r] < 0) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: src_rows[%lld] is negative", (long long)r);
+      if (s->src_rows[r] > max_src) max_src = s->src_rows[r];
+    }
+  }
+  if (!s->src_rows) max_src = (int)rows - 1;
+
+  // One block: sequences, rows, row -> sequence, masks, pages.
+  const size_t at_seqs = 0, at_rows = at_seqs + up(sizeof(SeqDev) * s->n_seqs),
+               at_rseq = at_rows + up(sizeof(RowDev) * rows), at_masks = at_rseq + up(4 * rows),
+               at_table = at_masks + (s->masks ? up(8 * rows) : 0), total = at_table + up(4 * pages);
+  cudaError_t e = enter(b, stream);
+  if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+  if (total > b->cap) {
+    // The old plan's readers and its upload are done before it goes.
+    if (b->used && (e = cudaEventSynchronize(b->tail)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+    b->planned = false;
+    if (b->dev) cudaFree(b->dev);
+    if (b->host) cudaFreeHost(b->host);
+    b->dev = b->host = nullptr;
+    b->cap = 0;
+    const size_t cap = total + total / 2;
+    if ((e = cudaMalloc(reinterpret_cast<void**>(&b->dev), cap)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+    if ((e = cudaMallocHost(reinterpret_cast<void**>(&b->host), cap)) != cudaSuccess) {
+      cudaFree(b->dev);
+      b->dev = nullptr;
+      return fail_cuda(e, "spec_kv4_plan");
+    }
+    b->cap = cap;
+  } else if (b->planned && (e = cudaEventSynchronize(b->copied)) != cudaSuccess) {
+    return fail_cuda(e, "spec_kv4_plan");  // the staging buffer is still being read
+  }
+  b->planned = false;
+  SeqDev* hs = reinterpret_cast<SeqDev*>(b->host + at_seqs);
+  RowDev* hr = reinterpret_cast<RowDev*>(b->host + at_rows);
+  int* hq = reinterpret_cast<int*>(b->host + at_rseq);
+  int* ht = reinterpret_cast<int*>(b->host + at_table);
+  int r = 0, tp = 0;
+  for (int q = 0; q < s->n_seqs; ++q) {
+    const int32_t* t = s->page_table + (int64_t)q * s->table_stride;
+    const int n = s->kv_len[q], m = s->n_rows[q], np = (n + m + P - 1) / P;
+    hs[q] = SeqDev{n, m, r, tp};
+    memcpy(ht + tp, t, sizeof(int) * np);
+    tp += np;
+    for (int i = 0; i < m; ++i, ++r) {
+      const int pos = s->positions ? s->positions[r] : n + i;
+      if (pos < min_pos) min_pos = pos;
+      if (pos > max_pos) max_pos = pos;
+      hr[r] = RowDev{t[(n + i) / P], (n + i) % P, pos, s->src_rows ? s->src_rows[r] : r};
+      hq[r] = q;
+    }
+  }
+  if (s->masks) memcpy(b->host + at_masks, s->masks, 8 * (size_t)rows);
+  if (total && (e = cudaMemcpyAsync(b->dev, b->host, total, cudaMemcpyHostToDevice, stream)) != cudaSuccess)
+    return fail_cuda(e, "spec_kv4_plan");
+  if ((e = cudaEventRecord(b->copied, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+  if ((e = leave(b, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+  b->n_seqs = s->n_seqs;
+  b->n_rows = (int)rows;
+  b->max_src = max_src;
+  b->min_pos = rows ? min_pos : 0;
+  b->max_pos = max_pos;
+  b->has_src = s->src_rows != nullptr;
+  b->has_masks = s->masks != nullptr;
+  b->seqs = reinterpret_cast<const SeqDev*>(b->dev + at_seqs);
+  b->rows = reinterpret_cast<const RowDev*>(b->dev + at_rows);
+  b->row_seq = reinterpret_cast<const int*>(b->dev + at_rseq);
+  b->masks = s->masks ? reinterpret_cast<const unsigned long long*>(b->dev + at_masks) : nullptr;
+  b->table = reinterpret_cast<const int*>(b->dev + at_table);
+  b->planned = true;
+  return SPEC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t spec_kv4_pool_bytes(const spec_kv4_desc* d) {
+  const int rc = check_desc(d);
+  if (rc != SPEC_OK) return -rc;
+  return (int64_t)d->n_layers * d->n_pages * d->n_kv_heads * block_bytes(d->page_tokens, d->head_dim);
+}
+
+int spec_kv4_create(const spec_kv4_desc* d, void* pool_dev, int64_t pool_bytes, const float* cos_dev,
+                    const float* sin_dev, int n_positions, spec_kv4** out) {
+  if (!out) return fail(SPEC_ERR_INVALID, "spec_kv4_create: null argument");
+  *out = nullptr;
+  const int64_t need = spec_kv4_pool_bytes(d);
+  if (need < 0) return (int)-need;
+  if (!pool_dev || reinterpret_cast<uintptr_t>(pool_dev) % 128)
+    return fail(SPEC_ERR_INVALID, "spec_kv4_create: the pool is null or not 128-byte aligned");
+  if (pool_bytes < need)
+    return fail(SPEC_ERR_INVALID, "spec_kv4_create: the pool has %lld bytes, %lld are needed", (long long)pool_bytes,
+                (long long)need);
+  if (!cos_dev != !sin_dev || (cos_dev && n_positions < 1))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_create: both rotation tables or none, of at least one position");
+  if (reinterpret_cast<uintptr_t>(cos_dev) % 16 || reinterpret_cast<uintptr_t>(sin_dev) % 16)
+    return fail(SPEC_ERR_INVALID, "spec_kv4_create: the rotation tables are not 16-byte aligned");
+  try {
+    auto h = std::make_unique<spec_kv4>();
+    h->c = std::make_shared<Cache>();
+    h->c->d = *d;
+    h->c->pool = static_cast<uint8_t*>(pool_dev);
+    h->c->cos = cos_dev;
+    h->c->sin = sin_dev;
+    h->c->n_positions = cos_dev ? n_positions : 0;
+    *out = h.release();
+  } catch (const std::bad_alloc&) {
+    return fail(SPEC_ERR_OOM, "spec_kv4_create: out of host memory");
+  }
+  return SPEC_OK;
+}
+
+void spec_kv4_free(spec_kv4* c) { delete c; }
+
+int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
+  if (!c || !out) return fail(SPEC_ERR_INVALID, "spec_kv4_batch_create: null argument");
+  *out = nullptr;
+  DeviceGuard dg(c->c->d.device);
+  int rc = make_current(c->c->d.device);
+  if (rc != SPEC_OK) return rc;
+  spec_kv4_batch* b = new (std::nothrow) spec_kv4_batch;
+  if (!b) return fail(SPEC_ERR_OOM, "spec_kv4_batch_create: out of host memory");
+  b->c = c->c;
+  cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
+  if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
+  if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&b->err), 16);
+  if (e == cudaSuccess) e = cudaMemset(b->err, 0, 16);
+  if (e != cudaSuccess) {
+    release(b);
+    delete b;
+    return fail_cuda(e, "spec_kv4_batch_create");
+  }
+  *out = b;
+  return SPEC_OK;
+}
+
+void spec_kv4_batch_free(spec_kv4_batch* b) {
+  if (!b) return;
+  DeviceGuard dg(b->c->d.device);
+  release(b);
+  delete b;
+}
+
+int spec_kv4_plan(spec_kv4_batch* b, const spec_kv4_step* s, void* stream) {
+  if (!b || !s) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: null argument");
+  DeviceGuard dg(b->c->d.device);
+  int rc = make_current(b->c->d.device);
+  if (rc != SPEC_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (capturing(st)) return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4_plan: the stream is under capture");
+  try {
+    return plan(b, s, st);
+  } catch (const std::bad_alloc&) {
+    return fail(SPEC_ERR_OOM, "spec_kv4_plan: out of host memory");
+  }
+}
+
+int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* q_out,
+                    const spec_kv4_rows* k, const spec_kv4_rows* v, const spec_kv4_rows* k_out,
+                    const spec_kv4_rows* v_out, void* stream) {
+  if (!b || !k || !v || !q != !q_out) return fail(SPEC_ERR_INVALID, "spec_kv4_append: null argument, or q without q_out");
+  if (!b->planned) return fail(SPEC_ERR_INVALID, "spec_kv4_append: no plan");
+  const Cache& c = *b->c;
+  if (layer < 0 || layer >= c.d.n_layers)
+    return fail(SPEC_ERR_INVALID, "spec_kv4_append: layer %d of %d", layer, c.d.n_layers);
+  if (b->n_rows == 0) return SPEC_OK;
+  const int64_t src = (int64_t)b->max_src + 1, n = b->n_rows;
+  const int D = c.d.head_dim, hq = c.d.n_heads, hk = c.d.n_kv_heads;
+  int rc = check_rows("k", k, src, hk, D, false);
+  if (rc == SPEC_OK) rc = check_rows("v", v, src, hk, D, false);
+  if (rc == SPEC_OK && q) rc = check_rows("q", q, src, hq, D, false);
+  if (rc == SPEC_OK && q_out) rc = check_rows("q_out", q_out, n, hq, D, true);
+  if (rc == SPEC_OK && k_out) rc = check_rows("k_out", k_out, n, hk, D, true);
+  if (rc == SPEC_OK && v_out) rc = check_rows("v_out", v_out, n, hk, D, true);
+  if (rc != SPEC_OK) return rc;
+  if ((k_out && k_out->dtype != T_F16) || (v_out && v_out->dtype != T_F16))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_append: k_out and v_out are f16");
+  if (q && q->ptr == q_out->ptr &&
+      (b->has_src || q->dtype != q_out->dtype || q->row_stride != q_out->row_stride || q->head_stride != q_out->head_stride))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_append: q in place needs one type, one layout and no src_rows");
+  if (c.cos && (b->min_pos < 0 || b->max_pos >= c.n_positions))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_append: positions %d to %d, the rotation tables have %d", b->min_pos, b->max_pos,
+                c.n_positions);
+  DeviceGuard dg(c.d.device);
+  rc = make_current(c.d.device);
+  if (rc != SPEC_OK) return rc;
+  AppendParams p;
+  p.pool = c.pool + layer * c.layer_bytes();
+  p.cos = c.cos;
+  p.sin = c.sin;
+  p.rows = b->rows;
+  p.q = to_rows(q);
+  p.q_out = to_rows(q_out);
+  p.k = to_rows(k);
+  p.v = to_rows(v);
+  p.k_out = to_rows(k_out);
+  p.v_out = to_rows(v_out);
+  p.n_rows = b->n_rows;
+  p.n_heads = hq;
+  p.n_kv = hk;
+  p.P = c.d.page_tokens;
+  p.rope_half = c.d.rope_half ? 1 : 0;
+  p.wide_q = wide(q) && wide(q_out);
+  p.wide_k = wide(k);
+  p.wide_v = wide(v);
+  p.wide_ko = wide(k_out);
+  p.wide_vo = wide(v_out);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = enter(b, st);
+  if (e == cudaSuccess) e = launch_append(p, D, st);
+  if (e == cudaSuccess) e = leave(b, st);
+  return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_append");
+}
+
+int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* out, float scale,
+                    void* stream) {
+  if (!b || !q || !out) return fail(SPEC_ERR_INVALID, "spec_kv4_attend: null argument");
+  if (!b->planned) return fail(SPEC_ERR_INVALID, "spec_kv4_attend: no plan");
+  const Cache& c = *b->c;
+  if (layer < 0 || layer >= c.d.n_layers)
+    return fail(SPEC_ERR_INVALID, "spec_kv4_attend: layer %d of %d", layer, c.d.n_layers);
+  if (b->n_rows == 0) return SPEC_OK;
+  const int D = c.d.head_dim;
+  int rc = check_rows("q", q, b->n_rows, c.d.n_heads, D, false);
+  if (rc == SPEC_OK) rc = check_rows("out", out, b->n_rows, c.d.n_heads, D, true);
+  if (rc != SPEC_OK) return rc;
+  if (q->dtype == T_F32) return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4_attend: q is bf16 or f16");
+  if (!(scale == scale) || scale - scale != 0.f) return fail(SPEC_ERR_INVALID, "spec_kv4_attend: scale is not finite");
+  DeviceGuard dg(c.d.device);
+  rc = make_current(c.d.device);
+  if (rc != SPEC_OK) return rc;
+  AttendParams p;
+  p.pool = c.pool + layer * c.layer_bytes();
+  p.seqs = b->seqs;
+  p.table = b->table;
+  p.row_seq = b->row_seq;
+  p.masks = b->masks;
+  p.q = to_rows(q);
+  p.out = to_rows(out);
+  p.scale = scale;
+  p.n_rows = b->n_rows;
+  p.n_heads = c.d.n_heads;
+  p.n_kv = c.d.n_kv_heads;
+  p.P = c.d.page_tokens;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = enter(b, st);
+  if (e == cudaSuccess) e = launch_attend(p, D, st);
+  if (e == cudaSuccess) e = leave(b, st);
+  return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_attend");
+}
+
+int spec_kv4_status(spec_kv4_batch* b) {
+  if (!b) return fail(SPEC_ERR_INVALID, "spec_kv4_status: null argument");
+  DeviceGuard dg(b->c->d.device);
+  int rc = make_current(b->c->d.device);
+  if (rc != SPEC_OK) return rc;
+  if (b->used) {
+    const cudaError_t e = cudaEventSynchronize(b->tail);
+    if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_status");
+  }
+  char msg[256];
+  rc = take_device_error(b->err, nullptr, msg, sizeof msg);
+  if (rc != SPEC_OK) set_thread_error(msg);
+  return rc;
+}
+
+}  // extern "C"

@@ -1,0 +1,75 @@
+// 4-bit paged KV cache: what the host planner (kv4.cpp) and the kernels
+// (kv4_append.cu, kv4_attend.cu) share.  The byte layout of a page is
+// documented at spec_kv4 in include/spec_b200.h.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace specb200 {
+namespace kv4 {
+
+enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
+
+constexpr float kClamp = 20000.f;  // s = (hi - lo) * 16/15 and o = lo - s stay in f16 range
+constexpr int kGroup = 32;         // channels that share a scale pair
+
+// Byte offsets inside a block of P tokens of one kv head.
+__host__ __device__ constexpr int k_scales_at(int P, int D) { return P * D / 2; }
+__host__ __device__ constexpr int v_codes_at(int P, int D) { return P * D / 2 + P * D / 8; }
+__host__ __device__ constexpr int v_scales_at(int P, int D) { return P * D + P * D / 8; }
+__host__ __device__ constexpr int block_bytes(int P, int D) { return P * D + P * D / 4; }
+
+// Offset of 32-byte piece `piece` of token j's V codes inside the V code area.
+// A 128-byte line holds 2 (D = 128) or 4 (D = 64) tokens; the turn of its
+// quarters spreads tokens 0, 2, 4, 6 over all banks, which is how the
+// attention reads them.
+__host__ __device__ constexpr int v_piece_at(int D, int j, int piece) {
+  const int per = 256 / D;
+  const int line = j / per;
+  return line * 128 + 32 * (((j % per) * (D / 64) + piece) ^ (line % (D / 32)));
+}
+
+struct RowDev {
+  int page, slot;  // where the row is stored: page id, token within the page
+  int pos, src;    // rotation position, row of the input tensors
+};
+
+struct SeqDev {
+  int kv_len, n_rows;
+  int row0;   // first row of the sequence
+  int table;  // first entry of its pages in the plan's table
+};
+
+// Rows of heads (spec_kv4_rows).
+struct Rows {
+  void* ptr = nullptr;
+  long long row_stride = 0, head_stride = 0;
+  int dtype = 0;
+};
+
+struct AppendParams {
+  uint8_t* pool;  // of the layer
+  const float *cos, *sin;
+  const RowDev* rows;
+  Rows q, q_out, k, v, k_out, v_out;
+  int n_rows, n_heads, n_kv, P, rope_half;
+  int wide_q, wide_k, wide_v;  // inputs (and q_out) allow 16-byte accesses of 8 channels
+  int wide_ko, wide_vo;
+};
+cudaError_t launch_append(const AppendParams& p, int head_dim, cudaStream_t s);
+
+struct AttendParams {
+  const uint8_t* pool;  // of the layer
+  const SeqDev* seqs;
+  const int* table;
+  const int* row_seq;             // sequence of each row
+  const unsigned long long* masks;  // null: causal
+  Rows q, out;
+  float scale;
+  int n_rows, n_heads, n_kv, P;
+};
+cudaError_t launch_attend(const AttendParams& p, int head_dim, cudaStream_t s);
+
+}  // namespace kv4
+}  // namespace specb200

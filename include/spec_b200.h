@@ -485,6 +485,125 @@ int spec_qmatmul_time(spec_qweight* w, int M, int iters, int flush_l2, float* av
 #define SPEC_NOALLOC_SCRATCH_BYTES (16u << 20)
 int spec_qmatmul_noalloc(spec_qweight* w, const float* x_dev, int M, float* y_dev, void* stream);
 
+/* ---- 4-bit paged KV cache ---------------------------------------------------
+ * No counterpart in the reference (its cache is one contiguous 16-bit tensor a
+ * layer, crates/speculate/src/model/quantized_llama_local.rs:107-136).  For
+ * serving many sequences, or long ones, next to a speculative step: keys and
+ * values of all sequences live in one caller-owned device pool of pages,
+ * 5 bits an element (a 4-bit code and its share of a scale pair), and a step
+ * is one plan (which rows, where, what each row sees) shared by all layers:
+ *
+ *   spec_kv4_plan    once per step: lengths, page tables, tree masks
+ *   spec_kv4_append  per layer: rotate q and k, quantize k and v into the pages
+ *   spec_kv4_attend  per layer: softmax attention of the step's rows
+ *
+ * Pool: [layer][page][kv head][block].  A block holds page_tokens (P) tokens
+ * of one head (D = head_dim):
+ *   K codes   P rows of D/2 bytes; channel 2b is the low half of byte b
+ *   K scales  per token and group of 32 channels: f16 s, f16 o
+ *   V codes   rows of D/2 bytes, 256/D tokens to a 128-byte line: token j,
+ *             32-byte piece i of its row is quarter
+ *             ((j % (256/D)) * (D/64) + i) ^ ((j / (256/D)) % (D/32)) of its line
+ *   V scales  per pair of tokens and group: s, o of the even token, then of
+ *             the odd one
+ * value = s * (1 + code / 16) + o.  A group's x (f32 after the rotation,
+ * clamped to +-20000) has s = f16((hi - lo) * 16/15), o = f16(lo - s) and
+ * code = clamp(round((x - o) * (16 / s) - 16), 0, 15), every operation rounded
+ * by itself to f32.  A row of a head that holds a NaN is stored as NaN in
+ * every group (s = o = NaN, codes 0).
+ * A block is P * D * 5/4 bytes; a row's bytes are its own, so appending a row
+ * touches no other row.
+ *
+ * Conventions of these calls: every pointer marked "device" belongs to the
+ * caller; `stream` is the cudaStream_t the call's work is queued on (NULL =
+ * CUDA's default stream) and nothing is synchronised.  A batch handle orders
+ * its own calls: one made on another stream than the call before it waits for
+ * that call on the device.  Calls on a stream under capture are recorded
+ * without that ordering.  Messages: spec_last_error(NULL). */
+typedef struct spec_kv4 spec_kv4;
+typedef struct spec_kv4_batch spec_kv4_batch;
+typedef struct spec_kv4_desc {
+  int device;
+  int n_layers, n_heads, n_kv_heads; /* n_heads a multiple of n_kv_heads */
+  int head_dim;                      /* 64 or 128 */
+  int page_tokens;                   /* 16, 32, 64 or 128 */
+  int n_pages;
+  int rope_half;                     /* 1 = rotate-half pairs (i, i + D/2), 0 = neighbours (2i, 2i + 1) */
+  int reserved[8];
+} spec_kv4_desc;
+/* Bytes of the pool (a negated status on a bad description). */
+int64_t spec_kv4_pool_bytes(const spec_kv4_desc* d);
+/* pool_dev: device, 128-byte aligned, at least spec_kv4_pool_bytes; its
+ * contents are kept (an empty cache needs no clearing).  cos_dev / sin_dev:
+ * device, [n_positions][head_dim / 2] f32, 16-byte aligned, read by the
+ * appends; both NULL = no rotation.  The pool and the tables outlive the
+ * handle and its batches. */
+int spec_kv4_create(const spec_kv4_desc* d, void* pool_dev, int64_t pool_bytes, const float* cos_dev,
+                    const float* sin_dev, int n_positions, spec_kv4** out);
+void spec_kv4_free(spec_kv4* c);
+/* A batch handle: the plan of one step at a time and the attention's
+ * workspace.  One thread uses it at a time; it may outlive `c`'s handle. */
+int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out);
+void spec_kv4_batch_free(spec_kv4_batch* b);
+/* One step over n_seqs sequences (host arrays, copied before the call
+ * returns).  Sequence b holds kv_len[b] tokens and brings n_rows[b] >= 0 rows,
+ * which go to its slots kv_len[b] + i; rows are numbered sequence by sequence.
+ * Slot j of sequence b is in page page_table[b * table_stride + j / P].
+ * A row sees its sequence's first kv_len tokens and, of the step's rows, those
+ * whose bit is set in its mask (bit i = row i of the sequence; draft trees of
+ * at most 64 rows), or itself and the rows before it when masks is NULL.
+ * positions: rotation position of each row, NULL = kv_len[b] + i.
+ * src_rows: row of the append's input tensors each row is read from, NULL =
+ * its own number; committing an accepted tree path is an append of the
+ * accepted rows alone, kv_len as before the tree.
+ * Refused: a page outside the pool, a length past the table, and a page that
+ * a sequence writes and any table lists a second time. */
+typedef struct spec_kv4_step {
+  int n_seqs;
+  int table_stride;
+  const int32_t* kv_len;
+  const int32_t* n_rows;
+  const int32_t* page_table;
+  const int32_t* positions;
+  const uint64_t* masks;
+  const int32_t* src_rows;
+} spec_kv4_step;
+int spec_kv4_plan(spec_kv4_batch* b, const spec_kv4_step* s, void* stream);
+/* Rows of heads on the device: element (row, head, channel) is at
+ * ptr + row * row_stride + head * head_stride + channel (strides in elements;
+ * n_rows rows may be read or written).  Types: 0 = bf16, 1 = f16, 2 = f32. */
+#define SPEC_KV4_BF16 0
+#define SPEC_KV4_F16 1
+#define SPEC_KV4_F32 2
+typedef struct spec_kv4_rows {
+  void* ptr;
+  int64_t row_stride, head_stride;
+  int64_t n_rows;
+  int dtype;
+  int reserved;
+} spec_kv4_rows;
+/* Appends the step's rows to `layer`: k rotated and quantized, v quantized,
+ * and, when q is given, q rotated into q_out (which may be q itself, same type
+ * and strides, without src_rows).  q, k, v: any of the three types.  k_out /
+ * v_out (NULL, or f16): the values the stored rows stand for, rounded once to
+ * f16, for callers that go on with the new rows.  q and q_out: n_heads heads,
+ * the others n_kv_heads. */
+int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* q_out,
+                    const spec_kv4_rows* k, const spec_kv4_rows* v, const spec_kv4_rows* k_out,
+                    const spec_kv4_rows* v_out, void* stream);
+/* out = softmax(scale * q . k) v for every row and query head of the step
+ * over `layer`'s pages, whose rows of this step were appended before.  q: bf16
+ * or f16 rotated rows; out: any type.  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  Products take q and the stored values as f16
+ * (q after an exact power-of-two scaling of each row) and sum in f32.  A row
+ * that sees nothing gives zeros.  One call's result does not depend on
+ * timing; a row's last bits may depend on the other rows of the plan. */
+int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* out, float scale,
+                    void* stream);
+/* Synchronises the batch's last stream and reports (and clears) a device wait
+ * that gave up in an earlier call (SPEC_ERR_TIMEOUT). */
+int spec_kv4_status(spec_kv4_batch* b);
+
 #ifdef __cplusplus
 }
 #endif
