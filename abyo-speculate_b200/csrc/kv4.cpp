@@ -79,13 +79,23 @@ struct spec_kv4_batch {
   cudaEvent_t tail = nullptr, copied = nullptr;
   unsigned long long last = 0;  // id of the stream of the previous call
   bool planned = false, used = false;
-  int n_seqs = 0, n_rows = 0, max_src = -1;
+  int n_rows = 0, max_src = -1;
   int min_pos = 0, max_pos = -1;
-  bool has_src = false, has_masks = false;
-  const SeqDev* seqs = nullptr;
+  bool has_src = false;
   const RowDev* rows = nullptr;
-  const int *row_seq = nullptr, *table = nullptr;
+  const int* table = nullptr;
   const unsigned long long* masks = nullptr;
+  // The attention's schedule, and its workspace: arrival counters (zero
+  // between calls) and partial states.
+  const Unit* units = nullptr;
+  const int* cta_units = nullptr;
+  int n_ctas = 0, nt = 1, sms = 0;
+  int* arrived = nullptr;
+  size_t arrived_cap = 0;
+  float* parts = nullptr;
+  size_t parts_cap = 0;
+  std::vector<Unit> tiles, runs;
+  std::vector<int> cuts;
   std::vector<uint8_t> seen;  // per page: 1 = read, 2 = written; zero between plans
 };
 
@@ -117,8 +127,29 @@ void release(spec_kv4_batch* b) {
   if (b->dev) cudaFree(b->dev);
   if (b->host) cudaFreeHost(b->host);
   if (b->err) cudaFree(b->err);
+  if (b->arrived) cudaFree(b->arrived);
+  if (b->parts) cudaFree(b->parts);
   if (b->tail) cudaEventDestroy(b->tail);
   if (b->copied) cudaEventDestroy(b->copied);
+}
+
+// A device array of at least n elements; its old contents are dropped once
+// the batch's calls are done.
+template <class T>
+cudaError_t grow(spec_kv4_batch* b, T** p, size_t* cap, size_t n, bool zero) {
+  if (n <= *cap) return cudaSuccess;
+  cudaError_t e = cudaSuccess;
+  if (b->used) e = cudaEventSynchronize(b->tail);
+  if (e != cudaSuccess) return e;
+  if (*p) cudaFree(*p);
+  *p = nullptr;
+  *cap = 0;
+  n += n / 2;
+  e = cudaMalloc(reinterpret_cast<void**>(p), n * sizeof(T));
+  if (e == cudaSuccess && zero) e = cudaMemset(*p, 0, n * sizeof(T));
+  if (e == cudaSuccess && zero) e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) *cap = n;
+  return e;
 }
 
 int check_rows(const char* what, const spec_kv4_rows* r, int64_t need, int heads, int D, bool written) {
@@ -165,6 +196,75 @@ int make_current(int device) {
 }
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
+
+// Cuts the step's attention into units: per (sequence, kv head, tile of at
+// most 32 columns) the 128-token stages its rows see, then those stages, laid
+// end to end, into runs of equal length, one a CTA.  Returns the partial
+// states and arrival counters needed.
+void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_groups) {
+  const Cache& c = *b->c;
+  const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
+  b->tiles.clear();
+  b->runs.clear();
+  b->cuts.clear();
+  b->nt = 1;
+  int64_t stages = 0;
+  int row0 = 0, table = 0;
+  for (int q = 0; q < s->n_seqs; ++q) {
+    const int n = s->kv_len[q], m = s->n_rows[q], cols = m * G;
+    const int tiles = (cols + kMaxCols - 1) / kMaxCols;
+    const int size = tiles ? ((cols + tiles - 1) / tiles + 7) / 8 * 8 : 0;
+    for (int h = 0; h < c.d.n_kv_heads; ++h)
+      for (int c0 = 0; c0 < cols; c0 += size) {
+        Unit u{};
+        u.kvh = h;
+        u.row0 = row0;
+        u.col0 = c0;
+        u.n_cols = cols - c0 < size ? cols - c0 : size;
+        u.kv_len = n;
+        u.kv_end = s->masks ? n + m : n + (c0 + u.n_cols - 1) / G + 1;
+        u.st1 = (u.kv_end + kStageTokens - 1) / kStageTokens;
+        u.table = table;
+        stages += u.st1;
+        if ((u.n_cols + 7) / 8 > b->nt) b->nt = (u.n_cols + 7) / 8;
+        b->tiles.push_back(u);
+      }
+    row0 += m;
+    table += (n + m + P - 1) / P;
+  }
+  *n_parts = *n_groups = 0;
+  b->n_ctas = 0;
+  if (b->tiles.empty()) return;
+  const int64_t slots = (int64_t)b->sms * attend_ctas_per_sm(b->nt);
+  const int64_t run = (stages + slots - 1) / slots;
+  int64_t left = run;
+  b->cuts.push_back(0);
+  for (Unit u : b->tiles) {
+    const int end = u.st1;
+    const size_t first = b->runs.size();
+    for (int at = 0; at < end;) {
+      const int take = (int)(end - at < left ? end - at : left);
+      u.st0 = at;
+      u.st1 = at + take;
+      u.part = (int)(b->runs.size() - first);
+      b->runs.push_back(u);
+      at += take;
+      if ((left -= take) == 0) {
+        b->cuts.push_back((int)b->runs.size());
+        left = run;
+      }
+    }
+    const int parts = (int)(b->runs.size() - first);
+    for (size_t i = first; i < b->runs.size(); ++i) {
+      b->runs[i].n_parts = parts;
+      b->runs[i].part0 = *n_parts;
+      b->runs[i].group = *n_groups;
+    }
+    if (parts > 1) *n_parts += parts, ++*n_groups;
+  }
+  if (b->cuts.back() != (int)b->runs.size()) b->cuts.push_back((int)b->runs.size());
+  b->n_ctas = (int)b->cuts.size() - 1;
+}
 
 int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   const Cache& c = *b->c;
@@ -221,16 +321,18 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   }
   if (!s->src_rows) max_src = (int)rows - 1;
 
-  // One block: sequences, rows, row -> sequence, masks, pages.
-  const size_t at_seqs = 0, at_rows = at_seqs + up(sizeof(SeqDev) * s->n_seqs),
-               at_rseq = at_rows + up(sizeof(RowDev) * rows), at_masks = at_rseq + up(4 * rows),
-               at_table = at_masks + (s->masks ? up(8 * rows) : 0), total = at_table + up(4 * pages);
+  b->planned = false;
+  int n_parts = 0, n_groups = 0;
+  schedule(b, s, &n_parts, &n_groups);
+  // One block: rows, masks, pages, units, the CTAs' first units.
+  const size_t at_rows = 0, at_masks = at_rows + up(sizeof(RowDev) * rows), at_table = at_masks + (s->masks ? up(8 * rows) : 0),
+               at_units = at_table + up(4 * pages), at_cuts = at_units + up(sizeof(Unit) * b->runs.size()),
+               total = at_cuts + up(4 * b->cuts.size());
   cudaError_t e = enter(b, stream);
   if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
   if (total > b->cap) {
     // The old plan's readers and its upload are done before it goes.
     if (b->used && (e = cudaEventSynchronize(b->tail)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
-    b->planned = false;
     if (b->dev) cudaFree(b->dev);
     if (b->host) cudaFreeHost(b->host);
     b->dev = b->host = nullptr;
@@ -243,19 +345,18 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
       return fail_cuda(e, "spec_kv4_plan");
     }
     b->cap = cap;
-  } else if (b->planned && (e = cudaEventSynchronize(b->copied)) != cudaSuccess) {
+  } else if (b->used && (e = cudaEventSynchronize(b->copied)) != cudaSuccess) {
     return fail_cuda(e, "spec_kv4_plan");  // the staging buffer is still being read
   }
-  b->planned = false;
-  SeqDev* hs = reinterpret_cast<SeqDev*>(b->host + at_seqs);
+  if ((e = grow(b, &b->arrived, &b->arrived_cap, n_groups, true)) != cudaSuccess ||
+      (e = grow(b, &b->parts, &b->parts_cap, n_parts * attend_part_floats(c.d.head_dim, b->nt), false)) != cudaSuccess)
+    return fail_cuda(e, "spec_kv4_plan");
   RowDev* hr = reinterpret_cast<RowDev*>(b->host + at_rows);
-  int* hq = reinterpret_cast<int*>(b->host + at_rseq);
   int* ht = reinterpret_cast<int*>(b->host + at_table);
   int r = 0, tp = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int32_t* t = s->page_table + (int64_t)q * s->table_stride;
     const int n = s->kv_len[q], m = s->n_rows[q], np = (n + m + P - 1) / P;
-    hs[q] = SeqDev{n, m, r, tp};
     memcpy(ht + tp, t, sizeof(int) * np);
     tp += np;
     for (int i = 0; i < m; ++i, ++r) {
@@ -263,26 +364,25 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
       if (pos < min_pos) min_pos = pos;
       if (pos > max_pos) max_pos = pos;
       hr[r] = RowDev{t[(n + i) / P], (n + i) % P, pos, s->src_rows ? s->src_rows[r] : r};
-      hq[r] = q;
     }
   }
   if (s->masks) memcpy(b->host + at_masks, s->masks, 8 * (size_t)rows);
+  if (!b->runs.empty()) memcpy(b->host + at_units, b->runs.data(), sizeof(Unit) * b->runs.size());
+  if (!b->cuts.empty()) memcpy(b->host + at_cuts, b->cuts.data(), 4 * b->cuts.size());
   if (total && (e = cudaMemcpyAsync(b->dev, b->host, total, cudaMemcpyHostToDevice, stream)) != cudaSuccess)
     return fail_cuda(e, "spec_kv4_plan");
   if ((e = cudaEventRecord(b->copied, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
   if ((e = leave(b, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
-  b->n_seqs = s->n_seqs;
   b->n_rows = (int)rows;
   b->max_src = max_src;
   b->min_pos = rows ? min_pos : 0;
   b->max_pos = max_pos;
   b->has_src = s->src_rows != nullptr;
-  b->has_masks = s->masks != nullptr;
-  b->seqs = reinterpret_cast<const SeqDev*>(b->dev + at_seqs);
   b->rows = reinterpret_cast<const RowDev*>(b->dev + at_rows);
-  b->row_seq = reinterpret_cast<const int*>(b->dev + at_rseq);
   b->masks = s->masks ? reinterpret_cast<const unsigned long long*>(b->dev + at_masks) : nullptr;
   b->table = reinterpret_cast<const int*>(b->dev + at_table);
+  b->units = reinterpret_cast<const Unit*>(b->dev + at_units);
+  b->cta_units = reinterpret_cast<const int*>(b->dev + at_cuts);
   b->planned = true;
   return SPEC_OK;
 }
@@ -340,6 +440,7 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   b->c = c->c;
   cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&b->err), 16);
   if (e == cudaSuccess) e = cudaMemset(b->err, 0, 16);
   if (e != cudaSuccess) {
@@ -448,20 +549,24 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   if (rc != SPEC_OK) return rc;
   AttendParams p;
   p.pool = c.pool + layer * c.layer_bytes();
-  p.seqs = b->seqs;
+  p.units = b->units;
+  p.cta_units = b->cta_units;
   p.table = b->table;
-  p.row_seq = b->row_seq;
   p.masks = b->masks;
+  p.parts = b->parts;
+  p.arrived = b->arrived;
+  p.err = b->err;
   p.q = to_rows(q);
   p.out = to_rows(out);
   p.scale = scale;
-  p.n_rows = b->n_rows;
+  p.n_ctas = b->n_ctas;
+  p.wide_out = wide(out);
   p.n_heads = c.d.n_heads;
   p.n_kv = c.d.n_kv_heads;
   p.P = c.d.page_tokens;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = enter(b, st);
-  if (e == cudaSuccess) e = launch_attend(p, D, st);
+  if (e == cudaSuccess) e = launch_attend(p, D, b->nt, st);
   if (e == cudaSuccess) e = leave(b, st);
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_attend");
 }

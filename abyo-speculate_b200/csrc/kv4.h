@@ -35,12 +35,6 @@ struct RowDev {
   int pos, src;    // rotation position, row of the input tensors
 };
 
-struct SeqDev {
-  int kv_len, n_rows;
-  int row0;   // first row of the sequence
-  int table;  // first entry of its pages in the plan's table
-};
-
 // Rows of heads (spec_kv4_rows).
 struct Rows {
   void* ptr = nullptr;
@@ -59,17 +53,39 @@ struct AppendParams {
 };
 cudaError_t launch_append(const AppendParams& p, int head_dim, cudaStream_t s);
 
+constexpr int kStageTokens = 128;  // tokens of one ring stage of the attention
+constexpr int kMaxCols = 32;       // (row, query head) columns of one unit
+
+// A run of stages of one (sequence, kv head, column tile), done by one CTA.
+struct Unit {
+  int kvh;
+  int row0;            // first row of the sequence
+  int col0, n_cols;    // stacked columns (row * G + query head of the group)
+  int st0, st1;        // 128-token stages
+  int kv_len, kv_end;  // cached tokens; tokens any column of the tile sees
+  int table;           // the sequence's pages
+  int part0, part, n_parts;  // partial states of the tile; n_parts == 1: none
+  int group;                 // arrival counter
+  int pad[3];
+};
+
 struct AttendParams {
   const uint8_t* pool;  // of the layer
-  const SeqDev* seqs;
+  const Unit* units;
+  const int* cta_units;  // [n_ctas + 1]
   const int* table;
-  const int* row_seq;             // sequence of each row
   const unsigned long long* masks;  // null: causal
+  float* parts;
+  int* arrived;
+  unsigned* err;
   Rows q, out;
   float scale;
-  int n_rows, n_heads, n_kv, P;
+  int n_ctas, n_heads, n_kv, P, wide_out;
 };
-cudaError_t launch_attend(const AttendParams& p, int head_dim, cudaStream_t s);
+// nt: 8-column tiles a unit has at most.
+cudaError_t launch_attend(const AttendParams& p, int head_dim, int nt, cudaStream_t s);
+size_t attend_part_floats(int head_dim, int nt);
+int attend_ctas_per_sm(int nt);
 
 }  // namespace kv4
 }  // namespace specb200
