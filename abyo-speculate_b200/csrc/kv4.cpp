@@ -79,6 +79,7 @@ struct spec_kv4_batch {
   cudaEvent_t tail = nullptr, copied = nullptr;
   unsigned long long last = 0;  // id of the stream of the previous call
   bool planned = false, used = false;
+  bool many = false;  // calls on more than one stream were made: `tail` is recorded
   int n_rows = 0, max_src = -1;
   int min_pos = 0, max_pos = -1;
   bool has_src = false;
@@ -88,13 +89,12 @@ struct spec_kv4_batch {
   // The attention's schedule, and its workspace: arrival counters (zero
   // between calls) and partial states.
   const Unit* units = nullptr;
-  const int* cta_units = nullptr;
   int n_ctas = 0, nt = 1, sms = 0;
   int* arrived = nullptr;
   size_t arrived_cap = 0;
   float* parts = nullptr;
   size_t parts_cap = 0;
-  std::vector<Unit> tiles, runs;
+  std::vector<Unit> tiles, runs, order;
   std::vector<int> cuts;
   std::vector<uint8_t> seen;  // per page: 1 = read, 2 = written; zero between plans
 };
@@ -106,24 +106,57 @@ bool capturing(cudaStream_t s) {
   return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
 }
 
-// Orders a call on `s` after the batch's previous call.
-cudaError_t enter(spec_kv4_batch* b, cudaStream_t s) {
-  if (!b->used || capturing(s)) return cudaSuccess;
+// A call on stream `s`: ordered after the batch's previous call where that was
+// on another stream.  A batch that has only seen one stream records nothing
+// (an event costs a call about 1 us); the first change of stream waits for
+// the device once, since the old stream may no longer exist, and from then on
+// every call leaves an event for the next.  Under capture nothing is ordered.
+struct Turn {
+  spec_kv4_batch* b;
+  cudaStream_t s;
   unsigned long long id = 0;
-  const cudaError_t e = cudaStreamGetId(s, &id);
-  if (e != cudaSuccess || id == b->last) return e;
-  return cudaStreamWaitEvent(s, b->tail, 0);
-}
-cudaError_t leave(spec_kv4_batch* b, cudaStream_t s) {
-  if (capturing(s)) return cudaSuccess;
-  const cudaError_t e = cudaStreamGetId(s, &b->last);
-  if (e != cudaSuccess) return e;
-  b->used = true;
-  return cudaEventRecord(b->tail, s);
+  bool recorded = false;
+  cudaError_t enter() {
+    recorded = capturing(s);
+    if (recorded) return cudaSuccess;
+    cudaError_t e = cudaStreamGetId(s, &id);
+    if (e != cudaSuccess || !b->used || id == b->last) return e;
+    if (b->many) return cudaStreamWaitEvent(s, b->tail, 0);
+    e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) b->many = true;
+    return e;
+  }
+  cudaError_t leave() {
+    if (recorded) return cudaSuccess;
+    b->last = id;
+    b->used = true;
+    return b->many ? cudaEventRecord(b->tail, s) : cudaSuccess;
+  }
+};
+// Waits for the batch's calls.
+cudaError_t drain(spec_kv4_batch* b) {
+  if (!b->used) return cudaSuccess;
+  return b->many ? cudaEventSynchronize(b->tail) : cudaDeviceSynchronize();
 }
 
+// The batch's device is current during a call; the caller's comes back.
+struct Current {
+  int prev = -1, device;
+  int rc = SPEC_OK;
+  explicit Current(int d) : device(d) {
+    cudaError_t e = cudaGetDevice(&prev);
+    if (e == cudaSuccess && prev != d) e = cudaSetDevice(d);
+    if (e != cudaSuccess) rc = fail_cuda(e, "spec_kv4: cudaSetDevice");
+  }
+  ~Current() {
+    if (prev >= 0 && prev != device) cudaSetDevice(prev);
+  }
+  Current(const Current&) = delete;
+  Current& operator=(const Current&) = delete;
+};
+
 void release(spec_kv4_batch* b) {
-  if (b->used) cudaEventSynchronize(b->tail);
+  drain(b);
   if (b->dev) cudaFree(b->dev);
   if (b->host) cudaFreeHost(b->host);
   if (b->err) cudaFree(b->err);
@@ -138,8 +171,7 @@ void release(spec_kv4_batch* b) {
 template <class T>
 cudaError_t grow(spec_kv4_batch* b, T** p, size_t* cap, size_t n, bool zero) {
   if (n <= *cap) return cudaSuccess;
-  cudaError_t e = cudaSuccess;
-  if (b->used) e = cudaEventSynchronize(b->tail);
+  cudaError_t e = drain(b);
   if (e != cudaSuccess) return e;
   if (*p) cudaFree(*p);
   *p = nullptr;
@@ -189,12 +221,6 @@ bool wide(const spec_kv4_rows* r) {
   return reinterpret_cast<uintptr_t>(r->ptr) % 16 == 0 && r->row_stride * sz % 16 == 0 && r->head_stride * sz % 16 == 0;
 }
 
-int make_current(int device) {
-  int cur = -1;
-  if (cudaGetDevice(&cur) != cudaSuccess || cur != device) return fail(SPEC_ERR_CUDA, "spec_kv4: cudaSetDevice failed");
-  return SPEC_OK;
-}
-
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
 // Cuts the step's attention into units: per (sequence, kv head, tile of at
@@ -206,6 +232,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_gr
   const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
   b->tiles.clear();
   b->runs.clear();
+  b->order.clear();
   b->cuts.clear();
   b->nt = 1;
   int64_t stages = 0;
@@ -260,10 +287,27 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_gr
       b->runs[i].part0 = *n_parts;
       b->runs[i].group = *n_groups;
     }
-    if (parts > 1) *n_parts += parts, ++*n_groups;
+    for (int n = parts; n > 1;) {
+      *n_parts += n;
+      n = (n + kFanIn - 1) / kFanIn;
+      *n_groups += n;
+    }
   }
   if (b->cuts.back() != (int)b->runs.size()) b->cuts.push_back((int)b->runs.size());
   b->n_ctas = (int)b->cuts.size() - 1;
+  // The order the kernel reads: first units of all CTAs, then each CTA's others.
+  b->order.resize(b->runs.size());
+  int at = b->n_ctas;
+  for (int i = 0; i < b->n_ctas; ++i) {
+    const int first = b->cuts[i], n = b->cuts[i + 1] - first;
+    for (int k = 0; k < n; ++k) {
+      Unit& u = k == 0 ? b->order[i] : b->order[at + k - 1];
+      u = b->runs[first + k];
+      u.next = at + k;
+      u.last = at + n - 1;
+    }
+    at += n - 1;
+  }
 }
 
 int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
@@ -324,15 +368,15 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   b->planned = false;
   int n_parts = 0, n_groups = 0;
   schedule(b, s, &n_parts, &n_groups);
-  // One block: rows, masks, pages, units, the CTAs' first units.
+  // One block: rows, masks, pages, units.
   const size_t at_rows = 0, at_masks = at_rows + up(sizeof(RowDev) * rows), at_table = at_masks + (s->masks ? up(8 * rows) : 0),
-               at_units = at_table + up(4 * pages), at_cuts = at_units + up(sizeof(Unit) * b->runs.size()),
-               total = at_cuts + up(4 * b->cuts.size());
-  cudaError_t e = enter(b, stream);
+               at_units = at_table + up(4 * pages), total = at_units + up(sizeof(Unit) * b->order.size());
+  Turn turn{b, stream};
+  cudaError_t e = turn.enter();
   if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
   if (total > b->cap) {
     // The old plan's readers and its upload are done before it goes.
-    if (b->used && (e = cudaEventSynchronize(b->tail)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+    if ((e = drain(b)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
     if (b->dev) cudaFree(b->dev);
     if (b->host) cudaFreeHost(b->host);
     b->dev = b->host = nullptr;
@@ -367,12 +411,15 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
     }
   }
   if (s->masks) memcpy(b->host + at_masks, s->masks, 8 * (size_t)rows);
-  if (!b->runs.empty()) memcpy(b->host + at_units, b->runs.data(), sizeof(Unit) * b->runs.size());
-  if (!b->cuts.empty()) memcpy(b->host + at_cuts, b->cuts.data(), 4 * b->cuts.size());
+  for (Unit& u : b->order) {
+    const int per = kStageTokens / P, first = u.st0 * per, n = (u.kv_end + P - 1) / P - first;
+    for (int i = 0; i < per && i < n; ++i) u.pages[i] = ht[u.table + first + i];
+  }
+  if (!b->order.empty()) memcpy(b->host + at_units, b->order.data(), sizeof(Unit) * b->order.size());
   if (total && (e = cudaMemcpyAsync(b->dev, b->host, total, cudaMemcpyHostToDevice, stream)) != cudaSuccess)
     return fail_cuda(e, "spec_kv4_plan");
   if ((e = cudaEventRecord(b->copied, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
-  if ((e = leave(b, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
+  if ((e = turn.leave()) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
   b->n_rows = (int)rows;
   b->max_src = max_src;
   b->min_pos = rows ? min_pos : 0;
@@ -382,7 +429,6 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   b->masks = s->masks ? reinterpret_cast<const unsigned long long*>(b->dev + at_masks) : nullptr;
   b->table = reinterpret_cast<const int*>(b->dev + at_table);
   b->units = reinterpret_cast<const Unit*>(b->dev + at_units);
-  b->cta_units = reinterpret_cast<const int*>(b->dev + at_cuts);
   b->planned = true;
   return SPEC_OK;
 }
@@ -432,15 +478,15 @@ void spec_kv4_free(spec_kv4* c) { delete c; }
 int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   if (!c || !out) return fail(SPEC_ERR_INVALID, "spec_kv4_batch_create: null argument");
   *out = nullptr;
-  DeviceGuard dg(c->c->d.device);
-  int rc = make_current(c->c->d.device);
-  if (rc != SPEC_OK) return rc;
+  Current cur(c->c->d.device);
+  if (cur.rc != SPEC_OK) return cur.rc;
   spec_kv4_batch* b = new (std::nothrow) spec_kv4_batch;
   if (!b) return fail(SPEC_ERR_OOM, "spec_kv4_batch_create: out of host memory");
   b->c = c->c;
   cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);
+  if (e == cudaSuccess) e = attend_setup();
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&b->err), 16);
   if (e == cudaSuccess) e = cudaMemset(b->err, 0, 16);
   if (e != cudaSuccess) {
@@ -454,16 +500,15 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
 
 void spec_kv4_batch_free(spec_kv4_batch* b) {
   if (!b) return;
-  DeviceGuard dg(b->c->d.device);
+  Current cur(b->c->d.device);
   release(b);
   delete b;
 }
 
 int spec_kv4_plan(spec_kv4_batch* b, const spec_kv4_step* s, void* stream) {
   if (!b || !s) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: null argument");
-  DeviceGuard dg(b->c->d.device);
-  int rc = make_current(b->c->d.device);
-  if (rc != SPEC_OK) return rc;
+  Current cur(b->c->d.device);
+  if (cur.rc != SPEC_OK) return cur.rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (capturing(st)) return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4_plan: the stream is under capture");
   try {
@@ -499,9 +544,8 @@ int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   if (c.cos && (b->min_pos < 0 || b->max_pos >= c.n_positions))
     return fail(SPEC_ERR_INVALID, "spec_kv4_append: positions %d to %d, the rotation tables have %d", b->min_pos, b->max_pos,
                 c.n_positions);
-  DeviceGuard dg(c.d.device);
-  rc = make_current(c.d.device);
-  if (rc != SPEC_OK) return rc;
+  Current cur(c.d.device);
+  if (cur.rc != SPEC_OK) return cur.rc;
   AppendParams p;
   p.pool = c.pool + layer * c.layer_bytes();
   p.cos = c.cos;
@@ -518,15 +562,17 @@ int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   p.n_kv = hk;
   p.P = c.d.page_tokens;
   p.rope_half = c.d.rope_half ? 1 : 0;
-  p.wide_q = wide(q) && wide(q_out);
+  p.wide_q = wide(q);
+  p.wide_qo = wide(q_out);
   p.wide_k = wide(k);
   p.wide_v = wide(v);
   p.wide_ko = wide(k_out);
   p.wide_vo = wide(v_out);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = enter(b, st);
+  Turn turn{b, st};
+  cudaError_t e = turn.enter();
   if (e == cudaSuccess) e = launch_append(p, D, st);
-  if (e == cudaSuccess) e = leave(b, st);
+  if (e == cudaSuccess) e = turn.leave();
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_append");
 }
 
@@ -544,13 +590,11 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   if (rc != SPEC_OK) return rc;
   if (q->dtype == T_F32) return fail(SPEC_ERR_UNSUPPORTED, "spec_kv4_attend: q is bf16 or f16");
   if (!(scale == scale) || scale - scale != 0.f) return fail(SPEC_ERR_INVALID, "spec_kv4_attend: scale is not finite");
-  DeviceGuard dg(c.d.device);
-  rc = make_current(c.d.device);
-  if (rc != SPEC_OK) return rc;
+  Current cur(c.d.device);
+  if (cur.rc != SPEC_OK) return cur.rc;
   AttendParams p;
   p.pool = c.pool + layer * c.layer_bytes();
   p.units = b->units;
-  p.cta_units = b->cta_units;
   p.table = b->table;
   p.masks = b->masks;
   p.parts = b->parts;
@@ -560,28 +604,28 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   p.out = to_rows(out);
   p.scale = scale;
   p.n_ctas = b->n_ctas;
+  p.wide_q = wide(q);
   p.wide_out = wide(out);
   p.n_heads = c.d.n_heads;
   p.n_kv = c.d.n_kv_heads;
   p.P = c.d.page_tokens;
+  p.P_log2 = p.P == 16 ? 4 : p.P == 32 ? 5 : p.P == 64 ? 6 : 7;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = enter(b, st);
+  Turn turn{b, st};
+  cudaError_t e = turn.enter();
   if (e == cudaSuccess) e = launch_attend(p, D, b->nt, st);
-  if (e == cudaSuccess) e = leave(b, st);
+  if (e == cudaSuccess) e = turn.leave();
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_attend");
 }
 
 int spec_kv4_status(spec_kv4_batch* b) {
   if (!b) return fail(SPEC_ERR_INVALID, "spec_kv4_status: null argument");
-  DeviceGuard dg(b->c->d.device);
-  int rc = make_current(b->c->d.device);
-  if (rc != SPEC_OK) return rc;
-  if (b->used) {
-    const cudaError_t e = cudaEventSynchronize(b->tail);
-    if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_status");
-  }
+  Current cur(b->c->d.device);
+  if (cur.rc != SPEC_OK) return cur.rc;
+  const cudaError_t e = drain(b);
+  if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_status");
   char msg[256];
-  rc = take_device_error(b->err, nullptr, msg, sizeof msg);
+  const int rc = take_device_error(b->err, nullptr, msg, sizeof msg);
   if (rc != SPEC_OK) set_thread_error(msg);
   return rc;
 }

@@ -48,31 +48,35 @@ struct AppendParams {
   const RowDev* rows;
   Rows q, q_out, k, v, k_out, v_out;
   int n_rows, n_heads, n_kv, P, rope_half;
-  int wide_q, wide_k, wide_v;  // inputs (and q_out) allow 16-byte accesses of 8 channels
-  int wide_ko, wide_vo;
+  int wide_q, wide_k, wide_v;  // 8 channels are aligned 16-byte accesses
+  int wide_qo, wide_ko, wide_vo;
 };
 cudaError_t launch_append(const AppendParams& p, int head_dim, cudaStream_t s);
 
-constexpr int kStageTokens = 128;  // tokens of one ring stage of the attention
+constexpr int kStageTokens = 128;  // tokens the attention's work is cut by
+constexpr int kFanIn = 16;         // partial states joined at once
 constexpr int kMaxCols = 32;       // (row, query head) columns of one unit
 
 // A run of stages of one (sequence, kv head, column tile), done by one CTA.
-struct Unit {
+struct alignas(16) Unit {
   int kvh;
   int row0;            // first row of the sequence
   int col0, n_cols;    // stacked columns (row * G + query head of the group)
   int st0, st1;        // 128-token stages
   int kv_len, kv_end;  // cached tokens; tokens any column of the tile sees
   int table;           // the sequence's pages
-  int part0, part, n_parts;  // partial states of the tile; n_parts == 1: none
-  int group;                 // arrival counter
-  int pad[3];
+  // Partial states of the tile: n_parts at part0, then ceil(n / kFanIn) more
+  // a level; arrival counters likewise from `group` on.  n_parts == 1: none.
+  int part0, part, n_parts;
+  int group;
+  int next, last;      // the CTA's next unit and one past its last
+  int pad;
+  int pages[8];        // pages of the first stage
 };
 
 struct AttendParams {
   const uint8_t* pool;  // of the layer
-  const Unit* units;
-  const int* cta_units;  // [n_ctas + 1]
+  const Unit* units;  // [n_ctas] first units of the CTAs, then the others
   const int* table;
   const unsigned long long* masks;  // null: causal
   float* parts;
@@ -80,10 +84,12 @@ struct AttendParams {
   unsigned* err;
   Rows q, out;
   float scale;
-  int n_ctas, n_heads, n_kv, P, wide_out;
+  int n_ctas, n_heads, n_kv, P, P_log2, wide_q, wide_out;
 };
 // nt: 8-column tiles a unit has at most.
 cudaError_t launch_attend(const AttendParams& p, int head_dim, int nt, cudaStream_t s);
+// Once per device, with it current, before the first launch.
+cudaError_t attend_setup();
 size_t attend_part_floats(int head_dim, int nt);
 int attend_ctas_per_sm(int nt);
 

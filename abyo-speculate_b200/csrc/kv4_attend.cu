@@ -13,25 +13,27 @@
 // contracted axis will do, so a lane takes the channels of whole 32-bit words
 // and never shuffles nibbles; P^T is S^T's fragment through movmatrix.
 //
-// A CTA is 8 consumer warps, 16 tokens each of a 128-token stage, and one
-// producer warp that copies page blocks (K, V and scales of one head lie
-// together) by TMA bulk copies into a ring.  The host cuts the batch's stages
-// into equal runs, one a CTA; a (sequence, head, column tile) that several
-// CTAs share leaves partial (m, l, O) and the last of them to arrive joins
-// them in order, so a plan's results do not depend on timing.
+// A CTA is 4 warps that run on their own: warp w takes the 32-token tiles w,
+// w + 4, ... of the CTA's stages, copies them by TMA bulk copies into a ring
+// of its own and refills a slot as soon as it has read it, across unit
+// boundaries.  The host cuts the batch's 128-token stages into equal runs, one
+// a CTA.  A unit's warps join their (m, l, O) in shared memory; a (sequence,
+// head, column tile) that several CTAs share is joined by the last arriver of
+// every kFanIn of them, level by level and in order, so a plan's results do
+// not depend on timing.
 #include "common.cuh"
 #include "kv4.h"
+#include "kv4_rows.cuh"
 
 namespace specb200 {
 namespace kv4 {
 namespace {
 
-constexpr int kConsumers = 8;
-constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 32;  // tokens of one ring slot
 constexpr float kNone = -1e30f;  // the reference before any score
 constexpr float kSlack = 8.f;    // a score may pass the reference by this many octaves before it moves
-
-SPEC_DEV void bar_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
 
 SPEC_DEV float ex2(float x) {
   float r;
@@ -57,43 +59,50 @@ SPEC_DEV uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Values of nibbles n and n + 4 of w.
+// Values of nibbles N and N + 4 of w: s (1 + code / 16) + o.  The low nibbles
+// are read in place as 1 + code / 2^10 or 1 + code / 2^6 and brought to
+// 1 + code / 16 by an exact multiply-add, the high ones by a shift, which
+// loads the integer and the f16 pipe alike (6 and 6 instructions a word).
 template <int N>
 SPEC_DEV uint32_t dq(uint32_t w, uint32_t s2, uint32_t o2) {
-  const uint32_t x = N == 0 ? w << 6 : N == 1 ? w << 2 : N == 2 ? w >> 2 : w >> 6;
-  return hfma2(lop3_and_or(x, 0x03C003C0u, 0x3C003C00u), s2, o2);
+  uint32_t x;
+  if (N == 0) x = hfma2(lop3_and_or(w, 0x000F000Fu, 0x3C003C00u), 0x54005400u, 0xD3E0D3E0u);       // 64 x - 63
+  else if (N == 1) x = hfma2(lop3_and_or(w, 0x00F000F0u, 0x3C003C00u), 0x44004400u, 0xC200C200u);  // 4 x - 3
+  else x = lop3_and_or(N == 2 ? w >> 2 : w >> 6, 0x03C003C0u, 0x3C003C00u);
+  return hfma2(x, s2, o2);
 }
 SPEC_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  mma_f16(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+  // Not volatile: the compiler interleaves the chains with the unpacking.
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+
+// CTAs an SM holds: O^T alone takes 32 registers a thread and 8 columns.
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
 
 template <int D, int NT>
 struct Shape {
-  static constexpr int KS = D / 16;                    // 16-channel steps of q.k
-  static constexpr int MT = D / 16;                    // 16-channel tiles of O^T
-  static constexpr int STAGE = kStageTokens * D * 5 / 4;
-  static constexpr int STAGES = NT <= 1 ? 81920 / STAGE : 81920 / STAGE;
-  static constexpr int FRAG = MT * NT * 4;             // O^T floats a lane
-  static constexpr int MERGE = (kConsumers / 2) * FRAG * 128;
-  static constexpr int Q_AT = STAGES * STAGE + MERGE;
+  static constexpr int KS = D / 16;              // 16-channel steps of q.k
+  static constexpr int MT = D / 16;              // 16-channel tiles of O^T
+  static constexpr int TILE = kTile * D * 5 / 4;  // bytes of a ring slot
+  static constexpr int STAGES = (NT <= 2 ? 2 : 3) * (128 / D);
+  static constexpr int FRAG = MT * NT * 4;       // O^T floats a lane
+  static constexpr int MERGE_AT = kWarps * STAGES * TILE;
+  // Two warps' O^T, or the columns on their way out.
+  static constexpr int Q_AT = MERGE_AT + ((kWarps / 2) * FRAG * 128 > NT * 8 * (D + 4) * 4 ? (kWarps / 2) * FRAG * 128
+                                                                                            : NT * 8 * (D + 4) * 4);
   static constexpr int META_AT = Q_AT + NT * KS * 256;
-  static constexpr int SMEM = META_AT + 2048;
 };
 
 struct Meta {
-  unsigned long long full[8], empty[8];
+  unsigned long long full[kWarps][8];
   unsigned long long mask[32];
   float c[32];  // scale log2(e) 2^e of a column (q is held as q 2^-e)
   int idx[32];  // row of the sequence; -1: no such column
-  float m[kConsumers][32], l[kConsumers / 2][32];
+  float m[kWarps / 2][32], l[kWarps / 2][32];
   int last;
 };
-static_assert(sizeof(Meta) <= 2048 + 1024, "meta");
-
-SPEC_DEV float load1(const Rows& r, long long at) {
-  if (r.dtype == T_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(r.ptr)[at]);
-  return __half2float(static_cast<const __half*>(r.ptr)[at]);
-}
 
 // One warp's softmax state: lane (g, t) holds columns 8 nt + 2t + {0, 1}.
 template <int D, int NT>
@@ -125,7 +134,7 @@ SPEC_DEV void join_warps(State<D, NT>& s, float* buf, Meta* mt, int warp, int la
   constexpr int F = Shape<D, NT>::FRAG;
   const int t = lane & 3;
 #pragma unroll 1
-  for (int off = kConsumers / 2; off > 0; off >>= 1) {
+  for (int off = kWarps / 2; off > 0; off >>= 1) {
     if (warp >= off && warp < 2 * off) {
       float4* p = reinterpret_cast<float4*>(buf + (warp - off) * F * 32);
 #pragma unroll
@@ -143,7 +152,7 @@ SPEC_DEV void join_warps(State<D, NT>& s, float* buf, Meta* mt, int warp, int la
           }
       }
     }
-    bar_consumers();
+    __syncthreads();
     if (warp < off) {
       const float4* p = reinterpret_cast<const float4*>(buf + warp * F * 32);
       float b[NT][2];
@@ -168,320 +177,477 @@ SPEC_DEV void join_warps(State<D, NT>& s, float* buf, Meta* mt, int warp, int la
           s.o[a][n][3] += x.w * b[n][1];
         }
     }
-    bar_consumers();
+    __syncthreads();
   }
 }
 
-// Writes columns of a joined state: lane (g, t) holds D/8 consecutive channels.
+// Writes a joined state's columns: warp 0 lays them out in shared memory
+// (lane (g, t) holds D/8 consecutive channels of its columns), then D/8
+// threads take a column each.
 template <int D, int NT>
-SPEC_DEV void write_out(const State<D, NT>& s, const AttendParams& p, const Unit& u, int lane) {
-  constexpr int W = D / 8;
-  const int g = lane >> 2, t = lane & 3, G = p.n_heads / p.n_kv;
+SPEC_DEV void write_out(const State<D, NT>& s, const AttendParams& p, const Unit& u, float* buf, int warp, int lane) {
+  constexpr int LD = D + 4;
+  if (warp == 0) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = n * 8 + 2 * t + e;
-      if (col >= u.n_cols) continue;
-      const int r = u.col0 + col;
-      const float inv = s.l[n][e] == 0.f ? 0.f : 1.f / s.l[n][e];
-      const long long at = (u.row0 + r / G) * p.out.row_stride + (u.kvh * G + r % G) * p.out.head_stride + g * W;
-      float x[W];
+      for (int e = 0; e < 2; ++e) {
+        const float inv = s.l[n][e] == 0.f ? 0.f : 1.f / s.l[n][e];
+        float2* dst = reinterpret_cast<float2*>(buf + (n * 8 + 2 * t + e) * LD + g * (D / 8));
 #pragma unroll
-      for (int a = 0; a < Shape<D, NT>::MT; ++a) {
-        x[2 * a] = s.o[a][n][e] * inv;
-        x[2 * a + 1] = s.o[a][n][2 + e] * inv;
+        for (int a = 0; a < Shape<D, NT>::MT; ++a) dst[a] = make_float2(s.o[a][n][e] * inv, s.o[a][n][2 + e] * inv);
       }
-      if (p.out.dtype == T_F32) {
-        float* q = static_cast<float*>(p.out.ptr) + at;
-        if (p.wide_out) {
+  }
+  __syncthreads();
+  constexpr int TPC = D / 8;
+  const int G = p.n_heads / p.n_kv;
+#pragma unroll 1
+  for (int col = threadIdx.x / TPC; col < u.n_cols; col += kThreads / TPC) {
+    const int r = u.col0 + col, c = threadIdx.x % TPC * 8;
+    const float4 x = *reinterpret_cast<const float4*>(buf + col * LD + c);
+    const float4 y = *reinterpret_cast<const float4*>(buf + col * LD + c + 4);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    store8(p.out, (u.row0 + r / G) * p.out.row_stride + (u.kvh * G + r % G) * p.out.head_stride + c, p.wide_out, v);
+  }
+}
+
+// Adds partial state src (weights b = 2^(m' - m)) to s.  Half of its O^T is
+// under way before its m and l are used.
+template <int D, int NT>
+SPEC_DEV void take_part(State<D, NT>& s, const float* src, int lane) {
+  using Sh = Shape<D, NT>;
+  constexpr int H = Sh::MT / 2;
+  const int t = lane & 3;
+  const float4* o = reinterpret_cast<const float4*>(src) + lane;
+  float2 om[NT], ol[NT];
+  float b[NT][2];
+  float4 x[H][NT];
 #pragma unroll
-          for (int i = 0; i < W / 4; ++i)
-            reinterpret_cast<float4*>(q)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-        } else {
+  for (int n = 0; n < NT; ++n) {
+    om[n] = __ldcg(reinterpret_cast<const float2*>(src + Sh::FRAG * 32 + n * 8 + 2 * t));
+    ol[n] = __ldcg(reinterpret_cast<const float2*>(src + Sh::FRAG * 32 + NT * 8 + n * 8 + 2 * t));
+  }
 #pragma unroll
-          for (int i = 0; i < W; ++i) q[i] = x[i];
-        }
-      } else {
-        uint32_t w[W / 2];
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < W / 2; ++i) {
-          if (p.out.dtype == T_BF16) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-          } else {
-            w[i] = pack2(x[2 * i], x[2 * i + 1]);
-          }
-        }
-        uint16_t* q = static_cast<uint16_t*>(p.out.ptr) + at;
-        if (p.wide_out) {
+    for (int a = 0; a < H; ++a)
 #pragma unroll
-          for (int i = 0; i < W / 8; ++i)
-            reinterpret_cast<uint4*>(q)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        } else {
+      for (int n = 0; n < NT; ++n) x[a][n] = __ldcg(o + ((h * H + a) * NT + n) * 32);
+    if (h == 0) {
 #pragma unroll
-          for (int i = 0; i < W / 2; ++i) q[2 * i] = (uint16_t)w[i], q[2 * i + 1] = (uint16_t)(w[i] >> 16);
-        }
+      for (int n = 0; n < NT; ++n) {
+        s.rescale(n, 0, fmaxf(s.m[n][0], om[n].x));
+        s.rescale(n, 1, fmaxf(s.m[n][1], om[n].y));
+        b[n][0] = ex2(om[n].x - s.m[n][0]);
+        b[n][1] = ex2(om[n].y - s.m[n][1]);
+        s.l[n][0] += ol[n].x * b[n][0];
+        s.l[n][1] += ol[n].y * b[n][1];
       }
     }
+#pragma unroll
+    for (int a = 0; a < H; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float(&y)[4] = s.o[h * H + a][n];
+        y[0] += x[a][n].x * b[n][0];
+        y[1] += x[a][n].y * b[n][1];
+        y[2] += x[a][n].z * b[n][0];
+        y[3] += x[a][n].w * b[n][1];
+      }
+  }
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT <= 1 ? 2 : 1) attend_kernel(const __grid_constant__ AttendParams p) {
+SPEC_DEV void leave_part(const State<D, NT>& s, float* dst, int lane) {
+  using Sh = Shape<D, NT>;
+  const int t = lane & 3;
+#pragma unroll
+  for (int a = 0; a < Sh::MT; ++a)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      __stcg(reinterpret_cast<float4*>(dst) + (a * NT + n) * 32 + lane,
+             make_float4(s.o[a][n][0], s.o[a][n][1], s.o[a][n][2], s.o[a][n][3]));
+  if (lane < 4) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        __stcg(dst + Sh::FRAG * 32 + n * 8 + 2 * t + e, s.m[n][e]);
+        __stcg(dst + Sh::FRAG * 32 + NT * 8 + n * 8 + 2 * t + e, s.l[n][e]);
+      }
+  }
+}
+
+// One warp's way through the tiles of its CTA's units, ahead of the one it
+// computes.  The page ids of a tile are loaded when the tile before it is
+// issued; those of a unit's first stage lie in the unit, so that a copy can
+// start one load after the kernel does.
+struct Cursor {
+  int ui, next, last;  // unit; the CTA's units after it
+  int tile, end;       // tiles of 32 tokens
+  int kvh, kv_end, table;
+  int page[2];
+  SPEC_DEV bool more() const { return ui >= 0; }
+  SPEC_DEV void at_unit(const AttendParams& p, int warp) {
+    while (true) {
+      const Unit& u = p.units[ui];
+      const int* pg = u.pages + (warp * kTile >> p.P_log2);
+      page[0] = pg[0];
+      page[1] = p.P < kTile ? pg[1] : 0;
+      tile = u.st0 * (kStageTokens / kTile) + warp;
+      kv_end = u.kv_end;
+      end = min(u.st1 * (kStageTokens / kTile), (kv_end + kTile - 1) / kTile);
+      kvh = u.kvh;
+      table = u.table;
+      if (tile < end) return;
+      if (next == last) {
+        ui = -1;
+        return;
+      }
+      ui = next++;
+    }
+  }
+  SPEC_DEV void advance(const AttendParams& p, int warp) {
+    tile += kWarps;
+    if (tile >= end) {
+      if (next == last) {
+        ui = -1;
+        return;
+      }
+      ui = next++;
+      at_unit(p, warp);
+    } else {
+      const int* t = p.table + table + (tile * kTile >> p.P_log2);
+      page[0] = t[0];
+      page[1] = p.P < kTile && tile * kTile + p.P < kv_end ? t[1] : 0;
+    }
+  }
+};
+
+// Copies the cursor's tile into `dst` as blocks of min(P, 32) tokens: pages
+// of 16 and 32 tokens whole, a quarter of a block's four areas of larger ones.
+template <int D>
+SPEC_DEV void copy_tile(const AttendParams& p, const Cursor& c, uint8_t* dst, uint64_t* bar) {
+  const int P = p.P, blk = block_bytes(P, D);
+  const uint8_t* src = p.pool + ((long long)c.page[0] * p.n_kv + c.kvh) * blk;
+  if (P <= kTile) {
+    const int n = P < kTile && c.tile * kTile + P < c.kv_end ? 2 : 1;
+    mbar_arrive_expect_tx(bar, n * blk);
+    tma_bulk_g2s(dst, src, blk, bar);
+    if (n == 2) tma_bulk_g2s(dst + blk, p.pool + ((long long)c.page[1] * p.n_kv + c.kvh) * blk, blk, bar);
+  } else {
+    const int j = c.tile * kTile & (P - 1);
+    mbar_arrive_expect_tx(bar, block_bytes(kTile, D));
+    tma_bulk_g2s(dst, src + j * (D / 2), kTile * D / 2, bar);
+    tma_bulk_g2s(dst + k_scales_at(kTile, D), src + k_scales_at(P, D) + j * (D / 8), kTile * D / 8, bar);
+    tma_bulk_g2s(dst + v_codes_at(kTile, D), src + v_codes_at(P, D) + j * (D / 2), kTile * D / 2, bar);
+    tma_bulk_g2s(dst + v_scales_at(kTile, D), src + v_scales_at(P, D) + j * (D / 8), kTile * D / 8, bar);
+  }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const __grid_constant__ AttendParams p) {
   using Sh = Shape<D, NT>;
   constexpr int KW = D / 32;  // code words of K a lane holds of a token
   constexpr int VW = D / 64;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* merge = reinterpret_cast<float*>(smem + Sh::STAGES * Sh::STAGE);
+  float* merge = reinterpret_cast<float*>(smem + Sh::MERGE_AT);
   uint32_t* qs = reinterpret_cast<uint32_t*>(smem + Sh::Q_AT);  // [nt][kstep][lane][2]
   Meta* mt = reinterpret_cast<Meta*>(smem + Sh::META_AT);
-  uint64_t* full = reinterpret_cast<uint64_t*>(mt->full);
-  uint64_t* empty = reinterpret_cast<uint64_t*>(mt->empty);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int P = p.P, blk = block_bytes(P, D), per = kStageTokens / P;
-  if (threadIdx.x == 0) {
+  uint64_t* full = reinterpret_cast<uint64_t*>(mt->full[warp]);
+  uint8_t* ring = smem + warp * Sh::STAGES * Sh::TILE;
+  if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < Sh::STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], kConsumers);
-    }
+    for (int i = 0; i < Sh::STAGES; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
   }
-  __syncthreads();
-  const int u0 = p.cta_units[blockIdx.x], u1 = p.cta_units[blockIdx.x + 1];
-  int k = 0;  // stages so far
+  __syncwarp();
+  Unit u = p.units[blockIdx.x];
+  Cursor cur;
+  cur.ui = blockIdx.x;
+  cur.next = u.next;
+  cur.last = u.last;
+  cur.at_unit(p, warp);
+#pragma unroll 1
+  for (int i = 0; i < Sh::STAGES && cur.more(); ++i) {
+    if (lane == 0) copy_tile<D>(p, cur, ring + i * Sh::TILE, &full[i]);
+    cur.advance(p, warp);
+  }
+  int slot = 0, phase = 0;
   bool ok = true;
 
-  if (warp == kConsumers) {
-    // Producer: one lane a page.
-    for (int ui = u0; ui < u1 && ok; ++ui) {
-      const Unit u = p.units[ui];
-      for (int st = u.st0; st < u.st1; ++st, ++k) {
-        const int slot = k % Sh::STAGES;
-        const int pages = min(per, (u.kv_end + P - 1) / P - st * per);
-        const int page = lane < pages ? p.table[u.table + st * per + lane] : 0;
-        if (k >= Sh::STAGES) ok = mbar_wait_bounded(&empty[slot], (k / Sh::STAGES - 1) & 1, p.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(&full[slot], pages * blk);
-        __syncwarp();
-        if (lane < pages)
-          tma_bulk_g2s(smem + slot * Sh::STAGE + lane * blk, p.pool + ((long long)page * p.n_kv + u.kvh) * blk, blk,
-                       &full[slot]);
-      }
-    }
-    if (!ok) {  // leave no copy of this CTA in flight
-      for (int i = max(0, k - Sh::STAGES); i < k; ++i)
-        mbar_wait_bounded(&full[i % Sh::STAGES], (i / Sh::STAGES) & 1, p.err);
-    }
-    return;
-  }
-
   const int g = lane >> 2, t = lane & 3, G = p.n_heads / p.n_kv;
-  // Offsets of this lane's pieces from its tile's first token.
+  // The slot holds blocks of Pt tokens; the second 16 tokens are in the same
+  // block or the next one.
+  const int Pt = min(p.P, kTile);
+  const int ks0 = k_scales_at(Pt, D), vc0 = v_codes_at(Pt, D), vs0 = v_scales_at(Pt, D);
+  const int code16 = Pt == kTile ? 16 * (D / 2) : block_bytes(16, D);   // from the first 16 tokens to the second
+  const int scale16 = Pt == kTile ? 16 * (D / 8) : block_bytes(16, D);
+  // Offsets of this lane's pieces from a 16-token half's first token.
   const int k_at = g * (D / 2) + t * (KW * 4);
-  const int ks_at = (g * (D / 32) + t * (D / 32) / 4) * 4;
+  const int ks_at = ks0 + (g * (D / 32) + t * (D / 32) / 4) * 4;
   int v_at[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int j = 2 * t + (e & 1) + (e >> 1) * 8, byte = g * (VW * 4);
-    v_at[e] = v_piece_at(D, j, byte / 32) + byte % 32;
+    v_at[e] = vc0 + v_piece_at(D, j, byte / 32) + byte % 32;
   }
-  const int vs_at = t * (D / 32 * 8) + (g * (D / 32) / 8) * 8;
+  const int vs_at = vs0 + t * (D / 32 * 8) + (g * (D / 32) / 8) * 8;
 
-  for (int ui = u0; ui < u1; ++ui) {
-    const Unit u = p.units[ui];
+  for (int next = u.next;; ++next) {
     // Columns: q rows as f16 B fragments, scaled by a power of two where bf16
-    // could leave f16's range.
-    for (int col = warp; col < NT * 8; col += kConsumers) {
-      const bool live = col < u.n_cols;
-      const int r = u.col0 + (live ? col : 0), row = r / G;
-      float x[D / 32], a = 0.f;
-      const long long at = (u.row0 + row) * p.q.row_stride + (u.kvh * G + r % G) * p.q.head_stride + lane * (D / 32);
+    // could leave f16's range.  D/8 threads a column, 8 channels each: word
+    // w of the lanes t, pairs (n, n + 4).  All loads are issued first.
+    {
+      constexpr int TPC = D / 8, PASS = kThreads / TPC, QC = (NT * 8 + PASS - 1) / PASS;
+      const int ch = threadIdx.x % TPC, tt = ch / (D / 32), w = ch % (D / 32);
+      float x[QC][8];
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        x[i] = live ? load1(p.q, at + i) : 0.f;
-        a = fmaxf(a, fabsf(x[i]));
+      for (int i = 0; i < QC; ++i) {
+        const int col = i * PASS + threadIdx.x / TPC, r = u.col0 + (col < u.n_cols ? col : 0);
+        load8(p.q, (u.row0 + r / G) * p.q.row_stride + (u.kvh * G + r % G) * p.q.head_stride + ch * 8, p.wide_q, x[i]);
       }
-      int ex = 0;
-      if (p.q.dtype == T_BF16) {
-        a = warp_max(a);
-        if (a > 0.f && a < INFINITY) ex = min(max((__float_as_int(a) >> 23) - 127, -100), 126);
-      }
-      const float down = __int_as_float((127 - ex) << 23);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const int c = lane * (D / 32) + i, tt = c / (D / 4), w = c % (D / 4) / 8, n = c % 4, hi = c % 8 / 4;
-        __half* dst = reinterpret_cast<__half*>(
-            qs + (((col / 8) * Sh::KS + 2 * w + (n >> 1)) * 32 + (col % 8) * 4 + tt) * 2 + (n & 1));
-        dst[hi] = __float2half_rn(x[i] * down);
-      }
-      if (lane == 0) {
-        mt->c[col] = p.scale * 1.4426950408889634f * __int_as_float((min(ex + 127, 254)) << 23);
-        mt->idx[col] = live ? row : -1;
-        mt->mask[col] = live && p.masks ? p.masks[u.row0 + row] : 0ull;
+      for (int i = 0; i < QC; ++i) {
+        const int col = i * PASS + threadIdx.x / TPC;
+        const bool live = col < u.n_cols;
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(x[i][k]));
+#pragma unroll
+        for (int o = 1; o < TPC; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        int ex = 0;
+        if (p.q.dtype == T_BF16 && a > 0.f && a < INFINITY) ex = min(max((__float_as_int(a) >> 23) - 127, -100), 126);
+        const float down = __int_as_float((127 - ex) << 23);
+        if (col < NT * 8) {
+          uint32_t f[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[k] = live ? pack2(x[i][k] * down, x[i][k + 4] * down) : 0u;
+          uint32_t* dst = qs + (((col / 8) * Sh::KS + 2 * w) * 32 + (col % 8) * 4 + tt) * 2;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(f[0], f[1]);
+          *reinterpret_cast<uint2*>(dst + 64) = make_uint2(f[2], f[3]);
+          if (ch == 0) {
+            const int row = (u.col0 + col) / G;
+            mt->c[col] = p.scale * 1.4426950408889634f * __int_as_float((ex + 127) << 23);
+            mt->idx[col] = live ? row : -1;
+            mt->mask[col] = live && p.masks ? p.masks[u.row0 + row] : 0ull;
+          }
+        }
       }
     }
-    bar_consumers();
+    __syncthreads();
     State<D, NT> s;
     s.clear();
     float c[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) c[n][0] = mt->c[n * 8 + 2 * t], c[n][1] = mt->c[n * 8 + 2 * t + 1];
 
-    for (int st = u.st0; st < u.st1; ++st, ++k) {
-      const int slot = k % Sh::STAGES;
-      ok = ok && mbar_wait_bounded(&full[slot], (k / Sh::STAGES) & 1, p.err);
-      const int tok = st * kStageTokens + warp * 16;
-      if (ok && tok < u.kv_end) {
-        const int pi = warp * 16 / P, j0 = warp * 16 % P;
-        const uint8_t* b = smem + slot * Sh::STAGE + pi * blk;
-        const uint8_t* kc = b + j0 * (D / 2) + k_at;
-        const uint8_t* ksc = b + k_scales_at(P, D) + j0 * (D / 8) + ks_at;
-        const uint8_t* vc = b + v_codes_at(P, D) + j0 * (D / 2);
-        const uint8_t* vsc = b + v_scales_at(P, D) + j0 * (D / 8) + vs_at;
+    const int end = min(u.st1 * (kStageTokens / kTile), (u.kv_end + kTile - 1) / kTile);
+#pragma unroll 1
+    for (int tile = u.st0 * (kStageTokens / kTile) + warp; tile < end; tile += kWarps) {
+      ok = ok && mbar_wait_bounded(&full[slot], phase, p.err);
+      const int tok = tile * kTile;
+      const uint8_t* b = ring + slot * Sh::TILE;
+      // What column `lane` sees of the tile's tokens, and the tokens whose V
+      // counts.  A stored NaN row of V is NaN in every scale; its value is
+      // taken as zero and the NaN given to the scores of the columns that see
+      // it, so that no other column meets it.
+      const bool tail = tok + kTile > u.kv_len;
+      uint32_t sees = ~0u, live = ~0u, bad = 0u;
+      if (tail) {
+        const int x = tok - u.kv_len, left = u.kv_end - tok;
+        if (p.masks) {
+          const unsigned long long m = lane < NT * 8 ? mt->mask[lane] : 0ull;
+          sees = x >= 0 ? (uint32_t)(m >> min(x, 63)) : ((uint32_t)m << min(-x, 31)) | ((1u << min(-x, 31)) - 1);
+        } else {
+          const int n = (lane < NT * 8 ? mt->idx[lane] : -1) + 1 - x;
+          sees = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
+        }
+        live = left >= 32 ? ~0u : (1u << left) - 1;
+        const uint32_t one = *reinterpret_cast<const uint32_t*>(b + (lane >> 4) * scale16 + vs0 +
+                                                                (lane >> 1 & 7) * (D / 32 * 8) + (lane & 1) * 4);
+        bad = __ballot_sync(0xffffffffu, (one & 0x7fffu) > 0x7c00u) & live;
+        sees &= live;
+        live &= ~bad;
+      }
+      // Both 16-token halves at once: one at a time fetches half the code but
+      // leaves the chains of the few resident warps too short (24 sequences of
+      // 9 rows and 7 query heads: 94 us against 130).
+      constexpr int H = 2;
+#pragma unroll 1
+      for (int h0 = 0; h0 < 2; h0 += H) {
+        const uint8_t* bc = b + h0 * code16;
+        const uint8_t* bs = b + h0 * scale16;
         // S^T
-        float sc[NT][4];
+        float sc[H][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
         {
-          uint32_t wa[KW], wb[KW];
-          if constexpr (KW == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kc), y = *reinterpret_cast<const uint4*>(kc + 8 * (D / 2));
-            wa[0] = x.x, wa[1] = x.y, wa[2] = x.z, wa[3] = x.w;
-            wb[0] = y.x, wb[1] = y.y, wb[2] = y.z, wb[3] = y.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(kc), y = *reinterpret_cast<const uint2*>(kc + 8 * (D / 2));
-            wa[0] = x.x, wa[1] = x.y;
-            wb[0] = y.x, wb[1] = y.y;
-          }
-          const uint32_t ra = *reinterpret_cast<const uint32_t*>(ksc), rb = *reinterpret_cast<const uint32_t*>(ksc + D);
-          const uint32_t sa = prmt(ra, ra, 0x1010), oa = prmt(ra, ra, 0x3232);
-          const uint32_t sb = prmt(rb, rb, 0x1010), ob = prmt(rb, rb, 0x3232);
+          uint32_t w[H][2][KW], s2[H][2], o2[H][2];  // [half][token g / g + 8]
 #pragma unroll
-          for (int w = 0; w < KW; ++w) {
-            {
-              const uint32_t a0 = dq<0>(wa[w], sa, oa), a1 = dq<0>(wb[w], sb, ob);
-              const uint32_t a2 = dq<1>(wa[w], sa, oa), a3 = dq<1>(wb[w], sb, ob);
+          for (int h = 0; h < H; ++h)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint2 q = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * w) * 32 + lane) * 2);
-                mma(sc[n], a0, a1, a2, a3, q.x, q.y);
+            for (int e = 0; e < 2; ++e) {
+              const uint8_t* kc = bc + h * code16 + k_at + e * 8 * (D / 2);
+              if constexpr (KW == 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(kc);
+                w[h][e][0] = x.x, w[h][e][1] = x.y, w[h][e][2] = x.z, w[h][e][3] = x.w;
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(kc);
+                w[h][e][0] = x.x, w[h][e][1] = x.y;
               }
+              const uint32_t r = *reinterpret_cast<const uint32_t*>(bs + h * scale16 + ks_at + e * D);
+              s2[h][e] = prmt(r, r, 0x1010);
+              o2[h][e] = prmt(r, r, 0x3232);
             }
-            {
-              const uint32_t a0 = dq<2>(wa[w], sa, oa), a1 = dq<2>(wb[w], sb, ob);
-              const uint32_t a2 = dq<3>(wa[w], sa, oa), a3 = dq<3>(wb[w], sb, ob);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                const uint2 q = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * w + 1) * 32 + lane) * 2);
-                mma(sc[n], a0, a1, a2, a3, q.x, q.y);
-              }
+          for (int i = 0; i < KW; ++i) {
+            uint2 q[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              q[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i) * 32 + lane) * 2);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              const uint32_t a0 = dq<0>(w[h][0][i], s2[h][0], o2[h][0]), a1 = dq<0>(w[h][1][i], s2[h][1], o2[h][1]);
+              const uint32_t a2 = dq<1>(w[h][0][i], s2[h][0], o2[h][0]), a3 = dq<1>(w[h][1][i], s2[h][1], o2[h][1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(sc[h][n], a0, a1, a2, a3, q[n].x, q[n].y);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              q[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i + 1) * 32 + lane) * 2);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+              const uint32_t a0 = dq<2>(w[h][0][i], s2[h][0], o2[h][0]), a1 = dq<2>(w[h][1][i], s2[h][1], o2[h][1]);
+              const uint32_t a2 = dq<3>(w[h][0][i], s2[h][0], o2[h][0]), a3 = dq<3>(w[h][1][i], s2[h][1], o2[h][1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(sc[h][n], a0, a1, a2, a3, q[n].x, q[n].y);
             }
           }
         }
         // Scales of V, (s, s') and (o, o') of the token pairs (2t, 2t + 1), (2t + 8, 2t + 9).
-        uint32_t vs[2], vo[2];
+        uint32_t vs[H][2], vo[H][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint2 r = *reinterpret_cast<const uint2*>(vsc + h * (4 * (D / 32) * 8));
-          vs[h] = prmt(r.x, r.y, 0x5410);
-          vo[h] = prmt(r.x, r.y, 0x7632);
-        }
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int e = 0; e < 2; ++e) {
+            const uint2 r = *reinterpret_cast<const uint2*>(bs + h * scale16 + vs_at + e * (4 * (D / 32) * 8));
+            vs[h][e] = prmt(r.x, r.y, 0x5410);
+            vo[h][e] = prmt(r.x, r.y, 0x7632);
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[n][i] *= c[n][i & 1];
-        if (tok + 16 > u.kv_len) {
-          // Tokens of this step, or past the end.  A stored NaN row of V is NaN
-          // in every scale; its value is taken as zero and the NaN given to the
-          // scores of the columns that see it, so that no other column meets it.
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[h][n][i] *= c[n][i & 1];
+        if (tail) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int j = tok + 2 * t + 8 * h + e;
-              const uint32_t keep = e ? 0x0000ffffu : 0xffff0000u;
-              const bool bad = ((vs[h] >> (16 * e)) & 0x7fffu) > 0x7c00u;
-              if (j >= u.kv_end || bad) vs[h] &= keep, vo[h] &= keep;
+              const uint32_t two = live >> (16 * (h0 + h) + 8 * e + 2 * t);
+              const uint32_t keep = ((two & 1) ? 0x0000ffffu : 0u) | ((two & 2) ? 0xffff0000u : 0u);
+              vs[h][e] &= keep;
+              vo[h][e] &= keep;
             }
-            const int j = tok + g + 8 * h, w = j - u.kv_len;
-            const uint8_t* one = b + v_scales_at(P, D) + ((j0 + g + 8 * h) >> 1) * (D / 32 * 8) + (g & 1) * 4;
-            const bool bad = (*reinterpret_cast<const uint32_t*>(one) & 0x7fffu) > 0x7c00u;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int col = n * 8 + 2 * t + e;
-                const bool sees = w < 0 || (j < u.kv_end && (p.masks ? (mt->mask[col] >> w) & 1 : w <= mt->idx[col]));
-                float& x = sc[n][2 * h + e];
-                x = !sees ? -INFINITY : bad ? __int_as_float(0x7fffffff) : x;
-              }
-          }
+            for (int f = 0; f < 2; ++f) {
+              const uint32_t of_col = __shfl_sync(0xffffffffu, sees, n * 8 + 2 * t + f) >> (16 * h0 + g);
+              const uint32_t nan = (bad >> (16 * h0 + g)) & of_col;
+#pragma unroll
+              for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float& y = sc[h][n][2 * e + f];
+                  y = (of_col >> (16 * h + 8 * e)) & 1 ? y : -INFINITY;
+                  if ((nan >> (16 * h + 8 * e)) & 1) y = __int_as_float(0x7fffffff);
+                }
+            }
         }
         // Move the reference where a score passes it by more than kSlack.
         bool over = false;
+        float top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) over |= fmaxf(sc[n][e], sc[n][2 + e]) > s.m[n][e] + kSlack;
+          for (int e = 0; e < 2; ++e) {
+            top[n][e] = fmaxf(sc[0][n][e], sc[0][n][2 + e]);
+            if (H == 2) top[n][e] = fmaxf(top[n][e], fmaxf(sc[H - 1][n][e], sc[H - 1][n][2 + e]));
+            over |= top[n][e] > s.m[n][e] + kSlack;
+          }
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(sc[n][e], sc[n][2 + e]);
+              float x = top[n][e];
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
               s.rescale(n, e, fmaxf(s.m[n][e], x));
             }
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[H][NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[n][i] = ex2(sc[n][i] - s.m[n][i & 1]);
-          s.l[n][0] += sc[n][0] + sc[n][2];
-          s.l[n][1] += sc[n][1] + sc[n][3];
-          pb[n][0] = movmatrix(pack2(sc[n][0], sc[n][1]));
-          pb[n][1] = movmatrix(pack2(sc[n][2], sc[n][3]));
-        }
+          for (int n = 0; n < NT; ++n) {
+            float(&x)[4] = sc[h][n];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - s.m[n][i & 1]);
+            s.l[n][0] += x[0] + x[2];
+            s.l[n][1] += x[1] + x[3];
+            pb[h][n][0] = movmatrix(pack2(x[0], x[1]));
+            pb[h][n][1] = movmatrix(pack2(x[2], x[3]));
+          }
         // O^T
-        uint32_t w[4][VW];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (VW == 2) {
-            const uint2 x = *reinterpret_cast<const uint2*>(vc + v_at[e]);
-            w[e][0] = x.x, w[e][1] = x.y;
-          } else {
-            w[e][0] = *reinterpret_cast<const uint32_t*>(vc + v_at[e]);
+        for (int h = 0; h < H; ++h) {
+          uint32_t w[4][VW];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint8_t* vc = bc + h * code16 + v_at[e];
+            if constexpr (VW == 2) {
+              const uint2 x = *reinterpret_cast<const uint2*>(vc);
+              w[e][0] = x.x, w[e][1] = x.y;
+            } else {
+              w[e][0] = *reinterpret_cast<const uint32_t*>(vc);
+            }
           }
+#pragma unroll
+          for (int i = 0; i < VW; ++i)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const uint32_t sel = f ? 0x7632 : 0x5410;
+              const uint32_t x = prmt(w[0][i], w[1][i], sel), y = prmt(w[2][i], w[3][i], sel);
+              {
+                const uint32_t a0 = dq<0>(x, vs[h][0], vo[h][0]), a1 = dq<1>(x, vs[h][0], vo[h][0]);
+                const uint32_t a2 = dq<0>(y, vs[h][1], vo[h][1]), a3 = dq<1>(y, vs[h][1], vo[h][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(s.o[4 * i + 2 * f][n], a0, a1, a2, a3, pb[h][n][0], pb[h][n][1]);
+              }
+              {
+                const uint32_t a0 = dq<2>(x, vs[h][0], vo[h][0]), a1 = dq<3>(x, vs[h][0], vo[h][0]);
+                const uint32_t a2 = dq<2>(y, vs[h][1], vo[h][1]), a3 = dq<3>(y, vs[h][1], vo[h][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(s.o[4 * i + 2 * f + 1][n], a0, a1, a2, a3, pb[h][n][0], pb[h][n][1]);
+              }
+            }
         }
-#pragma unroll
-        for (int i = 0; i < VW; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t sel = h ? 0x7632 : 0x5410;
-            const uint32_t x = prmt(w[0][i], w[1][i], sel), y = prmt(w[2][i], w[3][i], sel);
-            {
-              const uint32_t a0 = dq<0>(x, vs[0], vo[0]), a1 = dq<1>(x, vs[0], vo[0]);
-              const uint32_t a2 = dq<0>(y, vs[1], vo[1]), a3 = dq<1>(y, vs[1], vo[1]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma(s.o[4 * i + 2 * h][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-            }
-            {
-              const uint32_t a0 = dq<2>(x, vs[0], vo[0]), a1 = dq<3>(x, vs[0], vo[0]);
-              const uint32_t a2 = dq<2>(y, vs[1], vo[1]), a3 = dq<3>(y, vs[1], vo[1]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma(s.o[4 * i + 2 * h + 1][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-            }
-          }
       }
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[slot])) : "memory");
+      __syncwarp();  // every lane has read the slot
+      if (cur.more() && ok) {
+        if (lane == 0) copy_tile<D>(p, cur, ring + slot * Sh::TILE, &full[slot]);
+        cur.advance(p, warp);
+      }
+      if (++slot == Sh::STAGES) slot = 0, phase ^= 1;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -490,85 +656,76 @@ __global__ void __launch_bounds__(kThreads, NT <= 1 ? 2 : 1) attend_kernel(const
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) s.l[n][e] += __shfl_xor_sync(0xffffffffu, s.l[n][e], o);
     join_warps<D, NT>(s, merge, mt, warp, lane);
-    if (u.n_parts == 1) {
-      if (warp == 0) write_out<D, NT>(s, p, u, lane);
-      continue;
-    }
-    // Leave a partial state; the last CTA of the group to arrive joins all.
+    // Up the tree: leave a partial state, and go on where this CTA is the last
+    // of its kFanIn to arrive.
     constexpr int PART = Sh::FRAG * 32 + NT * 16;  // floats
-    if (warp == 0) {
-      float* dst = p.parts + (long long)(u.part0 + u.part) * PART;
-#pragma unroll
-      for (int a = 0; a < Sh::MT; ++a)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          __stcg(reinterpret_cast<float4*>(dst) + (a * NT + n) * 32 + lane,
-                 make_float4(s.o[a][n][0], s.o[a][n][1], s.o[a][n][2], s.o[a][n][3]));
-      if (lane < 4) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            __stcg(dst + Sh::FRAG * 32 + n * 8 + 2 * t + e, s.m[n][e]);
-            __stcg(dst + Sh::FRAG * 32 + NT * 8 + n * 8 + 2 * t + e, s.l[n][e]);
-          }
+    int n = u.n_parts, at = u.part;
+    long long base = u.part0;
+    int* arrived = p.arrived + u.group;
+    while (n > 1) {
+      const int node = at / kFanIn, first = node * kFanIn, count = min(kFanIn, n - first);
+      if (warp == 0) {
+        leave_part<D, NT>(s, p.parts + (base + at) * PART, lane);
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+          const bool last = atomicAdd(arrived + node, 1) == count - 1;
+          if (last) arrived[node] = 0;  // ready for the next call
+          mt->last = last;
+        }
       }
+      __syncthreads();
+      const bool last = mt->last;
+      if (!last) break;
       __threadfence();
-      __syncwarp();
-      if (lane == 0) {
-        const int before = atomicAdd(p.arrived + u.group, 1);
-        mt->last = before == u.n_parts - 1;
-        if (mt->last) p.arrived[u.group] = 0;  // ready for the next call
-      }
+      s.clear();
+      for (int i = warp; i < count; i += kWarps) take_part<D, NT>(s, p.parts + (base + first + i) * PART, lane);
+      join_warps<D, NT>(s, merge, mt, warp, lane);
+      base += n;
+      n = (n + kFanIn - 1) / kFanIn;
+      arrived += n;
+      at = node;
     }
-    bar_consumers();
-    if (!mt->last) continue;
-    __threadfence();
-    s.clear();
-    for (int i = warp; i < u.n_parts; i += kConsumers) {
-      const float* src = p.parts + (long long)(u.part0 + i) * PART;
-      float b[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float om = __ldcg(src + Sh::FRAG * 32 + n * 8 + 2 * t + e);
-          const float mm = fmaxf(s.m[n][e], om);
-          s.rescale(n, e, mm);
-          b[n][e] = ex2(om - mm);
-          s.l[n][e] += __ldcg(src + Sh::FRAG * 32 + NT * 8 + n * 8 + 2 * t + e) * b[n][e];
-        }
-#pragma unroll
-      for (int a = 0; a < Sh::MT; ++a)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + (a * NT + n) * 32 + lane);
-          s.o[a][n][0] += x.x * b[n][0];
-          s.o[a][n][1] += x.y * b[n][1];
-          s.o[a][n][2] += x.z * b[n][0];
-          s.o[a][n][3] += x.w * b[n][1];
-        }
-    }
-    join_warps<D, NT>(s, merge, mt, warp, lane);
-    if (warp == 0) write_out<D, NT>(s, p, u, lane);
-    bar_consumers();  // mt->last is read before the next unit writes it
+    if (n == 1) write_out<D, NT>(s, p, u, merge, warp, lane);
+    if (next == u.last) break;
+    u = p.units[next];
+    __syncthreads();  // mt and qs are free for the next unit
+  }
+  if (!ok && lane == 0) {  // leave no copy of this warp in flight
+    for (int i = 0; i < Sh::STAGES; ++i) mbar_wait_bounded(&full[i], (i < slot ? phase ^ 1 : phase), p.err);
   }
 }
 
 template <int D, int NT>
+int smem_bytes() {
+  return Shape<D, NT>::META_AT + (int)sizeof(Meta);
+}
+
+template <int D, int NT>
 cudaError_t launch(const AttendParams& p, cudaStream_t s) {
-  constexpr int smem = Shape<D, NT>::SMEM + 1024;
-  const cudaError_t e =
-      cudaFuncSetAttribute(attend_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  attend_kernel<D, NT><<<p.n_ctas, kThreads, smem, s>>>(p);
+  attend_kernel<D, NT><<<p.n_ctas, kThreads, smem_bytes<D, NT>(), s>>>(p);
   return cudaGetLastError();
+}
+template <int D, int NT>
+cudaError_t allow() {
+  return cudaFuncSetAttribute(attend_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, NT>());
 }
 
 }  // namespace
 
+cudaError_t attend_setup() {
+  cudaError_t e = allow<128, 1>();
+  if (e == cudaSuccess) e = allow<128, 2>();
+  if (e == cudaSuccess) e = allow<128, 3>();
+  if (e == cudaSuccess) e = allow<128, 4>();
+  if (e == cudaSuccess) e = allow<64, 1>();
+  if (e == cudaSuccess) e = allow<64, 2>();
+  if (e == cudaSuccess) e = allow<64, 3>();
+  if (e == cudaSuccess) e = allow<64, 4>();
+  return e;
+}
 size_t attend_part_floats(int head_dim, int nt) { return (size_t)head_dim / 16 * nt * 4 * 32 + nt * 16; }
-int attend_ctas_per_sm(int nt) { return nt <= 1 ? 2 : 1; }
+int attend_ctas_per_sm(int nt) { return ctas_per_sm(nt); }
 
 cudaError_t launch_attend(const AttendParams& p, int head_dim, int nt, cudaStream_t s) {
   if (p.n_ctas <= 0) return cudaSuccess;

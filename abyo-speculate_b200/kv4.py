@@ -16,11 +16,15 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
 
 from . import _lib
+
+
+_ROWS = struct.Struct("=Qqqqii")  # spec_kv4_rows
 
 
 def _invalid(msg: str) -> _lib.SamplingError:
@@ -132,8 +136,18 @@ class KV4Batch:
         self._h = h
         self.n_rows = 0
         self._types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-        self._arg = [_lib.KV4Rows() for _ in range(6)]
-        self._ref = [ctypes.addressof(a) for a in self._arg]
+        # One buffer of spec_kv4_rows structures: a call packs its tensors into
+        # the first slots (a few hundred ns each, where a call is microseconds).
+        size = ctypes.sizeof(_lib.KV4Rows)
+        self._buf = ctypes.create_string_buffer(6 * size)
+        at = ctypes.addressof(self._buf)
+        self._slots = [(i * size, at + i * size) for i in range(6)]
+        self._index = cache.device.index
+        self._scale = cache.head_dim ** -0.5
+        # The raw handle of torch's current stream, without a Stream object around it.
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            self._stream = lambda: raw(self._index)
 
     def plan(self, kv_len: Sequence[int], n_rows: Sequence[int], page_table, positions=None, masks=None,
              src_rows=None) -> None:
@@ -163,27 +177,29 @@ class KV4Batch:
         self.n_rows = total
 
     def _stream(self) -> int:
-        return self._torch.cuda.current_stream(self.cache.device).cuda_stream
+        return self._torch.cuda.current_stream(self._index).cuda_stream
 
     def _rows(self, i: int, t, heads: int, what: str):
-        """Fills argument slot i from tensor t [rows, heads, head_dim]; returns its address."""
+        """Packs tensor t [rows, heads, head_dim] into slot i; returns the slot's address."""
         if t is None:
             return None
-        dim = self.cache.head_dim
-        shape = t.shape
-        if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
-            raise _invalid(f"{what} has shape {tuple(shape)}, [rows, {heads}, {dim}] is needed")
-        if t.device != self.cache.device:
-            raise _invalid(f"{what} is on {t.device}, the pool on {self.cache.device}")
-        row, head, ch = t.stride()
+        try:
+            n, h, d = t.shape
+            row, head, ch = t.stride()
+            kind = self._types[t.dtype]
+        except ValueError:
+            h = d = ch = None
+        except KeyError:
+            raise _invalid(f"{what} is {t.dtype}: bfloat16, float16 and float32 are taken") from None
+        if h != heads or d != self.cache.head_dim:
+            raise _invalid(f"{what} has shape {tuple(t.shape)}, [rows, {heads}, {self.cache.head_dim}] is needed")
         if ch != 1:
             raise _invalid(f"the channels of {what} are not contiguous")
-        kind = self._types.get(t.dtype)
-        if kind is None:
-            raise _invalid(f"{what} is {t.dtype}: bfloat16, float16 and float32 are taken")
-        a = self._arg[i]
-        a.ptr, a.row_stride, a.head_stride, a.n_rows, a.dtype = t.data_ptr(), row, head, shape[0], kind
-        return self._ref[i]
+        if t.get_device() != self._index:
+            raise _invalid(f"{what} is on {t.device}, the pool on {self.cache.device}")
+        off, ref = self._slots[i]
+        _ROWS.pack_into(self._buf, off, t.data_ptr(), row, head, n, kind, 0)
+        return ref
 
     def append(self, layer: int, q, k, v, q_out=None, k_out=None, v_out=None):
         """Stores the plan's rows of k and v in `layer`'s pages, k rotated, and
@@ -194,10 +210,12 @@ class KV4Batch:
         if q is not None and q_out is None:
             q_out = self._torch.empty((self.n_rows, c.n_heads, c.head_dim), dtype=q.dtype, device=c.device)
         rows = self._rows
-        _lib.check(self._lib.spec_kv4_append(
+        rc = self._lib.spec_kv4_append(
             self._h, layer, rows(0, q, c.n_heads, "q"), rows(1, q_out, c.n_heads, "q_out"),
             rows(2, k, c.n_kv_heads, "k"), rows(3, v, c.n_kv_heads, "v"), rows(4, k_out, c.n_kv_heads, "k_out"),
-            rows(5, v_out, c.n_kv_heads, "v_out"), self._stream()))
+            rows(5, v_out, c.n_kv_heads, "v_out"), self._stream())
+        if rc:
+            _lib.check(rc)
         return q_out
 
     def attend(self, layer: int, q, out=None, scale: Optional[float] = None):
@@ -207,9 +225,11 @@ class KV4Batch:
         c = self.cache
         if out is None:
             out = self._torch.empty((self.n_rows, c.n_heads, c.head_dim), dtype=q.dtype, device=c.device)
-        _lib.check(self._lib.spec_kv4_attend(self._h, layer, self._rows(0, q, c.n_heads, "q"),
-                                             self._rows(1, out, c.n_heads, "out"),
-                                             c.head_dim ** -0.5 if scale is None else scale, self._stream()))
+        rc = self._lib.spec_kv4_attend(self._h, layer, self._rows(0, q, c.n_heads, "q"),
+                                       self._rows(1, out, c.n_heads, "out"),
+                                       self._scale if scale is None else scale, self._stream())
+        if rc:
+            _lib.check(rc)
         return out
 
     def status(self) -> None:

@@ -516,10 +516,11 @@ int spec_qmatmul_noalloc(spec_qweight* w, const float* x_dev, int M, float* y_de
  *
  * Conventions of these calls: every pointer marked "device" belongs to the
  * caller; `stream` is the cudaStream_t the call's work is queued on (NULL =
- * CUDA's default stream) and nothing is synchronised.  A batch handle orders
- * its own calls: one made on another stream than the call before it waits for
- * that call on the device.  Calls on a stream under capture are recorded
- * without that ordering.  Messages: spec_last_error(NULL). */
+ * CUDA's default stream) and nothing is synchronised, but for a batch's first
+ * change of stream, which waits for the device once.  A batch handle orders
+ * its own calls: one made on another stream than the call before it runs after
+ * that call.  Calls on a stream under capture are recorded without that
+ * ordering.  Messages: spec_last_error(NULL). */
 typedef struct spec_kv4 spec_kv4;
 typedef struct spec_kv4_batch spec_kv4_batch;
 typedef struct spec_kv4_desc {
@@ -600,7 +601,7 @@ int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
  * timing; a row's last bits may depend on the other rows of the plan. */
 int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* out, float scale,
                     void* stream);
-/* Synchronises the batch's last stream and reports (and clears) a device wait
+/* Waits for the batch's calls and reports (and clears) a device wait
  * that gave up in an earlier call (SPEC_ERR_TIMEOUT). */
 int spec_kv4_status(spec_kv4_batch* b);
 
