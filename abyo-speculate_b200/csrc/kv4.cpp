@@ -2,6 +2,7 @@
 // argument that the kernels rely on.  A plan is validated on the host and kept
 // in device memory of the library's own, so the kernels need no bounds checks
 // on pages and slots.
+#include <stdlib.h>
 #include <limits.h>
 #include <stdio.h>
 #include <string.h>
@@ -70,6 +71,18 @@ struct spec_kv4 {
   std::shared_ptr<Cache> c;
 };
 
+namespace {
+
+// What one attention kernel does in a step.
+struct Schedule {
+  std::vector<Unit> order;  // first units of all CTAs, then each CTA's others
+  const Unit* units = nullptr;  // the same on the device
+  int n_ctas = 0, n_parts = 0, n_groups = 0;
+  int nt = 1;                   // 8-column tiles of the largest unit
+};
+
+}  // namespace
+
 struct spec_kv4_batch {
   std::shared_ptr<Cache> c;
   // The plan: one device allocation, written from one pinned one.
@@ -86,15 +99,15 @@ struct spec_kv4_batch {
   const RowDev* rows = nullptr;
   const int* table = nullptr;
   const unsigned long long* masks = nullptr;
-  // The attention's schedule, and its workspace: arrival counters (zero
-  // between calls) and partial states.
-  const Unit* units = nullptr;
-  int n_ctas = 0, nt = 1, sms = 0;
+  // The attention's schedules (narrow and wide kernel), and their workspace:
+  // arrival counters (zero between calls) and partial states.
+  Schedule narrow, wide;
+  int sms = 0;
   int* arrived = nullptr;
   size_t arrived_cap = 0;
   float* parts = nullptr;
   size_t parts_cap = 0;
-  std::vector<Unit> tiles, runs, order;
+  std::vector<Unit> tiles, runs;
   std::vector<int> cuts;
   std::vector<uint8_t> seen;  // per page: 1 = read, 2 = written; zero between plans
 };
@@ -223,25 +236,30 @@ bool wide(const spec_kv4_rows* r) {
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-// Cuts the step's attention into units: per (sequence, kv head, tile of at
-// most 32 columns) the 128-token stages its rows see, then those stages, laid
-// end to end, into runs of equal length, one a CTA.  Returns the partial
-// states and arrival counters needed.
-void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_groups) {
+const int kWideFrom = getenv("WIDE") ? atoi(getenv("WIDE")) : 64;
+// Cuts the step's attention into units: per (sequence, kv head, tile of
+// columns) the 128-token stages its rows see, then those stages, laid end to
+// end, into runs of equal length, one a CTA.  Sequences of more than kWideFrom
+// columns go to the wide kernel.
+void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
   const Cache& c = *b->c;
+  Schedule& out = wide ? b->wide : b->narrow;
   const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
+  const int most = wide ? kWideCols : kMaxCols;
   b->tiles.clear();
   b->runs.clear();
-  b->order.clear();
   b->cuts.clear();
-  b->nt = 1;
+  out.order.clear();
+  out.n_ctas = out.n_parts = out.n_groups = 0;
+  out.nt = 1;
   int64_t stages = 0;
   int row0 = 0, table = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int n = s->kv_len[q], m = s->n_rows[q], cols = m * G;
-    const int tiles = (cols + kMaxCols - 1) / kMaxCols;
-    const int size = tiles ? ((cols + tiles - 1) / tiles + 7) / 8 * 8 : 0;
-    for (int h = 0; h < c.d.n_kv_heads; ++h)
+    const int tiles = (cols + most - 1) / most;
+    // Narrow tiles are of equal size, wide ones full but for the last.
+    const int size = wide ? most : tiles ? ((cols + tiles - 1) / tiles + 7) / 8 * 8 : 0;
+    for (int h = 0; h < c.d.n_kv_heads && (cols > kWideFrom) == wide; ++h)
       for (int c0 = 0; c0 < cols; c0 += size) {
         Unit u{};
         u.kvh = h;
@@ -253,16 +271,14 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_gr
         u.st1 = (u.kv_end + kStageTokens - 1) / kStageTokens;
         u.table = table;
         stages += u.st1;
-        if ((u.n_cols + 7) / 8 > b->nt) b->nt = (u.n_cols + 7) / 8;
+        if ((u.n_cols + 7) / 8 > out.nt) out.nt = (u.n_cols + 7) / 8;
         b->tiles.push_back(u);
       }
     row0 += m;
     table += (n + m + P - 1) / P;
   }
-  *n_parts = *n_groups = 0;
-  b->n_ctas = 0;
   if (b->tiles.empty()) return;
-  const int64_t slots = (int64_t)b->sms * attend_ctas_per_sm(b->nt);
+  const int64_t slots = (int64_t)b->sms * (wide ? 1 : attend_ctas_per_sm(out.nt));
   const int64_t run = (stages + slots - 1) / slots;
   int64_t left = run;
   b->cuts.push_back(0);
@@ -284,26 +300,25 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, int* n_parts, int* n_gr
     const int parts = (int)(b->runs.size() - first);
     for (size_t i = first; i < b->runs.size(); ++i) {
       b->runs[i].n_parts = parts;
-      b->runs[i].part0 = *n_parts;
-      b->runs[i].group = *n_groups;
+      b->runs[i].part0 = out.n_parts;
+      b->runs[i].group = out.n_groups;
     }
     for (int n = parts; n > 1;) {
-      *n_parts += n;
+      out.n_parts += n;
       n = (n + kFanIn - 1) / kFanIn;
-      *n_groups += n;
+      out.n_groups += n;
     }
   }
   if (b->cuts.back() != (int)b->runs.size()) b->cuts.push_back((int)b->runs.size());
-  b->n_ctas = (int)b->cuts.size() - 1;
-  // The order the kernel reads: first units of all CTAs, then each CTA's others.
-  b->order.resize(b->runs.size());
-  int at = b->n_ctas;
-  for (int i = 0; i < b->n_ctas; ++i) {
+  out.n_ctas = (int)b->cuts.size() - 1;
+  out.order.resize(b->runs.size());
+  int at = out.n_ctas;
+  for (int i = 0; i < out.n_ctas; ++i) {
     const int first = b->cuts[i], n = b->cuts[i + 1] - first;
     for (int k = 0; k < n; ++k) {
-      Unit& u = k == 0 ? b->order[i] : b->order[at + k - 1];
+      Unit& u = k == 0 ? out.order[i] : out.order[at + k - 1];
       u = b->runs[first + k];
-      u.next = at + k;
+      u.next = at;
       u.last = at + n - 1;
     }
     at += n - 1;
@@ -366,11 +381,12 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   if (!s->src_rows) max_src = (int)rows - 1;
 
   b->planned = false;
-  int n_parts = 0, n_groups = 0;
-  schedule(b, s, &n_parts, &n_groups);
+  schedule(b, s, false);
+  schedule(b, s, true);
   // One block: rows, masks, pages, units.
   const size_t at_rows = 0, at_masks = at_rows + up(sizeof(RowDev) * rows), at_table = at_masks + (s->masks ? up(8 * rows) : 0),
-               at_units = at_table + up(4 * pages), total = at_units + up(sizeof(Unit) * b->order.size());
+               at_narrow = at_table + up(4 * pages), at_wide = at_narrow + up(sizeof(Unit) * b->narrow.order.size()),
+               total = at_wide + up(sizeof(Unit) * b->wide.order.size());
   Turn turn{b, stream};
   cudaError_t e = turn.enter();
   if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
@@ -392,8 +408,11 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   } else if (b->used && (e = cudaEventSynchronize(b->copied)) != cudaSuccess) {
     return fail_cuda(e, "spec_kv4_plan");  // the staging buffer is still being read
   }
-  if ((e = grow(b, &b->arrived, &b->arrived_cap, n_groups, true)) != cudaSuccess ||
-      (e = grow(b, &b->parts, &b->parts_cap, n_parts * attend_part_floats(c.d.head_dim, b->nt), false)) != cudaSuccess)
+  // The two kernels run one after the other and share the partial states.
+  const size_t floats_narrow = b->narrow.n_parts * attend_part_floats(c.d.head_dim, b->narrow.nt),
+               floats_wide = b->wide.n_parts * wide_part_floats(c.d.head_dim);
+  if ((e = grow(b, &b->arrived, &b->arrived_cap, b->narrow.n_groups + b->wide.n_groups, true)) != cudaSuccess ||
+      (e = grow(b, &b->parts, &b->parts_cap, floats_narrow > floats_wide ? floats_narrow : floats_wide, false)) != cudaSuccess)
     return fail_cuda(e, "spec_kv4_plan");
   RowDev* hr = reinterpret_cast<RowDev*>(b->host + at_rows);
   int* ht = reinterpret_cast<int*>(b->host + at_table);
@@ -411,11 +430,12 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
     }
   }
   if (s->masks) memcpy(b->host + at_masks, s->masks, 8 * (size_t)rows);
-  for (Unit& u : b->order) {
+  for (Unit& u : b->narrow.order) {
     const int per = kStageTokens / P, first = u.st0 * per, n = (u.kv_end + P - 1) / P - first;
     for (int i = 0; i < per && i < n; ++i) u.pages[i] = ht[u.table + first + i];
   }
-  if (!b->order.empty()) memcpy(b->host + at_units, b->order.data(), sizeof(Unit) * b->order.size());
+  if (b->narrow.n_ctas) memcpy(b->host + at_narrow, b->narrow.order.data(), sizeof(Unit) * b->narrow.order.size());
+  if (b->wide.n_ctas) memcpy(b->host + at_wide, b->wide.order.data(), sizeof(Unit) * b->wide.order.size());
   if (total && (e = cudaMemcpyAsync(b->dev, b->host, total, cudaMemcpyHostToDevice, stream)) != cudaSuccess)
     return fail_cuda(e, "spec_kv4_plan");
   if ((e = cudaEventRecord(b->copied, stream)) != cudaSuccess) return fail_cuda(e, "spec_kv4_plan");
@@ -428,7 +448,8 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   b->rows = reinterpret_cast<const RowDev*>(b->dev + at_rows);
   b->masks = s->masks ? reinterpret_cast<const unsigned long long*>(b->dev + at_masks) : nullptr;
   b->table = reinterpret_cast<const int*>(b->dev + at_table);
-  b->units = reinterpret_cast<const Unit*>(b->dev + at_units);
+  b->narrow.units = reinterpret_cast<const Unit*>(b->dev + at_narrow);
+  b->wide.units = reinterpret_cast<const Unit*>(b->dev + at_wide);
   b->planned = true;
   return SPEC_OK;
 }
@@ -487,6 +508,7 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);
   if (e == cudaSuccess) e = attend_setup();
+  if (e == cudaSuccess) e = wide_setup();
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&b->err), 16);
   if (e == cudaSuccess) e = cudaMemset(b->err, 0, 16);
   if (e != cudaSuccess) {
@@ -594,7 +616,6 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   if (cur.rc != SPEC_OK) return cur.rc;
   AttendParams p;
   p.pool = c.pool + layer * c.layer_bytes();
-  p.units = b->units;
   p.table = b->table;
   p.masks = b->masks;
   p.parts = b->parts;
@@ -603,7 +624,6 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   p.q = to_rows(q);
   p.out = to_rows(out);
   p.scale = scale;
-  p.n_ctas = b->n_ctas;
   p.wide_q = wide(q);
   p.wide_out = wide(out);
   p.n_heads = c.d.n_heads;
@@ -613,7 +633,17 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Turn turn{b, st};
   cudaError_t e = turn.enter();
-  if (e == cudaSuccess) e = launch_attend(p, D, b->nt, st);
+  if (e == cudaSuccess && b->wide.n_ctas) {
+    p.units = b->wide.units;
+    p.n_ctas = b->wide.n_ctas;
+    e = launch_wide(p, D, st);
+  }
+  if (e == cudaSuccess && b->narrow.n_ctas) {
+    p.units = b->narrow.units;
+    p.n_ctas = b->narrow.n_ctas;
+    p.arrived = b->arrived + b->wide.n_groups;
+    e = launch_attend(p, D, b->narrow.nt, st);
+  }
   if (e == cudaSuccess) e = turn.leave();
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, "spec_kv4_attend");
 }

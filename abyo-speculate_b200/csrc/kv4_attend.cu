@@ -24,6 +24,7 @@
 #include "common.cuh"
 #include "kv4.h"
 #include "kv4_rows.cuh"
+#include "kv4_mma.cuh"
 
 namespace specb200 {
 namespace kv4 {
@@ -32,44 +33,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;  // tokens of one ring slot
-constexpr float kNone = -1e30f;  // the reference before any score
-constexpr float kSlack = 8.f;    // a score may pass the reference by this many octaves before it moves
-
-SPEC_DEV float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-SPEC_DEV uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
-SPEC_DEV uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
 SPEC_DEV uint32_t movmatrix(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
-}
-SPEC_DEV uint32_t pack2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// Values of nibbles N and N + 4 of w: s (1 + code / 16) + o.  The low nibbles
-// are read in place as 1 + code / 2^10 or 1 + code / 2^6 and brought to
-// 1 + code / 16 by an exact multiply-add, the high ones by a shift, which
-// loads the integer and the f16 pipe alike (6 and 6 instructions a word).
-template <int N>
-SPEC_DEV uint32_t dq(uint32_t w, uint32_t s2, uint32_t o2) {
-  uint32_t x;
-  if (N == 0) x = hfma2(lop3_and_or(w, 0x000F000Fu, 0x3C003C00u), 0x54005400u, 0xD3E0D3E0u);       // 64 x - 63
-  else if (N == 1) x = hfma2(lop3_and_or(w, 0x00F000F0u, 0x3C003C00u), 0x44004400u, 0xC200C200u);  // 4 x - 3
-  else x = lop3_and_or(N == 2 ? w >> 2 : w >> 6, 0x03C003C0u, 0x3C003C00u);
-  return hfma2(x, s2, o2);
 }
 SPEC_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   // Not volatile: the compiler interleaves the chains with the unpacking.
@@ -418,9 +385,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
         for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(x[i][k]));
 #pragma unroll
         for (int o = 1; o < TPC; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        int ex = 0;
-        if (p.q.dtype == T_BF16 && a > 0.f && a < INFINITY) ex = min(max((__float_as_int(a) >> 23) - 127, -100), 126);
-        const float down = __int_as_float((127 - ex) << 23);
+        const int ex = row_exponent(p.q.dtype, a);
+        const float down = pow2i(-ex);
         if (col < NT * 8) {
           uint32_t f[4];
 #pragma unroll
@@ -430,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
           *reinterpret_cast<uint2*>(dst + 64) = make_uint2(f[2], f[3]);
           if (ch == 0) {
             const int row = (u.col0 + col) / G;
-            mt->c[col] = p.scale * 1.4426950408889634f * __int_as_float((ex + 127) << 23);
+            mt->c[col] = p.scale * kLog2e * pow2i(ex);
             mt->idx[col] = live ? row : -1;
             mt->mask[col] = live && p.masks ? p.masks[u.row0 + row] : 0ull;
           }
@@ -457,15 +423,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
       const bool tail = tok + kTile > u.kv_len;
       uint32_t sees = ~0u, live = ~0u, bad = 0u;
       if (tail) {
-        const int x = tok - u.kv_len, left = u.kv_end - tok;
-        if (p.masks) {
-          const unsigned long long m = lane < NT * 8 ? mt->mask[lane] : 0ull;
-          sees = x >= 0 ? (uint32_t)(m >> min(x, 63)) : ((uint32_t)m << min(-x, 31)) | ((1u << min(-x, 31)) - 1);
-        } else {
-          const int n = (lane < NT * 8 ? mt->idx[lane] : -1) + 1 - x;
-          sees = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1;
-        }
-        live = left >= 32 ? ~0u : (1u << left) - 1;
+        const bool col = lane < NT * 8;
+        sees = seen32(tok, u.kv_len, p.masks != nullptr, col ? mt->mask[lane] : 0ull, col ? mt->idx[lane] : -1);
+        live = first32(u.kv_end - tok);
         const uint32_t one = *reinterpret_cast<const uint32_t*>(b + (lane >> 4) * scale16 + vs0 +
                                                                 (lane >> 1 & 7) * (D / 32 * 8) + (lane & 1) * 4);
         bad = __ballot_sync(0xffffffffu, (one & 0x7fffu) > 0x7c00u) & live;
