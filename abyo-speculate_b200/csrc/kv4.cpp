@@ -75,8 +75,9 @@ namespace {
 
 // What one attention kernel does in a step.
 struct Schedule {
-  std::vector<Unit> order;  // first units of all CTAs, then each CTA's others
+  std::vector<Unit> order;  // first units of all CTAs, then each CTA's others, then (wide) the joins
   const Unit* units = nullptr;  // the same on the device
+  int n_units = 0, n_joins = 0;
   int n_ctas = 0, n_parts = 0, n_groups = 0;
   int nt = 1;                   // 8-column tiles of the largest unit
 };
@@ -107,7 +108,7 @@ struct spec_kv4_batch {
   size_t arrived_cap = 0;
   float* parts = nullptr;
   size_t parts_cap = 0;
-  std::vector<Unit> tiles, runs;
+  std::vector<Unit> tiles, runs, joins;
   std::vector<int> cuts;
   std::vector<uint8_t> seen;  // per page: 1 = read, 2 = written; zero between plans
 };
@@ -248,9 +249,10 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
   const int most = wide ? kWideCols : kMaxCols;
   b->tiles.clear();
   b->runs.clear();
+  b->joins.clear();
   b->cuts.clear();
   out.order.clear();
-  out.n_ctas = out.n_parts = out.n_groups = 0;
+  out.n_ctas = out.n_parts = out.n_groups = out.n_units = out.n_joins = 0;
   out.nt = 1;
   int64_t stages = 0;
   int row0 = 0, table = 0;
@@ -303,6 +305,10 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
       b->runs[i].part0 = out.n_parts;
       b->runs[i].group = out.n_groups;
     }
+    if (wide) {
+      if (parts > 1) out.n_parts += parts, b->joins.push_back(b->runs.back());
+      continue;
+    }
     for (int n = parts; n > 1;) {
       out.n_parts += n;
       n = (n + kFanIn - 1) / kFanIn;
@@ -323,6 +329,9 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
     }
     at += n - 1;
   }
+  out.n_units = (int)out.order.size();
+  out.n_joins = (int)b->joins.size();
+  out.order.insert(out.order.end(), b->joins.begin(), b->joins.end());
 }
 
 int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
@@ -635,6 +644,8 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   cudaError_t e = turn.enter();
   if (e == cudaSuccess && b->wide.n_ctas) {
     p.units = b->wide.units;
+    p.joins = b->wide.units + b->wide.n_units;
+    p.n_joins = b->wide.n_joins;
     p.n_ctas = b->wide.n_ctas;
     e = launch_wide(p, D, st);
   }

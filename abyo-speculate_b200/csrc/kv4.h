@@ -78,6 +78,8 @@ struct alignas(16) Unit {
 struct AttendParams {
   const uint8_t* pool;  // of the layer
   const Unit* units;  // [n_ctas] first units of the CTAs, then the others
+  const Unit* joins;  // wide kernel: a unit of every column tile that several CTAs share
+  int n_joins;
   const int* table;
   const unsigned long long* masks;  // null: causal
   float* parts;

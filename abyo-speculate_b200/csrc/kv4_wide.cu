@@ -8,10 +8,13 @@
 //   P = 2^(c S - m), rounded to f16 in place of S in tensor memory
 //   O [128 x D] += P V                          P from tensor memory, V^T from shared memory
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1, one thread a
-// column; warps 8-11 unpack the pages' codes into f16 operand tiles; lane 0 of
-// warp 12 issues the products.  While one tile's softmax runs, the other
-// tile's products do.  Unpacking is paid once for both tiles (1.5 instructions
-// an element and 256 columns).
+// column; warps 8-11 unpack K and 12-15 V, from page blocks that TMA bulk
+// copies bring, into f16 operand tiles; lane 0 of warp 16 issues the products.
+// While one tile's softmax runs, the other tile's products do.  Unpacking is
+// paid once for both tiles (1.5 instructions an element and 256 columns).
+// The loops are kept rolled: 17 warps in four roles share an instruction cache
+// that unrolled ones overflow (2048 rows over 6144 tokens: 407 us against the
+// figure below).
 //
 // Channels and tokens along a contracted axis may come in any order that both
 // operands share, and O's columns in any order that the output undoes: K's
@@ -19,9 +22,10 @@
 // V^T's row for channel 8 c + n is n * D/8 + c, so that the lanes of a warp
 // store neighbouring rows.
 //
-// O is scaled only when a column's reference moves, by a score more than
-// kSlack octaves above it.  Runs, partial states and joins are as in the
-// narrow kernel (kv4_attend.cu).
+// O is scaled only where a column's largest score passes its reference m by
+// more than kSlack octaves.  Runs are cut as for the narrow kernel (kv4_attend.cu); the partial
+// states of a column tile that several CTAs share are joined by a second
+// kernel, whose blocks spread over the channels.
 #include "common.cuh"
 #include "kv4.h"
 #include "kv4_mma.cuh"
@@ -32,8 +36,8 @@ namespace kv4 {
 namespace {
 
 constexpr int kTileCols = 128;
-constexpr int kThreads = 13 * 32;
-constexpr int kDequant = 8, kIssuer = 12;  // first warps of the roles
+constexpr int kThreads = 17 * 32;
+constexpr int kUnpackK = 8, kUnpackV = 12, kIssuer = 16;  // first warps of the roles
 
 // ---- tensor memory ----------------------------------------------------------
 template <int N>
@@ -55,16 +59,6 @@ SPEC_DEV void tm_load<32>(uint32_t a, float* r) {
         "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
         "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(a)
-      : "memory");
-}
-SPEC_DEV void tm_store32(uint32_t a, const float* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
-      "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
-      "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
-      "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
-      "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31])
       : "memory");
 }
 SPEC_DEV void tm_store16(uint32_t a, const uint32_t* r) {
@@ -109,182 +103,193 @@ SPEC_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
   return r;
 }
 
+SPEC_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 SPEC_DEV void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // Shared-memory writes of this thread become visible to the tensor core.
 SPEC_DEV void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-SPEC_DEV void bar_columns() { asm volatile("bar.sync 2, 256;" ::: "memory"); }
 
 template <int D>
 struct Shape {
   static constexpr int KS = D / 16;                 // 16-channel steps of Q K^T
   static constexpr int Q_TILE = kTileCols * D * 2;  // also a K tile and a V^T tile: 128 x D f16
-  static constexpr int K_AT = 2 * Q_TILE, V_AT = K_AT + 2 * Q_TILE, META_AT = V_AT + 2 * Q_TILE;
+  static constexpr int RAW = kStageTokens * D * 5 / 8;  // a stage's K, or V, as stored
+  static constexpr int K_AT = 2 * Q_TILE, V_AT = K_AT + 2 * Q_TILE;
+  static constexpr int RAW_K_AT = V_AT + 2 * Q_TILE, RAW_V_AT = RAW_K_AT + RAW, META_AT = RAW_V_AT + RAW;
   static constexpr int NC = D / 8;
 };
 
 struct Meta {
   unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full[2], idle;
+  unsigned long long raw_k, raw_v;
   uint32_t bad[2][4];  // tokens of a V stage whose row is NaN
   uint32_t tmem;
-  int last;
 };
 
-// A position in the CTA's run: unit fields and stage.
+// ---- unpacking: 128 threads for K, 128 for V --------------------------------
+// A position in the CTA's run: a stage, its unit's fields and (in the copying
+// warp) the page of lane `lane`.
 struct Walk {
   int next, last, st, st1;
+  int kvh, table, kv_len, kv_end;
+  int pages, page;
   bool more;
-  SPEC_DEV Walk(const Unit& u) : next(u.next), last(u.last), st(u.st0), st1(u.st1), more(true) {}
-  // Moves one stage on; returns the index of the unit entered, -1 within a unit or at the end.
-  SPEC_DEV int step(const AttendParams& p) {
-    if (++st < st1) return -1;
-    if (next == last) {
+  SPEC_DEV void enter(const AttendParams& p, int ui) {
+    const Unit& u = p.units[ui];
+    st = u.st0, st1 = u.st1;
+    kvh = u.kvh, table = u.table, kv_len = u.kv_len, kv_end = u.kv_end;
+    next = u.next, last = u.last;
+  }
+  SPEC_DEV void step(const AttendParams& p) {
+    if (++st < st1) return;
+    const int n = next;
+    if (n == last) {
       more = false;
-      return -1;
+      return;
     }
-    const int ui = next++;
-    st = p.units[ui].st0;
-    st1 = p.units[ui].st1;
-    return ui;
+    enter(p, n);
+    next = n + 1;
+  }
+  SPEC_DEV void look_up(const AttendParams& p, int lane) {
+    const int per = kStageTokens >> p.P_log2, first = st * per;
+    pages = more ? min(per, ((kv_end + p.P - 1) >> p.P_log2) - first) : 0;
+    page = lane < pages ? __ldg(p.table + table + first + lane) : 0;
   }
 };
 
-// ---- unpacking: 128 threads -------------------------------------------------
+// Copies a stage's K (V) halves of its page blocks; one lane a page.
 template <int D>
-struct Raw {
-  uint4 kc[D / 32];
-  uint32_t ks[D / 32];
-  uint32_t vc[D / 64][8];
-  uint2 vs[D / 64][4];
+SPEC_DEV void copy_raw(const AttendParams& p, const Walk& w, uint8_t* dst, uint64_t* bar, bool value, int lane) {
+  const int half = p.P * (D / 2 + D / 8);
+  if (lane == 0) mbar_arrive_expect_tx(bar, w.pages * half);
+  __syncwarp();
+  if (lane < w.pages)
+    tma_bulk_g2s(dst + lane * half, p.pool + ((long long)w.page * p.n_kv + w.kvh) * (2 * half) + (value ? half : 0), half,
+                 bar);
+}
 
-  SPEC_DEV void load_k(const AttendParams& p, int kvh, int table, int kv_end, int st, int th) {
-    const int tok = min(st * kStageTokens + th, kv_end - 1);
-    const int j = tok & (p.P - 1);
-    const uint8_t* b =
-        p.pool + ((long long)__ldg(p.table + table + (tok >> p.P_log2)) * p.n_kv + kvh) * block_bytes(p.P, D);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) kc[i] = *reinterpret_cast<const uint4*>(b + j * (D / 2) + i * 16);
-    const uint8_t* s = b + k_scales_at(p.P, D) + j * (D / 8);
-    if constexpr (D == 128) {
-      const uint4 x = *reinterpret_cast<const uint4*>(s);
-      ks[0] = x.x, ks[1] = x.y, ks[2] = x.z, ks[3] = x.w;
-    } else {
-      const uint2 x = *reinterpret_cast<const uint2*>(s);
-      ks[0] = x.x, ks[1] = x.y;
-    }
-  }
-  // Blocks of 8 tokens x 8 channels; tokens past the end read as the last block's.
-  SPEC_DEV void load_v(const AttendParams& p, int kvh, int table, int kv_end, int st, int th) {
-    constexpr int NC = D / 8;
-    const int c = th % NC;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const int tok = min(st * kStageTokens + (th / NC + i * (128 / NC)) * 8, (kv_end - 1) & ~7);
-      const int j = tok & (p.P - 1);
-      const uint8_t* b =
-          p.pool + ((long long)__ldg(p.table + table + (tok >> p.P_log2)) * p.n_kv + kvh) * block_bytes(p.P, D);
-      const uint8_t* code = b + v_codes_at(p.P, D) + (c % 8) * 4;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) vc[i][u] = *reinterpret_cast<const uint32_t*>(code + v_piece_at(D, j + u, c / 8));
-      const uint8_t* s = b + v_scales_at(p.P, D) + (j >> 1) * (D / 32 * 8) + (c / 4) * 8;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) vs[i][q] = *reinterpret_cast<const uint2*>(s + q * (D / 32 * 8));
-    }
-  }
-  // K tile: rows are tokens.
-  SPEC_DEV void put_k(uint8_t* dst, int th) const {
-    uint8_t* at = dst + (th / 8) * 256 + (th % 8) * 16;
-#pragma unroll
-    for (int g = 0; g < D / 32; ++g) {
-      const uint32_t s = prmt(ks[g], ks[g], 0x1010), o = prmt(ks[g], ks[g], 0x3232);
-      const uint32_t w[4] = {kc[g].x, kc[g].y, kc[g].z, kc[g].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint4*>(at + (2 * g + i / 2) * 4096 + (i % 2) * 128) =
-            make_uint4(dq<0>(w[i], s, o), dq<1>(w[i], s, o), dq<2>(w[i], s, o), dq<3>(w[i], s, o));
-    }
-  }
-  // V^T tile: rows are channels, 16 tokens a step.  `tail`: tokens past kv_end
-  // and NaN rows are zero.
-  SPEC_DEV void put_v(uint8_t* dst, int th, bool tail, int st, int kv_end) const {
-    constexpr int NC = D / 8;
-    const int c = th % NC;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      const int tb = th / NC + i * (128 / NC);
-      uint32_t out[8][4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t s = prmt(vs[i][q].x, vs[i][q].y, 0x5410), o = prmt(vs[i][q].x, vs[i][q].y, 0x7632);
-        if (tail) {
-          const int tok = st * kStageTokens + tb * 8 + 2 * q;
-          uint32_t keep = 0;
-          if (tok < kv_end && (s & 0x7fffu) <= 0x7c00u) keep |= 0x0000ffffu;
-          if (tok + 1 < kv_end && (s >> 16 & 0x7fffu) <= 0x7c00u) keep |= 0xffff0000u;
-          s &= keep;
-          o &= keep;
-        }
-        const uint32_t lo = prmt(vc[i][2 * q], vc[i][2 * q + 1], 0x5410), hi = prmt(vc[i][2 * q], vc[i][2 * q + 1], 0x7632);
-        out[0][q] = dq<0>(lo, s, o);
-        out[1][q] = dq<1>(lo, s, o);
-        out[2][q] = dq<2>(lo, s, o);
-        out[3][q] = dq<3>(lo, s, o);
-        out[4][q] = dq<0>(hi, s, o);
-        out[5][q] = dq<1>(hi, s, o);
-        out[6][q] = dq<2>(hi, s, o);
-        out[7][q] = dq<3>(hi, s, o);
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const int r = n * NC + c;
-        *reinterpret_cast<uint4*>(dst + (tb / 2) * (D * 32) + (r / 8) * 256 + (tb % 2) * 128 + (r % 8) * 16) =
-            make_uint4(out[n][0], out[n][1], out[n][2], out[n][3]);
-      }
-    }
-  }
-};
-
+// K tile: rows are tokens, one a thread.
 template <int D>
+SPEC_DEV void put_k(const uint8_t* raw, uint8_t* dst, int P, int P_log2, int th) {
+  const int j = th & (P - 1);
+  const uint8_t* b = raw + (th >> P_log2) * (P * (D / 2 + D / 8));
+  uint8_t* at = dst + (th / 8) * 256 + (th % 8) * 16;
+#pragma unroll 1
+  for (int g = 0; g < D / 32; ++g) {
+    const uint4 c = *reinterpret_cast<const uint4*>(b + j * (D / 2) + g * 16);
+    const uint32_t r = *reinterpret_cast<const uint32_t*>(b + P * (D / 2) + j * (D / 8) + g * 4);
+    const uint32_t s = prmt(r, r, 0x1010), o = prmt(r, r, 0x3232);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(at + (2 * g + i / 2) * 4096 + (i % 2) * 128) =
+          make_uint4(dq<0>(w[i], s, o), dq<1>(w[i], s, o), dq<2>(w[i], s, o), dq<3>(w[i], s, o));
+  }
+}
+
+// V^T tile: rows are channels, 16 tokens a step; a thread takes blocks of 8
+// tokens x 8 channels.  keep8: the tokens (of the stage, 32 a word) that count.
+template <int D>
+SPEC_DEV void put_v(const uint8_t* raw, uint8_t* dst, int P, int P_log2, int th, const uint32_t (&live)[4]) {
+  constexpr int NC = D / 8;
+  const int c = th % NC;
+#pragma unroll 1
+  for (int tb = th / NC; tb < kStageTokens / 8; tb += 128 / NC) {
+    const int j = tb * 8 & (P - 1);
+    const uint8_t* b = raw + (tb * 8 >> P_log2) * (P * (D / 2 + D / 8));
+    const uint8_t* code = b + (c % 8) * 4;
+    const uint8_t* scale = b + P * (D / 2) + (j >> 1) * (D / 32 * 8) + (c / 4) * 8;
+    const uint32_t word = tb < 4 ? live[0] : tb < 8 ? live[1] : tb < 12 ? live[2] : live[3];
+    const uint32_t keep8 = word >> (tb % 4 * 8);
+    uint32_t out[8][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint2 r = *reinterpret_cast<const uint2*>(scale + q * (D / 32 * 8));
+      const uint32_t keep = ((keep8 >> (2 * q)) & 1 ? 0x0000ffffu : 0u) | ((keep8 >> (2 * q)) & 2 ? 0xffff0000u : 0u);
+      const uint32_t s = prmt(r.x, r.y, 0x5410) & keep, o = prmt(r.x, r.y, 0x7632) & keep;
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(code + v_piece_at(D, j + 2 * q, c / 8));
+      const uint32_t y = *reinterpret_cast<const uint32_t*>(code + v_piece_at(D, j + 2 * q + 1, c / 8));
+      const uint32_t lo = prmt(x, y, 0x5410), hi = prmt(x, y, 0x7632);
+      out[0][q] = dq<0>(lo, s, o);
+      out[1][q] = dq<1>(lo, s, o);
+      out[2][q] = dq<2>(lo, s, o);
+      out[3][q] = dq<3>(lo, s, o);
+      out[4][q] = dq<0>(hi, s, o);
+      out[5][q] = dq<1>(hi, s, o);
+      out[6][q] = dq<2>(hi, s, o);
+      out[7][q] = dq<3>(hi, s, o);
+    }
+    uint8_t* at = dst + (tb / 2) * (D * 32) + (tb % 2) * 128;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int r = n * NC + c;
+      *reinterpret_cast<uint4*>(at + (r / 8) * 256 + (r % 8) * 16) = make_uint4(out[n][0], out[n][1], out[n][2], out[n][3]);
+    }
+  }
+}
+
+template <int D, bool VALUE>
 SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th) {
   using Sh = Shape<D>;
-  Unit u = p.units[blockIdx.x];
-  Walk w(u);
-  int kvh = u.kvh, table = u.table, kv_len = u.kv_len, kv_end = u.kv_end;
-  Raw<D> raw;
-  raw.load_k(p, kvh, table, kv_end, w.st, th);
-  raw.load_v(p, kvh, table, kv_end, w.st, th);
-  bool ok = true;
-  for (int k = 0; w.more; ++k) {
-    const int slot = k & 1, st = w.st;
-    const int now_len = kv_len, now_end = kv_end, now_table = table, now_kvh = kvh;
-    const int entered = w.step(p);
-    if (entered >= 0) {
-      const Unit& n = p.units[entered];
-      kvh = n.kvh, table = n.table, kv_len = n.kv_len, kv_end = n.kv_end;
-    }
-    if (k >= 2) ok = ok && mbar_wait_bounded(reinterpret_cast<uint64_t*>(&mt->k_free[slot]), (k / 2 - 1) & 1, p.err);
-    raw.put_k(smem + Sh::K_AT + slot * Sh::Q_TILE, th);
-    publish_smem();
-    arrive(reinterpret_cast<uint64_t*>(&mt->k_full[slot]));
-    if (w.more) raw.load_k(p, kvh, table, kv_end, w.st, th);
-    if (k >= 2) ok = ok && mbar_wait_bounded(reinterpret_cast<uint64_t*>(&mt->v_free[slot]), (k / 2 - 1) & 1, p.err);
-    const bool tail = (st + 1) * kStageTokens > now_len;
-    if (tail) {
-      // A stored NaN row of V is NaN in every scale: it is taken as zero here,
-      // and the columns that see it are told.
-      const int tok = min(st * kStageTokens + th, now_end - 1), j = tok & (p.P - 1);
-      const uint8_t* blk =
-          p.pool + ((long long)__ldg(p.table + now_table + (tok >> p.P_log2)) * p.n_kv + now_kvh) * block_bytes(p.P, D);
-      const uint32_t one = *reinterpret_cast<const uint32_t*>(blk + v_scales_at(p.P, D) + (j >> 1) * (D / 32 * 8) + (j & 1) * 4);
-      const uint32_t nans = __ballot_sync(0xffffffffu, (one & 0x7fffu) > 0x7c00u);
-      if ((th & 31) == 0) mt->bad[slot][th >> 5] = nans;
-    }
-    raw.put_v(smem + Sh::V_AT + slot * Sh::Q_TILE, th, tail, st, now_end);
-    publish_smem();
-    arrive(reinterpret_cast<uint64_t*>(&mt->v_full[slot]));
-    if (w.more) raw.load_v(p, kvh, table, kv_end, w.st, th);
+  auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
+  uint8_t* raw = smem + (VALUE ? Sh::RAW_V_AT : Sh::RAW_K_AT);
+  uint64_t* raw_full = bar(VALUE ? mt->raw_v : mt->raw_k);
+  unsigned long long* full = VALUE ? mt->v_full : mt->k_full;
+  unsigned long long* free_ = VALUE ? mt->v_free : mt->k_free;
+  Walk w;
+  w.more = true;
+  w.enter(p, blockIdx.x);
+  int copies = 0;
+  if (th < 32) {
+    w.look_up(p, th);
+    copy_raw<D>(p, w, raw, raw_full, VALUE, th);
+    ++copies;
   }
+  bool ok = true;
+#pragma unroll 1
+  for (int k = 0;; ++k) {
+    const int slot = k & 1, st = w.st, kv_len = w.kv_len, kv_end = w.kv_end;
+    w.step(p);
+    if (th < 32) w.look_up(p, th);
+    ok = ok && mbar_wait_bounded(raw_full, k & 1, p.err);
+    if (k >= 2) ok = ok && mbar_wait_bounded(bar(free_[slot]), (k / 2 - 1) & 1, p.err);
+    uint8_t* dst = smem + (VALUE ? Sh::V_AT : Sh::K_AT) + slot * Sh::Q_TILE;
+    if constexpr (VALUE) {
+      uint32_t live[4] = {~0u, ~0u, ~0u, ~0u};
+      if ((st + 1) * kStageTokens > kv_len) {
+        // Past the end V counts nothing.  A stored NaN row is NaN in every
+        // scale: it is taken as zero here, and the columns that see it are told.
+        const int j = th & (p.P - 1);
+        const uint32_t one = *reinterpret_cast<const uint32_t*>(
+            raw + (th >> p.P_log2) * (p.P * (D / 2 + D / 8)) + p.P * (D / 2) + (j >> 1) * (D / 32 * 8) + (j & 1) * 4);
+        const uint32_t nans = __ballot_sync(0xffffffffu, (one & 0x7fffu) > 0x7c00u);
+        if ((th & 31) == 0) mt->bad[slot][th >> 5] = nans;
+        asm volatile("bar.sync 4, 128;" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < 4; ++q) live[q] = first32(kv_end - st * kStageTokens - 32 * q) & ~mt->bad[slot][q];
+      }
+      put_v<D>(raw, dst, p.P, p.P_log2, th, live);
+    } else {
+      put_k<D>(raw, dst, p.P, p.P_log2, th);
+    }
+    publish_smem();
+    arrive(bar(full[slot]));
+    if (!w.more) break;
+    // All 128 threads have read the raw stage.
+    if (VALUE) asm volatile("bar.sync 4, 128;" ::: "memory");
+    else asm volatile("bar.sync 3, 128;" ::: "memory");
+    if (th < 32 && __all_sync(0xffffffffu, ok)) {
+      copy_raw<D>(p, w, raw, raw_full, VALUE, th);
+      ++copies;
+    }
+  }
+  if (!ok && copies) mbar_wait_bounded(raw_full, (copies - 1) & 1, p.err);  // leave no copy in flight
 }
 
 // ---- products: one thread ---------------------------------------------------
@@ -354,24 +359,22 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
   using Sh = Shape<D>;
   constexpr int NC = Sh::NC;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
-  const int th = threadIdx.x & 127, G = p.n_heads / p.n_kv;
+  const int th = threadIdx.x & 127, G = p.n_heads / p.n_kv, col = a * kTileCols + th;
   const uint32_t lane_at = (uint32_t)(th / 32 * 32) << 16;
   const uint32_t s_at = tmem + a * 128 + lane_at, o_at = tmem + 256 + a * 128 + lane_at;
-  constexpr int PART = (D + 2) * kWideCols;  // floats: [D][256], m, l
   bool ok = true;
   int k = 0, v = 0, unit = 0;  // stages of this tile, of the run; units of this tile
   Unit u = p.units[blockIdx.x];
   for (int next = u.next;; ++next) {
-    const int n = u.st1 - u.st0, col = a * kTileCols + th;
-    const bool on = a * kTileCols < u.n_cols, live = col < u.n_cols;
-    float m = kNone, l = 0.f;
-    const int r = u.col0 + (live ? col : 0), row = r / G, head = u.kvh * G + r % G;
-    if (on) {
-      // This column's q, in the order K's channels are unpacked.
+    if (a * kTileCols < u.n_cols) {
+      const bool live = col < u.n_cols;
+      const int r = u.col0 + (live ? col : 0), row = r / G, head = u.kvh * G + r % G;
+      // This column's q, in the order K's channels are unpacked.  A negative
+      // scale goes to q's sign, so that the largest product is the largest score.
       const long long at = (u.row0 + row) * p.q.row_stride + head * p.q.head_stride;
       uint8_t* dst = smem + a * Sh::Q_TILE + (th / 8) * 256 + (th % 8) * 16;
       float top = 0.f;
-#pragma unroll 4
+#pragma unroll 2
       for (int i = 0; i < NC; ++i) {
         float x[8];
         load8(p.q, at + i * 8, p.wide_q, x);
@@ -379,8 +382,8 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
       }
       const int ex = row_exponent(p.q.dtype, top);
-      const float down = pow2i(-ex);
-#pragma unroll 4
+      const float down = p.scale < 0.f ? -pow2i(-ex) : pow2i(-ex);
+#pragma unroll 2
       for (int i = 0; i < NC; ++i) {
         float x[8];
         load8(p.q, at + i * 8, p.wide_q, x);
@@ -392,87 +395,88 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       }
       publish_smem();
       arrive(bar(mt->q_full[a]));
-      const float c = p.scale * kLog2e * pow2i(ex);
+      const float c = fabsf(p.scale) * kLog2e * pow2i(ex);
       const unsigned long long mask = live && p.masks ? p.masks[u.row0 + row] : 0ull;
       const int idx = live ? row : -1;
+      float m = kNone, l = 0.f;
 
+#pragma unroll 1
       for (int st = u.st0; st < u.st1; ++st, ++k) {
-        ok = ok && mbar_wait_bounded(bar(mt->s_full[a]), k & 1, p.err);
-        tc_fence_after();
-        const int tok = st * kStageTokens;
+        const int tok = st * kStageTokens, stage = v + st - u.st0;
         const bool tail = tok + kStageTokens > u.kv_len;
         uint32_t sees[4];
-        float x[32];
         if (tail) {
-          // The V stage's NaN rows are known once it is unpacked.
-          const int slot = (v + st - u.st0) & 1;
-          ok = ok && mbar_wait_bounded(bar(mt->v_full[slot]), ((v + st - u.st0) >> 1) & 1, p.err);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 4; ++q)
             sees[q] = seen32(tok + 32 * q, u.kv_len, p.masks != nullptr, mask, idx) & first32(u.kv_end - tok - 32 * q);
-          }
         }
-        auto chunk = [&](int q) {  // scaled scores of tokens 32 q ..
+        ok = ok && mbar_wait_bounded(bar(mt->s_full[a]), k & 1, p.err);
+        tc_fence_after();
+        // The largest score of the stage.
+        float best = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          float x[32];
           tm_load<32>(s_at + 32 * q, x);
           tmem_wait_ld();
-        };
-        float top2 = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          chunk(q);
           if (tail) {
+            const uint32_t w = q == 0 ? sees[0] : q == 1 ? sees[1] : q == 2 ? sees[2] : sees[3];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = (sees[q] >> i) & 1 ? x[i] * c : -INFINITY;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] *= c;
+            for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1 ? x[i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top2 = fmaxf(top2, x[i]);
+          for (int i = 0; i < 32; i += 2) best = max3(best, x[i], x[i + 1]);
         }
-        const bool over = top2 > m + kSlack;
+        best = best > -INFINITY ? best * c : -INFINITY;
+        const bool over = best > m + kSlack;
         if (__any_sync(0xffffffffu, over)) {
-          const float mm = over ? top2 : m, f = ex2(m - mm);
+          const float mm = over ? best : m, by = ex2(m - mm);
           m = mm;
-          l *= f;
+          l *= by;
           if (st > u.st0) {
 #pragma unroll 1
-            for (int q = 0; q < D / 32; ++q) {
-              tm_load<32>(o_at + 32 * q, x);
+            for (int q = 0; q < D; q += 16) {
+              float x[16];
+              tm_load<8>(o_at + q, x);
+              tm_load<8>(o_at + q + 8, x + 8);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] *= f;
-              tm_store32(o_at + 32 * q, x);
+              for (int i = 0; i < 16; ++i) x[i] *= by;
+              tm_store16(o_at + q, reinterpret_cast<const uint32_t*>(x));
             }
           }
         }
         const unsigned long long c2 = two(c, c), m2 = two(-m, -m);
         unsigned long long sum = two(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
-          chunk(q);
+          float x[32];
+          tm_load<32>(s_at + 32 * q, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) apart(fma2(two(x[i], x[i + 1]), c2, m2), x[i], x[i + 1]);
+          if (tail) {
+            const uint32_t w = q == 0 ? sees[0] : q == 1 ? sees[1] : q == 2 ? sees[2] : sees[3];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1 ? x[i] : -INFINITY;
+          }
           uint32_t f[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float y, z;
-            apart(fma2(two(x[2 * i], x[2 * i + 1]), c2, m2), y, z);
-            if (tail) {
-              y = (sees[q] >> (2 * i)) & 1 ? y : -INFINITY;
-              z = (sees[q] >> (2 * i + 1)) & 1 ? z : -INFINITY;
-            }
-            y = ex2(y);
-            z = ex2(z);
-            sum = add2(sum, two(y, z));
-            f[i] = pack2(y, z);
+          for (int i = 0; i < 32; i += 2) {
+            x[i] = ex2(x[i]);
+            x[i + 1] = ex2(x[i + 1]);
+            sum = add2(sum, two(x[i], x[i + 1]));
+            f[i / 2] = pack2(x[i], x[i + 1]);
           }
           tm_store16(s_at + 16 * q, f);
         }
-        float y, z;
-        apart(sum, y, z);
-        l += y + z;
+        float sum_lo, sum_hi;
+        apart(sum, sum_lo, sum_hi);
+        l += sum_lo + sum_hi;
         if (tail) {
-          // A column that sees a NaN row of V is NaN.
-          const uint32_t* b = mt->bad[(v + st - u.st0) & 1];
+          // A column that sees a NaN row of V, known once V is unpacked, is NaN.
+          ok = ok && mbar_wait_bounded(bar(mt->v_full[stage & 1]), (stage >> 1) & 1, p.err);
+          const uint32_t* b = mt->bad[stage & 1];
           if ((b[0] & sees[0]) | (b[1] & sees[1]) | (b[2] & sees[2]) | (b[3] & sees[3])) l = __int_as_float(0x7fffffff);
         }
         tm_wait_st();
@@ -481,130 +485,68 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       }
       ok = ok && mbar_wait_bounded(bar(mt->o_full[a]), unit++ & 1, p.err);
       tc_fence_after();
-    }
-    v += n;
-
-    // This column's O, or what is joined from partial states, to the output.
-    const long long out_at = (u.row0 + row) * p.out.row_stride + head * p.out.head_stride;
-    auto write = [&](int c0, const float (&x)[8][8], float inv) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e][c] * inv;
-        if (live) store8(p.out, out_at + (c0 + c) * 8, p.wide_out, y);
-      }
-    };
-    auto inverse = [](float l) { return l == 0.f ? 0.f : 1.f / l; };
-    if (u.n_parts == 1) {
-      if (on) {
+      // O to the output, or as a partial state [D][256], m, l.
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const long long out_at = (u.row0 + row) * p.out.row_stride + head * p.out.head_stride;
+      float* part = p.parts + (long long)(u.part0 + u.part) * ((D + 2) * kWideCols) + col;
 #pragma unroll 1
-        for (int c0 = 0; c0 < NC; c0 += 8) {
-          float x[8][8];
+      for (int c0 = 0; c0 < NC; c0 += 8) {
+        float x[8][8];  // x[n][c] is channel 8 (c0 + c) + n
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tm_load<8>(o_at + e * NC + c0, x[e]);
-          tmem_wait_ld();
-          write(c0, x, inverse(l));
-        }
-        tc_fence_before();
-      }
-    } else {
-      int parts = u.n_parts, at = u.part;
-      long long base = u.part0;
-      int* arrived = p.arrived + u.group;
-      bool from_tmem = true;
-      float w[kFanIn];  // weights of the parts of the last join
-      long long src = 0;
-      int count = 0;
-      // x[e][c] of the current state: tensor memory, or the weighted parts.
-      auto state = [&](int c0, float (&x)[8][8]) {
-        if (from_tmem) {
+        for (int e = 0; e < 8; ++e) tm_load<8>(o_at + e * NC + c0, x[e]);
+        tmem_wait_ld();
+        if (u.n_parts == 1) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tm_load<8>(o_at + e * NC + c0, x[e]);
-          tmem_wait_ld();
-          return;
-        }
+          for (int i = 0; i < 8; ++i) {
+            float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) x[e][c] = 0.f;
-#pragma unroll 1
-        for (int i = 0; i < count; ++i) {
-          const float* s = p.parts + (src + i) * PART + col;
-          float f = 0.f;
-#pragma unroll
-          for (int q = 0; q < kFanIn; ++q) f = q == i ? w[q] : f;
+            for (int e = 0; e < 8; ++e) y[e] = x[e][i] * inv;
+            if (live) store8(p.out, out_at + (c0 + i) * 8, p.wide_out, y);
+          }
+        } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[e][c] += __ldcg(s + (e * NC + c0 + c) * kWideCols) * f;
-        }
-      };
-      while (parts > 1) {
-        const int node = at / kFanIn, first = node * kFanIn;
-        if (on) {
-          float* dst = p.parts + (base + at) * PART + col;
-#pragma unroll 1
-          for (int c0 = 0; c0 < NC; c0 += 8) {
-            float x[8][8];
-            state(c0, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-#pragma unroll
-              for (int c = 0; c < 8; ++c) __stcg(dst + (e * NC + c0 + c) * kWideCols, x[e][c]);
-          }
-          __stcg(dst + D * kWideCols, m);
-          __stcg(dst + (D + 1) * kWideCols, l);
-          tc_fence_before();
-        }
-        __threadfence();
-        bar_columns();
-        if (a == 0 && th == 0) {
-          const int of = min(kFanIn, parts - first);
-          const bool last = atomicAdd(arrived + node, 1) == of - 1;
-          if (last) arrived[node] = 0;  // ready for the next call
-          mt->last = last;
-        }
-        bar_columns();
-        if (!mt->last) break;
-        __threadfence();
-        count = min(kFanIn, parts - first);
-        src = base + first;
-        if (on) {
-          m = kNone;
-          float pm[kFanIn];
-#pragma unroll
-          for (int i = 0; i < kFanIn; ++i) {
-            pm[i] = i < count ? __ldcg(p.parts + (src + i) * PART + D * kWideCols + col) : kNone;
-            m = fmaxf(m, pm[i]);
-          }
-          l = 0.f;
-#pragma unroll
-          for (int i = 0; i < kFanIn; ++i) {
-            w[i] = ex2(pm[i] - m);
-            if (i < count) l += __ldcg(p.parts + (src + i) * PART + (D + 1) * kWideCols + col) * w[i];
-          }
-        }
-        from_tmem = false;
-        base += parts;
-        parts = (parts + kFanIn - 1) / kFanIn;
-        arrived += parts;
-        at = node;
-        bar_columns();  // mt->last is free for the next level
-      }
-      if (parts == 1 && on) {
-#pragma unroll 1
-        for (int c0 = 0; c0 < NC; c0 += 8) {
-          float x[8][8];
-          state(c0, x);
-          write(c0, x, inverse(l));
+            for (int i = 0; i < 8; ++i) part[((c0 + i) * 8 + e) * kWideCols] = x[e][i];
         }
       }
-      bar_columns();
+      if (u.n_parts > 1) {
+        part[D * kWideCols] = m;
+        part[(D + 1) * kWideCols] = l;
+      }
+      tc_fence_before();
     }
+    v += u.st1 - u.st0;
     if (next == u.last) break;
     u = p.units[next];
   }
+}
+
+// Joins the partial states of a column tile: a thread a column, 8 channels a
+// block.  The states are read once and in order.
+template <int D>
+__global__ void __launch_bounds__(kWideCols) wide_join_kernel(const __grid_constant__ AttendParams p) {
+  constexpr int PART = (D + 2) * kWideCols;
+  const Unit& u = p.joins[blockIdx.x];
+  const int col = threadIdx.x, c = blockIdx.y, n = u.n_parts, G = p.n_heads / p.n_kv;
+  if (col >= u.n_cols) return;
+  const float* s = p.parts + (long long)u.part0 * PART + col;
+  float m = kNone;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, s[(long long)i * PART + D * kWideCols]);
+  float l = 0.f, x[8] = {};
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float* q = s + (long long)i * PART;
+    const float w = ex2(q[D * kWideCols] - m);
+    l += q[(D + 1) * kWideCols] * w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += q[(c * 8 + e) * kWideCols] * w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= inv;
+  const int r = u.col0 + col;
+  store8(p.out, (u.row0 + r / G) * p.out.row_stride + (u.kvh * G + r % G) * p.out.head_stride + c * 8, p.wide_out, x);
 }
 
 template <int D>
@@ -626,6 +568,8 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       init(mt->o_full[i], 1);
     }
     init(mt->idle, 1);
+    init(mt->raw_k, 1);
+    init(mt->raw_v, 1);
     fence_mbar_init();
   }
   if (warp == kIssuer) tmem_alloc(&mt->tmem, 512);
@@ -633,10 +577,12 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = mt->tmem;
-  if (warp < kDequant) {
+  if (warp < kUnpackK) {
     softmax_role<D>(p, smem, mt, tmem, warp / 4);
+  } else if (warp < kUnpackV) {
+    unpack_role<D, false>(p, smem, mt, threadIdx.x - kUnpackK * 32);
   } else if (warp < kIssuer) {
-    unpack_role<D>(p, smem, mt, threadIdx.x - kDequant * 32);
+    unpack_role<D, true>(p, smem, mt, threadIdx.x - kUnpackV * 32);
   } else if ((threadIdx.x & 31) == 0) {
     issue_role<D>(p, smem, mt, tmem);
   }
@@ -665,6 +611,11 @@ cudaError_t launch_wide(const AttendParams& p, int head_dim, cudaStream_t s) {
   if (p.n_ctas <= 0) return cudaSuccess;
   if (head_dim == 128) wide_kernel<128><<<p.n_ctas, kThreads, smem_bytes<128>(), s>>>(p);
   else wide_kernel<64><<<p.n_ctas, kThreads, smem_bytes<64>(), s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !p.n_joins) return e;
+  const dim3 grid(p.n_joins, head_dim / 8);
+  if (head_dim == 128) wide_join_kernel<128><<<grid, kWideCols, 0, s>>>(p);
+  else wide_join_kernel<64><<<grid, kWideCols, 0, s>>>(p);
   return cudaGetLastError();
 }
 
