@@ -270,6 +270,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
         u.n_cols = cols - c0 < size ? cols - c0 : size;
         u.kv_len = n;
         u.kv_end = s->masks ? n + m : n + (c0 + u.n_cols - 1) / G + 1;
+        u.sure = s->masks ? n : n + c0 / G + 1;
         u.st1 = (u.kv_end + kStageTokens - 1) / kStageTokens;
         u.table = table;
         stages += u.st1;

@@ -65,13 +65,13 @@ struct alignas(16) Unit {
   int col0, n_cols;    // stacked columns (row * G + query head of the group)
   int st0, st1;        // 128-token stages
   int kv_len, kv_end;  // cached tokens; tokens any column of the tile sees
+  int sure;            // tokens every column of it sees
   int table;           // the sequence's pages
   // Partial states of the tile: n_parts at part0, then ceil(n / kFanIn) more
   // a level; arrival counters likewise from `group` on.  n_parts == 1: none.
   int part0, part, n_parts;
   int group;
   int next, last;      // the CTA's next unit and one past its last
-  int pad;
   int pages[8];        // pages of the first stage
 };
 

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
       // counts.  A stored NaN row of V is NaN in every scale; its value is
       // taken as zero and the NaN given to the scores of the columns that see
       // it, so that no other column meets it.
-      const bool tail = tok + kTile > u.kv_len;
+      const bool tail = tok + kTile > u.sure;
       uint32_t sees = ~0u, live = ~0u, bad = 0u;
       if (tail) {
         const bool col = lane < NT * 8;

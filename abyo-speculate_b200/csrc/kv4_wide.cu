@@ -5,7 +5,7 @@
 // takes up to 256 of them as two tiles of 128 and walks the 128-token stages
 // of its run:
 //   S [128 columns x 128 tokens] = Q K^T        tcgen05.mma, f16 from shared memory
-//   P = 2^(c S - m), rounded to f16 in place of S in tensor memory
+//   P = 2^(c S - m), rounded to f16 over the second half of S in tensor memory
 //   O [128 x D] += P V                          P from tensor memory, V^T from shared memory
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1, one thread a
 // column; warps 8-11 unpack K and 12-15 V, from page blocks that TMA bulk
@@ -40,6 +40,11 @@ constexpr int kThreads = 17 * 32;
 constexpr int kUnpackK = 8, kUnpackV = 12, kIssuer = 16;  // first warps of the roles
 
 // ---- tensor memory ----------------------------------------------------------
+SPEC_DEV float tm_load1(uint32_t a) {
+  float r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(r) : "r"(a) : "memory");
+  return r;
+}
 template <int N>
 SPEC_DEV void tm_load(uint32_t addr, float* r);
 template <>
@@ -50,23 +55,25 @@ SPEC_DEV void tm_load<8>(uint32_t a, float* r) {
                : "memory");
 }
 template <>
-SPEC_DEV void tm_load<32>(uint32_t a, float* r) {
+SPEC_DEV void tm_load<16>(uint32_t a, float* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
       : "r"(a)
       : "memory");
 }
-SPEC_DEV void tm_store16(uint32_t a, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+// Waits for the loads; the registers are used after it, not before.
+template <int N>
+SPEC_DEV void tm_wait(float (&r)[N]) {
+  tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i])::"memory");
+}
+SPEC_DEV void tm_store8(uint32_t a, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 SPEC_DEV void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -137,13 +144,13 @@ struct Meta {
 // warp) the page of lane `lane`.
 struct Walk {
   int next, last, st, st1;
-  int kvh, table, kv_len, kv_end;
+  int kvh, table, sure, kv_end;
   int pages, page;
   bool more;
   SPEC_DEV void enter(const AttendParams& p, int ui) {
     const Unit& u = p.units[ui];
     st = u.st0, st1 = u.st1;
-    kvh = u.kvh, table = u.table, kv_len = u.kv_len, kv_end = u.kv_end;
+    kvh = u.kvh, table = u.table, sure = u.sure, kv_end = u.kv_end;
     next = u.next, last = u.last;
   }
   SPEC_DEV void step(const AttendParams& p) {
@@ -254,7 +261,7 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
   bool ok = true;
 #pragma unroll 1
   for (int k = 0;; ++k) {
-    const int slot = k & 1, st = w.st, kv_len = w.kv_len, kv_end = w.kv_end;
+    const int slot = k & 1, st = w.st, sure = w.sure, kv_end = w.kv_end;
     w.step(p);
     if (th < 32) w.look_up(p, th);
     ok = ok && mbar_wait_bounded(raw_full, k & 1, p.err);
@@ -262,7 +269,7 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
     uint8_t* dst = smem + (VALUE ? Sh::V_AT : Sh::K_AT) + slot * Sh::Q_TILE;
     if constexpr (VALUE) {
       uint32_t live[4] = {~0u, ~0u, ~0u, ~0u};
-      if ((st + 1) * kStageTokens > kv_len) {
+      if ((st + 1) * kStageTokens > sure) {
         // Past the end V counts nothing.  A stored NaN row is NaN in every
         // scale: it is taken as zero here, and the columns that see it are told.
         const int j = th & (p.P - 1);
@@ -331,7 +338,7 @@ SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_
         tc_fence_after();
 #pragma unroll
         for (int j = 0; j < kStageTokens / 16; ++j)
-          mma_ts(tmem + 256 + a * 128, tmem + a * 128 + j * 8,
+          mma_ts(tmem + 256 + a * 128, tmem + a * 128 + 64 + j * 8,
                  umma_desc_kmajor(base + Sh::V_AT + slot * Sh::Q_TILE + j * (D * 32), 128, 256), kO, i > 0 || j > 0);
         if (i + 1 == n) {
           umma_commit(bar(mt->o_full[a]));
@@ -354,6 +361,32 @@ SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_
 }
 
 // ---- softmax: one thread a column -------------------------------------------
+SPEC_DEV uint4 raw8(const Rows& r, long long at, bool wide) {
+  const uint16_t* s = static_cast<const uint16_t*>(r.ptr) + at;
+  if (wide) return *reinterpret_cast<const uint4*>(s);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = s[2 * i] | (uint32_t)s[2 * i + 1] << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Chunk i of a q row as 8 f16 in the order K's channels are unpacked.
+template <int D>
+SPEC_DEV void put_q(uint8_t* row, int i, const uint4& w, int dtype, float down, bool live) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[e]));
+    x[2 * e] = dtype == T_BF16 ? __uint_as_float(v[e] << 16) : f.x;
+    x[2 * e + 1] = dtype == T_BF16 ? __uint_as_float(v[e] & 0xffff0000u) : f.y;
+  }
+  uint4 f = make_uint4(0, 0, 0, 0);
+  if (live)
+    f = make_uint4(pack2(x[0] * down, x[4] * down), pack2(x[1] * down, x[5] * down), pack2(x[2] * down, x[6] * down),
+                   pack2(x[3] * down, x[7] * down));
+  *reinterpret_cast<uint4*>(row + (i / 2) * 4096 + (i % 2) * 128) = f;
+}
+
 template <int D>
 SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem, int a) {
   using Sh = Shape<D>;
@@ -373,29 +406,36 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       // scale goes to q's sign, so that the largest product is the largest score.
       const long long at = (u.row0 + row) * p.q.row_stride + head * p.q.head_stride;
       uint8_t* dst = smem + a * Sh::Q_TILE + (th / 8) * 256 + (th % 8) * 16;
-      float top = 0.f;
-#pragma unroll 2
-      for (int i = 0; i < NC; ++i) {
-        float x[8];
-        load8(p.q, at + i * 8, p.wide_q, x);
+      // Converted as it is, four 16-byte loads in flight; a row whose largest
+      // magnitude (16-bit floats without their sign order as integers) is far
+      // from 1 is converted again, scaled by a power of two.
+      const float sign = p.scale < 0.f ? -1.f : 1.f;
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < NC; i0 += 4) {
+        uint4 w[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        for (int i = 0; i < 4; ++i) w[i] = raw8(p.q, at + (i0 + i) * 8, p.wide_q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          top = __vmaxu2(top, __vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu));
+          top = __vmaxu2(top, __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+          put_q<D>(dst, i0 + i, w[i], p.q.dtype, sign, live);
+        }
       }
-      const int ex = row_exponent(p.q.dtype, top);
-      const float down = p.scale < 0.f ? -pow2i(-ex) : pow2i(-ex);
-#pragma unroll 2
-      for (int i = 0; i < NC; ++i) {
-        float x[8];
-        load8(p.q, at + i * 8, p.wide_q, x);
-        uint4 f = make_uint4(0, 0, 0, 0);
-        if (live)
-          f = make_uint4(pack2(x[0] * down, x[4] * down), pack2(x[1] * down, x[5] * down),
-                         pack2(x[2] * down, x[6] * down), pack2(x[3] * down, x[7] * down));
-        *reinterpret_cast<uint4*>(dst + (i / 2) * 4096 + (i % 2) * 128) = f;
+      top = max(top & 0xffffu, top >> 16);
+      int ex = row_exponent(p.q.dtype, __uint_as_float(top << 16));
+      if (ex >= -4 && ex <= 14) {
+        ex = 0;
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < NC; ++i)
+          put_q<D>(dst, i, raw8(p.q, at + i * 8, p.wide_q), p.q.dtype, sign * pow2i(-ex), live);
       }
       publish_smem();
       arrive(bar(mt->q_full[a]));
-      const float c = fabsf(p.scale) * kLog2e * pow2i(ex);
+      // Not zero: a score that is not seen is -inf, and stays that when scaled.
+      const float c = fmaxf(fabsf(p.scale) * kLog2e * pow2i(ex), 1e-37f);
       const unsigned long long mask = live && p.masks ? p.masks[u.row0 + row] : 0ull;
       const int idx = live ? row : -1;
       float m = kNone, l = 0.f;
@@ -403,7 +443,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
 #pragma unroll 1
       for (int st = u.st0; st < u.st1; ++st, ++k) {
         const int tok = st * kStageTokens, stage = v + st - u.st0;
-        const bool tail = tok + kStageTokens > u.kv_len;
+        const bool tail = tok + kStageTokens > u.sure;
         uint32_t sees[4];
         if (tail) {
 #pragma unroll
@@ -412,20 +452,27 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         }
         ok = ok && mbar_wait_bounded(bar(mt->s_full[a]), k & 1, p.err);
         tc_fence_after();
-        // The largest score of the stage.
+        // The largest score of the stage, a half at a time; the second half
+        // stays in registers for the next pass.
         float best = -INFINITY;
+        float x[64];
+        auto mask = [&](float* y, uint32_t w) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = (w >> i) & 1 ? y[i] : -INFINITY;
+        };
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float x[32];
-          tm_load<32>(s_at + 32 * q, x);
-          tmem_wait_ld();
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tm_load<16>(s_at + 64 * h + 16 * b, x + 16 * b);
+          tm_wait(x);
           if (tail) {
-            const uint32_t w = q == 0 ? sees[0] : q == 1 ? sees[1] : q == 2 ? sees[2] : sees[3];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1 ? x[i] : -INFINITY;
+            mask(x, h ? sees[2] : sees[0]);
+            mask(x + 32, h ? sees[3] : sees[1]);
           }
+          float part[4] = {best, x[0], x[1], x[2]};
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) best = max3(best, x[i], x[i + 1]);
+          for (int i = 3; i < 63; i += 2) part[i / 2 % 4] = max3(part[i / 2 % 4], x[i], x[i + 1]);
+          best = max3(max3(part[0], part[1], x[63]), part[2], part[3]);
         }
         best = best > -INFINITY ? best * c : -INFINITY;
         const bool over = best > m + kSlack;
@@ -435,43 +482,47 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           l *= by;
           if (st > u.st0) {
 #pragma unroll 1
-            for (int q = 0; q < D; q += 16) {
-              float x[16];
-              tm_load<8>(o_at + q, x);
-              tm_load<8>(o_at + q + 8, x + 8);
-              tmem_wait_ld();
+            for (int q = 0; q < D; q += 8) {
+              float o[8];
+              tm_load<8>(o_at + q, o);
+              tm_wait(o);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] *= by;
-              tm_store16(o_at + q, reinterpret_cast<const uint32_t*>(x));
+              for (int i = 0; i < 8; ++i) o[i] *= by;
+              tm_store8(o_at + q, reinterpret_cast<const uint32_t*>(o));
             }
           }
         }
         const unsigned long long c2 = two(c, c), m2 = two(-m, -m);
-        unsigned long long sum = two(0.f, 0.f);
+        unsigned long long sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+        // P of the second half, then of the first, to the tile's upper 64 columns.
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float x[32];
-          tm_load<32>(s_at + 32 * q, x);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) apart(fma2(two(x[i], x[i + 1]), c2, m2), x[i], x[i + 1]);
-          if (tail) {
-            const uint32_t w = q == 0 ? sees[0] : q == 1 ? sees[1] : q == 2 ? sees[2] : sees[3];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = (w >> i) & 1 ? x[i] : -INFINITY;
+        for (int h = 1; h >= 0; --h) {
+          if (h == 0) {
+            tm_wait(x);
+            if (tail) {
+              mask(x, sees[0]);
+              mask(x + 32, sees[1]);
+            }
           }
-          uint32_t f[16];
+          uint32_t f[32];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            x[i] = ex2(x[i]);
-            x[i + 1] = ex2(x[i + 1]);
-            sum = add2(sum, two(x[i], x[i + 1]));
-            f[i / 2] = pack2(x[i], x[i + 1]);
+          for (int i = 0; i < 64; i += 2) {
+            float lo, hi;
+            apart(fma2(two(x[i], x[i + 1]), c2, m2), lo, hi);
+            lo = ex2(lo);
+            hi = ex2(hi);
+            sum[i / 2 % 2] = add2(sum[i / 2 % 2], two(lo, hi));
+            f[i / 2] = pack2(lo, hi);
           }
-          tm_store16(s_at + 16 * q, f);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) tm_store8(s_at + 64 + 32 * h + 8 * b, f + 8 * b);
+          if (h == 1) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) tm_load<16>(s_at + 16 * b, x + 16 * b);
+          }
         }
         float sum_lo, sum_hi;
-        apart(sum, sum_lo, sum_hi);
+        apart(add2(sum[0], sum[1]), sum_lo, sum_hi);
         l += sum_lo + sum_hi;
         if (tail) {
           // A column that sees a NaN row of V, known once V is unpacked, is NaN.
@@ -490,24 +541,18 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       const long long out_at = (u.row0 + row) * p.out.row_stride + head * p.out.head_stride;
       float* part = p.parts + (long long)(u.part0 + u.part) * ((D + 2) * kWideCols) + col;
 #pragma unroll 1
-      for (int c0 = 0; c0 < NC; c0 += 8) {
-        float x[8][8];  // x[n][c] is channel 8 (c0 + c) + n
+      for (int i = 0; i < NC; ++i) {
+        float y[8];  // channels 8 i ..
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tm_load<8>(o_at + e * NC + c0, x[e]);
-        tmem_wait_ld();
+        for (int e = 0; e < 8; ++e) y[e] = tm_load1(o_at + e * NC + i);
+        tm_wait(y);
         if (u.n_parts == 1) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[e][i] * inv;
-            if (live) store8(p.out, out_at + (c0 + i) * 8, p.wide_out, y);
-          }
+          for (int e = 0; e < 8; ++e) y[e] *= inv;
+          if (live) store8(p.out, out_at + i * 8, p.wide_out, y);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) part[((c0 + i) * 8 + e) * kWideCols] = x[e][i];
+          for (int e = 0; e < 8; ++e) part[(i * 8 + e) * kWideCols] = y[e];
         }
       }
       if (u.n_parts > 1) {
