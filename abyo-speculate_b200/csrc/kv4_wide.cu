@@ -8,11 +8,13 @@
 //   P = 2^(c S - m), rounded to f16 over the second half of S in tensor memory
 //   O [128 x D] += P V                          P from tensor memory, V^T from shared memory
 // Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1, one thread a
-// column; warps 8-11 unpack K and 12-15 V, from page blocks that TMA bulk
-// copies bring, into f16 operand tiles; lane 0 of warp 16 issues the products.
+// column; warps 8-10 unpack K and 11-14 V, from page blocks that TMA bulk
+// copies bring, into f16 operand tiles; lane 0 of warp 15 issues the products.
+// (16 warps leave 128 registers a thread; with a fourth warp for K it is 96,
+// and the softmax, which holds 64 scores, spills.)
 // While one tile's softmax runs, the other tile's products do.  Unpacking is
 // paid once for both tiles (1.5 instructions an element and 256 columns).
-// The loops are kept rolled: 17 warps in four roles share an instruction cache
+// The loops are kept rolled: 16 warps in four roles share an instruction cache
 // that unrolled ones overflow (2048 rows over 6144 tokens: 407 us against the
 // figure below).
 //
@@ -36,8 +38,9 @@ namespace kv4 {
 namespace {
 
 constexpr int kTileCols = 128;
-constexpr int kThreads = 17 * 32;
-constexpr int kUnpackK = 8, kUnpackV = 12, kIssuer = 16;  // first warps of the roles
+constexpr int kThreads = 16 * 32;
+constexpr int kUnpackK = 8, kUnpackV = 11, kIssuer = 15;  // first warps of the roles
+constexpr int kThreadsK = (kUnpackV - kUnpackK) * 32;
 
 // ---- tensor memory ----------------------------------------------------------
 SPEC_DEV float tm_load1(uint32_t a) {
@@ -139,7 +142,7 @@ struct Meta {
   uint32_t tmem;
 };
 
-// ---- unpacking: 128 threads for K, 128 for V --------------------------------
+// ---- unpacking: 96 threads for K, 128 for V --------------------------------
 // A position in the CTA's run: a stage, its unit's fields and (in the copying
 // warp) the page of lane `lane`.
 struct Walk {
@@ -181,22 +184,22 @@ SPEC_DEV void copy_raw(const AttendParams& p, const Walk& w, uint8_t* dst, uint6
                  bar);
 }
 
-// K tile: rows are tokens, one a thread.
+// K tile: rows are tokens; a thread takes groups of 32 channels of a token.
 template <int D>
 SPEC_DEV void put_k(const uint8_t* raw, uint8_t* dst, int P, int P_log2, int th) {
-  const int j = th & (P - 1);
-  const uint8_t* b = raw + (th >> P_log2) * (P * (D / 2 + D / 8));
-  uint8_t* at = dst + (th / 8) * 256 + (th % 8) * 16;
 #pragma unroll 1
-  for (int g = 0; g < D / 32; ++g) {
+  for (int i = th; i < kStageTokens * (D / 32); i += kThreadsK) {
+    const int tok = i % kStageTokens, g = i / kStageTokens, j = tok & (P - 1);
+    const uint8_t* b = raw + (tok >> P_log2) * (P * (D / 2 + D / 8));
     const uint4 c = *reinterpret_cast<const uint4*>(b + j * (D / 2) + g * 16);
     const uint32_t r = *reinterpret_cast<const uint32_t*>(b + P * (D / 2) + j * (D / 8) + g * 4);
     const uint32_t s = prmt(r, r, 0x1010), o = prmt(r, r, 0x3232);
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    uint8_t* at = dst + g * 8192 + (tok / 8) * 256 + (tok % 8) * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<uint4*>(at + (2 * g + i / 2) * 4096 + (i % 2) * 128) =
-          make_uint4(dq<0>(w[i], s, o), dq<1>(w[i], s, o), dq<2>(w[i], s, o), dq<3>(w[i], s, o));
+    for (int k = 0; k < 4; ++k)
+      *reinterpret_cast<uint4*>(at + (k / 2) * 4096 + (k % 2) * 128) =
+          make_uint4(dq<0>(w[k], s, o), dq<1>(w[k], s, o), dq<2>(w[k], s, o), dq<3>(w[k], s, o));
   }
 }
 
@@ -288,9 +291,9 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
     publish_smem();
     arrive(bar(full[slot]));
     if (!w.more) break;
-    // All 128 threads have read the raw stage.
+    // All its threads have read the raw stage.
     if (VALUE) asm volatile("bar.sync 4, 128;" ::: "memory");
-    else asm volatile("bar.sync 3, 128;" ::: "memory");
+    else asm volatile("bar.sync 3, %0;" ::"n"(kThreadsK) : "memory");
     if (th < 32 && __all_sync(0xffffffffu, ok)) {
       copy_raw<D>(p, w, raw, raw_full, VALUE, th);
       ++copies;
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
     auto init = [](unsigned long long& b, int n) { mbar_init(reinterpret_cast<uint64_t*>(&b), n); };
     for (int i = 0; i < 2; ++i) {
       init(mt->q_full[i], 128);
-      init(mt->k_full[i], 128);
+      init(mt->k_full[i], kThreadsK);
       init(mt->k_free[i], 1);
       init(mt->v_full[i], 128);
       init(mt->v_free[i], 1);
