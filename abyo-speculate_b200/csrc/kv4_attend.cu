@@ -7,11 +7,17 @@
 // 32 to a unit; both products are taken transposed so that the cache is the
 // 16-row operand of mma.sync and few columns cost little:
 //   S^T [16 tokens x 8 n] = K [16 x D] Q^T,   O^T [D x 8 n] += V^T [D x 16] P^T
-// Codes go to the f16 operand in registers: (w >> shift) & 0x03C003C0 | 0x3C003C00
-// is the pair 1 + code / 16, and one packed multiply-add by (s, o) gives the
-// values.  Any order of the channels (K) and of the tokens (V) along the
-// contracted axis will do, so a lane takes the channels of whole 32-bit words
-// and never shuffles nibbles; P^T is S^T's fragment through movmatrix.
+// K's codes are used as they are: (w & 0x000F000F) is a pair of f16 numbers
+// code 2^-24 (tensor cores take subnormals), (w & 0x00F000F0) code 2^-20, and
+// q carries the inverse powers.  A group's sum of code q is exact in f32 and
+// takes its scale there,
+//   s_j = sum_groups s / 16 (sum code q) + (s + o) (sum q),
+// so no rounding of K enters a score; the second term is one more product,
+// with the scale pairs as they are stored.  ldmatrix hands the lanes words of
+// one group.  V's codes become values in registers: (w >> shift) & 0x03C003C0 |
+// 0x3C003C00 is the pair 1 + code / 16, and one packed multiply-add by (s, o)
+// rounds the value to f16; P^T is S^T's fragment through movmatrix.  (V's
+// channels per m-tile span groups, so its scales cannot wait for the sum.)
 //
 // A CTA is 4 warps that run on their own: warp w takes the 32-token tiles w,
 // w + 4, ... of the CTA's stages, copies them by TMA bulk copies into a ring
@@ -59,7 +65,7 @@ struct Shape {
   // Two warps' O^T, or the columns on their way out.
   static constexpr int Q_AT = MERGE_AT + ((kWarps / 2) * FRAG * 128 > NT * 8 * (D + 4) * 4 ? (kWarps / 2) * FRAG * 128
                                                                                             : NT * 8 * (D + 4) * 4);
-  static constexpr int META_AT = Q_AT + NT * KS * 256;
+  static constexpr int META_AT = Q_AT + NT * (KS + 1) * 256;
 };
 
 struct Meta {
@@ -316,11 +322,12 @@ SPEC_DEV void copy_tile(const AttendParams& p, const Cursor& c, uint8_t* dst, ui
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const __grid_constant__ AttendParams p) {
   using Sh = Shape<D, NT>;
-  constexpr int KW = D / 32;  // code words of K a lane holds of a token
+  constexpr int GR = D / 32;  // groups of a token's channels
   constexpr int VW = D / 64;
   extern __shared__ __align__(128) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + Sh::MERGE_AT);
   uint32_t* qs = reinterpret_cast<uint32_t*>(smem + Sh::Q_AT);  // [nt][kstep][lane][2]
+  uint32_t* qoff = qs + NT * Sh::KS * 64;                       // [nt][lane][2]
   Meta* mt = reinterpret_cast<Meta*>(smem + Sh::META_AT);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t* full = reinterpret_cast<uint64_t*>(mt->full[warp]);
@@ -352,9 +359,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
   const int ks0 = k_scales_at(Pt, D), vc0 = v_codes_at(Pt, D), vs0 = v_scales_at(Pt, D);
   const int code16 = Pt == kTile ? 16 * (D / 2) : block_bytes(16, D);   // from the first 16 tokens to the second
   const int scale16 = Pt == kTile ? 16 * (D / 8) : block_bytes(16, D);
-  // Offsets of this lane's pieces from a 16-token half's first token.
-  const int k_at = g * (D / 2) + t * (KW * 4);
-  const int ks_at = ks0 + (g * (D / 32) + t * (D / 32) / 4) * 4;
+  // Offsets of this lane's pieces from a 16-token half's first token.  K: the
+  // row this lane addresses for ldmatrix (tokens 0-7, 8-15 of a group, then of
+  // the next group).
+  const int k_at = (lane % 16) * (D / 2) + lane / 16 * 16;
+  const int ks_at = ks0 + (g * GR + t % GR) * 4;
   int v_at[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -364,12 +373,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
   const int vs_at = vs0 + t * (D / 32 * 8) + (g * (D / 32) / 8) * 8;
 
   for (int next = u.next;; ++next) {
-    // Columns: q rows as f16 B fragments, scaled by a power of two where bf16
-    // could leave f16's range.  D/8 threads a column, 8 channels each: word
-    // w of the lanes t, pairs (n, n + 4).  All loads are issued first.
+    // Columns: q rows as f16 B fragments q 2^(13 - e), even pairs, and
+    // q 2^(9 - e), odd ones (2^e: about the row's largest magnitude), which
+    // undo the codes' places, and the sums of q over the groups, 2^(-7 - e).
+    // D/8 threads a column, 8 channels each.  All loads are issued first.
     {
       constexpr int TPC = D / 8, PASS = kThreads / TPC, QC = (NT * 8 + PASS - 1) / PASS;
-      const int ch = threadIdx.x % TPC, tt = ch / (D / 32), w = ch % (D / 32);
+      const int ch = threadIdx.x % TPC, tt = ch % 4, gr = ch / 4;
       float x[QC][8];
 #pragma unroll
       for (int i = 0; i < QC; ++i) {
@@ -385,18 +395,30 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
         for (int k = 0; k < 8; ++k) a = fmaxf(a, fabsf(x[i][k]));
 #pragma unroll
         for (int o = 1; o < TPC; o <<= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const int ex = row_exponent(p.q.dtype, a);
+        float sum = ((x[i][0] + x[i][1]) + (x[i][2] + x[i][3])) + ((x[i][4] + x[i][5]) + (x[i][6] + x[i][7]));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // of the group's 32 channels
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int ex = row_exponent(T_BF16, a);
         const float down = pow2i(-ex);
         if (col < NT * 8) {
           uint32_t f[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) f[k] = live ? pack2(x[i][k] * down, x[i][k + 4] * down) : 0u;
-          uint32_t* dst = qs + (((col / 8) * Sh::KS + 2 * w) * 32 + (col % 8) * 4 + tt) * 2;
+          for (int k = 0; k < 4; ++k) {
+            const float e = k % 2 ? 512.f * down : 8192.f * down;
+            f[k] = live ? pack2(x[i][k] * e, x[i][k + 4] * e) : 0u;
+          }
+          uint32_t* dst = qs + (((col / 8) * Sh::KS + 2 * gr) * 32 + (col % 8) * 4 + tt) * 2;
           *reinterpret_cast<uint2*>(dst) = make_uint2(f[0], f[1]);
           *reinterpret_cast<uint2*>(dst + 64) = make_uint2(f[2], f[3]);
+          if (tt < 4 / GR) {  // groups a head of 64 lacks are zero
+            const float v = live && tt == 0 ? sum * (down / 128.f) : 0.f;
+            const float hi = __half2float(__float2half_rn(v));
+            uint32_t* off = qoff + ((col / 8) * 32 + (col % 8) * 4 + tt * GR + gr) * 2;
+            *reinterpret_cast<uint2*>(off) = make_uint2(pack2(hi, hi), pack2(v - hi, v - hi));
+          }
           if (ch == 0) {
             const int row = (u.col0 + col) / G;
-            mt->c[col] = p.scale * kLog2e * pow2i(ex);
+            mt->c[col] = p.scale * kLog2e * 128.f * pow2i(ex);
             mt->idx[col] = live ? row : -1;
             mt->mask[col] = live && p.masks ? p.masks[u.row0 + row] : 0ull;
           }
@@ -447,45 +469,63 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
 #pragma unroll
           for (int n = 0; n < NT; ++n) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
         {
-          uint32_t w[H][2][KW], s2[H][2], o2[H][2];  // [half][token g / g + 8]
+          // (s + o) sum q: the scale pairs as they are stored against the sums of
+          // q over the groups, high and low part.
 #pragma unroll
-          for (int h = 0; h < H; ++h)
+          for (int h = 0; h < H; ++h) {
+            const uint32_t ra = *reinterpret_cast<const uint32_t*>(bs + h * scale16 + ks_at);
+            const uint32_t rb = *reinterpret_cast<const uint32_t*>(bs + h * scale16 + ks_at + D);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 q = *reinterpret_cast<const uint2*>(qoff + (n * 32 + lane) * 2);
+              mma(sc[h][n], ra, rb, ra, rb, q.x, q.y);
+            }
+          }
+          float sg[H][2][GR];  // s of tokens g and g + 8
+          uint32_t w[H][2][GR];
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+#pragma unroll
+            for (int i = 0; i < GR; i += 2) {
+              uint32_t r[4];
+              ldsm_x4(r, bc + h * code16 + k_at + i * 16);
+              w[h][0][i] = r[0], w[h][1][i] = r[1], w[h][0][i + 1] = r[2], w[h][1][i + 1] = r[3];
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const uint8_t* kc = bc + h * code16 + k_at + e * 8 * (D / 2);
-              if constexpr (KW == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(kc);
-                w[h][e][0] = x.x, w[h][e][1] = x.y, w[h][e][2] = x.z, w[h][e][3] = x.w;
+              const __half2* so = reinterpret_cast<const __half2*>(bs + h * scale16 + ks0 + (g + 8 * e) * (GR * 4));
+              if constexpr (GR == 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(so);
+                const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sg[h][e][i] = __low2float(*reinterpret_cast<const __half2*>(&y[i]));
               } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(kc);
-                w[h][e][0] = x.x, w[h][e][1] = x.y;
+                sg[h][e][0] = __low2float(so[0]);
+                sg[h][e][1] = __low2float(so[1]);
               }
-              const uint32_t r = *reinterpret_cast<const uint32_t*>(bs + h * scale16 + ks_at + e * D);
-              s2[h][e] = prmt(r, r, 0x1010);
-              o2[h][e] = prmt(r, r, 0x3232);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < GR; ++i) {
+            uint2 q0[NT], q1[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              q0[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i) * 32 + lane) * 2);
+              q1[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i + 1) * 32 + lane) * 2);
             }
 #pragma unroll
-          for (int i = 0; i < KW; ++i) {
-            uint2 q[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              q[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i) * 32 + lane) * 2);
-#pragma unroll
             for (int h = 0; h < H; ++h) {
-              const uint32_t a0 = dq<0>(w[h][0][i], s2[h][0], o2[h][0]), a1 = dq<0>(w[h][1][i], s2[h][1], o2[h][1]);
-              const uint32_t a2 = dq<1>(w[h][0][i], s2[h][0], o2[h][0]), a3 = dq<1>(w[h][1][i], s2[h][1], o2[h][1]);
+              const uint32_t x = w[h][0][i], y = w[h][1][i], x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma(sc[h][n], a0, a1, a2, a3, q[n].x, q[n].y);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              q[n] = *reinterpret_cast<const uint2*>(qs + ((n * Sh::KS + 2 * i + 1) * 32 + lane) * 2);
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-              const uint32_t a0 = dq<2>(w[h][0][i], s2[h][0], o2[h][0]), a1 = dq<2>(w[h][1][i], s2[h][1], o2[h][1]);
-              const uint32_t a2 = dq<3>(w[h][0][i], s2[h][0], o2[h][0]), a3 = dq<3>(w[h][1][i], s2[h][1], o2[h][1]);
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma(sc[h][n], a0, a1, a2, a3, q[n].x, q[n].y);
+              for (int n = 0; n < NT; ++n) {
+                float a[4] = {0.f, 0.f, 0.f, 0.f};
+                mma(a, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q0[n].x, q0[n].y);
+                mma(a, x8 & 0x000F000Fu, y8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x00F000F0u, q1[n].x, q1[n].y);
+                sc[h][n][0] = fmaf(sg[h][0][i], a[0], sc[h][n][0]);
+                sc[h][n][1] = fmaf(sg[h][0][i], a[1], sc[h][n][1]);
+                sc[h][n][2] = fmaf(sg[h][1][i], a[2], sc[h][n][2]);
+                sc[h][n][3] = fmaf(sg[h][1][i], a[3], sc[h][n][3]);
+              }
             }
           }
         }
