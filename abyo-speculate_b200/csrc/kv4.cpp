@@ -2,7 +2,6 @@
 // argument that the kernels rely on.  A plan is validated on the host and kept
 // in device memory of the library's own, so the kernels need no bounds checks
 // on pages and slots.
-#include <stdlib.h>
 #include <limits.h>
 #include <stdio.h>
 #include <string.h>
@@ -237,12 +236,52 @@ bool wide(const spec_kv4_rows* r) {
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
-const int kWideFrom = getenv("WIDE") ? atoi(getenv("WIDE")) : 64;
+// A unit's queries in and states out cost about as much as two of its stages
+// (64 sequences of 500 to 16000 tokens, one row: 163 us at 0, 149 at 1 and 2,
+// 153 at 3, 157 at 6).
+constexpr int kUnitCost = 2;
+
+// Whether the sequences of more than kWideFrom columns go to the wide kernel:
+// the smaller of two estimates in us, from measurements of both on a B200.  A
+// CTA's stage takes 2.7 us in the narrow kernel (at most 32 columns a unit,
+// two to four CTAs an SM) and 2.85 in the wide one (256 columns, one an SM); a
+// narrow call of more than 8 columns costs 20 besides, others 8, a wide one 15
+// and 10 to join states.  (Measured, narrow against wide: 32 sequences of 4096
+// tokens, 64 columns 175 / 166, 128 columns 324 / 170; one sequence, 128
+// columns at 2048 27 / 28, 256 at 512 25 / 19; eight short trees of 7 to 217
+// columns 20 / 33, as the wide call comes on top.)
+constexpr int kWideFrom = 64;
+bool use_wide(const spec_kv4_batch* b, const spec_kv4_step* s) {
+  const Cache& c = *b->c;
+  const int G = c.d.n_heads / c.d.n_kv_heads;
+  int64_t few = 0, many = 0, wide = 0;  // stages: narrow of each class, wide
+  int most_few = 0;                     // columns of a narrow unit without the many
+  for (int q = 0; q < s->n_seqs; ++q) {
+    const int64_t cols = (int64_t)s->n_rows[q] * G, st = (s->kv_len[q] + s->n_rows[q] + kStageTokens - 1) / kStageTokens;
+    if (cols > kWideFrom) {
+      many += (cols + kMaxCols - 1) / kMaxCols * st;
+      wide += (cols + kWideCols - 1) / kWideCols * st;
+    } else {
+      few += (cols + kMaxCols - 1) / kMaxCols * st;
+      if (cols > most_few) most_few = cols < kMaxCols ? (int)cols : kMaxCols;
+    }
+  }
+  if (!wide) return false;
+  const auto narrow_us = [&](int64_t stages, int cols) {
+    if (!stages) return 0.0;
+    const int64_t slots = (int64_t)b->sms * attend_ctas_per_sm((cols + 7) / 8);
+    return (cols > 8 ? 20.0 : 8.0) + 2.7 * ((stages * c.d.n_kv_heads + slots - 1) / slots);
+  };
+  const int64_t n = (wide * c.d.n_kv_heads + b->sms - 1) / b->sms;
+  const double split = 15.0 + 2.85 * n + (wide * c.d.n_kv_heads > b->sms / 2 ? 10.0 : 0.0) + narrow_us(few, most_few);
+  return split < narrow_us(few + many, kMaxCols);
+}
+
 // Cuts the step's attention into units: per (sequence, kv head, tile of
 // columns) the 128-token stages its rows see, then those stages, laid end to
-// end, into runs of equal length, one a CTA.  Sequences of more than kWideFrom
+// end, into runs of equal cost, one a CTA.  Sequences of more than wide_from
 // columns go to the wide kernel.
-void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
+void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_from) {
   const Cache& c = *b->c;
   Schedule& out = wide ? b->wide : b->narrow;
   const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
@@ -261,7 +300,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
     const int tiles = (cols + most - 1) / most;
     // Narrow tiles are of equal size, wide ones full but for the last.
     const int size = wide ? most : tiles ? ((cols + tiles - 1) / tiles + 7) / 8 * 8 : 0;
-    for (int h = 0; h < c.d.n_kv_heads && (cols > kWideFrom) == wide; ++h)
+    for (int h = 0; h < c.d.n_kv_heads && (cols > wide_from) == wide; ++h)
       for (int c0 = 0; c0 < cols; c0 += size) {
         Unit u{};
         u.kvh = h;
@@ -282,23 +321,64 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
   }
   if (b->tiles.empty()) return;
   const int64_t slots = (int64_t)b->sms * (wide ? 1 : attend_ctas_per_sm(out.nt));
-  const int64_t run = (stages + slots - 1) / slots;
-  int64_t left = run;
+  // A unit costs its stages and kUnitCost more (queries in, states joined and
+  // out).  Either every CTA gets one unit, each tile cut into equal parts of at
+  // most `len` stages; or the tiles are laid end to end and cut where the
+  // running cost passes a CTA's share.  The first does no unit twice a CTA, the
+  // second wastes no CTA where lengths differ: the smaller largest cost wins.
+  int64_t longest = 0;
+  for (const Unit& u : b->tiles) longest = u.st1 > longest ? u.st1 : longest;
+  int64_t lo = 1, len = longest;
+  const auto count = [&](int64_t l) {
+    int64_t n = 0;
+    for (const Unit& u : b->tiles) n += (u.st1 + l - 1) / l;
+    return n;
+  };
+  const bool fits = (int64_t)b->tiles.size() <= slots;
+  while (fits && lo < len) {
+    const int64_t mid = (lo + len) / 2;
+    if (count(mid) <= slots) len = mid;
+    else lo = mid + 1;
+  }
+  const int64_t cost = stages + kUnitCost * ((int64_t)b->tiles.size() + slots);
+  const bool even = fits && (len + kUnitCost - 1) * slots <= cost;
+  // Past kFanIn parts a tile's states are joined in two rounds; a longer run of
+  // up to two stages costs less.
+  const int64_t one_round = (longest + kFanIn - 1) / kFanIn;
+  if (!wide && len < one_round && one_round <= len + 2) len = one_round;
+  int64_t spent = 0;
+  int cta = 0;
   b->cuts.push_back(0);
+  const auto close = [&] {
+    if (b->cuts.back() != (int)b->runs.size()) b->cuts.push_back((int)b->runs.size());
+    ++cta;
+  };
   for (Unit u : b->tiles) {
     const int end = u.st1;
     const size_t first = b->runs.size();
-    for (int at = 0; at < end;) {
-      const int take = (int)(end - at < left ? end - at : left);
+    const int64_t n_even = (end + len - 1) / len;
+    for (int at = 0, i = 0; at < end; ++i) {
+      int64_t take;
+      if (even) {
+        take = end * (i + 1) / n_even - at;
+      } else {
+        // What is left of this CTA's share; at least a stage.
+        const int64_t share = cost * (cta + 1) / slots;
+        int64_t left = share - spent - kUnitCost;
+        if (left < 1 && b->cuts.back() != (int)b->runs.size() && cta + 1 < slots) {
+          close();
+          left = cost * (cta + 1) / slots - spent - kUnitCost;
+        }
+        take = left < 1 ? 1 : left;
+        if (cta + 1 >= slots || take > end - at) take = end - at;
+      }
       u.st0 = at;
-      u.st1 = at + take;
+      u.st1 = at + (int)take;
       u.part = (int)(b->runs.size() - first);
       b->runs.push_back(u);
-      at += take;
-      if ((left -= take) == 0) {
-        b->cuts.push_back((int)b->runs.size());
-        left = run;
-      }
+      at += (int)take;
+      spent += take + kUnitCost;
+      if (even || (spent >= cost * (cta + 1) / slots && cta + 1 < slots)) close();
     }
     const int parts = (int)(b->runs.size() - first);
     for (size_t i = first; i < b->runs.size(); ++i) {
@@ -316,7 +396,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide) {
       out.n_groups += n;
     }
   }
-  if (b->cuts.back() != (int)b->runs.size()) b->cuts.push_back((int)b->runs.size());
+  close();
   out.n_ctas = (int)b->cuts.size() - 1;
   out.order.resize(b->runs.size());
   int at = out.n_ctas;
@@ -391,8 +471,9 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   if (!s->src_rows) max_src = (int)rows - 1;
 
   b->planned = false;
-  schedule(b, s, false);
-  schedule(b, s, true);
+  const int wide_from = use_wide(b, s) ? kWideFrom : INT_MAX;
+  schedule(b, s, false, wide_from);
+  schedule(b, s, true, wide_from);
   // One block: rows, masks, pages, units.
   const size_t at_rows = 0, at_masks = at_rows + up(sizeof(RowDev) * rows), at_table = at_masks + (s->masks ? up(8 * rows) : 0),
                at_narrow = at_table + up(4 * pages), at_wide = at_narrow + up(sizeof(Unit) * b->narrow.order.size()),
