@@ -5,18 +5,22 @@
 // takes up to 256 of them as two tiles of 128 and walks the 128-token stages
 // of its run:
 //   S [128 columns x 128 tokens] = Q K^T        tcgen05.mma, f16 from shared memory
-//   P = 2^(c S - m), rounded to f16 over the second half of S in tensor memory
+//   P = 2^(c S - m), rounded to f16 in place of S in tensor memory (of every
+//       32 columns of S the first 16)
 //   O [128 x D] += P V                          P from tensor memory, V^T from shared memory
-// Roles: warps 0-3 and 4-7 are the softmax of tile 0 and 1, one thread a
-// column; warps 8-10 unpack K and 11-14 V, from page blocks that TMA bulk
-// copies bring, into f16 operand tiles; lane 0 of warp 15 issues the products.
-// (16 warps leave 128 registers a thread; with a fourth warp for K it is 96,
-// and the softmax, which holds 64 scores, spills.)
-// While one tile's softmax runs, the other tile's products do.  Unpacking is
-// paid once for both tiles (1.5 instructions an element and 256 columns).
-// The loops are kept rolled: 16 warps in four roles share an instruction cache
-// that unrolled ones overflow (2048 rows over 6144 tokens: 407 us against the
-// figure below).
+// Roles: warps 0-7 and 8-15 are the softmax of tile 0 and 1, two threads a
+// column (tokens 0-63 and 64-127 of a stage); warps 16-18 unpack K and 19-22
+// V, from page blocks that TMA bulk copies bring, into f16 operand tiles; lane
+// 0 of warp 23 issues the products.  While one tile's softmax runs, the other
+// tile's products do.  Unpacking is paid once for both tiles (1.5 instructions
+// an element and 256 columns).
+//
+// What bounds it: a stage is 2048 cycles of tensor core and 2048 of
+// exponentials an SM, and 2300 issue slots a scheduler.  The loops are kept
+// rolled and small: warps in four roles share an instruction cache that
+// unrolled ones overflow (2048 rows over 6144 tokens: 407 us unrolled, 361
+// rolled).  One thread a column held 64 scores and left the special function
+// unit idle three quarters of the time (272 us, against KV4_WIDE_US).
 //
 // Channels and tokens along a contracted axis may come in any order that both
 // operands share, and O's columns in any order that the output undoes: K's
@@ -38,8 +42,8 @@ namespace kv4 {
 namespace {
 
 constexpr int kTileCols = 128;
-constexpr int kThreads = 16 * 32;
-constexpr int kUnpackK = 8, kUnpackV = 11, kIssuer = 15;  // first warps of the roles
+constexpr int kThreads = 24 * 32;
+constexpr int kUnpackK = 16, kUnpackV = 19, kIssuer = 23;  // first warps of the roles
 constexpr int kThreadsK = (kUnpackV - kUnpackK) * 32;
 
 // ---- tensor memory ----------------------------------------------------------
@@ -81,10 +85,26 @@ SPEC_DEV void tm_store8(uint32_t a, const uint32_t* r) {
 SPEC_DEV void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // f16 A and B, f32 accumulator.
-__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
-// D (+)= A B^T, A and B in shared memory.
-SPEC_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  umma_bf16(d, a, b, idesc, accumulate);  // kind::f16; the types are the descriptor's
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// One lane of a converged warp.  The issuing warp runs its role whole and
+// elects a lane for the products only, so that descriptors stay in uniform
+// registers: a stage's 32 products must each be issued within 64 cycles, next
+// to five busy warps.
+SPEC_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// D (+)= A B^T, A and B in shared memory; FIRST: D is written, not added to.
+template <bool FIRST>
+SPEC_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(FIRST ? 0 : 1)
+      : "memory");
 }
 // A in tensor memory: two f16 a column, lane = row.
 SPEC_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -149,6 +169,7 @@ struct Meta {
   unsigned long long raw_k, raw_v;
   uint32_t bad[2][4];  // tokens of a V stage whose row is NaN
   uint32_t tmem;
+  float red[2][2][2][kTileCols];  // between the two threads of a column: maxima, sums
 };
 
 // ---- unpacking: 96 threads for K, 128 for V --------------------------------
@@ -311,68 +332,86 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
   if (!ok && copies) mbar_wait_bounded(raw_full, (copies - 1) & 1, p.err);  // leave no copy in flight
 }
 
-// ---- products: one thread ---------------------------------------------------
+// ---- products: one warp -----------------------------------------------------
 template <int D>
 SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem) {
   using Sh = Shape<D>;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
   constexpr uint32_t kS = idesc_f16(kTileCols, kStageTokens), kO = idesc_f16(kTileCols, D);
-  const uint32_t base = smem_u32(smem);
-  bool ok = true;
-  int k = 0;
-  int waits[2] = {0, 0}, units[2] = {0, 0};  // phases of p_full and q_full
-  auto scores = [&](int a, int slot) {
-#pragma unroll
-    for (int i = 0; i < Sh::KS; ++i)
-      mma_ss(tmem + a * 128, umma_desc_kmajor(base + a * Sh::Q_TILE + i * 4096, 128, 256),
-             umma_desc_kmajor(base + Sh::K_AT + slot * Sh::Q_TILE + i * 4096, 128, 256), kS, i > 0);
-    umma_commit(bar(mt->s_full[a]));
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  const uint64_t q0 = umma_desc_kmajor(smem_u32(smem), 128, 256);  // Q tile 0; the others lie at multiples of 16 bytes
+  constexpr uint64_t kTile16 = Sh::Q_TILE / 16, kK16 = Sh::K_AT / 16, kV16 = Sh::V_AT / 16;
+  auto wait = [&](unsigned long long& b, int parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar(b), parity, p.err)) != 0;
   };
-  int ui = blockIdx.x;
-  Unit u = p.units[ui];
-  for (int next = u.next; ok; ++next) {
-    const int tiles = u.n_cols > kTileCols ? 2 : 1, n = u.st1 - u.st0;
-    ok = ok && mbar_wait_bounded(bar(mt->k_full[k & 1]), (k >> 1) & 1, p.err);
-    for (int a = 0; a < tiles; ++a) {
-      ok = ok && mbar_wait_bounded(bar(mt->q_full[a]), units[a]++ & 1, p.err);
-      if (!ok) break;
-      tc_fence_after();
-      scores(a, k & 1);
-    }
-    if (!ok) break;
-    umma_commit(bar(mt->k_free[k & 1]));
-    for (int i = 0; i < n && ok; ++i, ++k) {
-      const int slot = k & 1, ahead = (k + 1) & 1;
-      ok = ok && mbar_wait_bounded(bar(mt->v_full[slot]), (k >> 1) & 1, p.err);
-      for (int a = 0; a < tiles && ok; ++a) {
-        ok = ok && mbar_wait_bounded(bar(mt->p_full[a]), waits[a]++ & 1, p.err);
-        if (!ok) break;
-        tc_fence_after();
+  auto scores = [&](int a, int slot, bool free_k) {
+    if (elect_one()) {
+      const uint64_t qa = q0 + a * kTile16, kb = q0 + kK16 + slot * kTile16;
+      const uint32_t d = tmem + a * 128;
+      mma_ss<true>(d, qa, kb, kS);
 #pragma unroll
-        for (int j = 0; j < kStageTokens / 16; ++j)
-          mma_ts(tmem + 256 + a * 128, tmem + a * 128 + 64 + j * 8,
-                 umma_desc_kmajor(base + Sh::V_AT + slot * Sh::Q_TILE + j * (D * 32), 128, 256), kO, i > 0 || j > 0);
-        if (i + 1 == n) {
-          umma_commit(bar(mt->o_full[a]));
-        } else {
-          if (a == 0) ok = ok && mbar_wait_bounded(bar(mt->k_full[ahead]), ((k + 1) >> 1) & 1, p.err);
+      for (int i = 1; i < Sh::KS; ++i) mma_ss<false>(d, qa + i * 256, kb + i * 256, kS);
+      umma_commit(bar(mt->s_full[a]));
+      if (free_k) umma_commit(bar(mt->k_free[slot]));
+    }
+    __syncwarp();
+  };
+  int k = 0;
+  int waits = 0, units = 0;  // phases of p_full and q_full, a bit a tile
+  Unit u = p.units[blockIdx.x];
+  bool ok = true;
+#pragma unroll 1
+  for (int next = __shfl_sync(0xffffffffu, u.next, 0);; ++next) {
+    const int tiles = __shfl_sync(0xffffffffu, u.n_cols, 0) > kTileCols ? 2 : 1;
+    const int n = __shfl_sync(0xffffffffu, u.st1 - u.st0, 0), last = __shfl_sync(0xffffffffu, u.last, 0);
+    ok = wait(mt->k_full[k & 1], (k >> 1) & 1);
+#pragma unroll 1
+    for (int a = 0; a < tiles && ok; ++a) {
+      ok = wait(mt->q_full[a], units >> a & 1);
+      if (!ok) break;
+      units ^= 1 << a;
+      tc_fence_after();
+      scores(a, k & 1, a == tiles - 1);
+    }
+#pragma unroll 1
+    for (int i = 0; i < n && ok; ++i, ++k) {
+      const int slot = k & 1, ahead = slot ^ 1;
+      const bool more = i + 1 < n;
+      ok = wait(mt->v_full[slot], (k >> 1) & 1);
+#pragma unroll 1
+      for (int a = 0; a < tiles && ok; ++a) {
+        ok = wait(mt->p_full[a], waits >> a & 1);
+        if (!ok) break;
+        waits ^= 1 << a;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vb = q0 + kV16 + slot * kTile16;
+          const uint32_t d = tmem + 256 + a * 128, pa = tmem + a * 128;
+          mma_ts(d, pa, vb, kO, i > 0);
+#pragma unroll
+          for (int j = 1; j < kStageTokens / 16; ++j)
+            mma_ts(d, pa + j / 2 * 32 + j % 2 * 8, vb + j * (D * 2), kO, 1);
+          if (!more) umma_commit(bar(mt->o_full[a]));
+          if (a == tiles - 1) umma_commit(bar(mt->v_free[slot]));
+        }
+        __syncwarp();
+        if (more) {
+          if (a == 0) ok = wait(mt->k_full[ahead], ((k + 1) >> 1) & 1);
           if (!ok) break;
-          scores(a, ahead);
+          scores(a, ahead, a == tiles - 1);
         }
       }
-      if (!ok) break;
-      umma_commit(bar(mt->v_free[slot]));
-      if (i + 1 < n) umma_commit(bar(mt->k_free[ahead]));
     }
-    if (next == u.last) break;
+    if (!ok || next == last) break;
     u = p.units[next];
   }
   // Nothing is left in flight when tensor memory is freed.
-  umma_commit(bar(mt->idle));
-  mbar_wait_bounded(bar(mt->idle), 0, p.err);
+  if (elect_one()) umma_commit(bar(mt->idle));
+  __syncwarp();
+  wait(mt->idle, 0);
 }
 
-// ---- softmax: one thread a column -------------------------------------------
+// ---- softmax: two threads a column ------------------------------------------
 SPEC_DEV uint4 raw8(const Rows& r, long long at, bool wide) {
   const uint16_t* s = static_cast<const uint16_t*>(r.ptr) + at;
   if (wide) return *reinterpret_cast<const uint4*>(s);
@@ -399,32 +438,48 @@ SPEC_DEV void put_q(uint8_t* row, int i, const uint4& w, int dtype, float down, 
   *reinterpret_cast<uint4*>(row + (i / 2) * 4096 + (i % 2) * 128) = f;
 }
 
+// Scores that are not seen.
+SPEC_DEV void hide(float (&x)[32], uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = (seen >> i) & 1 ? x[i] : -INFINITY;
+}
+
 template <int D>
-SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem, int a) {
+SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem, int a, int half) {
   using Sh = Shape<D>;
   constexpr int NC = Sh::NC;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
   const int th = threadIdx.x & 127, G = p.n_heads / p.n_kv, col = a * kTileCols + th;
   const uint32_t lane_at = (uint32_t)(th / 32 * 32) << 16;
-  const uint32_t s_at = tmem + a * 128 + lane_at, o_at = tmem + 256 + a * 128 + lane_at;
+  const uint32_t s_at = tmem + a * 128 + 64 * half + lane_at, o_at = tmem + 256 + a * 128 + lane_at;
+  // A value of this thread's for the column's other one, and back.  (Between
+  // two uses of a `kind` lies a barrier that both threads reach after reading:
+  // q_full or p_full.)
+  auto meet = [&](int kind, float mine) {
+    mt->red[kind][a][half][th] = mine;
+    asm volatile("bar.sync %0, 256;" ::"r"(5 + a) : "memory");
+    return mt->red[kind][a][half ^ 1][th];
+  };
   bool ok = true;
   int k = 0, v = 0, unit = 0;  // stages of this tile, of the run; units of this tile
   Unit u = p.units[blockIdx.x];
+#pragma unroll 1
   for (int next = u.next;; ++next) {
     if (a * kTileCols < u.n_cols) {
       const bool live = col < u.n_cols;
       const int r = u.col0 + (live ? col : 0), row = r / G, head = u.kvh * G + r % G;
-      // This column's q, in the order K's channels are unpacked.  A negative
-      // scale goes to q's sign, so that the largest product is the largest score.
+      // This column's q (half of its channels a thread), in the order K's
+      // channels are unpacked.  A negative scale goes to q's sign, so that the
+      // largest product is the largest score.  Converted as it is, four 16-byte
+      // loads in flight; a row whose largest magnitude (16-bit floats without
+      // their sign order as integers) is far from 1 is converted again, scaled
+      // by a power of two.
       const long long at = (u.row0 + row) * p.q.row_stride + head * p.q.head_stride;
       uint8_t* dst = smem + a * Sh::Q_TILE + (th / 8) * 256 + (th % 8) * 16;
-      // Converted as it is, four 16-byte loads in flight; a row whose largest
-      // magnitude (16-bit floats without their sign order as integers) is far
-      // from 1 is converted again, scaled by a power of two.
       const float sign = p.scale < 0.f ? -1.f : 1.f;
       uint32_t top = 0;
 #pragma unroll 1
-      for (int i0 = 0; i0 < NC; i0 += 4) {
+      for (int i0 = half * (NC / 2); i0 < (half + 1) * (NC / 2); i0 += 4) {
         uint4 w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = raw8(p.q, at + (i0 + i) * 8, p.wide_q);
@@ -436,12 +491,13 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         }
       }
       top = max(top & 0xffffu, top >> 16);
-      int ex = row_exponent(p.q.dtype, __uint_as_float(top << 16));
+      const float other_top = meet(0, __uint_as_float(top << 16));
+      int ex = row_exponent(p.q.dtype, fmaxf(__uint_as_float(top << 16), other_top));
       if (ex >= -4 && ex <= 14) {
         ex = 0;
       } else {
 #pragma unroll 1
-        for (int i = 0; i < NC; ++i)
+        for (int i = half * (NC / 2); i < (half + 1) * (NC / 2); ++i)
           put_q<D>(dst, i, raw8(p.q, at + i * 8, p.wide_q), p.q.dtype, sign * pow2i(-ex), live);
       }
       publish_smem();
@@ -454,38 +510,31 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
 
 #pragma unroll 1
       for (int st = u.st0; st < u.st1; ++st, ++k) {
-        const int tok = st * kStageTokens, stage = v + st - u.st0;
-        const bool tail = tok + kStageTokens > u.sure;
-        uint32_t sees[4];
+        const int tok = st * kStageTokens + 64 * half, stage = v + st - u.st0;
+        const bool tail = (st + 1) * kStageTokens > u.sure;
+        uint32_t sees[2] = {~0u, ~0u};
         if (tail) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
             sees[q] = seen32(tok + 32 * q, u.kv_len, p.masks != nullptr, mask, idx) & first32(u.kv_end - tok - 32 * q);
         }
         ok = ok && mbar_wait_bounded(bar(mt->s_full[a]), k & 1, p.err);
         tc_fence_after();
-        // The largest score of the stage, a half at a time; the second half
-        // stays in registers for the next pass.
+        // The column's largest score; tokens 32 to 63 stay in registers.
         float best = -INFINITY;
-        float x[64];
-        auto mask = [&](float* y, uint32_t w) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = (w >> i) & 1 ? y[i] : -INFINITY;
-        };
+        float x[32];
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) tm_load<16>(s_at + 64 * h + 16 * b, x + 16 * b);
+          tm_load<16>(s_at + 32 * h, x);
+          tm_load<16>(s_at + 32 * h + 16, x + 16);
           tm_wait(x);
-          if (tail) {
-            mask(x, h ? sees[2] : sees[0]);
-            mask(x + 32, h ? sees[3] : sees[1]);
-          }
+          if (tail) hide(x, h ? sees[1] : sees[0]);
           float part[4] = {best, x[0], x[1], x[2]};
 #pragma unroll
-          for (int i = 3; i < 63; i += 2) part[i / 2 % 4] = max3(part[i / 2 % 4], x[i], x[i + 1]);
-          best = max3(max3(part[0], part[1], x[63]), part[2], part[3]);
+          for (int i = 3; i < 31; i += 2) part[i / 2 % 4] = max3(part[i / 2 % 4], x[i], x[i + 1]);
+          best = max3(max3(part[0], part[1], x[31]), part[2], part[3]);
         }
+        best = fmaxf(best, meet(0, best));
         best = best > -INFINITY ? best * c : -INFINITY;
         const bool over = best > m + kSlack;
         if (__any_sync(0xffffffffu, over)) {
@@ -494,7 +543,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           l *= by;
           if (st > u.st0) {
 #pragma unroll 1
-            for (int q = 0; q < D; q += 8) {
+            for (int q = half * (D / 2); q < (half + 1) * (D / 2); q += 8) {
               float o[8];
               tm_load<8>(o_at + q, o);
               tm_wait(o);
@@ -506,36 +555,32 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         }
         const unsigned long long c2 = two(c, c), m2 = two(-m, -m);
         unsigned long long sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
-        // P of the second half, then of the first, to the tile's upper 64 columns.
 #pragma unroll 1
         for (int h = 1; h >= 0; --h) {
           if (h == 0) {
             tm_wait(x);
-            if (tail) {
-              mask(x, sees[0]);
-              mask(x + 32, sees[1]);
-            }
+            if (tail) hide(x, sees[0]);
           }
           // Two exponentials every 16 cycles is what the special function unit
-          // gives a warp; the pinned order keeps it fed, the multiply-adds two
-          // pairs ahead of it and the sums and roundings four pairs behind
-          // (64 scores: 655 cycles alone, 970 in the compiler's order).
-          uint32_t f[32];
+          // gives a scheduler; the pinned order keeps it fed, the multiply-adds
+          // two pairs ahead of it and the sums and roundings four pairs behind
+          // (32 scores: 328 cycles alone, 487 in the compiler's order).
+          uint32_t f[16];
 #pragma unroll
-          for (int j = 0; j < 32 + 6; ++j) {
-            if (j < 32) pin_fma2(x[2 * j], x[2 * j + 1], c2, m2);
-            if (j >= 2 && j < 34) pin_ex2(x[2 * j - 4]), pin_ex2(x[2 * j - 3]);
+          for (int j = 0; j < 16 + 6; ++j) {
+            if (j < 16) pin_fma2(x[2 * j], x[2 * j + 1], c2, m2);
+            if (j >= 2 && j < 18) pin_ex2(x[2 * j - 4]), pin_ex2(x[2 * j - 3]);
             if (j >= 6) {
               const int i = j - 6;
               pin_add2(sum[i % 2], x[2 * i], x[2 * i + 1]);
               f[i] = pin_pack2(x[2 * i], x[2 * i + 1]);
             }
           }
-#pragma unroll
-          for (int b = 0; b < 4; ++b) tm_store8(s_at + 64 + 32 * h + 8 * b, f + 8 * b);
+          tm_store8(s_at + 32 * h, f);
+          tm_store8(s_at + 32 * h + 8, f + 8);
           if (h == 1) {
-#pragma unroll
-            for (int b = 0; b < 4; ++b) tm_load<16>(s_at + 16 * b, x + 16 * b);
+            tm_load<16>(s_at, x);
+            tm_load<16>(s_at + 16, x + 16);
           }
         }
         float sum_lo, sum_hi;
@@ -544,8 +589,8 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         if (tail) {
           // A column that sees a NaN row of V, known once V is unpacked, is NaN.
           ok = ok && mbar_wait_bounded(bar(mt->v_full[stage & 1]), (stage >> 1) & 1, p.err);
-          const uint32_t* b = mt->bad[stage & 1];
-          if ((b[0] & sees[0]) | (b[1] & sees[1]) | (b[2] & sees[2]) | (b[3] & sees[3])) l = __int_as_float(0x7fffffff);
+          const uint32_t* b = mt->bad[stage & 1] + 2 * half;
+          if ((b[0] & sees[0]) | (b[1] & sees[1])) l = __int_as_float(0x7fffffff);
         }
         tm_wait_st();
         tc_fence_before();
@@ -553,12 +598,13 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       }
       ok = ok && mbar_wait_bounded(bar(mt->o_full[a]), unit++ & 1, p.err);
       tc_fence_after();
-      // O to the output, or as a partial state [D][256], m, l.
+      l += meet(1, l);
+      // O to the output, or as a partial state [D][256], m, l; half the channels a thread.
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long out_at = (u.row0 + row) * p.out.row_stride + head * p.out.head_stride;
       float* part = p.parts + (long long)(u.part0 + u.part) * ((D + 2) * kWideCols) + col;
 #pragma unroll 1
-      for (int i = 0; i < NC; ++i) {
+      for (int i = half * (NC / 2); i < (half + 1) * (NC / 2); ++i) {
         float y[8];  // channels 8 i ..
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = tm_load1(o_at + e * NC + i);
@@ -572,7 +618,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           for (int e = 0; e < 8; ++e) part[(i * 8 + e) * kWideCols] = y[e];
         }
       }
-      if (u.n_parts > 1) {
+      if (u.n_parts > 1 && half == 0) {
         part[D * kWideCols] = m;
         part[(D + 1) * kWideCols] = l;
       }
@@ -620,13 +666,13 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   if (threadIdx.x == 0) {
     auto init = [](unsigned long long& b, int n) { mbar_init(reinterpret_cast<uint64_t*>(&b), n); };
     for (int i = 0; i < 2; ++i) {
-      init(mt->q_full[i], 128);
+      init(mt->q_full[i], 256);
       init(mt->k_full[i], kThreadsK);
       init(mt->k_free[i], 1);
       init(mt->v_full[i], 128);
       init(mt->v_free[i], 1);
       init(mt->s_full[i], 1);
-      init(mt->p_full[i], 128);
+      init(mt->p_full[i], 256);
       init(mt->o_full[i], 1);
     }
     init(mt->idle, 1);
@@ -640,12 +686,12 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   tc_fence_after();
   const uint32_t tmem = mt->tmem;
   if (warp < kUnpackK) {
-    softmax_role<D>(p, smem, mt, tmem, warp / 4);
+    softmax_role<D>(p, smem, mt, tmem, warp / 8, warp / 4 % 2);
   } else if (warp < kUnpackV) {
     unpack_role<D, false>(p, smem, mt, threadIdx.x - kUnpackK * 32);
   } else if (warp < kIssuer) {
     unpack_role<D, true>(p, smem, mt, threadIdx.x - kUnpackV * 32);
-  } else if ((threadIdx.x & 31) == 0) {
+  } else {
     issue_role<D>(p, smem, mt, tmem);
   }
   __syncwarp();
