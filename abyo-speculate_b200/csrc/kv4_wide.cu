@@ -20,7 +20,7 @@
 // rolled and small: warps in four roles share an instruction cache that
 // unrolled ones overflow (2048 rows over 6144 tokens: 407 us unrolled, 361
 // rolled).  One thread a column held 64 scores and left the special function
-// unit idle three quarters of the time (272 us, against KV4_WIDE_US).
+// unit idle three quarters of the time (272 us against 237).
 //
 // Channels and tokens along a contracted axis may come in any order that both
 // operands share, and O's columns in any order that the output undoes: K's
@@ -29,7 +29,7 @@
 // store neighbouring rows.
 //
 // O is scaled only where a column's largest score passes its reference m by
-// more than kSlack octaves.  Runs are cut as for the narrow kernel (kv4_attend.cu); the partial
+// more than kSlack octaves; P is made before that is known.  Runs are cut as for the narrow kernel (kv4_attend.cu); the partial
 // states of a column tile that several CTAs share are joined by a second
 // kernel, whose blocks spread over the channels.
 #include "common.cuh"
@@ -169,7 +169,7 @@ struct Meta {
   unsigned long long raw_k, raw_v;
   uint32_t bad[2][4];  // tokens of a V stage whose row is NaN
   uint32_t tmem;
-  float red[2][2][2][kTileCols];  // between the two threads of a column: maxima, sums
+  float red[3][2][2][kTileCols];  // between the two threads of a column: largest, sum, largest again
 };
 
 // ---- unpacking: 96 threads for K, 128 for V --------------------------------
@@ -457,7 +457,9 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
   // q_full or p_full.)
   auto meet = [&](int kind, float mine) {
     mt->red[kind][a][half][th] = mine;
-    asm volatile("bar.sync %0, 256;" ::"r"(5 + a) : "memory");
+    // Of the two warps that share these 32 columns alone: how often they meet
+    // depends on the columns' scores.
+    asm volatile("bar.sync %0, 64;" ::"r"(5 + a * 4 + th / 32) : "memory");
     return mt->red[kind][a][half ^ 1][th];
   };
   bool ok = true;
@@ -520,25 +522,54 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         }
         ok = ok && mbar_wait_bounded(bar(mt->s_full[a]), k & 1, p.err);
         tc_fence_after();
-        // The column's largest score; tokens 32 to 63 stay in registers.
-        float best = -INFINITY;
-        float x[32];
+        // P against the column's last reference, kept in registers until the
+        // column's largest exponent is known.  Where that passes kSlack, or
+        // there is no reference yet, it moves the reference and P is made
+        // again; the scores are still there.
+        uint32_t f[32];
+        float added;
+        int kind = 0;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          tm_load<16>(s_at + 32 * h, x);
-          tm_load<16>(s_at + 32 * h + 16, x + 16);
-          tm_wait(x);
-          if (tail) hide(x, h ? sees[1] : sees[0]);
-          float part[4] = {best, x[0], x[1], x[2]};
+        while (true) {
+          const float base = m == kNone ? 0.f : m;
+          const unsigned long long c2 = two(c, c), m2 = two(-base, -base);
+          unsigned long long sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+          float best = -INFINITY;
 #pragma unroll
-          for (int i = 3; i < 31; i += 2) part[i / 2 % 4] = max3(part[i / 2 % 4], x[i], x[i + 1]);
-          best = max3(max3(part[0], part[1], x[31]), part[2], part[3]);
-        }
-        best = fmaxf(best, meet(0, best));
-        best = best > -INFINITY ? best * c : -INFINITY;
-        const bool over = best > m + kSlack;
-        if (__any_sync(0xffffffffu, over)) {
-          const float mm = over ? best : m, by = ex2(m - mm);
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            tm_load<16>(s_at + 32 * h, x);
+            tm_load<16>(s_at + 32 * h + 16, x + 16);
+            tm_wait(x);
+            if (tail) hide(x, sees[h]);
+            // Two exponentials every 16 cycles is what the special function
+            // unit gives a scheduler; the pinned order keeps it fed, the
+            // multiply-adds two pairs ahead of it and the sums and roundings
+            // four pairs behind (32 scores: 328 cycles alone, 487 in the
+            // compiler's order).
+#pragma unroll
+            for (int j = 0; j < 16 + 6; ++j) {
+              if (j < 16) {
+                pin_fma2(x[2 * j], x[2 * j + 1], c2, m2);
+                best = max3(best, x[2 * j], x[2 * j + 1]);
+              }
+              if (j >= 2 && j < 18) pin_ex2(x[2 * j - 4]), pin_ex2(x[2 * j - 3]);
+              if (j >= 6) {
+                const int i = j - 6;
+                pin_add2(sum[i % 2], x[2 * i], x[2 * i + 1]);
+                f[16 * h + i] = pin_pack2(x[2 * i], x[2 * i + 1]);
+              }
+            }
+          }
+          float sum_lo, sum_hi;
+          apart(add2(sum[0], sum[1]), sum_lo, sum_hi);
+          added = sum_lo + sum_hi;
+          best = fmaxf(best, meet(kind, best));
+          const bool over = m == kNone ? best > -INFINITY : best > kSlack;
+          // Both warps of these columns decide alike.
+          if (!__any_sync(0xffffffffu, over)) break;
+          kind = 2;
+          const float mm = over ? base + best : m, by = ex2(m - mm);
           m = mm;
           l *= by;
           if (st > u.st0) {
@@ -553,39 +584,9 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
             }
           }
         }
-        const unsigned long long c2 = two(c, c), m2 = two(-m, -m);
-        unsigned long long sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
-#pragma unroll 1
-        for (int h = 1; h >= 0; --h) {
-          if (h == 0) {
-            tm_wait(x);
-            if (tail) hide(x, sees[0]);
-          }
-          // Two exponentials every 16 cycles is what the special function unit
-          // gives a scheduler; the pinned order keeps it fed, the multiply-adds
-          // two pairs ahead of it and the sums and roundings four pairs behind
-          // (32 scores: 328 cycles alone, 487 in the compiler's order).
-          uint32_t f[16];
+        l += added;
 #pragma unroll
-          for (int j = 0; j < 16 + 6; ++j) {
-            if (j < 16) pin_fma2(x[2 * j], x[2 * j + 1], c2, m2);
-            if (j >= 2 && j < 18) pin_ex2(x[2 * j - 4]), pin_ex2(x[2 * j - 3]);
-            if (j >= 6) {
-              const int i = j - 6;
-              pin_add2(sum[i % 2], x[2 * i], x[2 * i + 1]);
-              f[i] = pin_pack2(x[2 * i], x[2 * i + 1]);
-            }
-          }
-          tm_store8(s_at + 32 * h, f);
-          tm_store8(s_at + 32 * h + 8, f + 8);
-          if (h == 1) {
-            tm_load<16>(s_at, x);
-            tm_load<16>(s_at + 16, x + 16);
-          }
-        }
-        float sum_lo, sum_hi;
-        apart(add2(sum[0], sum[1]), sum_lo, sum_hi);
-        l += sum_lo + sum_hi;
+        for (int b = 0; b < 4; ++b) tm_store8(s_at + b / 2 * 32 + b % 2 * 8, f + 8 * b);
         if (tail) {
           // A column that sees a NaN row of V, known once V is unpacked, is NaN.
           ok = ok && mbar_wait_bounded(bar(mt->v_full[stage & 1]), (stage >> 1) & 1, p.err);
