@@ -244,13 +244,13 @@ constexpr int kUnitCost = 2;
 // Whether the sequences of more than kWideFrom columns go to the wide kernel:
 // the smaller of two estimates in us, from measurements of both on a B200.  A
 // CTA's stage takes 2.7 us in the narrow kernel (at most 32 columns a unit,
-// two to four CTAs an SM) and 2.85 in the wide one (256 columns, one an SM); a
+// two to four CTAs an SM) and 2.5 in the wide one (256 columns, one an SM); a
 // narrow call of more than 8 columns costs 20 besides, others 8, a wide one 15
 // and 10 to join states.  (Measured, narrow against wide: 32 sequences of 4096
-// tokens, 64 columns 175 / 166, 128 columns 324 / 170; one sequence, 128
-// columns at 2048 27 / 28, 256 at 512 25 / 19; eight short trees of 7 to 217
-// columns 20 / 33, as the wide call comes on top.)
-constexpr int kWideFrom = 64;
+// tokens, 48 columns 135 / 146, 64 columns 175 / 146, 128 columns 324 / 146;
+// one sequence, 128 columns at 2048 27 / 22, 256 at 512 25 / 21; eight short
+// trees of 7 to 217 columns 20 / 33, as the wide call comes on top.)
+constexpr int kWideFrom = 48;
 bool use_wide(const spec_kv4_batch* b, const spec_kv4_step* s) {
   const Cache& c = *b->c;
   const int G = c.d.n_heads / c.d.n_kv_heads;
@@ -273,7 +273,7 @@ bool use_wide(const spec_kv4_batch* b, const spec_kv4_step* s) {
     return (cols > 8 ? 20.0 : 8.0) + 2.7 * ((stages * c.d.n_kv_heads + slots - 1) / slots);
   };
   const int64_t n = (wide * c.d.n_kv_heads + b->sms - 1) / b->sms;
-  const double split = 15.0 + 2.85 * n + (wide * c.d.n_kv_heads > b->sms / 2 ? 10.0 : 0.0) + narrow_us(few, most_few);
+  const double split = 15.0 + 2.5 * n + (wide * c.d.n_kv_heads > b->sms / 2 ? 10.0 : 0.0) + narrow_us(few, most_few);
   return split < narrow_us(few + many, kMaxCols);
 }
 
