@@ -433,7 +433,9 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
     rows += m;
     pages += (n + m + P - 1) / P;
   }
-  if (rows > (1 << 24)) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: %lld rows (at most 2^24)", (long long)rows);
+  if (rows > (1 << 24) || rows * (c.d.n_heads / c.d.n_kv_heads) > (1 << 30))
+    return fail(SPEC_ERR_INVALID, "spec_kv4_plan: %lld rows (at most 2^24, and 2^30 with the query heads of a kv head)",
+                (long long)rows);
   if (pages > (INT64_C(1) << 28)) return fail(SPEC_ERR_INVALID, "spec_kv4_plan: page tables of %lld entries", (long long)pages);
   // Pages: inside the pool, and a page that is written is listed once.
   b->seen.resize(c.d.n_pages, 0);
@@ -502,7 +504,7 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   // The two kernels run one after the other and share the partial states.
   const size_t floats_narrow = b->narrow.n_parts * attend_part_floats(c.d.head_dim, b->narrow.nt),
                floats_wide = b->wide.n_parts * wide_part_floats(c.d.head_dim);
-  if ((e = grow(b, &b->arrived, &b->arrived_cap, b->narrow.n_groups + b->wide.n_groups, true)) != cudaSuccess ||
+  if ((e = grow(b, &b->arrived, &b->arrived_cap, b->narrow.n_groups, true)) != cudaSuccess ||
       (e = grow(b, &b->parts, &b->parts_cap, floats_narrow > floats_wide ? floats_narrow : floats_wide, false)) != cudaSuccess)
     return fail_cuda(e, "spec_kv4_plan");
   RowDev* hr = reinterpret_cast<RowDev*>(b->host + at_rows);
@@ -710,7 +712,6 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   p.table = b->table;
   p.masks = b->masks;
   p.parts = b->parts;
-  p.arrived = b->arrived;
   p.err = b->err;
   p.q = to_rows(q);
   p.out = to_rows(out);
@@ -734,7 +735,7 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
   if (e == cudaSuccess && b->narrow.n_ctas) {
     p.units = b->narrow.units;
     p.n_ctas = b->narrow.n_ctas;
-    p.arrived = b->arrived + b->wide.n_groups;
+    p.arrived = b->arrived;
     e = launch_attend(p, D, b->narrow.nt, st);
   }
   if (e == cudaSuccess) e = turn.leave();
@@ -749,7 +750,12 @@ int spec_kv4_status(spec_kv4_batch* b) {
   if (e != cudaSuccess) return fail_cuda(e, "spec_kv4_status");
   char msg[256];
   const int rc = take_device_error(b->err, nullptr, msg, sizeof msg);
-  if (rc != SPEC_OK) set_thread_error(msg);
+  if (rc != SPEC_OK) {
+    set_thread_error(msg);
+    // A call that gave up may have left arrivals behind.
+    if (b->arrived) cudaMemset(b->arrived, 0, b->arrived_cap * sizeof(int));
+    cudaDeviceSynchronize();
+  }
   return rc;
 }
 

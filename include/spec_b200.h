@@ -595,10 +595,13 @@ int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
 /* out = softmax(scale * q . k) v for every row and query head of the step
  * over `layer`'s pages, whose rows of this step were appended before.  q: bf16
  * or f16 rotated rows; out: any type.  Query head h reads kv head
- * h / (n_heads / n_kv_heads).  Products take q and the stored values as f16
- * (q after an exact power-of-two scaling of each row) and sum in f32.  A row
- * that sees nothing gives zeros.  One call's result does not depend on
- * timing; a row's last bits may depend on the other rows of the plan. */
+ * h / (n_heads / n_kv_heads).  Products take the stored values rounded to f16
+ * or exactly, q after an exact power-of-two scaling of each row, and sum in
+ * f32; weights go to the second product as f16, their sums are f32.  A row
+ * that sees nothing gives zeros; a row that sees a stored NaN gives NaN.  One
+ * call's result does not depend on timing; a row's last bits may depend on the
+ * other rows of the plan.  A call recorded by stream capture holds the plan's
+ * addresses: replay it only until the batch's next plan. */
 int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const spec_kv4_rows* out, float scale,
                     void* stream);
 /* Waits for the batch's calls and reports (and clears) a device wait

@@ -279,25 +279,27 @@ def test_attend_trees(pkg, d, heads, kv_heads, page):
     check_attend(s, kv, rows, q, out, masks, "f16")
 
 
-def test_attend_rows_that_see_nothing_give_zeros(pkg):
+@pytest.mark.parametrize("heads", [4, 64])
+def test_attend_rows_that_see_nothing_give_zeros(pkg, heads):
     kv, rows = [0, 12], [5, 3]
-    s = Setup(pkg, 4, 2, 128, 16, [5, 15], seed=8)
+    s = Setup(pkg, heads, 2, 128, 16, [5, 15], seed=8)
     s.fill([5, 15])
     masks = [0, 1, 0, 8, 0b11111, 0, 0, 1]
-    q, _ = s.rows(8, 4, "bf16")
+    q, _ = s.rows(8, heads, "bf16")
     s.batch.plan(kv, rows, s.table, masks=masks)
     out = s.batch.attend(0, q)
     check_attend(s, kv, rows, q, out, masks, "bf16")
     assert (out[0] == 0).all() and (out[2] == 0).all() and not (out[5] == 0).all()
 
 
-def test_attend_nan_stays_where_it_is_seen(pkg):
+@pytest.mark.parametrize("heads", [4, 32])
+def test_attend_nan_stays_where_it_is_seen(pkg, heads):
     """A NaN key row, and a NaN value row, of a draft node reach the rows that
     see the node and no other; the unwritten bytes of a page read as NaN and
-    reach none."""
+    reach none.  12 and 96 columns."""
     import torch
     kv, rows = [9], [6]
-    s = Setup(pkg, 4, 2, 128, 16, [15], rope=False, seed=9)
+    s = Setup(pkg, heads, 2, 128, 16, [15], rope=False, seed=9)
     s.fill([9])
     k, kn = s.rows(6, 2, "f32")
     v, vn = s.rows(6, 2, "f32")
@@ -309,21 +311,22 @@ def test_attend_nan_stays_where_it_is_seen(pkg):
     s.batch.append(0, None, k, v)
     for i in range(6):
         s.store(0, 9 + i, kn[i], vn[i])
-    q, _ = s.rows(6, 4, "bf16")
+    q, _ = s.rows(6, heads, "bf16")
     out = s.batch.attend(0, q)
     check_attend(s, kv, rows, q, out, masks, "bf16")
     bad = torch.isnan(out).flatten(2).any(2).cpu().numpy()
-    want = np.zeros((6, 4), bool)
-    want[2, :2] = want[3, 2:] = True
+    want = np.zeros((6, heads), bool)
+    want[2, :heads // 2] = want[3, heads // 2:] = True
     assert (bad == want).all()
 
 
-def test_attend_peaked_and_large_scores(pkg):
+@pytest.mark.parametrize("heads", [4, 32])
+def test_attend_peaked_and_large_scores(pkg, heads):
     """Scores far apart (the running maximum moves late in the row), q beyond
-    f16's range, a scale of zero and a negative one."""
+    f16's range, a scale of zero and a negative one; 16 and 128 columns."""
     import torch
     kv, rows = [700], [4]
-    s = Setup(pkg, 4, 1, 128, 64, [704], rope=False, seed=12)
+    s = Setup(pkg, heads, 1, 128, 64, [704], rope=False, seed=12)
     k, kn = s.rows(704, 1, "f32")
     v, vn = s.rows(704, 1, "f32")
     grow = torch.linspace(0.1, 6.0, 704)[:, None, None]
@@ -334,7 +337,7 @@ def test_attend_peaked_and_large_scores(pkg):
     for i in range(704):
         s.store(0, i, k32[i], vn[i])
     s.batch.plan(kv, rows, s.table)
-    q, _ = s.rows(4, 4, "bf16", 3.0)
+    q, _ = s.rows(4, heads, "bf16", 3.0)
     for scale in (None, 0.0, -0.05):
         check_attend(s, kv, rows, q, s.batch.attend(0, q, scale=scale), None, "bf16", scale)
     big = q * 1e6
@@ -372,6 +375,102 @@ def test_attend_strides_and_streams(pkg):
     assert np.array_equal(s.device_pool(), s.host)
     check_attend(s, kv, rows, turned, wide[:, :, 3:67], None, "bf16")
     assert (wide[:, :, :3] == 0).all() and (wide[:, :, 67:] == 0).all()
+
+
+# Batches whose every sequence has over 48 columns (rows x query heads of a KV
+# head): these run on the tensor-core kernel for many columns.
+WIDE = [
+    # heads, kv heads, d, page, kv lengths, rows, trees
+    (8, 1, 128, 64, [0], [65], False),
+    (8, 1, 64, 16, [131], [70], False),
+    (14, 2, 64, 32, [50], [33], False),
+    (32, 1, 128, 128, [1000], [9], False),
+    (4, 1, 128, 16, [5], [300], False),
+    (8, 2, 128, 32, [700, 3], [20, 64], False),
+    (7, 1, 64, 128, [126, 0, 300], [19, 8, 40], False),
+    (8, 1, 128, 64, [200], [60], True),
+    (28, 4, 128, 16, [90], [31], True),
+    (16, 2, 64, 32, [0, 63], [64, 50], True),
+    (8, 1, 128, 64, [3000], [20], False),  # one tile split over many blocks and joined
+    (8, 1, 64, 64, [2500], [33], True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(WIDE)))
+@pytest.mark.parametrize("q_type,out_type,pad", [("bf16", "bf16", 0), ("f16", "f32", 0), ("bf16", "f16", 3)])
+def test_attend_many_columns(pkg, case, q_type, out_type, pad):
+    import torch
+    heads, kv_heads, d, page, kv, rows, trees = WIDE[case]
+    s = Setup(pkg, heads, kv_heads, d, page, [a + b for a, b in zip(kv, rows)], seed=100 + case)
+    s.fill([a + b for a, b in zip(kv, rows)])
+    masks = [m for n in rows for m in random_masks(s.rng, n)] if trees else None
+    q, _ = s.rows(sum(rows), heads, q_type, 1.5, pad=pad)
+    s.batch.plan(kv, rows, s.table, masks=masks)
+    out = torch.full((sum(rows), heads, d + pad), float("nan"), dtype=dtype_of(out_type), device="cuda")[:, :, :d]
+    s.batch.attend(0, q, out=out)
+    s.batch.status()
+    check_attend(s, kv, rows, q, out, masks, out_type)
+    again = torch.empty(sum(rows), heads, d, dtype=dtype_of(out_type), device="cuda")
+    assert torch.equal(s.batch.attend(0, q, out=again), out)
+
+
+def test_attend_few_and_many_columns_in_one_batch(pkg):
+    """A prompt chunk beside decoding sequences: both kernels in one call, the
+    partial states of the one after those of the other."""
+    kv, rows = [1500, 900, 40, 2200], [1, 200, 1, 2]
+    s = Setup(pkg, 16, 2, 128, 64, [a + b for a, b in zip(kv, rows)], seed=77)
+    s.fill([a + b for a, b in zip(kv, rows)])
+    q, _ = s.rows(sum(rows), 16, "bf16", 1.5)
+    s.batch.plan(kv, rows, s.table)
+    for _ in range(2):
+        out = s.batch.attend(0, q)
+        s.batch.status()
+        check_attend(s, kv, rows, q, out, None, "bf16")
+
+
+def test_append_many_rows_and_heads_off_the_block_size(pkg):
+    """300 rows (a block a row) of head counts that leave threads idle."""
+    import torch
+    s = Setup(pkg, 9, 3, 64, 32, [310], half=False, seed=50)
+    q, qn = s.rows(300, 9, "f16")
+    k, kn = s.rows(300, 3, "f16", 2.0)
+    v, vn = s.rows(300, 3, "f16")
+    s.batch.plan([10], [300], s.table)
+    q_out = s.batch.append(0, q, k, v)
+    for i in range(300):
+        s.store(0, 10 + i, s.turned(kn[i], 10 + i), vn[i])
+        assert torch.equal(q_out[i].cpu(), torch.from_numpy(s.turned(qn[i], 10 + i)).half()), i
+    assert np.array_equal(s.device_pool(), s.host)
+
+
+def test_calls_under_graph_capture(pkg):
+    """append and attend captured after a plan, and replayed on new rows."""
+    import torch
+    s = Setup(pkg, 4, 2, 128, 32, [40], seed=60)
+    s.fill([33])
+    q, _ = s.rows(2, 4, "bf16")
+    k, _ = s.rows(2, 2, "bf16", 2.0)
+    v, _ = s.rows(2, 2, "bf16")
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    turned, out = torch.empty_like(q), torch.empty_like(q)
+    s.batch.plan([33], [2], s.table)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        s.batch.append(0, q, k, v, q_out=turned)
+        s.batch.attend(0, turned, out=out)
+    with pytest.raises(pkg.UnsupportedMethodError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            s.batch.plan([33], [2], s.table)
+    for _ in range(2):
+        for t in (q, k, v):
+            t.copy_(torch.randn_like(t))
+        g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            s.store(0, 33 + i, s.turned(k[i].float().cpu().numpy(), 33 + i), v[i].float().cpu().numpy())
+        assert np.array_equal(s.device_pool(), s.host)
+        check_attend(s, [33], [2], turned, out, None, "bf16")
 
 
 def test_long_context_split_over_many_blocks(pkg):
@@ -474,3 +573,15 @@ def test_batch_outlives_its_cache_handle(pkg):
     q, _ = s.rows(1, 4, "bf16")
     s.batch.plan([19], [1], s.table)
     check_attend(s, [19], [1], q, s.batch.attend(0, q), None, "bf16")
+
+
+def test_tree_decoding_example(pkg):
+    """Draft trees over the paged cache commit the tokens of a token a step, in fewer steps."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "kv4_tree_decoding.py")
+    spec = importlib.util.spec_from_file_location("kv4_tree_decoding", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    same, steps, tokens = mod.run()
+    assert same and tokens > 1.3 * steps
