@@ -84,9 +84,12 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
   constexpr int SLOTS = kThreads / TPH;  // heads in flight
   const int l = threadIdx.x % TPH, slot = threadIdx.x / TPH;
   const int row = blockIdx.x;
-  const RowDev rd = p.rows[row];
+  pdl_launch_dependents();
+  const RowDev rd = p.rows[row];  // the plan is older than any kernel this one may overlap
   const int nq = p.q.ptr ? (p.n_heads + SLOTS - 1) / SLOTS : 0, nk = (p.n_kv + SLOTS - 1) / SLOTS;
   const bool rotate = p.cos != nullptr;
+
+  pdl_wait();
 
   // This thread's 8 channels of the rotation: cos / sin of pair index
   // c mod D/2 (rotate-half, sin negated in the first half) or c / 2
@@ -208,15 +211,15 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
 }
 
 template <int D>
-void launch(const AppendParams& p, int parts, cudaStream_t s) {
+cudaError_t launch(const AppendParams& p, int parts, cudaStream_t s) {
   const dim3 grid(p.n_rows, parts);
   // One instantiation a type for rows of 16-byte pieces, as projections leave
   // them; mixed types and odd strides take the general one.
   const bool same = (!p.q.ptr || p.q.dtype == p.k.dtype) && p.v.dtype == p.k.dtype && p.wide_q && p.wide_k && p.wide_v;
-  if (!same) append_kernel<D, -1><<<grid, kThreads, 0, s>>>(p);
-  else if (p.k.dtype == T_BF16) append_kernel<D, T_BF16><<<grid, kThreads, 0, s>>>(p);
-  else if (p.k.dtype == T_F16) append_kernel<D, T_F16><<<grid, kThreads, 0, s>>>(p);
-  else append_kernel<D, T_F32><<<grid, kThreads, 0, s>>>(p);
+  if (!same) return launch_overlapping(append_kernel<D, -1>, grid, kThreads, 0, s, p);
+  if (p.k.dtype == T_BF16) return launch_overlapping(append_kernel<D, T_BF16>, grid, kThreads, 0, s, p);
+  if (p.k.dtype == T_F16) return launch_overlapping(append_kernel<D, T_F16>, grid, kThreads, 0, s, p);
+  return launch_overlapping(append_kernel<D, T_F32>, grid, kThreads, 0, s, p);
 }
 
 }  // namespace
@@ -229,9 +232,7 @@ cudaError_t launch_append(const AppendParams& p, int head_dim, cudaStream_t s) {
   // of 48 heads: 2.4 us against 3.4).  Many: a block a row, which loads the
   // rotation once and reads ahead (1024 rows: 6.9 us against 10.2; equal at 256).
   const int parts = p.n_rows >= 256 ? 1 : most;
-  if (head_dim == 128) launch<128>(p, parts, s);
-  else launch<64>(p, parts, s);
-  return cudaGetLastError();
+  return head_dim == 128 ? launch<128>(p, parts, s) : launch<64>(p, parts, s);
 }
 
 }  // namespace kv4

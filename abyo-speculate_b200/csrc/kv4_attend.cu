@@ -338,12 +338,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
     fence_mbar_init();
   }
   __syncwarp();
-  Unit u = p.units[blockIdx.x];
+  pdl_launch_dependents();
+  Unit u = p.units[blockIdx.x];  // the plan is older than any kernel this one may overlap
   Cursor cur;
   cur.ui = blockIdx.x;
   cur.next = u.next;
   cur.last = u.last;
   cur.at_unit(p, warp);
+  pdl_wait();
 #pragma unroll 1
   for (int i = 0; i < Sh::STAGES && cur.more(); ++i) {
     if (lane == 0) copy_tile<D>(p, cur, ring + i * Sh::TILE, &full[i]);
@@ -703,8 +705,7 @@ int smem_bytes() {
 
 template <int D, int NT>
 cudaError_t launch(const AttendParams& p, cudaStream_t s) {
-  attend_kernel<D, NT><<<p.n_ctas, kThreads, smem_bytes<D, NT>(), s>>>(p);
-  return cudaGetLastError();
+  return launch_overlapping(attend_kernel<D, NT>, dim3(p.n_ctas), kThreads, smem_bytes<D, NT>(), s, p);
 }
 template <int D, int NT>
 cudaError_t allow() {

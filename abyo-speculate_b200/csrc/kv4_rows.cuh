@@ -78,5 +78,23 @@ SPEC_DEV void store8(const Rows& r, long long at, bool wide, const float (&x)[8]
   }
 }
 
+// Launches a kernel that may start while the kernel before it on the stream
+// still runs: it reads nothing but the plan, and writes nothing, before its
+// griddepcontrol.wait.
+template <class K, class P>
+cudaError_t launch_overlapping(K* kernel, dim3 grid, int threads, int smem, cudaStream_t s, const P& p) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 }  // namespace kv4
 }  // namespace specb200

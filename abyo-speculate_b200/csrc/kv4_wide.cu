@@ -636,6 +636,8 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
 template <int D>
 __global__ void __launch_bounds__(kWideCols) wide_join_kernel(const __grid_constant__ AttendParams p) {
   constexpr int PART = (D + 2) * kWideCols;
+  pdl_launch_dependents();
+  pdl_wait();
   const Unit& u = p.joins[blockIdx.x];
   const int col = threadIdx.x, c = blockIdx.y, n = u.n_parts, G = p.n_heads / p.n_kv;
   if (col >= u.n_cols) return;
@@ -686,6 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = mt->tmem;
+  pdl_wait();
   if (warp < kUnpackK) {
     softmax_role<D>(p, smem, mt, tmem, warp / 8, warp / 4 % 2);
   } else if (warp < kUnpackV) {
@@ -718,14 +721,14 @@ size_t wide_part_floats(int head_dim) { return (size_t)(head_dim + 2) * kWideCol
 
 cudaError_t launch_wide(const AttendParams& p, int head_dim, cudaStream_t s) {
   if (p.n_ctas <= 0) return cudaSuccess;
-  if (head_dim == 128) wide_kernel<128><<<p.n_ctas, kThreads, smem_bytes<128>(), s>>>(p);
-  else wide_kernel<64><<<p.n_ctas, kThreads, smem_bytes<64>(), s>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      head_dim == 128
+          ? launch_overlapping(wide_kernel<128>, dim3(p.n_ctas), kThreads, smem_bytes<128>(), s, p)
+          : launch_overlapping(wide_kernel<64>, dim3(p.n_ctas), kThreads, smem_bytes<64>(), s, p);
   if (e != cudaSuccess || !p.n_joins) return e;
   const dim3 grid(p.n_joins, head_dim / 8);
-  if (head_dim == 128) wide_join_kernel<128><<<grid, kWideCols, 0, s>>>(p);
-  else wide_join_kernel<64><<<grid, kWideCols, 0, s>>>(p);
-  return cudaGetLastError();
+  return head_dim == 128 ? launch_overlapping(wide_join_kernel<128>, grid, kWideCols, 0, s, p)
+                         : launch_overlapping(wide_join_kernel<64>, grid, kWideCols, 0, s, p);
 }
 
 }  // namespace kv4

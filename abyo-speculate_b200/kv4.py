@@ -24,7 +24,8 @@ import numpy as np
 from . import _lib
 
 
-_ROWS = struct.Struct("=Qqqqii")  # spec_kv4_rows
+_TWO_ROWS, _SIX_ROWS = struct.Struct("=" + "Qqqqii" * 2), struct.Struct("=" + "Qqqqii" * 6)  # spec_kv4_rows
+_NONE = (0,) * 6
 
 
 def _invalid(msg: str) -> _lib.SamplingError:
@@ -136,12 +137,12 @@ class KV4Batch:
         self._h = h
         self.n_rows = 0
         self._types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-        # One buffer of spec_kv4_rows structures: a call packs its tensors into
-        # the first slots (a few hundred ns each, where a call is microseconds).
+        # One buffer of spec_kv4_rows structures, packed at once (the host's part
+        # of a call takes longer than a small one's kernel).
         size = ctypes.sizeof(_lib.KV4Rows)
         self._buf = ctypes.create_string_buffer(6 * size)
-        at = ctypes.addressof(self._buf)
-        self._slots = [(i * size, at + i * size) for i in range(6)]
+        self._at = [ctypes.addressof(self._buf) + i * size for i in range(6)]
+        self._dim = cache.head_dim
         self._index = cache.device.index
         self._scale = cache.head_dim ** -0.5
         # The raw handle of torch's current stream, without a Stream object around it.
@@ -179,10 +180,10 @@ class KV4Batch:
     def _stream(self) -> int:
         return self._torch.cuda.current_stream(self._index).cuda_stream
 
-    def _rows(self, i: int, t, heads: int, what: str):
-        """Packs tensor t [rows, heads, head_dim] into slot i; returns the slot's address."""
+    def _rows(self, t, heads: int, what: str):
+        """The fields of spec_kv4_rows for tensor t [rows, heads, head_dim]."""
         if t is None:
-            return None
+            return _NONE
         try:
             n, h, d = t.shape
             row, head, ch = t.stride()
@@ -191,15 +192,13 @@ class KV4Batch:
             h = d = ch = None
         except KeyError:
             raise _invalid(f"{what} is {t.dtype}: bfloat16, float16 and float32 are taken") from None
-        if h != heads or d != self.cache.head_dim:
-            raise _invalid(f"{what} has shape {tuple(t.shape)}, [rows, {heads}, {self.cache.head_dim}] is needed")
+        if h != heads or d != self._dim:
+            raise _invalid(f"{what} has shape {tuple(t.shape)}, [rows, {heads}, {self._dim}] is needed")
         if ch != 1:
             raise _invalid(f"the channels of {what} are not contiguous")
         if t.get_device() != self._index:
             raise _invalid(f"{what} is on {t.device}, the pool on {self.cache.device}")
-        off, ref = self._slots[i]
-        _ROWS.pack_into(self._buf, off, t.data_ptr(), row, head, n, kind, 0)
-        return ref
+        return t.data_ptr(), row, head, n, kind, 0
 
     def append(self, layer: int, q, k, v, q_out=None, k_out=None, v_out=None):
         """Stores the plan's rows of k and v in `layer`'s pages, k rotated, and
@@ -209,11 +208,13 @@ class KV4Batch:
         c = self.cache
         if q is not None and q_out is None:
             q_out = self._torch.empty((self.n_rows, c.n_heads, c.head_dim), dtype=q.dtype, device=c.device)
-        rows = self._rows
-        rc = self._lib.spec_kv4_append(
-            self._h, layer, rows(0, q, c.n_heads, "q"), rows(1, q_out, c.n_heads, "q_out"),
-            rows(2, k, c.n_kv_heads, "k"), rows(3, v, c.n_kv_heads, "v"), rows(4, k_out, c.n_kv_heads, "k_out"),
-            rows(5, v_out, c.n_kv_heads, "v_out"), self._stream())
+        rows, nq, nk, at = self._rows, c.n_heads, c.n_kv_heads, self._at
+        _SIX_ROWS.pack_into(self._buf, 0, *rows(q, nq, "q"), *rows(q_out, nq, "q_out"), *rows(k, nk, "k"),
+                            *rows(v, nk, "v"), *rows(k_out, nk, "k_out"), *rows(v_out, nk, "v_out"))
+        rc = self._lib.spec_kv4_append(self._h, layer, at[0] if q is not None else None,
+                                       at[1] if q_out is not None else None, at[2] if k is not None else None,
+                                       at[3] if v is not None else None, at[4] if k_out is not None else None,
+                                       at[5] if v_out is not None else None, self._stream())
         if rc:
             _lib.check(rc)
         return q_out
@@ -225,8 +226,8 @@ class KV4Batch:
         c = self.cache
         if out is None:
             out = self._torch.empty((self.n_rows, c.n_heads, c.head_dim), dtype=q.dtype, device=c.device)
-        rc = self._lib.spec_kv4_attend(self._h, layer, self._rows(0, q, c.n_heads, "q"),
-                                       self._rows(1, out, c.n_heads, "out"),
+        _TWO_ROWS.pack_into(self._buf, 0, *self._rows(q, c.n_heads, "q"), *self._rows(out, c.n_heads, "out"))
+        rc = self._lib.spec_kv4_attend(self._h, layer, self._at[0], self._at[1],
                                        self._scale if scale is None else scale, self._stream())
         if rc:
             _lib.check(rc)
