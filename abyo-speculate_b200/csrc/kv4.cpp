@@ -4,6 +4,7 @@
 // on pages and slots.
 #include <limits.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <memory>
@@ -103,6 +104,7 @@ struct spec_kv4_batch {
   // arrival counters (zero between calls) and partial states.
   Schedule narrow, wide;
   int sms = 0;
+  int wide_from = -1;  // columns; -1: by estimate
   int* arrived = nullptr;
   size_t arrived_cap = 0;
   float* parts = nullptr;
@@ -241,40 +243,61 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 // 153 at 3, 157 at 6).
 constexpr int kUnitCost = 2;
 
-// Whether the sequences of more than kWideFrom columns go to the wide kernel:
-// the smaller of two estimates in us, from measurements of both on a B200.  A
-// CTA's stage takes 2.7 us in the narrow kernel (at most 32 columns a unit,
-// two to four CTAs an SM) and 2.5 in the wide one (256 columns, one an SM); a
-// narrow call of more than 8 columns costs 20 besides, others 8, a wide one 15
-// and 10 to join states.  (Measured, narrow against wide: 32 sequences of 4096
-// tokens, 48 columns 135 / 146, 64 columns 175 / 146, 128 columns 324 / 146;
-// one sequence, 128 columns at 2048 27 / 22, 256 at 512 25 / 21; eight short
-// trees of 7 to 217 columns 20 / 33, as the wide call comes on top.)
-constexpr int kWideFrom = 48;
-bool use_wide(const spec_kv4_batch* b, const spec_kv4_step* s) {
+// Columns of the narrow kernel's tiles of a sequence: of equal size, a multiple
+// of 8, at most kMaxCols.
+int narrow_tile(int64_t cols) {
+  const int64_t tiles = (cols + kMaxCols - 1) / kMaxCols;
+  return tiles ? (int)(((cols + tiles - 1) / tiles + 7) / 8 * 8) : 0;
+}
+
+// Expected time (us) of the step's attention when sequences of more than
+// wide_from columns go to the wide kernel; fitted to both on a B200, head size
+// 128 (measured / expected for one and for 32 sequences: narrow, 24 columns at
+// 4096 tokens 83 / 83, 48 151 / 150, 64 184 / 184; wide, 64 columns 142 / 143,
+// 256 185 / 186; one sequence of 2048 tokens and 64 columns, narrow 20 / 23,
+// wide 27 / 26).  A round is a 128-token stage in every resident CTA.
+double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from) {
+  static const double kCall[5] = {0, 8, 9, 16, 21}, kRound[5] = {0, 2.5, 2.6, 2.35, 2.86};  // narrow, by 8-column tiles
   const Cache& c = *b->c;
   const int G = c.d.n_heads / c.d.n_kv_heads;
-  int64_t few = 0, many = 0, wide = 0;  // stages: narrow of each class, wide
-  int most_few = 0;                     // columns of a narrow unit without the many
+  double narrow = 0, wide = 0, slowest = 0;
+  int64_t tiles = 0;
+  int nt = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int64_t cols = (int64_t)s->n_rows[q] * G, st = (s->kv_len[q] + s->n_rows[q] + kStageTokens - 1) / kStageTokens;
-    if (cols > kWideFrom) {
-      many += (cols + kMaxCols - 1) / kMaxCols * st;
-      wide += (cols + kWideCols - 1) / kWideCols * st;
+    if (!cols) continue;
+    if (cols > wide_from) {
+      const int64_t n = (cols + kWideCols - 1) / kWideCols;
+      const double round = cols <= kWideCols / 2 ? 2.25 : 3.0;
+      wide += (double)(n * st * c.d.n_kv_heads) * round;
+      if (round > slowest) slowest = round;
+      tiles += n * c.d.n_kv_heads;
     } else {
-      few += (cols + kMaxCols - 1) / kMaxCols * st;
-      if (cols > most_few) most_few = cols < kMaxCols ? (int)cols : kMaxCols;
+      const int size = narrow_tile(cols);
+      narrow += (double)((cols + size - 1) / size * st * c.d.n_kv_heads);
+      if (size / 8 > nt) nt = size / 8;
     }
   }
-  if (!wide) return false;
-  const auto narrow_us = [&](int64_t stages, int cols) {
-    if (!stages) return 0.0;
-    const int64_t slots = (int64_t)b->sms * attend_ctas_per_sm((cols + 7) / 8);
-    return (cols > 8 ? 20.0 : 8.0) + 2.7 * ((stages * c.d.n_kv_heads + slots - 1) / slots);
-  };
-  const int64_t n = (wide * c.d.n_kv_heads + b->sms - 1) / b->sms;
-  const double split = 15.0 + 2.5 * n + (wide * c.d.n_kv_heads > b->sms / 2 ? 10.0 : 0.0) + narrow_us(few, most_few);
-  return split < narrow_us(few + many, kMaxCols);
+  double us = 0;
+  if (nt) us += kCall[nt] + kRound[nt] * narrow / ((double)b->sms * attend_ctas_per_sm(nt));
+  if (tiles) {
+    const double parts = (double)b->sms / (double)tiles;  // a tile's, to be joined
+    us += 14 + (wide / b->sms > slowest ? wide / b->sms : slowest) + 0.55 * (parts < 1 ? 0 : parts > 18 ? 18 : parts);
+  }
+  return us;
+}
+
+// From how many columns a sequence goes to the wide kernel: the best of a few,
+// or what SPEC_B200_KV4_WIDE_FROM said when the batch was made.
+int choose_wide_from(const spec_kv4_batch* b, const spec_kv4_step* s) {
+  if (b->wide_from >= 0) return b->wide_from;
+  int best = INT_MAX;
+  double least = attend_us(b, s, best);
+  for (const int from : {kMaxCols, 64, 128}) {
+    const double us = attend_us(b, s, from);
+    if (us < least) least = us, best = from;
+  }
+  return best;
 }
 
 // Cuts the step's attention into units: per (sequence, kv head, tile of
@@ -285,7 +308,6 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_fro
   const Cache& c = *b->c;
   Schedule& out = wide ? b->wide : b->narrow;
   const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
-  const int most = wide ? kWideCols : kMaxCols;
   b->tiles.clear();
   b->runs.clear();
   b->joins.clear();
@@ -297,9 +319,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_fro
   int row0 = 0, table = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int n = s->kv_len[q], m = s->n_rows[q], cols = m * G;
-    const int tiles = (cols + most - 1) / most;
-    // Narrow tiles are of equal size, wide ones full but for the last.
-    const int size = wide ? most : tiles ? ((cols + tiles - 1) / tiles + 7) / 8 * 8 : 0;
+    const int size = wide ? kWideCols : narrow_tile(cols);
     for (int h = 0; h < c.d.n_kv_heads && (cols > wide_from) == wide; ++h)
       for (int c0 = 0; c0 < cols; c0 += size) {
         Unit u{};
@@ -473,7 +493,7 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   if (!s->src_rows) max_src = (int)rows - 1;
 
   b->planned = false;
-  const int wide_from = use_wide(b, s) ? kWideFrom : INT_MAX;
+  const int wide_from = choose_wide_from(b, s);
   schedule(b, s, false, wide_from);
   schedule(b, s, true, wide_from);
   // One block: rows, masks, pages, units.
@@ -597,6 +617,7 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   spec_kv4_batch* b = new (std::nothrow) spec_kv4_batch;
   if (!b) return fail(SPEC_ERR_OOM, "spec_kv4_batch_create: out of host memory");
   b->c = c->c;
+  if (const char* v = getenv("SPEC_B200_KV4_WIDE_FROM")) b->wide_from = atoi(v);
   cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);

@@ -543,7 +543,11 @@ int spec_kv4_create(const spec_kv4_desc* d, void* pool_dev, int64_t pool_bytes, 
                     const float* sin_dev, int n_positions, spec_kv4** out);
 void spec_kv4_free(spec_kv4* c);
 /* A batch handle: the plan of one step at a time and the attention's
- * workspace.  One thread uses it at a time; it may outlive `c`'s handle. */
+ * workspace.  One thread uses it at a time; it may outlive `c`'s handle.  The
+ * attention has a kernel for few (row, query head) columns a sequence and one
+ * for many, chosen per plan by an estimate of their times; the environment
+ * variable SPEC_B200_KV4_WIDE_FROM=<columns>, read here, sends every sequence
+ * of more columns to the latter instead. */
 int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out);
 void spec_kv4_batch_free(spec_kv4_batch* b);
 /* One step over n_seqs sequences (host arrays, copied before the call

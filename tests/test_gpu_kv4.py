@@ -214,6 +214,14 @@ def test_append_extreme_rows(pkg):
                 assert (np.abs(xs - vs) <= bound).all(), (i, h, g)
 
 
+def wide_from(monkeypatch, columns):
+    """Sends sequences of more columns to the kernel for many (None: the plan's estimate decides)."""
+    if columns is None:
+        monkeypatch.delenv("SPEC_B200_KV4_WIDE_FROM", raising=False)
+    else:
+        monkeypatch.setenv("SPEC_B200_KV4_WIDE_FROM", str(columns))
+
+
 CASES = [
     # heads, kv heads, d, page, kv lengths, rows
     (4, 2, 128, 64, [0, 1, 63, 64, 129], [1, 1, 1, 1, 1]),
@@ -228,9 +236,11 @@ CASES = [
 
 
 @pytest.mark.parametrize("case", range(len(CASES)))
-@pytest.mark.parametrize("q_type,out_type", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32")])
-def test_attend_causal(pkg, case, q_type, out_type):
+@pytest.mark.parametrize("q_type,out_type,columns", [("bf16", "bf16", None), ("f16", "f16", None), ("bf16", "f32", None),
+                                                     ("bf16", "bf16", 0)])
+def test_attend_causal(pkg, monkeypatch, case, q_type, out_type, columns):
     import torch
+    wide_from(monkeypatch, columns)
     heads, kv_heads, d, page, kv, rows = CASES[case]
     s = Setup(pkg, heads, kv_heads, d, page, [a + b for a, b in zip(kv, rows)], layers=2, layer=1, seed=10 + case)
     s.fill([a + b for a, b in zip(kv, rows)])
@@ -279,8 +289,9 @@ def test_attend_trees(pkg, d, heads, kv_heads, page):
     check_attend(s, kv, rows, q, out, masks, "f16")
 
 
-@pytest.mark.parametrize("heads", [4, 64])
-def test_attend_rows_that_see_nothing_give_zeros(pkg, heads):
+@pytest.mark.parametrize("heads,columns", [(4, None), (64, None), (4, 0), (64, 0)])
+def test_attend_rows_that_see_nothing_give_zeros(pkg, monkeypatch, heads, columns):
+    wide_from(monkeypatch, columns)
     kv, rows = [0, 12], [5, 3]
     s = Setup(pkg, heads, 2, 128, 16, [5, 15], seed=8)
     s.fill([5, 15])
@@ -292,12 +303,13 @@ def test_attend_rows_that_see_nothing_give_zeros(pkg, heads):
     assert (out[0] == 0).all() and (out[2] == 0).all() and not (out[5] == 0).all()
 
 
-@pytest.mark.parametrize("heads", [4, 32])
-def test_attend_nan_stays_where_it_is_seen(pkg, heads):
+@pytest.mark.parametrize("heads,columns", [(4, None), (32, None), (4, 0), (32, 0)])
+def test_attend_nan_stays_where_it_is_seen(pkg, monkeypatch, heads, columns):
     """A NaN key row, and a NaN value row, of a draft node reach the rows that
     see the node and no other; the unwritten bytes of a page read as NaN and
     reach none.  12 and 96 columns."""
     import torch
+    wide_from(monkeypatch, columns)
     kv, rows = [9], [6]
     s = Setup(pkg, heads, 2, 128, 16, [15], rope=False, seed=9)
     s.fill([9])
@@ -320,11 +332,12 @@ def test_attend_nan_stays_where_it_is_seen(pkg, heads):
     assert (bad == want).all()
 
 
-@pytest.mark.parametrize("heads", [4, 32])
-def test_attend_peaked_and_large_scores(pkg, heads):
+@pytest.mark.parametrize("heads,columns", [(4, None), (32, None), (4, 0), (32, 0)])
+def test_attend_peaked_and_large_scores(pkg, monkeypatch, heads, columns):
     """Scores far apart (the running maximum moves late in the row), q beyond
     f16's range, a scale of zero and a negative one; 16 and 128 columns."""
     import torch
+    wide_from(monkeypatch, columns)
     kv, rows = [700], [4]
     s = Setup(pkg, heads, 1, 128, 64, [704], rope=False, seed=12)
     k, kn = s.rows(704, 1, "f32")
@@ -377,8 +390,8 @@ def test_attend_strides_and_streams(pkg):
     assert (wide[:, :, :3] == 0).all() and (wide[:, :, 67:] == 0).all()
 
 
-# Batches whose every sequence has over 48 columns (rows x query heads of a KV
-# head): these run on the tensor-core kernel for many columns.
+# Sequences of many columns (rows x query heads of a KV head), on the kernel the
+# plan estimates to be faster and on the one for many columns.
 WIDE = [
     # heads, kv heads, d, page, kv lengths, rows, trees
     (8, 1, 128, 64, [0], [65], False),
@@ -397,9 +410,11 @@ WIDE = [
 
 
 @pytest.mark.parametrize("case", range(len(WIDE)))
-@pytest.mark.parametrize("q_type,out_type,pad", [("bf16", "bf16", 0), ("f16", "f32", 0), ("bf16", "f16", 3)])
-def test_attend_many_columns(pkg, case, q_type, out_type, pad):
+@pytest.mark.parametrize("q_type,out_type,pad,columns", [("bf16", "bf16", 0, 0), ("f16", "f32", 0, 0),
+                                                         ("bf16", "f16", 3, 0), ("bf16", "bf16", 0, None)])
+def test_attend_many_columns(pkg, monkeypatch, case, q_type, out_type, pad, columns):
     import torch
+    wide_from(monkeypatch, columns)
     heads, kv_heads, d, page, kv, rows, trees = WIDE[case]
     s = Setup(pkg, heads, kv_heads, d, page, [a + b for a, b in zip(kv, rows)], seed=100 + case)
     s.fill([a + b for a, b in zip(kv, rows)])
@@ -414,9 +429,10 @@ def test_attend_many_columns(pkg, case, q_type, out_type, pad):
     assert torch.equal(s.batch.attend(0, q, out=again), out)
 
 
-def test_attend_few_and_many_columns_in_one_batch(pkg):
+def test_attend_few_and_many_columns_in_one_batch(pkg, monkeypatch):
     """A prompt chunk beside decoding sequences: both kernels in one call, the
     partial states of the one after those of the other."""
+    wide_from(monkeypatch, 64)
     kv, rows = [1500, 900, 40, 2200], [1, 200, 1, 2]
     s = Setup(pkg, 16, 2, 128, 64, [a + b for a, b in zip(kv, rows)], seed=77)
     s.fill([a + b for a, b in zip(kv, rows)])
