@@ -643,9 +643,10 @@ __global__ void __launch_bounds__(kWideCols) wide_join_kernel(const __grid_const
   if (col >= u.n_cols) return;
   const float* s = p.parts + (long long)u.part0 * PART + col;
   float m = kNone;
+#pragma unroll 8
   for (int i = 0; i < n; ++i) m = fmaxf(m, s[(long long)i * PART + D * kWideCols]);
   float l = 0.f, x[8] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
     const float* q = s + (long long)i * PART;
     const float w = ex2(q[D * kWideCols] - m);
