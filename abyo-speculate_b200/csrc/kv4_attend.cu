@@ -27,6 +27,13 @@
 // head, column tile) that several CTAs share is joined by the last arriver of
 // every kFanIn of them, level by level and in order, so a plan's results do
 // not depend on timing.
+//
+// Bound by the integer pipe (55 %) and instruction issue (61 %) together: about
+// 630 warp instructions per 32 tokens of a head of 128 and 8 columns, a third of
+// them V's unpacking, and 160 more per 8 columns.  One row each of 64 sequences
+// of 500 to 16000 tokens, 32 query heads on 8 kv heads: 149 us, 4.4 TB/s of the
+// cache's bytes; one of 131072 tokens 50 us; one of 2048 tokens 8.9 us, of
+// which launch and one stage are 3.9 and a round of joins 2 to 4.
 #include "common.cuh"
 #include "kv4.h"
 #include "kv4_rows.cuh"
@@ -39,6 +46,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;  // tokens of one ring slot
+
 SPEC_DEV uint32_t movmatrix(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -458,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attend_kernel(const
       }
       // Both 16-token halves at once: one at a time fetches half the code but
       // leaves the chains of the few resident warps too short (24 sequences of
-      // 9 rows and 7 query heads: 94 us against 130).
+      // 9 rows and 7 query heads, on this kernel: 94 us against 130).
       constexpr int H = 2;
 #pragma unroll 1
       for (int h0 = 0; h0 < 2; h0 += H) {
