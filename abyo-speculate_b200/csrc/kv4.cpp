@@ -105,6 +105,8 @@ struct spec_kv4_batch {
   Schedule narrow, wide;
   int sms = 0;
   int wide_from = -1;  // columns; -1: by estimate
+  int wide_pair = -1;  // units in pairs of stages: 0, 1; -1: by estimate
+  bool pair = false;   // and the plan's choice
   int* arrived = nullptr;
   size_t arrived_cap = 0;
   float* parts = nullptr;
@@ -251,15 +253,17 @@ int narrow_tile(int64_t cols) {
 }
 
 // Expected time (us) of the step's attention when sequences of more than
-// wide_from columns go to the wide kernel; fitted to both on a B200, head size
-// 128 (measured / expected for one and for 32 sequences: narrow, 24 columns at
-// 4096 tokens 83 / 83, 48 151 / 150, 64 184 / 184; wide, 64 columns 142 / 143,
-// 256 185 / 186; one sequence of 2048 tokens and 64 columns, narrow 20 / 23,
-// wide 27 / 26).  A round is a 128-token stage in every resident CTA.
-double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from) {
+// wide_from columns go to the wide kernel, in the form `pair`; fitted to all on
+// a B200, head size 128.  Measured / expected for 32 sequences at 4096 tokens
+// and 8 kv heads: narrow, 48 columns 151 / 150, 64 184 / 184; wide, 64 columns
+// 143 / 140, in pairs 130 / 134; 256 columns 180 / 182, in pairs 252 / 251.
+// One sequence, 2048 tokens: 64 columns narrow 20 / 23, wide 24 / 26, in pairs
+// 25 / 28; 256 wide 29 / 27, in pairs 24 / 25.  A round is a 128-token stage in
+// every resident CTA.
+double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from, bool pair) {
   static const double kCall[5] = {0, 8, 9, 16, 21}, kRound[5] = {0, 2.5, 2.6, 2.35, 2.86};  // narrow, by 8-column tiles
   const Cache& c = *b->c;
-  const int G = c.d.n_heads / c.d.n_kv_heads;
+  const int G = c.d.n_heads / c.d.n_kv_heads, wide_cols = pair ? kPairCols : kWideCols;
   double narrow = 0, wide = 0, slowest = 0;
   int64_t tiles = 0;
   int nt = 0;
@@ -267,10 +271,11 @@ double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from)
     const int64_t cols = (int64_t)s->n_rows[q] * G, st = (s->kv_len[q] + s->n_rows[q] + kStageTokens - 1) / kStageTokens;
     if (!cols) continue;
     if (cols > wide_from) {
-      const int64_t n = (cols + kWideCols - 1) / kWideCols;
-      const double round = cols <= kWideCols / 2 ? 2.25 : 3.0;
+      const int64_t n = (cols + wide_cols - 1) / wide_cols;
+      const double round = pair ? 2.12 : cols <= kWideCols / 2 ? 2.25 : 3.0;
       wide += (double)(n * st * c.d.n_kv_heads) * round;
-      if (round > slowest) slowest = round;
+      if (pair) slowest = 3.0;  // a stage alone
+      else if (round > slowest) slowest = round;
       tiles += n * c.d.n_kv_heads;
     } else {
       const int size = narrow_tile(cols);
@@ -282,29 +287,34 @@ double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from)
   if (nt) us += kCall[nt] + kRound[nt] * narrow / ((double)b->sms * attend_ctas_per_sm(nt));
   if (tiles) {
     const double parts = (double)b->sms / (double)tiles;  // a tile's, to be joined
-    us += 14 + (wide / b->sms > slowest ? wide / b->sms : slowest) + 0.55 * (parts < 1 ? 0 : parts > 18 ? 18 : parts);
+    us += (pair ? 15.5 : 14) + (wide / b->sms > slowest ? wide / b->sms : slowest) +
+          0.55 * (parts < 1 ? 0 : parts > 18 ? 18 : parts);
   }
   return us;
 }
 
-// From how many columns a sequence goes to the wide kernel: the best of a few,
-// or what SPEC_B200_KV4_WIDE_FROM said when the batch was made.
-int choose_wide_from(const spec_kv4_batch* b, const spec_kv4_step* s) {
-  if (b->wide_from >= 0) return b->wide_from;
-  int best = INT_MAX;
-  double least = attend_us(b, s, best);
-  for (const int from : {kMaxCols, 64, 128}) {
-    const double us = attend_us(b, s, from);
-    if (us < least) least = us, best = from;
-  }
+// From how many columns a sequence goes to the wide kernel, and that one's form:
+// the best of a few, or what SPEC_B200_KV4_WIDE_FROM and SPEC_B200_KV4_WIDE_PAIR
+// said when the batch was made.
+int choose_wide_from(const spec_kv4_batch* b, const spec_kv4_step* s, bool* pair) {
+  int best = 0;
+  double least = 1e300;
+  for (const int from : {INT_MAX, 128, 64, kMaxCols})
+    for (const bool form : {false, true}) {
+      if (b->wide_pair >= 0 && form != (b->wide_pair > 0)) continue;
+      const int limit = b->wide_from >= 0 ? b->wide_from : from;
+      const double us = attend_us(b, s, limit, form);
+      if (us < least) least = us, best = limit, *pair = form;
+    }
   return best;
 }
 
 // Cuts the step's attention into units: per (sequence, kv head, tile of
 // columns) the 128-token stages its rows see, then those stages, laid end to
 // end, into runs of equal cost, one a CTA.  Sequences of more than wide_from
-// columns go to the wide kernel.
-void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_from) {
+// columns go to the wide kernel, which takes kWideCols of them a unit, or in
+// pairs of stages kPairCols.
+void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_from, bool pair) {
   const Cache& c = *b->c;
   Schedule& out = wide ? b->wide : b->narrow;
   const int G = c.d.n_heads / c.d.n_kv_heads, P = c.d.page_tokens;
@@ -319,7 +329,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_fro
   int row0 = 0, table = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int n = s->kv_len[q], m = s->n_rows[q], cols = m * G;
-    const int size = wide ? kWideCols : narrow_tile(cols);
+    const int size = !wide ? narrow_tile(cols) : pair ? kPairCols : kWideCols;
     for (int h = 0; h < c.d.n_kv_heads && (cols > wide_from) == wide; ++h)
       for (int c0 = 0; c0 < cols; c0 += size) {
         Unit u{};
@@ -493,9 +503,9 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   if (!s->src_rows) max_src = (int)rows - 1;
 
   b->planned = false;
-  const int wide_from = choose_wide_from(b, s);
-  schedule(b, s, false, wide_from);
-  schedule(b, s, true, wide_from);
+  const int wide_from = choose_wide_from(b, s, &b->pair);
+  schedule(b, s, false, wide_from, b->pair);
+  schedule(b, s, true, wide_from, b->pair);
   // One block: rows, masks, pages, units.
   const size_t at_rows = 0, at_masks = at_rows + up(sizeof(RowDev) * rows), at_table = at_masks + (s->masks ? up(8 * rows) : 0),
                at_narrow = at_table + up(4 * pages), at_wide = at_narrow + up(sizeof(Unit) * b->narrow.order.size()),
@@ -618,6 +628,7 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   if (!b) return fail(SPEC_ERR_OOM, "spec_kv4_batch_create: out of host memory");
   b->c = c->c;
   if (const char* v = getenv("SPEC_B200_KV4_WIDE_FROM")) b->wide_from = atoi(v);
+  if (const char* v = getenv("SPEC_B200_KV4_WIDE_PAIR")) b->wide_pair = atoi(v);
   cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);
@@ -751,7 +762,7 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
     p.joins = b->wide.units + b->wide.n_units;
     p.n_joins = b->wide.n_joins;
     p.n_ctas = b->wide.n_ctas;
-    e = launch_wide(p, D, st);
+    e = launch_wide(p, D, b->pair, st);
   }
   if (e == cudaSuccess && b->narrow.n_ctas) {
     p.units = b->narrow.units;

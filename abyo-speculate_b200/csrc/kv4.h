@@ -57,6 +57,7 @@ constexpr int kStageTokens = 128;  // tokens the attention's work is cut by
 constexpr int kFanIn = 16;         // partial states joined at once
 constexpr int kMaxCols = 32;       // (row, query head) columns of one unit
 constexpr int kWideCols = 256;     // of one unit of the wide kernel
+constexpr int kPairCols = 128;     // of one whose stages alternate between two accumulators
 
 // A run of stages of one (sequence, kv head, column tile), done by one CTA.
 struct alignas(16) Unit {
@@ -96,7 +97,8 @@ cudaError_t attend_setup();
 size_t attend_part_floats(int head_dim, int nt);
 int attend_ctas_per_sm(int nt);
 // The same for sequences of many columns, one CTA an SM.
-cudaError_t launch_wide(const AttendParams& p, int head_dim, cudaStream_t s);
+// pair: units have at most kPairCols columns, and their stages alternate.
+cudaError_t launch_wide(const AttendParams& p, int head_dim, bool pair, cudaStream_t s);
 cudaError_t wide_setup();
 size_t wide_part_floats(int head_dim);
 

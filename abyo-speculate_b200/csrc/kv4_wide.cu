@@ -2,18 +2,19 @@
 // chunks and draft trees, on the 5th-generation tensor cores.
 //
 // A column is a (row of the step, query head of the KV head's group).  A CTA
-// takes up to 256 of them as two tiles of 128 and walks the 128-token stages
-// of its run:
+// walks the 128-token stages of its run, either (PAIR false) for up to 256
+// columns, two tiles of 128, or (PAIR) for one tile whose stages go to two
+// accumulators in turn, which are added at the end:
 //   S [128 columns x 128 tokens] = Q K^T        tcgen05.mma, f16 from shared memory
 //   P = 2^(c S - m), rounded to f16 in place of S in tensor memory (of every
 //       32 columns of S the first 16)
 //   O [128 x D] += P V                          P from tensor memory, V^T from shared memory
 // Roles: warps 0-7 and 8-15 are the softmax of tile 0 and 1, two threads a
-// column (tokens 0-63 and 64-127 of a stage); warps 16-18 unpack K and 19-22
-// V, from page blocks that TMA bulk copies bring, into f16 operand tiles; lane
-// 0 of warp 23 issues the products.  While one tile's softmax runs, the other
-// tile's products do.  Unpacking is paid once for both tiles (1.5 instructions
-// an element and 256 columns).
+// column (tokens 0-63 and 64-127 of a stage), or of the accumulators of the one
+// tile; warps 16-18 unpack K and 19-22 V, from page blocks that TMA bulk copies
+// bring, into f16 operand tiles; warp 23 issues the products.  While the softmax
+// of one runs, the products of the other do.  Unpacking a stage is paid once for
+// both tiles (1.5 instructions an element and 256 columns), in pairs for one.
 //
 // What bounds it: a stage is 2048 cycles of tensor core and 2048 of
 // exponentials an SM, and 2300 issue slots a scheduler.  The loops are kept
@@ -23,7 +24,13 @@
 // unit idle three quarters of the time (272 us against 237).  Now 237 us: 1015
 // TFLOP/s, the tensor pipe and the exponentials busy half the time each, the
 // rest the chain of scores, exponentials and product of two tiles.  A 60-node
-// tree at 4096 tokens, 32 query heads on 8 kv heads: 31 us.
+// tree at 4096 tokens, 32 query heads on 8 kv heads: 31 us, and 26 in pairs,
+// where a CTA has half the columns to write out and twice the stages to overlap.
+// In pairs a stage serves one tile, and unpacking it (2300 cycles of K's three
+// warps, 1500 of V's four) is the longest part: 32 sequences of 64 columns at
+// 4096 tokens 143 -> 130 us, but of 256 columns 180 -> 252, so the planner
+// chooses.  V stored by tokens, unpacked like K, took 120 and 232 of these and
+// made the second product slower (2048 rows over 6144 tokens 237 -> 250 us).
 //
 // Channels and tokens along a contracted axis may come in any order that both
 // operands share, and O's columns in any order that the output undoes: K's
@@ -45,7 +52,7 @@ namespace specb200 {
 namespace kv4 {
 namespace {
 
-constexpr int kTileCols = 128;
+constexpr int kTileCols = kPairCols;
 constexpr int kThreads = 24 * 32;
 constexpr int kUnpackK = 16, kUnpackV = 19, kIssuer = 23;  // first warps of the roles
 constexpr int kThreadsK = (kUnpackV - kUnpackK) * 32;
@@ -158,22 +165,25 @@ SPEC_DEV void arrive(uint64_t* bar) {
 // Shared-memory writes of this thread become visible to the tensor core.
 SPEC_DEV void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-template <int D>
+template <int D, bool PAIR>
 struct Shape {
   static constexpr int KS = D / 16;                 // 16-channel steps of Q K^T
   static constexpr int Q_TILE = kTileCols * D * 2;  // also a K tile and a V^T tile: 128 x D f16
   static constexpr int RAW = kStageTokens * D * 5 / 8;  // a stage's K, or V, as stored
-  static constexpr int K_AT = 2 * Q_TILE, V_AT = K_AT + 2 * Q_TILE;
-  static constexpr int RAW_K_AT = V_AT + 2 * Q_TILE, RAW_V_AT = RAW_K_AT + RAW, META_AT = RAW_V_AT + RAW;
+  static constexpr int RING = PAIR ? 2 : 1;             // of those
+  static constexpr int K_AT = (PAIR ? 1 : 2) * Q_TILE, V_AT = K_AT + 2 * Q_TILE;
+  static constexpr int RAW_K_AT = V_AT + 2 * Q_TILE, RAW_V_AT = RAW_K_AT + RING * RAW;
+  static constexpr int META_AT = RAW_V_AT + RING * RAW;
   static constexpr int NC = D / 8;
 };
 
 struct Meta {
   unsigned long long q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full[2], idle;
-  unsigned long long raw_k, raw_v;
+  unsigned long long raw_k[2], raw_v[2];
   uint32_t bad[2][4];  // tokens of a V stage whose row is NaN
   uint32_t tmem;
   float red[3][2][2][kTileCols];  // between the two threads of a column: largest, sum, largest again
+  float end[2][2][kTileCols];     // PAIR: the two accumulators' m and l
 };
 
 // ---- unpacking: 96 threads for K, 128 for V --------------------------------
@@ -278,35 +288,42 @@ SPEC_DEV void put_v(const uint8_t* raw, uint8_t* dst, int P, int P_log2, int th,
   }
 }
 
-template <int D, bool VALUE>
+template <int D, bool PAIR, bool VALUE>
 SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, PAIR>;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
-  uint8_t* raw = smem + (VALUE ? Sh::RAW_V_AT : Sh::RAW_K_AT);
-  uint64_t* raw_full = bar(VALUE ? mt->raw_v : mt->raw_k);
+  uint8_t* ring = smem + (VALUE ? Sh::RAW_V_AT : Sh::RAW_K_AT);
+  unsigned long long* raw_full = VALUE ? mt->raw_v : mt->raw_k;
   unsigned long long* full = VALUE ? mt->v_full : mt->k_full;
   unsigned long long* free_ = VALUE ? mt->v_free : mt->k_free;
-  Walk w;
+  Walk w;  // the next stage to copy
   w.more = true;
   w.enter(p, blockIdx.x);
   int copies = 0;
-  if (th < 32) {
-    w.look_up(p, th);
-    copy_raw<D>(p, w, raw, raw_full, VALUE, th);
+  int st[2], sure[2], kv_end[2];  // of the stages under way
+  auto copy = [&](int at, bool ok) {
+    if (th < 32 && ok) copy_raw<D>(p, w, ring + copies % Sh::RING * Sh::RAW, bar(raw_full[copies % Sh::RING]), VALUE, th);
+    st[at] = w.st, sure[at] = w.sure, kv_end[at] = w.kv_end;
     ++copies;
+    w.step(p);
+  };
+#pragma unroll
+  for (int i = 0; i < Sh::RING; ++i) {
+    if (th < 32) w.look_up(p, th);
+    if (w.more) copy(i, true);
   }
   bool ok = true;
 #pragma unroll 1
   for (int k = 0;; ++k) {
-    const int slot = k & 1, st = w.st, sure = w.sure, kv_end = w.kv_end;
-    w.step(p);
+    const int slot = k & 1;
+    const uint8_t* raw = ring + k % Sh::RING * Sh::RAW;
     if (th < 32) w.look_up(p, th);
-    ok = ok && mbar_wait_bounded(raw_full, k & 1, p.err);
+    ok = ok && mbar_wait_bounded(bar(raw_full[k % Sh::RING]), k / Sh::RING & 1, p.err);
     if (k >= 2) ok = ok && mbar_wait_bounded(bar(free_[slot]), (k / 2 - 1) & 1, p.err);
     uint8_t* dst = smem + (VALUE ? Sh::V_AT : Sh::K_AT) + slot * Sh::Q_TILE;
     if constexpr (VALUE) {
       uint32_t live[4] = {~0u, ~0u, ~0u, ~0u};
-      if ((st + 1) * kStageTokens > sure) {
+      if ((st[0] + 1) * kStageTokens > sure[0]) {
         // Past the end V counts nothing.  A stored NaN row is NaN in every
         // scale: it is taken as zero here, and the columns that see it are told.
         const int j = th & (p.P - 1);
@@ -316,7 +333,7 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
         if ((th & 31) == 0) mt->bad[slot][th >> 5] = nans;
         asm volatile("bar.sync 4, 128;" ::: "memory");
 #pragma unroll
-        for (int q = 0; q < 4; ++q) live[q] = first32(kv_end - st * kStageTokens - 32 * q) & ~mt->bad[slot][q];
+        for (int q = 0; q < 4; ++q) live[q] = first32(kv_end[0] - st[0] * kStageTokens - 32 * q) & ~mt->bad[slot][q];
       }
       put_v<D>(raw, dst, p.P, p.P_log2, th, live);
     } else {
@@ -324,22 +341,26 @@ SPEC_DEV void unpack_role(const AttendParams& p, uint8_t* smem, Meta* mt, int th
     }
     publish_smem();
     arrive(bar(full[slot]));
-    if (!w.more) break;
-    // All its threads have read the raw stage.
-    if (VALUE) asm volatile("bar.sync 4, 128;" ::: "memory");
-    else asm volatile("bar.sync 3, %0;" ::"n"(kThreadsK) : "memory");
-    if (th < 32 && __all_sync(0xffffffffu, ok)) {
-      copy_raw<D>(p, w, raw, raw_full, VALUE, th);
-      ++copies;
+    if (k + 1 == copies && !w.more) break;
+    if constexpr (PAIR) st[0] = st[1], sure[0] = sure[1], kv_end[0] = kv_end[1];
+    if (w.more) {
+      // All its threads have read the raw stage.
+      if (VALUE) asm volatile("bar.sync 4, 128;" ::: "memory");
+      else asm volatile("bar.sync 3, %0;" ::"n"(kThreadsK) : "memory");
+      copy(Sh::RING - 1, th >= 32 || __all_sync(0xffffffffu, ok));
     }
   }
-  if (!ok && copies) mbar_wait_bounded(raw_full, (copies - 1) & 1, p.err);  // leave no copy in flight
+  // Leave no copy in flight.
+  if (!ok)
+#pragma unroll 1
+    for (int i = 1; i <= Sh::RING && i <= copies; ++i)
+      mbar_wait_bounded(bar(raw_full[(copies - i) % Sh::RING]), (copies - i) / Sh::RING & 1, p.err);
 }
 
 // ---- products: one warp -----------------------------------------------------
-template <int D>
+template <int D, bool PAIR>
 SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, PAIR>;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
   constexpr uint32_t kS = idesc_f16(kTileCols, kStageTokens), kO = idesc_f16(kTileCols, D);
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
@@ -350,7 +371,7 @@ SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_
   };
   auto scores = [&](int a, int slot, bool free_k) {
     if (elect_one()) {
-      const uint64_t qa = q0 + a * kTile16, kb = q0 + kK16 + slot * kTile16;
+      const uint64_t qa = PAIR ? q0 : q0 + a * kTile16, kb = q0 + kK16 + slot * kTile16;
       const uint32_t d = tmem + a * 128;
       mma_ss<true>(d, qa, kb, kS);
 #pragma unroll
@@ -360,30 +381,34 @@ SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_
     }
     __syncwarp();
   };
+  constexpr int kAhead = PAIR ? 2 : 1;  // stages from one of an accumulator to its next
   int k = 0;
   int waits = 0, units = 0;  // phases of p_full and q_full, a bit a tile
   Unit u = p.units[blockIdx.x];
   bool ok = true;
 #pragma unroll 1
   for (int next = __shfl_sync(0xffffffffu, u.next, 0);; ++next) {
-    const int tiles = __shfl_sync(0xffffffffu, u.n_cols, 0) > kTileCols ? 2 : 1;
     const int n = __shfl_sync(0xffffffffu, u.st1 - u.st0, 0), last = __shfl_sync(0xffffffffu, u.last, 0);
-    ok = wait(mt->k_full[k & 1], (k >> 1) & 1);
+    const int tiles = PAIR ? 1 : __shfl_sync(0xffffffffu, u.n_cols, 0) > kTileCols ? 2 : 1;
+    const int first = PAIR ? (n > 1 ? 2 : 1) : tiles;  // accumulators that begin
+    ok = true;
 #pragma unroll 1
-    for (int a = 0; a < tiles && ok; ++a) {
-      ok = wait(mt->q_full[a], units >> a & 1);
+    for (int a = 0; a < first && ok; ++a) {
+      const int at = PAIR ? k + a : k;
+      ok = wait(mt->k_full[at & 1], (at >> 1) & 1) && wait(mt->q_full[a], units >> a & 1);
       if (!ok) break;
       units ^= 1 << a;
       tc_fence_after();
-      scores(a, k & 1, a == tiles - 1);
+      scores(a, at & 1, PAIR || a == tiles - 1);
     }
 #pragma unroll 1
     for (int i = 0; i < n && ok; ++i, ++k) {
-      const int slot = k & 1, ahead = slot ^ 1;
-      const bool more = i + 1 < n;
+      const int slot = k & 1, ahead = k + kAhead;  // the stage whose scores follow
+      const bool more = i + kAhead < n;
       ok = wait(mt->v_full[slot], (k >> 1) & 1);
 #pragma unroll 1
-      for (int a = 0; a < tiles && ok; ++a) {
+      for (int t = 0; t < tiles && ok; ++t) {
+        const int a = PAIR ? i & 1 : t;
         ok = wait(mt->p_full[a], waits >> a & 1);
         if (!ok) break;
         waits ^= 1 << a;
@@ -391,18 +416,18 @@ SPEC_DEV void issue_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_
         if (elect_one()) {
           const uint64_t vb = q0 + kV16 + slot * kTile16;
           const uint32_t d = tmem + 256 + a * 128, pa = tmem + a * 128;
-          mma_ts(d, pa, vb, kO, i > 0);
+          mma_ts(d, pa, vb, kO, i >= kAhead);
 #pragma unroll
           for (int j = 1; j < kStageTokens / 16; ++j)
             mma_ts(d, pa + j / 2 * 32 + j % 2 * 8, vb + j * (D * 2), kO, 1);
           if (!more) umma_commit(bar(mt->o_full[a]));
-          if (a == tiles - 1) umma_commit(bar(mt->v_free[slot]));
+          if (t == tiles - 1) umma_commit(bar(mt->v_free[slot]));
         }
         __syncwarp();
         if (more) {
-          if (a == 0) ok = wait(mt->k_full[ahead], ((k + 1) >> 1) & 1);
+          if (t == 0) ok = wait(mt->k_full[ahead & 1], (ahead >> 1) & 1);
           if (!ok) break;
-          scores(a, ahead, a == tiles - 1);
+          scores(a, ahead & 1, t == tiles - 1);
         }
       }
     }
@@ -448,12 +473,12 @@ SPEC_DEV void hide(float (&x)[32], uint32_t seen) {
   for (int i = 0; i < 32; ++i) x[i] = (seen >> i) & 1 ? x[i] : -INFINITY;
 }
 
-template <int D>
+template <int D, bool PAIR>
 SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint32_t tmem, int a, int half) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, PAIR>;
   constexpr int NC = Sh::NC;
   auto bar = [](unsigned long long& b) { return reinterpret_cast<uint64_t*>(&b); };
-  const int th = threadIdx.x & 127, G = p.n_heads / p.n_kv, col = a * kTileCols + th;
+  const int th = threadIdx.x & 127, G = p.n_heads / p.n_kv, col = PAIR ? th : a * kTileCols + th;
   const uint32_t lane_at = (uint32_t)(th / 32 * 32) << 16;
   const uint32_t s_at = tmem + a * 128 + 64 * half + lane_at, o_at = tmem + 256 + a * 128 + lane_at;
   // A value of this thread's for the column's other one, and back.  (Between
@@ -466,12 +491,14 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
     asm volatile("bar.sync %0, 64;" ::"r"(5 + a * 4 + th / 32) : "memory");
     return mt->red[kind][a][half ^ 1][th];
   };
+  constexpr int kStep = PAIR ? 2 : 1;
   bool ok = true;
   int k = 0, v = 0, unit = 0;  // stages of this tile, of the run; units of this tile
   Unit u = p.units[blockIdx.x];
 #pragma unroll 1
   for (int next = u.next;; ++next) {
-    if (a * kTileCols < u.n_cols) {
+    const bool both = PAIR && u.st1 - u.st0 > 1;  // accumulators of this unit
+    if (a == 0 || (PAIR ? both : u.n_cols > kTileCols)) {
       const bool live = col < u.n_cols;
       const int r = u.col0 + (live ? col : 0), row = r / G, head = u.kvh * G + r % G;
       // This column's q (half of its channels a thread), in the order K's
@@ -481,7 +508,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       // their sign order as integers) is far from 1 is converted again, scaled
       // by a power of two.
       const long long at = (u.row0 + row) * p.q.row_stride + head * p.q.head_stride;
-      uint8_t* dst = smem + a * Sh::Q_TILE + (th / 8) * 256 + (th % 8) * 16;
+      uint8_t* dst = smem + (PAIR ? 0 : a * Sh::Q_TILE) + (th / 8) * 256 + (th % 8) * 16;
       const float sign = p.scale < 0.f ? -1.f : 1.f;
       uint32_t top = 0;
 #pragma unroll 1
@@ -493,7 +520,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         for (int i = 0; i < 4; ++i) {
           top = __vmaxu2(top, __vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu));
           top = __vmaxu2(top, __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
-          put_q<D>(dst, i0 + i, w[i], p.q.dtype, sign, live);
+          if (!PAIR || a == 0) put_q<D>(dst, i0 + i, w[i], p.q.dtype, sign, live);
         }
       }
       top = max(top & 0xffffu, top >> 16);
@@ -501,7 +528,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       int ex = row_exponent(p.q.dtype, fmaxf(__uint_as_float(top << 16), other_top));
       if (ex >= -4 && ex <= 14) {
         ex = 0;
-      } else {
+      } else if (!PAIR || a == 0) {
 #pragma unroll 1
         for (int i = half * (NC / 2); i < (half + 1) * (NC / 2); ++i)
           put_q<D>(dst, i, raw8(p.q, at + i * 8, p.wide_q), p.q.dtype, sign * pow2i(-ex), live);
@@ -515,7 +542,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       float m = kNone, l = 0.f;
 
 #pragma unroll 1
-      for (int st = u.st0; st < u.st1; ++st, ++k) {
+      for (int st = u.st0 + (PAIR ? a : 0); st < u.st1; st += kStep, ++k) {
         const int tok = st * kStageTokens + 64 * half, stage = v + st - u.st0;
         const bool tail = (st + 1) * kStageTokens > u.sure;
         uint32_t sees[2] = {~0u, ~0u};
@@ -576,7 +603,7 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           const float mm = over ? base + best : m, by = ex2(m - mm);
           m = mm;
           l *= by;
-          if (st > u.st0) {
+          if (st >= u.st0 + kStep) {
 #pragma unroll 1
             for (int q = half * (D / 2); q < (half + 1) * (D / 2); q += 8) {
               float o[8];
@@ -604,16 +631,43 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
       ok = ok && mbar_wait_bounded(bar(mt->o_full[a]), unit++ & 1, p.err);
       tc_fence_after();
       l += meet(1, l);
-      // O to the output, or as a partial state [D][256], m, l; half the channels a thread.
+      // PAIR: a thread reads both accumulators, which lie in the same lanes.
+      float by[2] = {1.f, 0.f};
+      if (both) {
+        if (half == 0) mt->end[a][0][th] = m, mt->end[a][1][th] = l;
+        tc_fence_before();
+        asm volatile("bar.sync 2, 512;" ::: "memory");
+        tc_fence_after();
+        m = fmaxf(mt->end[0][0][th], mt->end[1][0][th]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) by[i] = ex2(mt->end[i][0][th] - m);
+        l = mt->end[0][1][th] * by[0] + mt->end[1][1][th] * by[1];
+      }
+      // O to the output, or as a partial state [D][256], m, l; half (a quarter)
+      // of the channels a thread.
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long out_at = (u.row0 + row) * p.out.row_stride + head * p.out.head_stride;
       float* part = p.parts + (long long)(u.part0 + u.part) * ((D + 2) * kWideCols) + col;
+      const int share = both ? NC / 4 : NC / 2, i0 = (both ? 2 * a + half : half) * share;
 #pragma unroll 1
-      for (int i = half * (NC / 2); i < (half + 1) * (NC / 2); ++i) {
+      for (int i = i0; i < i0 + share; ++i) {
         float y[8];  // channels 8 i ..
+        if (both) {
+          float z[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = tm_load1(o_at + e * NC + i);
-        tm_wait(y);
+          for (int e = 0; e < 8; ++e) {
+            y[e] = tm_load1(o_at - a * 128 + e * NC + i);
+            z[e] = tm_load1(o_at - a * 128 + 128 + e * NC + i);
+          }
+          tm_wait(y);
+          tm_wait(z);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = y[e] * by[0] + z[e] * by[1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = tm_load1(o_at + e * NC + i);
+          tm_wait(y);
+        }
         if (u.n_parts == 1) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] *= inv;
@@ -623,11 +677,13 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           for (int e = 0; e < 8; ++e) part[(i * 8 + e) * kWideCols] = y[e];
         }
       }
-      if (u.n_parts > 1 && half == 0) {
+      if (u.n_parts > 1 && half == 0 && (!PAIR || a == 0)) {
         part[D * kWideCols] = m;
         part[(D + 1) * kWideCols] = l;
       }
       tc_fence_before();
+      // Before an accumulator, or the states above, are written again.
+      if (both) asm volatile("bar.sync 2, 512;" ::: "memory");
     }
     v += u.st1 - u.st0;
     if (next == u.last) break;
@@ -665,9 +721,9 @@ __global__ void __launch_bounds__(kWideCols) wide_join_kernel(const __grid_const
   store8(p.out, (u.row0 + r / G) * p.out.row_stride + (u.kvh * G + r % G) * p.out.head_stride + c * 8, p.wide_out, x);
 }
 
-template <int D>
+template <int D, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant__ AttendParams p) {
-  using Sh = Shape<D>;
+  using Sh = Shape<D, PAIR>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Meta* mt = reinterpret_cast<Meta*>(smem + Sh::META_AT);
   const int warp = threadIdx.x >> 5;
@@ -682,10 +738,10 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
       init(mt->s_full[i], 1);
       init(mt->p_full[i], 256);
       init(mt->o_full[i], 1);
+      init(mt->raw_k[i], 1);
+      init(mt->raw_v[i], 1);
     }
     init(mt->idle, 1);
-    init(mt->raw_k, 1);
-    init(mt->raw_v, 1);
     fence_mbar_init();
   }
   if (warp == kIssuer) tmem_alloc(&mt->tmem, 512);
@@ -695,13 +751,13 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   const uint32_t tmem = mt->tmem;
   pdl_wait();
   if (warp < kUnpackK) {
-    softmax_role<D>(p, smem, mt, tmem, warp / 8, warp / 4 % 2);
+    softmax_role<D, PAIR>(p, smem, mt, tmem, warp / 8, warp / 4 % 2);
   } else if (warp < kUnpackV) {
-    unpack_role<D, false>(p, smem, mt, threadIdx.x - kUnpackK * 32);
+    unpack_role<D, PAIR, false>(p, smem, mt, threadIdx.x - kUnpackK * 32);
   } else if (warp < kIssuer) {
-    unpack_role<D, true>(p, smem, mt, threadIdx.x - kUnpackV * 32);
+    unpack_role<D, PAIR, true>(p, smem, mt, threadIdx.x - kUnpackV * 32);
   } else {
-    issue_role<D>(p, smem, mt, tmem);
+    issue_role<D, PAIR>(p, smem, mt, tmem);
   }
   __syncwarp();
   tc_fence_before();
@@ -709,31 +765,37 @@ __global__ void __launch_bounds__(kThreads, 1) wide_kernel(const __grid_constant
   if (warp == kIssuer) tmem_dealloc(tmem, 512);
 }
 
-template <int D>
+template <int D, bool PAIR>
 int smem_bytes() {
-  return Shape<D>::META_AT + (int)sizeof(Meta);
+  return Shape<D, PAIR>::META_AT + (int)sizeof(Meta);
+}
+template <int D, bool PAIR>
+cudaError_t allow() {
+  return cudaFuncSetAttribute(wide_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, PAIR>());
+}
+template <int D, bool PAIR>
+cudaError_t launch(const AttendParams& p, cudaStream_t s) {
+  const cudaError_t e =
+      launch_overlapping(wide_kernel<D, PAIR>, dim3(p.n_ctas), kThreads, smem_bytes<D, PAIR>(), s, p);
+  if (e != cudaSuccess || !p.n_joins) return e;
+  return launch_overlapping(wide_join_kernel<D>, dim3(p.n_joins, D / 8), PAIR ? kTileCols : kWideCols, 0, s, p);
 }
 
 }  // namespace
 
 cudaError_t wide_setup() {
-  cudaError_t e = cudaFuncSetAttribute(wide_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<128>());
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(wide_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<64>());
+  cudaError_t e = allow<128, false>();
+  if (e == cudaSuccess) e = allow<128, true>();
+  if (e == cudaSuccess) e = allow<64, false>();
+  if (e == cudaSuccess) e = allow<64, true>();
   return e;
 }
 size_t wide_part_floats(int head_dim) { return (size_t)(head_dim + 2) * kWideCols; }
 
-cudaError_t launch_wide(const AttendParams& p, int head_dim, cudaStream_t s) {
+cudaError_t launch_wide(const AttendParams& p, int head_dim, bool pair, cudaStream_t s) {
   if (p.n_ctas <= 0) return cudaSuccess;
-  const cudaError_t e =
-      head_dim == 128
-          ? launch_overlapping(wide_kernel<128>, dim3(p.n_ctas), kThreads, smem_bytes<128>(), s, p)
-          : launch_overlapping(wide_kernel<64>, dim3(p.n_ctas), kThreads, smem_bytes<64>(), s, p);
-  if (e != cudaSuccess || !p.n_joins) return e;
-  const dim3 grid(p.n_joins, head_dim / 8);
-  return head_dim == 128 ? launch_overlapping(wide_join_kernel<128>, grid, kWideCols, 0, s, p)
-                         : launch_overlapping(wide_join_kernel<64>, grid, kWideCols, 0, s, p);
+  if (head_dim == 128) return pair ? launch<128, true>(p, s) : launch<128, false>(p, s);
+  return pair ? launch<64, true>(p, s) : launch<64, false>(p, s);
 }
 
 }  // namespace kv4

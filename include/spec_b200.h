@@ -547,7 +547,8 @@ void spec_kv4_free(spec_kv4* c);
  * attention has a kernel for few (row, query head) columns a sequence and one
  * for many, chosen per plan by an estimate of their times; the environment
  * variable SPEC_B200_KV4_WIDE_FROM=<columns>, read here, sends every sequence
- * of more columns to the latter instead. */
+ * of more columns to the latter instead, and SPEC_B200_KV4_WIDE_PAIR=0|1 fixes
+ * that one's form (256 columns a block, or 128 in two accumulators). */
 int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out);
 void spec_kv4_batch_free(spec_kv4_batch* b);
 /* One step over n_seqs sequences (host arrays, copied before the call

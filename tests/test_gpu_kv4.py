@@ -429,6 +429,46 @@ def test_attend_many_columns(pkg, monkeypatch, case, q_type, out_type, pad, colu
     assert torch.equal(s.batch.attend(0, q, out=again), out)
 
 
+def one_tile(monkeypatch, on):
+    """The kernel for many columns: one tile of 128 with its stages in pairs, or two tiles."""
+    monkeypatch.setenv("SPEC_B200_KV4_WIDE_PAIR", str(int(on)))
+
+
+@pytest.mark.parametrize("case", range(len(WIDE)))
+@pytest.mark.parametrize("q_type,out_type,pad", [("bf16", "bf16", 0), ("f16", "f32", 3)])
+def test_attend_many_columns_stages_in_pairs(pkg, monkeypatch, case, q_type, out_type, pad):
+    one_tile(monkeypatch, True)
+    test_attend_many_columns(pkg, monkeypatch, case, q_type, out_type, pad, 0)
+
+
+@pytest.mark.parametrize("heads", [4, 32])
+def test_attend_odd_rows_stages_in_pairs(pkg, monkeypatch, heads):
+    """Rows that see nothing, NaN and large scores, through two accumulators."""
+    one_tile(monkeypatch, True)
+    test_attend_rows_that_see_nothing_give_zeros(pkg, monkeypatch, heads, 0)
+    test_attend_nan_stays_where_it_is_seen(pkg, monkeypatch, heads, 0)
+    test_attend_peaked_and_large_scores(pkg, monkeypatch, heads, 0)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("pair", [False, True])
+def test_attend_many_columns_many_sequences(pkg, monkeypatch, d, pair):
+    """More tiles than blocks: a block takes several, of 1 to 3 stages."""
+    one_tile(monkeypatch, pair)
+    wide_from(monkeypatch, 0)
+    kv = [(97 * i) % 280 for i in range(44)]
+    rows = [40 if i == 9 else 1 + i % 4 for i in range(44)]
+    ends = [a + b for a, b in zip(kv, rows)]
+    s = Setup(pkg, 16, 4, d, 64, ends, seed=91)
+    s.fill(ends)
+    q, _ = s.rows(sum(rows), 16, "bf16", 1.5)
+    s.batch.plan(kv, rows, s.table)
+    for _ in range(2):
+        out = s.batch.attend(0, q)
+        s.batch.status()
+        check_attend(s, kv, rows, q, out, None, "bf16")
+
+
 def test_attend_few_and_many_columns_in_one_batch(pkg, monkeypatch):
     """A prompt chunk beside decoding sequences: both kernels in one call, the
     partial states of the one after those of the other."""
