@@ -107,6 +107,7 @@ struct spec_kv4_batch {
   int wide_from = -1;  // columns; -1: by estimate
   int wide_pair = -1;  // units in pairs of stages: 0, 1; -1: by estimate
   bool pair = false;   // and the plan's choice
+  int force_cols = -1, narrow_cols = kMaxCols;  // columns of a narrow unit at most, likewise
   int* arrived = nullptr;
   size_t arrived_cap = 0;
   float* parts = nullptr;
@@ -245,23 +246,27 @@ size_t up(size_t n) { return (n + 255) / 256 * 256; }
 // 153 at 3, 157 at 6).
 constexpr int kUnitCost = 2;
 
+constexpr int kNarrowCols[] = {8, 16, kMaxCols};
+
 // Columns of the narrow kernel's tiles of a sequence: of equal size, a multiple
-// of 8, at most kMaxCols.
-int narrow_tile(int64_t cols) {
-  const int64_t tiles = (cols + kMaxCols - 1) / kMaxCols;
+// of 8, at most `most`.
+int narrow_tile(int64_t cols, int most) {
+  const int64_t tiles = (cols + most - 1) / most;
   return tiles ? (int)(((cols + tiles - 1) / tiles + 7) / 8 * 8) : 0;
 }
 
 // Expected time (us) of the step's attention when sequences of more than
-// wide_from columns go to the wide kernel, in the form `pair`; fitted to all on
-// a B200, head size 128.  Measured / expected for 32 sequences at 4096 tokens
-// and 8 kv heads: narrow, 48 columns 151 / 150, 64 184 / 184; wide, 64 columns
-// 143 / 140, in pairs 130 / 134; 256 columns 180 / 182, in pairs 252 / 251.
-// One sequence, 2048 tokens: 64 columns narrow 20 / 23, wide 24 / 26, in pairs
-// 25 / 28; 256 wide 29 / 27, in pairs 24 / 25.  A round is a 128-token stage in
-// every resident CTA.
-double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from, bool pair) {
-  static const double kCall[5] = {0, 8, 9, 16, 21}, kRound[5] = {0, 2.5, 2.6, 2.35, 2.86};  // narrow, by 8-column tiles
+// wide_from columns go to the wide kernel, in the form `pair`, and the others to
+// the narrow one in tiles of at most narrow_cols; fitted to all on a B200, head
+// size 128, 8 kv heads.  Smaller tiles unpack the cache more often, by code that
+// is shorter and in more CTAs: measured / expected for 20 columns of one sequence
+// of 2048 tokens in tiles of 8, 16, 24 columns 12 / 10, 13 / 14, 15 / 16 us, of
+// 32 sequences of 4096 tokens 120 / 145, 109 / 110, 83 / 82.  Wide, 32 sequences
+// of 4096 tokens: 64 columns 143 / 140, in pairs 130 / 134; 256 columns 180 / 182,
+// in pairs 252 / 251; one of 2048: 64 columns 24 / 26, in pairs 25 / 28, 256 29 /
+// 27, in pairs 24 / 25.  A round is a 128-token stage in every resident CTA.
+double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from, bool pair, int narrow_cols) {
+  static const double kCall[5] = {0, 8, 12.6, 15, 21}, kRound[5] = {0, 3.2, 2.55, 2.35, 2.86};  // narrow, by 8-column tiles
   const Cache& c = *b->c;
   const int G = c.d.n_heads / c.d.n_kv_heads, wide_cols = pair ? kPairCols : kWideCols;
   double narrow = 0, wide = 0, slowest = 0;
@@ -278,7 +283,7 @@ double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from,
       else if (round > slowest) slowest = round;
       tiles += n * c.d.n_kv_heads;
     } else {
-      const int size = narrow_tile(cols);
+      const int size = narrow_tile(cols, narrow_cols);
       narrow += (double)((cols + size - 1) / size * st * c.d.n_kv_heads);
       if (size / 8 > nt) nt = size / 8;
     }
@@ -293,18 +298,21 @@ double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from,
   return us;
 }
 
-// From how many columns a sequence goes to the wide kernel, and that one's form:
-// the best of a few, or what SPEC_B200_KV4_WIDE_FROM and SPEC_B200_KV4_WIDE_PAIR
-// said when the batch was made.
-int choose_wide_from(const spec_kv4_batch* b, const spec_kv4_step* s, bool* pair) {
+// From how many columns a sequence goes to the wide kernel, that one's form and
+// the narrow one's tiles: the best of a few, or what SPEC_B200_KV4_WIDE_FROM,
+// SPEC_B200_KV4_WIDE_PAIR and SPEC_B200_KV4_NARROW_COLS said when the batch was made.
+int choose_wide_from(const spec_kv4_batch* b, const spec_kv4_step* s, bool* pair, int* narrow_cols) {
   int best = 0;
   double least = 1e300;
   for (const int from : {INT_MAX, 128, 64, kMaxCols})
     for (const bool form : {false, true}) {
       if (b->wide_pair >= 0 && form != (b->wide_pair > 0)) continue;
       const int limit = b->wide_from >= 0 ? b->wide_from : from;
-      const double us = attend_us(b, s, limit, form);
-      if (us < least) least = us, best = limit, *pair = form;
+      for (const int most : kNarrowCols) {
+        if (b->force_cols > 0 && most != b->force_cols) continue;
+        const double us = attend_us(b, s, limit, form, most);
+        if (us < least) least = us, best = limit, *pair = form, *narrow_cols = most;
+      }
     }
   return best;
 }
@@ -329,7 +337,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_fro
   int row0 = 0, table = 0;
   for (int q = 0; q < s->n_seqs; ++q) {
     const int n = s->kv_len[q], m = s->n_rows[q], cols = m * G;
-    const int size = !wide ? narrow_tile(cols) : pair ? kPairCols : kWideCols;
+    const int size = !wide ? narrow_tile(cols, b->narrow_cols) : pair ? kPairCols : kWideCols;
     for (int h = 0; h < c.d.n_kv_heads && (cols > wide_from) == wide; ++h)
       for (int c0 = 0; c0 < cols; c0 += size) {
         Unit u{};
@@ -503,7 +511,7 @@ int plan(spec_kv4_batch* b, const spec_kv4_step* s, cudaStream_t stream) {
   if (!s->src_rows) max_src = (int)rows - 1;
 
   b->planned = false;
-  const int wide_from = choose_wide_from(b, s, &b->pair);
+  const int wide_from = choose_wide_from(b, s, &b->pair, &b->narrow_cols);
   schedule(b, s, false, wide_from, b->pair);
   schedule(b, s, true, wide_from, b->pair);
   // One block: rows, masks, pages, units.
@@ -629,6 +637,9 @@ int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out) {
   b->c = c->c;
   if (const char* v = getenv("SPEC_B200_KV4_WIDE_FROM")) b->wide_from = atoi(v);
   if (const char* v = getenv("SPEC_B200_KV4_WIDE_PAIR")) b->wide_pair = atoi(v);
+  if (const char* v = getenv("SPEC_B200_KV4_NARROW_COLS"))
+    for (const int most : kNarrowCols)
+      if (atoi(v) == most) b->force_cols = most;
   cudaError_t e = cudaEventCreateWithFlags(&b->tail, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaEventCreateWithFlags(&b->copied, cudaEventDisableTiming);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, c->c->d.device);

@@ -548,7 +548,9 @@ void spec_kv4_free(spec_kv4* c);
  * for many, chosen per plan by an estimate of their times; the environment
  * variable SPEC_B200_KV4_WIDE_FROM=<columns>, read here, sends every sequence
  * of more columns to the latter instead, and SPEC_B200_KV4_WIDE_PAIR=0|1 fixes
- * that one's form (256 columns a block, or 128 in two accumulators). */
+ * that one's form (256 columns a block, or 128 in two accumulators);
+ * SPEC_B200_KV4_NARROW_COLS=8|16|32 fixes the most columns a block of the
+ * former takes. */
 int spec_kv4_batch_create(spec_kv4* c, spec_kv4_batch** out);
 void spec_kv4_batch_free(spec_kv4_batch* b);
 /* One step over n_seqs sequences (host arrays, copied before the call

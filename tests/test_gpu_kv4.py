@@ -429,6 +429,24 @@ def test_attend_many_columns(pkg, monkeypatch, case, q_type, out_type, pad, colu
     assert torch.equal(s.batch.attend(0, q, out=again), out)
 
 
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("most", [8, 16, 32])
+def test_attend_causal_in_tiles_of_few_columns(pkg, monkeypatch, case, most):
+    """The kernel for few columns in each of its tile sizes."""
+    monkeypatch.setenv("SPEC_B200_KV4_NARROW_COLS", str(most))
+    test_attend_causal(pkg, monkeypatch, case, "bf16", "f32", 1 << 20)
+
+
+@pytest.mark.parametrize("most", [8, 16, 32])
+def test_attend_odd_rows_in_tiles_of_few_columns(pkg, monkeypatch, most):
+    """Rows that see nothing, NaN and large scores, and trees."""
+    monkeypatch.setenv("SPEC_B200_KV4_NARROW_COLS", str(most))
+    test_attend_rows_that_see_nothing_give_zeros(pkg, monkeypatch, 32, 1 << 20)
+    test_attend_nan_stays_where_it_is_seen(pkg, monkeypatch, 32, 1 << 20)
+    test_attend_peaked_and_large_scores(pkg, monkeypatch, 32, 1 << 20)
+    test_attend_trees(pkg, 128, 8, 2, 64)
+
+
 def one_tile(monkeypatch, on):
     """The kernel for many columns: one tile of 128 with its stages in pairs, or two tiles."""
     monkeypatch.setenv("SPEC_B200_KV4_WIDE_PAIR", str(int(on)))
