@@ -56,6 +56,7 @@ constexpr int kTileCols = kPairCols;
 constexpr int kThreads = 24 * 32;
 constexpr int kUnpackK = 16, kUnpackV = 19, kIssuer = 23;  // first warps of the roles
 constexpr int kThreadsK = (kUnpackV - kUnpackK) * 32;
+constexpr float kFar = 1048576.f;  // 2^20: references from which scores are rounded before they are compared
 
 // ---- tensor memory ----------------------------------------------------------
 SPEC_DEV float tm_load1(uint32_t a) {
@@ -182,7 +183,7 @@ struct Meta {
   unsigned long long raw_k[2], raw_v[2];
   uint32_t bad[2][4];  // tokens of a V stage whose row is NaN
   uint32_t tmem;
-  float red[3][2][2][kTileCols];  // between the two threads of a column: largest, sum, largest again
+  float red[4][2][2][kTileCols];  // between the two threads of a column: largest, sum, and largest of two more turns
   float end[2][2][kTileCols];     // PAIR: the two accumulators' m and l
 };
 
@@ -556,14 +557,19 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
         // P against the column's last reference, kept in registers until the
         // column's largest exponent is known.  Where that passes kSlack, or
         // there is no reference yet, it moves the reference and P is made
-        // again; the scores are still there.
+        // again; the scores are still there.  Two passes, by construction: the
+        // second decides nothing.  Its largest exponent is what rounding took
+        // off the reference, an eighth at most below kFar.  Above, that would
+        // be octaves (8 from 2^27 on): there the scores are rounded in place
+        // first and the reference is the largest of them, so that it is 0.
         uint32_t f[32];
         float added;
         int kind = 0;
 #pragma unroll 1
         while (true) {
           const float base = m == kNone ? 0.f : m;
-          const unsigned long long c2 = two(c, c), m2 = two(-base, -base);
+          const float by_c = kind == 3 ? 1.f : c;
+          const unsigned long long c2 = two(by_c, by_c), m2 = two(-base, -base);
           unsigned long long sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
           float best = -INFINITY;
 #pragma unroll
@@ -596,11 +602,33 @@ SPEC_DEV void softmax_role(const AttendParams& p, uint8_t* smem, Meta* mt, uint3
           apart(add2(sum[0], sum[1]), sum_lo, sum_hi);
           added = sum_lo + sum_hi;
           best = fmaxf(best, meet(kind, best));
-          const bool over = m == kNone ? best > -INFINITY : best > kSlack;
+          bool over = m == kNone ? best > -INFINITY : best > kSlack;
           // Both warps of these columns decide alike.
-          if (!__any_sync(0xffffffffu, over)) break;
+          if (kind || !__any_sync(0xffffffffu, over || fabsf(base) >= kFar)) break;
           kind = 2;
-          const float mm = over ? base + best : m, by = ex2(m - mm);
+          float mm = over ? base + best : m;
+          if (__any_sync(0xffffffffu, fabsf(base) >= kFar || (over && fabsf(mm) >= kFar))) {
+            kind = 3;
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int q = 0; q < 64; q += 8) {
+              float x[8];
+              tm_load<8>(s_at + q, x);
+              tm_wait(x);
+              const uint32_t seen = (q < 32 ? sees[0] : sees[1]) >> (q & 31);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                x[i] = __fmul_rn(x[i], c);
+                if ((seen >> i) & 1) top = fmaxf(top, x[i]);
+              }
+              tm_store8(s_at + q, reinterpret_cast<const uint32_t*>(x));
+            }
+            tm_wait_st();
+            top = fmaxf(top, meet(2, top));
+            over = m == kNone ? top > -INFINITY : top - base > kSlack;
+            mm = over ? top : m;
+          }
+          const float by = ex2(m - mm);
           m = mm;
           l *= by;
           if (st >= u.st0 + kStep) {

@@ -1,0 +1,97 @@
+"""4-bit paged KV cache on the GPU, edges: scores of any finite size."""
+
+import numpy as np
+import pytest
+
+from test_gpu_kv4 import Setup, one_tile, wide_from
+
+pytestmark = pytest.mark.gpu
+
+# Which kernel takes the columns: the one for few, the one for many in two tiles, and in one with stages in pairs.
+KERNELS = ["few", "many", "pairs"]
+
+
+def on(monkeypatch, kernel):
+    wide_from(monkeypatch, 1 << 20 if kernel == "few" else 0)
+    if kernel != "few":
+        one_tile(monkeypatch, kernel == "pairs")
+
+
+def stored_rows(s, n, k, v):
+    """Appends f32 rows k, v [n, kv heads, d] to the one sequence; their stored values in float64."""
+    import torch
+    s.batch.plan([0], [n], s.table)
+    s.batch.append(0, None, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
+    for i in range(n):
+        s.store(0, i, k[i], v[i])
+    return s.values(0, n)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("logit", [1e4, 1e7, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("d,heads,rows", [(128, 8, 4), (64, 6, 30)])
+def test_attend_far_scores_take_the_largest(pkg, monkeypatch, kernel, logit, sign, d, heads, rows):
+    """One score of every column stands far above the others: the output is its
+    token's value, at any size of the scores.  The largest score grows from
+    stage to stage, so the reference moves late as well as early."""
+    import torch
+    on(monkeypatch, kernel)
+    n = 700
+    s = Setup(pkg, heads, 1, d, 64, [n], rope=False, seed=int(np.log10(logit)))
+    # Keys along one pattern of signs, lengths of both signs, every stage's
+    # extremes 10 % past the others and 30 % past the stage before.
+    pattern = np.sign(s.rng.standard_normal(d)).astype(np.float32)
+    size = s.rng.uniform(-1, 1, n).astype(np.float32)
+    for st in range(0, n, 128):
+        top, low = s.rng.permutation(min(128, n - rows - st))[:2] + st
+        size[top], size[low] = 1.1, -1.1
+        size[st:st + 128] *= np.float32(1.3 ** (st // 128))
+    k = size[:, None, None] * pattern[None, None]
+    v = s.rng.standard_normal((n, 1, d)).astype(np.float32)
+    kk, vv = stored_rows(s, n, k, v)
+    q = (pattern * s.rng.uniform(0.5, 1, (rows, heads, 1)) * logit / np.sqrt(d)).astype(np.float32)
+    q = torch.from_numpy(q).cuda().bfloat16()
+    s.batch.plan([n - rows], [rows], s.table)
+    scale = sign * d ** -0.5
+    out = s.batch.attend(0, q, out=torch.empty(rows, heads, d, device="cuda"), scale=scale)
+    s.batch.status()
+    got, qn = out.cpu().numpy(), q.float().cpu().numpy().astype(np.float64)
+    for i in range(rows):
+        seen = n - rows + i + 1
+        scores = np.einsum("td,hd->ht", kk[:seen, 0], qn[i]) * scale
+        order = np.sort(scores, 1)
+        # Far enough apart for f16 keys (2^-11) and their exponentials.
+        assert (order[:, -1] - order[:, -2] > 0.02 * np.abs(order[:, -1]) + 30).all()
+        want = vv[scores.argmax(1), 0]
+        # One weight and one value, each rounded to f16: kv4_ref.attend's term of 2.5 roundings.
+        assert (np.abs(got[i] - want) <= 2.5 * 2.0 ** -11 * np.abs(want) + 1e-6).all(), i
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("logit", [1e3, 1e6, 1e8, 1e9, 3e9, 1e12, 1e20])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("d,heads", [(128, 32), (64, 5)])
+def test_attend_equal_scores_share_alike(pkg, monkeypatch, kernel, logit, sign, d, heads):
+    """All keys are one row: every output is the mean of the values seen, at any size of the scores."""
+    import torch
+    on(monkeypatch, kernel)
+    n, rows = 300, 5
+    s = Setup(pkg, heads, 1, d, 32, [n], rope=False, seed=77)
+    k = np.repeat(s.rng.standard_normal((1, 1, d)).astype(np.float32), n, 0)
+    v = s.rng.standard_normal((n, 1, d)).astype(np.float32)
+    kk, vv = stored_rows(s, n, k, v)
+    # q along the key, so that the score is the sum of |.| and columns differ in size.
+    q = np.sign(kk[0, 0]) * s.rng.uniform(0.5, 1, (rows, heads, 1)) * logit / np.abs(kk[0, 0]).sum() * np.sqrt(d)
+    q = torch.from_numpy(q.astype(np.float32)).cuda().bfloat16()
+    s.batch.plan([n - rows], [rows], s.table)
+    out = s.batch.attend(0, q, out=torch.empty(rows, heads, d, device="cuda"), scale=sign * d ** -0.5)
+    s.batch.status()
+    got = out.cpu().numpy()
+    for i in range(rows):
+        seen = vv[:n - rows + i + 1, 0]
+        want = seen.mean(0)
+        # Values as f16 (2^-11), weights all alike (as f16 2^-11 once more where
+        # the largest exponent is not 0), sums in f32.
+        bound = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -18) * np.abs(seen).mean(0) + 1e-6
+        assert (np.abs(got[i] - want) <= bound).all(), i
