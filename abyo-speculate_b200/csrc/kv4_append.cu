@@ -159,16 +159,21 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
     if (value) r.get(x);
     else turn(r, x);
 
-    // Clamping lo and hi is clamping every x: a value past the clamp has the
-    // code of lo or hi either way.
     float lo = x[0], hi = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) {
       lo = min_nan(lo, x[i]);
       hi = max_nan(hi, x[i]);
     }
-    lo = min_nan(max_nan(lo, -kClamp), kClamp);
-    hi = min_nan(max_nan(hi, -kClamp), kClamp);
+    // Out of range (hardly ever): every value is clamped, not lo and hi alone.
+    // o is rounded to 16 near the clamp, so a value past it need not have the
+    // least or the largest code.
+    if (!(lo >= -kClamp && hi <= kClamp)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -kClamp), kClamp);
+      lo = min_nan(max_nan(lo, -kClamp), kClamp);
+      hi = min_nan(max_nan(hi, -kClamp), kClamp);
+    }
     // A NaN anywhere in the head's row makes the whole stored row NaN, so that
     // the attention can tell from one scale pair.
     const uint32_t nans = __ballot_sync(0xffffffffu, lo != lo);

@@ -1,4 +1,4 @@
-"""4-bit paged KV cache on the GPU, edges: scores of any finite size."""
+"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp."""
 
 import numpy as np
 import pytest
@@ -95,3 +95,41 @@ def test_attend_equal_scores_share_alike(pkg, monkeypatch, kernel, logit, sign, 
         # the largest exponent is not 0), sums in f32.
         bound = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -18) * np.abs(seen).mean(0) + 1e-6
         assert (np.abs(got[i] - want) <= bound).all(), i
+
+
+def same_bytes_or_nan(got, want):
+    """Equal pools, but for the payloads of NaN scales."""
+    a, b = (np.frombuffer(x.tobytes(), np.float16) for x in (got, want))
+    pair = (got == want).reshape(-1, 2).all(1) | (np.isnan(a) & np.isnan(b))
+    return pair.all()
+
+
+@pytest.mark.parametrize("d,wide", [(128, True), (64, True), (128, False)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_append_rows_around_the_clamp(pkg, d, wide, dtype):
+    """Groups that lie across +-20000 are clamped before they are coded: their
+    clamped range is small and o is rounded to 16 there, so that a value past
+    the clamp need not have the least or the largest code."""
+    import torch
+    n, kv = 40, 2
+    s = Setup(pkg, 2, kv, d, 16, [n], rope=False, seed=d)
+    x = np.empty((n, kv, d), np.float32)
+    for i in range(n):
+        half_width = [10, 40, 100, 1000, 9000][i % 5]
+        x[i] = (20000 + s.rng.uniform(-1, 1, (kv, d)) * half_width) * (1 if i % 2 else -1)
+    x[0, 0], x[1, 0] = np.linspace(19990, 20010, d), np.linspace(-20010, -19990, d)
+    x[2, 1, 3], x[3, 1, d - 1], x[4, 0, 7] = np.inf, -np.inf, -30000
+    x[5] = 25000  # a group all past the clamp
+    k = torch.from_numpy(x).cuda().to(torch.float32 if dtype == "f32" else torch.bfloat16)
+    v = k.flip(0).contiguous()
+    if not wide:  # rows that are not 16-byte pieces
+        k, v = (torch.cat([t, t[:, :, :1]], 2)[:, :, :d] for t in (k, v))
+    k_out, v_out = (torch.empty(n, kv, d, dtype=torch.float16, device="cuda") for _ in range(2))
+    s.batch.plan([0], [n], s.table)
+    s.batch.append(0, None, k, v, k_out=k_out, v_out=v_out)
+    kn, vn = k.float().cpu().numpy(), v.float().cpu().numpy()
+    for i in range(n):
+        val = s.store(0, i, kn[i], vn[i])
+        assert np.array_equal(k_out[i].cpu().numpy(), val[0].astype(np.float16)), i
+        assert np.array_equal(v_out[i].cpu().numpy(), val[1].astype(np.float16)), i
+    assert same_bytes_or_nan(s.device_pool(), s.host)
