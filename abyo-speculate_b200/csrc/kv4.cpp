@@ -398,7 +398,7 @@ void schedule(spec_kv4_batch* b, const spec_kv4_step* s, bool wide, int wide_fro
     for (int at = 0, i = 0; at < end; ++i) {
       int64_t take;
       if (even) {
-        take = end * (i + 1) / n_even - at;
+        take = (int64_t)end * (i + 1) / n_even - at;  // stages x parts pass 32 bits
       } else {
         // What is left of this CTA's share; at least a stage.
         const int64_t share = cost * (cta + 1) / slots;

@@ -1,4 +1,4 @@
-"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp."""
+"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context of half a billion tokens."""
 
 import numpy as np
 import pytest
@@ -133,3 +133,37 @@ def test_append_rows_around_the_clamp(pkg, d, wide, dtype):
         assert np.array_equal(k_out[i].cpu().numpy(), val[0].astype(np.float16)), i
         assert np.array_equal(v_out[i].cpu().numpy(), val[1].astype(np.float16)), i
     assert same_bytes_or_nan(s.device_pool(), s.host)
+
+
+def test_attend_length_times_parts_past_32_bits(pkg, monkeypatch):
+    """A context of 4.2 million stages in some hundred parts.  Its table lists
+    one page over and over, so the attention is that over the page's tokens."""
+    import torch
+    on(monkeypatch, "few")
+    d, p = 64, 128
+    stages = 4_200_000
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert stages * sms * 4 > 1 << 31
+    s = Setup(pkg, 1, 1, d, p, [p + 1], rope=False, seed=6)
+    s.fill([p + 1])
+    table = np.full((1, stages + 1), s.table[0][0], np.int32)
+    table[0, -1] = s.table[0][1]
+    q, _ = s.rows(1, 1, "bf16", 1.5)
+    s.batch.plan([p], [1], s.table)
+    want = s.batch.attend(0, q, out=torch.empty(1, 1, d, device="cuda")).cpu().numpy()[0, 0]
+    s.batch.plan([stages * p], [1], table)
+    got = s.batch.attend(0, q, out=torch.empty(1, 1, d, device="cuda")).cpu().numpy()[0, 0]
+    s.batch.status()
+    # The token after the pages weighs 1 / 4.2e6 of them here and is an
+    # 129th of what is seen there: it is taken out of the first.
+    k, v = s.values(0, p + 1)
+    score = np.exp(k[:, 0] @ q[0, 0].float().cpu().numpy().astype(np.float64) * d ** -0.5)
+    mean = score[:p] @ v[:p, 0] / score[:p].sum()
+    one = score @ v[:, 0] / score.sum()
+    near = np.abs(v[:p + 1, 0]).max()
+    assert np.abs(want - one).max() <= 2.5 * 2.0 ** -11 * near + 1e-6
+    # f32 running sums of a warp: 4.2e6 * 4 / (4 sms * 4 warps) tiles of 32
+    # tokens, 8 additions a lane and tile, half an ulp (2^-24) each and the
+    # matrix products' truncation (2^-23) as much again, all one way.
+    tiles = stages * 4 / (sms * 4 * 4)
+    assert np.abs(got - mean).max() <= (2.5 * 2.0 ** -11 + tiles * 8 * 2.0 ** -23) * near + 1e-6
