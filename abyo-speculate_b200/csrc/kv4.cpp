@@ -202,6 +202,21 @@ cudaError_t grow(spec_kv4_batch* b, T** p, size_t* cap, size_t n, bool zero) {
   return e;
 }
 
+// Whether two of rows x heads runs of D elements meet: rows lie `row` elements
+// apart, heads `head`.
+bool shares_elements(int64_t rows, int64_t heads, int64_t row, int64_t head, int64_t D) {
+  if (heads > 1 && head < D) return true;
+  if (rows > 1 && row < D) return true;
+  if (rows <= 1 || heads <= 1 || row / heads >= head || head / rows >= row) return false;
+  // Neither lies inside a step of the other: a run (dr, 0) against (0, dh), for
+  // every dh the two dr around it.
+  for (int64_t dh = 1; dh < heads; ++dh) {
+    const int64_t at = dh * head, dr = at / row;
+    if ((dr < rows && at - dr * row < D) || (dr + 1 < rows && (dr + 1) * row - at < D)) return true;
+  }
+  return false;
+}
+
 int check_rows(const char* what, const spec_kv4_rows* r, int64_t need, int heads, int D, bool written) {
   if (!r->ptr) return fail(SPEC_ERR_INVALID, "spec_kv4: %s has no data", what);
   if (r->dtype < T_BF16 || r->dtype > T_F32) return fail(SPEC_ERR_INVALID, "spec_kv4: %s has type %d", what, r->dtype);
@@ -213,11 +228,9 @@ int check_rows(const char* what, const spec_kv4_rows* r, int64_t need, int heads
     return fail(SPEC_ERR_INVALID, "spec_kv4: %s has a stride outside [0, 2^40]", what);
   if (reinterpret_cast<uintptr_t>(r->ptr) % (r->dtype == T_F32 ? 4 : 2))
     return fail(SPEC_ERR_INVALID, "spec_kv4: %s is not aligned to its element size", what);
-  // Outputs must not overlap themselves.
-  if (written && heads > 1 && r->head_stride < D)
-    return fail(SPEC_ERR_INVALID, "spec_kv4: heads of %s overlap (stride %lld)", what, (long long)r->head_stride);
-  if (written && need > 1 && r->row_stride < D)
-    return fail(SPEC_ERR_INVALID, "spec_kv4: rows of %s overlap (stride %lld)", what, (long long)r->row_stride);
+  if (written && shares_elements(need, heads, r->row_stride, r->head_stride, D))
+    return fail(SPEC_ERR_INVALID, "spec_kv4: rows or heads of %s overlap (strides %lld and %lld)", what,
+                (long long)r->row_stride, (long long)r->head_stride);
   return SPEC_OK;
 }
 

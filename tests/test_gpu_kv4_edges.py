@@ -1,4 +1,5 @@
-"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context of half a billion tokens."""
+"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context
+of half a billion tokens, outputs that overlap themselves."""
 
 import numpy as np
 import pytest
@@ -167,3 +168,38 @@ def test_attend_length_times_parts_past_32_bits(pkg, monkeypatch):
     # matrix products' truncation (2^-23) as much again, all one way.
     tiles = stages * 4 / (sms * 4 * 4)
     assert np.abs(got - mean).max() <= (2.5 * 2.0 ** -11 + tiles * 8 * 2.0 ** -23) * near + 1e-6
+
+
+def test_outputs_that_overlap_themselves_are_refused(pkg):
+    """Rows and heads whose strides make them meet, and layouts that look alike but do not."""
+    import torch
+    s = Setup(pkg, 4, 2, 64, 16, [40], seed=42)
+    s.fill([36])
+    b, d = s.batch, 64
+    q = torch.randn(4, 4, d, device="cuda").bfloat16()
+    k = torch.randn(4, 2, d, device="cuda").bfloat16()
+    b.plan([32], [4], s.table)
+    room = torch.zeros(40 * d, dtype=torch.bfloat16, device="cuda")
+
+    def out(heads, row, head, dtype=None):
+        t = room if dtype is None else room.to(dtype)
+        return t.as_strided((4, heads, d), (row, head, 1))
+
+    want = b.attend(0, q)
+    for row, head in ((d, d), (2 * d, d), (3 * d, 2 * d), (d + 8, d), (d, d + 8), (4 * d - 8, d), (d, 4 * d - 8),
+                      (5 * d, 5 * d)):
+        with pytest.raises(pkg.SamplingError, match="overlap"):
+            b.attend(0, q, out=out(4, row, head))
+    for row, head in ((4 * d, d), (d, 4 * d), (d + 8, 4 * (d + 8)), (2 * d, 8 * d), (5 * d, d + 8), (3 * d, 4 * d)):
+        got = b.attend(0, q, out=out(4, row, head))
+        assert torch.equal(got, want), (row, head)
+    got = b.append(0, q, k, k, q_out=torch.empty_like(q))
+    with pytest.raises(pkg.SamplingError, match="overlap"):
+        b.append(0, q, k, k, q_out=out(4, d, d))
+    with pytest.raises(pkg.SamplingError, match="overlap"):
+        b.append(0, q, k, k, q_out=got, k_out=out(2, d, d, torch.float16))
+    with pytest.raises(pkg.SamplingError, match="overlap"):
+        b.append(0, q, k, k, q_out=got, v_out=out(2, d, d, torch.float16))
+    b.append(0, q, k, k, q_out=got, k_out=out(2, 3 * d, 2 * d, torch.float16))  # interleaved, nothing shared
+    b.plan([32], [1], s.table)  # one row: its stride is not used
+    assert torch.equal(b.attend(0, q[:1], out=out(4, d, d)[:1]), b.attend(0, q[:1]))
