@@ -14,6 +14,7 @@ without waiting for it.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 import struct
@@ -32,9 +33,31 @@ def _invalid(msg: str) -> _lib.SamplingError:
     return _lib.SamplingError(_lib.SPEC_ERR_INVALID, msg)
 
 
+_CODES = {np.int32: "i", np.uint64: "Q"}
+
+
 def _host(a, dtype, what: str, n: Optional[int] = None) -> np.ndarray:
+    """Whole numbers `a` as a flat contiguous array of `dtype`, every one of them
+    as it is: what is not whole or does not fit is refused.  (Signed 64-bit
+    arrays stand for 64-bit masks bit by bit.)"""
+    x = None
     try:
-        out = np.ascontiguousarray(np.asarray(a, dtype=dtype).reshape(-1))
+        if isinstance(a, (list, tuple)):
+            try:
+                x = np.asarray(array.array(_CODES[dtype], a))
+            except TypeError:  # not flat, or not whole
+                pass
+        if x is None:
+            x = np.asarray(a)
+            if x.size and x.dtype.kind not in "iub":
+                raise _invalid(f"{what}: {x.dtype} entries, whole numbers are needed")
+            if x.dtype == np.int64 and dtype == np.uint64 and not isinstance(a, (list, tuple)):
+                x = x.view(np.uint64)
+            if x.size and not np.can_cast(x.dtype, dtype):
+                lo, hi, ends = x.min(), x.max(), np.iinfo(dtype)
+                if lo < ends.min or hi > ends.max:
+                    raise _invalid(f"{what}: entries {lo} to {hi} do not fit {np.dtype(dtype)}")
+        out = np.ascontiguousarray(x.reshape(-1), dtype=dtype)
     except (OverflowError, ValueError, TypeError) as e:
         raise _invalid(f"{what}: {e}") from None
     if n is not None and out.size != n:
@@ -163,10 +186,16 @@ class KV4Batch:
         if isinstance(page_table, np.ndarray) and page_table.ndim == 2:
             stride, flat = page_table.shape[1], _host(page_table, np.int32, "page_table")
         else:
-            stride = max([len(t) for t in page_table], default=1)
+            sizes = [len(t) for t in page_table]
+            stride = max(sizes, default=1)
             flat = np.full((kv.size, max(stride, 1)), -1, dtype=np.int32)
-            for b, t in enumerate(page_table):
-                flat[b, :len(t)] = _host(t, np.int32, "page_table")
+            try:  # lists, the usual form, in one go
+                pages = array.array("i")
+                for t in page_table:
+                    pages.fromlist(t)
+            except (OverflowError, TypeError):
+                pages = np.concatenate([_host(t, np.int32, "page_table", len(t)) for t in page_table])
+            flat[np.arange(flat.shape[1]) < np.array(sizes, np.int64)[:, None]] = pages
         total = int(m.sum()) if (m >= 0).all() else None
         pos = None if positions is None else _host(positions, np.int32, "positions", total)
         msk = None if masks is None else _host(masks, np.uint64, "masks", total)
