@@ -183,7 +183,7 @@ class KV4Batch:
         m = _host(n_rows, np.int32, "n_rows", kv.size)
         if len(page_table) != kv.size:
             raise _invalid(f"page_table has {len(page_table)} rows, {kv.size} are needed")
-        if isinstance(page_table, np.ndarray) and page_table.ndim == 2:
+        if isinstance(page_table, np.ndarray) and page_table.ndim == 2 and page_table.shape[1]:
             stride, flat = page_table.shape[1], _host(page_table, np.int32, "page_table")
         else:
             sizes = [len(t) for t in page_table]

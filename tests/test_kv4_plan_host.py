@@ -82,3 +82,10 @@ def test_numbers_that_would_change_are_refused(pkg, batch, bad):
 def test_masks_that_would_change_are_refused(pkg, batch, bad):
     with pytest.raises(pkg.SamplingError, match="masks"):
         batch.plan([0], [1], [[0]], masks=bad)
+
+
+@pytest.mark.parametrize("table", [[[], []], np.zeros((2, 0), np.int32), np.zeros((2, 0)), [np.zeros(0, np.int32)] * 2])
+def test_tables_without_pages_list_none(batch, table):
+    """A table of no columns still has one entry a sequence, which is no page."""
+    batch.plan([0, 0], [1, 1], table)
+    assert (batch._lib.stride, batch._lib.table) == (1, [-1, -1])
