@@ -171,7 +171,8 @@ class KV4Batch:
         # The raw handle of torch's current stream, without a Stream object around it.
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         if raw is not None:
-            self._stream = lambda: raw(self._index)
+            index = self._index  # not self: the batch would hold itself
+            self._stream = lambda: raw(index)
 
     def plan(self, kv_len: Sequence[int], n_rows: Sequence[int], page_table, positions=None, masks=None,
              src_rows=None) -> None:

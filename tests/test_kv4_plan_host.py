@@ -1,6 +1,9 @@
 """What KV4Batch.plan hands to the library, on the CPU: the library's plan is replaced by one that copies its arguments."""
 
 import ctypes
+import gc
+import types
+import weakref
 from importlib import import_module
 
 import numpy as np
@@ -89,3 +92,31 @@ def test_tables_without_pages_list_none(batch, table):
     """A table of no columns still has one entry a sequence, which is no page."""
     batch.plan([0, 0], [1, 1], table)
     assert (batch._lib.stride, batch._lib.table) == (1, [-1, -1])
+
+
+def test_a_dropped_batch_is_freed_at_once(monkeypatch):
+    """Its workspace goes with the last reference, not when the collector finds
+    a cycle (which may be inside somebody's stream capture)."""
+    import torch  # noqa: F401  (a first import inside the constructor would keep its frame)
+    freed = []
+
+    class Lib:
+        def spec_kv4_batch_create(self, cache, out):
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_void_p))[0] = 16
+            return 0
+
+        def spec_kv4_batch_free(self, handle):
+            freed.append(handle.value)
+
+    monkeypatch.setattr(kv4._lib, "load", Lib)
+    cache = types.SimpleNamespace(_h=ctypes.c_void_p(8), head_dim=64, device=types.SimpleNamespace(index=0))
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        batch = kv4.KV4Batch(cache)
+        seen = weakref.ref(batch)
+        del batch
+        assert seen() is None and freed == [16]
+    finally:
+        if on:
+            gc.enable()
