@@ -43,6 +43,7 @@ int fail(int rc, const char* fmt, A... a) {
   return rc;
 }
 int fail_cuda(cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here: the next launch's check is not to find it
   return fail(e == cudaErrorMemoryAllocation ? SPEC_ERR_OOM : SPEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
@@ -121,7 +122,9 @@ namespace {
 
 bool capturing(cudaStream_t s) {
   cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &st) == cudaSuccess) return st != cudaStreamCaptureStatusNone;
+  cudaGetLastError();
+  return false;
 }
 
 // A call on stream `s`: ordered after the batch's previous call where that was

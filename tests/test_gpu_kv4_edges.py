@@ -1,5 +1,5 @@
 """4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context
-of half a billion tokens, outputs that overlap themselves."""
+of half a billion tokens, outputs that overlap themselves, errors left behind."""
 
 import numpy as np
 import pytest
@@ -203,3 +203,27 @@ def test_outputs_that_overlap_themselves_are_refused(pkg):
     b.append(0, q, k, k, q_out=got, k_out=out(2, 3 * d, 2 * d, torch.float16))  # interleaved, nothing shared
     b.plan([32], [1], s.table)  # one row: its stride is not used
     assert torch.equal(b.attend(0, q[:1], out=out(4, d, d)[:1]), b.attend(0, q[:1]))
+
+
+def test_a_failed_call_leaves_no_error_behind(pkg):
+    """A CUDA error that a call returned is not the next call's: an upload and a
+    matmul, whose launches are checked, go through after it."""
+    import ctypes
+    from importlib import import_module
+    import torch
+    raw = import_module("abyo-speculate_b200._lib")
+    synth = import_module("abyo-speculate_b200.gguf_synth")
+    lib = raw.load()
+    pool = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    desc = raw.KV4Desc(9999, 1, 2, 2, 64, 16, 4, 1)  # no such device
+    cache, batch = ctypes.c_void_p(), ctypes.c_void_p()
+    assert lib.spec_kv4_create(ctypes.byref(desc), pool.data_ptr(), pool.numel(), None, None, 0, ctypes.byref(cache)) == 0
+    x, y = torch.ones(1, 256, device="cuda"), torch.zeros(1, 128, device="cuda")
+    for _ in range(2):
+        assert lib.spec_kv4_batch_create(cache, ctypes.byref(batch)) == raw.SPEC_ERR_CUDA
+        w = pkg.QWeight(8, synth.quantize(np.ones((128, 256), np.float32), 8), 128, 256)
+        assert lib.spec_kv4_batch_create(cache, ctypes.byref(batch)) == raw.SPEC_ERR_CUDA
+        w.matmul(x.data_ptr(), 1, y.zero_().data_ptr(), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.allclose(y, torch.full_like(y, 256.0), rtol=1e-2)
+    lib.spec_kv4_free(cache)
