@@ -7,7 +7,7 @@
 namespace specb200 {
 namespace kv4 {
 
-constexpr float kNone = -1e30f;  // the softmax reference before any score
+constexpr float kNone = -3.402823466e38f;  // the softmax reference before any score: no finite one is below it
 constexpr float kSlack = 8.f;    // a score may pass the reference by this many octaves before it moves
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -1,5 +1,5 @@
 """4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context
-of half a billion tokens, outputs that overlap themselves, errors left behind."""
+of half a billion tokens, outputs that overlap themselves, errors left behind, scores past 1e30."""
 
 import numpy as np
 import pytest
@@ -227,3 +227,27 @@ def test_a_failed_call_leaves_no_error_behind(pkg):
         torch.cuda.synchronize()
         assert torch.allclose(y, torch.full_like(y, 256.0), rtol=1e-2)
     lib.spec_kv4_free(cache)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("logit", [-1e31, -1e34, -2e37, 2e37])
+@pytest.mark.parametrize("n", [40, 300, 3000])
+def test_attend_scores_past_1e30(pkg, monkeypatch, kernel, logit, n):
+    """Equal scores of any finite size: a row that sees tokens gives their mean,
+    in one part, two accumulators and many parts alike."""
+    import torch
+    on(monkeypatch, kernel)
+    d, heads, rows = 64, 4, 2
+    s = Setup(pkg, heads, 1, d, 64, [n], rope=False, seed=5)
+    k = np.repeat(s.rng.standard_normal((1, 1, d)).astype(np.float32), n, 0)
+    v = s.rng.standard_normal((n, 1, d)).astype(np.float32)
+    kk, vv = stored_rows(s, n, k, v)
+    q = np.sign(kk[0, 0]) * s.rng.uniform(0.5, 1, (rows, heads, 1)) * logit / np.abs(kk[0, 0]).sum() * np.sqrt(d)
+    q = torch.from_numpy(q.astype(np.float32)).cuda().bfloat16()
+    s.batch.plan([n - rows], [rows], s.table)
+    got = s.batch.attend(0, q, out=torch.empty(rows, heads, d, device="cuda")).cpu().numpy()
+    s.batch.status()
+    for i in range(rows):
+        seen = vv[:n - rows + i + 1, 0]
+        bound = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -16) * np.abs(seen).mean(0) + 1e-6
+        assert (np.abs(got[i] - seen.mean(0)) <= bound).all(), i
