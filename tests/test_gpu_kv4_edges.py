@@ -1,9 +1,11 @@
 """4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context
-of half a billion tokens, outputs that overlap themselves, errors left behind, scores past 1e30."""
+of half a billion tokens, outputs that overlap themselves, errors left behind, scores past 1e30;
+and the size of the error, and joins of more than one round."""
 
 import numpy as np
 import pytest
 
+from kv4_error import exact_and_deviation, in_deviations
 from test_gpu_kv4 import Setup, one_tile, wide_from
 
 pytestmark = pytest.mark.gpu
@@ -251,3 +253,62 @@ def test_attend_scores_past_1e30(pkg, monkeypatch, kernel, logit, n):
         seen = vv[:n - rows + i + 1, 0]
         bound = (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -16) * np.abs(seen).mean(0) + 1e-6
         assert (np.abs(got[i] - seen.mean(0)) <= bound).all(), i
+
+
+def narrow_tiles(monkeypatch, most):
+    monkeypatch.setenv("SPEC_B200_KV4_NARROW_COLS", str(most))
+
+
+@pytest.mark.parametrize("kernel,most", [("few", 8), ("few", 16), ("few", 32), ("many", 32), ("pairs", 32)])
+@pytest.mark.parametrize("d,page,q_type", [(128, 64, "bf16"), (128, 16, "f16"), (64, 32, "bf16"), (64, 128, "f16")])
+def test_attend_error_is_that_of_its_roundings(pkg, monkeypatch, kernel, most, d, page, q_type):
+    """Values and weights rounded to f16 once each; keys too in the kernel for
+    many columns, and not in the one for few."""
+    import torch
+    on(monkeypatch, kernel)
+    narrow_tiles(monkeypatch, most)
+    n, rows, heads, kv_heads = 600, 7, 8, 2
+    s = Setup(pkg, heads, kv_heads, d, page, [n], seed=d + most)
+    s.fill([n])
+    q, qn = s.rows(rows, heads, q_type, 2.0)
+    s.batch.plan([n - rows], [rows], s.table)
+    got = s.batch.attend(0, q, out=torch.empty(rows, heads, d, device="cuda")).cpu().numpy()
+    s.batch.status()
+    k, v = s.values(0, n)
+    want, dev = exact_and_deviation(qn.astype(np.float64), k, v, np.tri(rows, n, n - rows), d ** -0.5, kernel != "few")
+    assert in_deviations(got, want, dev) < 1
+
+
+@pytest.mark.parametrize("kernel,most", [("few", 8), ("few", 16), ("few", 32), ("many", 32), ("pairs", 32)])
+@pytest.mark.parametrize("tokens", [2200, 12000, 40000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_contexts_in_many_parts(pkg, monkeypatch, kernel, most, tokens, d):
+    """Long contexts of one KV head: 18, 94 and 313 stages, up to one a block, so
+    that partial states are joined in two and three rounds.  The table lists 20
+    pages over and over."""
+    import torch
+    on(monkeypatch, kernel)
+    narrow_tiles(monkeypatch, most)
+    p, rows, heads = 32, 3, 4
+    s = Setup(pkg, heads, 1, d, p, [20 * p + rows], rope=False, seed=tokens + d)
+    s.fill([20 * p])
+    listed = s.rng.integers(0, 20, tokens // p)
+    kv_len = len(listed) * p
+    table = [s.table[0][i] for i in listed] + [s.table[0][20]]
+    k, kn = s.rows(rows, 1, "f32", 1.5)
+    v, vn = s.rows(rows, 1, "f32")
+    s.batch.plan([kv_len], [rows], [table])
+    s.batch.append(0, None, k, v)
+    for i in range(rows):
+        s.store(0, 20 * p + i, kn[i], vn[i])
+    q, qn = s.rows(rows, heads, "bf16", 2.0)
+    got = s.batch.attend(0, q, out=torch.empty(rows, heads, d, device="cuda"))
+    again = s.batch.attend(0, q, out=torch.empty_like(got))
+    s.batch.status()
+    assert torch.equal(got, again)
+    kk, vv = s.values(0, 20 * p + rows)
+    times = np.concatenate([np.repeat(np.bincount(listed, minlength=20), p), np.zeros(rows)])
+    see = np.repeat(times[None], rows, 0)
+    see[:, 20 * p:] = np.tri(rows)
+    want, dev = exact_and_deviation(qn.astype(np.float64), kk, vv, see, d ** -0.5, kernel != "few")
+    assert in_deviations(got.cpu().numpy(), want, dev) < 1
