@@ -273,14 +273,20 @@ int narrow_tile(int64_t cols, int most) {
 
 // Expected time (us) of the step's attention when sequences of more than
 // wide_from columns go to the wide kernel, in the form `pair`, and the others to
-// the narrow one in tiles of at most narrow_cols; fitted to all on a B200, head
-// size 128, 8 kv heads.  Smaller tiles unpack the cache more often, by code that
-// is shorter and in more CTAs: measured / expected for 20 columns of one sequence
-// of 2048 tokens in tiles of 8, 16, 24 columns 12 / 10, 13 / 14, 15 / 16 us, of
-// 32 sequences of 4096 tokens 120 / 145, 109 / 110, 83 / 82.  Wide, 32 sequences
-// of 4096 tokens: 64 columns 143 / 140, in pairs 130 / 134; 256 columns 180 / 182,
-// in pairs 252 / 251; one of 2048: 64 columns 24 / 26, in pairs 25 / 28, 256 29 /
-// 27, in pairs 24 / 25.  A round is a 128-token stage in every resident CTA.
+// the narrow one in tiles of at most narrow_cols; fitted to all on a B200 at head
+// size 128 and 8 kv heads, and used as it is elsewhere.  Of 105 shapes (1 to 64
+// rows, one sequence of 500 to 16384 tokens or 8 and 32 of 4096; 4, 7 and 1 query
+// heads a kv head) the choice is within 5 % of the best form for 101 at head size
+// 128, 1.26 times it at worst (33 rows of 7 heads at 16384 tokens: 48 us, 38 in
+// pairs), and for 96 at head size 64, 2.6 times it at worst (the same on 2 kv
+// heads: 59 us, 23 in tiles of 16).  Smaller tiles unpack the cache more often,
+// by code that is shorter and in more CTAs: measured / expected for 20 columns of
+// one sequence of 2048 tokens in tiles of 8, 16, 24 columns 12 / 10, 13 / 14,
+// 15 / 16 us, of 32 sequences of 4096 tokens 120 / 145, 109 / 110, 83 / 82.
+// Wide, 32 sequences of 4096 tokens: 64 columns 143 / 140, in pairs 130 / 134;
+// 256 columns 180 / 182, in pairs 252 / 251; one of 2048: 64 columns 24 / 26, in
+// pairs 25 / 28, 256 29 / 27, in pairs 24 / 25.  A round is a 128-token stage in
+// every resident CTA.
 double attend_us(const spec_kv4_batch* b, const spec_kv4_step* s, int wide_from, bool pair, int narrow_cols) {
   static const double kCall[5] = {0, 8, 12.6, 15, 21}, kRound[5] = {0, 3.2, 2.55, 2.35, 2.86};  // narrow, by 8-column tiles
   const Cache& c = *b->c;

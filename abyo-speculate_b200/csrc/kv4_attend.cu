@@ -9,15 +9,18 @@
 //   S^T [16 tokens x 8 n] = K [16 x D] Q^T,   O^T [D x 8 n] += V^T [D x 16] P^T
 // K's codes are used as they are: (w & 0x000F000F) is a pair of f16 numbers
 // code 2^-24 (tensor cores take subnormals), (w & 0x00F000F0) code 2^-20, and
-// q carries the inverse powers.  A group's sum of code q is exact in f32 and
-// takes its scale there,
+// q carries the inverse powers.  The products code q are exact; a group's sum
+// of 32 of them is f32 and takes its scale there,
 //   s_j = sum_groups s / 16 (sum code q) + (s + o) (sum q),
 // so no rounding of K enters a score; the second term is one more product,
 // with the scale pairs as they are stored.  ldmatrix hands the lanes words of
 // one group.  V's codes become values in registers: (w >> shift) & 0x03C003C0 |
 // 0x3C003C00 is the pair 1 + code / 16, and one packed multiply-add by (s, o)
 // rounds the value to f16; P^T is S^T's fragment through movmatrix.  (V's
-// channels per m-tile span groups, so its scales cannot wait for the sum.)
+// channels per m-tile span groups, so its scales cannot wait for the sum.)  V
+// and P are rounded to f16, the widest that this rate of mma.sync takes: each
+// moves an output by at most 2^-11 of the weighted mean of |v|, about what
+// rounding the output to f16 does and an eighth of rounding it to bf16.
 //
 // A CTA is 4 warps that run on their own: warp w takes the 32-token tiles w,
 // w + 4, ... of the CTA's stages, copies them by TMA bulk copies into a ring
@@ -31,9 +34,10 @@
 // Bound by the integer pipe (55 %) and instruction issue (61 %) together: about
 // 630 warp instructions per 32 tokens of a head of 128 and 8 columns, a third of
 // them V's unpacking, and 160 more per 8 columns.  One row each of 64 sequences
-// of 500 to 16000 tokens, 32 query heads on 8 kv heads: 149 us, 4.4 TB/s of the
-// cache's bytes; one of 131072 tokens 50 us; one of 2048 tokens 8.9 us, of
-// which launch and one stage are 3.9 and a round of joins 2 to 4.
+// of 500 to 16000 tokens, 32 query heads on 8 kv heads: 147 us back to back in a
+// graph, 4.5 TB/s of the cache's bytes, and 159 where caches change from call
+// to call; one of 131072 tokens 50 us; one of 2048 tokens 9.0 us, of which
+// launch and one stage are 3.9 and a round of joins 2 to 4.
 #include "common.cuh"
 #include "kv4.h"
 #include "kv4_rows.cuh"

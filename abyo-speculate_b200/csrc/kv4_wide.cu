@@ -21,10 +21,12 @@
 // rolled and small: warps in four roles share an instruction cache that
 // unrolled ones overflow (2048 rows over 6144 tokens: 407 us unrolled, 361
 // rolled).  One thread a column held 64 scores and left the special function
-// unit idle three quarters of the time (272 us against 237).  Now 237 us: 1015
-// TFLOP/s, the tensor pipe and the exponentials busy half the time each, the
-// rest the chain of scores, exponentials and product of two tiles.  A 60-node
-// tree at 4096 tokens, 32 query heads on 8 kv heads: 31 us, and 26 in pairs,
+// unit idle three quarters of the time (272 us against 237).  Now 235 us, 1023
+// TFLOP/s, in bursts at 1965 MHz; without a pause the power cap holds the clock
+// near 1710 MHz and it takes 269 to 274, 880 TFLOP/s.  The tensor pipe and the
+// exponentials are busy half the time each, the rest is the chain of scores,
+// exponentials and product of two tiles.  A 60-node tree at 4096 tokens, 32
+// query heads on 8 kv heads: 31 us, and 26 in pairs,
 // where a CTA has half the columns to write out and twice the stages to overlap.
 // In pairs a stage serves one tile, and unpacking it (2300 cycles of K's three
 // warps, 1500 of V's four) is the longest part: 32 sequences of 64 columns at
@@ -37,6 +39,12 @@
 // channels are stored in the order a word's nibbles unpack (n, n + 4), and
 // V^T's row for channel 8 c + n is n * D/8 + c, so that the lanes of a warp
 // store neighbouring rows.
+//
+// K, V and P are rounded to f16, the widest operands of this rate; K's codes
+// cannot enter as they are, as they do for few columns, since its scales change
+// every 32 channels and one accumulator spans them all.  A rounding of K moves a
+// score by 2^-11 of its terms' norm: f16 outputs of 24 sequences of 9 rows are
+// off by 0.00022 of their norm, the f32 form by 0.00020.
 //
 // O is scaled only where a column's largest score passes its reference m by
 // more than kSlack octaves; P is made before that is known.  Runs are cut as

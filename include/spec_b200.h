@@ -516,8 +516,11 @@ int spec_qmatmul_noalloc(spec_qweight* w, const float* x_dev, int M, float* y_de
  *
  * Conventions of these calls: every pointer marked "device" belongs to the
  * caller; `stream` is the cudaStream_t the call's work is queued on (NULL =
- * CUDA's default stream) and nothing is synchronised, but for a batch's first
- * change of stream, which waits for the device once.  A batch handle orders
+ * CUDA's default stream).  append and attend wait for nothing, but for a
+ * batch's first change of stream, which waits for the device once.  A plan
+ * waits on the host for the upload of the plan before it, which lies in its
+ * stream behind the calls queued earlier (so the host plans one step ahead at
+ * most), and for the batch's calls where its buffers grow.  A batch handle orders
  * its own calls: one made on another stream than the call before it runs after
  * that call.  Calls on a stream under capture are recorded without that
  * ordering.  Messages: spec_last_error(NULL). */
@@ -579,7 +582,8 @@ typedef struct spec_kv4_step {
 int spec_kv4_plan(spec_kv4_batch* b, const spec_kv4_step* s, void* stream);
 /* Rows of heads on the device: element (row, head, channel) is at
  * ptr + row * row_stride + head * head_stride + channel (strides in elements;
- * n_rows rows may be read or written).  Types: 0 = bf16, 1 = f16, 2 = f32. */
+ * n_rows rows may be read or written).  Types: 0 = bf16, 1 = f16, 2 = f32.
+ * Refused: outputs of which two rows or heads share an element. */
 #define SPEC_KV4_BF16 0
 #define SPEC_KV4_F16 1
 #define SPEC_KV4_F32 2
@@ -602,9 +606,12 @@ int spec_kv4_append(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
 /* out = softmax(scale * q . k) v for every row and query head of the step
  * over `layer`'s pages, whose rows of this step were appended before.  q: bf16
  * or f16 rotated rows; out: any type.  Query head h reads kv head
- * h / (n_heads / n_kv_heads).  Products take the stored values rounded to f16
- * or exactly, q after an exact power-of-two scaling of each row, and sum in
- * f32; weights go to the second product as f16, their sums are f32.  A row
+ * h / (n_heads / n_kv_heads).  Both products sum in f32.  Their operands are
+ * f16: K as it is stored (few columns) or rounded (many), V and the weights
+ * rounded; the weights' sums are f32.  An f32 `out` has the error of these
+ * roundings all the same.  q is taken to within 2^-21 of its row's largest
+ * value, each row scaled by a power of two where that needs it.  Scores may
+ * have any finite size.  A row
  * that sees nothing gives zeros; a row that sees a stored NaN gives NaN.  One
  * call's result does not depend on timing; a row's last bits may depend on the
  * other rows of the plan.  A call recorded by stream capture holds the plan's
