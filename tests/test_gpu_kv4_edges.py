@@ -1,6 +1,7 @@
-"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows around the clamp, a context
-of half a billion tokens, outputs that overlap themselves, errors left behind, scores past 1e30;
-and the size of the error, and joins of more than one round."""
+"""4-bit paged KV cache on the GPU, edges: scores of any finite size, rows
+around the clamp, a context of half a billion tokens, outputs that overlap
+themselves, errors left behind, the size of the error, and joins of more than
+one round."""
 
 import numpy as np
 import pytest
