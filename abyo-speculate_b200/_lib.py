@@ -118,6 +118,15 @@ class KV4Rows(ctypes.Structure):
                 ("n_rows", ctypes.c_int64), ("dtype", ctypes.c_int), ("reserved", ctypes.c_int)]
 
 
+class BatchLogits(ctypes.Structure):
+    """spec_batch_logits (include/spec_b200.h)."""
+
+    _fields_ = [("device", ctypes.c_int), ("vocab", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("temperature", ctypes.c_float), ("logits", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("n_rows", ctypes.c_int64), ("temperatures", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
 # (name, restype, argtypes) of every function declared in include/spec_b200.h
 SIGNATURES = [
     ("spec_load_gguf", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(LoadOpts), ctypes.POINTER(ctypes.c_void_p)]),
@@ -218,6 +227,14 @@ SIGNATURES = [
     ("spec_kv4_attend", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p]),
     ("spec_kv4_status", ctypes.c_int, [ctypes.c_void_p]),
+    ("spec_batch_workspace_bytes", ctypes.c_int64, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
+    ("spec_batch_sample", ctypes.c_int,
+     [ctypes.POINTER(BatchLogits), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    ("spec_batch_verify", ctypes.c_int,
+     [ctypes.POINTER(BatchLogits), ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
+     + [ctypes.c_void_p] * 3),
+    ("spec_batch_verify_tree", ctypes.c_int,
+     [ctypes.POINTER(BatchLogits), ctypes.c_int] + [ctypes.c_void_p] * 7),
 ]
 
 _lib: Optional[ctypes.CDLL] = None

@@ -622,6 +622,82 @@ int spec_kv4_attend(spec_kv4_batch* b, int layer, const spec_kv4_rows* q, const 
  * that gave up in an earlier call (SPEC_ERR_TIMEOUT). */
 int spec_kv4_status(spec_kv4_batch* b);
 
+/* ---- sampling and verification of a batch ------------------------------------
+ * The device side of a round over many sequences, next to spec_kv4_*: drawing
+ * tokens from rows of logits, and accepting drafts against them.  The rules are
+ * those of spec_verify_rejection (crates/speculate/src/sampling/tokens.rs:14-55,
+ * 99-120; methods/vanilla.rs:59-106, 172-210) with the sums in 64 bits instead
+ * of sequential f32, for rows of several sequences, each with its own
+ * temperature, on device memory, and without a host decision:
+ *   weights      w_j = exp((l_j - max l) / T); T = 0: the first largest logit
+ *                alone; p = w / sum w
+ *   token of u   the first j with w_0 + ... + w_j > u sum w
+ *   acceptance   draft x, drawn from q, is kept iff q(x) <= 0 or u q(x) <= p(x)
+ *   rejection    the token is drawn from max(p - q, 0) (from p where that is 0
+ *                everywhere)
+ * Every decision is the one that 64-bit arithmetic takes.  Temperatures below
+ * 2^-60 (but not 0) count as 2^-60, above 2^60 as 2^60; uniforms outside [0, 1]
+ * as the nearest of the two (NaN as 0).  A row that has no distribution (a NaN,
+ * a +inf, nothing above -inf, or a temperature that is negative or not finite)
+ * gives token -1 and probabilities 0.
+ *
+ * Calls keep no state: what they need beyond inputs and outputs is the
+ * workspace, whose contents need not be kept and which no two calls that may
+ * run at the same time (two graphs being replayed, say) can share.  They wait
+ * for nothing, allocate nothing and can be captured.  `stream` is the
+ * cudaStream_t (NULL = CUDA's default stream); all pointers are device memory
+ * of `device`.  Inputs and outputs do not overlap.  Messages:
+ * spec_last_error(NULL). */
+#define SPEC_BATCH_MAX_VOCAB (1 << 20)
+#define SPEC_BATCH_MAX_ROWS (1 << 20)
+typedef struct spec_batch_logits {
+  int device;
+  int vocab;                 /* columns of a row */
+  int dtype;                 /* 0 = bf16, 1 = f16, 2 = f32 */
+  float temperature;         /* of every row where temperatures is NULL */
+  const void* logits;        /* row r at r * row_stride elements */
+  int64_t row_stride;
+  int64_t n_rows;
+  const float* temperatures; /* [n_rows] or NULL */
+  const float* uniforms;     /* [n_rows] */
+  void* workspace;           /* 16-byte aligned */
+  int64_t workspace_bytes;   /* at least spec_batch_workspace_bytes */
+} spec_batch_logits;
+/* Workspace of a call over n_rows rows (a negated status on a bad shape). */
+int64_t spec_batch_workspace_bytes(int64_t n_rows, int vocab, int dtype);
+/* tokens_out[r]: the token of row r's uniform.  probs_out (may be NULL): row r
+ * of p, f32, at r * probs_stride: what spec_batch_verify takes as the
+ * distribution that a drafted token was drawn from. */
+int spec_batch_sample(const spec_batch_logits* l, float* probs_out, int64_t probs_stride, int32_t* tokens_out,
+                      void* stream);
+/* Drafted chains.  Sequence b has rows row_start[b] .. row_start[b + 1] - 1 (one
+ * more than its drafts, as spec_batched_logits returns them).  drafts[r] is the
+ * token that row r judges and row r of draft_probs (at r * probs_stride) the
+ * distribution it was drawn from; those of a sequence's last row are not read.
+ * Row r's uniform decides about drafts[r]; the token after a rejection takes the
+ * next row's, the token behind the last draft its own row's: the order in which
+ * spec_verify_rejection uses them.  A draft outside the vocabulary (-1, say)
+ * ends a sequence's drafts.  n_accepted[b]: drafts kept; next_token[b]: the
+ * token that follows them.  A row without a distribution ends the walk with
+ * next_token -1; a sequence whose rows are not within the batch, or that has
+ * none, gets 0 and -1. */
+int spec_batch_verify(const spec_batch_logits* l, int n_seqs, const int32_t* row_start, const int32_t* drafts,
+                      const float* draft_probs, int64_t probs_stride, int32_t* n_accepted, int32_t* next_token,
+                      void* stream);
+/* Draft trees (and chains) whose candidates were picked, not drawn: EAGLE's and
+ * Medusa's top-k, prompt lookup.  The token drawn at a node from p with its row's
+ * uniform leads to the node's first child that holds it; where none does, it is
+ * the token that follows.  So the tokens are distributed as the target's own
+ * samples.  Rows of sequence b as above, node i at row row_start[b] + i;
+ * tokens / parents [n_rows] as in spec_tree_logits (parents count within the
+ * sequence; node 0 is the root, its entries are not read; a parent comes before
+ * its children, others are never reached).  path[row_start[b] + j]: the j-th
+ * node of the accepted path, root first; every other row's path is -1.
+ * path_len[b] >= 1: its length, next_token[b] the token after it (-1: the row has no distribution).
+ * A sequence without sound rows gets 0 and -1. */
+int spec_batch_verify_tree(const spec_batch_logits* l, int n_seqs, const int32_t* row_start, const int32_t* tokens,
+                           const int32_t* parents, int32_t* path, int32_t* path_len, int32_t* next_token, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
