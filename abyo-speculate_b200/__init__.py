@@ -10,6 +10,7 @@ from ._lib import (CacheRollbackError, DeviceError, IoError, SamplingError, Spec
                    UnsupportedMethodError, LIB_PATH, MAX_ROWS, load)
 from .decoder import B200Decoder, QWeight, exchange_tp_handles  # noqa: F401
 from .kv4 import KV4Batch, KV4Cache, rope_tables  # noqa: F401
+from .lora import LoraBank, LoraPlan  # noqa: F401
 from .sampling import sample_rows, verify_drafts, verify_trees  # noqa: F401
 from .tree import DraftTree  # noqa: F401
 
@@ -17,4 +18,5 @@ __all__ = [
     "B200Decoder", "QWeight", "DraftTree", "SpecError", "SamplingError", "CacheRollbackError",
     "UnsupportedMethodError", "IoError", "DeviceError", "LIB_PATH", "MAX_ROWS", "load", "exchange_tp_handles",
     "KV4Cache", "KV4Batch", "rope_tables", "sample_rows", "verify_drafts", "verify_trees",
+    "LoraBank", "LoraPlan",
 ]

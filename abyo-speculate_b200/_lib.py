@@ -127,6 +127,29 @@ class BatchLogits(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
 
 
+class LoraBankDesc(ctypes.Structure):
+    """spec_lora_bank (include/spec_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("device", "n_adapters", "k", "n", "rank", "dtype")] + [
+        (n, ctypes.c_void_p) for n in ("a", "b")] + [
+        (n, ctypes.c_int64) for n in ("a_adapter_stride", "a_row_stride", "b_adapter_stride", "b_row_stride")] + [
+        (n, ctypes.c_void_p) for n in ("ranks", "scales")]
+
+
+class LoraPlanDesc(ctypes.Structure):
+    """spec_lora_plan (include/spec_b200.h)."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_units", "n_bare")] + [
+        ("device_copy", ctypes.c_void_p)]
+
+
+class LoraRows(ctypes.Structure):
+    """spec_lora_rows (include/spec_b200.h)."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("n_rows", ctypes.c_int64),
+                ("dtype", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
 # (name, restype, argtypes) of every function declared in include/spec_b200.h
 SIGNATURES = [
     ("spec_load_gguf", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(LoadOpts), ctypes.POINTER(ctypes.c_void_p)]),
@@ -235,6 +258,11 @@ SIGNATURES = [
      + [ctypes.c_void_p] * 3),
     ("spec_batch_verify_tree", ctypes.c_int,
      [ctypes.POINTER(BatchLogits), ctypes.c_int] + [ctypes.c_void_p] * 7),
+    ("spec_lora_plan_bytes", ctypes.c_int64, [ctypes.c_int64]),
+    ("spec_lora_plan_make", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(LoraPlanDesc)]),
+    ("spec_lora_apply", ctypes.c_int,
+     [ctypes.POINTER(LoraBankDesc), ctypes.POINTER(LoraPlanDesc)] + [ctypes.POINTER(LoraRows)] * 3 + [ctypes.c_void_p]),
 ]
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,54 +1,15 @@
-// Sampling and verification of a batch, and low-rank adapters: the C entry
-// points and the checks of their arguments.  No state is kept: what a call
+// Sampling and verification of a batch: the C entry points and the checks of
+// their arguments.  No state is kept: what a call
 // needs beyond its inputs is a workspace of the caller's.
-#include <limits.h>
-#include <stdio.h>
-
-#include "../../include/spec_b200.h"
 #include "batch.h"
-#include "model.h"
+#include "host_call.h"
 
 using namespace specb200;
 using namespace specb200::batch;
 
 namespace {
 
-int fail(int rc, const char* msg) {
-  set_thread_error(msg);
-  return rc;
-}
-template <class... A>
-int fail(int rc, const char* fmt, A... a) {
-  char msg[256];
-  snprintf(msg, sizeof msg, fmt, a...);
-  set_thread_error(msg);
-  return rc;
-}
-int fail_cuda(cudaError_t e, const char* what) {
-  cudaGetLastError();  // reported here: the next launch's check is not to find it
-  return fail(e == cudaErrorMemoryAllocation ? SPEC_ERR_OOM : SPEC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-// The call's device is current during a call; the caller's comes back.
-struct Current {
-  int prev = -1, device;
-  int rc = SPEC_OK;
-  Current(int d, const char* what) : device(d) {
-    cudaError_t e = cudaGetDevice(&prev);
-    if (e == cudaSuccess && prev != d) e = cudaSetDevice(d);
-    if (e != cudaSuccess) rc = fail_cuda(e, what);
-  }
-  ~Current() {
-    if (prev >= 0 && prev != device) cudaSetDevice(prev);
-  }
-  Current(const Current&) = delete;
-  Current& operator=(const Current&) = delete;
-};
-
-constexpr int64_t kMaxStride = INT64_C(1) << 40;
-
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
-bool misaligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
 
 int check_shape(const char* what, int64_t n_rows, int vocab, int dtype) {
   if (dtype < T_BF16 || dtype > T_F32) return fail(SPEC_ERR_INVALID, "%s: logits have type %d", what, dtype);
@@ -102,11 +63,6 @@ Rows to_rows(const spec_batch_logits* l) {
   r.path = nullptr;
   r.drawn = reinterpret_cast<int*>(w + up(cells * sizeof(float2)) + up(cells * sizeof(double)));
   return r;
-}
-
-// Multiprocessors of the current device.
-cudaError_t multiprocessors(int device, int* sms) {
-  return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
 }
 
 int verify(const char* what, const spec_batch_logits* l, VerifyParams& p, int32_t* path, bool trees, void* stream) {

@@ -1,0 +1,170 @@
+// Low-rank adapters of many requests: the plan of a step's rows, the C entry
+// points and the checks of their arguments.  No state is kept.
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "host_call.h"
+#include "lora.h"
+
+using namespace specb200;
+using namespace specb200::lora;
+
+namespace {
+
+constexpr int kPlanRows = 1 << 20;
+
+// Layout of a plan: units (narrow, then those without an adapter), then the rows in their order.
+int64_t plan_bytes(int64_t n_rows) { return n_rows * (int64_t)(sizeof(Unit) + sizeof(int)); }
+
+struct Matrix {
+  const char* name;
+  const void* ptr;
+  int64_t outer, row;  // strides
+};
+
+// Whether 8 elements from any multiple of 8 on are aligned 16-byte accesses.
+bool wide(const void* p, int64_t row, int64_t outer, int size) {
+  return !misaligned(p, 16) && row * size % 16 == 0 && outer * size % 16 == 0;
+}
+
+int check_plan_shape(const char* what, int64_t n_rows) {
+  if (n_rows < 0 || n_rows > kPlanRows) return fail(SPEC_ERR_INVALID, "%s: %lld rows, 0 to %d are taken", what, (long long)n_rows, kPlanRows);
+  return SPEC_OK;
+}
+
+int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapters, void* buf, spec_lora_plan* out) {
+  for (int i = 0; i < n_rows; ++i)
+    if (adapters[i] < -1 || adapters[i] >= n_adapters)
+      return fail(SPEC_ERR_INVALID, "%s: row %d has adapter %d of %d (-1: none)", what, i, adapters[i], n_adapters);
+  std::vector<int> order(n_rows);
+  for (int i = 0; i < n_rows; ++i) order[i] = i;
+  // By adapter, rows in their order; rows without one last.
+  std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return (unsigned)adapters[x] < (unsigned)adapters[y]; });
+  std::vector<Unit> units;
+  int with = 0;
+  for (int i = 0; i < n_rows;) {
+    int e = i;
+    const int a = adapters[order[i]];
+    while (e < n_rows && adapters[order[e]] == a) ++e;
+    for (int at = i; at < e; at += kNarrowRows) units.push_back(Unit{a, at, std::min(kNarrowRows, e - at), 0});
+    if (a >= 0) with = (int)units.size();
+    i = e;
+  }
+  uint8_t* b = static_cast<uint8_t*>(buf);
+  if (n_rows) {
+    memcpy(b, units.data(), units.size() * sizeof(Unit));
+    memcpy(b + (size_t)n_rows * sizeof(Unit), order.data(), (size_t)n_rows * sizeof(int));
+  }
+  *out = spec_lora_plan{};
+  out->n_rows = n_rows;
+  out->n_adapters = n_adapters;
+  out->n_units = with;
+  out->n_bare = (int)units.size() - with;
+  return SPEC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t spec_lora_plan_bytes(int64_t n_rows) {
+  const int rc = check_plan_shape("spec_lora_plan_bytes", n_rows);
+  return rc == SPEC_OK ? plan_bytes(n_rows) : -rc;
+}
+
+int spec_lora_plan_make(const int32_t* adapters, int n_rows, int n_adapters, void* buf, int64_t buf_bytes,
+                        spec_lora_plan* out) {
+  const char* what = "spec_lora_plan_make";
+  if (!out || (n_rows > 0 && (!adapters || !buf))) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
+  const int rc = check_plan_shape(what, n_rows);
+  if (rc != SPEC_OK) return rc;
+  if (n_adapters < 0) return fail(SPEC_ERR_INVALID, "%s: %d adapters", what, n_adapters);
+  if (buf_bytes < plan_bytes(n_rows))
+    return fail(SPEC_ERR_INVALID, "%s: a buffer of %lld bytes, %lld are needed", what, (long long)buf_bytes,
+                (long long)plan_bytes(n_rows));
+  try {
+    return make_plan(what, adapters, n_rows, n_adapters, buf, out);
+  } catch (const std::bad_alloc&) {
+    return fail(SPEC_ERR_OOM, "%s: out of host memory", what);
+  }
+}
+
+int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const spec_lora_rows* x, const spec_lora_rows* y,
+                    const spec_lora_rows* out, void* stream) {
+  const char* what = "spec_lora_apply";
+  if (!b || !plan || !x || !y || !out) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
+  if (b->dtype != T_BF16 && b->dtype != T_F16) return fail(SPEC_ERR_UNSUPPORTED, "%s: adapters of type %d (bf16 and f16 are built)", what, b->dtype);
+  if (b->k < 1 || b->n < 1 || b->k > (1 << 24) || b->n > (1 << 24) || b->n_adapters < 0)
+    return fail(SPEC_ERR_INVALID, "%s: %d adapters of %d to %d channels", what, b->n_adapters, b->k, b->n);
+  if (b->rank < 0 || b->rank > kMaxRank) return fail(SPEC_ERR_UNSUPPORTED, "%s: rank %d (up to %d is built)", what, b->rank, kMaxRank);
+  if (b->device < 0) return fail(SPEC_ERR_INVALID, "%s: device %d", what, b->device);
+  if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_units < 0 || plan->n_bare < 0 ||
+      plan->n_units + (int64_t)plan->n_bare > plan->n_rows)
+    return fail(SPEC_ERR_INVALID, "%s: not a plan", what);
+  if (plan->n_adapters > b->n_adapters)
+    return fail(SPEC_ERR_INVALID, "%s: a plan for %d adapters, the bank has %d", what, plan->n_adapters, b->n_adapters);
+  if (plan->n_rows == 0) return SPEC_OK;
+  if (!plan->device_copy || misaligned(plan->device_copy, 16))
+    return fail(SPEC_ERR_INVALID, "%s: the plan's copy on the device is missing or not aligned to 16 bytes", what);
+  for (const spec_lora_rows* r : {x, y, out}) {
+    const char* name = r == x ? "x" : r == y ? "y" : "out";
+    if (!r->ptr) return fail(SPEC_ERR_INVALID, "%s: %s has no data", what, name);
+    if (r->dtype != b->dtype && r->dtype != T_F32)
+      return fail(SPEC_ERR_UNSUPPORTED, "%s: %s has type %d (f32 and the adapters' type are built)", what, name, r->dtype);
+    if (r->n_rows < plan->n_rows)
+      return fail(SPEC_ERR_INVALID, "%s: %s has %lld rows, the plan %d", what, name, (long long)r->n_rows, plan->n_rows);
+    if (r->row_stride < 0 || r->row_stride > kMaxStride)
+      return fail(SPEC_ERR_INVALID, "%s: %s has rows %lld apart", what, name, (long long)r->row_stride);
+    if (misaligned(r->ptr, r->dtype == T_F32 ? 4 : 2))
+      return fail(SPEC_ERR_INVALID, "%s: %s is not aligned to its element size", what, name);
+  }
+  if (y->dtype != out->dtype) return fail(SPEC_ERR_INVALID, "%s: y and out have types %d and %d", what, y->dtype, out->dtype);
+  if (plan->n_rows > 1 && out->row_stride < b->n)
+    return fail(SPEC_ERR_INVALID, "%s: rows of out overlap (%lld apart, %d wide)", what, (long long)out->row_stride, b->n);
+  const bool in_place = y->ptr == out->ptr;
+  if (in_place && plan->n_rows > 1 && y->row_stride != out->row_stride)
+    return fail(SPEC_ERR_INVALID, "%s: y in place needs one row stride", what);
+  if (plan->n_units) {
+    if ((b->rank > 0 && (!b->a || !b->b)) || misaligned(b->a, 2) || misaligned(b->b, 2) || misaligned(b->ranks, 4) || misaligned(b->scales, 4))
+      return fail(SPEC_ERR_INVALID, "%s: a pointer of the bank is null or not aligned to its element size", what);
+    for (const int64_t s : {b->a_adapter_stride, b->a_row_stride, b->b_adapter_stride, b->b_row_stride})
+      if (s < 0 || s > kMaxStride) return fail(SPEC_ERR_INVALID, "%s: a stride of the bank is outside [0, 2^40]", what);
+  }
+  Current cur(b->device, what);
+  if (cur.rc != SPEC_OK) return cur.rc;
+  Params p{};
+  p.a = b->a;
+  p.b = b->b;
+  p.a_adapter = b->a_adapter_stride;
+  p.a_row = b->a_row_stride;
+  p.b_adapter = b->b_adapter_stride;
+  p.b_row = b->b_row_stride;
+  p.ranks = b->ranks;
+  p.scales = b->scales;
+  p.x = x->ptr;
+  p.y = y->ptr;
+  p.out = out->ptr;
+  p.x_row = x->row_stride;
+  p.y_row = y->row_stride;
+  p.out_row = out->row_stride;
+  p.units = static_cast<const Unit*>(plan->device_copy);
+  p.order = reinterpret_cast<const int*>(p.units + plan->n_rows);
+  p.K = b->k;
+  p.N = b->n;
+  p.rank = b->rank;
+  p.a_wide = wide(b->a, b->a_row_stride, b->a_adapter_stride, 2);
+  p.b_wide = wide(b->b, b->b_row_stride, b->b_adapter_stride, 2);
+  p.x_wide = wide(x->ptr, x->row_stride, 0, x->dtype == T_F32 ? 4 : 2);
+  int sms = 0;
+  cudaError_t e = multiprocessors(b->device, &sms);
+  const int n = plan->n_units + (in_place ? 0 : plan->n_bare);
+  int size = 8;
+  while (size > 1 && (int64_t)n * size > (int64_t)sms * 4) size /= 2;
+  if (e == cudaSuccess) e = launch(p, b->dtype, x->dtype == T_F32, y->dtype == T_F32, n, size, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
+}
+
+}  // extern "C"

@@ -1,0 +1,40 @@
+// Low-rank adapters of many requests: what the host entry points (lora.cpp)
+// and the kernels (lora.cu) share.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace specb200 {
+namespace lora {
+
+enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
+
+constexpr int kMaxRank = 256;
+constexpr int kNarrowRows = 8;  // rows of a unit: one n-tile of the products
+
+// Rows of one adapter (-1: none) that one cluster takes.
+struct Unit {
+  int adapter, first, n_rows, pad;  // rows order[first ..]
+};
+
+struct Params {
+  const void *a, *b;  // of the adapters' type
+  long long a_adapter, a_row, b_adapter, b_row;  // strides in elements
+  const int* ranks;      // or null: all `rank`
+  const float* scales;   // or null: 1
+  const void* x;
+  const void* y;
+  void* out;
+  long long x_row, y_row, out_row;
+  const Unit* units;
+  const int* order;
+  int K, N, rank;
+  int a_wide, b_wide, x_wide;  // 8 consecutive elements from a multiple of 8 on are aligned 16-byte accesses
+};
+
+// n_units units on clusters of `size` blocks.
+cudaError_t launch(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
+
+}  // namespace lora
+}  // namespace specb200

@@ -1,0 +1,127 @@
+"""Low-rank adapters of many requests over torch tensors: the host side of spec_lora_* (include/spec_b200.h).
+
+    bank = LoraBank(a, b, ranks=..., scales=...)     # of one projection: a [adapters, rank, k], b [adapters, n, rank]
+    plan = LoraPlan(adapter_of_each_row, n_adapters)  # once per step, for all projections and layers
+    w.matmul(x.data_ptr(), rows, y.data_ptr(), stream)  # the shared projection
+    bank.apply(plan, x, y)                            # y += scale (x A^T) B^T
+
+Calls are queued on torch's current stream of the bank's device and return
+without waiting for it.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import numpy as np
+
+from . import _lib
+from .kv4 import _host
+
+
+def _invalid(msg: str) -> _lib.SamplingError:
+    return _lib.SamplingError(_lib.SPEC_ERR_INVALID, msg)
+
+
+class LoraPlan:
+    """Which adapter each row of a step has (spec_lora_plan_make).
+
+    adapters: one whole number a row, -1 for a row without an adapter; rows of
+    one adapter need not be neighbours.  The plan does not change: a captured
+    call replays with it as long as it lives."""
+
+    def __init__(self, adapters, n_adapters: int, device="cuda"):
+        import torch
+        lib = _lib.load()
+        ids = _host(adapters, np.int32, "adapters")
+        self.n_rows, self.n_adapters = int(ids.size), int(n_adapters)
+        size = lib.spec_lora_plan_bytes(self.n_rows)
+        if size < 0:
+            _lib.check(-size)
+        buf = np.empty(max(size, 1), np.uint8)
+        self._desc = _lib.LoraPlanDesc()
+        _lib.check(lib.spec_lora_plan_make(ids.ctypes.data, self.n_rows, self.n_adapters, buf.ctypes.data, size,
+                                           ctypes.byref(self._desc)))
+        self._copy = torch.from_numpy(buf).to(device)
+        self.device = self._copy.device
+        if not self._copy.is_cuda:
+            raise _invalid(f"a plan on {self.device}: a CUDA device is needed")
+        self._desc.device_copy = self._copy.data_ptr()
+        self._made_on = torch.cuda.current_stream(self.device).cuda_stream
+
+
+class LoraBank:
+    """The adapters of one projection (spec_lora_bank).
+
+    a [adapters, rank, k] and b [adapters, n, rank]: bfloat16 or float16 CUDA
+    tensors with contiguous rows, kept as they are.  ranks: adapters' own ranks
+    (the rest of their a and b is not read), whole numbers or an int32 tensor
+    on the device; scales: numbers or a float32 tensor on the device."""
+
+    def __init__(self, a, b, ranks=None, scales=None):
+        import torch
+        self._lib = _lib.load()
+        types = {torch.bfloat16: 0, torch.float16: 1}
+        if not all(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 for t in (a, b)):
+            raise _invalid("a and b are not CUDA tensors of three dimensions")
+        if a.dtype not in types or b.dtype != a.dtype or a.device != b.device:
+            raise _invalid(f"a is {a.dtype} on {a.device}, b {b.dtype} on {b.device}: both bfloat16 or float16 on one device")
+        n, r, k = a.shape
+        if b.shape[0] != n or b.shape[2] != r:
+            raise _invalid(f"a has shape {tuple(a.shape)}, b {tuple(b.shape)}: [adapters, rank, k] and [adapters, n, rank]")
+        for t, what in ((a, "a"), (b, "b")):
+            if t.shape[2] > 1 and t.stride(2) != 1:
+                raise _invalid(f"the rows of {what} are not contiguous")
+        self.device, self.n_adapters, self.rank, self.k, self.n = a.device, n, r, k, b.shape[1]
+        if ranks is not None and not isinstance(ranks, torch.Tensor):
+            host = _host(ranks, np.int32, "ranks", n)
+            if host.size and (host.min() < 0 or host.max() > r):
+                raise _invalid(f"ranks from {host.min()} to {host.max()}, 0 to {r} are taken")
+            ranks = torch.from_numpy(host.copy()).to(self.device)
+        if scales is not None and not isinstance(scales, torch.Tensor):
+            scales = torch.tensor([float(s) for s in scales], dtype=torch.float32, device=self.device)
+        for t, dtype, what in ((ranks, torch.int32, "ranks"), (scales, torch.float32, "scales")):
+            if t is not None and not (t.dtype == dtype and t.device == self.device and tuple(t.shape) == (n,) and
+                                      t.is_contiguous()):
+                raise _invalid(f"{what} is not a contiguous {dtype} tensor [{n}] on {self.device}")
+        self._keep = (a, b, ranks, scales)
+        self._made_on = torch.cuda.current_stream(self.device).cuda_stream
+        self._types = {a.dtype: types[a.dtype], torch.float32: 2}
+        self._desc = _lib.LoraBankDesc(
+            a.device.index, n, k, self.n, r, types[a.dtype], a.data_ptr(), b.data_ptr(), a.stride(0), a.stride(1),
+            b.stride(0), b.stride(1), ranks.data_ptr() if ranks is not None else None,
+            scales.data_ptr() if scales is not None else None)
+
+    def _rows(self, t, width: int, what: str) -> _lib.LoraRows:
+        import torch
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise _invalid(f"{what} is not a tensor on {self.device}")
+        if t.dim() != 2 or t.shape[1] != width:
+            raise _invalid(f"{what} has shape {tuple(t.shape)}, [rows, {width}] is needed")
+        if t.dtype not in self._types:
+            raise _invalid(f"{what} is {t.dtype}: float32 and the adapters' type are taken")
+        if width > 1 and t.stride(1) != 1:
+            raise _invalid(f"the rows of {what} are not contiguous")
+        return _lib.LoraRows(t.data_ptr(), t.stride(0), t.shape[0], self._types[t.dtype], 0)
+
+    def apply(self, plan: LoraPlan, x, y, out=None):
+        """out = y + scale (x A^T) B^T, each row with its own adapter; x [rows, k],
+        y and out [rows, n] (out None: y itself).  Returns out."""
+        import torch
+        if plan.device != self.device:
+            raise _invalid(f"the plan is on {plan.device}, the bank on {self.device}")
+        if out is None:
+            out = y
+        rx, ry, ro = self._rows(x, self.k, "x"), self._rows(y, self.n, "y"), self._rows(out, self.n, "out")
+        stream = torch.cuda.current_stream(self.device)
+        _lib.check(self._lib.spec_lora_apply(ctypes.byref(self._desc), ctypes.byref(plan._desc), ctypes.byref(rx),
+                                             ctypes.byref(ry), ctypes.byref(ro), stream.cuda_stream))
+        # Memory of a plan or bank that is dropped is not handed out before this stream is done with it.
+        if stream.cuda_stream != plan._made_on:
+            plan._copy.record_stream(stream)
+        if stream.cuda_stream != self._made_on:
+            for t in self._keep:
+                if t is not None:
+                    t.record_stream(stream)
+        return out

@@ -698,6 +698,54 @@ int spec_batch_verify(const spec_batch_logits* l, int n_seqs, const int32_t* row
 int spec_batch_verify_tree(const spec_batch_logits* l, int n_seqs, const int32_t* row_start, const int32_t* tokens,
                            const int32_t* parents, int32_t* path, int32_t* path_len, int32_t* next_token, void* stream);
 
+/* ---- low-rank adapters of many requests -----------------------------------------
+ * No counterpart in the reference.  Beside a projection that all requests share
+ * (spec_qmatmul, say), each row's own adapter:
+ *   out = y + scale (x A^T) B^T,   A [rank x k], B [n x rank]
+ * A bank holds the adapters of one projection in caller-owned device memory, a
+ * plan says which adapter each row of a step has (once per step, for all
+ * projections and layers).  Sums and x A^T are f32 (the latter is split into
+ * parts of 16 bits in all or more for the second product), each result is
+ * rounded once.  Calls keep no state, wait for nothing, allocate nothing and can
+ * be captured.  Pointers are device memory of `device` unless said otherwise. */
+typedef struct spec_lora_bank {
+  int device;
+  int n_adapters;
+  int k, n;                    /* channels of x and y */
+  int rank;                    /* rows of every A, columns of every B: at most 256 */
+  int dtype;                   /* of A and B: 0 = bf16, 1 = f16 */
+  const void *a, *b;           /* element (adapter, row, column) at adapter * adapter_stride + row * row_stride + column */
+  int64_t a_adapter_stride, a_row_stride;
+  int64_t b_adapter_stride, b_row_stride;
+  const int32_t* ranks;        /* [n_adapters]: an adapter's own rank (the rest of its A and B is not read), or NULL */
+  const float* scales;         /* [n_adapters], or NULL: 1 */
+} spec_lora_bank;
+/* Rows of a step by adapter.  adapters: host, n_rows numbers of 0 .. n_adapters
+ * - 1, or -1 for a row without one; rows of one adapter need not be neighbours,
+ * and are taken together.  Writes the plan to buf (host, spec_lora_plan_bytes)
+ * and fills *out but for device_copy: the caller copies buf to the device, sets
+ * it, and keeps both unchanged until the calls that use them are done. */
+typedef struct spec_lora_plan {
+  int n_rows, n_adapters, n_units, n_bare;
+  const void* device_copy;     /* 16-byte aligned */
+} spec_lora_plan;
+int64_t spec_lora_plan_bytes(int64_t n_rows);
+int spec_lora_plan_make(const int32_t* adapters, int n_rows, int n_adapters, void* buf, int64_t buf_bytes,
+                        spec_lora_plan* out);
+/* Rows on the device: row r at r * row_stride elements.  Types: the bank's, or
+ * 2 = f32. */
+typedef struct spec_lora_rows {
+  void* ptr;
+  int64_t row_stride, n_rows;
+  int dtype;
+  int reserved;
+} spec_lora_rows;
+/* y and out have one type; out may be y itself (same row stride), or overlaps
+ * neither x nor y.  Rows without an adapter are copied (in place: not touched),
+ * rows behind the plan's last one are left as they are. */
+int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const spec_lora_rows* x, const spec_lora_rows* y,
+                    const spec_lora_rows* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

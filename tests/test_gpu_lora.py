@@ -1,0 +1,287 @@
+"""Low-rank adapters of many requests on the GPU against float64.
+
+Tolerances, with u = 2^-24, |.| sums of magnitudes: t = x A^T has f32 sums of k
+terms, taken by the tensor core in blocks of 8 or 16, which may drop what lies
+below 2^-23 of the running sum at every step: |dt| <= 2^-23 (k / 8 + 32) |x| |A|
+(operands exact, or f32 rows as two tf32 numbers, 2^-24 more).  The second
+product likewise over the rank, t split into parts that leave 2^-22 of the
+row's largest (f16), 2^-16 (bf16 for a bf16 result) or 2^-24 (bf16 for f32).  The
+result is rounded once to its type.  The bound is the worst case, so the norm
+of the error is checked too, against a sixteenth of it."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+EPS = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
+
+
+def kinds():
+    import torch
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def dev(x, dtype):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x, np.float32)).cuda().to(kinds()[dtype])
+
+
+class Case:
+    """A bank, rows and their adapters; views into wider memory where `pad` says so."""
+
+    def __init__(self, pkg, ids, n_adapters, k, n, rank, dtype="bf16", x="same", y="same", ranks=None, scaled=True, seed=0,
+                 pad=(0, 0, 0, 0)):
+        import torch
+        rng = np.random.default_rng(seed)
+        self.pkg, self.ids, self.dtype = pkg, np.asarray(ids), dtype
+        self.xt, self.yt = (dtype if x == "same" else "f32"), (dtype if y == "same" else "f32")
+        rows = len(ids)
+
+        def view(a, kind, extra):
+            t = torch.full((*a.shape[:-1], a.shape[-1] + extra), float("nan"), dtype=kinds()[kind], device="cuda")
+            t[..., :a.shape[-1]] = dev(a, kind)
+            return t[..., :a.shape[-1]]
+
+        self.a = view(rng.standard_normal((n_adapters, rank, k)) / np.sqrt(k), dtype, pad[0])
+        self.b = view(rng.standard_normal((n_adapters, n, rank)), dtype, pad[1])
+        self.x = view(rng.standard_normal((rows, k)) * (1 + 6 * (rng.random((1, k)) < 0.02)), self.xt, pad[2])
+        self.y = view(rng.standard_normal((rows, n)), self.yt, pad[3])
+        self.ranks = ranks
+        self.scales = rng.uniform(0.25, 2, n_adapters).astype(np.float32) if scaled else None
+        if ranks is not None:  # what lies behind an adapter's rank is not read
+            for i, r in enumerate(ranks):
+                self.a[i, r:] = float("nan")
+                self.b[i, :, r:] = float("nan")
+        self.bank = pkg.LoraBank(self.a, self.b, ranks=ranks, scales=self.scales)
+        self.plan = pkg.LoraPlan(self.ids.astype(np.int32), n_adapters)
+
+    def exact(self):
+        """The result and the bound of its error, in float64."""
+        a, b, x, y = (t.double().cpu().numpy() for t in (self.a, self.b, self.x, self.y))
+        want, bound = y.copy(), np.zeros_like(y)
+        for i in np.unique(self.ids):
+            if i < 0:
+                continue
+            at = np.flatnonzero(self.ids == i)
+            r = a.shape[1] if self.ranks is None else self.ranks[i]
+            s = 1.0 if self.scales is None else float(self.scales[i])
+            A, B = a[i, :r], b[i, :, :r]
+            t = s * (x[at] @ A.T)
+            want[at] += t @ B.T
+            if not r:
+                continue
+            dt = s * (np.abs(x[at]) @ np.abs(A).T) * (2.0 ** -23 * (a.shape[2] / 8 + 32) + 2.0 ** -23) + np.abs(t) * 2.0 ** -22
+            split = 2.0 ** -22 if self.dtype == "f16" else 2.0 ** -16 if self.yt == "bf16" else 2.0 ** -23
+            dt += split * (np.abs(t).max(1, keepdims=True) if self.dtype == "f16" else np.abs(t))
+            bound[at] = dt @ np.abs(B).T + 2.0 ** -23 * (r / 8 + 16) * (np.abs(t) @ np.abs(B).T)
+        return want, bound
+
+    def check(self, out=None):
+        import torch
+        want, bound = self.exact()
+        keep = self.y.clone()
+        got = self.bank.apply(self.plan, self.x, self.y, out=out)
+        assert got is (self.y if out is None else out)
+        if out is not None:
+            assert torch.equal(self.y, keep)
+        g = got[:len(self.ids)].double().cpu().numpy()
+        half = EPS[self.yt] * (np.abs(want) + bound) + (2.0 ** -25 if self.yt == "f16" else 0)
+        assert (np.abs(g - want) <= bound + half).all()
+        none = self.ids < 0
+        assert torch.equal(got[:len(self.ids)][torch.from_numpy(none).cuda()], keep[torch.from_numpy(none).cuda()])
+        assert np.linalg.norm(g - want) <= np.linalg.norm(bound) / 16 + np.linalg.norm(half)
+        return g
+
+
+TYPES = [("bf16", "same", "same"), ("bf16", "f32", "f32"), ("bf16", "same", "f32"), ("bf16", "f32", "same"),
+         ("f16", "same", "same"), ("f16", "f32", "f32"), ("f16", "same", "f32"), ("f16", "f32", "same")]
+
+
+def mixed(rows, adapters, seed=0, none=0.1):
+    rng = np.random.default_rng(seed)
+    ids = rng.integers(0, adapters, rows)
+    ids[rng.random(rows) < none] = -1
+    return ids
+
+
+@pytest.mark.parametrize("dtype,x,y", TYPES)
+@pytest.mark.parametrize("rows,adapters,k,n,rank", [(1, 1, 64, 48, 8), (1, 2, 4096, 4096, 16), (64, 64, 896, 1152, 16),
+                                                    (37, 5, 1000, 333, 24), (130, 3, 257, 1025, 64), (300, 2, 512, 2048, 32),
+                                                    (9, 1, 33, 17, 5), (70, 4, 128, 128, 128), (20, 2, 640, 96, 256)])
+def test_sizes_and_types(pkg, rows, adapters, k, n, rank, dtype, x, y):
+    import torch
+    ids = mixed(rows, adapters, seed=rows) if rows > 1 else [adapters - 1]
+    c = Case(pkg, ids, adapters, k, n, rank, dtype, x, y, seed=k)
+    c.check(out=torch.empty_like(c.y))
+    c.check()
+
+
+@pytest.mark.parametrize("rank", [1, 2, 3, 7, 8, 9, 15, 16, 17, 31, 33, 48, 63, 65, 100, 129, 200])
+def test_ranks(pkg, rank):
+    Case(pkg, mixed(40, 3, seed=rank), 3, 320, 272, rank, seed=rank).check()
+
+
+@pytest.mark.parametrize("dtype,x,y", TYPES)
+def test_adapters_of_their_own_ranks(pkg, dtype, x, y):
+    """Every rank from 0 to the bank's; NaN behind each adapter's own."""
+    ranks = [0, 1, 5, 8, 13, 16, 24, 31, 32, 0, 3]
+    c = Case(pkg, mixed(120, len(ranks), seed=2), len(ranks), 500, 700, 32, dtype, x, y, ranks=ranks)
+    import torch
+    c.check(out=torch.full_like(c.y, float("nan")))
+
+
+@pytest.mark.parametrize("pad", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (8, 8, 8, 8), (4, 4, 4, 4), (3, 5, 7, 9)])
+@pytest.mark.parametrize("dtype,x,y", [("bf16", "same", "same"), ("f16", "f32", "f32")])
+def test_strides(pkg, pad, dtype, x, y):
+    import torch
+    for rows in (11, 150):
+        c = Case(pkg, mixed(rows, 3, seed=4), 3, 264, 200, 24, dtype, x, y, pad=pad, seed=5)
+        wide = torch.full((rows + 2, 200 + 6), -7.0, dtype=c.y.dtype, device="cuda")
+        c.check(out=wide[:rows, 2:202])
+        assert (wide[:, :2] == -7).all() and (wide[:, 202:] == -7).all() and (wide[rows:] == -7).all()
+
+
+def test_expanded_inputs(pkg):
+    """Rows and adapters that share memory, where they are only read."""
+    import torch
+    c = Case(pkg, mixed(30, 4, seed=1), 4, 256, 128, 16)
+    c.x = c.x[:1].expand(30, 256)
+    c.a = c.a[:1].expand(4, 16, 256)
+    c.y = c.y[:1].expand(30, 128)
+    c.bank = pkg.LoraBank(c.a, c.b, scales=c.scales)
+    c.check(out=torch.empty(30, 128, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(pkg.SamplingError):
+        c.bank.apply(c.plan, c.x, c.y)  # rows of the result on one another
+
+
+@pytest.mark.parametrize("counts", [[1], [8], [9], [16], [17], [64], [65], [127], [128], [129], [500, 1, 40], [2000, 3]])
+def test_rows_of_one_adapter(pkg, counts):
+    ids = np.concatenate([np.full(c, i) for i, c in enumerate(counts)])
+    np.random.default_rng(0).shuffle(ids)
+    for dtype, x, y in TYPES[:2]:
+        Case(pkg, ids, len(counts), 288, 352, 16, dtype, x, y, seed=len(ids)).check()
+
+
+def test_long_sums(pkg):
+    for rows in (3, 100):
+        Case(pkg, [0] * rows, 1, 18944, 3584, 16, "bf16", seed=1).check()
+        Case(pkg, [0] * rows, 1, 18944, 256, 64, "f16", "f32", "f32", seed=2).check()
+
+
+def test_many_rows_of_many_adapters(pkg):
+    Case(pkg, mixed(3000, 70, seed=3, none=0.3), 70, 128, 160, 8, seed=3).check()
+
+
+def test_rows_behind_the_plan_are_left(pkg):
+    import torch
+    c = Case(pkg, mixed(20, 2, seed=6), 2, 96, 80, 8)
+    x = torch.cat([c.x, torch.full((5, 96), float("nan"), device="cuda", dtype=c.x.dtype)])
+    y = torch.cat([c.y, torch.full((5, 80), 3.0, device="cuda", dtype=c.y.dtype)])
+    c.x, c.y = x, y
+    c.bank.apply(c.plan, x, y)
+    assert (y[20:] == 3).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("scale", [1e-6, 1e-3, 1e4])
+def test_small_and_large_values(pkg, dtype, scale):
+    """f32 rows of any size: t is split relative to its row's largest value."""
+    for rows in (4, 90):
+        c = Case(pkg, [0] * rows, 1, 512, 256, 16, dtype, "f32", "f32", seed=7)
+        c.x.mul_(scale)
+        c.y.mul_(scale)
+        c.check()
+
+
+@pytest.mark.parametrize("rows", [5, 80])
+@pytest.mark.parametrize("dtype,x,y", [("bf16", "same", "same"), ("f16", "same", "same"), ("bf16", "f32", "f32")])
+def test_a_bad_row_stays_alone(pkg, rows, dtype, x, y):
+    """NaN and infinities of one row reach that row only."""
+    import torch
+    c = Case(pkg, [0] * rows, 1, 256, 192, 16, dtype, x, y, seed=8)
+    good = torch.empty_like(c.y)
+    c.bank.apply(c.plan, c.x, c.y, out=good)
+    c.x[2, 17] = float("nan")
+    c.x[3, 5] = float("inf")
+    got = torch.empty_like(c.y)
+    c.bank.apply(c.plan, c.x, c.y, out=got)
+    rest = [i for i in range(rows) if i not in (2, 3)]
+    assert torch.equal(got[rest], good[rest])
+    assert got[2].isnan().all() and not got[3].isfinite().any()
+
+
+def test_far_strides(pkg):
+    """Offsets past 32 bits in the bank and the rows."""
+    import torch
+    c = Case(pkg, [2, 0, 1, 2], 3, 64, 40, 8)
+    far = torch.empty(3, (1 << 31) + 8, dtype=torch.bfloat16, device="cuda")
+    a = far[:, :8 * 64].view(3, 8, 64)
+    a.copy_(c.a)
+    c.a, c.bank = a, pkg.LoraBank(a, c.b, scales=c.scales)
+    c.check(out=torch.empty_like(c.y))
+    far_x = torch.empty(4, 1 << 30, dtype=torch.bfloat16, device="cuda")
+    far_x[:, :64] = c.x
+    c.x = far_x[:, :64]
+    c.check()
+    del far, far_x, a
+    c.a = c.x = c.bank = None
+    torch.cuda.empty_cache()
+
+
+def test_the_result_does_not_depend_on_other_adapters(pkg):
+    """Rows of an adapter give the same bits with and without other requests in the step."""
+    import torch
+    c = Case(pkg, [0] * 5 + [1] * 40, 2, 512, 384, 16, seed=9)
+    both = torch.empty_like(c.y)
+    c.bank.apply(c.plan, c.x, c.y, out=both)
+    again = torch.empty_like(c.y)
+    c.bank.apply(c.plan, c.x, c.y, out=again)
+    assert torch.equal(both, again)
+
+
+def test_capture_and_other_streams(pkg):
+    import torch
+    c = Case(pkg, mixed(50, 4, seed=2), 4, 300, 400, 16, seed=10)
+    out = torch.empty_like(c.y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.bank.apply(c.plan, c.x, c.y, out=out)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.bank.apply(c.plan, c.x, c.y, out=out)
+    for seed in range(2):
+        c.x.copy_(torch.randn_like(c.x))
+        c.y.copy_(torch.randn_like(c.y))
+        eager = c.bank.apply(c.plan, c.x, c.y, out=torch.empty_like(c.y))
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, out)
+
+
+def test_refusals(pkg):
+    import torch
+    c = Case(pkg, [0, 1, -1], 2, 64, 32, 8)
+    a, b, x, y, plan = c.a, c.b, c.x, c.y, c.plan
+    bad = [lambda: pkg.LoraBank(a, b.half()), lambda: pkg.LoraBank(a.float(), b.float()), lambda: pkg.LoraBank(a[:1], b),
+           lambda: pkg.LoraBank(a, b[..., :4]), lambda: pkg.LoraBank(a[0], b), lambda: pkg.LoraBank(a.transpose(1, 2), b),
+           lambda: pkg.LoraBank(a, b, ranks=[1]), lambda: pkg.LoraBank(a, b, ranks=[1, 9]), lambda: pkg.LoraBank(a, b, ranks=[-1, 2]),
+           lambda: pkg.LoraBank(a, b, ranks=[1.5, 2]), lambda: pkg.LoraBank(a, b, scales=[1.0]),
+           lambda: pkg.LoraBank(a, b, scales=torch.ones(2)), lambda: pkg.LoraPlan([2], 2), lambda: pkg.LoraPlan([-2], 2),
+           lambda: c.bank.apply(plan, x[:2], y), lambda: c.bank.apply(plan, x, y[:, :31]), lambda: c.bank.apply(plan, x.half(), y),
+           lambda: c.bank.apply(plan, x, y, out=y.float()), lambda: c.bank.apply(plan, x.T, y),
+           lambda: c.bank.apply(plan, x.cpu(), y), lambda: c.bank.apply(pkg.LoraPlan([0], 3), x, y),
+           lambda: c.bank.apply(plan, x, y, out=torch.empty(3, 64, device="cuda", dtype=y.dtype)[:, ::2])]
+    for call in bad:
+        with pytest.raises(pkg.SpecError):
+            call()
+    with pytest.raises(pkg.UnsupportedMethodError):
+        pkg.LoraBank(torch.zeros(1, 300, 8, device="cuda").half(), torch.zeros(1, 8, 300, device="cuda").half()).apply(
+            pkg.LoraPlan([0], 1), torch.zeros(1, 8, device="cuda"), torch.zeros(1, 8, device="cuda"))
+    keep = y.clone()
+    c.bank.apply(pkg.LoraPlan([], 2), x[:0], y[:0])
+    c.bank.apply(pkg.LoraPlan([-1] * 3, 2), x, y)
+    assert torch.equal(y, keep)

@@ -1,0 +1,106 @@
+"""Low-rank adapters, what needs no GPU: plans and refusals, which come before any CUDA call."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+P = 1 << 20  # a pointer that nothing follows
+
+
+@pytest.fixture(scope="module")
+def mod():
+    from importlib import import_module
+    return import_module("abyo-speculate_b200._lib")
+
+
+def make(mod, ids, n_adapters):
+    lib = mod.load()
+    ids = np.asarray(ids, np.int32)
+    buf = np.zeros(max(1, lib.spec_lora_plan_bytes(ids.size)), np.uint8)
+    plan = mod.LoraPlanDesc()
+    rc = lib.spec_lora_plan_make(ids.ctypes.data, ids.size, n_adapters, buf.ctypes.data, buf.size, ctypes.byref(plan))
+    return rc, plan, buf
+
+
+@pytest.mark.parametrize("n,adapters,seed", [(1, 1, 0), (7, 3, 1), (64, 64, 2), (300, 2, 3), (2000, 5, 4), (40, 1, 5)])
+def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
+    rng = np.random.default_rng(seed)
+    ids = rng.integers(-1, adapters, n)
+    rc, plan, buf = make(mod, ids, adapters)
+    assert rc == 0 and plan.n_rows == n and plan.n_adapters == adapters
+    units = buf[:16 * (plan.n_units + plan.n_bare)].view(np.int32).reshape(-1, 4)
+    order = buf[16 * n:].view(np.int32)
+    seen = []
+    for i, (a, first, count, _) in enumerate(units):
+        assert count > 0 and (a >= 0) == (i < plan.n_units)
+        rows = order[first:first + count]
+        assert (ids[rows] == a).all()
+        seen += rows.tolist()
+    assert sorted(seen) == list(range(n))
+
+
+def test_empty_plans(mod):
+    rc, plan, _ = make(mod, [], 3)
+    assert rc == 0 and plan.n_units == plan.n_bare == 0
+    rc, plan, _ = make(mod, [-1, -1], 0)
+    assert rc == 0 and plan.n_units == 0 and plan.n_bare == 1
+
+
+def test_bad_plans_are_refused(mod):
+    lib = mod.load()
+    assert make(mod, [0, 3], 3)[0] == 1 and make(mod, [-2], 3)[0] == 1 and make(mod, [0], -1)[0] == 1
+    assert lib.spec_lora_plan_bytes(-1) == -1 and lib.spec_lora_plan_bytes(1 << 21) == -1
+    ids, buf, plan = np.zeros(4, np.int32), np.zeros(100, np.uint8), mod.LoraPlanDesc()
+    args = [ids.ctypes.data, 4, 1, buf.ctypes.data, 100, ctypes.byref(plan)]
+    assert lib.spec_lora_plan_make(*args) == 0
+    for at, bad in ((0, None), (1, -1), (3, None), (4, 79), (5, None)):
+        assert lib.spec_lora_plan_make(*args[:at], bad, *args[at + 1:]) == 1
+
+
+def test_bad_calls_are_refused(mod):
+    lib = mod.load()
+
+    def call(bank=(), plan=(), x=(), y=(), out=()):
+        b = dict(device=0, n_adapters=2, k=64, n=32, rank=8, dtype=0, a=P, b=P, a_adapter_stride=512, a_row_stride=64,
+                 b_adapter_stride=256, b_row_stride=8, ranks=None, scales=None)
+        p = dict(n_rows=3, n_adapters=2, n_units=1, n_bare=1, device_copy=P)
+        r = [dict(ptr=P, row_stride=64, n_rows=3, dtype=0, reserved=0), dict(ptr=P, row_stride=32, n_rows=3, dtype=0, reserved=0),
+             dict(ptr=P + 4096, row_stride=32, n_rows=3, dtype=0, reserved=0)]
+        b.update(bank), p.update(plan)
+        for d, change in zip(r, (x, y, out)):
+            d.update(change)
+        rows = [ctypes.byref(mod.LoraRows(**d)) for d in r]
+        return lib.spec_lora_apply(ctypes.byref(mod.LoraBankDesc(**b)), ctypes.byref(mod.LoraPlanDesc(**p)), *rows, None)
+
+    for change in (dict(k=0), dict(n=0), dict(k=1 << 25), dict(device=-1), dict(n_adapters=-1), dict(n_adapters=1), dict(a=None),
+                   dict(b=None), dict(a=P + 1), dict(ranks=P + 2), dict(scales=P + 1), dict(a_row_stride=-1),
+                   dict(b_adapter_stride=1 << 41)):
+        assert call(bank=change) == 1, change
+    for change in (dict(dtype=2), dict(dtype=-1), dict(rank=257), dict(rank=-1)):
+        assert call(bank=change) == 3, change
+    for change in (dict(n_rows=-1), dict(n_units=-1), dict(n_units=3), dict(device_copy=None), dict(device_copy=P + 8),
+                   dict(n_rows=(1 << 20) + 1)):
+        assert call(plan=change) == 1, change
+    for which in ("x", "y", "out"):
+        for change in (dict(ptr=None), dict(ptr=P + 1), dict(n_rows=2), dict(row_stride=-1), dict(row_stride=1 << 41)):
+            assert call(**{which: change}) == 1, (which, change)
+        assert call(**{which: dict(dtype=1)}) == 3
+    assert call(y=dict(dtype=2)) == 1                                # y and out of two types
+    assert call(out=dict(row_stride=31)) == 1                        # rows that overlap
+    assert call(out=dict(ptr=P, row_stride=40)) == 1                 # in place, two strides
+    assert lib.spec_lora_apply(None, None, None, None, None, None) == 1
+    assert call(plan=dict(n_rows=0, n_units=0, n_bare=0)) == 0       # nothing to do
+
+
+def test_python_refuses_host_tensors(pkg):
+    import torch
+    a, b = torch.zeros(2, 4, 8, dtype=torch.bfloat16), torch.zeros(2, 6, 4, dtype=torch.bfloat16)
+    with pytest.raises(pkg.SamplingError):
+        pkg.LoraBank(a, b)
+    with pytest.raises(pkg.SamplingError):
+        pkg.LoraPlan([0, 1], 2, device="cpu")
+    with pytest.raises(pkg.SamplingError):
+        pkg.LoraPlan([0, 2], 2, device="cpu")
+    with pytest.raises(pkg.SamplingError):
+        pkg.LoraPlan([0.5], 2, device="cpu")
