@@ -252,17 +252,17 @@ SIGNATURES = [
     ("spec_kv4_status", ctypes.c_int, [ctypes.c_void_p]),
     ("spec_batch_workspace_bytes", ctypes.c_int64, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
     ("spec_batch_sample", ctypes.c_int,
-     [ctypes.POINTER(BatchLogits), ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
     ("spec_batch_verify", ctypes.c_int,
-     [ctypes.POINTER(BatchLogits), ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
+     [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
      + [ctypes.c_void_p] * 3),
     ("spec_batch_verify_tree", ctypes.c_int,
-     [ctypes.POINTER(BatchLogits), ctypes.c_int] + [ctypes.c_void_p] * 7),
+     [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 7),
     ("spec_lora_plan_bytes", ctypes.c_int64, [ctypes.c_int64]),
     ("spec_lora_plan_make", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(LoraPlanDesc)]),
     ("spec_lora_apply", ctypes.c_int,
-     [ctypes.POINTER(LoraBankDesc), ctypes.POINTER(LoraPlanDesc)] + [ctypes.POINTER(LoraRows)] * 3 + [ctypes.c_void_p]),
+     [ctypes.c_void_p] * 6),
 ]
 
 _lib: Optional[ctypes.CDLL] = None

@@ -11,11 +11,12 @@ namespace batch {
 enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
 
 // A row is cut into chunks of kChunk columns that start at multiples of 16
-// bytes; the first may hold a few columns less.
+// bytes; the first may hold a few columns less.  Their number is a multiple of
+// 8, the last ones may be empty.
 constexpr int kChunk = 512;
 inline int chunks_of(int vocab, int dtype) {
   const int per_vector = dtype == T_F32 ? 4 : 8;
-  return (vocab + per_vector - 1 + kChunk - 1) / kChunk;
+  return (vocab + per_vector - 1 + 8 * kChunk - 1) / (8 * kChunk) * 8;
 }
 
 struct Rows {

@@ -8,21 +8,23 @@
 //
 // Decisions are those of 64-bit arithmetic.  The sums are taken in f32 with
 // a bound on their error, and where a comparison falls inside it the row is
-// summed again in 64 bits by the whole cluster.  With u = 2^-24 and d = (M - l) / T:
-// l - M, the scale log2(e) / T and their product are off by u each, so a weight
-// e^-d by 3 u d, the hardware's 2^x by 4 u more, a chunk's sum of positive terms
-// by 9 u (16 a lane in pairs, 5 rounds of shuffles), a chunk's own scale by
-// another 4 u.  The mean of d under the weights of any set of columns is their
-// entropy less the logarithm of their sum S, at most ln V - ln S; for S >= 1
-// and V <= 2^20 that makes (17 + 3 * 13.9) u < 2^-18 of S (kErr), for S > 2^-33
-// twice that.  Smaller sums are left to 64 bits.
+// summed again in 64 bits by the whole cluster.  A weight is 2^(l h - R) with
+// h = log2(e) / T and a whole number R next to h times the largest logit, one
+// multiply-add, so that sums of different R join exactly.  With u = 2^-24 and
+// d = (M - l) / T: h is off by 1.5 u and the multiply-add by u, a weight by
+// (2.5 d + 0.5) u, the hardware's 2^x by 4 u more, a chunk's sum of positive
+// terms by 9 u (16 a lane in pairs, 5 rounds of shuffles).  The mean of d under
+// the weights of any set of columns is their entropy less the logarithm of their
+// sum S, at most ln V - ln S; for S >= 1 and V <= 2^20 that makes
+// (13.5 + 2.5 * 13.9) u < 2^-18 of S (kErr), for S > 2^-33 less than twice that.
+// Smaller sums, and rows with |M| h of 2^22 and more, are left to 64 bits.
 //
-// Two kernels.  stats_kernel reads every row once, a warp a chunk of 512
-// columns, and leaves each chunk's largest logit and sum.  The second kernel
-// runs a cluster a row (sample) or a sequence (chains, trees); a warp joins a
-// row's chunks by a scan over their sums, finds the chunk of the token and reads
-// that alone.  A rejected draft's max(p - q, 0) is summed by all warps of the
-// cluster, from p and q once more.
+// Two kernels.  stats_kernel reads every row once, a warp one chunk of 512
+// columns or four, and leaves each chunk's reference and sum.  The second
+// kernel runs a cluster a row (sample) or a sequence (chains, trees); a warp
+// joins a row's chunks by a scan over their sums, finds the chunk of the token
+// and reads that alone.  A rejected draft's max(p - q, 0) is summed by all warps
+// of the cluster, from p and q once more.
 #include "batch.h"
 #include "common.cuh"
 #include "kv4_rows.cuh"
@@ -81,9 +83,56 @@ struct Row {
     h = hi * L;
     h += fmaf(hi, L, -h) + fmaf(hi, Llo, lo * L);
   }
-  SPEC_DEV int column(int c, int i, int lane) const { return c * kChunk - shift + (i * 32 + lane) * Vec<T>::N; }
 };
 
+// The reference of weights whose largest logit is m.
+struct Ref {
+  float h, m, R;
+  bool whole;  // R is a whole number; otherwise m h is too large for one
+  SPEC_DEV Ref() {}
+  SPEC_DEV Ref(float m_, float h_) : h(h_), m(m_) {
+    const float y = m * h;
+    whole = fabsf(y) < 0x1p22f;
+    R = whole ? rintf(y) : y;
+  }
+  SPEC_DEV float weight(float x) const { return ex2(whole ? fmaf(x, h, -R) : (x - m) * h); }
+};
+
+template <class T>
+struct Fill;  // a vector of -inf
+template <>
+struct Fill<float> {
+  static constexpr uint32_t kWord = 0xff800000u;
+};
+template <>
+struct Fill<__nv_bfloat16> {
+  static constexpr uint32_t kWord = 0xff80ff80u;
+};
+template <>
+struct Fill<__half> {
+  static constexpr uint32_t kWord = 0xfc00fc00u;
+};
+
+// Columns e .. of a row (e from a 16-byte boundary); those outside the row are -inf.
+template <class T>
+SPEC_DEV uint4 load_vec(const Row<T>& r, int e) {
+  constexpr int N = Vec<T>::N;
+  if (e >= 0 && e + N <= r.V) return *reinterpret_cast<const uint4*>(r.p + e);
+  uint32_t w[4] = {Fill<T>::kWord, Fill<T>::kWord, Fill<T>::kWord, Fill<T>::kWord};
+  if (e > -N && e < r.V) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (e + k >= 0 && e + k < r.V) {
+        if constexpr (N == 4) {
+          w[k] = __float_as_uint(r.p[e + k]);
+        } else {
+          const uint32_t v = reinterpret_cast<const uint16_t*>(r.p)[e + k];
+          w[k / 2] = k % 2 ? (w[k / 2] & 0xffffu) | v << 16 : (w[k / 2] & 0xffff0000u) | v;
+        }
+      }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 SPEC_DEV void unpack(const uint4& v, float (&x)[4], const float*) {
   x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
 }
@@ -100,44 +149,69 @@ SPEC_DEV void unpack(const uint4& v, float (&x)[8], const __half*) {
     x[2 * k] = f.x, x[2 * k + 1] = f.y;
   }
 }
+// Largest element of vectors; a NaN counts only where all are.
+template <int NV>
+SPEC_DEV float largest(const uint4 (&v)[NV], const float*) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v[i].x), __uint_as_float(v[i].y)),
+                       fmaxf(__uint_as_float(v[i].z), __uint_as_float(v[i].w))));
+  return m;
+}
+template <int NV, class H, class H2>
+SPEC_DEV float largest_of_pairs(const uint4 (&v)[NV]) {
+  H2 m;
+  *reinterpret_cast<uint32_t*>(&m) = Fill<H>::kWord;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = __hmax2(m, *reinterpret_cast<const H2*>(&w[k]));
+  }
+  return fmaxf((float)m.x, (float)m.y);
+}
+template <int NV>
+SPEC_DEV float largest(const uint4 (&v)[NV], const __nv_bfloat16*) {
+  return largest_of_pairs<NV, __nv_bfloat16, __nv_bfloat162>(v);
+}
+template <int NV>
+SPEC_DEV float largest(const uint4 (&v)[NV], const __half*) {
+  return largest_of_pairs<NV, __half, __half2>(v);
+}
 SPEC_DEV float to_float(float x) { return x; }
 SPEC_DEV float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 SPEC_DEV float to_float(__half x) { return __half2float(x); }
 
-// This lane's 16 columns of chunk c: vectors lane, 32 + lane, ...; columns
-// outside the row are -inf.
-template <class T>
+// Where this lane's i-th vector of a chunk starts: vectors 32 i + lane (read
+// along the row by all lanes), or the lane's own 16 columns one after another.
+template <class T, bool RUN>
+SPEC_DEV int column(const Row<T>& r, int c, int i, int lane) {
+  return c * kChunk - r.shift + (RUN ? lane * (kPer / Vec<T>::N) + i : i * 32 + lane) * Vec<T>::N;
+}
+template <class T, bool RUN>
 SPEC_DEV void load_chunk(const Row<T>& r, int c, int lane, float (&x)[kPer]) {
   constexpr int N = Vec<T>::N;
   uint4 v[kPer / N];
 #pragma unroll
-  for (int i = 0; i < kPer / N; ++i) {
-    const int e = r.column(c, i, lane);
-    if (e >= 0 && e + N <= r.V) v[i] = *reinterpret_cast<const uint4*>(r.p + e);
-  }
+  for (int i = 0; i < kPer / N; ++i) v[i] = load_vec(r, column<T, RUN>(r, c, i, lane));
 #pragma unroll
   for (int i = 0; i < kPer / N; ++i) {
-    const int e = r.column(c, i, lane);
     float y[N];
-    if (e >= 0 && e + N <= r.V) {
-      unpack(v[i], y, r.p);
-    } else {
-#pragma unroll
-      for (int k = 0; k < N; ++k) y[k] = e + k >= 0 && e + k < r.V ? to_float(r.p[e + k]) : -INFINITY;
-    }
+    unpack(v[i], y, r.p);
 #pragma unroll
     for (int k = 0; k < N; ++k) x[i * N + k] = y[k];
   }
 }
 
 // The same columns of a row of f32 probabilities; zeros outside.
-template <class T>
+template <class T, bool RUN>
 SPEC_DEV void load_probs(const Row<T>& r, const float* q, int c, int lane, float (&x)[kPer]) {
   constexpr int N = Vec<T>::N;
   const bool wide = (reinterpret_cast<uintptr_t>(q) / 4 - r.shift) % 4 == 0;
 #pragma unroll
   for (int i = 0; i < kPer / N; ++i) {
-    const int e = r.column(c, i, lane);
+    const int e = column<T, RUN>(r, c, i, lane);
     if (wide && e >= 0 && e + N <= r.V) {
 #pragma unroll
       for (int k = 0; k < N; k += 4) {
@@ -162,28 +236,69 @@ SPEC_DEV float pair_sum(const float (&x)[kPer]) {
   return s[0];
 }
 
-// A NaN or +inf makes its chunk's sum NaN.
-template <class T>
+SPEC_DEV float redux_max(float x) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(x));
+  return m;
+}
+
+// A warp takes C chunks, whose sums share one reference.  A NaN or +inf makes
+// its chunk's sum NaN.
+template <class T, int C>
 __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows r) {
+  constexpr int N = Vec<T>::N, NV = kPer / N;
   const int lane = threadIdx.x & 31;
-  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const unsigned per_row = (unsigned)r.nch / C, at = blockIdx.x * 8 + (threadIdx.x >> 5);
   pdl_launch_dependents();
   pdl_wait();
-  if (at >= (long long)r.n_rows * r.nch) return;
-  const int row = (int)(at / r.nch), c = (int)(at - (long long)row * r.nch);
-  if (r.path && c == 0 && lane == 0) r.path[row] = -1;
+  const int row = (int)(at / per_row), c0 = (int)(at - row * per_row) * C;
+  if (row >= r.n_rows) return;
+  if (r.path && c0 == 0 && lane == 0) r.path[row] = -1;
   const Row<T> rr(r, row);
-  float x[kPer];
-  load_chunk(rr, c, lane, x);
-  float m = x[0];
+  uint4 v[C * NV];
 #pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
-  m = warp_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
+  for (int c = 0; c < C; ++c)
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = ex2((x[i] - ref) * rr.h);
-  const float s = warp_sum(pair_sum(x));
-  if (lane == 0) r.stats[at] = make_float2(m, s);
+    for (int i = 0; i < NV; ++i) v[c * NV + i] = load_vec(rr, column<T, false>(rr, c0 + c, i, lane));
+  const float m = redux_max(largest(v, rr.p));
+  const Ref ref(m == -INFINITY ? 0.f : m, rr.h);
+  float s[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    float x[kPer];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float y[N];
+      unpack(v[c * NV + i], y, rr.p);
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[i * N + k] = y[k];
+    }
+    if (ref.whole) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = ex2(fmaf(x[i], ref.h, -ref.R));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = ex2((x[i] - ref.m) * ref.h);
+    }
+    s[c] = pair_sum(x);
+  }
+  float2* out = r.stats + (long long)row * r.nch + c0;
+  if constexpr (C == 4) {
+    // Four sums over the lanes at once: lanes 8 c .. end with chunk c's.
+    const bool up = lane & 16, odd = lane & 8;
+    float a = up ? s[2] : s[0], b = up ? s[3] : s[1];
+    a += __shfl_xor_sync(0xffffffffu, up ? s[0] : s[2], 16);
+    b += __shfl_xor_sync(0xffffffffu, up ? s[1] : s[3], 16);
+    float t = odd ? b : a;
+    t += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+    t += __shfl_xor_sync(0xffffffffu, t, 4);
+    t += __shfl_xor_sync(0xffffffffu, t, 2);
+    t += __shfl_xor_sync(0xffffffffu, t, 1);
+    if (lane % 8 == 0) out[lane / 8] = make_float2(m, t);
+  } else {
+    const float t = specb200::warp_sum(s[0]);
+    if (lane == 0) out[0] = make_float2(m, t);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -203,224 +318,329 @@ SPEC_DEV double warp_scan(double v, int lane) {  // inclusive
   return v;
 }
 
-struct Joined {
-  float M;
-  double Z;
-  bool ok;  // the row has a finite largest logit and no NaN
+// 8 chunks a lane: of chunks 256 b .. 256 b + 255 those from 8 lane on.
+constexpr int kBlock = 256;
+
+// A row's chunk statistics: the first 256 chunks in registers, longer rows'
+// others loaded where they are needed.
+struct Stats {
+  const float2* p;
+  int nch, lane;
+  float2 first[8];
+  SPEC_DEV void load(int b, float2 (&v)[8]) const {
+    const int c = b * kBlock + lane * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float4 x = c < nch ? __ldcg(reinterpret_cast<const float4*>(p + c + i)) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      v[i] = make_float2(x.x, x.y);
+      v[i + 1] = make_float2(x.z, x.w);
+    }
+  }
+  SPEC_DEV Stats(const float2* p_, int nch_, int lane_) : p(p_), nch(nch_), lane(lane_) { load(0, first); }
+  // f(chunk block, its 8 statistics) -> whether to go on
+  template <class F>
+  SPEC_DEV void each(F f) const {
+    if (!f(0, first)) return;
+#pragma unroll 1
+    for (int b = 1; b * kBlock < nch; ++b) {
+      float2 v[8];
+      load(b, v);
+      if (!f(b, v)) return;
+    }
+  }
 };
-// Weight of chunk statistics (m, s) with the row's largest logit as reference.
-SPEC_DEV double chunk_weight(float2 v, float M, float h) { return (double)(v.y * ex2((v.x - M) * h)); }
+// 2^e for a whole e <= 0.
+SPEC_DEV float whole_pow2(float e) { return e < -126.f ? 0.f : __int_as_float((127 + (int)e) << 23); }
+// Weight of a chunk's statistics with the row's reference.
+SPEC_DEV double chunk_weight(float2 v, const Ref& row) {
+  const Ref own(v.x, row.h);
+  if (own.whole && row.whole) return (double)(v.y * whole_pow2(own.R - row.R));
+  return (double)(v.y * ex2(row.whole ? fmaf(v.x, row.h, -row.R) : own.whole ? fmaf(-row.m, row.h, own.R) : (v.x - row.m) * row.h));
+}
+
+struct Joined {
+  Ref ref;
+  double Z;  // where the reference is whole
+  bool ok;   // the row has a finite largest logit, no NaN and a temperature
+};
 
 template <class T>
-SPEC_DEV Joined join(const Row<T>& r, const float2* st, int nch, int lane) {
+SPEC_DEV Joined join(const Row<T>& r, const Stats& st) {
   Joined j;
-  j.M = -INFINITY;
-  for (int c = lane; c < nch; c += 32) j.M = fmaxf(j.M, __ldcg(st + c).x);
-  j.M = specb200::warp_max(j.M);
+  float m = -INFINITY;
+  bool nan = false;
+  st.each([&](int, const float2(&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, v[i].x), nan |= v[i].y != v[i].y;
+    return true;
+  });
+  m = redux_max(m);
+  j.ref = Ref(m, r.h);
+  j.ok = r.ok && m > -INFINITY && m < INFINITY && !__any_sync(0xffffffffu, nan);
   double z = 0;
-  for (int c = lane; c < nch; c += 32) z += chunk_weight(__ldcg(st + c), j.M, r.h);
+  st.each([&](int, const float2(&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z += chunk_weight(v[i], j.ref);
+    return true;
+  });
   j.Z = warp_sum(z);
-  j.ok = r.ok && j.M > -INFINITY && j.M < INFINITY && j.Z > 0 && j.Z < INFINITY;
   return j;
 }
 
-// The first chunk whose cumulative weight passes `target`, and the weight
-// before it; -1: none does.  weight(c): of chunk c.
-template <class F>
-SPEC_DEV int find_chunk(F weight, int nch, double target, int lane, double* before) {
-  const int per = (nch + 31) / 32, c0 = min(lane * per, nch), c1 = min(c0 + per, nch);
+// Of 8 values a lane in 256 chunks: the first chunk whose cumulative weight
+// passes `target` (run: the weight before them, moved past them where none does).
+SPEC_DEV int find_in_block(const double (&w)[8], int b, double target, int lane, double* run) {
   double own = 0;
-  for (int c = c0; c < c1; ++c) own += weight(c);
-  const double incl = warp_scan(own, lane);
-  double run = __shfl_up_sync(0xffffffffu, incl, 1);  // not above the target where incl passes it
-  if (lane == 0) run = 0;
-  int found = -1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) own += w[i];
+  const double incl = warp_scan(own, lane) + *run;
+  double at = __shfl_up_sync(0xffffffffu, incl, 1);  // not above the target where incl passes it
+  if (lane == 0) at = *run;
   const unsigned hit = __ballot_sync(0xffffffffu, incl > target);
-  if (!hit) return -1;
-  const int who = __ffs(hit) - 1;
-  if (lane == who) {
-    for (int c = c0; c < c1; ++c) {
-      const double w = weight(c);
-      if (w > 0) found = c;
-      if (run + w > target) break;
-      run += w;
-    }
-    // Rounding may leave the sum of all a step below the scanned one: the last chunk of some weight.
+  if (!hit) {
+    *run = __shfl_sync(0xffffffffu, incl, 31);
+    return -1;
   }
-  found = __shfl_sync(0xffffffffu, found, who);
-  *before = __shfl_sync(0xffffffffu, run, who);
-  return found;
+  const int who = __ffs(hit) - 1;
+  // Rounding may leave the sum of all a step below the scanned one: then the last chunk of some weight.
+  int found = -1;
+  double before = at;
+  bool open = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (open && w[i] > 0) {
+      found = b * kBlock + lane * 8 + i;
+      before = at;
+      at += w[i];
+      open = at <= target;
+    }
+  *run = __shfl_sync(0xffffffffu, before, who);
+  return __shfl_sync(0xffffffffu, found, who);
 }
 
 // The first of a chunk's columns whose cumulative weight passes `target`;
-// w(i): weight of this lane's i-th column.  Where none does, the last column
-// of some weight.  [lo, hi): cumulative weights around the column.
-template <class T, class F>
-SPEC_DEV int find_column(const Row<T>& r, int c, F w, double before, double target, int lane, double* lo, double* hi) {
-  constexpr int N = Vec<T>::N;
-  int last = -1;
-#pragma unroll 1
-  for (int i = 0; i < kPer / N; ++i) {
-    double own = 0;
-    int mine = -1;
+// w[i]: weights of this lane's 16 columns, one after another.  Where none
+// does, the last column of some weight.  [lo, hi): cumulative weights around it.
+template <class T, class W>
+SPEC_DEV int find_column(const Row<T>& r, int c, const W (&w)[kPer], double before, double target, int lane, double* lo,
+                         double* hi) {
+  const int e = column<T, true>(r, c, 0, lane);
+  double own = 0;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const double x = w(i * N + k);
-      own += x;
-      if (x > 0) mine = r.column(c, i, lane) + k;
-    }
-    const double incl = warp_scan(own, lane) + before;
-    double run = __shfl_up_sync(0xffffffffu, incl, 1);
-    if (lane == 0) run = before;
-    const unsigned hit = __ballot_sync(0xffffffffu, incl > target);
-    if (hit) {
-      const int who = __ffs(hit) - 1;
-      int tok = mine;
-      double next = incl;
-      if (lane == who) {
-        double cum = run;
-        bool open = true;
+  for (int i = 0; i < kPer; ++i) own += (double)w[i];
+  const double incl = warp_scan(own, lane) + before;
+  double at = __shfl_up_sync(0xffffffffu, incl, 1);
+  if (lane == 0) at = before;
+  const unsigned hit = __ballot_sync(0xffffffffu, incl > target), some = __ballot_sync(0xffffffffu, own > 0);
+  if (!some) return -1;
+  const int who = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+  int tok = -1;
+  double from = at;
+  bool open = true;
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const double x = w(i * N + k);
-          if (open && cum + x > target) tok = r.column(c, i, lane) + k, run = cum, next = cum + x, open = false;
-          cum += x;
-        }
-      }
-      *lo = __shfl_sync(0xffffffffu, run, who);
-      *hi = __shfl_sync(0xffffffffu, next, who);
-      return __shfl_sync(0xffffffffu, tok, who);
+  for (int i = 0; i < kPer; ++i)
+    if (open && w[i] > 0) {
+      tok = e + i;
+      from = at;
+      at += (double)w[i];
+      open = !hit || at <= target;
     }
-    before = __shfl_sync(0xffffffffu, incl, 31);
-    const unsigned some = __ballot_sync(0xffffffffu, mine >= 0);
-    if (some) last = __shfl_sync(0xffffffffu, mine, 31 - __clz(some));
-  }
-  *lo = *hi = -1;
-  return last;
+  *lo = __shfl_sync(0xffffffffu, hit ? from : -1.0, who);
+  *hi = __shfl_sync(0xffffffffu, at, who);
+  return __shfl_sync(0xffffffffu, tok, who);
 }
 
 // The first column with the row's largest logit.
 template <class T>
-SPEC_DEV int first_largest(const Row<T>& r, const float2* st, int nch, float M, int lane) {
+SPEC_DEV int first_largest(const Row<T>& r, const Stats& st, float M) {
   int c = 0x7fffffff;
-  for (int i = lane; i < nch; i += 32)
-    if (__ldcg(st + i).x == M) {
-      c = i;
-      break;
-    }
-  c = __reduce_min_sync(0xffffffffu, c);
-  float x[kPer];
-  load_chunk(r, c, lane, x);
-  int e = 0x7fffffff;
+  st.each([&](int b, const float2(&v)[8]) {
 #pragma unroll
-  for (int i = kPer - 1; i >= 0; --i)
-    if (x[i] == M) e = r.column(c, i / Vec<T>::N, lane) + i % Vec<T>::N;
-  return __reduce_min_sync(0xffffffffu, e);
+    for (int i = 7; i >= 0; --i)
+      if (v[i].x == M) c = b * kBlock + st.lane * 8 + i;
+    return !__any_sync(0xffffffffu, c < 0x7fffffff);
+  });
+  c = __reduce_min_sync(0xffffffffu, c);
+  // Chunks with one reference share the largest logit that stands beside their sums.
+#pragma unroll 1
+  for (; c < st.nch; ++c) {
+    float x[kPer];
+    load_chunk<T, true>(r, c, st.lane, x);
+    int e = 0x7fffffff;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i)
+      if (x[i] == M) e = column<T, true>(r, c, 0, st.lane) + i;
+    e = __reduce_min_sync(0xffffffffu, e);
+    if (e < 0x7fffffff) return e;
+  }
+  return kBad;
 }
 
 SPEC_DEV double unit(float u) { return (double)fminf(fmaxf(u, 0.f), 1.f); }  // NaN: 0
 
 // A token of p, or kBad, or kUnsure where f32 does not decide.
 template <class T>
-SPEC_DEV int draw(const Row<T>& r, const float2* st, int nch, const Joined& j, float u, int lane) {
+SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
   if (!j.ok) return kBad;
-  if (r.t == 0.f) return first_largest(r, st, nch, j.M, lane);
+  if (r.t == 0.f) return first_largest(r, st, j.ref.m);
   const double target = unit(u) * j.Z, slack = (target < 1 ? 4 : 2) * kErr * target;
-  if (target <= 0x1p-33) return kUnsure;
-  double before, lo, hi;
-  const int c = find_chunk([&](int i) { return chunk_weight(__ldcg(st + i), j.M, r.h); }, nch, target, lane, &before);
+  if (!j.ref.whole || target <= 0x1p-33) return kUnsure;
+  double run = 0, lo, hi;
+  int c = -1;
+  st.each([&](int b, const float2(&v)[8]) {
+    double w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = chunk_weight(v[i], j.ref);
+    c = find_in_block(w, b, target, st.lane, &run);
+    return c < 0;
+  });
   if (c < 0) return kUnsure;
   float x[kPer];
-  load_chunk(r, c, lane, x);
+  load_chunk<T, true>(r, c, st.lane, x);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = ex2((x[i] - j.M) * r.h);
-  const int tok = find_column(r, c, [&](int i) { return (double)x[i]; }, before, target, lane, &lo, &hi);
-  return lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
+  for (int i = 0; i < kPer; ++i) x[i] = ex2(fmaf(x[i], j.ref.h, -j.ref.R));
+  const int tok = find_column(r, c, x, run, target, st.lane, &lo, &hi);
+  return tok >= 0 && lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
 }
 
 // ---------------------------------------------------------------------------
-// 64-bit sums by a cluster
+// Sums by a cluster
 // ---------------------------------------------------------------------------
-template <class T>
-SPEC_DEV double weight64(const Row<T>& r, float x, float M) {
-  return exp(((double)x - (double)M) * (1.0 / (double)r.t));
+// What the columns of a row are weighed by: p in 64 bits (P64), max(p - q, 0)
+// in f32 (REST32) or in 64 bits (REST64).
+enum : int { P64 = 0, REST32 = 1, REST64 = 2 };
+
+// 2^y for y <= 0 in 64 bits: the Taylor series of 2^f, |f| <= 1/2, to
+// (f ln 2)^13 / 13! (the next term is below 2^-57), times the whole power.
+SPEC_DEV double pow2_64(double y) {
+  constexpr double kLn2 = 0.693147180559945309;
+  const double n = rint(fmax(y, -1100.0)), f = (fmax(y, -1100.0) - n) * kLn2;
+  double s = 1.0 / 6227020800;
+  s = fma(s, f, 1.0 / 479001600);
+  s = fma(s, f, 1.0 / 39916800);
+  s = fma(s, f, 1.0 / 3628800);
+  s = fma(s, f, 1.0 / 362880);
+  s = fma(s, f, 1.0 / 40320);
+  s = fma(s, f, 1.0 / 5040);
+  s = fma(s, f, 1.0 / 720);
+  s = fma(s, f, 1.0 / 120);
+  s = fma(s, f, 1.0 / 24);
+  s = fma(s, f, 1.0 / 6);
+  s = fma(s, f, 0.5);
+  s = fma(s, f, 1.0);
+  s = fma(s, f, 1.0);
+  // In two steps, so that results below 2^-1022 keep what bits they have.
+  const int e = (int)n, half = e / 2;
+  return s * __hiloint2double((1023 + half) << 20, 0) * __hiloint2double((1023 + e - half) << 20, 0);
 }
 
-// Sums of a row's chunks into `sums`, by all warps of the cluster.
-// kind 0: p in 64 bits; 1: max(p - q, 0) in f32; 2: the same in 64 bits.
-// The caller syncs the cluster.
 template <class T>
-SPEC_DEV void sum_chunks(const Row<T>& r, float M, double Z, const float* q, int kind, double* sums, int nch, int lane) {
-  const int nw = blockDim.x >> 5, step = nw * cluster_size();
-  const double inv_t = 1.0 / (double)r.t, inv_z = kind ? 1.0 / Z : 0;
-  const float inv_zf = (float)inv_z;
-#pragma unroll 1
-  for (int c = cluster_rank() * nw + (threadIdx.x >> 5); c < nch; c += step) {
-    float x[kPer], y[kPer];
-    load_chunk(r, c, lane, x);
-    if (kind) load_probs(r, q, c, lane, y);
-    double s;
-    if (kind == 1) {
+struct Weigher {
+  const Row<T>& r;
+  const Ref& ref;
+  const float* q;
+  double h, inv_z;
+  SPEC_DEV Weigher(const Row<T>& r_, const Ref& ref_, const float* q_, double Z) : r(r_), ref(ref_), q(q_) {
+    h = 1.44269504088896341 / (double)r.t;
+    inv_z = q ? 1.0 / Z : 0.0;
+  }
+  SPEC_DEV double p64(float x) const { return pow2_64(((double)x - (double)ref.m) * h); }
+  template <bool RUN>
+  SPEC_DEV void rest32(int c, int lane, float (&w)[kPer]) const {
+    float y[kPer];
+    load_chunk<T, RUN>(r, c, lane, w);
+    load_probs<T, RUN>(r, q, c, lane, y);
+    const float z = (float)inv_z;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = fmaxf(fmaf(ex2((x[i] - M) * r.h), inv_zf, -y[i]), 0.f);
-      s = (double)specb200::warp_sum(pair_sum(x));
-    } else {
-      s = 0;
-#pragma unroll 4
-      for (int i = 0; i < kPer; ++i) {
-        const double w = exp(((double)x[i] - (double)M) * inv_t);
-        s += kind ? fmax(w * inv_z - (double)y[i], 0.0) : w;
-      }
-      s = warp_sum(s);
+    for (int i = 0; i < kPer; ++i) w[i] = fmaxf(fmaf(ex2(fmaf(w[i], ref.h, -ref.R)), z, -y[i]), 0.f);
+  }
+  template <bool RUN>
+  SPEC_DEV void exact(int kind, int c, int lane, double (&w)[kPer]) const {
+    float x[kPer];
+    load_chunk<T, RUN>(r, c, lane, x);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) w[i] = p64(x[i]);
+    if (kind == REST64) {
+      load_probs<T, RUN>(r, q, c, lane, x);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) w[i] = fmax(w[i] * inv_z - (double)x[i], 0.0);
     }
-    if (lane == 0) __stcg(sums + c, s);
+  }
+  // Chunk sums by all warps of the cluster; the caller syncs it.
+  SPEC_DEV void sum(int kind, double* sums, int nch, int lane) const {
+    const int nw = blockDim.x >> 5, step = nw * cluster_size();
+#pragma unroll 1
+    for (int c = cluster_rank() * nw + (threadIdx.x >> 5); c < nch; c += step) {
+      double s = 0;
+      if (kind == REST32) {
+        float w[kPer];
+        rest32<false>(c, lane, w);
+        s = (double)specb200::warp_sum(pair_sum(w));
+      } else {
+        double w[kPer];
+        exact<false>(kind, c, lane, w);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s += w[i];
+        s = warp_sum(s);
+      }
+      if (lane == 0) __stcg(sums + c, s);
+    }
+  }
+};
+
+// A row's chunk sums, 8 a lane.
+SPEC_DEV void load_sums(const double* p, int b, int nch, int lane, double (&w)[8]) {
+  const int c = b * kBlock + lane * 8;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const double2 x = c < nch ? __ldcg(reinterpret_cast<const double2*>(p + c + i)) : make_double2(0, 0);
+    w[i] = x.x, w[i + 1] = x.y;
   }
 }
 SPEC_DEV double total(const double* sums, int nch, int lane) {
   double s = 0;
-  for (int c = lane; c < nch; c += 32) s += __ldcg(sums + c);
+  for (int b = 0; b * kBlock < nch; ++b) {
+    double w[8];
+    load_sums(sums, b, nch, lane, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += w[i];
+  }
   return warp_sum(s);
 }
-SPEC_DEV int last_chunk(const double* sums, int nch, int lane) {
-  int last = -1;
-  for (int c = lane; c < nch; c += 32)
-    if (__ldcg(sums + c) > 0) last = c;
-  return __reduce_max_sync(0xffffffffu, last);
-}
 
-// A token of the weights that sum_chunks(kind) summed: exact for kinds 0 and 2.
+// A token of the weights in `sums`, whose sum is Zs: exact for P64 and REST64.
 template <class T>
-SPEC_DEV int draw_sums(const Row<T>& r, float M, double Z, const float* q, int kind, const double* sums, int nch, double Zs,
-                       float u, int lane) {
+SPEC_DEV int draw_sums(const Weigher<T>& f, int kind, const double* sums, int nch, double Zs, float u, int lane) {
   const double target = unit(u) * Zs;
-  double before = 0, lo, hi;
-  int c = find_chunk([&](int i) { return __ldcg(sums + i); }, nch, target, lane, &before);
-  if (c < 0) {
-    if (kind == 1) return kUnsure;
-    c = last_chunk(sums, nch, lane);
-    if (c < 0) return kBad;
-    before = -1;  // its last column of some weight
+  double run = 0, lo = -1, hi;
+  int c = -1, last = -1;
+  for (int b = 0; b * kBlock < nch && c < 0; ++b) {
+    double w[8];
+    load_sums(sums, b, nch, lane, w);
+    c = find_in_block(w, b, target, lane, &run);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (w[i] > 0) last = b * kBlock + lane * 8 + i;
   }
-  float x[kPer], y[kPer];
-  load_chunk(r, c, lane, x);
-  if (kind) load_probs(r, q, c, lane, y);
-  const double inv_z = kind ? 1.0 / Z : 0;
-  const float inv_zf = (float)inv_z;
-  const double end = before < 0 ? INFINITY : target;
-  if (before < 0) before = 0;
-  const int tok = find_column(
-      r, c,
-      [&](int i) -> double {
-        if (kind == 1) return (double)fmaxf(fmaf(ex2((x[i] - M) * r.h), inv_zf, -y[i]), 0.f);
-        const double w = weight64(r, x[i], M);
-        return kind ? fmax(w * inv_z - (double)y[i], 0.0) : w;
-      },
-      before, end, lane, &lo, &hi);
-  if (kind != 1) return tok;
-  // The weights and Z are off by kErr of Z in all, max(p - q, 0) by no more
-  // than p; so the prefix by 2 kErr, and u times the sum likewise.
-  const double slack = 4.25 * kErr;
-  return lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
+  double goal = target;
+  if (c < 0) {  // the target is the whole sum: the last column of some weight
+    if (kind == REST32) return kUnsure;
+    c = __reduce_max_sync(0xffffffffu, last);
+    if (c < 0) return kBad;
+    goal = INFINITY;
+  }
+  if (kind == REST32) {
+    float w[kPer];
+    f.template rest32<true>(c, lane, w);
+    const int tok = find_column(f.r, c, w, run, goal, lane, &lo, &hi);
+    // The weights and Z are off by kErr of Z in all, max(p - q, 0) by no more
+    // than p; so the prefix by 2 kErr, and u times the sum likewise.
+    const double slack = 4.25 * kErr;
+    return tok >= 0 && lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
+  }
+  double w[kPer];
+  f.template exact<true>(kind, c, lane, w);
+  return find_column(f.r, c, w, run, goal, lane, &lo, &hi);
 }
 
 // ---------------------------------------------------------------------------
@@ -437,33 +657,31 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   pdl_wait();
   const Row<T> r(p.r, row);
   const int nch = p.r.nch;
-  const float2* st = p.r.stats + (long long)row * nch;
-  double* sums = p.r.sums + (long long)row * nch;
-  const Joined j = join(r, st, nch, lane);
   const float u = p.r.u[row];
+  const Stats st(p.r.stats + (long long)row * nch, nch, lane);
+  double* sums = p.r.sums + (long long)row * nch;
+  const Joined j = join(r, st);
   int tok = kUnsure;
   if (warp == 0) {
-    tok = draw(r, st, nch, j, u, lane);
+    tok = draw(r, st, j, u);
     if (lane == 0) s_tok = tok;
   }
   if (p.probs) {
     float* out = p.probs + row * p.probs_stride;
-    const float inv = j.ok ? (float)(1.0 / j.Z) : 0.f;
-    const int top = j.ok && r.t == 0.f ? first_largest(r, st, nch, j.M, lane) : -1;
+    const float inv = (float)(1.0 / j.Z);
+    const int top = j.ok && r.t == 0.f ? first_largest(r, st, j.ref.m) : -1;
     const bool wide = (reinterpret_cast<uintptr_t>(out) / 4 - r.shift) % 4 == 0;
     constexpr int N = Vec<T>::N;
 #pragma unroll 1
     for (int c = rank * nw + warp; c < nch; c += nw * size) {
       float x[kPer];
-      load_chunk(r, c, lane, x);
+      load_chunk<T, false>(r, c, lane, x);
 #pragma unroll
       for (int i = 0; i < kPer / N; ++i) {
-        const int e = r.column(c, i, lane);
+        const int e = column<T, false>(r, c, i, lane);
         float y[N];
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-          y[k] = !j.ok ? 0.f : r.t == 0.f ? (e + k == top ? 1.f : 0.f) : ex2((x[i * N + k] - j.M) * r.h) * inv;
-        }
+        for (int k = 0; k < N; ++k) y[k] = !j.ok ? 0.f : r.t == 0.f ? (e + k == top ? 1.f : 0.f) : j.ref.weight(x[i * N + k]) * inv;
         if (wide && e >= 0 && e + N <= r.V) {
 #pragma unroll
           for (int k = 0; k < N; k += 4)
@@ -479,10 +697,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
   __syncthreads();
   tok = s_tok;
   if (tok == kUnsure) {
-    sum_chunks(r, j.M, 0, nullptr, 0, sums, nch, lane);
+    const Weigher<T> f(r, j.ref, nullptr, 0);
+    f.sum(P64, sums, nch, lane);
     cluster_sync();
     if (rank || warp) return;
-    tok = draw_sums(r, j.M, 0, nullptr, 0, sums, nch, total(sums, nch, lane), u, lane);
+    tok = draw_sums(f, P64, sums, nch, total(sums, nch, lane), u, lane);
   }
   if (rank == 0 && threadIdx.x == 0) p.tokens[row] = tok;
 }
@@ -513,33 +732,35 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
   int r0;
   const int n = rows_of(p, b, &r0);
   double* sums = p.r.sums + (long long)(n ? r0 : 0) * nch;
+  bool used = false;  // other blocks may still read `sums`
   int at = 0, verdict = n ? A_ACCEPT : A_BAD;  // the row under decision; why the walk stopped
-  Joined j{0.f, 0, false};
+  Joined j;
   double z64 = 0;  // of row `at`, once summed in 64 bits
   // The walk, a row a warp.  Every block of the cluster comes to the same verdicts.
 #pragma unroll 1
   for (int base = 0; base < n && verdict == A_ACCEPT; base += kVerifyWarps) {
     if (base + warp < n) {
       const int i = base + warp, row = r0 + i;
-      const Row<T> r(p.r, row);
-      const float2* st = p.r.stats + (long long)row * nch;
-      const Joined w = join(r, st, nch, lane);
       const int x = i + 1 < n ? p.tokens[row] : -1;
+      const Row<T> r(p.r, row);
+      const Stats st(p.r.stats + (long long)row * nch, nch, lane);
+      const bool judged = x >= 0 && x < p.r.V;
+      const float u = p.r.u[row], q = judged ? p.q[row * p.q_stride + x] : 0.f, lx = judged ? to_float(r.p[x]) : 0.f;
+      const Joined w = join(r, st);
       int v = A_END;
       if (!w.ok) {
         v = A_BAD;
-      } else if (x >= 0 && x < p.r.V) {
-        const float q = p.q[row * p.q_stride + x];
-        const double left = unit(p.r.u[row]) * (double)q;
+      } else if (judged) {
+        const double left = unit(u) * (double)q;
         if (q <= 0.f) {
           v = A_ACCEPT;
         } else if (r.t == 0.f) {
-          v = left <= (x == first_largest(r, st, nch, w.M, lane) ? 1.0 : 0.0);
+          v = left <= (x == first_largest(r, st, w.ref.m) ? 1.0 : 0.0);
         } else {
-          const double px = (double)ex2((to_float(r.p[x]) - w.M) * r.h), lz = left * w.Z;
-          // w_x alone: off by (4 + 3 * 23) u where it is above 2^-33.
+          const double px = (double)w.ref.weight(lx), lz = left * w.Z;
+          // w_x alone: off by (4.5 + 2.5 * 23) u where it is above 2^-33.
           const double slack = 3 * kErr * lz + 0x1p-33;
-          v = lz + slack < px ? A_ACCEPT : lz > px + slack ? A_REJECT : A_UNSURE;
+          v = !w.ref.whole ? A_UNSURE : lz + slack < px ? A_ACCEPT : lz > px + slack ? A_REJECT : A_UNSURE;
           if (q != q) v = A_REJECT;
         }
       }
@@ -553,13 +774,15 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
       j = s_join[w];
       if (verdict == A_UNSURE) {
         const Row<T> r(p.r, r0 + at);
+        const Weigher<T> f(r, j.ref, nullptr, 0);
+        if (used) cluster_sync();
+        f.sum(P64, sums, nch, lane);
         cluster_sync();
-        sum_chunks(r, j.M, 0, nullptr, 0, sums, nch, lane);
-        cluster_sync();
+        used = true;
         z64 = total(sums, nch, lane);
         const int x = p.tokens[r0 + at];
         const double left = unit(p.r.u[r0 + at]) * (double)p.q[(r0 + at) * p.q_stride + x];
-        verdict = left * z64 <= weight64(r, to_float(r.p[x]), j.M) ? A_ACCEPT : A_REJECT;
+        verdict = left * z64 <= f.p64(to_float(r.p[x])) ? A_ACCEPT : A_REJECT;
         if (verdict == A_ACCEPT) z64 = 0;
       }
       if (verdict != A_ACCEPT) break;
@@ -570,53 +793,57 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
   if (verdict != A_BAD) {
     const int row = r0 + at;
     const Row<T> r(p.r, row);
-    const float2* st = p.r.stats + (long long)row * nch;
-    const float* q = nullptr;
-    int kind = 0;
-    float u = p.r.u[row];
+    const Stats st(p.r.stats + (long long)row * nch, nch, lane);
+    const bool rest = verdict == A_REJECT;
+    const float* q = rest ? p.q + row * p.q_stride : nullptr;
+    const float u = p.r.u[row + rest];  // a row follows every draft
     tok = kUnsure;
-    if (verdict == A_REJECT) {
-      u = p.r.u[row + 1];  // a row follows every draft
-      q = p.q + row * p.q_stride;
-      kind = 2;
-    }
     if (r.t == 0.f) {
       // All of p on one token: what is left of it is that token, unless q holds it all too.
-      if (warp == 0) tok = first_largest(r, st, nch, j.M, lane);
-    } else if (verdict == A_END) {
-      if (warp == 0) tok = draw(r, st, nch, j, u, lane);
-    } else if (z64 == 0) {
+      if (warp == 0) tok = first_largest(r, st, j.ref.m);
+    } else if (!rest) {
+      if (warp == 0) tok = draw(r, st, j, u);
+    } else if (j.ref.whole && z64 == 0) {
+      const Weigher<T> f(r, j.ref, q, j.Z);
+      if (used) cluster_sync();
+      f.sum(REST32, sums, nch, lane);
       cluster_sync();
-      sum_chunks(r, j.M, j.Z, q, 1, sums, nch, lane);
-      cluster_sync();
-      if (warp == 0) tok = draw_sums(r, j.M, j.Z, q, 1, sums, nch, total(sums, nch, lane), u, lane);
+      used = true;
+      if (warp == 0) tok = draw_sums(f, REST32, sums, nch, total(sums, nch, lane), u, lane);
     }
     if (threadIdx.x == 0) s_tok = tok;
     __syncthreads();
     tok = s_tok;
     if (tok == kUnsure) {
+      const Weigher<T> f(r, j.ref, nullptr, 0);
       double z = z64;
       if (z == 0) {
-        cluster_sync();
-        sum_chunks(r, j.M, 0, nullptr, 0, sums, nch, lane);
+        if (used) cluster_sync();
+        f.sum(P64, sums, nch, lane);
         cluster_sync();
         z = total(sums, nch, lane);
       }
+      int kind = P64;
       double zs = z;
-      if (kind == 2) {
+      if (rest) {
+        const Weigher<T> g(r, j.ref, q, z);
         cluster_sync();
-        sum_chunks(r, j.M, z, q, 2, sums, nch, lane);
+        g.sum(REST64, sums, nch, lane);
         cluster_sync();
+        kind = REST64;
         zs = total(sums, nch, lane);
         if (!(zs > 0)) {  // p is nowhere above q: p itself
           cluster_sync();
-          sum_chunks(r, j.M, 0, nullptr, 0, sums, nch, lane);
+          f.sum(P64, sums, nch, lane);
           cluster_sync();
-          kind = 0;
+          kind = P64;
           zs = z;
         }
       }
-      if (rank == 0 && warp == 0) tok = draw_sums(r, j.M, z, q, kind, sums, nch, zs, u, lane);
+      if (rank == 0 && warp == 0) {
+        const Weigher<T> g(r, j.ref, kind == P64 ? nullptr : q, z);
+        tok = draw_sums(g, kind, sums, nch, zs, u, lane);
+      }
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
@@ -640,8 +867,9 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_kernel(const __grid_const
 #pragma unroll 1
   for (int i = rank * kVerifyWarps + warp; i < n; i += size * kVerifyWarps) {
     const Row<T> r(p.r, r0 + i);
-    const float2* st = p.r.stats + (long long)(r0 + i) * nch;
-    const int tok = draw(r, st, nch, join(r, st, nch, lane), p.r.u[r0 + i], lane);
+    const float u = p.r.u[r0 + i];
+    const Stats st(p.r.stats + (long long)(r0 + i) * nch, nch, lane);
+    const int tok = draw(r, st, join(r, st), u);
     if (lane == 0) __stcg(p.r.drawn + r0 + i, tok);
   }
   cluster_sync();
@@ -654,12 +882,13 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_kernel(const __grid_const
     tok = __ldcg(p.r.drawn + r0 + cur);
     if (tok == kUnsure) {
       const Row<T> r(p.r, r0 + cur);
-      const Joined j = join(r, p.r.stats + (long long)(r0 + cur) * nch, nch, lane);
+      const Joined j = join(r, Stats(p.r.stats + (long long)(r0 + cur) * nch, nch, lane));
+      const Weigher<T> f(r, j.ref, nullptr, 0);
       cluster_sync();
-      sum_chunks(r, j.M, 0, nullptr, 0, sums, nch, lane);
+      f.sum(P64, sums, nch, lane);
       cluster_sync();
       if (warp == 0) {
-        tok = draw_sums(r, j.M, 0, nullptr, 0, sums, nch, total(sums, nch, lane), p.r.u[r0 + cur], lane);
+        tok = draw_sums(f, P64, sums, nch, total(sums, nch, lane), p.r.u[r0 + cur], lane);
         if (lane == 0) s_tok = tok;
       }
       __syncthreads();
@@ -711,20 +940,22 @@ int cluster_for(int n, int threads, int sms) {
   return size;
 }
 
+// A chunk a warp where that is less than the warps that the device holds, else four.
 template <class T>
-cudaError_t stats(const Rows& r, cudaStream_t s) {
-  const long long blocks = ((long long)r.n_rows * r.nch + 7) / 8;
-  return kv4::launch_overlapping(stats_kernel<T>, dim3((unsigned)blocks), 256, 0, s, r);
+cudaError_t stats(const Rows& r, int sms, cudaStream_t s) {
+  const long long chunks = (long long)r.n_rows * r.nch;
+  if (chunks <= sms * 64LL) return kv4::launch_overlapping(stats_kernel<T, 1>, dim3((unsigned)(chunks / 8)), 256, 0, s, r);
+  return kv4::launch_overlapping(stats_kernel<T, 4>, dim3((unsigned)((chunks / 4 + 7) / 8)), 256, 0, s, r);
 }
 template <class T>
 cudaError_t sample(const SampleParams& p, int sms, cudaStream_t s) {
-  const cudaError_t e = stats<T>(p.r, s);
+  const cudaError_t e = stats<T>(p.r, sms, s);
   if (e != cudaSuccess) return e;
   return launch_clusters(sample_kernel<T>, p.r.n_rows, cluster_for(p.r.n_rows, kSampleThreads, sms), kSampleThreads, s, p);
 }
 template <class T>
 cudaError_t verify(const VerifyParams& p, bool trees, int sms, cudaStream_t s) {
-  const cudaError_t e = p.r.n_rows ? stats<T>(p.r, s) : cudaSuccess;
+  const cudaError_t e = p.r.n_rows ? stats<T>(p.r, sms, s) : cudaSuccess;
   if (e != cudaSuccess) return e;
   const int size = cluster_for(p.n_seqs, kVerifyThreads, sms);
   return trees ? launch_clusters(tree_kernel<T>, p.n_seqs, size, kVerifyThreads, s, p)

@@ -12,12 +12,17 @@ without waiting for it.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import numpy as np
 
 from . import _lib
+from .sampling import _setup
 from .kv4 import _host
+
+
+_THREE_ROWS = struct.Struct("=" + "Qqqii" * 3)  # spec_lora_rows
 
 
 def _invalid(msg: str) -> _lib.SamplingError:
@@ -48,6 +53,7 @@ class LoraPlan:
         if not self._copy.is_cuda:
             raise _invalid(f"a plan on {self.device}: a CUDA device is needed")
         self._desc.device_copy = self._copy.data_ptr()
+        self._at = ctypes.addressof(self._desc)
         self._made_on = torch.cuda.current_stream(self.device).cuda_stream
 
 
@@ -92,36 +98,43 @@ class LoraBank:
             a.device.index, n, k, self.n, r, types[a.dtype], a.data_ptr(), b.data_ptr(), a.stride(0), a.stride(1),
             b.stride(0), b.stride(1), ranks.data_ptr() if ranks is not None else None,
             scales.data_ptr() if scales is not None else None)
+        self._at, self._index = ctypes.addressof(self._desc), a.device.index
 
-    def _rows(self, t, width: int, what: str) -> _lib.LoraRows:
-        import torch
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
+    def _rows(self, t, width: int, what: str):
+        """The fields of spec_lora_rows for tensor t [rows, width]."""
+        torch = _setup()[0]
+        if not isinstance(t, torch.Tensor) or t.get_device() != self._index:
             raise _invalid(f"{what} is not a tensor on {self.device}")
+        kind = self._types.get(t.dtype)
+        if kind is None:
+            raise _invalid(f"{what} is {t.dtype}: float32 and the adapters' type are taken")
         if t.dim() != 2 or t.shape[1] != width:
             raise _invalid(f"{what} has shape {tuple(t.shape)}, [rows, {width}] is needed")
-        if t.dtype not in self._types:
-            raise _invalid(f"{what} is {t.dtype}: float32 and the adapters' type are taken")
-        if width > 1 and t.stride(1) != 1:
+        row, column = t.stride()
+        if column != 1 and width > 1:
             raise _invalid(f"the rows of {what} are not contiguous")
-        return _lib.LoraRows(t.data_ptr(), t.stride(0), t.shape[0], self._types[t.dtype], 0)
+        return t.data_ptr(), row, t.shape[0], kind, 0
 
     def apply(self, plan: LoraPlan, x, y, out=None):
         """out = y + scale (x A^T) B^T, each row with its own adapter; x [rows, k],
         y and out [rows, n] (out None: y itself).  Returns out."""
-        import torch
+        torch, lib, _, current = _setup()
         if plan.device != self.device:
             raise _invalid(f"the plan is on {plan.device}, the bank on {self.device}")
         if out is None:
             out = y
-        rx, ry, ro = self._rows(x, self.k, "x"), self._rows(y, self.n, "y"), self._rows(out, self.n, "out")
-        stream = torch.cuda.current_stream(self.device)
-        _lib.check(self._lib.spec_lora_apply(ctypes.byref(self._desc), ctypes.byref(plan._desc), ctypes.byref(rx),
-                                             ctypes.byref(ry), ctypes.byref(ro), stream.cuda_stream))
+        rows = _THREE_ROWS.pack(*self._rows(x, self.k, "x"), *self._rows(y, self.n, "y"), *self._rows(out, self.n, "out"))
+        stream = current(self._index)
+        # The three structures lie behind one another.
+        at = ctypes.cast(ctypes.c_char_p(rows), ctypes.c_void_p).value
+        rc = lib.spec_lora_apply(self._at, plan._at, at, at + 32, at + 64, stream)
+        if rc:
+            _lib.check(rc)
         # Memory of a plan or bank that is dropped is not handed out before this stream is done with it.
-        if stream.cuda_stream != plan._made_on:
-            plan._copy.record_stream(stream)
-        if stream.cuda_stream != self._made_on:
+        if stream != plan._made_on:
+            plan._copy.record_stream(torch.cuda.current_stream(self.device))
+        if stream != self._made_on:
             for t in self._keep:
                 if t is not None:
-                    t.record_stream(stream)
+                    t.record_stream(torch.cuda.current_stream(self.device))
         return out

@@ -11,74 +11,95 @@ are those of 64-bit arithmetic on the given logits, probabilities and uniforms.
 
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 from typing import Tuple
 
 from . import _lib
+
+_LOGITS = struct.Struct("=iiifQqqQQQq")  # spec_batch_logits (packing takes less time than a ctypes structure)
 
 
 def _invalid(msg: str) -> _lib.SamplingError:
     return _lib.SamplingError(_lib.SPEC_ERR_INVALID, msg)
 
 
-def _on(t, what: str, device, dtype, shape=None):
-    """Data pointer of a contiguous tensor of `dtype` on `device`."""
+@functools.lru_cache(maxsize=None)
+def _setup():
+    """torch, the library, the element types, and torch's current stream of a device as a raw handle."""
     import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return (torch, _lib.load(), {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2},
+            raw or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(n: int, v: int, kind: int) -> int:
+    size = _lib.load().spec_batch_workspace_bytes(n, v, kind)
+    if size < 0:
+        _lib.check(-size)
+    return size
+
+
+def _on(t, what: str, index: int, dtype, n=None) -> int:
+    """Data pointer of a contiguous one-dimensional tensor of `dtype` on device `index`, of n elements."""
+    torch = _setup()[0]
     if not isinstance(t, torch.Tensor):
         raise _invalid(f"{what} is not a tensor")
-    if t.device != device:
-        raise _invalid(f"{what} is on {t.device}, the logits on {device}")
+    if t.get_device() != index:
+        raise _invalid(f"{what} is on {t.device}, the logits on cuda:{index}")
     if t.dtype != dtype:
         raise _invalid(f"{what} is {t.dtype}, {dtype} is needed")
-    if shape is not None and tuple(t.shape) != shape:
-        raise _invalid(f"{what} has shape {tuple(t.shape)}, {shape} is needed")
+    if t.dim() != 1 or (n is not None and t.numel() != n):
+        raise _invalid(f"{what} has shape {tuple(t.shape)}, {'[sequences + 1]' if n is None else (n,)} is needed")
     if not t.is_contiguous():
         raise _invalid(f"{what} is not contiguous")
     return t.data_ptr()
 
 
-def _rows_of(t, what: str, device, dtype, n: int, v: int):
+def _rows_of(t, what: str, index: int, dtype, n: int, v: int):
     """Data pointer and row stride of a tensor [n, v] whose columns are contiguous."""
-    import torch
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype:
-        raise _invalid(f"{what} is not a {dtype} tensor on {device}")
-    if tuple(t.shape) != (n, v):
+    torch = _setup()[0]
+    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype != dtype:
+        raise _invalid(f"{what} is not a {dtype} tensor on cuda:{index}")
+    if t.shape != (n, v):
         raise _invalid(f"{what} has shape {tuple(t.shape)}, {(n, v)} is needed")
-    if v > 1 and t.stride(1) != 1:
+    row, column = t.stride()
+    if column != 1 and v > 1:
         raise _invalid(f"the columns of {what} are not contiguous")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), row
 
 
 def _logits(logits, uniforms, temperature):
-    """spec_batch_logits of a call, and what has to live until it is queued."""
-    import torch
-    types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    """spec_batch_logits of a call, its workspace (which lives until the call is queued), and the device's index."""
+    torch, _, types, _ = _setup()
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda):
         raise _invalid("logits are not a CUDA tensor")
     if logits.dim() != 2:
         raise _invalid(f"logits have shape {tuple(logits.shape)}, [rows, vocabulary] is needed")
-    if logits.dtype not in types:
-        raise _invalid(f"logits are {logits.dtype}: bfloat16, float16 and float32 are taken")
+    dtype = logits.dtype
+    if dtype not in types:
+        raise _invalid(f"logits are {dtype}: bfloat16, float16 and float32 are taken")
     n, v = logits.shape
-    device = logits.device
-    ptr, stride = _rows_of(logits, "logits", device, logits.dtype, n, v)
-    u = _on(uniforms, "uniforms", device, torch.float32, (n,))
-    temps, temp = None, 0.0
+    index = logits.get_device()
+    row, column = logits.stride()
+    if column != 1 and v > 1:
+        raise _invalid("the columns of logits are not contiguous")
+    u = _on(uniforms, "uniforms", index, torch.float32, n)
+    temps, temp = 0, 0.0
     if isinstance(temperature, torch.Tensor):
-        temps = _on(temperature, "temperature", device, torch.float32, (n,))
+        temps = _on(temperature, "temperature", index, torch.float32, n)
     else:
-        temp = float(temperature)
-    kind = types[logits.dtype]
-    size = _lib.load().spec_batch_workspace_bytes(n, v, kind)
-    if size < 0:
-        _lib.check(-size)
-    work = torch.empty(size, dtype=torch.uint8, device=device)
-    return _lib.BatchLogits(device.index, v, kind, temp, ptr, stride, n, temps, u, work.data_ptr(), size), work
-
-
-def _stream(device) -> int:
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+        try:
+            temp = float(temperature)
+        except (TypeError, ValueError) as e:
+            raise _invalid(f"temperature: {e}") from None
+        if not 0.0 <= temp <= 3.4e38:
+            raise _invalid(f"temperature {temp}")
+    kind = types[dtype]
+    size = _workspace_bytes(n, v, kind)
+    work = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    return _LOGITS.pack(index, v, kind, temp, logits.data_ptr(), row, n, temps, u, work.data_ptr(), size), work, index
 
 
 def sample_rows(logits, uniforms, temperature=1.0, probs_out=None, tokens_out=None):
@@ -87,15 +108,18 @@ def sample_rows(logits, uniforms, temperature=1.0, probs_out=None, tokens_out=No
     uniforms: float32 [rows]; temperature: a number, or float32 [rows] (0: the
     first largest logit).  probs_out: float32 [rows, vocabulary] for the rows'
     probabilities; tokens_out: contiguous int32 [rows]."""
-    import torch
-    a, work = _logits(logits, uniforms, temperature)
+    torch, lib, _, stream = _setup()
+    a, work, index = _logits(logits, uniforms, temperature)
     n, v = logits.shape
     if tokens_out is None:
         tokens_out = torch.empty(n, dtype=torch.int32, device=logits.device)
+        tokens = tokens_out.data_ptr()
     else:
-        _on(tokens_out, "tokens_out", logits.device, torch.int32, (n,))
-    probs, stride = (None, 0) if probs_out is None else _rows_of(probs_out, "probs_out", logits.device, torch.float32, n, v)
-    _lib.check(_lib.load().spec_batch_sample(ctypes.byref(a), probs, stride, tokens_out.data_ptr(), _stream(logits.device)))
+        tokens = _on(tokens_out, "tokens_out", index, torch.int32, n)
+    probs, row = (None, 0) if probs_out is None else _rows_of(probs_out, "probs_out", index, torch.float32, n, v)
+    rc = lib.spec_batch_sample(a, probs, row, tokens, stream(index))
+    if rc:
+        _lib.check(rc)
     return tokens_out
 
 
@@ -107,18 +131,18 @@ def verify_drafts(logits, drafts, draft_probs, uniforms, row_start, temperature=
     token that row r judges, drawn from row r of draft_probs (float32 [rows,
     vocabulary]); those of a sequence's last row are not read.  uniforms: float32
     [rows]; temperature: a number, or float32 [rows]."""
-    import torch
-    a, work = _logits(logits, uniforms, temperature)
+    torch, lib, _, stream = _setup()
+    a, work, index = _logits(logits, uniforms, temperature)
     n, v = logits.shape
-    start = _on(row_start, "row_start", logits.device, torch.int32)
-    if row_start.dim() != 1 or row_start.numel() < 1:
-        raise _invalid(f"row_start has shape {tuple(row_start.shape)}, [sequences + 1] is needed")
-    d = _on(drafts, "drafts", logits.device, torch.int32, (n,))
-    q, stride = _rows_of(draft_probs, "draft_probs", logits.device, torch.float32, n, v)
-    out = torch.empty(2, row_start.numel() - 1, dtype=torch.int32, device=logits.device)
-    count, token = out[0], out[1]
-    _lib.check(_lib.load().spec_batch_verify(ctypes.byref(a), row_start.numel() - 1, start, d, q, stride, count.data_ptr(),
-                                             token.data_ptr(), _stream(logits.device)))
+    start, seqs = _on(row_start, "row_start", index, torch.int32), row_start.numel() - 1
+    if seqs < 0:
+        raise _invalid("row_start is empty, [sequences + 1] is needed")
+    d = _on(drafts, "drafts", index, torch.int32, n)
+    q, row = _rows_of(draft_probs, "draft_probs", index, torch.float32, n, v)
+    count, token = torch.empty(2, seqs, dtype=torch.int32, device=logits.device).unbind()
+    rc = lib.spec_batch_verify(a, seqs, start, d, q, row, count.data_ptr(), token.data_ptr(), stream(index))
+    if rc:
+        _lib.check(rc)
     return count, token
 
 
@@ -129,17 +153,17 @@ def verify_trees(logits, tokens, parents, uniforms, row_start, temperature=1.0) 
     [rows] (parents within the sequence, node 0 the root).  path: int32 [rows],
     a sequence's accepted nodes from its first row on, root first, -1 in all
     other rows; path_len and next_token: int32 [sequences]."""
-    import torch
-    a, work = _logits(logits, uniforms, temperature)
+    torch, lib, _, stream = _setup()
+    a, work, index = _logits(logits, uniforms, temperature)
     n = logits.shape[0]
-    start = _on(row_start, "row_start", logits.device, torch.int32)
-    if row_start.dim() != 1 or row_start.numel() < 1:
-        raise _invalid(f"row_start has shape {tuple(row_start.shape)}, [sequences + 1] is needed")
-    t = _on(tokens, "tokens", logits.device, torch.int32, (n,))
-    up = _on(parents, "parents", logits.device, torch.int32, (n,))
-    path = torch.empty(n, dtype=torch.int32, device=logits.device)
-    out = torch.empty(2, row_start.numel() - 1, dtype=torch.int32, device=logits.device)
-    count, token = out[0], out[1]
-    _lib.check(_lib.load().spec_batch_verify_tree(ctypes.byref(a), row_start.numel() - 1, start, t, up, path.data_ptr(),
-                                                  count.data_ptr(), token.data_ptr(), _stream(logits.device)))
+    start, seqs = _on(row_start, "row_start", index, torch.int32), row_start.numel() - 1
+    if seqs < 0:
+        raise _invalid("row_start is empty, [sequences + 1] is needed")
+    t = _on(tokens, "tokens", index, torch.int32, n)
+    up = _on(parents, "parents", index, torch.int32, n)
+    path, count, token = torch.empty(n + 2 * seqs, dtype=torch.int32, device=logits.device).split((n, seqs, seqs))
+    rc = lib.spec_batch_verify_tree(a, seqs, start, t, up, path.data_ptr(), count.data_ptr(), token.data_ptr(),
+                                    stream(index))
+    if rc:
+        _lib.check(rc)
     return path, count, token
