@@ -22,7 +22,7 @@ int check_shape(const char* what, int64_t n_rows, int vocab, int dtype) {
 
 int64_t workspace_bytes(int64_t n_rows, int vocab, int dtype) {
   const size_t cells = (size_t)n_rows * chunks_of(vocab, dtype);
-  return (int64_t)(up(cells * sizeof(float2)) + up(cells * sizeof(double)) + up((size_t)n_rows * sizeof(int)));
+  return (int64_t)(up(cells * sizeof(float2)) + up(cells * sizeof(double)) + up((size_t)n_rows * sizeof(float2)));
 }
 
 int check_logits(const char* what, const spec_batch_logits* l) {
@@ -61,7 +61,12 @@ Rows to_rows(const spec_batch_logits* l) {
   r.stats = reinterpret_cast<float2*>(w);
   r.sums = reinterpret_cast<double*>(w + up(cells * sizeof(float2)));
   r.path = nullptr;
-  r.drawn = reinterpret_cast<int*>(w + up(cells * sizeof(float2)) + up(cells * sizeof(double)));
+  r.drafts = nullptr;
+  r.q = nullptr;
+  r.q_stride = 0;
+  uint8_t* last = w + up(cells * sizeof(float2)) + up(cells * sizeof(double));  // a chain's or a tree's
+  r.seen = reinterpret_cast<float2*>(last);
+  r.drawn = reinterpret_cast<int*>(last);
   return r;
 }
 
@@ -77,6 +82,7 @@ int verify(const char* what, const spec_batch_logits* l, VerifyParams& p, int32_
   if (cur.rc != SPEC_OK) return cur.rc;
   p.r = to_rows(l);
   p.r.path = path;
+  if (!trees) p.r.drafts = p.tokens, p.r.q = p.q, p.r.q_stride = p.q_stride;
   int sms = 0;
   cudaError_t e = multiprocessors(l->device, &sms);
   if (e == cudaSuccess) e = launch_verify(p, l->dtype, trees, sms, static_cast<cudaStream_t>(stream));

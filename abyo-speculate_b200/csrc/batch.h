@@ -25,6 +25,10 @@ struct Rows {
   const float* temps;  // per row, or null: `temp`
   float temp;
   const float* u;
+  const int* drafts;   // chains: the tokens that the rows judge, and the draft's rows
+  const float* q;
+  long long q_stride;
+  float2* seen;        // [n_rows]: the draft's probability of it, and the row's logit
   int n_rows, V, nch;
   float2* stats;  // [n_rows][nch]: largest logit, sum of exp((l - largest) / T)
   double* sums;   // [n_rows][nch]: sums of one row that a cluster works on

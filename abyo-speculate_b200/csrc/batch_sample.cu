@@ -12,15 +12,17 @@
 // h = log2(e) / T and a whole number R next to h times the largest logit, one
 // multiply-add, so that sums of different R join exactly.  With u = 2^-24 and
 // d = (M - l) / T: h is off by 1.5 u and the multiply-add by u, a weight by
-// (2.5 d + 0.5) u, the hardware's 2^x by 4 u more, a chunk's sum of positive
-// terms by 9 u (16 a lane in pairs, 5 rounds of shuffles).  The mean of d under
-// the weights of any set of columns is their entropy less the logarithm of their
-// sum S, at most ln V - ln S; for S >= 1 and V <= 2^20 that makes
-// (13.5 + 2.5 * 13.9) u < 2^-18 of S (kErr), for S > 2^-33 less than twice that.
-// Smaller sums, and rows with |M| h of 2^22 and more, are left to 64 bits.
+// (2.5 d + 0.5) u, the hardware's 2^x by 4 u more.  Of positive terms a chunk's
+// sum is off by 9 u (16 a lane in pairs, 5 rounds of shuffles), a prefix of
+// chunks by 12 u more (7 additions, 5 rounds), one inside a chunk by 20 u
+// (15 and 5).  The mean of d under the weights of any set of columns is their
+// entropy less the logarithm of their sum S, at most ln V - ln S; for S >= 1
+// and V <= 2^20 that makes (4.5 + 21 + 2.5 * 13.9) u < 2^-18 of S (kErr), for
+// S > 2^-33 less than twice that.  Smaller sums, and rows with |M| h of 2^22
+// and more, are left to 64 bits.
 //
 // Two kernels.  stats_kernel reads every row once, a warp one chunk of 512
-// columns or four, and leaves each chunk's reference and sum.  The second
+// columns or 8 KB, and leaves each chunk's reference and sum.  The second
 // kernel runs a cluster a row (sample) or a sequence (chains, trees); a warp
 // joins a row's chunks by a scan over their sums, finds the chunk of the token
 // and reads that alone.  A rejected draft's max(p - q, 0) is summed by all warps
@@ -70,10 +72,14 @@ struct Row {
   float h;       // log2(e) / t
   bool ok;       // the temperature is finite and not negative
 
-  SPEC_DEV Row(const Rows& r, int row) {
+  SPEC_DEV Row() {}
+  SPEC_DEV void place(const Rows& r, int row) {
     p = static_cast<const T*>(r.logits) + row * r.stride;
     V = r.V;
     shift = (int)(reinterpret_cast<uintptr_t>(p) / sizeof(T) % Vec<T>::N);
+  }
+  SPEC_DEV Row(const Rows& r, int row) {
+    place(r, row);
     t = r.temps ? r.temps[row] : r.temp;
     ok = t >= 0.f && t < INFINITY;
     if (t > 0.f) t = fminf(fmaxf(t, 0x1p-60f), 0x1p60f);
@@ -151,7 +157,7 @@ SPEC_DEV void unpack(const uint4& v, float (&x)[8], const __half*) {
 }
 // Largest element of vectors; a NaN counts only where all are.
 template <int NV>
-SPEC_DEV float largest(const uint4 (&v)[NV], const float*) {
+SPEC_DEV float largest(const uint4* v, const float*) {
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -160,7 +166,7 @@ SPEC_DEV float largest(const uint4 (&v)[NV], const float*) {
   return m;
 }
 template <int NV, class H, class H2>
-SPEC_DEV float largest_of_pairs(const uint4 (&v)[NV]) {
+SPEC_DEV float largest_of_pairs(const uint4* v) {
   H2 m;
   *reinterpret_cast<uint32_t*>(&m) = Fill<H>::kWord;
 #pragma unroll
@@ -172,11 +178,11 @@ SPEC_DEV float largest_of_pairs(const uint4 (&v)[NV]) {
   return fmaxf((float)m.x, (float)m.y);
 }
 template <int NV>
-SPEC_DEV float largest(const uint4 (&v)[NV], const __nv_bfloat16*) {
+SPEC_DEV float largest(const uint4* v, const __nv_bfloat16*) {
   return largest_of_pairs<NV, __nv_bfloat16, __nv_bfloat162>(v);
 }
 template <int NV>
-SPEC_DEV float largest(const uint4 (&v)[NV], const __half*) {
+SPEC_DEV float largest(const uint4* v, const __half*) {
   return largest_of_pairs<NV, __half, __half2>(v);
 }
 SPEC_DEV float to_float(float x) { return x; }
@@ -189,19 +195,40 @@ template <class T, bool RUN>
 SPEC_DEV int column(const Row<T>& r, int c, int i, int lane) {
   return c * kChunk - r.shift + (RUN ? lane * (kPer / Vec<T>::N) + i : i * 32 + lane) * Vec<T>::N;
 }
+// Whether all of a chunk's columns are the row's.
+template <class T>
+SPEC_DEV bool inside(const Row<T>& r, int c) {
+  return c * kChunk >= r.shift && (c + 1) * kChunk - r.shift <= r.V;
+}
 template <class T, bool RUN>
-SPEC_DEV void load_chunk(const Row<T>& r, int c, int lane, float (&x)[kPer]) {
-  constexpr int N = Vec<T>::N;
-  uint4 v[kPer / N];
+SPEC_DEV void load_raw(const Row<T>& r, int c, int lane, uint4 (&v)[kPer / Vec<T>::N]) {
+  constexpr int N = Vec<T>::N, NV = kPer / N;
+  const int e = column<T, RUN>(r, c, 0, lane);
+  if (inside(r, c)) {
+    const uint4* at = reinterpret_cast<const uint4*>(r.p + e);
 #pragma unroll
-  for (int i = 0; i < kPer / N; ++i) v[i] = load_vec(r, column<T, RUN>(r, c, i, lane));
+    for (int i = 0; i < NV; ++i) v[i] = at[RUN ? i : i * 32];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = load_vec(r, e + (RUN ? i : i * 32) * N);
+  }
+}
+template <class T>
+SPEC_DEV void unpack_chunk(const uint4* v, float (&x)[kPer], const T* tag) {
+  constexpr int N = Vec<T>::N;
 #pragma unroll
   for (int i = 0; i < kPer / N; ++i) {
     float y[N];
-    unpack(v[i], y, r.p);
+    unpack(v[i], y, tag);
 #pragma unroll
     for (int k = 0; k < N; ++k) x[i * N + k] = y[k];
   }
+}
+template <class T, bool RUN>
+SPEC_DEV void load_chunk(const Row<T>& r, int c, int lane, float (&x)[kPer]) {
+  uint4 v[kPer / Vec<T>::N];
+  load_raw<T, RUN>(r, c, lane, v);
+  unpack_chunk(v, x, r.p);
 }
 
 // The same columns of a row of f32 probabilities; zeros outside.
@@ -209,28 +236,48 @@ template <class T, bool RUN>
 SPEC_DEV void load_probs(const Row<T>& r, const float* q, int c, int lane, float (&x)[kPer]) {
   constexpr int N = Vec<T>::N;
   const bool wide = (reinterpret_cast<uintptr_t>(q) / 4 - r.shift) % 4 == 0;
+  const int first = column<T, RUN>(r, c, 0, lane);
+  if (wide && inside(r, c)) {
 #pragma unroll
-  for (int i = 0; i < kPer / N; ++i) {
-    const int e = column<T, RUN>(r, c, i, lane);
-    if (wide && e >= 0 && e + N <= r.V) {
+    for (int i = 0; i < kPer / N; ++i) {
 #pragma unroll
       for (int k = 0; k < N; k += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(q + e + k);
+        const float4 v = *reinterpret_cast<const float4*>(q + first + (RUN ? i : i * 32) * N + k);
         x[i * N + k] = v.x, x[i * N + k + 1] = v.y, x[i * N + k + 2] = v.z, x[i * N + k + 3] = v.w;
       }
-    } else {
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer / N; ++i) {
+      const int e = first + (RUN ? i : i * 32) * N;
 #pragma unroll
       for (int k = 0; k < N; ++k) x[i * N + k] = e + k >= 0 && e + k < r.V ? q[e + k] : 0.f;
     }
   }
 }
 
-SPEC_DEV float pair_sum(const float (&x)[kPer]) {
-  float s[kPer];
+template <class W>
+SPEC_DEV W warp_total(W v) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s[i] = x[i];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+template <class W>
+SPEC_DEV W warp_scan(W v, int lane) {  // inclusive
 #pragma unroll
-  for (int o = kPer / 2; o > 0; o >>= 1)
+  for (int o = 1; o < 32; o <<= 1) {
+    const W w = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += w;
+  }
+  return v;
+}
+template <class W, int N>
+SPEC_DEV W tree_sum(const W (&x)[N]) {
+  W s[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] = x[i];
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1)
 #pragma unroll
     for (int i = 0; i < o; ++i) s[i] += s[i + o];
   return s[0];
@@ -253,14 +300,48 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
   pdl_wait();
   const int row = (int)(at / per_row), c0 = (int)(at - row * per_row) * C;
   if (row >= r.n_rows) return;
-  if (r.path && c0 == 0 && lane == 0) r.path[row] = -1;
+  if (c0 == 0 && lane == 0) {
+    if (r.path) r.path[row] = -1;
+    if (r.drafts) {  // what the verification asks about the row's draft
+      const int x = r.drafts[row];
+      const bool judged = x >= 0 && x < r.V;
+      r.seen[row] = judged ? make_float2(r.q[row * r.q_stride + x], to_float((static_cast<const T*>(r.logits) + row * r.stride)[x]))
+                           : make_float2(0.f, 0.f);
+    }
+  }
   const Row<T> rr(r, row);
   uint4 v[C * NV];
+  const int first = c0 * kChunk - rr.shift;
+  if (first >= 0 && first + C * kChunk <= rr.V) {
+    const uint4* at = reinterpret_cast<const uint4*>(rr.p + first) + lane;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
+    for (int i = 0; i < C * NV; ++i) v[i] = at[i * 32];
+  } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[c * NV + i] = load_vec(rr, column<T, false>(rr, c0 + c, i, lane));
-  const float m = redux_max(largest(v, rr.p));
+    for (int i = 0; i < C * NV; ++i) v[i] = load_vec(rr, first + (i * 32 + lane) * N);
+  }
+  const float m = redux_max(largest<C * NV>(v, rr.p));
+  if (rr.t == 0.f) {  // only the first largest logit counts: its column stands in the sum's place
+    bool nan = false;
+    int at_column = 0x7fffffff;
+#pragma unroll
+    for (int i = C * NV - 1; i >= 0; --i) {
+      float y[N];
+      unpack(v[i], y, rr.p);
+#pragma unroll
+      for (int k = N - 1; k >= 0; --k) {
+        nan |= y[k] != y[k];
+        if (y[k] == m) at_column = first + (i * 32 + lane) * N + k;
+      }
+    }
+    at_column = __reduce_min_sync(0xffffffffu, at_column);
+    nan = __any_sync(0xffffffffu, nan);
+    if (m == -INFINITY) at_column = 0;  // outside the row as well
+    if (lane < C)
+      r.stats[(long long)row * r.nch + c0 + lane] =
+          lane ? make_float2(-INFINITY, 0.f) : make_float2(m, nan ? NAN : __int_as_float(at_column));
+    return;
+  }
   const Ref ref(m == -INFINITY ? 0.f : m, rr.h);
   float s[C];
 #pragma unroll
@@ -280,44 +361,31 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
 #pragma unroll
       for (int i = 0; i < kPer; ++i) x[i] = ex2((x[i] - ref.m) * ref.h);
     }
-    s[c] = pair_sum(x);
+    s[c] = tree_sum(x);
   }
-  float2* out = r.stats + (long long)row * r.nch + c0;
-  if constexpr (C == 4) {
-    // Four sums over the lanes at once: lanes 8 c .. end with chunk c's.
-    const bool up = lane & 16, odd = lane & 8;
-    float a = up ? s[2] : s[0], b = up ? s[3] : s[1];
-    a += __shfl_xor_sync(0xffffffffu, up ? s[0] : s[2], 16);
-    b += __shfl_xor_sync(0xffffffffu, up ? s[1] : s[3], 16);
-    float t = odd ? b : a;
-    t += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
-    t += __shfl_xor_sync(0xffffffffu, t, 4);
-    t += __shfl_xor_sync(0xffffffffu, t, 2);
-    t += __shfl_xor_sync(0xffffffffu, t, 1);
-    if (lane % 8 == 0) out[lane / 8] = make_float2(m, t);
-  } else {
-    const float t = specb200::warp_sum(s[0]);
-    if (lane == 0) out[0] = make_float2(m, t);
+  // The sums over the lanes, C at once: each round halves the sums that a lane holds, until it has one.
+  int mine = 0;
+#pragma unroll
+  for (int n = C, o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      const bool up = lane & o;
+      n /= 2;
+      mine = mine * 2 + up;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const float keep = up ? s[i + n] : s[i], give = up ? s[i] : s[i + n];
+        s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    } else {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    }
   }
+  if (lane % (32 / C) == 0) r.stats[(long long)row * r.nch + c0 + mine] = make_float2(m, s[0]);
 }
 
 // ---------------------------------------------------------------------------
 // Joining a row's chunks (one warp)
 // ---------------------------------------------------------------------------
-SPEC_DEV double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-SPEC_DEV double warp_scan(double v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double w = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += w;
-  }
-  return v;
-}
-
 // 8 chunks a lane: of chunks 256 b .. 256 b + 255 those from 8 lane on.
 constexpr int kBlock = 256;
 
@@ -352,15 +420,15 @@ struct Stats {
 // 2^e for a whole e <= 0.
 SPEC_DEV float whole_pow2(float e) { return e < -126.f ? 0.f : __int_as_float((127 + (int)e) << 23); }
 // Weight of a chunk's statistics with the row's reference.
-SPEC_DEV double chunk_weight(float2 v, const Ref& row) {
+SPEC_DEV float chunk_weight(float2 v, const Ref& row) {
   const Ref own(v.x, row.h);
-  if (own.whole && row.whole) return (double)(v.y * whole_pow2(own.R - row.R));
-  return (double)(v.y * ex2(row.whole ? fmaf(v.x, row.h, -row.R) : own.whole ? fmaf(-row.m, row.h, own.R) : (v.x - row.m) * row.h));
+  if (own.whole && row.whole) return v.y * whole_pow2(own.R - row.R);
+  return v.y * ex2(row.whole ? fmaf(v.x, row.h, -row.R) : own.whole ? fmaf(-row.m, row.h, own.R) : (v.x - row.m) * row.h);
 }
 
 struct Joined {
   Ref ref;
-  double Z;  // where the reference is whole
+  float Z;  // where the reference is whole
   bool ok;   // the row has a finite largest logit, no NaN and a temperature
 };
 
@@ -377,103 +445,74 @@ SPEC_DEV Joined join(const Row<T>& r, const Stats& st) {
   m = redux_max(m);
   j.ref = Ref(m, r.h);
   j.ok = r.ok && m > -INFINITY && m < INFINITY && !__any_sync(0xffffffffu, nan);
-  double z = 0;
+  j.Z = 0;
   st.each([&](int, const float2(&v)[8]) {
+    float w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) z += chunk_weight(v[i], j.ref);
+    for (int i = 0; i < 8; ++i) w[i] = chunk_weight(v[i], j.ref);
+    j.Z += warp_total(tree_sum(w));
     return true;
   });
-  j.Z = warp_sum(z);
   return j;
 }
 
-// Of 8 values a lane in 256 chunks: the first chunk whose cumulative weight
-// passes `target` (run: the weight before them, moved past them where none does).
-SPEC_DEV int find_in_block(const double (&w)[8], int b, double target, int lane, double* run) {
-  double own = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) own += w[i];
-  const double incl = warp_scan(own, lane) + *run;
-  double at = __shfl_up_sync(0xffffffffu, incl, 1);  // not above the target where incl passes it
-  if (lane == 0) at = *run;
-  const unsigned hit = __ballot_sync(0xffffffffu, incl > target);
+// Of N values a lane, one lane's after another: the first whose cumulative
+// sum passes `target`, and the sums before and with it (from `base` on).  Where
+// rounding leaves the lane's own sum a step below the scanned one, its last of
+// some weight.  -1: none; then *with is the sum of all.
+template <class W, int N>
+SPEC_DEV int find(const W (&w)[N], double base, double target, int lane, double* before, double* with) {
+  const W own = tree_sum(w), incl = warp_scan(own, lane);
+  W excl = __shfl_up_sync(0xffffffffu, incl, 1);
+  if (lane == 0) excl = 0;
+  // Of a weight: the lanes' sums are added in different orders, so that one of
+  // no weight may stand a step above the lane before it.
+  const unsigned hit = __ballot_sync(0xffffffffu, own > 0 && base + (double)incl > target);
   if (!hit) {
-    *run = __shfl_sync(0xffffffffu, incl, 31);
+    *with = base + (double)__shfl_sync(0xffffffffu, incl, 31);
     return -1;
   }
   const int who = __ffs(hit) - 1;
-  // Rounding may leave the sum of all a step below the scanned one: then the last chunk of some weight.
-  int found = -1;
-  double before = at;
+  // In the lane: sums from its own start, against what is left of the target.
+  const W left = (W)(target - (base + (double)excl));
+  int at = 0;
+  W from = 0, run = 0;
   bool open = true;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (open && w[i] > 0) {
-      found = b * kBlock + lane * 8 + i;
-      before = at;
-      at += w[i];
-      open = at <= target;
-    }
-  *run = __shfl_sync(0xffffffffu, before, who);
-  return __shfl_sync(0xffffffffu, found, who);
-}
-
-// The first of a chunk's columns whose cumulative weight passes `target`;
-// w[i]: weights of this lane's 16 columns, one after another.  Where none
-// does, the last column of some weight.  [lo, hi): cumulative weights around it.
-template <class T, class W>
-SPEC_DEV int find_column(const Row<T>& r, int c, const W (&w)[kPer], double before, double target, int lane, double* lo,
-                         double* hi) {
-  const int e = column<T, true>(r, c, 0, lane);
-  double own = 0;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) own += (double)w[i];
-  const double incl = warp_scan(own, lane) + before;
-  double at = __shfl_up_sync(0xffffffffu, incl, 1);
-  if (lane == 0) at = before;
-  const unsigned hit = __ballot_sync(0xffffffffu, incl > target), some = __ballot_sync(0xffffffffu, own > 0);
-  if (!some) return -1;
-  const int who = hit ? __ffs(hit) - 1 : 31 - __clz(some);
-  int tok = -1;
-  double from = at;
-  bool open = true;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (open && w[i] > 0) {
-      tok = e + i;
-      from = at;
-      at += (double)w[i];
-      open = !hit || at <= target;
-    }
-  *lo = __shfl_sync(0xffffffffu, hit ? from : -1.0, who);
-  *hi = __shfl_sync(0xffffffffu, at, who);
-  return __shfl_sync(0xffffffffu, tok, who);
-}
-
-// The first column with the row's largest logit.
-template <class T>
-SPEC_DEV int first_largest(const Row<T>& r, const Stats& st, float M) {
-  int c = 0x7fffffff;
-  st.each([&](int b, const float2(&v)[8]) {
-#pragma unroll
-    for (int i = 7; i >= 0; --i)
-      if (v[i].x == M) c = b * kBlock + st.lane * 8 + i;
-    return !__any_sync(0xffffffffu, c < 0x7fffffff);
-  });
-  c = __reduce_min_sync(0xffffffffu, c);
-  // Chunks with one reference share the largest logit that stands beside their sums.
-#pragma unroll 1
-  for (; c < st.nch; ++c) {
-    float x[kPer];
-    load_chunk<T, true>(r, c, st.lane, x);
-    int e = 0x7fffffff;
-#pragma unroll
-    for (int i = kPer - 1; i >= 0; --i)
-      if (x[i] == M) e = column<T, true>(r, c, 0, st.lane) + i;
-    e = __reduce_min_sync(0xffffffffu, e);
-    if (e < 0x7fffffff) return e;
+  for (int i = 0; i < N; ++i) {
+    const W next = run + w[i];
+    const bool take = open && w[i] > 0;
+    at = take ? i : at;
+    from = take ? run : from;
+    run = open ? next : run;
+    open = open && !(next > left);
   }
-  return kBad;
+  *before = base + (double)excl + (double)from;
+  *with = base + (double)excl + (double)run;
+  *before = __shfl_sync(0xffffffffu, *before, who);
+  *with = __shfl_sync(0xffffffffu, *with, who);
+  return who * N + __shfl_sync(0xffffffffu, at, who);
+}
+// The last of some weight, or -1.
+template <class W, int N>
+SPEC_DEV int find_last(const W (&w)[N], int lane) {
+  int at = -1;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (w[i] > 0) at = lane * N + i;
+  return __reduce_max_sync(0xffffffffu, at);
+}
+
+// The first column with the row's largest logit, at temperature 0.
+SPEC_DEV int first_largest(const Stats& st, float M) {
+  int e = 0x7fffffff;
+  st.each([&](int, const float2(&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (v[i].x == M) e = min(e, __float_as_int(v[i].y));
+    return true;
+  });
+  return __reduce_min_sync(0xffffffffu, e);
 }
 
 SPEC_DEV double unit(float u) { return (double)fminf(fmaxf(u, 0.f), 1.f); }  // NaN: 0
@@ -482,25 +521,31 @@ SPEC_DEV double unit(float u) { return (double)fminf(fmaxf(u, 0.f), 1.f); }  // 
 template <class T>
 SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
   if (!j.ok) return kBad;
-  if (r.t == 0.f) return first_largest(r, st, j.ref.m);
-  const double target = unit(u) * j.Z, slack = (target < 1 ? 4 : 2) * kErr * target;
+  if (r.t == 0.f) return first_largest(st, j.ref.m);
+  const double target = unit(u) * (double)j.Z, slack = (target < 1 ? 4 : 2) * kErr * target;
   if (!j.ref.whole || target <= 0x1p-33) return kUnsure;
   double run = 0, lo, hi;
   int c = -1;
   st.each([&](int b, const float2(&v)[8]) {
-    double w[8];
+    float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = chunk_weight(v[i], j.ref);
-    c = find_in_block(w, b, target, st.lane, &run);
-    return c < 0;
+    c = find(w, run, target, st.lane, &lo, &hi);
+    if (c < 0) {
+      run = hi;
+      return true;
+    }
+    c += b * kBlock;
+    run = lo;
+    return false;
   });
   if (c < 0) return kUnsure;
   float x[kPer];
   load_chunk<T, true>(r, c, st.lane, x);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) x[i] = ex2(fmaf(x[i], j.ref.h, -j.ref.R));
-  const int tok = find_column(r, c, x, run, target, st.lane, &lo, &hi);
-  return tok >= 0 && lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
+  const int e = find(x, run, target, st.lane, &lo, &hi);
+  return e >= 0 && lo + slack <= target && target + slack < hi ? c * kChunk - r.shift + e : kUnsure;
 }
 
 // ---------------------------------------------------------------------------
@@ -510,80 +555,107 @@ SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
 // in f32 (REST32) or in 64 bits (REST64).
 enum : int { P64 = 0, REST32 = 1, REST64 = 2 };
 
-// 2^y for y <= 0 in 64 bits: the Taylor series of 2^f, |f| <= 1/2, to
-// (f ln 2)^13 / 13! (the next term is below 2^-57), times the whole power.
-SPEC_DEV double pow2_64(double y) {
-  constexpr double kLn2 = 0.693147180559945309;
-  const double n = rint(fmax(y, -1100.0)), f = (fmax(y, -1100.0) - n) * kLn2;
-  double s = 1.0 / 6227020800;
-  s = fma(s, f, 1.0 / 479001600);
-  s = fma(s, f, 1.0 / 39916800);
-  s = fma(s, f, 1.0 / 3628800);
-  s = fma(s, f, 1.0 / 362880);
-  s = fma(s, f, 1.0 / 40320);
-  s = fma(s, f, 1.0 / 5040);
-  s = fma(s, f, 1.0 / 720);
-  s = fma(s, f, 1.0 / 120);
-  s = fma(s, f, 1.0 / 24);
-  s = fma(s, f, 1.0 / 6);
-  s = fma(s, f, 0.5);
-  s = fma(s, f, 1.0);
-  s = fma(s, f, 1.0);
-  // In two steps, so that results below 2^-1022 keep what bits they have.
-  const int e = (int)n, half = e / 2;
-  return s * __hiloint2double((1023 + half) << 20, 0) * __hiloint2double((1023 + e - half) << 20, 0);
-}
+// 2^y for y <= 0 in 64 bits: y = n + i / 64 + f, |f| <= 1 / 128, 2^(i / 64) from
+// a table and the Taylor series of 2^f to (f ln 2)^5 / 5! (the next term is below
+// 2^-54).  Below 2^-1000: zero.
+struct Powers {
+  double of[64];
+  SPEC_DEV void fill() {  // all threads of the block; they sync before its use
+    if (threadIdx.x < 64) of[threadIdx.x] = exp2((double)(int)threadIdx.x / 64);
+  }
+  // y in 64ths
+  SPEC_DEV double pow(double y) const {
+    constexpr double kLn2 = 0.693147180559945309 / 64, kWhole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    y = fmax(y, -64.0 * 1100);
+    const double t = y + kWhole, f = (y - (t - kWhole)) * kLn2;
+    double s = fma(f, 1.0 / 120, 1.0 / 24);
+    s = fma(s, f, 1.0 / 6);
+    s = fma(s, f, 0.5);
+    s = fma(s, f, 1.0);
+    s = s * f;
+    const int n = __double2loint(t);
+    const double b = of[n & 63], w = fma(s, b, b);
+    const int e = n >> 6;
+    return e < -1000 ? 0.0 : __hiloint2double(__double2hiint(w) + (e << 20), __double2loint(w));
+  }
+};
 
 template <class T>
 struct Weigher {
   const Row<T>& r;
   const Ref& ref;
   const float* q;
+  float inv_zf;
   double h, inv_z;
-  SPEC_DEV Weigher(const Row<T>& r_, const Ref& ref_, const float* q_, double Z) : r(r_), ref(ref_), q(q_) {
-    h = 1.44269504088896341 / (double)r.t;
-    inv_z = q ? 1.0 / Z : 0.0;
+  const Powers* powers;
+  SPEC_DEV Weigher(const Row<T>& r_, const Ref& ref_, const float* q_, int kind, double Z, const Powers* powers_ = nullptr)
+      : r(r_), ref(ref_), q(q_), powers(powers_) {
+    if (kind == REST32) {
+      inv_zf = 1.f / (float)Z;
+    } else {
+      h = 64 * 1.44269504088896341 / (double)r.t;
+      inv_z = 1.0 / Z;
+    }
   }
-  SPEC_DEV double p64(float x) const { return pow2_64(((double)x - (double)ref.m) * h); }
-  template <bool RUN>
-  SPEC_DEV void rest32(int c, int lane, float (&w)[kPer]) const {
-    float y[kPer];
-    load_chunk<T, RUN>(r, c, lane, w);
-    load_probs<T, RUN>(r, q, c, lane, y);
-    const float z = (float)inv_z;
+  SPEC_DEV double p64(float x) const { return powers->pow(((double)x - (double)ref.m) * h); }
+  SPEC_DEV void rest32(float (&x)[kPer], const float (&y)[kPer]) const {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] = fmaxf(fmaf(ex2(fmaf(w[i], ref.h, -ref.R)), z, -y[i]), 0.f);
+    for (int i = 0; i < kPer; ++i) x[i] = fmaxf(fmaf(ex2(fmaf(x[i], ref.h, -ref.R)), inv_zf, -y[i]), 0.f);
   }
-  template <bool RUN>
-  SPEC_DEV void exact(int kind, int c, int lane, double (&w)[kPer]) const {
-    float x[kPer];
-    load_chunk<T, RUN>(r, c, lane, x);
+  SPEC_DEV void exact(int kind, const float (&x)[kPer], const float (&y)[kPer], double (&w)[kPer]) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) w[i] = p64(x[i]);
     if (kind == REST64) {
-      load_probs<T, RUN>(r, q, c, lane, x);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) w[i] = fmax(w[i] * inv_z - (double)x[i], 0.0);
+      for (int i = 0; i < kPer; ++i) w[i] = fmax(w[i] * inv_z - (double)y[i], 0.0);
     }
   }
-  // Chunk sums by all warps of the cluster; the caller syncs it.
+  // Chunk sums by all warps of the cluster, a chunk's loads ahead; the caller syncs it.
   SPEC_DEV void sum(int kind, double* sums, int nch, int lane) const {
+    constexpr int NV = kPer / Vec<T>::N;
+    const int nw = blockDim.x >> 5, step = nw * cluster_size();
+    int c = cluster_rank() * nw + (threadIdx.x >> 5);
+    uint4 v[NV];
+    if (c < nch) load_raw<T, false>(r, c, lane, v);
+#pragma unroll 1
+    for (; c < nch; c += step) {
+      float x[kPer], y[kPer];
+      unpack_chunk(v, x, r.p);
+      if (kind == REST64) load_probs<T, false>(r, q, c, lane, y);
+      if (c + step < nch) load_raw<T, false>(r, c + step, lane, v);
+      double s = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const double w = p64(x[i]);
+        s += kind == REST64 ? fmax(w * inv_z - (double)y[i], 0.0) : w;
+      }
+      s = warp_total(s);
+      if (lane == 0) __stcg(sums + c, s);
+    }
+  }
+  // The same of REST32, two chunks' loads at a time.
+  SPEC_DEV void sum32(float* sums, int nch, int lane) const {
+    constexpr int NV = kPer / Vec<T>::N;
     const int nw = blockDim.x >> 5, step = nw * cluster_size();
 #pragma unroll 1
-    for (int c = cluster_rank() * nw + (threadIdx.x >> 5); c < nch; c += step) {
-      double s = 0;
-      if (kind == REST32) {
-        float w[kPer];
-        rest32<false>(c, lane, w);
-        s = (double)specb200::warp_sum(pair_sum(w));
-      } else {
-        double w[kPer];
-        exact<false>(kind, c, lane, w);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) s += w[i];
-        s = warp_sum(s);
+    for (int c = cluster_rank() * nw + (threadIdx.x >> 5); c < nch; c += 2 * step) {
+      const int d = c + step < nch ? c + step : c;
+      uint4 v[NV], w[NV];
+      float y[kPer], z[kPer], x[kPer];
+      load_raw<T, false>(r, c, lane, v);
+      load_probs<T, false>(r, q, c, lane, y);
+      load_raw<T, false>(r, d, lane, w);
+      load_probs<T, false>(r, q, d, lane, z);
+      unpack_chunk(v, x, r.p);
+      rest32(x, y);
+      const float s = warp_total(tree_sum(x));
+      unpack_chunk(w, x, r.p);
+      rest32(x, z);
+      const float t = warp_total(tree_sum(x));
+      if (lane == 0) {
+        __stcg(sums + c, s);
+        if (d != c) __stcg(sums + d, t);
       }
-      if (lane == 0) __stcg(sums + c, s);
     }
   }
 };
@@ -602,102 +674,159 @@ SPEC_DEV double total(const double* sums, int nch, int lane) {
   for (int b = 0; b * kBlock < nch; ++b) {
     double w[8];
     load_sums(sums, b, nch, lane, w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += w[i];
+    s += warp_total(tree_sum(w));
   }
-  return warp_sum(s);
+  return s;
 }
 
-// A token of the weights in `sums`, whose sum is Zs: exact for P64 and REST64.
+// A token of the weights in `sums`, whose sum is Zs, in 64 bits.
 template <class T>
 SPEC_DEV int draw_sums(const Weigher<T>& f, int kind, const double* sums, int nch, double Zs, float u, int lane) {
   const double target = unit(u) * Zs;
-  double run = 0, lo = -1, hi;
+  double run = 0, lo, hi;
   int c = -1, last = -1;
   for (int b = 0; b * kBlock < nch && c < 0; ++b) {
     double w[8];
     load_sums(sums, b, nch, lane, w);
-    c = find_in_block(w, b, target, lane, &run);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (w[i] > 0) last = b * kBlock + lane * 8 + i;
+    c = find(w, run, target, lane, &lo, &hi);
+    run = c < 0 ? hi : lo;
+    if (c >= 0) c += b * kBlock;
+    const int some = find_last(w, lane);
+    if (some >= 0) last = b * kBlock + some;
   }
-  double goal = target;
-  if (c < 0) {  // the target is the whole sum: the last column of some weight
-    if (kind == REST32) return kUnsure;
-    c = __reduce_max_sync(0xffffffffu, last);
-    if (c < 0) return kBad;
-    goal = INFINITY;
-  }
-  if (kind == REST32) {
-    float w[kPer];
-    f.template rest32<true>(c, lane, w);
-    const int tok = find_column(f.r, c, w, run, goal, lane, &lo, &hi);
-    // The weights and Z are off by kErr of Z in all, max(p - q, 0) by no more
-    // than p; so the prefix by 2 kErr, and u times the sum likewise.
-    const double slack = 4.25 * kErr;
-    return tok >= 0 && lo >= 0 && lo + slack <= target && target + slack < hi ? tok : kUnsure;
-  }
+  const bool whole = c < 0;  // the target is the sum of all: the last column of some weight
+  if (whole) c = last;
+  if (c < 0) return kBad;
+  float x[kPer], y[kPer];
+  load_chunk<T, true>(f.r, c, lane, x);
+  if (kind == REST64) load_probs<T, true>(f.r, f.q, c, lane, y);
   double w[kPer];
-  f.template exact<true>(kind, c, lane, w);
-  return find_column(f.r, c, w, run, goal, lane, &lo, &hi);
+  f.exact(kind, x, y, w);
+  int e = whole ? -1 : find(w, run, target, lane, &lo, &hi);
+  if (e < 0) e = find_last(w, lane);
+  return e < 0 ? kBad : c * kChunk - f.r.shift + e;
+}
+
+// A token of max(p - q, 0) from REST32 sums, or kUnsure.
+template <class T>
+SPEC_DEV int draw_rest(const Weigher<T>& f, const float* sums, int nch, float u, int lane) {
+  float w[8];
+  auto load = [&](int b) {
+    const int c = b * kBlock + lane * 8;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 x = c < nch ? __ldcg(reinterpret_cast<const float4*>(sums + c + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    }
+  };
+  load(0);
+  double Zs = (double)warp_total(tree_sum(w));
+  for (int b = 1; b * kBlock < nch; ++b) {
+    load(b);
+    Zs += (double)warp_total(tree_sum(w));
+  }
+  const double target = unit(u) * Zs;
+  double run = 0, lo, hi;
+  int c = -1;
+  for (int b = 0; b * kBlock < nch && c < 0; ++b) {
+    if (nch > kBlock) load(b);
+    c = find(w, run, target, lane, &lo, &hi);
+    run = c < 0 ? hi : lo;
+    if (c >= 0) c += b * kBlock;
+  }
+  if (c < 0) return kUnsure;
+  float x[kPer], y[kPer];
+  load_chunk<T, true>(f.r, c, lane, x);
+  load_probs<T, true>(f.r, f.q, c, lane, y);
+  f.rest32(x, y);
+  const int e = find(x, run, target, lane, &lo, &hi);
+  // Weights and Z are off by (39.2 + 60.2) u of Z, max(p - q, 0) by no more
+  // than p, its sums by 41 u: the prefix, and u times the sum likewise.
+  const double slack = 4.5 * kErr;
+  return e >= 0 && lo + slack <= target && target + slack < hi ? c * kChunk - f.r.shift + e : kUnsure;
 }
 
 // ---------------------------------------------------------------------------
 // A cluster a row
 // ---------------------------------------------------------------------------
-constexpr int kSampleThreads = 128;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 
+// Probabilities of this warp's chunks, two chunks' loads at a time.
 template <class T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleParams p) {
+SPEC_DEV void write_probs(const SampleParams& p, const Row<T>& r, const Joined& j, int top, int row, int warp, int lane) {
+  constexpr int N = Vec<T>::N, NV = kPer / N;
+  const int nch = p.r.nch, step = kWarps * cluster_size();
+  float* out = p.probs + row * p.probs_stride;
+  const float inv = 1.f / j.Z;
+  const bool wide = (reinterpret_cast<uintptr_t>(out) / 4 - r.shift) % 4 == 0;
+  auto write = [&](int c, const uint4* v) {
+    float x[kPer];
+    unpack_chunk(v, x, r.p);
+    const int first = column<T, false>(r, c, 0, lane);
+    if (!j.ok || r.t == 0.f) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = j.ok && first + i / N * 32 * N + i % N == top ? 1.f : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = j.ref.weight(x[i]) * inv;
+    }
+    const bool all = wide && inside(r, c);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = first + i * 32 * N;
+      if (all) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4)
+          *reinterpret_cast<float4*>(out + e + k) = make_float4(x[i * N + k], x[i * N + k + 1], x[i * N + k + 2], x[i * N + k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (e + k >= 0 && e + k < r.V) out[e + k] = x[i * N + k];
+      }
+    }
+  };
+#pragma unroll 1
+  for (int c = cluster_rank() * kWarps + warp; c < nch; c += 2 * step) {
+    const int d = c + step < nch ? c + step : c;
+    uint4 v[NV], w[NV];
+    load_raw<T, false>(r, c, lane, v);
+    load_raw<T, false>(r, d, lane, w);
+    write(c, v);
+    if (d != c) write(d, w);
+  }
+}
+
+template <class T, bool PROBS>
+__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_constant__ SampleParams p) {
   __shared__ int s_tok;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = kSampleThreads / 32;
-  const int rank = cluster_rank(), size = cluster_size(), row = blockIdx.x / size;
+  __shared__ Powers s_powers;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = cluster_rank(), row = blockIdx.x / cluster_size();
   pdl_launch_dependents();
   pdl_wait();
   const Row<T> r(p.r, row);
   const int nch = p.r.nch;
   const float u = p.r.u[row];
-  const Stats st(p.r.stats + (long long)row * nch, nch, lane);
   double* sums = p.r.sums + (long long)row * nch;
-  const Joined j = join(r, st);
-  int tok = kUnsure;
-  if (warp == 0) {
-    tok = draw(r, st, j, u);
-    if (lane == 0) s_tok = tok;
-  }
-  if (p.probs) {
-    float* out = p.probs + row * p.probs_stride;
-    const float inv = (float)(1.0 / j.Z);
-    const int top = j.ok && r.t == 0.f ? first_largest(r, st, j.ref.m) : -1;
-    const bool wide = (reinterpret_cast<uintptr_t>(out) / 4 - r.shift) % 4 == 0;
-    constexpr int N = Vec<T>::N;
-#pragma unroll 1
-    for (int c = rank * nw + warp; c < nch; c += nw * size) {
-      float x[kPer];
-      load_chunk<T, false>(r, c, lane, x);
-#pragma unroll
-      for (int i = 0; i < kPer / N; ++i) {
-        const int e = column<T, false>(r, c, i, lane);
-        float y[N];
-#pragma unroll
-        for (int k = 0; k < N; ++k) y[k] = !j.ok ? 0.f : r.t == 0.f ? (e + k == top ? 1.f : 0.f) : j.ref.weight(x[i * N + k]) * inv;
-        if (wide && e >= 0 && e + N <= r.V) {
-#pragma unroll
-          for (int k = 0; k < N; k += 4)
-            *reinterpret_cast<float4*>(out + e + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; ++k)
-            if (e + k >= 0 && e + k < r.V) out[e + k] = y[k];
-        }
-      }
+  Joined j;
+  if (PROBS || warp == 0) {
+    const Stats st(p.r.stats + (long long)row * nch, nch, lane);
+    j = join(r, st);
+    if (PROBS && warp) write_probs(p, r, j, r.t == 0.f && j.ok ? first_largest(st, j.ref.m) : -1, row, warp, lane);
+    if (warp == 0) {
+      const int tok = draw(r, st, j, u);
+      if (PROBS) write_probs(p, r, j, tok, row, warp, lane);
+      if (lane == 0) s_tok = tok;
     }
   }
   __syncthreads();
-  tok = s_tok;
+  int tok = s_tok;
   if (tok == kUnsure) {
-    const Weigher<T> f(r, j.ref, nullptr, 0);
+    if (!PROBS && warp) j = join(r, Stats(p.r.stats + (long long)row * nch, nch, lane));
+    s_powers.fill();
+    __syncthreads();
+    const Weigher<T> f(r, j.ref, nullptr, P64, 1, &s_powers);
     f.sum(P64, sums, nch, lane);
     cluster_sync();
     if (rank || warp) return;
@@ -709,9 +838,6 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
 // ---------------------------------------------------------------------------
 // A cluster a sequence: chains
 // ---------------------------------------------------------------------------
-constexpr int kVerifyThreads = 256;
-constexpr int kVerifyWarps = kVerifyThreads / 32;
-
 enum : int { A_REJECT = 0, A_ACCEPT = 1, A_UNSURE = 2, A_BAD = 3, A_END = 4 };
 
 // Rows first .. last of sequence b, empty where row_start says nothing sound.
@@ -721,10 +847,19 @@ SPEC_DEV int rows_of(const VerifyParams& p, int b, int* first) {
   return r0 >= 0 && r1 >= r0 && r1 <= p.r.n_rows ? r1 - r0 : 0;
 }
 
+// What the walk knows of a row.
+struct Judged {
+  Joined join;
+  int verdict, x;    // its draft
+  float qx, lx;      // the draft's probability and the row's logit of it
+  float u, t, h;
+};
+
 template <class T>
-__global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_constant__ VerifyParams p) {
-  __shared__ int s_verdict[kVerifyWarps], s_tok;
-  __shared__ Joined s_join[kVerifyWarps];
+__global__ void __launch_bounds__(kThreads, 3) chain_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ Judged s_row[kWarps];
+  __shared__ int s_tok;
+  __shared__ Powers s_powers;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), b = blockIdx.x / cluster_size(), nch = p.r.nch;
   pdl_launch_dependents();
@@ -734,55 +869,60 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
   double* sums = p.r.sums + (long long)(n ? r0 : 0) * nch;
   bool used = false;  // other blocks may still read `sums`
   int at = 0, verdict = n ? A_ACCEPT : A_BAD;  // the row under decision; why the walk stopped
-  Joined j;
+  Judged row;
   double z64 = 0;  // of row `at`, once summed in 64 bits
   // The walk, a row a warp.  Every block of the cluster comes to the same verdicts.
 #pragma unroll 1
-  for (int base = 0; base < n && verdict == A_ACCEPT; base += kVerifyWarps) {
+  for (int base = 0; base < n && verdict == A_ACCEPT; base += kWarps) {
     if (base + warp < n) {
-      const int i = base + warp, row = r0 + i;
-      const int x = i + 1 < n ? p.tokens[row] : -1;
-      const Row<T> r(p.r, row);
-      const Stats st(p.r.stats + (long long)row * nch, nch, lane);
-      const bool judged = x >= 0 && x < p.r.V;
-      const float u = p.r.u[row], q = judged ? p.q[row * p.q_stride + x] : 0.f, lx = judged ? to_float(r.p[x]) : 0.f;
-      const Joined w = join(r, st);
+      const int i = base + warp, at_row = r0 + i;
+      const Stats st(p.r.stats + (long long)at_row * nch, nch, lane);
+      const float2 seen = __ldcg(p.r.seen + at_row);
+      const Row<T> r(p.r, at_row);
+      Judged w;
+      w.x = i + 1 < n ? p.tokens[at_row] : -1;
+      w.u = p.r.u[at_row];
+      w.t = r.t, w.h = r.h;
+      w.qx = seen.x, w.lx = seen.y;
+      w.join = join(r, st);
       int v = A_END;
-      if (!w.ok) {
+      if (!w.join.ok) {
         v = A_BAD;
-      } else if (judged) {
-        const double left = unit(u) * (double)q;
-        if (q <= 0.f) {
+      } else if (w.x >= 0 && w.x < p.r.V) {
+        const double left = unit(w.u) * (double)w.qx;
+        if (w.qx <= 0.f) {
           v = A_ACCEPT;
         } else if (r.t == 0.f) {
-          v = left <= (x == first_largest(r, st, w.ref.m) ? 1.0 : 0.0);
+          v = left <= (w.x == first_largest(st, w.join.ref.m) ? 1.0 : 0.0);
         } else {
-          const double px = (double)w.ref.weight(lx), lz = left * w.Z;
+          const double px = (double)w.join.ref.weight(w.lx), lz = left * (double)w.join.Z;
           // w_x alone: off by (4.5 + 2.5 * 23) u where it is above 2^-33.
           const double slack = 3 * kErr * lz + 0x1p-33;
-          v = !w.ref.whole ? A_UNSURE : lz + slack < px ? A_ACCEPT : lz > px + slack ? A_REJECT : A_UNSURE;
-          if (q != q) v = A_REJECT;
+          v = !w.join.ref.whole ? A_UNSURE : lz + slack < px ? A_ACCEPT : lz > px + slack ? A_REJECT : A_UNSURE;
+          if (w.qx != w.qx) v = A_REJECT;
         }
       }
-      if (lane == 0) s_verdict[warp] = v, s_join[warp] = w;
+      w.verdict = v;
+      if (lane == 0) s_row[warp] = w;
     }
     __syncthreads();
 #pragma unroll 1
-    for (int w = 0; w < kVerifyWarps && base + w < n; ++w) {
+    for (int w = 0; w < kWarps && base + w < n; ++w) {
       at = base + w;
-      verdict = s_verdict[w];
-      j = s_join[w];
+      verdict = s_row[w].verdict;
+      if (verdict == A_ACCEPT) continue;
+      row = s_row[w];
       if (verdict == A_UNSURE) {
         const Row<T> r(p.r, r0 + at);
-        const Weigher<T> f(r, j.ref, nullptr, 0);
+        const Weigher<T> f(r, row.join.ref, nullptr, P64, 1, &s_powers);
+        s_powers.fill();
+        __syncthreads();
         if (used) cluster_sync();
         f.sum(P64, sums, nch, lane);
         cluster_sync();
         used = true;
         z64 = total(sums, nch, lane);
-        const int x = p.tokens[r0 + at];
-        const double left = unit(p.r.u[r0 + at]) * (double)p.q[(r0 + at) * p.q_stride + x];
-        verdict = left * z64 <= f.p64(to_float(r.p[x])) ? A_ACCEPT : A_REJECT;
+        verdict = unit(row.u) * (double)row.qx * z64 <= f.p64(row.lx) ? A_ACCEPT : A_REJECT;
         if (verdict == A_ACCEPT) z64 = 0;
       }
       if (verdict != A_ACCEPT) break;
@@ -791,31 +931,36 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
   }
   int tok = kBad;
   if (verdict != A_BAD) {
-    const int row = r0 + at;
-    const Row<T> r(p.r, row);
-    const Stats st(p.r.stats + (long long)row * nch, nch, lane);
     const bool rest = verdict == A_REJECT;
-    const float* q = rest ? p.q + row * p.q_stride : nullptr;
-    const float u = p.r.u[row + rest];  // a row follows every draft
+    const float* q = rest ? p.q + (r0 + at) * p.q_stride : nullptr;
+    const float u = rest ? p.r.u[r0 + at + 1] : row.u;  // a row follows every draft
+    Row<T> r;
+    r.place(p.r, r0 + at);
+    r.t = row.t, r.h = row.h, r.ok = true;
+    const Ref ref = row.join.ref;
     tok = kUnsure;
-    if (r.t == 0.f) {
-      // All of p on one token: what is left of it is that token, unless q holds it all too.
-      if (warp == 0) tok = first_largest(r, st, j.ref.m);
-    } else if (!rest) {
-      if (warp == 0) tok = draw(r, st, j, u);
-    } else if (j.ref.whole && z64 == 0) {
-      const Weigher<T> f(r, j.ref, q, j.Z);
+    if (r.t == 0.f || !rest) {
+      // Temperature 0, all of p on one token: what q leaves of it is that token.
+      if (warp == 0) {
+        const Stats st(p.r.stats + (long long)(r0 + at) * nch, nch, lane);
+        tok = draw(r, st, row.join, u);
+      }
+    } else if (ref.whole && z64 == 0) {
+      const Weigher<T> f(r, ref, q, REST32, (double)row.join.Z);
+      float* sums32 = reinterpret_cast<float*>(sums);
       if (used) cluster_sync();
-      f.sum(REST32, sums, nch, lane);
+      f.sum32(sums32, nch, lane);
       cluster_sync();
       used = true;
-      if (warp == 0) tok = draw_sums(f, REST32, sums, nch, total(sums, nch, lane), u, lane);
+      if (warp == 0) tok = draw_rest(f, sums32, nch, u, lane);
     }
     if (threadIdx.x == 0) s_tok = tok;
     __syncthreads();
     tok = s_tok;
     if (tok == kUnsure) {
-      const Weigher<T> f(r, j.ref, nullptr, 0);
+      s_powers.fill();
+      __syncthreads();
+      const Weigher<T> f(r, ref, nullptr, P64, 1, &s_powers);
       double z = z64;
       if (z == 0) {
         if (used) cluster_sync();
@@ -826,7 +971,7 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
       int kind = P64;
       double zs = z;
       if (rest) {
-        const Weigher<T> g(r, j.ref, q, z);
+        const Weigher<T> g(r, ref, q, REST64, z, &s_powers);
         cluster_sync();
         g.sum(REST64, sums, nch, lane);
         cluster_sync();
@@ -840,10 +985,7 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
           zs = z;
         }
       }
-      if (rank == 0 && warp == 0) {
-        const Weigher<T> g(r, j.ref, kind == P64 ? nullptr : q, z);
-        tok = draw_sums(g, kind, sums, nch, zs, u, lane);
-      }
+      if (rank == 0 && warp == 0) tok = draw_sums(Weigher<T>(r, ref, q, kind, z, &s_powers), kind, sums, nch, zs, u, lane);
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
@@ -855,17 +997,22 @@ __global__ void __launch_bounds__(kVerifyThreads) chain_kernel(const __grid_cons
 // ---------------------------------------------------------------------------
 // A cluster a sequence: trees
 // ---------------------------------------------------------------------------
+constexpr int kTreeNodes = 512;  // that the walk finds in shared memory
+
 template <class T>
-__global__ void __launch_bounds__(kVerifyThreads) tree_kernel(const __grid_constant__ VerifyParams p) {
-  __shared__ int s_tok;
+__global__ void __launch_bounds__(kThreads, 3) tree_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ int s_tok, s_drawn[kTreeNodes];
+  __shared__ int2 s_node[kTreeNodes];  // parent, token
+  __shared__ Powers s_powers;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), size = cluster_size(), b = blockIdx.x / size, nch = p.r.nch;
   pdl_launch_dependents();
   pdl_wait();
   int r0;
-  const int n = rows_of(p, b, &r0);
+  const int n = rows_of(p, b, &r0), near = min(n, kTreeNodes);
+  for (int i = threadIdx.x; i < near; i += kThreads) s_node[i] = make_int2(p.parents[r0 + i], p.tokens[r0 + i]);
 #pragma unroll 1
-  for (int i = rank * kVerifyWarps + warp; i < n; i += size * kVerifyWarps) {
+  for (int i = rank * kWarps + warp; i < n; i += size * kWarps) {
     const Row<T> r(p.r, r0 + i);
     const float u = p.r.u[r0 + i];
     const Stats st(p.r.stats + (long long)(r0 + i) * nch, nch, lane);
@@ -873,17 +1020,21 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_kernel(const __grid_const
     if (lane == 0) __stcg(p.r.drawn + r0 + i, tok);
   }
   cluster_sync();
+  for (int i = threadIdx.x; i < near; i += kThreads) s_drawn[i] = __ldcg(p.r.drawn + r0 + i);
+  __syncthreads();
   double* sums = p.r.sums + (long long)(n ? r0 : 0) * nch;
   int cur = 0, len = 0, tok = kBad;
 #pragma unroll 1
   while (len < n) {
     if (rank == 0 && threadIdx.x == 0) p.r.path[r0 + len] = cur;
     ++len;
-    tok = __ldcg(p.r.drawn + r0 + cur);
+    tok = cur < kTreeNodes ? s_drawn[cur] : __ldcg(p.r.drawn + r0 + cur);
     if (tok == kUnsure) {
       const Row<T> r(p.r, r0 + cur);
       const Joined j = join(r, Stats(p.r.stats + (long long)(r0 + cur) * nch, nch, lane));
-      const Weigher<T> f(r, j.ref, nullptr, 0);
+      const Weigher<T> f(r, j.ref, nullptr, P64, 1, &s_powers);
+      s_powers.fill();
+      __syncthreads();
       cluster_sync();
       f.sum(P64, sums, nch, lane);
       cluster_sync();
@@ -899,7 +1050,10 @@ __global__ void __launch_bounds__(kVerifyThreads) tree_kernel(const __grid_const
     int child = -1;
 #pragma unroll 1
     for (int i = cur + 1; i < n && tok >= 0; i += 32) {
-      const bool hit = i + lane < n && p.parents[r0 + i + lane] == cur && p.tokens[r0 + i + lane] == tok;
+      int2 node = make_int2(-1, -1);
+      if (i + lane < near) node = s_node[i + lane];
+      else if (i + lane < n) node = make_int2(p.parents[r0 + i + lane], p.tokens[r0 + i + lane]);
+      const bool hit = node.x == cur && node.y == tok;
       const unsigned mask = __ballot_sync(0xffffffffu, hit);
       if (mask) {
         child = i + __ffs(mask) - 1;
@@ -933,33 +1087,36 @@ cudaError_t launch_clusters(K* kernel, int n, int size, int threads, cudaStream_
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-// Blocks a cluster: 8, fewer where those of all clusters would not be resident at once.
-int cluster_for(int n, int threads, int sms) {
+// Blocks a cluster: 8, fewer where all clusters' blocks are more than one and a half times those that are resident at once.
+int cluster_for(int n, int per_sm, int sms) {
   int size = 8;
-  while (size > 1 && (long long)n * size > (long long)sms * (2048 / threads)) size /= 2;
+  while (size > 1 && (long long)n * size * 2 > (long long)sms * per_sm * 3) size /= 2;
   return size;
 }
 
-// A chunk a warp where that is less than the warps that the device holds, else four.
+// A chunk a warp where that is less than the warps that the device holds, else 8 KB.
 template <class T>
 cudaError_t stats(const Rows& r, int sms, cudaStream_t s) {
   const long long chunks = (long long)r.n_rows * r.nch;
   if (chunks <= sms * 64LL) return kv4::launch_overlapping(stats_kernel<T, 1>, dim3((unsigned)(chunks / 8)), 256, 0, s, r);
-  return kv4::launch_overlapping(stats_kernel<T, 4>, dim3((unsigned)((chunks / 4 + 7) / 8)), 256, 0, s, r);
+  constexpr int C = sizeof(T) == 4 ? 4 : 8;
+  return kv4::launch_overlapping(stats_kernel<T, C>, dim3((unsigned)((chunks / C + 7) / 8)), 256, 0, s, r);
 }
 template <class T>
 cudaError_t sample(const SampleParams& p, int sms, cudaStream_t s) {
   const cudaError_t e = stats<T>(p.r, sms, s);
   if (e != cudaSuccess) return e;
-  return launch_clusters(sample_kernel<T>, p.r.n_rows, cluster_for(p.r.n_rows, kSampleThreads, sms), kSampleThreads, s, p);
+  const int size = cluster_for(p.r.n_rows, 4, sms);
+  return p.probs ? launch_clusters(sample_kernel<T, true>, p.r.n_rows, size, kThreads, s, p)
+                 : launch_clusters(sample_kernel<T, false>, p.r.n_rows, size, kThreads, s, p);
 }
 template <class T>
 cudaError_t verify(const VerifyParams& p, bool trees, int sms, cudaStream_t s) {
   const cudaError_t e = p.r.n_rows ? stats<T>(p.r, sms, s) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  const int size = cluster_for(p.n_seqs, kVerifyThreads, sms);
-  return trees ? launch_clusters(tree_kernel<T>, p.n_seqs, size, kVerifyThreads, s, p)
-               : launch_clusters(chain_kernel<T>, p.n_seqs, size, kVerifyThreads, s, p);
+  const int size = cluster_for(p.n_seqs, 3, sms);
+  return trees ? launch_clusters(tree_kernel<T>, p.n_seqs, size, kThreads, s, p)
+               : launch_clusters(chain_kernel<T>, p.n_seqs, size, kThreads, s, p);
 }
 
 }  // namespace
@@ -977,3 +1134,4 @@ cudaError_t launch_verify(const VerifyParams& p, int dtype, bool trees, int sms,
 
 }  // namespace batch
 }  // namespace specb200
+

@@ -23,10 +23,10 @@ def logits(**change):
 
 def test_workspace_bytes(lib):
     assert lib.spec_batch_workspace_bytes(0, 1000, 2) == 0
-    # 16 bytes a chunk of 512 columns (of which up to 7 lie before the row), a multiple of 8 chunks, and 4 a row.
+    # 16 bytes a chunk of 512 columns (of which up to 7 lie before the row), a multiple of 8 chunks, and 8 a row.
     for n, v, dtype, chunks in ((1, 1, 0, 8), (3, 4090, 0, 16), (3, 4089, 0, 8), (3, 4094, 2, 16), (64, 128256, 2, 256)):
         size = lib.spec_batch_workspace_bytes(n, v, dtype)
-        assert n * (16 * chunks + 4) <= size < n * (16 * chunks + 4) + 3 * 256
+        assert n * (16 * chunks + 8) <= size < n * (16 * chunks + 8) + 3 * 256
     for bad in ((-1, 10, 0), (1 << 21, 10, 0), (1, 0, 0), (1, (1 << 20) + 1, 0), (1, 10, 3), (1, 10, -1)):
         assert lib.spec_batch_workspace_bytes(*bad) == -1
 
