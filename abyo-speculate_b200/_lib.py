@@ -139,7 +139,7 @@ class LoraBankDesc(ctypes.Structure):
 class LoraPlanDesc(ctypes.Structure):
     """spec_lora_plan (include/spec_b200.h)."""
 
-    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_units", "n_bare")] + [
+    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_wide", "n_narrow", "n_bare", "reserved")] + [
         ("device_copy", ctypes.c_void_p)]
 
 

@@ -15,8 +15,9 @@ using namespace specb200::lora;
 namespace {
 
 constexpr int kPlanRows = 1 << 20;
+constexpr int kNarrowMost = 16;  // rows of an adapter that the kernel for few rows takes, in units of 8
 
-// Layout of a plan: units (narrow, then those without an adapter), then the rows in their order.
+// Layout of a plan: units (of many rows, of few, those without an adapter), then the rows in their order.
 int64_t plan_bytes(int64_t n_rows) { return n_rows * (int64_t)(sizeof(Unit) + sizeof(int)); }
 
 struct Matrix {
@@ -28,6 +29,13 @@ struct Matrix {
 // Whether 8 elements from any multiple of 8 on are aligned 16-byte accesses.
 bool wide(const void* p, int64_t row, int64_t outer, int size) {
   return !misaligned(p, 16) && row * size % 16 == 0 && outer * size % 16 == 0;
+}
+
+// Blocks a cluster: 8, fewer where all clusters' blocks would not be resident at once.
+int cluster_for(int n, int per_sm, int sms) {
+  int size = 8;
+  while (size > 1 && (int64_t)n * size > (int64_t)sms * per_sm) size /= 2;
+  return size;
 }
 
 int check_plan_shape(const char* what, int64_t n_rows) {
@@ -43,26 +51,37 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   for (int i = 0; i < n_rows; ++i) order[i] = i;
   // By adapter, rows in their order; rows without one last.
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return (unsigned)adapters[x] < (unsigned)adapters[y]; });
-  std::vector<Unit> units;
-  int with = 0;
+  // An adapter's rows in units of equal size.
+  std::vector<Unit> units[3];
   for (int i = 0; i < n_rows;) {
     int e = i;
     const int a = adapters[order[i]];
     while (e < n_rows && adapters[order[e]] == a) ++e;
-    for (int at = i; at < e; at += kNarrowRows) units.push_back(Unit{a, at, std::min(kNarrowRows, e - at), 0});
-    if (a >= 0) with = (int)units.size();
+    const int kind = a < 0 ? 2 : e - i > kNarrowMost ? 0 : 1, most = kind ? kNarrowRows : kWideRows;
+    const int n = (e - i + most - 1) / most;
+    for (int k = 0; k < n; ++k) {
+      const int at = i + (int)((int64_t)(e - i) * k / n), end = i + (int)((int64_t)(e - i) * (k + 1) / n);
+      Unit u{a, at, end - at, 0, {}};
+      for (int j = 0; j < kNarrowRows && at + j < end; ++j) u.row[j] = order[at + j];
+      units[kind].push_back(u);
+    }
     i = e;
   }
   uint8_t* b = static_cast<uint8_t*>(buf);
   if (n_rows) {
-    memcpy(b, units.data(), units.size() * sizeof(Unit));
+    size_t at = 0;
+    for (const auto& v : units) {
+      if (!v.empty()) memcpy(b + at, v.data(), v.size() * sizeof(Unit));
+      at += v.size() * sizeof(Unit);
+    }
     memcpy(b + (size_t)n_rows * sizeof(Unit), order.data(), (size_t)n_rows * sizeof(int));
   }
   *out = spec_lora_plan{};
   out->n_rows = n_rows;
   out->n_adapters = n_adapters;
-  out->n_units = with;
-  out->n_bare = (int)units.size() - with;
+  out->n_wide = (int)units[0].size();
+  out->n_narrow = (int)units[1].size();
+  out->n_bare = (int)units[2].size();
   return SPEC_OK;
 }
 
@@ -101,8 +120,8 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
     return fail(SPEC_ERR_INVALID, "%s: %d adapters of %d to %d channels", what, b->n_adapters, b->k, b->n);
   if (b->rank < 0 || b->rank > kMaxRank) return fail(SPEC_ERR_UNSUPPORTED, "%s: rank %d (up to %d is built)", what, b->rank, kMaxRank);
   if (b->device < 0) return fail(SPEC_ERR_INVALID, "%s: device %d", what, b->device);
-  if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_units < 0 || plan->n_bare < 0 ||
-      plan->n_units + (int64_t)plan->n_bare > plan->n_rows)
+  if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_wide < 0 || plan->n_narrow < 0 || plan->n_bare < 0 ||
+      (int64_t)plan->n_wide + plan->n_narrow + plan->n_bare > plan->n_rows)
     return fail(SPEC_ERR_INVALID, "%s: not a plan", what);
   if (plan->n_adapters > b->n_adapters)
     return fail(SPEC_ERR_INVALID, "%s: a plan for %d adapters, the bank has %d", what, plan->n_adapters, b->n_adapters);
@@ -127,7 +146,7 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool in_place = y->ptr == out->ptr;
   if (in_place && plan->n_rows > 1 && y->row_stride != out->row_stride)
     return fail(SPEC_ERR_INVALID, "%s: y in place needs one row stride", what);
-  if (plan->n_units) {
+  if (plan->n_wide || plan->n_narrow) {
     if ((b->rank > 0 && (!b->a || !b->b)) || misaligned(b->a, 2) || misaligned(b->b, 2) || misaligned(b->ranks, 4) || misaligned(b->scales, 4))
       return fail(SPEC_ERR_INVALID, "%s: a pointer of the bank is null or not aligned to its element size", what);
     for (const int64_t s : {b->a_adapter_stride, b->a_row_stride, b->b_adapter_stride, b->b_row_stride})
@@ -150,20 +169,25 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   p.x_row = x->row_stride;
   p.y_row = y->row_stride;
   p.out_row = out->row_stride;
-  p.units = static_cast<const Unit*>(plan->device_copy);
-  p.order = reinterpret_cast<const int*>(p.units + plan->n_rows);
+  const Unit* units = static_cast<const Unit*>(plan->device_copy);
+  p.order = reinterpret_cast<const int*>(units + plan->n_rows);
   p.K = b->k;
   p.N = b->n;
   p.rank = b->rank;
   p.a_wide = wide(b->a, b->a_row_stride, b->a_adapter_stride, 2);
   p.b_wide = wide(b->b, b->b_row_stride, b->b_adapter_stride, 2);
   p.x_wide = wide(x->ptr, x->row_stride, 0, x->dtype == T_F32 ? 4 : 2);
+  p.y_wide = wide(y->ptr, y->row_stride, 0, y->dtype == T_F32 ? 4 : 2);
+  p.out_wide = wide(out->ptr, out->row_stride, 0, y->dtype == T_F32 ? 4 : 2);
   int sms = 0;
   cudaError_t e = multiprocessors(b->device, &sms);
-  const int n = plan->n_units + (in_place ? 0 : plan->n_bare);
-  int size = 8;
-  while (size > 1 && (int64_t)n * size > (int64_t)sms * 4) size /= 2;
-  if (e == cudaSuccess) e = launch(p, b->dtype, x->dtype == T_F32, y->dtype == T_F32, n, size, static_cast<cudaStream_t>(stream));
+  const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  p.units = units;
+  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, plan->n_wide, cluster_for(plan->n_wide, 2, sms), s);
+  p.units = units + plan->n_wide;
+  const int n = plan->n_narrow + (in_place ? 0 : plan->n_bare);
+  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 4, sms), s);
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
 }
 

@@ -11,11 +11,13 @@ namespace lora {
 enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
 
 constexpr int kMaxRank = 256;
-constexpr int kNarrowRows = 8;  // rows of a unit: one n-tile of the products
+constexpr int kNarrowRows = 8;  // rows of a unit of the kernel for few rows: one n-tile of the products
+constexpr int kWideRows = 64;   // of the one for many
 
 // Rows of one adapter (-1: none) that one cluster takes.
 struct Unit {
   int adapter, first, n_rows, pad;  // rows order[first ..]
+  int row[kNarrowRows];             // the first of them
 };
 
 struct Params {
@@ -30,11 +32,13 @@ struct Params {
   const Unit* units;
   const int* order;
   int K, N, rank;
-  int a_wide, b_wide, x_wide;  // 8 consecutive elements from a multiple of 8 on are aligned 16-byte accesses
+  int a_wide, b_wide, x_wide, y_wide, out_wide;  // 8 consecutive elements from a multiple of 8 on are aligned 16-byte accesses
 };
 
-// n_units units on clusters of `size` blocks.
-cudaError_t launch(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
+// n_units units on clusters of `size` blocks: of at most kNarrowRows rows (and
+// those without an adapter), or of at most kWideRows.
+cudaError_t launch_narrow(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
+cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
 
 }  // namespace lora
 }  // namespace specb200

@@ -1,0 +1,186 @@
+// What the two kernels of the low-rank adapters share: products on mma.sync from
+// 16-byte pieces, parts that f32 numbers are split into, and clusters.
+//
+// A product's sum may run in any order, so a lane takes 8 consecutive elements of
+// its row for two instructions of 16 (its 2t, 2t + 1, 2t + 8, 2t + 9 of each).
+#pragma once
+
+#include "common.cuh"
+#include "kv4_rows.cuh"
+#include "lora.h"
+
+namespace specb200 {
+namespace lora {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+SPEC_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+SPEC_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+SPEC_DEV int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+SPEC_DEV int cluster_size() {
+  int r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+SPEC_DEV float remote_float(const float* p, int rank) {
+  uint32_t at;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
+SPEC_DEV float4 remote_float4(const float* p, int rank) {
+  uint32_t at;
+  float4 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
+}
+
+SPEC_DEV void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                    const __half*) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+SPEC_DEV void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                    const __nv_bfloat16*) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+SPEC_DEV void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+SPEC_DEV uint32_t tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+
+SPEC_DEV float rest(float x, uint32_t hi) { return fabsf(x) < INFINITY ? x - __uint_as_float(hi) : 0.f; }
+
+// Words of 8 consecutive 16-bit elements from `k` on; those at `n` and behind are zeros.
+template <class T>
+SPEC_DEV uint4 load8(const T* p, int k, int n, bool wide) {
+  if (wide && k + 8 <= n) return *reinterpret_cast<const uint4*>(p + k);
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (k + 2 * i < n ? q[k + 2 * i] : 0u) | (k + 2 * i + 1 < n ? (uint32_t)q[k + 2 * i + 1] << 16 : 0u);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+SPEC_DEV void load8(const float* p, int k, int n, bool wide, float (&x)[8]) {
+  if (wide && k + 8 <= n) {
+    const float4 a = *reinterpret_cast<const float4*>(p + k), b = *reinterpret_cast<const float4*>(p + k + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = k + i < n ? p[k + i] : 0.f;
+}
+SPEC_DEV void widen(const uint4& v, float (&x)[8], const __nv_bfloat16*) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+SPEC_DEV void widen(const uint4& v, float (&x)[8], const __half*) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+// 8 elements from column k on as f32, and each rounded once; those at `n` and behind are left out.
+template <class T>
+SPEC_DEV void load8(const T* p, int k, int n, bool wide, float (&x)[8]) {
+  widen(load8(p, k, n, wide), x, p);
+}
+SPEC_DEV uint32_t pack2(float lo, float hi, const __half*) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+SPEC_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <class T>
+SPEC_DEV void store8(T* p, int k, int n, bool wide, const float (&x)[8]) {
+  const uint4 v = make_uint4(pack2(x[0], x[1], p), pack2(x[2], x[3], p), pack2(x[4], x[5], p), pack2(x[6], x[7], p));
+  if (wide && k + 8 <= n) {
+    *reinterpret_cast<uint4*>(p + k) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < n) reinterpret_cast<uint16_t*>(p)[k + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+}
+SPEC_DEV void store8(float* p, int k, int n, bool wide, const float (&x)[8]) {
+  if (wide && k + 8 <= n) {
+    *reinterpret_cast<float4*>(p + k) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + k + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < n) p[k + i] = x[i];
+}
+SPEC_DEV uint16_t bits(__half h) { return __half_as_ushort(h); }
+SPEC_DEV uint16_t bits(__nv_bfloat16 h) { return __bfloat16_as_ushort(h); }
+SPEC_DEV float to_float(float x) { return x; }
+SPEC_DEV float to_float(__half x) { return __half2float(x); }
+SPEC_DEV float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+SPEC_DEV void from_float(float x, float* p) { *p = x; }
+SPEC_DEV void from_float(float x, __half* p) { *p = __float2half_rn(x); }
+SPEC_DEV void from_float(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
+
+// Numbers of type T that t is split into.
+template <class TY>
+__host__ __device__ constexpr int parts_of(const __half*) {
+  return 2;
+}
+template <class TY>
+__host__ __device__ constexpr int parts_of(const __nv_bfloat16*) {
+  return sizeof(TY) == 4 ? 3 : 2;
+}
+
+// The power of two that a row of t is divided by before it goes to f16.
+SPEC_DEV int exponent(float top, const __half*) {
+  return top > 0.f && top < INFINITY ? min(max((__float_as_int(top) >> 23) - 127, -100), 126) : 0;
+}
+SPEC_DEV int exponent(float, const __nv_bfloat16*) { return 0; }
+SPEC_DEV float pow2i(int e) { return __int_as_float((127 + e) << 23); }
+
+template <class K, class Q>
+cudaError_t launch_clusters(K* kernel, int n, int size, int threads, int smem, cudaStream_t s, const Q& p) {
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = size;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)n * size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+}  // namespace
+}  // namespace lora
+}  // namespace specb200

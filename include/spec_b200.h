@@ -726,7 +726,7 @@ typedef struct spec_lora_bank {
  * and fills *out but for device_copy: the caller copies buf to the device, sets
  * it, and keeps both unchanged until the calls that use them are done. */
 typedef struct spec_lora_plan {
-  int n_rows, n_adapters, n_units, n_bare;
+  int n_rows, n_adapters, n_wide, n_narrow, n_bare, reserved;
   const void* device_copy;     /* 16-byte aligned */
 } spec_lora_plan;
 int64_t spec_lora_plan_bytes(int64_t n_rows);

@@ -29,11 +29,13 @@ def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
     ids = rng.integers(-1, adapters, n)
     rc, plan, buf = make(mod, ids, adapters)
     assert rc == 0 and plan.n_rows == n and plan.n_adapters == adapters
-    units = buf[:16 * (plan.n_units + plan.n_bare)].view(np.int32).reshape(-1, 4)
-    order = buf[16 * n:].view(np.int32)
+    with_one = plan.n_wide + plan.n_narrow
+    units = buf[:48 * (with_one + plan.n_bare)].view(np.int32).reshape(-1, 12)
+    order = buf[48 * n:].view(np.int32)
     seen = []
-    for i, (a, first, count, _) in enumerate(units):
-        assert count > 0 and (a >= 0) == (i < plan.n_units)
+    for i, (a, first, count, _, *near) in enumerate(units):
+        assert 0 < count <= (64 if i < plan.n_wide else 8) and (a >= 0) == (i < with_one)
+        assert near[:count] == order[first:first + min(count, 8)].tolist()
         rows = order[first:first + count]
         assert (ids[rows] == a).all()
         seen += rows.tolist()
@@ -42,19 +44,19 @@ def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
 
 def test_empty_plans(mod):
     rc, plan, _ = make(mod, [], 3)
-    assert rc == 0 and plan.n_units == plan.n_bare == 0
+    assert rc == 0 and plan.n_wide == plan.n_narrow == plan.n_bare == 0
     rc, plan, _ = make(mod, [-1, -1], 0)
-    assert rc == 0 and plan.n_units == 0 and plan.n_bare == 1
+    assert rc == 0 and plan.n_narrow == 0 and plan.n_bare == 1
 
 
 def test_bad_plans_are_refused(mod):
     lib = mod.load()
     assert make(mod, [0, 3], 3)[0] == 1 and make(mod, [-2], 3)[0] == 1 and make(mod, [0], -1)[0] == 1
     assert lib.spec_lora_plan_bytes(-1) == -1 and lib.spec_lora_plan_bytes(1 << 21) == -1
-    ids, buf, plan = np.zeros(4, np.int32), np.zeros(100, np.uint8), mod.LoraPlanDesc()
-    args = [ids.ctypes.data, 4, 1, buf.ctypes.data, 100, ctypes.byref(plan)]
+    ids, buf, plan = np.zeros(4, np.int32), np.zeros(208, np.uint8), mod.LoraPlanDesc()
+    args = [ids.ctypes.data, 4, 1, buf.ctypes.data, 208, ctypes.byref(plan)]
     assert lib.spec_lora_plan_make(*args) == 0
-    for at, bad in ((0, None), (1, -1), (3, None), (4, 79), (5, None)):
+    for at, bad in ((0, None), (1, -1), (3, None), (4, 207), (5, None)):
         assert lib.spec_lora_plan_make(*args[:at], bad, *args[at + 1:]) == 1
 
 
@@ -64,7 +66,7 @@ def test_bad_calls_are_refused(mod):
     def call(bank=(), plan=(), x=(), y=(), out=()):
         b = dict(device=0, n_adapters=2, k=64, n=32, rank=8, dtype=0, a=P, b=P, a_adapter_stride=512, a_row_stride=64,
                  b_adapter_stride=256, b_row_stride=8, ranks=None, scales=None)
-        p = dict(n_rows=3, n_adapters=2, n_units=1, n_bare=1, device_copy=P)
+        p = dict(n_rows=3, n_adapters=2, n_wide=0, n_narrow=1, n_bare=1, reserved=0, device_copy=P)
         r = [dict(ptr=P, row_stride=64, n_rows=3, dtype=0, reserved=0), dict(ptr=P, row_stride=32, n_rows=3, dtype=0, reserved=0),
              dict(ptr=P + 4096, row_stride=32, n_rows=3, dtype=0, reserved=0)]
         b.update(bank), p.update(plan)
@@ -79,7 +81,7 @@ def test_bad_calls_are_refused(mod):
         assert call(bank=change) == 1, change
     for change in (dict(dtype=2), dict(dtype=-1), dict(rank=257), dict(rank=-1)):
         assert call(bank=change) == 3, change
-    for change in (dict(n_rows=-1), dict(n_units=-1), dict(n_units=3), dict(device_copy=None), dict(device_copy=P + 8),
+    for change in (dict(n_rows=-1), dict(n_narrow=-1), dict(n_wide=-1), dict(n_bare=-1), dict(n_narrow=3), dict(n_wide=2), dict(device_copy=None), dict(device_copy=P + 8),
                    dict(n_rows=(1 << 20) + 1)):
         assert call(plan=change) == 1, change
     for which in ("x", "y", "out"):
@@ -90,7 +92,7 @@ def test_bad_calls_are_refused(mod):
     assert call(out=dict(row_stride=31)) == 1                        # rows that overlap
     assert call(out=dict(ptr=P, row_stride=40)) == 1                 # in place, two strides
     assert lib.spec_lora_apply(None, None, None, None, None, None) == 1
-    assert call(plan=dict(n_rows=0, n_units=0, n_bare=0)) == 0       # nothing to do
+    assert call(plan=dict(n_rows=0, n_narrow=0, n_bare=0)) == 0       # nothing to do
 
 
 def test_python_refuses_host_tensors(pkg):
