@@ -31,7 +31,7 @@ struct Smem {
 };
 
 template <class T, class TX, class TY>
-__global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_constant__ Params p) {
   __shared__ __align__(16) Smem sm;
   constexpr bool kSplitX = sizeof(TX) == 4;
   constexpr int P = parts_of<TY>((const T*)nullptr);
@@ -146,39 +146,74 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
   const int ra = 2 * t, rb = 2 * t + 1;
   const bool has_a = ra < u.n_rows, has_b = rb < u.n_rows;
   const float fa = sm.factor[ra], fb = sm.factor[rb];
+  // The next step's loads are under way while one is computed.
+  const TY* py[2] = {static_cast<const TY*>(p.y) + (has_a ? rows[ra] : 0) * p.y_row,
+                     static_cast<const TY*>(p.y) + (has_b ? rows[rb] : 0) * p.y_row};
+  TY* po[2] = {static_cast<TY*>(p.out) + (has_a ? rows[ra] : 0) * p.out_row,
+               static_cast<TY*>(p.out) + (has_b ? rows[rb] : 0) * p.out_row};
+  // B's pieces as they lie in memory (columns behind the last one repeat it,
+  // ranks behind the adapter's are cut off where they are used).
+  uint4 v[8];
+  const bool cut = r % 32 != 0;
+  auto load_b = [&](int m, int s) {
+    const int k = s * 32 + 8 * t;
+    if (p.b_wide && s * 32 + 32 <= p.rank) {
+      const T* b = B + k;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint4*>(b + min(m + j, n1 - 1) * p.b_row);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = load8(B + min(m + j, n1 - 1) * p.b_row, k, r, p.b_wide);
+    }
+  };
+  float ya[8], yb[8];
+  auto load_y = [&](int m) {
+    if (has_a) load8(py[0], m, n1, p.y_wide, ya);
+    if (has_b) load8(py[1], m, n1, p.y_wide, yb);
+  };
+  int n = n0 + warp * 64;
+  if (n < n1) {
+    if (steps) load_b(n + 8 * g, 0);
+    load_y(n + 8 * g);
+  }
 #pragma unroll 1
-  for (int n = n0 + warp * 64; n < n1; n += kWarps * 64) {
+  for (; n < n1; n += kWarps * 64) {
     const int m = n + 8 * g;
-    float ya[8], yb[8];
-    if (has_a) load8(static_cast<const TY*>(p.y) + rows[ra] * p.y_row, m, n1, p.y_wide, ya);
-    if (has_b) load8(static_cast<const TY*>(p.y) + rows[rb] * p.y_row, m, n1, p.y_wide, yb);
+    const bool more = n + kWarps * 64 < n1;
     float d[4][4] = {};
-    const T* b = B + m * p.b_row;
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-      const int at = s * 32 + 8 * t;
-      uint4 v[8];
+      uint4 w[8];
+      if (cut) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = load8(b + j * p.b_row, at, m + j < n1 ? r : 0, p.b_wide);
+        for (int j = 0; j < 8; ++j) w[j] = first_of(v[j], r - s * 32 - 8 * t);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = v[j];
+      }
+      if (s + 1 < steps) load_b(m, s + 1);
+      else if (more) load_b(m + kWarps * 64, 0);
 #pragma unroll
       for (int q = 0; q < P; ++q) {
-        const uint4 w = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
+        const uint4 f = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          mma16(d[j], v[2 * j].x, v[2 * j + 1].x, v[2 * j].y, v[2 * j + 1].y, w.x, w.y, A);
-          mma16(d[j], v[2 * j].z, v[2 * j + 1].z, v[2 * j].w, v[2 * j + 1].w, w.z, w.w, A);
+          mma16(d[j], w[2 * j].x, w[2 * j + 1].x, w[2 * j].y, w[2 * j + 1].y, f.x, f.y, A);
+          mma16(d[j], w[2 * j].z, w[2 * j + 1].z, w[2 * j].w, w[2 * j + 1].w, f.z, f.w, A);
         }
       }
     }
+    float oa[8], ob[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      ya[2 * j] = fmaf(d[j][0], fa, ya[2 * j]);
-      ya[2 * j + 1] = fmaf(d[j][2], fa, ya[2 * j + 1]);
-      yb[2 * j] = fmaf(d[j][1], fb, yb[2 * j]);
-      yb[2 * j + 1] = fmaf(d[j][3], fb, yb[2 * j + 1]);
+      oa[2 * j] = fmaf(d[j][0], fa, ya[2 * j]);
+      oa[2 * j + 1] = fmaf(d[j][2], fa, ya[2 * j + 1]);
+      ob[2 * j] = fmaf(d[j][1], fb, yb[2 * j]);
+      ob[2 * j + 1] = fmaf(d[j][3], fb, yb[2 * j + 1]);
     }
-    if (has_a) store8(static_cast<TY*>(p.out) + rows[ra] * p.out_row, m, n1, p.out_wide, ya);
-    if (has_b) store8(static_cast<TY*>(p.out) + rows[rb] * p.out_row, m, n1, p.out_wide, yb);
+    if (more) load_y(m + kWarps * 64);
+    if (has_a) store8(po[0], m, n1, p.out_wide, oa);
+    if (has_b) store8(po[1], m, n1, p.out_wide, ob);
   }
   cluster_wait();
 }

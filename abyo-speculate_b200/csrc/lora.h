@@ -10,7 +10,7 @@ namespace lora {
 
 enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
 
-constexpr int kMaxRank = 256;
+constexpr int kMaxRank = 128;
 constexpr int kNarrowRows = 8;  // rows of a unit of the kernel for few rows: one n-tile of the products
 constexpr int kWideRows = 64;   // of the one for many
 

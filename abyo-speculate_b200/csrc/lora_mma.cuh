@@ -80,6 +80,22 @@ SPEC_DEV uint4 load8(const T* p, int k, int n, bool wide) {
     w[i] = (k + 2 * i < n ? q[k + 2 * i] : 0u) | (k + 2 * i + 1 < n ? (uint32_t)q[k + 2 * i + 1] << 16 : 0u);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// The words' elements before place n (of 8), zeros for the others.
+SPEC_DEV uint4 first_of(const uint4& v, int n) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = n >= 2 * i + 2 ? w[i] : n == 2 * i + 1 ? w[i] & 0xffffu : 0u;
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// 8 ranks from `k` on of a column's row of B: those at `r` and behind, which lie
+// in the row's memory up to `rank`, are zeros.
+template <class T>
+SPEC_DEV uint4 load_ranks(const T* p, int k, int r, int rank, bool wide) {
+  if (k >= r) return make_uint4(0u, 0u, 0u, 0u);
+  if (wide && k + 8 <= rank) return first_of(*reinterpret_cast<const uint4*>(p + k), r - k);
+  return load8(p, k, r, false);
+}
 SPEC_DEV void load8(const float* p, int k, int n, bool wide, float (&x)[8]) {
   if (wide && k + 8 <= n) {
     const float4 a = *reinterpret_cast<const float4*>(p + k), b = *reinterpret_cast<const float4*>(p + k + 4);

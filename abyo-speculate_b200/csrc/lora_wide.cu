@@ -7,9 +7,9 @@
 // stage's four slices of 32 columns, and add up what the slices gave at the end.
 // The blocks' parts meet in distributed shared memory, each adding up a slice of T
 // and all of them collecting the slices.  Second product, Y += T B^T: the
-// blocks share N; T's parts are the 16-row operand from shared memory, B comes by
-// 16-byte loads, 32 columns a warp and step, arranged so that a lane ends with 8
-// columns of its rows behind one another.
+// blocks share N; y and B come in stages of 128 columns in the same way, T's parts
+// are the 16-row operand, and B's columns are taken in an order that leaves a lane
+// with 8 columns of its rows behind one another.
 //
 // A slice lies as [row][64 bytes], slices 64 bytes apart, so that neither the
 // copies (16 bytes a thread along a row) nor the operands' loads (16 bytes a lane)
@@ -36,37 +36,41 @@ __host__ __device__ constexpr int stage_bytes(int RA) {
 
 struct WideParams {
   Params p;
-  int RA, stages;
+  int RA, stages, bytes;  // ranks' capacity; stages of the first product; of shared memory
 };
 
-SPEC_DEV void cp_async16(uint32_t dst, const void* src, int bytes) {  // the rest of the 16 is zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+SPEC_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
 }
 SPEC_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+SPEC_DEV float2 widen2(uint32_t w, const __nv_bfloat16*) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+SPEC_DEV float2 widen2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// 16 bytes of row `src` from column k on to shared memory; zeros from `end` on.
+// Up to 16 bytes from `src`, of which `left` elements are there, to shared memory; zeros behind them.
 template <class E>
-SPEC_DEV void copy16(uint8_t* dst, const E* src, int k, int end, bool wide) {
+SPEC_DEV void copy16(uint8_t* dst, const E* src, int left, bool wide) {
   constexpr int N = 16 / sizeof(E);
-  const int left = min(max(end - k, 0), N);
-  if (wide) {
-    cp_async16(smem_u32(dst), left ? src + k : src, left * (int)sizeof(E));
-  } else {
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i < left) {
-        if constexpr (N == 4) w[i] = reinterpret_cast<const uint32_t*>(src)[k + i];
-        else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[k + i] << (i % 2 * 16);
-      }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (wide && left >= N) {
+    cp_async16(smem_u32(dst), src);
+    return;
   }
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < left) {
+      if constexpr (N == 4) w[i] = reinterpret_cast<const uint32_t*>(src)[i];
+      else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[i] << (i % 2 * 16);
+    }
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <class T, class TX, class TY, int NT>
 __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant__ WideParams wp) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_factor[kRows];
+  __shared__ const void* s_row[kRows];  // the rows of x, from this block's first column on
   const Params& p = wp.p;
   constexpr bool kSplitX = sizeof(TX) == 4;
   constexpr int P = parts_of<TY>((const T*)nullptr);
@@ -92,81 +96,104 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     const int xs = x_slice<TX>(), as = a_slice(RA), sb = stage_bytes<TX>(RA);
     constexpr int XC = kSplitX ? 32 : 16, XR = kThreads / XC, XN = kRows / XR;  // pieces a row; rows a pass; passes
     const int xc = threadIdx.x % XC, xr = threadIdx.x / XC, ac = threadIdx.x % 16, ar = threadIdx.x / 16;
-    const TX* xp[XN];
-#pragma unroll
-    for (int i = 0; i < XN; ++i) {
-      const int row = xr + i * XR;
-      xp[i] = static_cast<const TX*>(p.x) + rows[row < u.n_rows ? row : 0] * p.x_row;
-    }
+    // Rows behind the last one are copies of it, T's columns behind the adapter's
+    // rank whatever the memory holds: neither is used.
+    if (threadIdx.x < kRows)
+      s_row[threadIdx.x] = static_cast<const TX*>(p.x) + rows[min((int)threadIdx.x, u.n_rows - 1)] * p.x_row + k0;
+    __syncthreads();
+    const TX* const* xp = reinterpret_cast<const TX* const*>(s_row) + xr;
+    const T* ap = A + ar * p.a_row + k0 + ac * 8;
+    const long long a_pass = p.a_row * (kThreads / 16);
     // f32: piece c of a slice is columns 4 c ..; half c % 2, place c / 2 of its row.
-    const int x_at = kSplitX ? xc / 8 * xs + xc % 2 * (kRows * 64) + xc % 8 / 2 * 16 : xc / 4 * xs + xc % 4 * 16;
-    const int a_at = kSlices * xs + ac / 4 * as + ac % 4 * 16;
-    auto fetch = [&](int step) {
-      uint8_t* st = smem + step % stages * sb;
-      const int k = k0 + step * 128;
+    const int x_at = xr * 64 + (kSplitX ? xc / 8 * xs + xc % 2 * (kRows * 64) + xc % 8 / 2 * 16 : xc / 4 * xs + xc % 4 * 16);
+    const int a_at = ar * 64 + kSlices * xs + ac / 4 * as + ac % 4 * 16;
+    const uint32_t base = smem_u32(smem);
+    const bool fast = p.x_wide && p.a_wide;
+    const int width = k1 - k0;
+    int at = 0, k = 0;  // of the next stage to fetch: its offset, its first column
+    auto fetch = [&]() {
+      const int xk = k + xc * (16 / (int)sizeof(TX));
+      const T* a = ap + k;
+      if (fast && k + 128 <= width) {
 #pragma unroll
-      for (int i = 0; i < XN; ++i)
-        copy16(st + x_at + (xr + i * XR) * 64, xp[i], k + xc * (16 / (int)sizeof(TX)), xr + i * XR < u.n_rows ? k1 : 0, p.x_wide);
-      for (int j = ar; j < W; j += kThreads / 16)
-        copy16(st + a_at + j * 64, A + min(j, r - 1) * p.a_row, k + ac * 8, j < r ? k1 : 0, p.a_wide);
+        for (int i = 0; i < XN; ++i) cp_async16(base + at + x_at + i * XR * 64, xp[i * XR] + xk);
+        for (int j = ar, o = at + a_at; j < r; j += kThreads / 16, o += kThreads / 16 * 64, a += a_pass) cp_async16(base + o, a);
+      } else {
+#pragma unroll
+        for (int i = 0; i < XN; ++i) copy16(smem + at + x_at + i * XR * 64, xp[i * XR] + xk, width - xk, p.x_wide);
+        for (int j = ar, o = at + a_at; j < r; j += kThreads / 16, o += kThreads / 16 * 64, a += a_pass)
+          copy16(smem + o, a, width - k - ac * 8, p.a_wide);
+      }
+      k += 128;
+      at = at + sb == stages * sb ? 0 : at + sb;
     };
     for (int s = 0; s < stages - 1; ++s) {
-      if (s < n_steps) fetch(s);
+      if (s < n_steps) fetch();
       cp_async_commit();
     }
+    // Slices of this warp: every turns-th, of 8 turns one of every other stage.
+    const int i0 = kg % kSlices, di = turns < kSlices ? turns : kSlices, xo = (mg * 32 + g) * 64 + t * 16,
+              ao = kSlices * xs + (nb * NT * 8 + g) * 64 + t * 16;
+    const uint8_t* st = smem;
 #pragma unroll 1
     for (int step = 0; step < n_steps; ++step) {
       if (stages == 2) cp_async_wait<0>();
       else if (stages == 3) cp_async_wait<1>();
       else cp_async_wait<2>();
       __syncthreads();
-      if (step + stages - 1 < n_steps) fetch(step + stages - 1);
+      if (step + stages - 1 < n_steps) fetch();
       cp_async_commit();
-      const uint8_t* st = smem + step % stages * sb;
-      for (int i = 0; i < kSlices; ++i) {
-        if ((step * kSlices + i) % turns != kg) continue;
-        const uint8_t* xb = st + i * xs + (mg * 32 + g) * 64 + t * 16;
-        const uint8_t* ab = st + kSlices * xs + i * as + (nb * NT * 8 + g) * 64 + t * 16;
-        if constexpr (kSplitX) {
-          // Columns 8 t .. 8 t + 7 of two rows a tile: hi and lo.
+      if (kg < turns && (turns <= kSlices || (step ^ kg / kSlices) % 2 == 0)) {
+#pragma unroll 1
+        for (int i = i0; i < kSlices; i += di) {
+          const uint8_t *xb = st + i * xs + xo, *ab = st + i * as + ao;
+          if constexpr (kSplitX) {
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            float x0[8], x1[8];
+            for (int n0 = 0; n0 < NT; n0 += 4) {  // four rank tiles at a time
+              uint4 a[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float4 v = *reinterpret_cast<const float4*>(xb + h * (kRows * 64) + m * 1024);
-              const float4 w = *reinterpret_cast<const float4*>(xb + h * (kRows * 64) + m * 1024 + 512);
-              x0[h * 4] = v.x, x0[h * 4 + 1] = v.y, x0[h * 4 + 2] = v.z, x0[h * 4 + 3] = v.w;
-              x1[h * 4] = w.x, x1[h * 4 + 1] = w.y, x1[h * 4 + 2] = w.z, x1[h * 4 + 3] = w.w;
-            }
+              for (int n = 0; n < 4; ++n) a[n] = lds128(ab + (n0 + n) * 512);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              float a[8];
-              widen(lds128(ab + n * 512), a, A);
+              for (int m = 0; m < 2; ++m) {
+                // Columns 8 t .. 8 t + 7 of two rows, as hi and lo.
 #pragma unroll
-              for (int e = 0; e < 8; e += 2) {
-                const uint32_t h0 = tf32(x0[e]), h1 = tf32(x1[e]), h2 = tf32(x0[e + 1]), h3 = tf32(x1[e + 1]);
-                mma8(d[m][n], h0, h1, h2, h3, __float_as_uint(a[e]), __float_as_uint(a[e + 1]));
-                mma8(d[m][n], tf32(rest(x0[e], h0)), tf32(rest(x1[e], h1)), tf32(rest(x0[e + 1], h2)), tf32(rest(x1[e + 1], h3)),
-                     __float_as_uint(a[e]), __float_as_uint(a[e + 1]));
+                for (int h = 0; h < 2; ++h) {
+                  const uint4 v = lds128(xb + h * (kRows * 64) + m * 1024), w = lds128(xb + h * (kRows * 64) + m * 1024 + 512);
+                  const float x[8] = {__uint_as_float(v.x), __uint_as_float(w.x), __uint_as_float(v.y), __uint_as_float(w.y),
+                                      __uint_as_float(v.z), __uint_as_float(w.z), __uint_as_float(v.w), __uint_as_float(w.w)};
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) hi[c] = tf32(x[e * 4 + c]), lo[c] = tf32(rest(x[e * 4 + c], hi[c]));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                      const uint32_t pair = h ? (e ? a[n].w : a[n].z) : (e ? a[n].y : a[n].x);
+                      const float2 f = widen2(pair, A);
+                      mma8(d[m][n0 + n], hi[0], hi[1], hi[2], hi[3], __float_as_uint(f.x), __float_as_uint(f.y));
+                      mma8(d[m][n0 + n], lo[0], lo[1], lo[2], lo[3], __float_as_uint(f.x), __float_as_uint(f.y));
+                    }
+                  }
+                }
               }
             }
-          }
-        } else {
-          uint4 x[2][2];
+          } else {
+            uint4 x[2][2];
 #pragma unroll
-          for (int m = 0; m < 2; ++m) x[m][0] = lds128(xb + m * 1024), x[m][1] = lds128(xb + m * 1024 + 512);
+            for (int m = 0; m < 2; ++m) x[m][0] = lds128(xb + m * 1024), x[m][1] = lds128(xb + m * 1024 + 512);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 a = lds128(ab + n * 512);
+            for (int n = 0; n < NT; ++n) {
+              const uint4 a = lds128(ab + n * 512);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              mma16(d[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
-              mma16(d[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
+              for (int m = 0; m < 2; ++m) {
+                mma16(d[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
+                mma16(d[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
+              }
             }
           }
         }
       }
+      st = st + sb == smem + stages * sb ? smem : st + sb;
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -258,56 +285,109 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   // ---- Y ----
   {
     const int n_per = ((p.N + size * 32 - 1) / (size * 32)) * 32, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
+    // Stages of 128 columns behind T's parts, laid out as those of the first
+    // product: y's rows in slices of 32 columns, and for each 32 ranks B's 128
+    // columns.  A warp takes the slices of its rows in turn.
+    const int ys = x_slice<TY>(), bs = a_slice(128), sb = kSlices * ys + steps * bs;
+    uint8_t* ring = smem + (P * steps * frag + 127) / 128 * 128;
+    const int stages = min((wp.bytes - (int)(ring - smem)) / sb, 4), n_steps = (n1 - n0 + 127) / 128;
+    constexpr int YC = sizeof(TY) == 4 ? 32 : 16, YR = kThreads / YC, YN = kRows / YR;
+    const int yc = threadIdx.x % YC, yr = threadIdx.x / YC;
+    const int y_at = yr * 64 + (sizeof(TY) == 4 ? yc / 8 * ys + yc % 2 * (kRows * 64) + yc % 8 / 2 * 16 : yc / 4 * ys + yc % 4 * 16);
+    const TY* const* yp = reinterpret_cast<const TY* const*>(s_row) + yr;
+    if (threadIdx.x < kRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, u.n_rows - 1)] * p.y_row + n0;
+    __syncthreads();
+    const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
+    const int width = n1 - n0, pieces = steps * 4;  // of a column of B
+    int at = 0, k = 0;
+    auto fetch = [&]() {
+      const int yk = k + yc * (16 / (int)sizeof(TY));
+      const bool whole = fast && k + 128 <= width;
+#pragma unroll
+      for (int i = 0; i < YN; ++i) {
+        uint8_t* to = ring + at + y_at + i * YR * 64;
+        if (yr + i * YR >= u.n_rows) continue;
+        if (whole) cp_async16(smem_u32(to), yp[i * YR] + yk);
+        else copy16(to, yp[i * YR] + yk, width - yk, p.y_wide);
+      }
+      for (int i = threadIdx.x; i < 128 * pieces; i += kThreads) {
+        const int column = i / pieces, piece = i - column * pieces;
+        uint8_t* to = ring + at + kSlices * ys + piece / 4 * bs + column * 64 + piece % 4 * 16;
+        const T* from = B + (n0 + min(k + column, width - 1)) * p.b_row + piece * 8;
+        if (whole && piece * 8 < r) cp_async16(smem_u32(to), from);
+        else copy16(to, from, r - piece * 8, p.b_wide);
+      }
+      k += 128;
+      at = at + sb == stages * sb ? 0 : at + sb;
+    };
+    for (int s = 0; s < stages - 1; ++s) {
+      if (s < n_steps) fetch();
+      cp_async_commit();
+    }
     const int ways = kWarps / groups, ng = warp / groups, first = (warp % groups) * 32 + g;
-    long long at[4];
+    TY* op[4];
     float factor[4];
-    bool has[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = first + i * 8;
-      has[i] = row < u.n_rows;
-      at[i] = has[i] ? rows[row] : 0;
-      factor[i] = has[i] ? s_factor[row] : 0.f;
+      op[i] = row < u.n_rows ? static_cast<TY*>(p.out) + rows[row] * p.out_row : nullptr;
+      factor[i] = row < u.n_rows ? s_factor[row] : 0.f;
     }
+    const uint8_t* st = ring;
 #pragma unroll 1
-    for (int n = n0 + ng * 32; n < n1; n += ways * 32) {
-      float y[4][8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (has[i]) load8(static_cast<const TY*>(p.y) + at[i] * p.y_row, n + 8 * t, n1, p.y_wide, y[i]);
-      float d2[2][4][4] = {};
-      const int column = n + g / 2 * 8 + g % 2;
+    for (int step = 0; step < n_steps; ++step) {
+      if (stages == 2) cp_async_wait<0>();
+      else if (stages == 3) cp_async_wait<1>();
+      else cp_async_wait<2>();
+      __syncthreads();
+      if (step + stages - 1 < n_steps) fetch();
+      cp_async_commit();
+      for (int slice = ng; slice < kSlices; slice += ways) {
+        const int n = n0 + step * 128 + slice * 32;
+        if (n >= n1) break;
+        float d2[2][4][4] = {};
+        const uint8_t* bb = st + kSlices * ys + (slice * 32 + g / 2 * 8 + g % 2) * 64 + t * 16;
 #pragma unroll 1
-      for (int s = 0; s < steps; ++s) {
-        uint4 b[4];
+        for (int s = 0; s < steps; ++s, bb += bs) {
+          uint4 b[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          b[j] = load8(B + (column + 2 * j) * p.b_row, s * 32 + 8 * t, column + 2 * j < n1 ? r : 0, p.b_wide);
+          for (int j = 0; j < 4; ++j) b[j] = lds128(bb + j * 128);
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-          const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + t * 16;
+          for (int q = 0; q < P; ++q) {
+            const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + t * 16;
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint4 x0 = lds128(f + m * 1024), x1 = lds128(f + m * 1024 + 512);
+            for (int m = 0; m < 2; ++m) {
+              const uint4 x0 = lds128(f + m * 1024), x1 = lds128(f + m * 1024 + 512);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              mma16(d2[m][j], x0.x, x1.x, x0.y, x1.y, b[j].x, b[j].y, A);
-              mma16(d2[m][j], x0.z, x1.z, x0.w, x1.w, b[j].z, b[j].w, A);
+              for (int j = 0; j < 4; ++j) {
+                mma16(d2[m][j], x0.x, x1.x, x0.y, x1.y, b[j].x, b[j].y, A);
+                mma16(d2[m][j], x0.z, x1.z, x0.w, x1.w, b[j].z, b[j].w, A);
+              }
             }
           }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!has[i]) continue;
+        for (int i = 0; i < 4; ++i) {
+          if (!op[i]) continue;
+          float y[8];
+          const uint8_t* yb = st + slice * ys + (first + i * 8) * 64 + t * 16;
+          if constexpr (sizeof(TY) == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(yb), w = *reinterpret_cast<const float4*>(yb + kRows * 64);
+            y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w, y[4] = w.x, y[5] = w.y, y[6] = w.z, y[7] = w.w;
+          } else {
+            widen(lds128(yb), y, A);
+          }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          y[i][2 * j] = fmaf(d2[i / 2][j][i % 2 * 2], factor[i], y[i][2 * j]);
-          y[i][2 * j + 1] = fmaf(d2[i / 2][j][i % 2 * 2 + 1], factor[i], y[i][2 * j + 1]);
+          for (int j = 0; j < 4; ++j) {
+            y[2 * j] = fmaf(d2[i / 2][j][i % 2 * 2], factor[i], y[2 * j]);
+            y[2 * j + 1] = fmaf(d2[i / 2][j][i % 2 * 2 + 1], factor[i], y[2 * j + 1]);
+          }
+          store8(op[i], n + 8 * t, n1, p.out_wide, y);
         }
-        store8(static_cast<TY*>(p.out) + at[i] * p.out_row, n + 8 * t, n1, p.out_wide, y[i]);
       }
+      st = st + sb == ring + stages * sb ? ring : st + sb;
     }
+    cp_async_wait<0>();
   }
   if (size > 1) cluster_wait();
 }
@@ -315,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 template <class T, class TX, class TY, int NT>
 cudaError_t run(const Params& p, int n_units, int size, cudaStream_t s) {
   constexpr int B = 8 * NT;
-  WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0};
+  WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0, 0};
   const int stage = stage_bytes<TX>(w.RA);
   // As many stages, up to 4, as let an SM hold two blocks; two at least.
   w.stages = 112 * 1024 / stage;
@@ -324,6 +404,10 @@ cudaError_t run(const Params& p, int n_units, int size, cudaStream_t s) {
   // The warps' parts of T: 32 rows and a block of ranks each; T whole, and the numbers it is split into.
   if (bytes < kWarps * 32 * B * 4) bytes = kWarps * 32 * B * 4;
   if (bytes < kRows * w.RA * 10) bytes = kRows * w.RA * 10;
+  // The numbers that T is split into, and two stages of the second product at least.
+  const int steps = (w.RA + 31) / 32, second = kSlices * x_slice<TY>() + steps * a_slice(128);
+  if (bytes < 3 * steps * kRows * 64 + 2 * second) bytes = 3 * steps * kRows * 64 + 2 * second;
+  w.bytes = bytes;
   const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T, TX, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
   return launch_clusters(wide_kernel<T, TX, TY, NT>, n_units, size, kThreads, bytes, s, w);

@@ -62,7 +62,7 @@ class LoraBank:
 
     a [adapters, rank, k] and b [adapters, n, rank]: bfloat16 or float16 CUDA
     tensors with contiguous rows, kept as they are.  ranks: adapters' own ranks
-    (the rest of their a and b is not read), whole numbers or an int32 tensor
+    (what lies behind them in a and b does not count), whole numbers or an int32 tensor
     on the device; scales: numbers or a float32 tensor on the device."""
 
     def __init__(self, a, b, ranks=None, scales=None):

@@ -712,12 +712,12 @@ typedef struct spec_lora_bank {
   int device;
   int n_adapters;
   int k, n;                    /* channels of x and y */
-  int rank;                    /* rows of every A, columns of every B: at most 256 */
+  int rank;                    /* rows of every A, columns of every B: at most 128 */
   int dtype;                   /* of A and B: 0 = bf16, 1 = f16 */
   const void *a, *b;           /* element (adapter, row, column) at adapter * adapter_stride + row * row_stride + column */
   int64_t a_adapter_stride, a_row_stride;
   int64_t b_adapter_stride, b_row_stride;
-  const int32_t* ranks;        /* [n_adapters]: an adapter's own rank (the rest of its A and B is not read), or NULL */
+  const int32_t* ranks;        /* [n_adapters]: an adapter's own rank (what lies behind it in A and B does not count), or NULL */
   const float* scales;         /* [n_adapters], or NULL: 1 */
 } spec_lora_bank;
 /* Rows of a step by adapter.  adapters: host, n_rows numbers of 0 .. n_adapters

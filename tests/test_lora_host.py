@@ -79,7 +79,7 @@ def test_bad_calls_are_refused(mod):
                    dict(b=None), dict(a=P + 1), dict(ranks=P + 2), dict(scales=P + 1), dict(a_row_stride=-1),
                    dict(b_adapter_stride=1 << 41)):
         assert call(bank=change) == 1, change
-    for change in (dict(dtype=2), dict(dtype=-1), dict(rank=257), dict(rank=-1)):
+    for change in (dict(dtype=2), dict(dtype=-1), dict(rank=129), dict(rank=-1)):
         assert call(bank=change) == 3, change
     for change in (dict(n_rows=-1), dict(n_narrow=-1), dict(n_wide=-1), dict(n_bare=-1), dict(n_narrow=3), dict(n_wide=2), dict(device_copy=None), dict(device_copy=P + 8),
                    dict(n_rows=(1 << 20) + 1)):
