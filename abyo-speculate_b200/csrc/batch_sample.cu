@@ -289,27 +289,11 @@ SPEC_DEV float redux_max(float x) {
   return m;
 }
 
-// A warp takes C chunks, whose sums share one reference.  A NaN or +inf makes
+// A warp takes C chunks.  A NaN or +inf makes
 // its chunk's sum NaN.
 template <class T, int C>
-__global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows r) {
+SPEC_DEV void chunk_stats(const Rows& r, const Row<T>& rr, int row, int c0, int lane) {
   constexpr int N = Vec<T>::N, NV = kPer / N;
-  const int lane = threadIdx.x & 31;
-  const unsigned per_row = (unsigned)r.nch / C, at = blockIdx.x * 8 + (threadIdx.x >> 5);
-  pdl_launch_dependents();
-  pdl_wait();
-  const int row = (int)(at / per_row), c0 = (int)(at - row * per_row) * C;
-  if (row >= r.n_rows) return;
-  if (c0 == 0 && lane == 0) {
-    if (r.path) r.path[row] = -1;
-    if (r.drafts) {  // what the verification asks about the row's draft
-      const int x = r.drafts[row];
-      const bool judged = x >= 0 && x < r.V;
-      r.seen[row] = judged ? make_float2(r.q[row * r.q_stride + x], to_float((static_cast<const T*>(r.logits) + row * r.stride)[x]))
-                           : make_float2(0.f, 0.f);
-    }
-  }
-  const Row<T> rr(r, row);
   uint4 v[C * NV];
   const int first = c0 * kChunk - rr.shift;
   if (first >= 0 && first + C * kChunk <= rr.V) {
@@ -320,7 +304,7 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
 #pragma unroll
     for (int i = 0; i < C * NV; ++i) v[i] = load_vec(rr, first + (i * 32 + lane) * N);
   }
-  const float m = redux_max(largest<C * NV>(v, rr.p));
+  const float m = C == 1 || rr.t == 0.f ? redux_max(largest<C * NV>(v, rr.p)) : 0.f;
   if (rr.t == 0.f) {  // only the first largest logit counts: its column stands in the sum's place
     bool nan = false;
     int at_column = 0x7fffffff;
@@ -342,10 +326,11 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
           lane ? make_float2(-INFINITY, 0.f) : make_float2(m, nan ? NAN : __int_as_float(at_column));
     return;
   }
-  const Ref ref(m == -INFINITY ? 0.f : m, rr.h);
-  float s[C];
+  float s[C], ms[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
+    ms[c] = C == 1 ? m : redux_max(largest<NV>(v + c * NV, rr.p));
+    const Ref ref(ms[c] == -INFINITY ? 0.f : ms[c], rr.h);
     float x[kPer];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -373,6 +358,7 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
       mine = mine * 2 + up;
 #pragma unroll
       for (int i = 0; i < n; ++i) {
+        ms[i] = up ? ms[i + n] : ms[i];
         const float keep = up ? s[i + n] : s[i], give = up ? s[i] : s[i + n];
         s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
       }
@@ -380,7 +366,27 @@ __global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows
       s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
     }
   }
-  if (lane % (32 / C) == 0) r.stats[(long long)row * r.nch + c0 + mine] = make_float2(m, s[0]);
+  if (lane % (32 / C) == 0) r.stats[(long long)row * r.nch + c0 + mine] = make_float2(ms[0], s[0]);
+}
+
+template <class T, int C>
+__global__ void __launch_bounds__(256) stats_kernel(const __grid_constant__ Rows r) {
+  const int lane = threadIdx.x & 31;
+  const unsigned per_row = (unsigned)r.nch / C, at = blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int row = (int)(at / per_row), c0 = (int)(at - row * per_row) * C;
+  if (row >= r.n_rows) return;
+  if (c0 == 0 && lane == 0) {
+    if (r.path) r.path[row] = -1;
+    if (r.drafts) {  // what the verification asks about the row's draft
+      const int x = r.drafts[row];
+      const bool judged = x >= 0 && x < r.V;
+      r.seen[row] = judged ? make_float2(r.q[row * r.q_stride + x], to_float((static_cast<const T*>(r.logits) + row * r.stride)[x]))
+                           : make_float2(0.f, 0.f);
+    }
+  }
+  chunk_stats<T, C>(r, Row<T>(r, row), row, c0, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -797,8 +803,9 @@ SPEC_DEV void write_probs(const SampleParams& p, const Row<T>& r, const Joined& 
   }
 }
 
-template <class T, bool PROBS>
-__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_constant__ SampleParams p) {
+// ALONE: without the kernel before it, each cluster sums its own row.
+template <class T, bool PROBS, bool ALONE>
+__global__ void __launch_bounds__(kThreads, ALONE ? 2 : 4) sample_kernel(const __grid_constant__ SampleParams p) {
   __shared__ int s_tok;
   __shared__ Powers s_powers;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -809,6 +816,11 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const __grid_consta
   const int nch = p.r.nch;
   const float u = p.r.u[row];
   double* sums = p.r.sums + (long long)row * nch;
+  if constexpr (ALONE) {
+#pragma unroll 1
+    for (int c = (rank * kWarps + warp) * 4; c < nch; c += cluster_size() * kWarps * 4) chunk_stats<T, 4>(p.r, r, row, c, lane);
+    cluster_sync();
+  }
   Joined j;
   if (PROBS || warp == 0) {
     const Stats st(p.r.stats + (long long)row * nch, nch, lane);
@@ -1102,13 +1114,18 @@ cudaError_t stats(const Rows& r, int sms, cudaStream_t s) {
   constexpr int C = sizeof(T) == 4 ? 4 : 8;
   return kv4::launch_overlapping(stats_kernel<T, C>, dim3((unsigned)((chunks / C + 7) / 8)), 256, 0, s, r);
 }
-template <class T>
+template <class T, bool PROBS>
 cudaError_t sample(const SampleParams& p, int sms, cudaStream_t s) {
+  // One launch where all clusters are resident with a multiprocessor a block
+  // (one row of 128256: 4.9 us in two kernels, which cost the host 3 us more).
+  if ((long long)p.r.n_rows * 8 <= sms) return launch_clusters(sample_kernel<T, PROBS, true>, p.r.n_rows, 8, kThreads, s, p);
   const cudaError_t e = stats<T>(p.r, sms, s);
   if (e != cudaSuccess) return e;
-  const int size = cluster_for(p.r.n_rows, 4, sms);
-  return p.probs ? launch_clusters(sample_kernel<T, true>, p.r.n_rows, size, kThreads, s, p)
-                 : launch_clusters(sample_kernel<T, false>, p.r.n_rows, size, kThreads, s, p);
+  return launch_clusters(sample_kernel<T, PROBS, false>, p.r.n_rows, cluster_for(p.r.n_rows, 4, sms), kThreads, s, p);
+}
+template <class T>
+cudaError_t sample(const SampleParams& p, int sms, cudaStream_t s) {
+  return p.probs ? sample<T, true>(p, sms, s) : sample<T, false>(p, sms, s);
 }
 template <class T>
 cudaError_t verify(const VerifyParams& p, bool trees, int sms, cudaStream_t s) {

@@ -15,6 +15,7 @@ using namespace specb200::lora;
 namespace {
 
 constexpr int kPlanRows = 1 << 20;
+constexpr int kHalvesMost = 36;  // units of 32 rows: as many clusters of 8 blocks as a B200 holds, two blocks an SM
 constexpr int kNarrowMost = 16;  // rows of an adapter that the kernel for few rows takes, in units of 8
 
 // Layout of a plan: units (of many rows, of few, those without an adapter), then the rows in their order.
@@ -51,13 +52,23 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   for (int i = 0; i < n_rows; ++i) order[i] = i;
   // By adapter, rows in their order; rows without one last.
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return (unsigned)adapters[x] < (unsigned)adapters[y]; });
-  // An adapter's rows in units of equal size.
+  // An adapter's rows in units of equal size; rows without one are copied one by
+  // one.  Units of 64 rows read A and B half as often as those of 32, which are
+  // taken where there are few of them.
+  int64_t halves = 0;
+  for (int i = 0; i < n_rows;) {
+    int e = i;
+    while (e < n_rows && adapters[order[e]] == adapters[order[i]]) ++e;
+    if (adapters[order[i]] >= 0 && e - i > kNarrowMost) halves += (e - i + kWideRows / 2 - 1) / (kWideRows / 2);
+    i = e;
+  }
+  const int wide_rows = halves <= kHalvesMost ? kWideRows / 2 : kWideRows;
   std::vector<Unit> units[3];
   for (int i = 0; i < n_rows;) {
     int e = i;
     const int a = adapters[order[i]];
     while (e < n_rows && adapters[order[e]] == a) ++e;
-    const int kind = a < 0 ? 2 : e - i > kNarrowMost ? 0 : 1, most = kind ? kNarrowRows : kWideRows;
+    const int kind = a < 0 ? 2 : e - i > kNarrowMost ? 0 : 1, most = kind == 2 ? 1 : kind ? kNarrowRows : wide_rows;
     const int n = (e - i + most - 1) / most;
     for (int k = 0; k < n; ++k) {
       const int at = i + (int)((int64_t)(e - i) * k / n), end = i + (int)((int64_t)(e - i) * (k + 1) / n);
@@ -184,10 +195,10 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.units = units;
-  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, plan->n_wide, cluster_for(plan->n_wide, 2, sms), s);
+  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, plan->n_wide, cluster_for(plan->n_wide, 2, sms), sms, s);
   p.units = units + plan->n_wide;
   const int n = plan->n_narrow + (in_place ? 0 : plan->n_bare);
-  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 4, sms), s);
+  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 2, sms), s);
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
 }
 

@@ -5,13 +5,14 @@
 // A cluster takes the rows of one adapter (up to 8), so that A and B are
 // read once for all of them.  Each block forms the part of t = x A^T over its
 // share of K; the parts meet in distributed shared memory, and each block
-// then adds t B^T for its share of N.  Both products are taken transposed, so
+// then adds t B^T for its share of N; a warp has its stages of B under way
+// from the start.  Both products are taken transposed, so
 // that the adapter is the 16-row operand of mma.sync and the rows are its 8
 // columns:
 //   T^T [16 ranks x 8 rows] += A [16 x 32] X^T,   Y^T [16 n x 8 rows] += B [16 x 32] T^T
 // A product's sum may run in any order, so a lane takes 8 consecutive elements of
 // its row for two instructions of 16 (its 2t, 2t + 1, 2t + 8, 2t + 9 of each):
-// every operand comes by 16-byte loads from where it lies, without shared memory.
+// x and A come by 16-byte loads from where they lie, without shared memory.
 //
 // f32 rows enter as two tf32 numbers, hi + lo, off by 2^-24.  t stays f32;
 // for the second product it is split into bf16 numbers (three, 24 bits, for an
@@ -23,16 +24,21 @@ namespace specb200 {
 namespace lora {
 namespace {
 
+constexpr int kStages = 3;  // of B a warp has under way: 64 columns by 32 ranks
+constexpr int kStageBytes = 64 * 64;
+
 struct Smem {
-  float part[16 * kNarrowRows * 16];         // [k part x rank tile][row][16 ranks]
-  float t[kNarrowRows][kMaxRank];            // this block's share of x A^T
-  uint16_t frag[3][kMaxRank / 32][32 * 8];   // t's parts as the second product takes them
+  uint8_t ring[kWarps][kStages][kStageBytes];  // column 8 g + j at place 8 j + g
+  float part[kWarps * kNarrowRows * 16];       // [k part x rank tile][row][16 ranks]
+  float t[kNarrowRows][kMaxRank];              // this block's share of x A^T
+  uint16_t frag[3][kMaxRank / 32][32 * 8];     // t's parts as the second product takes them
   float factor[kNarrowRows];
 };
 
 template <class T, class TX, class TY>
 __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_constant__ Params p) {
-  __shared__ __align__(16) Smem sm;
+  extern __shared__ __align__(128) uint8_t smem[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem);
   constexpr bool kSplitX = sizeof(TX) == 4;
   constexpr int P = parts_of<TY>((const T*)nullptr);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -42,18 +48,47 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   const Unit& u = p.units[blockIdx.x / size];
   const int* rows = u.row;
   const int n_per = ((p.N + size * 64 - 1) / (size * 64)) * 64, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
-  if (u.adapter < 0) {  // rows without an adapter: y as it is
-    for (int i = 0; i < u.n_rows; ++i) {
-      const long long row = p.order[u.first + i];
-      for (int n = n0 + threadIdx.x; n < n1; n += kThreads)
-        static_cast<TY*>(p.out)[row * p.out_row + n] = static_cast<const TY*>(p.y)[row * p.y_row + n];
-    }
+  if (u.adapter < 0) {  // a row without an adapter: y as it is
+    const TY* y = static_cast<const TY*>(p.y) + rows[0] * p.y_row;
+    TY* o = static_cast<TY*>(p.out) + rows[0] * p.out_row;
+    constexpr int V = 16 / sizeof(TY);
+    const int vectors = p.y_wide && p.out_wide ? (n1 - n0) / V : 0;  // n0 is a multiple of V
+#pragma unroll 4
+    for (int i = threadIdx.x; i < vectors; i += kThreads)
+      reinterpret_cast<uint4*>(o + n0)[i] = reinterpret_cast<const uint4*>(y + n0)[i];
+#pragma unroll 4
+    for (int n = n0 + vectors * V + threadIdx.x; n < n1; n += kThreads) o[n] = y[n];
     return;
   }
   const int r = p.ranks ? min(max(p.ranks[u.adapter], 0), p.rank) : p.rank;
   const T* A = static_cast<const T*>(p.a) + u.adapter * p.a_adapter;
   const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
   const int tiles = (r + 15) / 16, kparts = tiles ? max(kWarps / tiles, 1) : 1;
+
+  // The stream of B's stages of this warp: chunks of 64 columns, in each the ranks
+  // by 32.  It starts before x A^T is known.
+  const int steps = (r + 31) / 32;
+  int next_n = n0 + warp * 64, next_s = 0, next_slot = 0;  // the next stage to fetch
+  auto fetch = [&]() {
+    if (steps && next_n < n1) {
+      const int k = next_s * 32 + 8 * t, m = next_n + 8 * g;
+      uint8_t* to = sm.ring[warp][next_slot] + g * 64 + t * 16;
+      if (k < r) {
+        if (p.b_wide && k + 8 <= p.rank) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) cp_async16(to + j * 512, B + min(m + j, n1 - 1) * p.b_row + k);
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(to + j * 512) = load8(B + min(m + j, n1 - 1) * p.b_row, k, r, false);
+        }
+      }
+      next_slot = next_slot + 1 == kStages ? 0 : next_slot + 1;
+      if (++next_s == steps) next_s = 0, next_n += kWarps * 64;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch();
 
   // This block's part of T^T: warps share the rank tiles and the K steps.
   {
@@ -107,7 +142,6 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   cluster_wait();
 
   // All of t, a warp a row, split into parts.
-  const int steps = (r + 31) / 32;
   {
     const int row = warp;
     const float scale = p.scales ? p.scales[u.adapter] : 1.f;
@@ -116,8 +150,11 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
     for (int i = 0; i < kMaxRank / 32; ++i) {
       const int j = i * 32 + lane;
       v[i] = 0.f;
-      if (j < r)
-        for (int q = 0; q < size; ++q) v[i] += remote_float(&sm.t[row][j], q);
+      if (j < r) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < size) v[i] += remote_float(&sm.t[row][j], q);
+      }
       v[i] *= scale;
       top = fmaxf(top, fabsf(v[i]));
     }
@@ -146,81 +183,67 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   const int ra = 2 * t, rb = 2 * t + 1;
   const bool has_a = ra < u.n_rows, has_b = rb < u.n_rows;
   const float fa = sm.factor[ra], fb = sm.factor[rb];
-  // The next step's loads are under way while one is computed.
   const TY* py[2] = {static_cast<const TY*>(p.y) + (has_a ? rows[ra] : 0) * p.y_row,
                      static_cast<const TY*>(p.y) + (has_b ? rows[rb] : 0) * p.y_row};
   TY* po[2] = {static_cast<TY*>(p.out) + (has_a ? rows[ra] : 0) * p.out_row,
                static_cast<TY*>(p.out) + (has_b ? rows[rb] : 0) * p.out_row};
-  // B's pieces as they lie in memory (columns behind the last one repeat it,
-  // ranks behind the adapter's are cut off where they are used).
-  uint4 v[8];
-  const bool cut = r % 32 != 0;
-  auto load_b = [&](int m, int s) {
-    const int k = s * 32 + 8 * t;
-    if (p.b_wide && s * 32 + 32 <= p.rank) {
-      const T* b = B + k;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint4*>(b + min(m + j, n1 - 1) * p.b_row);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = load8(B + min(m + j, n1 - 1) * p.b_row, k, r, p.b_wide);
-    }
-  };
-  float ya[8], yb[8];
+  const bool cut = r % 32 != 0;  // what lies behind the rank is cut off
+  int slot = 0;
+  float ya[8], yb[8];  // of the next 64 columns
   auto load_y = [&](int m) {
-    if (has_a) load8(py[0], m, n1, p.y_wide, ya);
-    if (has_b) load8(py[1], m, n1, p.y_wide, yb);
+    if (has_a && m < n1) load8(py[0], m, n1, p.y_wide, ya);
+    if (has_b && m < n1) load8(py[1], m, n1, p.y_wide, yb);
   };
-  int n = n0 + warp * 64;
-  if (n < n1) {
-    if (steps) load_b(n + 8 * g, 0);
-    load_y(n + 8 * g);
-  }
+  load_y(n0 + warp * 64 + 8 * g);
 #pragma unroll 1
-  for (; n < n1; n += kWarps * 64) {
+  for (int n = n0 + warp * 64; n < n1; n += kWarps * 64) {
     const int m = n + 8 * g;
-    const bool more = n + kWarps * 64 < n1;
     float d[4][4] = {};
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
-      uint4 w[8];
-      if (cut) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      uint4 f[P];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = first_of(v[j], r - s * 32 - 8 * t);
-      } else {
+      for (int q = 0; q < P; ++q) f[q] = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = v[j];
-      }
-      if (s + 1 < steps) load_b(m, s + 1);
-      else if (more) load_b(m + kWarps * 64, 0);
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* at = sm.ring[warp][slot] + j * 1024 + g * 64 + t * 16;
+        uint4 v = *reinterpret_cast<const uint4*>(at), w = *reinterpret_cast<const uint4*>(at + 512);
+        if (cut) v = first_of(v, r - s * 32 - 8 * t), w = first_of(w, r - s * 32 - 8 * t);
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const uint4 f = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mma16(d[j], w[2 * j].x, w[2 * j + 1].x, w[2 * j].y, w[2 * j + 1].y, f.x, f.y, A);
-          mma16(d[j], w[2 * j].z, w[2 * j + 1].z, w[2 * j].w, w[2 * j + 1].w, f.z, f.w, A);
+        for (int q = 0; q < P; ++q) {
+          mma16(d[j], v.x, w.x, v.y, w.y, f[q].x, f[q].y, A);
+          mma16(d[j], v.z, w.z, v.w, w.w, f[q].z, f[q].w, A);
         }
       }
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+      __syncwarp();
+      fetch();
     }
-    float oa[8], ob[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      oa[2 * j] = fmaf(d[j][0], fa, ya[2 * j]);
-      oa[2 * j + 1] = fmaf(d[j][2], fa, ya[2 * j + 1]);
-      ob[2 * j] = fmaf(d[j][1], fb, yb[2 * j]);
-      ob[2 * j + 1] = fmaf(d[j][3], fb, yb[2 * j + 1]);
+      d[j][0] = fmaf(d[j][0], fa, ya[2 * j]);
+      d[j][2] = fmaf(d[j][2], fa, ya[2 * j + 1]);
+      d[j][1] = fmaf(d[j][1], fb, yb[2 * j]);
+      d[j][3] = fmaf(d[j][3], fb, yb[2 * j + 1]);
     }
-    if (more) load_y(m + kWarps * 64);
+    load_y(m + kWarps * 64);
+    const float oa[8] = {d[0][0], d[0][2], d[1][0], d[1][2], d[2][0], d[2][2], d[3][0], d[3][2]};
+    const float ob[8] = {d[0][1], d[0][3], d[1][1], d[1][3], d[2][1], d[2][3], d[3][1], d[3][3]};
     if (has_a) store8(po[0], m, n1, p.out_wide, oa);
     if (has_b) store8(po[1], m, n1, p.out_wide, ob);
   }
+  cp_async_wait<0>();
   cluster_wait();
 }
 
 template <class T, class TX, class TY>
 cudaError_t run(const Params& p, int n_units, int size, cudaStream_t s) {
-  return launch_clusters(narrow_kernel<T, TX, TY>, n_units, size, kThreads, 0, s, p);
+  const int bytes = (int)sizeof(Smem);
+  const cudaError_t e = cudaFuncSetAttribute(narrow_kernel<T, TX, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(narrow_kernel<T, TX, TY>, n_units, size, kThreads, bytes, s, p);
 }
 template <class T>
 cudaError_t run(const Params& p, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s) {

@@ -38,7 +38,7 @@ struct Params {
 // n_units units on clusters of `size` blocks: of at most kNarrowRows rows (and
 // those without an adapter), or of at most kWideRows.
 cudaError_t launch_narrow(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
-cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
+cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, int sms, cudaStream_t s);
 
 }  // namespace lora
 }  // namespace specb200

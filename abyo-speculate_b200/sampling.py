@@ -98,7 +98,7 @@ def _logits(logits, uniforms, temperature):
             raise _invalid(f"temperature {temp}")
     kind = types[dtype]
     size = _workspace_bytes(n, v, kind)
-    work = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    work = logits.new_empty(size, dtype=torch.uint8)
     return _LOGITS.pack(index, v, kind, temp, logits.data_ptr(), row, n, temps, u, work.data_ptr(), size), work, index
 
 
@@ -112,7 +112,7 @@ def sample_rows(logits, uniforms, temperature=1.0, probs_out=None, tokens_out=No
     a, work, index = _logits(logits, uniforms, temperature)
     n, v = logits.shape
     if tokens_out is None:
-        tokens_out = torch.empty(n, dtype=torch.int32, device=logits.device)
+        tokens_out = logits.new_empty(n, dtype=torch.int32)
         tokens = tokens_out.data_ptr()
     else:
         tokens = _on(tokens_out, "tokens_out", index, torch.int32, n)
@@ -139,7 +139,7 @@ def verify_drafts(logits, drafts, draft_probs, uniforms, row_start, temperature=
         raise _invalid("row_start is empty, [sequences + 1] is needed")
     d = _on(drafts, "drafts", index, torch.int32, n)
     q, row = _rows_of(draft_probs, "draft_probs", index, torch.float32, n, v)
-    count, token = torch.empty(2, seqs, dtype=torch.int32, device=logits.device).unbind()
+    count, token = logits.new_empty(seqs, dtype=torch.int32), logits.new_empty(seqs, dtype=torch.int32)
     rc = lib.spec_batch_verify(a, seqs, start, d, q, row, count.data_ptr(), token.data_ptr(), stream(index))
     if rc:
         _lib.check(rc)
@@ -161,7 +161,7 @@ def verify_trees(logits, tokens, parents, uniforms, row_start, temperature=1.0) 
         raise _invalid("row_start is empty, [sequences + 1] is needed")
     t = _on(tokens, "tokens", index, torch.int32, n)
     up = _on(parents, "parents", index, torch.int32, n)
-    path, count, token = torch.empty(n + 2 * seqs, dtype=torch.int32, device=logits.device).split((n, seqs, seqs))
+    path, count, token = (logits.new_empty(size, dtype=torch.int32) for size in (n, seqs, seqs))
     rc = lib.spec_batch_verify_tree(a, seqs, start, t, up, path.data_ptr(), count.data_ptr(), token.data_ptr(),
                                     stream(index))
     if rc:

@@ -23,7 +23,7 @@ def make(mod, ids, n_adapters):
     return rc, plan, buf
 
 
-@pytest.mark.parametrize("n,adapters,seed", [(1, 1, 0), (7, 3, 1), (64, 64, 2), (300, 2, 3), (2000, 5, 4), (40, 1, 5)])
+@pytest.mark.parametrize("n,adapters,seed", [(1, 1, 0), (7, 3, 1), (64, 64, 2), (300, 2, 3), (2000, 5, 4), (40, 1, 5), (9000, 2, 6)])
 def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
     rng = np.random.default_rng(seed)
     ids = rng.integers(-1, adapters, n)
@@ -46,7 +46,7 @@ def test_empty_plans(mod):
     rc, plan, _ = make(mod, [], 3)
     assert rc == 0 and plan.n_wide == plan.n_narrow == plan.n_bare == 0
     rc, plan, _ = make(mod, [-1, -1], 0)
-    assert rc == 0 and plan.n_narrow == 0 and plan.n_bare == 1
+    assert rc == 0 and plan.n_narrow == 0 and plan.n_bare == 2
 
 
 def test_bad_plans_are_refused(mod):
