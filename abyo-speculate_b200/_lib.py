@@ -139,7 +139,7 @@ class LoraBankDesc(ctypes.Structure):
 class LoraPlanDesc(ctypes.Structure):
     """spec_lora_plan (include/spec_b200.h)."""
 
-    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_wide", "n_narrow", "n_bare", "reserved")] + [
+    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_wide", "n_narrow", "n_bare", "n_tall", "n_big", "reserved")] + [
         ("device_copy", ctypes.c_void_p)]
 
 
@@ -261,8 +261,8 @@ SIGNATURES = [
     ("spec_lora_plan_bytes", ctypes.c_int64, [ctypes.c_int64]),
     ("spec_lora_plan_make", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.POINTER(LoraPlanDesc)]),
-    ("spec_lora_apply", ctypes.c_int,
-     [ctypes.c_void_p] * 6),
+    ("spec_lora_apply", ctypes.c_int, [ctypes.c_void_p] * 6),
+    ("spec_lora_status", ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
 ]
 
 _lib: Optional[ctypes.CDLL] = None

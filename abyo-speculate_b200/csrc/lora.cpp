@@ -16,10 +16,12 @@ namespace {
 
 constexpr int kPlanRows = 1 << 20;
 constexpr int kHalvesMost = 36;  // units of 32 rows: as many clusters of 8 blocks as a B200 holds, two blocks an SM
+constexpr int kTallFrom = 8;     // units of 128 rows from which on they are taken
 constexpr int kNarrowMost = 16;  // rows of an adapter that the kernel for few rows takes, in units of 8
 
-// Layout of a plan: units (of many rows, of few, those without an adapter), then the rows in their order.
-int64_t plan_bytes(int64_t n_rows) { return n_rows * (int64_t)(sizeof(Unit) + sizeof(int)); }
+// Layout of a plan: units (of adapters of very many rows by 128, the same by 64,
+// those of other adapters of many rows, those of few, rows without one), then the rows in their order, then the word of the device's waits.
+int64_t plan_bytes(int64_t n_rows) { return n_rows * (int64_t)(sizeof(Unit) + sizeof(int)) + 16; }
 
 struct Matrix {
   const char* name;
@@ -39,6 +41,11 @@ int cluster_for(int n, int per_sm, int sms) {
   return size;
 }
 
+unsigned* status_of(const spec_lora_plan* plan) {
+  const uint8_t* b = static_cast<const uint8_t*>(plan->device_copy);
+  return const_cast<unsigned*>(reinterpret_cast<const unsigned*>(b + (size_t)plan->n_rows * (sizeof(Unit) + sizeof(int))));
+}
+
 int check_plan_shape(const char* what, int64_t n_rows) {
   if (n_rows < 0 || n_rows > kPlanRows) return fail(SPEC_ERR_INVALID, "%s: %lld rows, 0 to %d are taken", what, (long long)n_rows, kPlanRows);
   return SPEC_OK;
@@ -54,29 +61,41 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return (unsigned)adapters[x] < (unsigned)adapters[y]; });
   // An adapter's rows in units of equal size; rows without one are copied one by
   // one.  Units of 64 rows read A and B half as often as those of 32, which are
-  // taken where there are few of them.
-  int64_t halves = 0;
+  // taken where there are few of them; adapters of more than 64 rows are also cut
+  // by 128, where that gives enough units.
+  struct Run {
+    int adapter, begin, end;
+  };
+  std::vector<Run> runs;
+  int64_t halves = 0, tall = 0;
   for (int i = 0; i < n_rows;) {
     int e = i;
     while (e < n_rows && adapters[order[e]] == adapters[order[i]]) ++e;
-    if (adapters[order[i]] >= 0 && e - i > kNarrowMost) halves += (e - i + kWideRows / 2 - 1) / (kWideRows / 2);
+    runs.push_back(Run{adapters[order[i]], i, e});
+    if (adapters[order[i]] >= 0 && e - i > kNarrowMost) {
+      halves += (e - i + kWideRows / 2 - 1) / (kWideRows / 2);
+      if (e - i > kWideRows) tall += (e - i + kTallRows - 1) / kTallRows;
+    }
     i = e;
   }
   const int wide_rows = halves <= kHalvesMost ? kWideRows / 2 : kWideRows;
-  std::vector<Unit> units[3];
-  for (int i = 0; i < n_rows;) {
-    int e = i;
-    const int a = adapters[order[i]];
-    while (e < n_rows && adapters[order[e]] == a) ++e;
-    const int kind = a < 0 ? 2 : e - i > kNarrowMost ? 0 : 1, most = kind == 2 ? 1 : kind ? kNarrowRows : wide_rows;
-    const int n = (e - i + most - 1) / most;
+  std::vector<Unit> units[5];
+  auto cut = [&](std::vector<Unit>& to, const Run& r, int most) {
+    const int rows = r.end - r.begin, n = (rows + most - 1) / most;
     for (int k = 0; k < n; ++k) {
-      const int at = i + (int)((int64_t)(e - i) * k / n), end = i + (int)((int64_t)(e - i) * (k + 1) / n);
-      Unit u{a, at, end - at, 0, {}};
+      const int at = r.begin + (int)((int64_t)rows * k / n), end = r.begin + (int)((int64_t)rows * (k + 1) / n);
+      Unit u{r.adapter, at, end - at, 0, {}};
       for (int j = 0; j < kNarrowRows && at + j < end; ++j) u.row[j] = order[at + j];
-      units[kind].push_back(u);
+      to.push_back(u);
     }
-    i = e;
+  };
+  for (const Run& r : runs) {
+    const int rows = r.end - r.begin;
+    const bool big = r.adapter >= 0 && rows > kWideRows && tall >= kTallFrom;
+    if (big) cut(units[0], r, kTallRows);
+    if (r.adapter < 0) cut(units[4], r, 1);
+    else if (rows <= kNarrowMost) cut(units[3], r, kNarrowRows);
+    else cut(units[big ? 1 : 2], r, wide_rows);
   }
   uint8_t* b = static_cast<uint8_t*>(buf);
   if (n_rows) {
@@ -87,12 +106,15 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
     }
     memcpy(b + (size_t)n_rows * sizeof(Unit), order.data(), (size_t)n_rows * sizeof(int));
   }
+  memset(b + (size_t)n_rows * (sizeof(Unit) + sizeof(int)), 0, 16);
   *out = spec_lora_plan{};
   out->n_rows = n_rows;
   out->n_adapters = n_adapters;
-  out->n_wide = (int)units[0].size();
-  out->n_narrow = (int)units[1].size();
-  out->n_bare = (int)units[2].size();
+  out->n_tall = (int)units[0].size();
+  out->n_big = (int)units[1].size();
+  out->n_wide = (int)units[2].size();
+  out->n_narrow = (int)units[3].size();
+  out->n_bare = (int)units[4].size();
   return SPEC_OK;
 }
 
@@ -108,7 +130,7 @@ int64_t spec_lora_plan_bytes(int64_t n_rows) {
 int spec_lora_plan_make(const int32_t* adapters, int n_rows, int n_adapters, void* buf, int64_t buf_bytes,
                         spec_lora_plan* out) {
   const char* what = "spec_lora_plan_make";
-  if (!out || (n_rows > 0 && (!adapters || !buf))) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
+  if (!out || !buf || (n_rows > 0 && !adapters)) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
   const int rc = check_plan_shape(what, n_rows);
   if (rc != SPEC_OK) return rc;
   if (n_adapters < 0) return fail(SPEC_ERR_INVALID, "%s: %d adapters", what, n_adapters);
@@ -131,8 +153,8 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
     return fail(SPEC_ERR_INVALID, "%s: %d adapters of %d to %d channels", what, b->n_adapters, b->k, b->n);
   if (b->rank < 0 || b->rank > kMaxRank) return fail(SPEC_ERR_UNSUPPORTED, "%s: rank %d (up to %d is built)", what, b->rank, kMaxRank);
   if (b->device < 0) return fail(SPEC_ERR_INVALID, "%s: device %d", what, b->device);
-  if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_wide < 0 || plan->n_narrow < 0 || plan->n_bare < 0 ||
-      (int64_t)plan->n_wide + plan->n_narrow + plan->n_bare > plan->n_rows)
+  if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_wide < 0 || plan->n_narrow < 0 || plan->n_bare < 0 || plan->n_tall < 0 || plan->n_big < 0 ||
+      (int64_t)plan->n_tall + plan->n_big + plan->n_wide + plan->n_narrow + plan->n_bare > plan->n_rows)
     return fail(SPEC_ERR_INVALID, "%s: not a plan", what);
   if (plan->n_adapters > b->n_adapters)
     return fail(SPEC_ERR_INVALID, "%s: a plan for %d adapters, the bank has %d", what, plan->n_adapters, b->n_adapters);
@@ -157,7 +179,7 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool in_place = y->ptr == out->ptr;
   if (in_place && plan->n_rows > 1 && y->row_stride != out->row_stride)
     return fail(SPEC_ERR_INVALID, "%s: y in place needs one row stride", what);
-  if (plan->n_wide || plan->n_narrow) {
+  if (plan->n_big || plan->n_wide || plan->n_narrow) {
     if ((b->rank > 0 && (!b->a || !b->b)) || misaligned(b->a, 2) || misaligned(b->b, 2) || misaligned(b->ranks, 4) || misaligned(b->scales, 4))
       return fail(SPEC_ERR_INVALID, "%s: a pointer of the bank is null or not aligned to its element size", what);
     for (const int64_t s : {b->a_adapter_stride, b->a_row_stride, b->b_adapter_stride, b->b_row_stride})
@@ -195,11 +217,28 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.units = units;
-  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, plan->n_wide, cluster_for(plan->n_wide, 2, sms), sms, s);
-  p.units = units + plan->n_wide;
+  bool taken = false;
+  if (e == cudaSuccess && plan->n_tall && !x_f32)
+    e = launch_tall(p, status_of(plan), b->dtype, y_f32, plan->n_tall, cluster_for(plan->n_tall, 1, sms), s, &taken);
+  p.units = units + plan->n_tall + (taken ? plan->n_big : 0);
+  const int wide = plan->n_wide + (taken ? 0 : plan->n_big);
+  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, cluster_for(wide, 2, sms), sms, s);
+  p.units = units + plan->n_tall + plan->n_big + plan->n_wide;
   const int n = plan->n_narrow + (in_place ? 0 : plan->n_bare);
   if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 2, sms), s);
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
+}
+
+int spec_lora_status(const spec_lora_plan* plan, int device, void* stream) {
+  const char* what = "spec_lora_status";
+  if (!plan || plan->n_rows < 0 || plan->n_rows > kPlanRows || !plan->device_copy || misaligned(plan->device_copy, 16) || device < 0)
+    return fail(SPEC_ERR_INVALID, "%s: not a plan on a device", what);
+  Current cur(device, what);
+  if (cur.rc != SPEC_OK) return cur.rc;
+  char msg[256];
+  const int rc = take_device_error(status_of(plan), static_cast<cudaStream_t>(stream), msg, sizeof msg);
+  if (rc != SPEC_OK) set_thread_error(msg);
+  return rc;
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@ enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
 constexpr int kMaxRank = 128;
 constexpr int kNarrowRows = 8;  // rows of a unit of the kernel for few rows: one n-tile of the products
 constexpr int kWideRows = 64;   // of the one for many
+constexpr int kTallRows = 128;  // and of the one for very many
 
 // Rows of one adapter (-1: none) that one cluster takes.
 struct Unit {
@@ -39,6 +40,8 @@ struct Params {
 // those without an adapter), or of at most kWideRows.
 cudaError_t launch_narrow(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
 cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, int sms, cudaStream_t s);
+// The same of at most kTallRows rows, x of the adapters' type; *taken: the rank fits.  A device wait that gives up sets *err.
+cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int size, cudaStream_t s, bool* taken);
 
 }  // namespace lora
 }  // namespace specb200

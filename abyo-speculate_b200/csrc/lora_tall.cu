@@ -1,0 +1,431 @@
+// Low-rank adapters, very many rows of one adapter: out = y + s (x A^T) B^T for up
+// to 128 rows a cluster of blocks, on tcgen05 with accumulators in tensor memory.
+//
+// First product, T [128 x N] = X [128 x K] A^T (N: the rank up to a multiple of
+// 16): the blocks of a cluster share K; stages of 128 columns of the rows and of A
+// are copied asynchronously into the K-major operand layout without swizzle ([8
+// columns][8-row group][8 rows x 16 bytes], so that 8 lanes write a group's 128
+// bytes), and one elected thread issues the stage's 8 products.  The blocks'
+// parts join as in the kernel for fewer rows.  Second product: T's parts are the
+// 128-row operand, B's 64 columns a stage the other; while a stage's products
+// run, all threads add the stage before it to y, which came with B into rows 16
+// bytes further apart than they are long, and store it along the rows.
+//
+// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels: bound by
+// the copies, whose 16-byte pieces go through the load units.
+#include "lora_mma.cuh"
+
+namespace specb200 {
+namespace lora {
+namespace {
+
+constexpr int kStep = 128;        // columns of a stage of the first product
+constexpr int kCols = 64;         // and of the second
+constexpr int kMaxStages = 6;
+constexpr int kGroups = kTallRows / 8;
+constexpr int kTmem = 256;        // columns: T, and two accumulators of the second product from 128 on
+
+struct TallParams {
+  Params p;
+  unsigned* err;
+  int N, stages, stages2, all_at;  // ring sizes; where T whole lies
+};
+
+template <class TY>
+__host__ __device__ constexpr int y_pitch() {
+  return kCols * (int)sizeof(TY) + 16;
+}
+template <class TY>
+__host__ __device__ constexpr int stage2(int N) {
+  return kTallRows * y_pitch<TY>() + N * 2 * kCols;
+}
+__host__ __device__ constexpr int stage1(int N) { return (kTallRows + N) * 2 * kStep; }
+__host__ __device__ constexpr int frag_bytes(int P, int N) { return P * N * 2 * kTallRows; }
+
+SPEC_DEV uint32_t idesc(int N, const __nv_bfloat16*) { return umma_idesc_bf16(128, N); }
+SPEC_DEV uint32_t idesc(int N, const __half*) { return umma_idesc_bf16(128, N) & ~((7u << 7) | (7u << 10)); }  // formats 0: f16
+
+SPEC_DEV void cp_async_wait_for(int n) {
+  switch (n) {
+    case 0: cp_async_wait<0>(); break;
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    default: cp_async_wait<4>(); break;
+  }
+}
+SPEC_DEV void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Up to 8 elements from `src`, of which `left` are there, to shared memory; zeros behind them.
+template <class T>
+SPEC_DEV void copy8(uint8_t* dst, const T* src, int left, bool wide) {
+  if (wide && left >= 8) {
+    cp_async16(dst, src);
+    return;
+  }
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < left) w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[i] << (i % 2 * 16);
+  *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+SPEC_DEV void unpack16(const uint8_t* p, float (&x)[4], const float*) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+template <class T>
+SPEC_DEV void unpack16(const uint8_t* p, float (&x)[8], const T* tag) {
+  widen(*reinterpret_cast<const uint4*>(p), x, tag);
+}
+SPEC_DEV void pack16(uint8_t* p, const float (&x)[4], const float*) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <class T>
+SPEC_DEV void pack16(uint8_t* p, const float (&x)[8], const T* tag) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2(x[0], x[1], tag), pack2(x[2], x[3], tag), pack2(x[4], x[5], tag), pack2(x[6], x[7], tag));
+}
+
+template <class T, class TY>
+__global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant__ TallParams tp) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t s_free[kMaxStages], s_done[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ const TY* s_row[kTallRows];
+  const Params& p = tp.p;
+  constexpr int P = parts_of<TY>((const T*)nullptr);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = cluster_rank(), size = cluster_size(), N = tp.N;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Unit& u = p.units[blockIdx.x / size];
+  const int* rows = p.order + u.first;
+  const int n_rows = u.n_rows;
+  const int r = p.ranks ? min(max(p.ranks[u.adapter], 0), p.rank) : p.rank;
+  const T* A = static_cast<const T*>(p.a) + u.adapter * p.a_adapter;
+  const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kMaxStages; ++i) mbar_init(&s_free[i], 1);
+    mbar_init(&s_done[0], 1);
+    mbar_init(&s_done[1], 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) tmem_alloc(&s_tmem, kTmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  bool ok = true;  // no wait gave up
+
+  // ---- T ----
+  float* part = reinterpret_cast<float*>(smem);
+  const int Wp = N + 4;  // floats between T's rows
+  {
+    const int k_per = (p.K + size * kStep - 1) / (size * kStep) * kStep, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K);
+    const int width = k1 - k0, n_steps = r ? (width + kStep - 1) / kStep : 0, stages = tp.stages, sb = stage1(N);
+    const int a_lbo = N * 16;  // bytes of 8 columns of A
+    // Rows of this lane: two 8-row groups a warp.  Rows behind the last one are
+    // copies of it, T's columns behind the adapter's rank whatever the memory
+    // holds: neither is used.
+    const int row0 = warp * 16 + lane % 8, kp = lane / 8;
+    const T* x0 = static_cast<const T*>(p.x) + rows[min(row0, n_rows - 1)] * p.x_row + k0 + kp * 8;
+    const T* x1 = static_cast<const T*>(p.x) + rows[min(row0 + 8, n_rows - 1)] * p.x_row + k0 + kp * 8;
+    const T* a0 = A + (warp * 8 + lane % 8) * p.a_row + k0 + kp * 8;
+    const bool fast = p.x_wide && p.a_wide;
+    int next = 0, at = 0;  // of the next stage to fetch: its first column, its offset
+    auto fetch = [&]() {
+      uint8_t* xt = smem + at + kp * (kGroups * 128) + warp * 256 + lane % 8 * 16;
+      uint8_t* ta = smem + at + kTallRows * 2 * kStep + kp * a_lbo + warp * 128 + lane % 8 * 16;
+      const bool whole = fast && next + kStep <= width;
+#pragma unroll
+      for (int q = 0; q < kStep / 32; ++q) {
+        const int k = next + q * 32, left = width - k - kp * 8;
+        if (whole) {
+          cp_async16(xt + q * (kGroups * 512), x0 + k);
+          cp_async16(xt + q * (kGroups * 512) + 128, x1 + k);
+        } else {
+          copy8(xt + q * (kGroups * 512), x0 + k, left, p.x_wide);
+          copy8(xt + q * (kGroups * 512) + 128, x1 + k, left, p.x_wide);
+        }
+      }
+      for (int j = warp * 8 + lane % 8, o = 0; j < r; j += kWarps * 8, ++o) {
+        const T* a = a0 + o * (kWarps * 8) * p.a_row + next;
+#pragma unroll
+        for (int q = 0; q < kStep / 32; ++q) {
+          uint8_t* to = ta + o * (kWarps * 128) + q * 4 * a_lbo;
+          if (whole) cp_async16(to, a + q * 32);
+          else copy8(to, a + q * 32, width - next - q * 32 - kp * 8, p.a_wide);
+        }
+      }
+      next += kStep;
+      at = at + sb == stages * sb ? 0 : at + sb;
+    };
+    for (int s = 0; s < stages - 1; ++s) {
+      if (s < n_steps) fetch();
+      cp_async_commit();
+    }
+    const uint32_t id = idesc(N, A), base = smem_u32(smem);
+    int slot = 0, phase = 0;  // of this step; phase: of the slot before it
+#pragma unroll 1
+    for (int step = 0; step < n_steps; ++step) {
+      cp_async_wait_for(stages - 2);
+      publish_smem();
+      ok = __syncthreads_and(ok);
+      if (!ok) break;
+      if (threadIdx.x == 0) {
+        tc_fence_after();
+        const uint32_t xs = base + slot * sb, as = xs + kTallRows * 2 * kStep;
+#pragma unroll 1
+        for (int k = 0; k < kStep / 16; ++k)
+          umma_bf16(tmem, umma_desc_kmajor(xs + k * 2 * kGroups * 128, kGroups * 128, 128),
+                    umma_desc_kmajor(as + k * 2 * a_lbo, a_lbo, 128), id, step | k);
+        umma_commit(&s_free[slot]);
+      }
+      // The slot before this one is filled again once its products are done.
+      if (step > 0) {
+        const int before = slot ? slot - 1 : stages - 1;
+        ok = mbar_wait_bounded(&s_free[before], phase, tp.err);
+        if (before == stages - 1) phase ^= 1;
+      }
+      if (step + stages - 1 < n_steps && ok) fetch();
+      cp_async_commit();
+      slot = slot + 1 == stages ? 0 : slot + 1;
+    }
+    ok = __syncthreads_and(ok);
+    if (n_steps && ok) ok = mbar_wait_bounded(&s_free[slot ? slot - 1 : stages - 1], phase, tp.err);
+    cp_async_wait<0>();
+    ok = __syncthreads_and(ok);
+    tc_fence_after();
+    // A warp reads 32 rows, half of the columns.
+    float* o = part + (warp % 4 * 32 + lane) * Wp + warp / 4 * (N / 2);
+    for (int c = 0; c < N / 2; c += 8) {
+      uint32_t v[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+      if (n_steps) {  // else this block has no part of K
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                     : "r"(tmem + ((uint32_t)(warp % 4 * 32) << 16) + warp / 4 * (N / 2) + c)
+                     : "memory");
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i])::"memory");
+      }
+      *reinterpret_cast<uint4*>(o + c) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint4*>(o + c + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+    tc_fence_before();
+    __syncthreads();
+  }
+
+  // ---- the parts of T join ----
+  float* all = reinterpret_cast<float*>(smem + tp.all_at);
+  const int live = kTallRows * Wp;
+  cluster_arrive();
+  cluster_wait();
+  const int share = (live / 4 + size - 1) / size * 4;
+  for (int i = rank * share + threadIdx.x * 4; i < min((rank + 1) * share, live); i += kThreads * 4) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < size; ++q) {
+      const float4 v = remote_float4(part + i, q);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    *reinterpret_cast<float4*>(all + i) = s;
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int i = threadIdx.x * 4; i < live; i += kThreads * 4)
+    if (i / share != rank) *reinterpret_cast<float4*>(all + i) = remote_float4(all + i, i / share);
+  cluster_arrive();  // nothing of the other blocks is read any more
+  __syncthreads();
+  // In part's place: the numbers that T is split into, two threads a row.  A
+  // thread keeps the factor of the row that it finishes.
+  const int my_row = warp % 4 * 32 + lane;
+  float factor;
+  {
+    const int row = threadIdx.x / 2, h = threadIdx.x % 2;
+    const float scale = p.scales ? p.scales[u.adapter] : 1.f;
+    float top = 0.f;
+    for (int j = h * 8; j < r; j += 16)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (j + k < r) top = fmaxf(top, fabsf(all[row * Wp + j + k] * scale));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const int e = exponent(top, A);
+    const float down = pow2i(-e);
+    for (int j = h * 8; j < N; j += 16) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = j + k < r ? all[row * Wp + j + k] * scale * down : 0.f;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          w[k] = pack2(v[2 * k], v[2 * k + 1], A);
+          T hl[2];
+          *reinterpret_cast<uint32_t*>(hl) = w[k];
+          v[2 * k] = fabsf(v[2 * k]) < INFINITY ? v[2 * k] - to_float(hl[0]) : 0.f;
+          v[2 * k + 1] = fabsf(v[2 * k + 1]) < INFINITY ? v[2 * k + 1] - to_float(hl[1]) : 0.f;
+        }
+        *reinterpret_cast<uint4*>(smem + q * (N * 2 * kTallRows) + j / 8 * (kGroups * 128) + row / 8 * 128 + row % 8 * 16) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    // Row of thread 2 i is i: the factors change hands through the rows' pads.
+    if (h == 0) all[row * Wp + N] = pow2i(e);
+    __syncthreads();
+    factor = all[my_row * Wp + N];
+  }
+  cluster_wait();  // nor anything of this one
+  __syncthreads();
+
+  // ---- Y ----
+  if (ok) {
+    const int n_per = (p.N + size * kCols - 1) / (size * kCols) * kCols, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
+    const int width = n1 - n0, n_steps = (width + kCols - 1) / kCols, stages = tp.stages2, sb = stage2<TY>(N);
+    constexpr int YP = kCols * (int)sizeof(TY) / 16, YR = 32 / YP, YN = kTallRows / kWarps / YR, E = 16 / (int)sizeof(TY);
+    uint8_t* ring = smem + frag_bytes(P, N);  // `all` is not used any more
+    if (threadIdx.x < kTallRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
+    __syncthreads();
+    const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
+    const int quads = (N + 31) / 32, y_row = warp * 16 + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
+    int next = 0, at = 0;
+    auto fetch = [&]() {
+      const bool whole = fast && next + kCols <= width;
+      const int yk = next + lane % YP * E;
+#pragma unroll
+      for (int i = 0; i < YN; ++i) {
+        uint8_t* to = ring + at + y_at + i * YR * y_pitch<TY>();
+        const TY* from = s_row[y_row + i * YR] + yk;
+        if (whole) {
+          cp_async16(to, from);
+        } else if (p.y_wide && yk + E <= width) {
+          cp_async16(to, from);
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < E; ++e)
+            if (yk + e < width) reinterpret_cast<TY*>(to)[e] = from[e];
+        }
+      }
+      uint8_t* tb = ring + at + kTallRows * y_pitch<TY>() + lane % 8 * 16;
+      for (int i = warp; i < 8 * quads; i += kWarps) {
+        const int k8 = i / 8 * 4 + lane / 8, column = min(next + i % 8 * 8 + lane % 8, width - 1);
+        if (k8 * 8 >= N) continue;
+        const T* from = B + (n0 + column) * p.b_row + k8 * 8;
+        uint8_t* to = tb + k8 * (kCols * 16) + i % 8 * 128;
+        if (whole && k8 * 8 < r) cp_async16(to, from);
+        else copy8(to, from, r - k8 * 8, p.b_wide);
+      }
+      next += kCols;
+      at = at + sb == stages * sb ? 0 : at + sb;
+    };
+    publish_smem();  // T's parts
+    for (int s = 0; s < stages - 2; ++s) {
+      if (s < n_steps) fetch();
+      cp_async_commit();
+    }
+    const uint32_t id = idesc(kCols, A), frag = smem_u32(smem);
+    int slot = 0;
+    // One step more than there are stages: the last one only finishes.
+#pragma unroll 1
+    for (int step = 0; step <= n_steps; ++step) {
+      cp_async_wait_for(stages - 3);
+      publish_smem();
+      ok = __syncthreads_and(ok);  // also: the stage before is stored
+      if (!ok) break;
+      if (threadIdx.x == 0 && step < n_steps && r) {
+        tc_fence_after();
+        const uint32_t bs = smem_u32(ring) + slot * sb + kTallRows * y_pitch<TY>(), to = tmem + 128 + step % 2 * kCols;
+#pragma unroll 1
+        for (int q = 0; q < P; ++q)
+#pragma unroll 1
+          for (int k = 0; k < N / 16; ++k)
+            umma_bf16(to, umma_desc_kmajor(frag + q * (N * 2 * kTallRows) + k * 2 * kGroups * 128, kGroups * 128, 128),
+                      umma_desc_kmajor(bs + k * 2 * (kCols * 16), kCols * 16, 128), id, q | k);
+        umma_commit(&s_done[step % 2]);
+      }
+      // The slot of two steps ago is free.
+      if (step + stages - 2 < n_steps) fetch();
+      cp_async_commit();
+      if (step > 0) {
+        const int before = slot ? slot - 1 : stages - 1, n = (step - 1) * kCols;
+        uint8_t* st = ring + before * sb;
+        if (r) {
+          ok = mbar_wait_bounded(&s_done[(step - 1) % 2], (step - 1) / 2 % 2, tp.err);
+          tc_fence_after();
+          uint32_t v[2][16];
+          const uint32_t from = tmem + ((uint32_t)(warp % 4 * 32) << 16) + 128 + (step - 1) % 2 * kCols + warp / 4 * 32;
+          tmem_ld16(from, v[0]);
+          tmem_ld16(from + 16, v[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i / 16][i % 16])::"memory");
+          tc_fence_before();
+          uint8_t* y = st + my_row * y_pitch<TY>() + warp / 4 * 32 * (int)sizeof(TY);
+#pragma unroll
+          for (int i = 0; i < 32 / E; ++i) {
+            float f[E];
+            unpack16(y + i * 16, f, (const TY*)nullptr);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = fmaf(__uint_as_float(v[(i * E + e) / 16][(i * E + e) % 16]), factor, f[e]);
+            pack16(y + i * 16, f, (const TY*)nullptr);
+          }
+        }
+        __syncthreads();
+        const bool whole = p.out_wide && n + kCols <= width;
+#pragma unroll
+        for (int i = 0; i < YN; ++i) {
+          const int row = y_row + i * YR;
+          if (row >= n_rows) continue;
+          TY* o = static_cast<TY*>(p.out) + rows[row] * p.out_row + n0 + n + lane % YP * E;
+          const uint8_t* v = st + y_at + i * YR * y_pitch<TY>();
+          if (whole) {
+            *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
+          } else {
+#pragma unroll 1
+            for (int e = 0; e < E; ++e)
+              if (n + lane % YP * E + e < width) o[e] = reinterpret_cast<const TY*>(v)[e];
+          }
+        }
+      }
+      slot = slot + 1 == stages ? 0 : slot + 1;
+    }
+    cp_async_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, kTmem);
+}
+
+// Shared memory of the form for N columns of T, 0 where it does not fit.
+template <class T, class TY>
+int plan_memory(TallParams* t, int N) {
+  constexpr int P = parts_of<TY>((const T*)nullptr), kMost = 222 * 1024;
+  const int whole = kTallRows * (N + 4) * 4, frag = frag_bytes(P, N);
+  t->N = N;
+  t->all_at = (whole > frag ? whole : frag) / 128 * 128 + 128;
+  t->stages = kMost / stage1(N) < kMaxStages ? kMost / stage1(N) : kMaxStages;
+  t->stages2 = (kMost - frag) / stage2<TY>(N) < kMaxStages ? (kMost - frag) / stage2<TY>(N) : kMaxStages;
+  return t->stages >= 2 && t->stages2 >= 3 && t->all_at + whole <= kMost ? kMost : 0;
+}
+
+template <class T, class TY>
+cudaError_t run(const Params& p, unsigned* err, int n_units, int size, cudaStream_t s, bool* taken) {
+  TallParams t{p, err, 0, 0, 0, 0};
+  const int bytes = plan_memory<T, TY>(&t, p.rank > 16 ? (p.rank + 15) / 16 * 16 : 16);
+  *taken = bytes > 0;
+  if (!bytes) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(tall_kernel<T, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(tall_kernel<T, TY>, n_units, size, kThreads, bytes, s, t);
+}
+
+}  // namespace
+
+cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int size, cudaStream_t s, bool* taken) {
+  if (type == T_BF16)
+    return y_f32 ? run<__nv_bfloat16, float>(p, err, n_units, size, s, taken) : run<__nv_bfloat16, __nv_bfloat16>(p, err, n_units, size, s, taken);
+  return y_f32 ? run<__half, float>(p, err, n_units, size, s, taken) : run<__half, __half>(p, err, n_units, size, s, taken);
+}
+
+}  // namespace lora
+}  // namespace specb200

@@ -285,6 +285,8 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   }
   __syncthreads();
 
+  if (size > 1) cluster_wait();  // nor anything of this one: the rings may take its place
+
   // ---- Y ----
   {
     const int n_per = (p.N + size * 32 - 1) / (size * 32) * 32, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N), width = n1 - n0;
@@ -391,7 +393,6 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     }
     cp_async_wait<0>();
   }
-  if (size > 1) cluster_wait();
 }
 
 template <class T, class TX, class TY, int NT>

@@ -56,6 +56,11 @@ class LoraPlan:
         self._at = ctypes.addressof(self._desc)
         self._made_on = torch.cuda.current_stream(self.device).cuda_stream
 
+    def status(self) -> None:
+        """Waits for the current stream's calls; raises if a device wait in a call with this plan gave up."""
+        _, lib, _, current = _setup()
+        _lib.check(lib.spec_lora_status(self._at, self.device.index, current(self.device.index)))
+
 
 class LoraBank:
     """The adapters of one projection (spec_lora_bank).

@@ -726,7 +726,7 @@ typedef struct spec_lora_bank {
  * and fills *out but for device_copy: the caller copies buf to the device, sets
  * it, and keeps both unchanged until the calls that use them are done. */
 typedef struct spec_lora_plan {
-  int n_rows, n_adapters, n_wide, n_narrow, n_bare, reserved;
+  int n_rows, n_adapters, n_wide, n_narrow, n_bare, n_tall, n_big, reserved;
   const void* device_copy;     /* 16-byte aligned */
 } spec_lora_plan;
 int64_t spec_lora_plan_bytes(int64_t n_rows);
@@ -745,6 +745,9 @@ typedef struct spec_lora_rows {
  * rows behind the plan's last one are left as they are. */
 int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const spec_lora_rows* x, const spec_lora_rows* y,
                     const spec_lora_rows* out, void* stream);
+/* Waits for the stream and reports (and clears) a device wait that gave up in
+ * an earlier call with this plan (SPEC_ERR_TIMEOUT; its results are incomplete). */
+int spec_lora_status(const spec_lora_plan* plan, int device, void* stream);
 
 #ifdef __cplusplus
 }

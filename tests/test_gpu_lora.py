@@ -163,6 +163,26 @@ def test_rows_of_one_adapter(pkg, counts):
         Case(pkg, ids, len(counts), 288, 352, 16, dtype, x, y, seed=len(ids)).check()
 
 
+@pytest.mark.parametrize("dtype,x,y", TYPES)
+@pytest.mark.parametrize("counts,k,n,rank", [([1100], 256, 320, 16), ([700, 65, 500, 9, 3], 1000, 333, 24), ([1500, 40], 129, 1025, 64),
+                                             ([1024], 4096, 128, 128), ([900, 201], 64, 64, 1), ([1300], 640, 200, 90)])
+def test_very_many_rows(pkg, counts, k, n, rank, dtype, x, y):
+    import torch
+    ids = np.concatenate([np.full(c, i) for i, c in enumerate(counts)] + [np.full(7, -1)])
+    np.random.default_rng(1).shuffle(ids)
+    c = Case(pkg, ids, len(counts), k, n, rank, dtype, x, y, seed=k)
+    c.check(out=torch.full_like(c.y, float("nan")))
+    c.check()
+    c.plan.status()
+
+
+@pytest.mark.parametrize("pad", [(1, 0, 0, 0), (0, 3, 0, 0), (0, 0, 5, 0), (0, 0, 0, 7), (8, 8, 8, 8)])
+def test_very_many_rows_of_other_strides_and_ranks(pkg, pad):
+    ids = np.random.default_rng(2).integers(0, 4, 1600)
+    for dtype, y in (("bf16", "same"), ("f16", "f32")):
+        Case(pkg, ids, 4, 264, 200, 32, dtype, "same", y, ranks=[0, 5, 16, 31], pad=pad, seed=5).check()
+
+
 def test_long_sums(pkg):
     for rows in (3, 100):
         Case(pkg, [0] * rows, 1, 18944, 3584, 16, "bf16", seed=1).check()

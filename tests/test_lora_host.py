@@ -29,17 +29,20 @@ def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
     ids = rng.integers(-1, adapters, n)
     rc, plan, buf = make(mod, ids, adapters)
     assert rc == 0 and plan.n_rows == n and plan.n_adapters == adapters
-    with_one = plan.n_wide + plan.n_narrow
-    units = buf[:48 * (with_one + plan.n_bare)].view(np.int32).reshape(-1, 12)
-    order = buf[48 * n:].view(np.int32)
-    seen = []
-    for i, (a, first, count, _, *near) in enumerate(units):
-        assert 0 < count <= (64 if i < plan.n_wide else 8) and (a >= 0) == (i < with_one)
+    counts = [plan.n_tall, plan.n_big, plan.n_wide, plan.n_narrow, plan.n_bare]
+    units = buf[:48 * sum(counts)].view(np.int32).reshape(-1, 12)
+    order = buf[48 * n:52 * n].view(np.int32)
+    kind = np.repeat(np.arange(5), counts)
+    seen = [[], [], [], [], []]
+    for k, (a, first, count, _, *near) in zip(kind, units):
+        assert 0 < count <= (128, 64, 64, 8, 1)[k] and (a >= 0) == (k < 4)
         assert near[:count] == order[first:first + min(count, 8)].tolist()
         rows = order[first:first + count]
         assert (ids[rows] == a).all()
-        seen += rows.tolist()
-    assert sorted(seen) == list(range(n))
+        seen[k] += rows.tolist()
+    assert sorted(sum(seen[1:], [])) == list(range(n))
+    assert sorted(seen[0]) == sorted(seen[1])  # the same rows, for another kernel
+    assert (buf[52 * n:] == 0).all()
 
 
 def test_empty_plans(mod):
@@ -53,10 +56,10 @@ def test_bad_plans_are_refused(mod):
     lib = mod.load()
     assert make(mod, [0, 3], 3)[0] == 1 and make(mod, [-2], 3)[0] == 1 and make(mod, [0], -1)[0] == 1
     assert lib.spec_lora_plan_bytes(-1) == -1 and lib.spec_lora_plan_bytes(1 << 21) == -1
-    ids, buf, plan = np.zeros(4, np.int32), np.zeros(208, np.uint8), mod.LoraPlanDesc()
-    args = [ids.ctypes.data, 4, 1, buf.ctypes.data, 208, ctypes.byref(plan)]
+    ids, buf, plan = np.zeros(4, np.int32), np.zeros(224, np.uint8), mod.LoraPlanDesc()
+    args = [ids.ctypes.data, 4, 1, buf.ctypes.data, 224, ctypes.byref(plan)]
     assert lib.spec_lora_plan_make(*args) == 0
-    for at, bad in ((0, None), (1, -1), (3, None), (4, 207), (5, None)):
+    for at, bad in ((0, None), (1, -1), (3, None), (4, 223), (5, None)):
         assert lib.spec_lora_plan_make(*args[:at], bad, *args[at + 1:]) == 1
 
 
@@ -66,7 +69,7 @@ def test_bad_calls_are_refused(mod):
     def call(bank=(), plan=(), x=(), y=(), out=()):
         b = dict(device=0, n_adapters=2, k=64, n=32, rank=8, dtype=0, a=P, b=P, a_adapter_stride=512, a_row_stride=64,
                  b_adapter_stride=256, b_row_stride=8, ranks=None, scales=None)
-        p = dict(n_rows=3, n_adapters=2, n_wide=0, n_narrow=1, n_bare=1, reserved=0, device_copy=P)
+        p = dict(n_rows=3, n_adapters=2, n_wide=0, n_narrow=1, n_bare=1, n_tall=0, n_big=0, reserved=0, device_copy=P)
         r = [dict(ptr=P, row_stride=64, n_rows=3, dtype=0, reserved=0), dict(ptr=P, row_stride=32, n_rows=3, dtype=0, reserved=0),
              dict(ptr=P + 4096, row_stride=32, n_rows=3, dtype=0, reserved=0)]
         b.update(bank), p.update(plan)
@@ -81,7 +84,7 @@ def test_bad_calls_are_refused(mod):
         assert call(bank=change) == 1, change
     for change in (dict(dtype=2), dict(dtype=-1), dict(rank=129), dict(rank=-1)):
         assert call(bank=change) == 3, change
-    for change in (dict(n_rows=-1), dict(n_narrow=-1), dict(n_wide=-1), dict(n_bare=-1), dict(n_narrow=3), dict(n_wide=2), dict(device_copy=None), dict(device_copy=P + 8),
+    for change in (dict(n_rows=-1), dict(n_narrow=-1), dict(n_wide=-1), dict(n_bare=-1), dict(n_narrow=3), dict(n_wide=2), dict(n_tall=-1), dict(n_tall=2), dict(n_big=-1), dict(device_copy=None), dict(device_copy=P + 8),
                    dict(n_rows=(1 << 20) + 1)):
         assert call(plan=change) == 1, change
     for which in ("x", "y", "out"):
@@ -92,6 +95,7 @@ def test_bad_calls_are_refused(mod):
     assert call(out=dict(row_stride=31)) == 1                        # rows that overlap
     assert call(out=dict(ptr=P, row_stride=40)) == 1                 # in place, two strides
     assert lib.spec_lora_apply(None, None, None, None, None, None) == 1
+    assert lib.spec_lora_status(None, 0, None) == 1
     assert call(plan=dict(n_rows=0, n_narrow=0, n_bare=0)) == 0       # nothing to do
 
 
