@@ -3,9 +3,9 @@
 //
 // First product, T [128 x N] = X [128 x K] A^T (N: the rank up to a multiple of
 // 16): the blocks of a cluster share K; stages of 128 columns of the rows and of A
-// are copied asynchronously into the K-major operand layout without swizzle ([8
-// columns][8-row group][8 rows x 16 bytes], so that 8 lanes write a group's 128
-// bytes), and one elected thread issues the stage's 8 products.  The blocks'
+// are copied asynchronously into the K-major operand layout of 128-byte rows
+// whose 16-byte pieces are swizzled (piece c of row i lies at c ^ (i % 8)), so that
+// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products.  The blocks'
 // parts join as in the kernel for fewer rows.  Second product: T's parts are the
 // 128-row operand, B's 64 columns a stage the other; while a stage's products
 // run, all threads add the stage before it to y, which came with B into rows 16
@@ -22,7 +22,6 @@ namespace {
 constexpr int kStep = 128;        // columns of a stage of the first product
 constexpr int kCols = 64;         // and of the second
 constexpr int kMaxStages = 6;
-constexpr int kGroups = kTallRows / 8;
 constexpr int kTmem = 256;        // columns: T, and two accumulators of the second product from 128 on
 
 struct TallParams {
@@ -31,16 +30,23 @@ struct TallParams {
   int N, stages, stages2, all_at;  // ring sizes; where T whole lies
 };
 
+// Operands lie in blocks of 64 columns: rows of 128 bytes.
+SPEC_DEV int swizzled(int row, int piece) { return row * 128 + (piece ^ (row & 7)) * 16; }
+// Descriptor of a block: 8-row groups 1024 bytes apart, 128-byte swizzle; 16
+// columns further on are 32 bytes.
+SPEC_DEV uint64_t block_desc(uint32_t at) { return umma_desc_kmajor(at, 16, 1024) | (2ull << 61); }
+__host__ __device__ constexpr int blocks_of(int N) { return (N + 63) / 64; }
+
 template <class TY>
 __host__ __device__ constexpr int y_pitch() {
   return kCols * (int)sizeof(TY) + 16;
 }
 template <class TY>
 __host__ __device__ constexpr int stage2(int N) {
-  return kTallRows * y_pitch<TY>() + N * 2 * kCols;
+  return (kTallRows * y_pitch<TY>() + 1023) / 1024 * 1024 + blocks_of(N) * kCols * 128;
 }
-__host__ __device__ constexpr int stage1(int N) { return (kTallRows + N) * 2 * kStep; }
-__host__ __device__ constexpr int frag_bytes(int P, int N) { return P * N * 2 * kTallRows; }
+__host__ __device__ constexpr int stage1(int N) { return kStep / 64 * (kTallRows * 128 + (N * 128 + 1023) / 1024 * 1024); }
+__host__ __device__ constexpr int frag_bytes(int P, int N) { return P * blocks_of(N) * kTallRows * 128; }
 
 SPEC_DEV uint32_t idesc(int N, const __nv_bfloat16*) { return umma_idesc_bf16(128, N); }
 SPEC_DEV uint32_t idesc(int N, const __half*) { return umma_idesc_bf16(128, N) & ~((7u << 7) | (7u << 10)); }  // formats 0: f16
@@ -88,7 +94,8 @@ SPEC_DEV void pack16(uint8_t* p, const float (&x)[8], const T* tag) {
 
 template <class T, class TY>
 __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant__ TallParams tp) {
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t dynamic[];
+  uint8_t* smem = dynamic + (1024 - smem_u32(dynamic) % 1024) % 1024;  // the same in every block of the cluster
   __shared__ uint64_t s_free[kMaxStages], s_done[2];
   __shared__ uint32_t s_tmem;
   __shared__ const TY* s_row[kTallRows];
@@ -123,38 +130,36 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
   {
     const int k_per = (p.K + size * kStep - 1) / (size * kStep) * kStep, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K);
     const int width = k1 - k0, n_steps = r ? (width + kStep - 1) / kStep : 0, stages = tp.stages, sb = stage1(N);
-    const int a_lbo = N * 16;  // bytes of 8 columns of A
-    // Rows of this lane: two 8-row groups a warp.  Rows behind the last one are
+    constexpr int xb = kTallRows * 128;             // bytes of a block of x, and of A
+    const int ab = (N * 128 + 1023) / 1024 * 1024;
+    // Rows of this lane: four of the warp's 16.  Rows behind the last one are
     // copies of it, T's columns behind the adapter's rank whatever the memory
     // holds: neither is used.
-    const int row0 = warp * 16 + lane % 8, kp = lane / 8;
-    const T* x0 = static_cast<const T*>(p.x) + rows[min(row0, n_rows - 1)] * p.x_row + k0 + kp * 8;
-    const T* x1 = static_cast<const T*>(p.x) + rows[min(row0 + 8, n_rows - 1)] * p.x_row + k0 + kp * 8;
-    const T* a0 = A + (warp * 8 + lane % 8) * p.a_row + k0 + kp * 8;
+    const int row0 = warp * 16 + lane / 8, piece = lane % 8;
+    const T* x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = static_cast<const T*>(p.x) + rows[min(row0 + i * 4, n_rows - 1)] * p.x_row + k0 + piece * 8;
+    const int a_row = warp * 4 + lane / 8;
+    const T* a0 = A + a_row * p.a_row + k0 + piece * 8;
     const bool fast = p.x_wide && p.a_wide;
     int next = 0, at = 0;  // of the next stage to fetch: its first column, its offset
     auto fetch = [&]() {
-      uint8_t* xt = smem + at + kp * (kGroups * 128) + warp * 256 + lane % 8 * 16;
-      uint8_t* ta = smem + at + kTallRows * 2 * kStep + kp * a_lbo + warp * 128 + lane % 8 * 16;
       const bool whole = fast && next + kStep <= width;
 #pragma unroll
-      for (int q = 0; q < kStep / 32; ++q) {
-        const int k = next + q * 32, left = width - k - kp * 8;
-        if (whole) {
-          cp_async16(xt + q * (kGroups * 512), x0 + k);
-          cp_async16(xt + q * (kGroups * 512) + 128, x1 + k);
-        } else {
-          copy8(xt + q * (kGroups * 512), x0 + k, left, p.x_wide);
-          copy8(xt + q * (kGroups * 512) + 128, x1 + k, left, p.x_wide);
-        }
-      }
-      for (int j = warp * 8 + lane % 8, o = 0; j < r; j += kWarps * 8, ++o) {
-        const T* a = a0 + o * (kWarps * 8) * p.a_row + next;
+      for (int q = 0; q < kStep / 64; ++q) {
+        const int k = next + q * 64, left = width - k - piece * 8;
+        uint8_t* to = smem + at + q * xb;
 #pragma unroll
-        for (int q = 0; q < kStep / 32; ++q) {
-          uint8_t* to = ta + o * (kWarps * 128) + q * 4 * a_lbo;
-          if (whole) cp_async16(to, a + q * 32);
-          else copy8(to, a + q * 32, width - next - q * 32 - kp * 8, p.a_wide);
+        for (int i = 0; i < 4; ++i) {
+          if (whole) cp_async16(to + swizzled(row0 + i * 4, piece), x[i] + k);
+          else copy8(to + swizzled(row0 + i * 4, piece), x[i] + k, left, p.x_wide);
+        }
+        to = smem + at + kStep / 64 * xb + q * ab;
+        const T* a = a0 + k;
+        for (int j = a_row; j < r; j += kWarps * 4, a += kWarps * 4 * p.a_row) {
+          if (whole) cp_async16(to + swizzled(j, piece), a);
+          else copy8(to + swizzled(j, piece), a, left, p.a_wide);
         }
       }
       next += kStep;
@@ -174,11 +179,10 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
       if (!ok) break;
       if (threadIdx.x == 0) {
         tc_fence_after();
-        const uint32_t xs = base + slot * sb, as = xs + kTallRows * 2 * kStep;
+        const uint32_t xs = base + slot * sb, as = xs + kStep / 64 * xb;
 #pragma unroll 1
         for (int k = 0; k < kStep / 16; ++k)
-          umma_bf16(tmem, umma_desc_kmajor(xs + k * 2 * kGroups * 128, kGroups * 128, 128),
-                    umma_desc_kmajor(as + k * 2 * a_lbo, a_lbo, 128), id, step | k);
+          umma_bf16(tmem, block_desc(xs + k / 4 * xb + k % 4 * 32), block_desc(as + k / 4 * ab + k % 4 * 32), id, step | k);
         umma_commit(&s_free[slot]);
       }
       // The slot before this one is filled again once its products are done.
@@ -252,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
     const int e = exponent(top, A);
     const float down = pow2i(-e);
     for (int j = h * 8; j < N; j += 16) {
+      uint8_t* to = smem + j / 64 * (kTallRows * 128) + swizzled(row, j / 8 % 8);
       float v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = j + k < r ? all[row * Wp + j + k] * scale * down : 0.f;
@@ -266,8 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
           v[2 * k] = fabsf(v[2 * k]) < INFINITY ? v[2 * k] - to_float(hl[0]) : 0.f;
           v[2 * k + 1] = fabsf(v[2 * k + 1]) < INFINITY ? v[2 * k + 1] - to_float(hl[1]) : 0.f;
         }
-        *reinterpret_cast<uint4*>(smem + q * (N * 2 * kTallRows) + j / 8 * (kGroups * 128) + row / 8 * 128 + row % 8 * 16) =
-            make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(to + q * frag_bytes(1, N)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     // Row of thread 2 i is i: the factors change hands through the rows' pads.
@@ -287,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
     if (threadIdx.x < kTallRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
     __syncthreads();
     const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
-    const int quads = (N + 31) / 32, y_row = warp * 16 + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
+    constexpr int yb = (kTallRows * y_pitch<TY>() + 1023) / 1024 * 1024;  // bytes of a stage's y
+    const int y_row = warp * 16 + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
     int next = 0, at = 0;
     auto fetch = [&]() {
       const bool whole = fast && next + kCols <= width;
@@ -306,14 +311,14 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
             if (yk + e < width) reinterpret_cast<TY*>(to)[e] = from[e];
         }
       }
-      uint8_t* tb = ring + at + kTallRows * y_pitch<TY>() + lane % 8 * 16;
-      for (int i = warp; i < 8 * quads; i += kWarps) {
-        const int k8 = i / 8 * 4 + lane / 8, column = min(next + i % 8 * 8 + lane % 8, width - 1);
-        if (k8 * 8 >= N) continue;
-        const T* from = B + (n0 + column) * p.b_row + k8 * 8;
-        uint8_t* to = tb + k8 * (kCols * 16) + i % 8 * 128;
-        if (whole && k8 * 8 < r) cp_async16(to, from);
-        else copy8(to, from, r - k8 * 8, p.b_wide);
+      // B: ranks behind the adapter's are zeros, columns behind the last one copies of it.
+      for (int i = warp * 4 + lane / 8; i < blocks_of(N) * kCols; i += kWarps * 4) {
+        const int k = i / kCols * 64 + lane % 8 * 8, column = i % kCols;
+        if (k >= N) continue;
+        const T* from = B + (n0 + min(next + column, width - 1)) * p.b_row + k;
+        uint8_t* to = ring + at + yb + i / kCols * (kCols * 128) + swizzled(column, lane % 8);
+        if (whole && k < r) cp_async16(to, from);
+        else copy8(to, from, r - k, p.b_wide);
       }
       next += kCols;
       at = at + sb == stages * sb ? 0 : at + sb;
@@ -334,13 +339,13 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
       if (!ok) break;
       if (threadIdx.x == 0 && step < n_steps && r) {
         tc_fence_after();
-        const uint32_t bs = smem_u32(ring) + slot * sb + kTallRows * y_pitch<TY>(), to = tmem + 128 + step % 2 * kCols;
+        const uint32_t bs = smem_u32(ring) + slot * sb + yb, to = tmem + 128 + step % 2 * kCols;
 #pragma unroll 1
         for (int q = 0; q < P; ++q)
 #pragma unroll 1
           for (int k = 0; k < N / 16; ++k)
-            umma_bf16(to, umma_desc_kmajor(frag + q * (N * 2 * kTallRows) + k * 2 * kGroups * 128, kGroups * 128, 128),
-                      umma_desc_kmajor(bs + k * 2 * (kCols * 16), kCols * 16, 128), id, q | k);
+            umma_bf16(to, block_desc(frag + q * frag_bytes(1, N) + k / 4 * (kTallRows * 128) + k % 4 * 32),
+                      block_desc(bs + k / 4 * (kCols * 128) + k % 4 * 32), id, q | k);
         umma_commit(&s_done[step % 2]);
       }
       // The slot of two steps ago is free.
@@ -405,7 +410,7 @@ int plan_memory(TallParams* t, int N) {
   t->all_at = (whole > frag ? whole : frag) / 128 * 128 + 128;
   t->stages = kMost / stage1(N) < kMaxStages ? kMost / stage1(N) : kMaxStages;
   t->stages2 = (kMost - frag) / stage2<TY>(N) < kMaxStages ? (kMost - frag) / stage2<TY>(N) : kMaxStages;
-  return t->stages >= 2 && t->stages2 >= 3 && t->all_at + whole <= kMost ? kMost : 0;
+  return t->stages >= 2 && t->stages2 >= 3 && t->all_at + whole <= kMost ? kMost + 1024 : 0;
 }
 
 template <class T, class TY>
