@@ -19,6 +19,7 @@ namespace specb200 {
 namespace lora {
 namespace {
 
+constexpr int kTallThreads = 512, kTallWarps = kTallThreads / 32;
 constexpr int kStep = 128;        // columns of a stage of the first product
 constexpr int kCols = 64;         // and of the second
 constexpr int kMaxStages = 6;
@@ -93,7 +94,7 @@ SPEC_DEV void pack16(uint8_t* p, const float (&x)[8], const T* tag) {
 }
 
 template <class T, class TY>
-__global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant__ TallParams tp) {
+__global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_constant__ TallParams tp) {
   extern __shared__ __align__(128) uint8_t dynamic[];
   uint8_t* smem = dynamic + (1024 - smem_u32(dynamic) % 1024) % 1024;  // the same in every block of the cluster
   __shared__ uint64_t s_free[kMaxStages], s_done[2];
@@ -132,13 +133,13 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
     const int width = k1 - k0, n_steps = r ? (width + kStep - 1) / kStep : 0, stages = tp.stages, sb = stage1(N);
     constexpr int xb = kTallRows * 128;             // bytes of a block of x, and of A
     const int ab = (N * 128 + 1023) / 1024 * 1024;
-    // Rows of this lane: four of the warp's 16.  Rows behind the last one are
+    // Rows of this lane: two of the warp's 8.  Rows behind the last one are
     // copies of it, T's columns behind the adapter's rank whatever the memory
     // holds: neither is used.
-    const int row0 = warp * 16 + lane / 8, piece = lane % 8;
-    const T* x[4];
+    const int row0 = warp * 8 + lane / 8, piece = lane % 8;
+    const T* x[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
       x[i] = static_cast<const T*>(p.x) + rows[min(row0 + i * 4, n_rows - 1)] * p.x_row + k0 + piece * 8;
     const int a_row = warp * 4 + lane / 8;
     const T* a0 = A + a_row * p.a_row + k0 + piece * 8;
@@ -151,13 +152,13 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
         const int k = next + q * 64, left = width - k - piece * 8;
         uint8_t* to = smem + at + q * xb;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           if (whole) cp_async16(to + swizzled(row0 + i * 4, piece), x[i] + k);
           else copy8(to + swizzled(row0 + i * 4, piece), x[i] + k, left, p.x_wide);
         }
         to = smem + at + kStep / 64 * xb + q * ab;
         const T* a = a0 + k;
-        for (int j = a_row; j < r; j += kWarps * 4, a += kWarps * 4 * p.a_row) {
+        for (int j = a_row; j < r; j += kTallWarps * 4, a += kTallWarps * 4 * p.a_row) {
           if (whole) cp_async16(to + swizzled(j, piece), a);
           else copy8(to + swizzled(j, piece), a, left, p.a_wide);
         }
@@ -200,14 +201,14 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
     cp_async_wait<0>();
     ok = __syncthreads_and(ok);
     tc_fence_after();
-    // A warp reads 32 rows, half of the columns.
-    float* o = part + (warp % 4 * 32 + lane) * Wp + warp / 4 * (N / 2);
-    for (int c = 0; c < N / 2; c += 8) {
+    // A warp reads 32 rows, 8 columns in 32.
+    float* o = part + (warp % 4 * 32 + lane) * Wp;
+    for (int c = warp / 4 * 8; c < N; c += kTallWarps / 4 * 8) {
       uint32_t v[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
       if (n_steps) {  // else this block has no part of K
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                     : "r"(tmem + ((uint32_t)(warp % 4 * 32) << 16) + warp / 4 * (N / 2) + c)
+                     : "r"(tmem + ((uint32_t)(warp % 4 * 32) << 16) + c)
                      : "memory");
         tmem_wait_ld();
 #pragma unroll
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
   cluster_arrive();
   cluster_wait();
   const int share = (live / 4 + size - 1) / size * 4;
-  for (int i = rank * share + threadIdx.x * 4; i < min((rank + 1) * share, live); i += kThreads * 4) {
+  for (int i = rank * share + threadIdx.x * 4; i < min((rank + 1) * share, live); i += kTallThreads * 4) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int q = 0; q < size; ++q) {
       const float4 v = remote_float4(part + i, q);
@@ -236,26 +237,27 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
   }
   cluster_arrive();
   cluster_wait();
-  for (int i = threadIdx.x * 4; i < live; i += kThreads * 4)
+  for (int i = threadIdx.x * 4; i < live; i += kTallThreads * 4)
     if (i / share != rank) *reinterpret_cast<float4*>(all + i) = remote_float4(all + i, i / share);
   cluster_arrive();  // nothing of the other blocks is read any more
   __syncthreads();
-  // In part's place: the numbers that T is split into, two threads a row.  A
+  // In part's place: the numbers that T is split into, four threads a row.  A
   // thread keeps the factor of the row that it finishes.
   const int my_row = warp % 4 * 32 + lane;
   float factor;
   {
-    const int row = threadIdx.x / 2, h = threadIdx.x % 2;
+    const int row = threadIdx.x / 4, h = threadIdx.x % 4;
     const float scale = p.scales ? p.scales[u.adapter] : 1.f;
     float top = 0.f;
-    for (int j = h * 8; j < r; j += 16)
+    for (int j = h * 8; j < r; j += 32)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (j + k < r) top = fmaxf(top, fabsf(all[row * Wp + j + k] * scale));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = exponent(top, A);
     const float down = pow2i(-e);
-    for (int j = h * 8; j < N; j += 16) {
+    for (int j = h * 8; j < N; j += 32) {
       uint8_t* to = smem + j / 64 * (kTallRows * 128) + swizzled(row, j / 8 % 8);
       float v[8];
 #pragma unroll
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
         *reinterpret_cast<uint4*>(to + q * frag_bytes(1, N)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    // Row of thread 2 i is i: the factors change hands through the rows' pads.
+    // Row of thread 4 i is i: the factors change hands through the rows' pads.
     if (h == 0) all[row * Wp + N] = pow2i(e);
     __syncthreads();
     factor = all[my_row * Wp + N];
@@ -286,13 +288,13 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
   if (ok) {
     const int n_per = (p.N + size * kCols - 1) / (size * kCols) * kCols, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
     const int width = n1 - n0, n_steps = (width + kCols - 1) / kCols, stages = tp.stages2, sb = stage2<TY>(N);
-    constexpr int YP = kCols * (int)sizeof(TY) / 16, YR = 32 / YP, YN = kTallRows / kWarps / YR, E = 16 / (int)sizeof(TY);
+    constexpr int YP = kCols * (int)sizeof(TY) / 16, YR = 32 / YP, YN = kTallRows / kTallWarps / YR, E = 16 / (int)sizeof(TY);
     uint8_t* ring = smem + frag_bytes(P, N);  // `all` is not used any more
     if (threadIdx.x < kTallRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
     __syncthreads();
     const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
     constexpr int yb = (kTallRows * y_pitch<TY>() + 1023) / 1024 * 1024;  // bytes of a stage's y
-    const int y_row = warp * 16 + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
+    const int y_row = warp * (kTallRows / kTallWarps) + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
     int next = 0, at = 0;
     auto fetch = [&]() {
       const bool whole = fast && next + kCols <= width;
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
         }
       }
       // B: ranks behind the adapter's are zeros, columns behind the last one copies of it.
-      for (int i = warp * 4 + lane / 8; i < blocks_of(N) * kCols; i += kWarps * 4) {
+      for (int i = warp * 4 + lane / 8; i < blocks_of(N) * kCols; i += kTallWarps * 4) {
         const int k = i / kCols * 64 + lane % 8 * 8, column = i % kCols;
         if (k >= N) continue;
         const T* from = B + (n0 + min(next + column, width - 1)) * p.b_row + k;
@@ -357,21 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1) tall_kernel(const __grid_constant
         if (r) {
           ok = mbar_wait_bounded(&s_done[(step - 1) % 2], (step - 1) / 2 % 2, tp.err);
           tc_fence_after();
-          uint32_t v[2][16];
-          const uint32_t from = tmem + ((uint32_t)(warp % 4 * 32) << 16) + 128 + (step - 1) % 2 * kCols + warp / 4 * 32;
-          tmem_ld16(from, v[0]);
-          tmem_ld16(from + 16, v[1]);
+          uint32_t v[16];
+          tmem_ld16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + 128 + (step - 1) % 2 * kCols + warp / 4 * 16, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(v[i / 16][i % 16])::"memory");
+          for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i])::"memory");
           tc_fence_before();
-          uint8_t* y = st + my_row * y_pitch<TY>() + warp / 4 * 32 * (int)sizeof(TY);
+          uint8_t* y = st + my_row * y_pitch<TY>() + warp / 4 * 16 * (int)sizeof(TY);
 #pragma unroll
-          for (int i = 0; i < 32 / E; ++i) {
+          for (int i = 0; i < 16 / E; ++i) {
             float f[E];
             unpack16(y + i * 16, f, (const TY*)nullptr);
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = fmaf(__uint_as_float(v[(i * E + e) / 16][(i * E + e) % 16]), factor, f[e]);
+            for (int e = 0; e < E; ++e) f[e] = fmaf(__uint_as_float(v[i * E + e]), factor, f[e]);
             pack16(y + i * 16, f, (const TY*)nullptr);
           }
         }
@@ -421,7 +421,7 @@ cudaError_t run(const Params& p, unsigned* err, int n_units, int size, cudaStrea
   if (!bytes) return cudaSuccess;
   const cudaError_t e = cudaFuncSetAttribute(tall_kernel<T, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  return launch_clusters(tall_kernel<T, TY>, n_units, size, kThreads, bytes, s, t);
+  return launch_clusters(tall_kernel<T, TY>, n_units, size, kTallThreads, bytes, s, t);
 }
 
 }  // namespace
