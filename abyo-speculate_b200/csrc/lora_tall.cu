@@ -292,6 +292,12 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
     uint8_t* ring = smem + frag_bytes(P, N);  // `all` is not used any more
     if (threadIdx.x < kTallRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
     __syncthreads();
+    TY* out[YN];  // where this thread stores
+#pragma unroll
+    for (int i = 0; i < YN; ++i) {
+      const int row = warp * (kTallRows / kTallWarps) + lane / YP + i * YR;
+      out[i] = row < n_rows ? static_cast<TY*>(p.out) + rows[row] * p.out_row + n0 + lane % YP * E : nullptr;
+    }
     const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
     constexpr int yb = (kTallRows * y_pitch<TY>() + 1023) / 1024 * 1024;  // bytes of a stage's y
     const int y_row = warp * (kTallRows / kTallWarps) + lane / YP, y_at = y_row * y_pitch<TY>() + lane % YP * 16;
@@ -379,9 +385,8 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
         const bool whole = p.out_wide && n + kCols <= width;
 #pragma unroll
         for (int i = 0; i < YN; ++i) {
-          const int row = y_row + i * YR;
-          if (row >= n_rows) continue;
-          TY* o = static_cast<TY*>(p.out) + rows[row] * p.out_row + n0 + n + lane % YP * E;
+          if (!out[i]) continue;
+          TY* o = out[i] + n;
           const uint8_t* v = st + y_at + i * YR * y_pitch<TY>();
           if (whole) {
             *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(v);
