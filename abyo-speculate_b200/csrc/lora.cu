@@ -27,8 +27,58 @@ namespace {
 constexpr int kStages = 3;  // of B a warp has under way: 64 columns by 32 ranks
 constexpr int kStageBytes = 64 * 64;
 
+// The second product's 64 columns: a lane ends with its eight as two runs of four
+// (f32 results) or one of eight (16-bit ones), so that a store's 16 bytes lie next to
+// the neighbour lane's.  Column i of tile row g, and the place i * 8 + g of a column.
+template <class TY>
+SPEC_DEV int place_of(int column) {
+  return sizeof(TY) == 4 ? (column / 32 * 4 + column % 4) * 8 + column % 32 / 4 : column % 8 * 8 + column / 8;
+}
+// The first of a lane's columns, and how far its second run of four is from the first.
+template <class TY>
+SPEC_DEV int run_of(int g) {
+  return sizeof(TY) == 4 ? 4 * g : 8 * g;
+}
+template <class TY>
+constexpr int kRunStep = sizeof(TY) == 4 ? 32 : 4;
+
+template <class TY>
+SPEC_DEV void load_runs(const TY* p, int m, int n, bool wide, float (&x)[8]) {
+  load8(p, m, n, wide, x);
+}
+SPEC_DEV void load_runs(const float* p, int m, int n, bool wide, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = m + h * kRunStep<float>;
+    if (wide && k + 4 <= n) {
+      const float4 v = *reinterpret_cast<const float4*>(p + k);
+      x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * h + i] = k + i < n ? p[k + i] : 0.f;
+    }
+  }
+}
+template <class TY>
+SPEC_DEV void store_runs(TY* p, int m, int n, bool wide, const float (&x)[8]) {
+  store8(p, m, n, wide, x);
+}
+SPEC_DEV void store_runs(float* p, int m, int n, bool wide, const float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = m + h * kRunStep<float>;
+    if (wide && k + 4 <= n) {
+      *reinterpret_cast<float4*>(p + k) = make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k + i < n) p[k + i] = x[4 * h + i];
+    }
+  }
+}
+
 struct Smem {
-  uint8_t ring[kWarps][kStages][kStageBytes];  // column 8 g + j at place 8 j + g
+  uint8_t ring[kWarps][kStages][kStageBytes];  // a column's 64 bytes at its place
   float part[kWarps * kNarrowRows * 16];       // [k part x rank tile][row][16 ranks]
   float t[kNarrowRows][kMaxRank];              // this block's share of x A^T
   uint16_t frag[3][kMaxRank / 32][32 * 8];     // t's parts as the second product takes them
@@ -44,10 +94,13 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = cluster_rank(), size = cluster_size();
   pdl_launch_dependents();
-  pdl_wait();
+  // The plan is older than any kernel that this one may overlap, and what L2 holds
+  // follows later writes: B is asked for before the wait.
   const Unit& u = p.units[blockIdx.x / size];
   const int* rows = u.row;
   const int n_per = ((p.N + size * 64 - 1) / (size * 64)) * 64, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
+  if (u.adapter >= 0) prefetch_b(p, static_cast<const T*>(p.b) + u.adapter * p.b_adapter, n0, n1);
+  pdl_wait();
   if (u.adapter < 0) {  // a row without an adapter: y as it is
     const TY* y = static_cast<const TY*>(p.y) + rows[0] * p.y_row;
     TY* o = static_cast<TY*>(p.out) + rows[0] * p.out_row;
@@ -71,15 +124,17 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   int next_n = n0 + warp * 64, next_s = 0, next_slot = 0;  // the next stage to fetch
   auto fetch = [&]() {
     if (steps && next_n < n1) {
-      const int k = next_s * 32 + 8 * t, m = next_n + 8 * g;
-      uint8_t* to = sm.ring[warp][next_slot] + g * 64 + t * 16;
+      const int k = next_s * 32 + 8 * t;
+      uint8_t* to = sm.ring[warp][next_slot] + t * 16;
       if (k < r) {
+        const T* b = B + k;
         if (p.b_wide && k + 8 <= p.rank) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) cp_async16(to + j * 512, B + min(m + j, n1 - 1) * p.b_row + k);
+          for (int j = 0; j < 8; ++j) cp_async16(to + place_of<TY>(j * 8 + g) * 64, b + min(next_n + j * 8 + g, n1 - 1) * p.b_row);
         } else {
 #pragma unroll 1
-          for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(to + j * 512) = load8(B + min(m + j, n1 - 1) * p.b_row, k, r, false);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(to + place_of<TY>(j * 8 + g) * 64) = load8(B + min(next_n + j * 8 + g, n1 - 1) * p.b_row, k, r, false);
         }
       }
       next_slot = next_slot + 1 == kStages ? 0 : next_slot + 1;
@@ -177,9 +232,7 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   }
   __syncthreads();
 
-  // Y^T += B T^T over this block's columns, 64 a warp and step: row g of
-  // tile j's halves is column 8 g + 2 j, + 1, so that a lane ends with 8
-  // columns of its two rows behind one another.
+  // Y^T += B T^T over this block's columns, 64 a warp and step.
   const int ra = 2 * t, rb = 2 * t + 1;
   const bool has_a = ra < u.n_rows, has_b = rb < u.n_rows;
   const float fa = sm.factor[ra], fb = sm.factor[rb];
@@ -191,13 +244,13 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   int slot = 0;
   float ya[8], yb[8];  // of the next 64 columns
   auto load_y = [&](int m) {
-    if (has_a && m < n1) load8(py[0], m, n1, p.y_wide, ya);
-    if (has_b && m < n1) load8(py[1], m, n1, p.y_wide, yb);
+    if (has_a && m < n1) load_runs(py[0], m, n1, p.y_wide, ya);
+    if (has_b && m < n1) load_runs(py[1], m, n1, p.y_wide, yb);
   };
-  load_y(n0 + warp * 64 + 8 * g);
+  load_y(n0 + warp * 64 + run_of<TY>(g));
 #pragma unroll 1
   for (int n = n0 + warp * 64; n < n1; n += kWarps * 64) {
-    const int m = n + 8 * g;
+    const int m = n + run_of<TY>(g);
     float d[4][4] = {};
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
@@ -206,16 +259,19 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
       uint4 f[P];
 #pragma unroll
       for (int q = 0; q < P; ++q) f[q] = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
+      uint4 v[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint8_t* at = sm.ring[warp][slot] + j * 1024 + g * 64 + t * 16;
-        uint4 v = *reinterpret_cast<const uint4*>(at), w = *reinterpret_cast<const uint4*>(at + 512);
-        if (cut) v = first_of(v, r - s * 32 - 8 * t), w = first_of(w, r - s * 32 - 8 * t);
+      for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint4*>(sm.ring[warp][slot] + (j * 8 + g) * 64 + t * 16);
+      if (cut) {
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-          mma16(d[j], v.x, w.x, v.y, w.y, f[q].x, f[q].y, A);
-          mma16(d[j], v.z, w.z, v.w, w.w, f[q].z, f[q].w, A);
-        }
+        for (int j = 0; j < 8; ++j) v[j] = first_of(v[j], r - s * 32 - 8 * t);
+      }
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma16(d[j], v[2 * j].x, v[2 * j + 1].x, v[2 * j].y, v[2 * j + 1].y, f[q].x, f[q].y, A);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma16(d[j], v[2 * j].z, v[2 * j + 1].z, v[2 * j].w, v[2 * j + 1].w, f[q].z, f[q].w, A);
       }
       slot = slot + 1 == kStages ? 0 : slot + 1;
       __syncwarp();
@@ -231,8 +287,8 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
     load_y(m + kWarps * 64);
     const float oa[8] = {d[0][0], d[0][2], d[1][0], d[1][2], d[2][0], d[2][2], d[3][0], d[3][2]};
     const float ob[8] = {d[0][1], d[0][3], d[1][1], d[1][3], d[2][1], d[2][3], d[3][1], d[3][3]};
-    if (has_a) store8(po[0], m, n1, p.out_wide, oa);
-    if (has_b) store8(po[1], m, n1, p.out_wide, ob);
+    if (has_a) store_runs(po[0], m, n1, p.out_wide, oa);
+    if (has_b) store_runs(po[1], m, n1, p.out_wide, ob);
   }
   cp_async_wait<0>();
   cluster_wait();

@@ -48,6 +48,23 @@ SPEC_DEV void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
+// Asks for `n` elements from `p` on to be brought to L2 (whole 16-byte pieces of
+// them, up to 64 KB).
+template <class E>
+SPEC_DEV void prefetch(const E* p, long long n) {
+  const uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) / 16 * 16, e = reinterpret_cast<uintptr_t>(p + n) / 16 * 16;
+  if (e > a) tma_prefetch_l2(reinterpret_cast<const void*>(a), (uint32_t)(e - a < 65536 ? e - a : 65536));
+}
+// The same of rows n0 .. n1 - 1 of B, in pieces of 32 KB a thread, where all of a
+// row is wanted or the row is no longer than the memory's 64 bytes.
+template <class T>
+SPEC_DEV void prefetch_b(const Params& p, const T* B, int n0, int n1) {
+  if (p.ranks && p.b_row > 32) return;
+  if (p.b_row > 2 * p.rank || !p.rank) return;
+  const long long begin = n0 * p.b_row, end = n1 * p.b_row - (p.b_row - p.rank), piece = 32768 / (int)sizeof(T);
+  for (long long at = begin + threadIdx.x * piece; at < end; at += blockDim.x * piece) prefetch(B + at, end - at < piece ? end - at : piece);
+}
+
 SPEC_DEV void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                     const __half*) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

@@ -9,8 +9,8 @@
 // a slice of T and all of them collecting the slices.  Second product, Y += T
 // B^T: the blocks share N, the warps rows and columns, 32 of each; y and B come
 // through the warps' rings, T's parts are the 16-row operand, and B's columns are
-// taken in an order that leaves a lane with 8 columns of its rows behind one
-// another.
+// taken in an order that leaves a lane with 16 bytes of its rows next to its
+// neighbour's.
 //
 // Pieces lie as [row][64 bytes], areas 64 bytes further apart than they are long, so
 // that neither the copies (16 bytes a lane along a row) nor the operands' loads
@@ -74,6 +74,16 @@ SPEC_DEV int piece_at(int c) {
   return sizeof(E) == 4 ? c % 2 * kArea + c / 2 * 16 : c / 4 * kArea + c % 4 * 16;
 }
 
+SPEC_DEV void store4(float* p, int k, int n, bool wide, const float (&x)[4]) {
+  if (wide && k + 4 <= n) {
+    *reinterpret_cast<float4*>(p + k) = make_float4(x[0], x[1], x[2], x[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k + i < n) p[k + i] = x[i];
+}
+
 template <class T, class TX, class TY, int NT>
 __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant__ WideParams wp) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -85,10 +95,15 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = cluster_rank(), size = cluster_size(), RA = wp.RA;
   pdl_launch_dependents();
-  pdl_wait();
+  // The plan is older than any kernel that this one may overlap, and what L2 holds
+  // follows later writes: B is asked for before the wait, y behind it.
   const Unit& u = p.units[blockIdx.x / size];
   const int* rows = p.order + u.first;
   const int n_rows = u.n_rows;
+  const int n_per = (p.N + size * 32 - 1) / (size * 32) * 32, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N), width = n1 - n0;
+  prefetch_b(p, static_cast<const T*>(p.b) + u.adapter * p.b_adapter, n0, n1);
+  pdl_wait();
+  if (threadIdx.x < n_rows) prefetch(static_cast<const TY*>(p.y) + rows[threadIdx.x] * p.y_row + n0, width);
   const int r = p.ranks ? min(max(p.ranks[u.adapter], 0), p.rank) : p.rank;
   const T* A = static_cast<const T*>(p.a) + u.adapter * p.a_adapter;
   const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
@@ -102,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   {
     constexpr int C = 128 / (int)sizeof(TX), S = C / 32;  // columns of a piece of work; slices of 32 in it
     constexpr int kSlot = 2 * kArea + S * area(8 * NT);
-    const int k_per = (p.K + size * C - 1) / (size * C) * C, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K), width = k1 - k0;
+    const int k_per = (p.K + size * C - 1) / (size * C) * C, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K), length = k1 - k0;
     if (threadIdx.x < kWideRows)
       s_row[threadIdx.x] = static_cast<const TX*>(p.x) + rows[min((int)threadIdx.x, n_rows - 1)] * p.x_row + k0;
     __syncthreads();
@@ -115,14 +130,14 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     uint8_t* ring = smem + warp * wp.ring;
     const int slots = min(wp.ring / kSlot, kMaxSlots);
     const bool fast = p.x_wide && p.a_wide;
-    int next = kg < turns && r ? kg * C : width, at = 0;  // the next to fetch: its first column, its slot
+    int next = kg < turns && r ? kg * C : length, at = 0;  // the next to fetch: its first column, its slot
     auto fetch = [&]() {
-      if (next < width) {
+      if (next < length) {
         uint8_t* to = ring + at + piece_at<TX>(lane % 8) + lane / 8 * 64;
         const int xk = next + lane % 8 * (16 / (int)sizeof(TX));
         uint8_t* ta = ring + at + 2 * kArea + lane % AP / 4 * area(8 * NT) + lane % 4 * 16 + lane / AP * 64;
         const T* a = ap + next;
-        if (fast && next + C <= width) {
+        if (fast && next + C <= length) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) cp_async16(to + i * 256, xp[i * 4] + xk);
 #pragma unroll
@@ -130,10 +145,10 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
             if (lane / AP + i * AR < ranks) cp_async16(ta + i * AR * 64, a + i * AR * p.a_row);
         } else {
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) copy16(to + i * 256, xp[i * 4] + xk, width - xk, p.x_wide);
+          for (int i = 0; i < 8; ++i) copy16(to + i * 256, xp[i * 4] + xk, length - xk, p.x_wide);
 #pragma unroll 1
           for (int i = 0; i < NT * 8 / AR; ++i)
-            if (lane / AP + i * AR < ranks) copy16(ta + i * AR * 64, a + i * AR * p.a_row, width - next - lane % AP * 8, p.a_wide);
+            if (lane / AP + i * AR < ranks) copy16(ta + i * AR * 64, a + i * AR * p.a_row, length - next - lane % AP * 8, p.a_wide);
         }
         next += turns * C;
         at = at + kSlot == slots * kSlot ? 0 : at + kSlot;
@@ -143,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     for (int i = 0; i < slots - 1; ++i) fetch();
     const uint8_t* st = ring;
 #pragma unroll 1
-    for (int k = kg < turns && r ? kg * C : width; k < width; k += turns * C) {
+    for (int k = kg < turns && r ? kg * C : length; k < length; k += turns * C) {
       cp_async_wait_for(slots - 2);
       __syncwarp();
       fetch();
@@ -289,7 +304,6 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 
   // ---- Y ----
   {
-    const int n_per = (p.N + size * 32 - 1) / (size * 32) * 32, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N), width = n1 - n0;
     if (threadIdx.x < kWideRows)
       s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
     __syncthreads();
@@ -342,6 +356,11 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
       op[i] = row < n_rows ? static_cast<TY*>(p.out) + rows[row] * p.out_row : nullptr;
       factor[i] = row < n_rows ? s_factor[row] : 0.f;
     }
+    // Column of tile j that this lane's B operand is, so that its results are columns
+    // 8 t .. (16-bit), or 4 t .. and 16 + 4 t .. (f32).
+    auto column_of = [&](int j) {
+      return sizeof(TY) == 4 ? j / 2 * 16 + g / 2 * 4 + j % 2 * 2 + g % 2 : g / 2 * 8 + j * 2 + g % 2;
+    };
     const uint8_t* st = ring;
 #pragma unroll 1
     for (int n = ng < ways ? ng * 32 : width; n < width; n += ways * 32) {
@@ -349,14 +368,14 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
       __syncwarp();
       fetch();
       float d2[2][4][4] = {};
-      const uint8_t* bb = st + YA + (g / 2 * 8 + g % 2) * 64 + t * 16;
+      const uint8_t* bb = st + YA + column_of(0) * 64 + t * 16;
 #pragma unroll 1
       for (int s = 0; s < steps; ++s, bb += kArea) {
         uint4 b[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          b[j] = ring_steps ? lds128(bb + j * 128)
-                            : load_ranks(B + (n0 + min(n + g / 2 * 8 + g % 2 + 2 * j, width - 1)) * p.b_row, s * 32 + 8 * t, r, p.rank, p.b_wide);
+          b[j] = ring_steps ? lds128(bb + (column_of(j) - column_of(0)) * 64)
+                            : load_ranks(B + (n0 + min(n + column_of(j), width - 1)) * p.b_row, s * 32 + 8 * t, r, p.rank, p.b_wide);
 #pragma unroll
         for (int q = 0; q < P; ++q) {
           const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + t * 16;
@@ -374,19 +393,26 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
       for (int i = 0; i < 4; ++i) {
         if (!op[i]) continue;
         float y[8];
-        const uint8_t* yb = st + (g + i * 8) * 64 + t * 16;
         if constexpr (sizeof(TY) == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(yb), w = *reinterpret_cast<const float4*>(yb + kArea);
+          // Pieces t and 4 + t of the row.
+          const float4 v = *reinterpret_cast<const float4*>(st + (g + i * 8) * 64 + piece_at<float>(t));
+          const float4 w = *reinterpret_cast<const float4*>(st + (g + i * 8) * 64 + piece_at<float>(4 + t));
           y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w, y[4] = w.x, y[5] = w.y, y[6] = w.z, y[7] = w.w;
         } else {
-          widen(lds128(yb), y, A);
+          widen(lds128(st + (g + i * 8) * 64 + t * 16), y, A);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           y[2 * j] = fmaf(d2[i / 2][j][i % 2 * 2], factor[i], y[2 * j]);
           y[2 * j + 1] = fmaf(d2[i / 2][j][i % 2 * 2 + 1], factor[i], y[2 * j + 1]);
         }
-        store8(op[i], n0 + n + 8 * t, n1, p.out_wide, y);
+        if constexpr (sizeof(TY) == 4) {
+          const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+          store4(op[i], n0 + n + 4 * t, n1, p.out_wide, lo);
+          store4(op[i], n0 + n + 16 + 4 * t, n1, p.out_wide, hi);
+        } else {
+          store8(op[i], n0 + n + 8 * t, n1, p.out_wide, y);
+        }
       }
       __syncwarp();
       st = st + slot == ring + slots * slot ? ring : st + slot;
