@@ -225,7 +225,7 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, cluster_for(wide, 2, sms), sms, s);
   p.units = units + plan->n_tall + plan->n_big + plan->n_wide;
   const int n = plan->n_narrow + (in_place ? 0 : plan->n_bare);
-  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 2, sms), s);
+  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 3, sms), s);
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
 }
 

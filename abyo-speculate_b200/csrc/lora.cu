@@ -24,69 +24,55 @@ namespace specb200 {
 namespace lora {
 namespace {
 
-constexpr int kStages = 3;  // of B a warp has under way: 64 columns by 32 ranks
-constexpr int kStageBytes = 64 * 64;
+constexpr int kStages = 4;   // of B a warp has under way
+constexpr int kColumns = 32;  // of a stage, by 32 ranks
+constexpr int kStageBytes = kColumns * 64;
 
-// The second product's 64 columns: a lane ends with its eight as two runs of four
-// (f32 results) or one of eight (16-bit ones), so that a store's 16 bytes lie next to
-// the neighbour lane's.  Column i of tile row g, and the place i * 8 + g of a column.
-template <class TY>
-SPEC_DEV int place_of(int column) {
-  return sizeof(TY) == 4 ? (column / 32 * 4 + column % 4) * 8 + column % 32 / 4 : column % 8 * 8 + column / 8;
-}
-// The first of a lane's columns, and how far its second run of four is from the first.
-template <class TY>
-SPEC_DEV int run_of(int g) {
-  return sizeof(TY) == 4 ? 4 * g : 8 * g;
-}
-template <class TY>
-constexpr int kRunStep = sizeof(TY) == 4 ? 32 : 4;
+// A lane ends with four columns of its rows behind one another, 4 g + i; in a stage,
+// column c lies where tile c % 4 / 2 of the product takes it.
+SPEC_DEV int place_of(int c) { return c % 4 * 8 + c / 4; }
 
 template <class TY>
-SPEC_DEV void load_runs(const TY* p, int m, int n, bool wide, float (&x)[8]) {
-  load8(p, m, n, wide, x);
-}
-SPEC_DEV void load_runs(const float* p, int m, int n, bool wide, float (&x)[8]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int k = m + h * kRunStep<float>;
-    if (wide && k + 4 <= n) {
+SPEC_DEV void load4(const TY* p, int k, int n, bool wide, float (&x)[4]) {
+  if (wide && k + 4 <= n) {
+    if constexpr (sizeof(TY) == 4) {
       const float4 v = *reinterpret_cast<const float4*>(p + k);
-      x[4 * h] = v.x, x[4 * h + 1] = v.y, x[4 * h + 2] = v.z, x[4 * h + 3] = v.w;
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p + k);
+      const TY* e = reinterpret_cast<const TY*>(&v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = k + i < n ? p[k + i] : 0.f;
+      for (int i = 0; i < 4; ++i) x[i] = to_float(e[i]);
     }
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = k + i < n ? to_float(p[k + i]) : 0.f;
 }
 template <class TY>
-SPEC_DEV void store_runs(TY* p, int m, int n, bool wide, const float (&x)[8]) {
-  store8(p, m, n, wide, x);
-}
-SPEC_DEV void store_runs(float* p, int m, int n, bool wide, const float (&x)[8]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int k = m + h * kRunStep<float>;
-    if (wide && k + 4 <= n) {
-      *reinterpret_cast<float4*>(p + k) = make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (k + i < n) p[k + i] = x[4 * h + i];
-    }
+SPEC_DEV void store4(TY* p, int k, int n, bool wide, const float (&x)[4]) {
+  if (wide && k + 4 <= n) {
+    if constexpr (sizeof(TY) == 4) *reinterpret_cast<float4*>(p + k) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<uint2*>(p + k) = make_uint2(pack2(x[0], x[1], p), pack2(x[2], x[3], p));
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k + i < n) from_float(x[i], p + k + i);
 }
 
 struct Smem {
-  uint8_t ring[kWarps][kStages][kStageBytes];  // a column's 64 bytes at its place
-  float part[kWarps * kNarrowRows * 16];       // [k part x rank tile][row][16 ranks]
-  float t[kNarrowRows][kMaxRank];              // this block's share of x A^T
-  uint16_t frag[3][kMaxRank / 32][32 * 8];     // t's parts as the second product takes them
+  uint8_t ring[kWarps][kStages][kStageBytes];
+  union {
+    float part[kWarps * kNarrowRows * 16];      // [k part x rank tile][row][16 ranks]
+    uint16_t frag[3][kMaxRank / 32][32 * 8];    // then t's parts as the second product takes them
+  };
+  float t[kNarrowRows][kMaxRank];               // this block's share of x A^T
   float factor[kNarrowRows];
 };
 
 template <class T, class TX, class TY>
-__global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   Smem& sm = *reinterpret_cast<Smem*>(smem);
   constexpr bool kSplitX = sizeof(TX) == 4;
@@ -98,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   // follows later writes: B is asked for before the wait.
   const Unit& u = p.units[blockIdx.x / size];
   const int* rows = u.row;
-  const int n_per = ((p.N + size * 64 - 1) / (size * 64)) * 64, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
+  const int n_per = (p.N + size * kColumns - 1) / (size * kColumns) * kColumns, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
   if (u.adapter >= 0) prefetch_b(p, static_cast<const T*>(p.b) + u.adapter * p.b_adapter, n0, n1);
   pdl_wait();
   if (u.adapter < 0) {  // a row without an adapter: y as it is
@@ -118,10 +104,10 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
   const int tiles = (r + 15) / 16, kparts = tiles ? max(kWarps / tiles, 1) : 1;
 
-  // The stream of B's stages of this warp: chunks of 64 columns, in each the ranks
+  // The stream of B's stages of this warp: chunks of 32 columns, in each the ranks
   // by 32.  It starts before x A^T is known.
   const int steps = (r + 31) / 32;
-  int next_n = n0 + warp * 64, next_s = 0, next_slot = 0;  // the next stage to fetch
+  int next_n = n0 + warp * kColumns, next_s = 0, next_slot = 0;  // the next stage to fetch
   auto fetch = [&]() {
     if (steps && next_n < n1) {
       const int k = next_s * 32 + 8 * t;
@@ -130,15 +116,15 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
         const T* b = B + k;
         if (p.b_wide && k + 8 <= p.rank) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) cp_async16(to + place_of<TY>(j * 8 + g) * 64, b + min(next_n + j * 8 + g, n1 - 1) * p.b_row);
+          for (int j = 0; j < kColumns / 8; ++j) cp_async16(to + place_of(j * 8 + g) * 64, b + min(next_n + j * 8 + g, n1 - 1) * p.b_row);
         } else {
 #pragma unroll 1
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(to + place_of<TY>(j * 8 + g) * 64) = load8(B + min(next_n + j * 8 + g, n1 - 1) * p.b_row, k, r, false);
+          for (int j = 0; j < kColumns / 8; ++j)
+            *reinterpret_cast<uint4*>(to + place_of(j * 8 + g) * 64) = load8(B + min(next_n + j * 8 + g, n1 - 1) * p.b_row, k, r, false);
         }
       }
       next_slot = next_slot + 1 == kStages ? 0 : next_slot + 1;
-      if (++next_s == steps) next_s = 0, next_n += kWarps * 64;
+      if (++next_s == steps) next_s = 0, next_n += kWarps * kColumns;
     }
     cp_async_commit();
   };
@@ -232,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
   }
   __syncthreads();
 
-  // Y^T += B T^T over this block's columns, 64 a warp and step.
+  // Y^T += B T^T over this block's columns, 32 a warp and step.
   const int ra = 2 * t, rb = 2 * t + 1;
   const bool has_a = ra < u.n_rows, has_b = rb < u.n_rows;
   const float fa = sm.factor[ra], fb = sm.factor[rb];
@@ -242,53 +228,44 @@ __global__ void __launch_bounds__(kThreads, 2) narrow_kernel(const __grid_consta
                static_cast<TY*>(p.out) + (has_b ? rows[rb] : 0) * p.out_row};
   const bool cut = r % 32 != 0;  // what lies behind the rank is cut off
   int slot = 0;
-  float ya[8], yb[8];  // of the next 64 columns
+  float ya[4], yb[4];  // of the next columns
   auto load_y = [&](int m) {
-    if (has_a && m < n1) load_runs(py[0], m, n1, p.y_wide, ya);
-    if (has_b && m < n1) load_runs(py[1], m, n1, p.y_wide, yb);
+    if (has_a && m < n1) load4(py[0], m, n1, p.y_wide, ya);
+    if (has_b && m < n1) load4(py[1], m, n1, p.y_wide, yb);
   };
-  load_y(n0 + warp * 64 + run_of<TY>(g));
+  load_y(n0 + warp * kColumns + 4 * g);
 #pragma unroll 1
-  for (int n = n0 + warp * 64; n < n1; n += kWarps * 64) {
-    const int m = n + run_of<TY>(g);
-    float d[4][4] = {};
+  for (int n = n0 + warp * kColumns; n < n1; n += kWarps * kColumns) {
+    const int m = n + 4 * g;
+    float d[2][4] = {};
 #pragma unroll 1
     for (int s = 0; s < steps; ++s) {
       cp_async_wait<kStages - 2>();
       __syncwarp();
-      uint4 f[P];
+      uint4 v[4];
 #pragma unroll
-      for (int q = 0; q < P; ++q) f[q] = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
-      uint4 v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint4*>(sm.ring[warp][slot] + (j * 8 + g) * 64 + t * 16);
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(sm.ring[warp][slot] + (j * 8 + g) * 64 + t * 16);
       if (cut) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = first_of(v[j], r - s * 32 - 8 * t);
+        for (int j = 0; j < 4; ++j) v[j] = first_of(v[j], r - s * 32 - 8 * t);
       }
 #pragma unroll
       for (int q = 0; q < P; ++q) {
+        const uint4 f = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma16(d[j], v[2 * j].x, v[2 * j + 1].x, v[2 * j].y, v[2 * j + 1].y, f[q].x, f[q].y, A);
+        for (int j = 0; j < 2; ++j) mma16(d[j], v[2 * j].x, v[2 * j + 1].x, v[2 * j].y, v[2 * j + 1].y, f.x, f.y, A);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma16(d[j], v[2 * j].z, v[2 * j + 1].z, v[2 * j].w, v[2 * j + 1].w, f[q].z, f[q].w, A);
+        for (int j = 0; j < 2; ++j) mma16(d[j], v[2 * j].z, v[2 * j + 1].z, v[2 * j].w, v[2 * j + 1].w, f.z, f.w, A);
       }
       slot = slot + 1 == kStages ? 0 : slot + 1;
       __syncwarp();
       fetch();
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      d[j][0] = fmaf(d[j][0], fa, ya[2 * j]);
-      d[j][2] = fmaf(d[j][2], fa, ya[2 * j + 1]);
-      d[j][1] = fmaf(d[j][1], fb, yb[2 * j]);
-      d[j][3] = fmaf(d[j][3], fb, yb[2 * j + 1]);
-    }
-    load_y(m + kWarps * 64);
-    const float oa[8] = {d[0][0], d[0][2], d[1][0], d[1][2], d[2][0], d[2][2], d[3][0], d[3][2]};
-    const float ob[8] = {d[0][1], d[0][3], d[1][1], d[1][3], d[2][1], d[2][3], d[3][1], d[3][3]};
-    if (has_a) store_runs(po[0], m, n1, p.out_wide, oa);
-    if (has_b) store_runs(po[1], m, n1, p.out_wide, ob);
+    const float oa[4] = {fmaf(d[0][0], fa, ya[0]), fmaf(d[0][2], fa, ya[1]), fmaf(d[1][0], fa, ya[2]), fmaf(d[1][2], fa, ya[3])};
+    const float ob[4] = {fmaf(d[0][1], fb, yb[0]), fmaf(d[0][3], fb, yb[1]), fmaf(d[1][1], fb, yb[2]), fmaf(d[1][3], fb, yb[3])};
+    load_y(m + kWarps * kColumns);
+    if (has_a) store4(po[0], m, n1, p.out_wide, oa);
+    if (has_b) store4(po[1], m, n1, p.out_wide, ob);
   }
   cp_async_wait<0>();
   cluster_wait();
