@@ -74,14 +74,27 @@ SPEC_DEV int piece_at(int c) {
   return sizeof(E) == 4 ? c % 2 * kArea + c / 2 * 16 : c / 4 * kArea + c % 4 * 16;
 }
 
-SPEC_DEV void store4(float* p, int k, int n, bool wide, const float (&x)[4]) {
-  if (wide && k + 4 <= n) {
-    *reinterpret_cast<float4*>(p + k) = make_float4(x[0], x[1], x[2], x[3]);
-    return;
-  }
+// 16 bytes of a row from element k on, of n; what lies behind them is left.
+template <class E>
+SPEC_DEV uint4 load_piece(const E* p, int k, int n) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (k + i < n) p[k + i] = x[i];
+  for (int i = 0; i < 16 / (int)sizeof(E); ++i)
+    if (k + i < n) {
+      if constexpr (sizeof(E) == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[k + i];
+      else w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[k + i] << (i % 2 * 16);
+    }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class E>
+SPEC_DEV void store_piece(E* p, int k, int n, const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(E); ++i)
+    if (k + i < n) {
+      if constexpr (sizeof(E) == 4) reinterpret_cast<uint32_t*>(p)[k + i] = w[i];
+      else reinterpret_cast<uint16_t*>(p)[k + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
+    }
 }
 
 template <class T, class TX, class TY, int NT>
@@ -304,120 +317,129 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 
   // ---- Y ----
   {
-    if (threadIdx.x < kWideRows)
-      s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
-    __syncthreads();
-    constexpr int YP = 32 * (int)sizeof(TY) / 16, YR = 32 / YP, YA = (int)sizeof(TY) / 2 * kArea;  // pieces a row; rows a pass; bytes
-    const TY* const* yp = reinterpret_cast<const TY* const*>(s_row) + mg * 32 + lane / YP;
-    const int ways = kWarps / groups, ng = warp / groups, ring_steps = steps <= 2 ? steps : 0, slot = YA + ring_steps * kArea;
-    uint8_t* base = smem + (P * steps * frag + 127) / 128 * 128;
-    const int room = (wp.bytes - (int)(base - smem)) / kWarps / 16 * 16, slots = min(room / slot, kMaxSlots);
-    uint8_t* ring = base + warp * room;
-    const bool fast = p.y_wide && p.b_wide && r % 8 == 0;
-    int next = ng < ways ? ng * 32 : width, at = 0;
-    auto fetch = [&]() {
-      if (next < width) {
-        const bool whole = fast && next + 32 <= width;
-        uint8_t* to = ring + at + piece_at<TY>(lane % YP) + lane / YP * 64;
-        const int yk = next + lane % YP * (16 / (int)sizeof(TY));
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 32 / YR; ++i) cp_async16(to + i * YR * 64, yp[i * YR] + yk);
-        } else {
-#pragma unroll 1
-          for (int i = 0; i < 32 / YR; ++i) copy16(to + i * YR * 64, yp[i * YR] + yk, width - yk, p.y_wide);
-        }
-        // B, up to 64 ranks: those behind the adapter's are zeros, columns behind the last one copies of it.
-        uint8_t* tb = ring + at + YA + lane / 4 * 64 + t * 16;
-#pragma unroll 1
-        for (int s = 0; s < ring_steps; ++s, tb += kArea) {
-          const int k = s * 32 + t * 8;
-          const T* b = B + n0 * p.b_row + k;
-          if (whole && k < r) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) cp_async16(tb + i * 512, b + (next + g + i * 8) * p.b_row);
-          } else {
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) copy16(tb + i * 512, b + min(next + g + i * 8, width - 1) * p.b_row, r - k, p.b_wide);
-          }
-        }
-        next += ways * 32;
-        at = at + slot == slots * slot ? 0 : at + slot;
-      }
-      cp_async_commit();
-    };
-    for (int i = 0; i < slots - 1; ++i) fetch();
-    const int first = mg * 32 + g;
+    constexpr int V = (int)sizeof(TY) / 2;  // 16-byte pieces of 8 columns
+    const int ways = kWarps / groups, ng = warp / groups, first = mg * 32 + g;
+    const bool half = r <= 16, cut = r % (half ? 4 : 8) != 0, b_fast = p.b_wide && p.rank % 8 == 0;
+    const int per = half ? 4 : 8;  // ranks a lane takes of a step
+    const TY* yp[4];
     TY* op[4];
     float factor[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = first + i * 8;
-      op[i] = row < n_rows ? static_cast<TY*>(p.out) + rows[row] * p.out_row : nullptr;
-      factor[i] = row < n_rows ? s_factor[row] : 0.f;
+      const int row = first + i * 8, at = rows[min(row, n_rows - 1)];
+      yp[i] = static_cast<const TY*>(p.y) + at * p.y_row + n0;
+      op[i] = row < n_rows ? static_cast<TY*>(p.out) + at * p.out_row + n0 : nullptr;
+      factor[i] = s_factor[row];
     }
-    // Column of tile j that this lane's B operand is, so that its results are columns
-    // 8 t .. (16-bit), or 4 t .. and 16 + 4 t .. (f32).
+    // Where a lane's 8 columns of a row lie: 8 t .. (16-bit), or 4 t .. and 16 + 4 t .. (f32);
+    // and so the column of B that is its operand of tile j.
     auto column_of = [&](int j) {
       return sizeof(TY) == 4 ? j / 2 * 16 + g / 2 * 4 + j % 2 * 2 + g % 2 : g / 2 * 8 + j * 2 + g % 2;
     };
-    const uint8_t* st = ring;
-#pragma unroll 1
-    for (int n = ng < ways ? ng * 32 : width; n < width; n += ways * 32) {
-      cp_async_wait_for(slots - 2);
-      __syncwarp();
-      fetch();
-      float d2[2][4][4] = {};
-      const uint8_t* bb = st + YA + column_of(0) * 64 + t * 16;
-#pragma unroll 1
-      for (int s = 0; s < steps; ++s, bb += kArea) {
-        uint4 b[4];
+    uint4 y[4][V], b[4];  // of the next tile of 32 columns, of the next 32 ranks of it
+    auto load_y = [&](int n) {
+      if (n >= width) return;
+      if (p.y_wide && n + 32 <= width) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          b[j] = ring_steps ? lds128(bb + (column_of(j) - column_of(0)) * 64)
-                            : load_ranks(B + (n0 + min(n + column_of(j), width - 1)) * p.b_row, s * 32 + 8 * t, r, p.rank, p.b_wide);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-          const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + t * 16;
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const uint4 x0 = lds128(f + m * 1024), x1 = lds128(f + m * 1024 + 512);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma16(d2[m][j], x0.x, x1.x, x0.y, x1.y, b[j].x, b[j].y, A);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma16(d2[m][j], x0.z, x1.z, x0.w, x1.w, b[j].z, b[j].w, A);
-          }
-        }
+          for (int v = 0; v < V; ++v)
+            if (op[i]) y[i][v] = *reinterpret_cast<const uint4*>(yp[i] + n + (V == 2 ? 16 * v + 4 * t : 8 * t));
+        return;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!op[i]) continue;
-        float y[8];
-        if constexpr (sizeof(TY) == 4) {
-          // Pieces t and 4 + t of the row.
-          const float4 v = *reinterpret_cast<const float4*>(st + (g + i * 8) * 64 + piece_at<float>(t));
-          const float4 w = *reinterpret_cast<const float4*>(st + (g + i * 8) * 64 + piece_at<float>(4 + t));
-          y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w, y[4] = w.x, y[5] = w.y, y[6] = w.z, y[7] = w.w;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (op[i]) y[i][v] = load_piece(yp[i], n + (V == 2 ? 16 * v + 4 * t : 8 * t), width);
+    };
+    auto load_b = [&](int n, int s) {
+      const int k = s * 32 + per * t;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        b[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (k >= r || n >= width) continue;
+        const T* q = B + (n0 + min(n + column_of(j), width - 1)) * p.b_row;
+        if (!b_fast) {
+          b[j] = load8(q, k, min(r, k + per), false);
+        } else if (half) {
+          const uint2 w = *reinterpret_cast<const uint2*>(q + k);
+          b[j].x = w.x, b[j].y = w.y;
         } else {
-          widen(lds128(st + (g + i * 8) * 64 + t * 16), y, A);
+          b[j] = *reinterpret_cast<const uint4*>(q + k);
+        }
+      }
+    };
+    const int begin = ng < ways ? ng * 32 : width;
+    load_b(begin, 0);
+    load_y(begin);
+#pragma unroll 1
+    for (int n = begin; n < width; n += ways * 32) {
+      float d2[2][4][4] = {};
+#pragma unroll 1
+      for (int s = 0; s < steps; ++s) {
+        if (cut) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = first_of(b[j], r - s * 32 - per * t);
+        }
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + per * 2 * t;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            if (half) {
+              const uint2 x0 = *reinterpret_cast<const uint2*>(f + m * 1024), x1 = *reinterpret_cast<const uint2*>(f + m * 1024 + 512);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma16(d2[m][j], x0.x, x1.x, x0.y, x1.y, b[j].x, b[j].y, A);
+            } else {
+              const uint4 x0 = lds128(f + m * 1024), x1 = lds128(f + m * 1024 + 512);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma16(d2[m][j], x0.x, x1.x, x0.y, x1.y, b[j].x, b[j].y, A);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma16(d2[m][j], x0.z, x1.z, x0.w, x1.w, b[j].z, b[j].w, A);
+            }
+          }
+        }
+        if (s + 1 < steps) load_b(n, s + 1);
+        else load_b(n + ways * 32, 0);
+      }
+      const bool whole = p.out_wide && n + 32 <= width;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[8];
+        if constexpr (sizeof(TY) == 4) {
+#pragma unroll
+          for (int h = 0; h < V; ++h) {
+            v[4 * h] = __uint_as_float(y[i][h].x), v[4 * h + 1] = __uint_as_float(y[i][h].y);
+            v[4 * h + 2] = __uint_as_float(y[i][h].z), v[4 * h + 3] = __uint_as_float(y[i][h].w);
+          }
+        } else {
+          widen(y[i][0], v, A);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          y[2 * j] = fmaf(d2[i / 2][j][i % 2 * 2], factor[i], y[2 * j]);
-          y[2 * j + 1] = fmaf(d2[i / 2][j][i % 2 * 2 + 1], factor[i], y[2 * j + 1]);
+          v[2 * j] = fmaf(d2[i / 2][j][i % 2 * 2], factor[i], v[2 * j]);
+          v[2 * j + 1] = fmaf(d2[i / 2][j][i % 2 * 2 + 1], factor[i], v[2 * j + 1]);
         }
         if constexpr (sizeof(TY) == 4) {
-          const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-          store4(op[i], n0 + n + 4 * t, n1, p.out_wide, lo);
-          store4(op[i], n0 + n + 16 + 4 * t, n1, p.out_wide, hi);
+#pragma unroll
+          for (int h = 0; h < V; ++h)
+            y[i][h] = make_uint4(__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3]));
         } else {
-          store8(op[i], n0 + n + 8 * t, n1, p.out_wide, y);
+          y[i][0] = make_uint4(pack2(v[0], v[1], A), pack2(v[2], v[3], A), pack2(v[4], v[5], A), pack2(v[6], v[7], A));
         }
       }
-      __syncwarp();
-      st = st + slot == ring + slots * slot ? ring : st + slot;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < V; ++h) {
+          const int c = n + (V == 2 ? 16 * h + 4 * t : 8 * t);
+          if (!op[i]) continue;
+          if (whole) *reinterpret_cast<uint4*>(op[i] + c) = y[i][h];
+          else store_piece(op[i], c, width, y[i][h]);
+        }
+      load_y(n + ways * 32);
     }
-    cp_async_wait<0>();
   }
 }
 
@@ -425,12 +447,12 @@ template <class T, class TX, class TY, int NT>
 cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s) {
   constexpr int B = 8 * NT, kSlot = 2 * kArea + (sizeof(TX) == 4 ? 1 : 2) * area(B);
   WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0, 0};
-  const int steps = (w.RA + 31) / 32, second = (int)sizeof(TY) / 2 * kArea + (steps < 2 ? steps : 2) * kArea;
+  const int steps = (w.RA + 31) / 32;
   // Two blocks an SM where there are that many.  At least: two slots a warp; the
   // warps' parts of T, 32 rows and a block of ranks each; T whole behind the
-  // numbers that it is split into; those, and two slots a warp of the second product.
+  // numbers that it is split into.
   int bytes = (long long)n_units * size > sms ? 112 * 1024 : 224 * 1024;
-  for (const int need : {kWarps * 2 * kSlot, kWarps * 32 * B * 4, kWideRows * w.RA * 10, 3 * steps * kWideRows * 64 + 128 + kWarps * (2 * second + 16)})
+  for (const int need : {kWarps * 2 * kSlot, kWarps * 32 * B * 4, kWideRows * w.RA * 10, 3 * steps * kWideRows * 64})
     if (bytes < need) bytes = need;
   w.ring = bytes / kWarps / 16 * 16;
   w.bytes = bytes;
