@@ -109,14 +109,13 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   const int rank = cluster_rank(), size = cluster_size(), RA = wp.RA;
   pdl_launch_dependents();
   // The plan is older than any kernel that this one may overlap, and what L2 holds
-  // follows later writes: B is asked for before the wait, y behind it.
+  // follows later writes: B is asked for before the wait, y once x is there.
   const Unit& u = p.units[blockIdx.x / size];
   const int* rows = p.order + u.first;
   const int n_rows = u.n_rows;
   const int n_per = (p.N + size * 32 - 1) / (size * 32) * 32, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N), width = n1 - n0;
   prefetch_b(p, static_cast<const T*>(p.b) + u.adapter * p.b_adapter, n0, n1);
   pdl_wait();
-  if (threadIdx.x < n_rows) prefetch(static_cast<const TY*>(p.y) + rows[threadIdx.x] * p.y_row + n0, width);
   const int r = p.ranks ? min(max(p.ranks[u.adapter], 0), p.rank) : p.rank;
   const T* A = static_cast<const T*>(p.a) + u.adapter * p.a_adapter;
   const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
@@ -227,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
       st = st + kSlot == ring + slots * kSlot ? ring : st + kSlot;
     }
     cp_async_wait<0>();
+    if (threadIdx.x < n_rows) prefetch(static_cast<const TY*>(p.y) + rows[threadIdx.x] * p.y_row + n0, width);
     __syncthreads();
   }
 
