@@ -6,7 +6,7 @@
     bank.apply(plan, x, y)                            # y += scale (x A^T) B^T
 
 Calls are queued on torch's current stream of the bank's device and return
-without waiting for it.
+without waiting for it.  No gradients are recorded.
 """
 
 from __future__ import annotations

@@ -7,6 +7,7 @@
 Calls are queued on torch's current stream of the logits' device and return
 without waiting for it; results are new int32 tensors on that device.  Decisions
 are those of 64-bit arithmetic on the given logits, probabilities and uniforms.
+No gradients are recorded.
 """
 
 from __future__ import annotations
@@ -129,8 +130,8 @@ def verify_drafts(logits, drafts, draft_probs, uniforms, row_start, temperature=
     Sequence b has rows row_start[b] .. row_start[b + 1] - 1 (int32, on the
     device), one more than its drafts.  drafts: int32 [rows], drafts[r] is the
     token that row r judges, drawn from row r of draft_probs (float32 [rows,
-    vocabulary]); those of a sequence's last row are not read.  uniforms: float32
-    [rows]; temperature: a number, or float32 [rows]."""
+    vocabulary]); what they hold in a sequence's last row does not matter.
+    uniforms: float32 [rows]; temperature: a number, or float32 [rows]."""
     torch, lib, _, stream = _setup()
     a, work, index = _logits(logits, uniforms, temperature)
     n, v = logits.shape

@@ -673,7 +673,8 @@ int spec_batch_sample(const spec_batch_logits* l, float* probs_out, int64_t prob
 /* Drafted chains.  Sequence b has rows row_start[b] .. row_start[b + 1] - 1 (one
  * more than its drafts, as spec_batched_logits returns them).  drafts[r] is the
  * token that row r judges and row r of draft_probs (at r * probs_stride) the
- * distribution it was drawn from; those of a sequence's last row are not read.
+ * distribution it was drawn from; what they hold in a sequence's last row does
+ * not matter.  No row belongs to two sequences.
  * Row r's uniform decides about drafts[r]; the token after a rejection takes the
  * next row's, the token behind the last draft its own row's: the order in which
  * spec_verify_rejection uses them.  A draft outside the vocabulary (-1, say)
@@ -724,7 +725,9 @@ typedef struct spec_lora_bank {
  * - 1, or -1 for a row without one; rows of one adapter need not be neighbours,
  * and are taken together.  Writes the plan to buf (host, spec_lora_plan_bytes)
  * and fills *out but for device_copy: the caller copies buf to the device, sets
- * it, and keeps both unchanged until the calls that use them are done. */
+ * it, and keeps both unchanged until the calls that use them are done.  The copy
+ * is a cudaMemcpy of some kind or done before a call is queued: a call looks at
+ * its plan while the kernel queued before it still runs. */
 typedef struct spec_lora_plan {
   int n_rows, n_adapters, n_wide, n_narrow, n_bare, n_tall, n_big, reserved;
   const void* device_copy;     /* 16-byte aligned */
