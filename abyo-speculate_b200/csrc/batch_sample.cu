@@ -38,6 +38,8 @@ namespace {
 constexpr float kErr = 1.f / (1 << 18);  // of a sum of weights, relative
 constexpr int kBad = -1, kUnsure = -2;
 constexpr int kPer = kChunk / 32;  // columns of a lane
+constexpr int kThreads = 256;      // of the second kernels
+constexpr int kWarps = kThreads / 32;
 
 SPEC_DEV float ex2(float x) {
   float r;
@@ -561,27 +563,23 @@ SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
 // in f32 (REST32) or in 64 bits (REST64).
 enum : int { P64 = 0, REST32 = 1, REST64 = 2 };
 
-// 2^y for y <= 0 in 64 bits: y = n + i / 64 + f, |f| <= 1 / 128, 2^(i / 64) from
-// a table and the Taylor series of 2^f to (f ln 2)^5 / 5! (the next term is below
+// 2^y for y <= 0 in 64 bits: y = n + i / 256 + f, |f| <= 1 / 512, 2^(i / 256) from
+// a table and the Taylor series of 2^f to (f ln 2)^4 / 4! (the next term is below
 // 2^-54).  Below 2^-1000: zero.
 struct Powers {
-  double of[64];
-  SPEC_DEV void fill() {  // all threads of the block; they sync before its use
-    if (threadIdx.x < 64) of[threadIdx.x] = exp2((double)(int)threadIdx.x / 64);
-  }
-  // y in 64ths
+  double of[256];
+  SPEC_DEV void fill() { of[threadIdx.x] = exp2((double)(int)threadIdx.x / 256); }  // by kThreads threads; the block syncs before its use
+  // y in 256ths, above -2^31
   SPEC_DEV double pow(double y) const {
-    constexpr double kLn2 = 0.693147180559945309 / 64, kWhole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-    y = fmax(y, -64.0 * 1100);
-    const double t = y + kWhole, f = (y - (t - kWhole)) * kLn2;
-    double s = fma(f, 1.0 / 120, 1.0 / 24);
-    s = fma(s, f, 1.0 / 6);
-    s = fma(s, f, 0.5);
-    s = fma(s, f, 1.0);
+    constexpr double c = 0.693147180559945309 / 256, kWhole = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double t = y + kWhole, f = y - (t - kWhole);
+    double s = fma(f, c * c * c * c / 24, c * c * c / 6);
+    s = fma(s, f, c * c / 2);
+    s = fma(s, f, c);
     s = s * f;
     const int n = __double2loint(t);
-    const double b = of[n & 63], w = fma(s, b, b);
-    const int e = n >> 6;
+    const double b = of[n & 255], w = fma(s, b, b);
+    const int e = n >> 8;
     return e < -1000 ? 0.0 : __hiloint2double(__double2hiint(w) + (e << 20), __double2loint(w));
   }
 };
@@ -592,6 +590,7 @@ struct Weigher {
   const Ref& ref;
   const float* q;
   float inv_zf;
+  float low;  // logits below it weigh nothing; (x - m) h of the others, low's rounding included, is above -2^31
   double h, inv_z;
   const Powers* powers;
   SPEC_DEV Weigher(const Row<T>& r_, const Ref& ref_, const float* q_, int kind, double Z, const Powers* powers_ = nullptr)
@@ -599,11 +598,15 @@ struct Weigher {
     if (kind == REST32) {
       inv_zf = 1.f / (float)Z;
     } else {
-      h = 64 * 1.44269504088896341 / (double)r.t;
+      h = 256 * 1.44269504088896341 / (double)r.t;
+      low = ref.m - 1e5f * r.t;
       inv_z = 1.0 / Z;
     }
   }
-  SPEC_DEV double p64(float x) const { return powers->pow(((double)x - (double)ref.m) * h); }
+  SPEC_DEV double p64(float x) const {
+    const double w = powers->pow(((double)fmaxf(x, low) - (double)ref.m) * h);
+    return x >= low ? w : 0.0;
+  }
   SPEC_DEV void rest32(float (&x)[kPer], const float (&y)[kPer]) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = fmaxf(fmaf(ex2(fmaf(x[i], ref.h, -ref.R)), inv_zf, -y[i]), 0.f);
@@ -755,8 +758,6 @@ SPEC_DEV int draw_rest(const Weigher<T>& f, const float* sums, int nch, float u,
 // ---------------------------------------------------------------------------
 // A cluster a row
 // ---------------------------------------------------------------------------
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 
 // Probabilities of this warp's chunks, two chunks' loads at a time.
 template <class T>
@@ -811,6 +812,7 @@ __global__ void __launch_bounds__(kThreads, ALONE ? 2 : 4) sample_kernel(const _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), row = blockIdx.x / cluster_size();
   pdl_launch_dependents();
+  s_powers.fill();
   pdl_wait();
   const Row<T> r(p.r, row);
   const int nch = p.r.nch;
@@ -836,8 +838,6 @@ __global__ void __launch_bounds__(kThreads, ALONE ? 2 : 4) sample_kernel(const _
   int tok = s_tok;
   if (tok == kUnsure) {
     if (!PROBS && warp) j = join(r, Stats(p.r.stats + (long long)row * nch, nch, lane));
-    s_powers.fill();
-    __syncthreads();
     const Weigher<T> f(r, j.ref, nullptr, P64, 1, &s_powers);
     f.sum(P64, sums, nch, lane);
     cluster_sync();
@@ -875,6 +875,7 @@ __global__ void __launch_bounds__(kThreads, 3) chain_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), b = blockIdx.x / cluster_size(), nch = p.r.nch;
   pdl_launch_dependents();
+  s_powers.fill();
   pdl_wait();
   int r0;
   const int n = rows_of(p, b, &r0);
@@ -927,8 +928,6 @@ __global__ void __launch_bounds__(kThreads, 3) chain_kernel(const __grid_constan
       if (verdict == A_UNSURE) {
         const Row<T> r(p.r, r0 + at);
         const Weigher<T> f(r, row.join.ref, nullptr, P64, 1, &s_powers);
-        s_powers.fill();
-        __syncthreads();
         if (used) cluster_sync();
         f.sum(P64, sums, nch, lane);
         cluster_sync();
@@ -970,8 +969,6 @@ __global__ void __launch_bounds__(kThreads, 3) chain_kernel(const __grid_constan
     __syncthreads();
     tok = s_tok;
     if (tok == kUnsure) {
-      s_powers.fill();
-      __syncthreads();
       const Weigher<T> f(r, ref, nullptr, P64, 1, &s_powers);
       double z = z64;
       if (z == 0) {
@@ -1019,6 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 3) tree_kernel(const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), size = cluster_size(), b = blockIdx.x / size, nch = p.r.nch;
   pdl_launch_dependents();
+  s_powers.fill();
   pdl_wait();
   int r0;
   const int n = rows_of(p, b, &r0), near = min(n, kTreeNodes);
@@ -1045,8 +1043,6 @@ __global__ void __launch_bounds__(kThreads, 3) tree_kernel(const __grid_constant
       const Row<T> r(p.r, r0 + cur);
       const Joined j = join(r, Stats(p.r.stats + (long long)(r0 + cur) * nch, nch, lane));
       const Weigher<T> f(r, j.ref, nullptr, P64, 1, &s_powers);
-      s_powers.fill();
-      __syncthreads();
       cluster_sync();
       f.sum(P64, sums, nch, lane);
       cluster_sync();
