@@ -14,12 +14,18 @@
 // d = (M - l) / T: h is off by 1.5 u and the multiply-add by u, a weight by
 // (2.5 d + 0.5) u, the hardware's 2^x by 4 u more.  Of positive terms a chunk's
 // sum is off by 9 u (16 a lane in pairs, 5 rounds of shuffles), a prefix of
-// chunks by 12 u more (7 additions, 5 rounds), one inside a chunk by 20 u
-// (15 and 5).  The mean of d under the weights of any set of columns is their
-// entropy less the logarithm of their sum S, at most ln V - ln S; for S >= 1
-// and V <= 2^20 that makes (4.5 + 21 + 2.5 * 13.9) u < 2^-18 of S (kErr), for
-// S > 2^-33 less than twice that.  Smaller sums, and rows with |M| h of 2^22
-// and more, are left to 64 bits.
+// chunks by 12 u more (7 additions, 5 rounds), Z by 15 (8 and, of 8 blocks, 7),
+// one inside a chunk by 20 u (15 and 5).  The mean of d under the weights of any
+// set of columns is their entropy less the logarithm of their sum S, at most
+// ln V - ln S, so that weights of sum S are off by (4.5 + 2.5 (ln V - ln S)) u S
+// in all (spread(S) below; it grows with S up to V / e).  For S >= 1 and V <= 2^20
+// that makes (4.5 + 24 + 2.5 * 13.9) u < 2^-18 of S (kErr).
+//
+// A comparison of a prefix with v Z, 0 <= v <= 1, is off by what its two sides
+// are, or, as the columns before the chunk of the token are summed once for both,
+// by max(v, 1 - v) of what all weights are off by and less than twice what the
+// chunk's are: the smaller of the two counts.  Targets up to 2^-33, and rows
+// with |M| h of 2^22 and more, are left to 64 bits.
 //
 // Two kernels.  stats_kernel reads every row once, a warp one chunk of 512
 // columns or 8 KB, and leaves each chunk's reference and sum.  The second
@@ -523,6 +529,12 @@ SPEC_DEV int first_largest(const Stats& st, float M) {
   return __reduce_min_sync(0xffffffffu, e);
 }
 
+// What weights of sum S are off by in all, in units of 2^-24, of a row of V columns.
+SPEC_DEV float spread(float S, int V) {
+  const float nats = 0.6932f * (__log2f((float)V) - __log2f(S)) + 0.01f;  // the logarithm is off by less than 0.001
+  return (4.5f + 2.5f * fmaxf(nats, 1.f)) * S;
+}
+
 SPEC_DEV double unit(float u) { return (double)fminf(fmaxf(u, 0.f), 1.f); }  // NaN: 0
 
 // A token of p, or kBad, or kUnsure where f32 does not decide.
@@ -530,7 +542,7 @@ template <class T>
 SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
   if (!j.ok) return kBad;
   if (r.t == 0.f) return first_largest(st, j.ref.m);
-  const double target = unit(u) * (double)j.Z, slack = (target < 1 ? 4 : 2) * kErr * target;
+  const double v = unit(u), target = v * (double)j.Z;
   if (!j.ref.whole || target <= 0x1p-33) return kUnsure;
   double run = 0, lo, hi;
   int c = -1;
@@ -550,6 +562,9 @@ SPEC_DEV int draw(const Row<T>& r, const Stats& st, const Joined& j, float u) {
   if (c < 0) return kUnsure;
   float x[kPer];
   load_chunk<T, true>(r, c, st.lane, x);
+  const float t = (float)target, all = spread(j.Z, r.V), apart = spread(t, r.V) + (float)v * all;
+  const float shared = (float)fmax(v, 1 - v) * all + 2 * spread(fmaxf((float)(hi - run), 0x1p-60f), r.V);
+  const double slack = 1.01 * 0x1p-24 * (double)(45.f * t + fminf(apart, shared));
 #pragma unroll
   for (int i = 0; i < kPer; ++i) x[i] = ex2(fmaf(x[i], j.ref.h, -j.ref.R));
   const int e = find(x, run, target, st.lane, &lo, &hi);
@@ -611,12 +626,13 @@ struct Weigher {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = fmaxf(fmaf(ex2(fmaf(x[i], ref.h, -ref.R)), inv_zf, -y[i]), 0.f);
   }
-  SPEC_DEV void exact(int kind, const float (&x)[kPer], const float (&y)[kPer], double (&w)[kPer]) const {
+  template <int N>
+  SPEC_DEV void exact(int kind, const float (&x)[N], const float (&y)[N], double (&w)[N]) const {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) w[i] = p64(x[i]);
+    for (int i = 0; i < N; ++i) w[i] = p64(x[i]);
     if (kind == REST64) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) w[i] = fmax(w[i] * inv_z - (double)y[i], 0.0);
+      for (int i = 0; i < N; ++i) w[i] = fmax(w[i] * inv_z - (double)y[i], 0.0);
     }
   }
   // Chunk sums by all warps of the cluster, a chunk's loads ahead; the caller syncs it.
@@ -688,12 +704,16 @@ SPEC_DEV double total(const double* sums, int nch, int lane) {
   return s;
 }
 
-// A token of the weights in `sums`, whose sum is Zs, in 64 bits.
+// A token of the weights in `sums`, whose sum is Zs, in 64 bits.  One warp runs
+// this once, and code that runs once is fetched from L2: a vector of columns a turn
+// (8.7 us with the chunk's 16 columns of a lane at once, 7 so).
 template <class T>
 SPEC_DEV int draw_sums(const Weigher<T>& f, int kind, const double* sums, int nch, double Zs, float u, int lane) {
+  constexpr int N = Vec<T>::N;
   const double target = unit(u) * Zs;
   double run = 0, lo, hi;
   int c = -1, last = -1;
+#pragma unroll 1
   for (int b = 0; b * kBlock < nch && c < 0; ++b) {
     double w[8];
     load_sums(sums, b, nch, lane, w);
@@ -706,14 +726,23 @@ SPEC_DEV int draw_sums(const Weigher<T>& f, int kind, const double* sums, int nc
   const bool whole = c < 0;  // the target is the sum of all: the last column of some weight
   if (whole) c = last;
   if (c < 0) return kBad;
-  float x[kPer], y[kPer];
-  load_chunk<T, true>(f.r, c, lane, x);
-  if (kind == REST64) load_probs<T, true>(f.r, f.q, c, lane, y);
-  double w[kPer];
-  f.exact(kind, x, y, w);
-  int e = whole ? -1 : find(w, run, target, lane, &lo, &hi);
-  if (e < 0) e = find_last(w, lane);
-  return e < 0 ? kBad : c * kChunk - f.r.shift + e;
+  int token = -1, tail = kBad;
+#pragma unroll 1
+  for (int i = 0; i < kPer / N && token < 0; ++i) {
+    const int first = c * kChunk - f.r.shift + i * 32 * N, e = first + lane * N;
+    float x[N], y[N];
+    unpack(load_vec(f.r, e), x, f.r.p);
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] = kind == REST64 && e + k >= 0 && e + k < f.r.V ? f.q[e + k] : 0.f;
+    double w[N];
+    f.exact(kind, x, y, w);
+    const int some = find_last(w, lane);
+    if (some >= 0) tail = first + some;
+    const int at = whole ? -1 : find(w, run, target, lane, &lo, &hi);
+    if (at >= 0) token = first + at;
+    run = hi;
+  }
+  return token < 0 ? tail : token;
 }
 
 // A token of max(p - q, 0) from REST32 sums, or kUnsure.
@@ -749,9 +778,11 @@ SPEC_DEV int draw_rest(const Weigher<T>& f, const float* sums, int nch, float u,
   load_probs<T, true>(f.r, f.q, c, lane, y);
   f.rest32(x, y);
   const int e = find(x, run, target, lane, &lo, &hi);
-  // Weights and Z are off by (39.2 + 60.2) u of Z, max(p - q, 0) by no more
-  // than p, its sums by 41 u: the prefix, and u times the sum likewise.
-  const double slack = 4.5 * kErr;
+  // max(p - q, 0) is off by no more than p: by the weights' errors and Z's (24 u for its sum and 1
+  // for 1 / Z besides), each at most once, as a prefix and u times the whole share the columns.
+  // The sums' own are 21 u each, and 2 for the multiply-add.
+  const float Z = 1.f / f.inv_zf;
+  const double slack = 1.01 * 0x1p-24 * (2.0 * (double)(spread(Z, f.r.V) / Z) + 25 + 44 * Zs);
   return e >= 0 && lo + slack <= target && target + slack < hi ? c * kChunk - f.r.shift + e : kUnsure;
 }
 
@@ -969,32 +1000,22 @@ __global__ void __launch_bounds__(kThreads, 3) chain_kernel(const __grid_constan
     __syncthreads();
     tok = s_tok;
     if (tok == kUnsure) {
-      const Weigher<T> f(r, ref, nullptr, P64, 1, &s_powers);
-      double z = z64;
-      if (z == 0) {
-        if (used) cluster_sync();
-        f.sum(P64, sums, nch, lane);
-        cluster_sync();
-        z = total(sums, nch, lane);
-      }
+      // The sums of p, then those of max(p - q, 0); where that is 0 everywhere, p's again.
+      Weigher<T> f(r, ref, q, P64, 1, &s_powers);
       int kind = P64;
-      double zs = z;
-      if (rest) {
-        const Weigher<T> g(r, ref, q, REST64, z, &s_powers);
+      double zs = z64;
+#pragma unroll 1
+      for (int turn = z64 == 0 ? 0 : 1; turn < 3; ++turn) {
+        if (turn && (!rest || (turn == 2 && zs > 0))) break;
+        if (turn == 1) f.inv_z = 1.0 / zs;
+        kind = turn == 1 ? REST64 : P64;
+        if (used) cluster_sync();
+        f.sum(kind, sums, nch, lane);
         cluster_sync();
-        g.sum(REST64, sums, nch, lane);
-        cluster_sync();
-        kind = REST64;
+        used = true;
         zs = total(sums, nch, lane);
-        if (!(zs > 0)) {  // p is nowhere above q: p itself
-          cluster_sync();
-          f.sum(P64, sums, nch, lane);
-          cluster_sync();
-          kind = P64;
-          zs = z;
-        }
       }
-      if (rank == 0 && warp == 0) tok = draw_sums(Weigher<T>(r, ref, q, kind, z, &s_powers), kind, sums, nch, zs, u, lane);
+      if (rank == 0 && warp == 0) tok = draw_sums(f, kind, sums, nch, zs, u, lane);
     }
   }
   if (rank == 0 && threadIdx.x == 0) {
