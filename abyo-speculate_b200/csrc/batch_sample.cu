@@ -790,11 +790,11 @@ SPEC_DEV int draw_rest(const Weigher<T>& f, const float* sums, int nch, float u,
 // A cluster a row
 // ---------------------------------------------------------------------------
 
-// Probabilities of this warp's chunks, two chunks' loads at a time.
+// Probabilities of this warp's chunks (all warps but the first, which draws), two chunks' loads at a time.
 template <class T>
 SPEC_DEV void write_probs(const SampleParams& p, const Row<T>& r, const Joined& j, int top, int row, int warp, int lane) {
   constexpr int N = Vec<T>::N, NV = kPer / N;
-  const int nch = p.r.nch, step = kWarps * cluster_size();
+  const int nch = p.r.nch, step = (kWarps - 1) * cluster_size();
   float* out = p.probs + row * p.probs_stride;
   const float inv = 1.f / j.Z;
   const bool wide = (reinterpret_cast<uintptr_t>(out) / 4 - r.shift) % 4 == 0;
@@ -814,9 +814,24 @@ SPEC_DEV void write_probs(const SampleParams& p, const Row<T>& r, const Joined& 
     for (int i = 0; i < NV; ++i) {
       const int e = first + i * 32 * N;
       if (all) {
+        if constexpr (N == 8) {
+          // Two lanes exchange halves, so that a store is 512 bytes behind one another.
+          const bool odd = lane & 1;
+          float4 a, b;
+          float* p0 = &a.x;
+          float* p1 = &b.x;
 #pragma unroll
-        for (int k = 0; k < N; k += 4)
-          *reinterpret_cast<float4*>(out + e + k) = make_float4(x[i * N + k], x[i * N + k + 1], x[i * N + k + 2], x[i * N + k + 3]);
+          for (int k = 0; k < 4; ++k) {
+            const float lo = x[i * N + k], hi = x[i * N + 4 + k], got = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
+            p0[k] = odd ? got : lo;
+            p1[k] = odd ? hi : got;
+          }
+          float* to = out + e - (odd ? 4 : 0);
+          *reinterpret_cast<float4*>(to) = a;
+          *reinterpret_cast<float4*>(to + 8) = b;
+        } else {
+          *reinterpret_cast<float4*>(out + e) = make_float4(x[i * N], x[i * N + 1], x[i * N + 2], x[i * N + 3]);
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < N; ++k)
@@ -825,7 +840,7 @@ SPEC_DEV void write_probs(const SampleParams& p, const Row<T>& r, const Joined& 
     }
   };
 #pragma unroll 1
-  for (int c = cluster_rank() * kWarps + warp; c < nch; c += 2 * step) {
+  for (int c = cluster_rank() * (kWarps - 1) + warp - 1; c < nch; c += 2 * step) {
     const int d = c + step < nch ? c + step : c;
     uint4 v[NV], w[NV];
     load_raw<T, false>(r, c, lane, v);
@@ -861,7 +876,6 @@ __global__ void __launch_bounds__(kThreads, ALONE ? 2 : 4) sample_kernel(const _
     if (PROBS && warp) write_probs(p, r, j, r.t == 0.f && j.ok ? first_largest(st, j.ref.m) : -1, row, warp, lane);
     if (warp == 0) {
       const int tok = draw(r, st, j, u);
-      if (PROBS) write_probs(p, r, j, tok, row, warp, lane);
       if (lane == 0) s_tok = tok;
     }
   }
