@@ -139,7 +139,8 @@ class LoraBankDesc(ctypes.Structure):
 class LoraPlanDesc(ctypes.Structure):
     """spec_lora_plan (include/spec_b200.h)."""
 
-    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_wide", "n_narrow", "n_bare", "n_tall", "n_big", "reserved")] + [
+    _fields_ = [(n, ctypes.c_int) for n in ("n_rows", "n_adapters", "n_wide", "n_narrow", "n_bare", "n_tall", "n_big", "reserved",
+                                            "n_mid", "n_mid_wide", "mid_all")] + [
         ("device_copy", ctypes.c_void_p)]
 
 

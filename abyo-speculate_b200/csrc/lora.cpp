@@ -15,9 +15,26 @@ using namespace specb200::lora;
 namespace {
 
 constexpr int kPlanRows = 1 << 20;
-constexpr int kHalvesMost = 36;  // units of 32 rows: as many clusters of 8 blocks as a B200 holds, two blocks an SM
-constexpr int kTallFrom = 8;     // units of 128 rows from which on they are taken
-constexpr int kNarrowMost = 16;  // rows of an adapter that the kernel for few rows takes, in units of 8
+// Which kernel takes an adapter's rows.  us for (a) rank 16, 4096 to 4096 channels in
+// bf16, (b) rank 64, 2048 to 8192, f32 rows, (c) rank 16, 4096 to 14336, f32 rows:
+// - up to kNarrowMost rows in units of 8: 24 adapters of 16 rows 9.4 / 24, 18.7 / 47
+//   (a / b) in units of 32;
+// - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows 16.9 / 37 /
+//   38, 21.6 / 53 / 44 in units of 32; one of 256 8.9 / 21 / 21, 10.8 / 26 / 31.  For
+//   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are too
+//   many: 24 of 64 31 / 66 / 69, 33 / 90 / 82 in units of 64.  Not where A and B, read
+//   again for every 8 rows, are more than kAgainMost times the rows (known when the
+//   plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
+// - units of 32 rows, not 64, for up to kHalvesMost of them: 4 of 64 11 / 26, 15 / 43; 24
+//   of 64 31 / 88, 33 / 90;
+// - units of 128, not 64, from kTallFrom of them on: 4 of them 21 / 28, 20.5 / 31 (8192
+//   to 2048 in bf16 for b), 8 of them 21 / 28, 31 / 49.
+constexpr int kNarrowMost = 16;
+constexpr int kFewUnits = 111;   // four blocks a cluster, three an SM
+constexpr int kSomeUnits = 222;  // two
+constexpr int kAgainMost = 4;
+constexpr int kHalvesMost = 36;  // as many clusters of 8 blocks as a B200 holds, two an SM
+constexpr int kTallFrom = 5;
 
 // Layout of a plan: units (of adapters of very many rows by 128, the same by 64,
 // those of other adapters of many rows, those of few, rows without one), then the rows in their order, then the word of the device's waits.
@@ -41,6 +58,13 @@ int cluster_for(int n, int per_sm, int sms) {
   return size;
 }
 
+// Three blocks an SM at once; a single block a unit only for many: 256 units of 8
+// rows (c above) 141 us, 116 in clusters of two, a few of which start late.
+int narrow_cluster(int n, int sms) {
+  const int size = cluster_for(n, 3, sms);
+  return size == 1 && (int64_t)n * 2 <= (int64_t)sms * 5 ? 2 : size;
+}
+
 unsigned* status_of(const spec_lora_plan* plan) {
   const uint8_t* b = static_cast<const uint8_t*>(plan->device_copy);
   return const_cast<unsigned*>(reinterpret_cast<const unsigned*>(b + (size_t)plan->n_rows * (sizeof(Unit) + sizeof(int))));
@@ -60,18 +84,20 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   // By adapter, rows in their order; rows without one last.
   std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return (unsigned)adapters[x] < (unsigned)adapters[y]; });
   // An adapter's rows in units of equal size; rows without one are copied one by
-  // one.  Units of 64 rows read A and B half as often as those of 32, which are
-  // taken where there are few of them; adapters of more than 64 rows are also cut
-  // by 128, where that gives enough units.
+  // one.  Runs of rows that two kernels can take, by x's type or the bank's size, are
+  // cut for both.
   struct Run {
     int adapter, begin, end;
   };
   std::vector<Run> runs;
-  int64_t halves = 0, tall = 0;
+  int64_t halves = 0, tall = 0, eighths = 0, near = 0;  // units of 32, 128 and 8 rows; of 8 of runs of at most 64
   for (int i = 0; i < n_rows;) {
     int e = i;
     while (e < n_rows && adapters[order[e]] == adapters[order[i]]) ++e;
     runs.push_back(Run{adapters[order[i]], i, e});
+    const int64_t n = adapters[order[i]] >= 0 ? (e - i + kNarrowRows - 1) / kNarrowRows : 0;
+    eighths += n;
+    if (e - i <= kWideRows) near += n;
     if (adapters[order[i]] >= 0 && e - i > kNarrowMost) {
       halves += (e - i + kWideRows / 2 - 1) / (kWideRows / 2);
       if (e - i > kWideRows) tall += (e - i + kTallRows - 1) / kTallRows;
@@ -79,7 +105,8 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
     i = e;
   }
   const int wide_rows = halves <= kHalvesMost ? kWideRows / 2 : kWideRows;
-  std::vector<Unit> units[5];
+  const bool few = eighths <= kFewUnits, some = few || (halves > kHalvesMost && near <= kSomeUnits);
+  std::vector<Unit> units[5], mid_wide, mid;
   auto cut = [&](std::vector<Unit>& to, const Run& r, int most) {
     const int rows = r.end - r.begin, n = (rows + most - 1) / most;
     for (int k = 0; k < n; ++k) {
@@ -95,8 +122,10 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
     if (big) cut(units[0], r, kTallRows);
     if (r.adapter < 0) cut(units[4], r, 1);
     else if (rows <= kNarrowMost) cut(units[3], r, kNarrowRows);
+    else if (few || (some && rows <= kWideRows)) cut(big ? units[1] : mid_wide, r, wide_rows), cut(mid, r, kNarrowRows);
     else cut(units[big ? 1 : 2], r, wide_rows);
   }
+  units[2].insert(units[2].end(), mid_wide.begin(), mid_wide.end());
   uint8_t* b = static_cast<uint8_t*>(buf);
   if (n_rows) {
     size_t at = 0;
@@ -104,6 +133,8 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
       if (!v.empty()) memcpy(b + at, v.data(), v.size() * sizeof(Unit));
       at += v.size() * sizeof(Unit);
     }
+    // Behind them, at most a row's worth of units a row in all.
+    if (!mid.empty()) memcpy(b + at, mid.data(), mid.size() * sizeof(Unit));
     memcpy(b + (size_t)n_rows * sizeof(Unit), order.data(), (size_t)n_rows * sizeof(int));
   }
   memset(b + (size_t)n_rows * (sizeof(Unit) + sizeof(int)), 0, 16);
@@ -115,6 +146,9 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   out->n_wide = (int)units[2].size();
   out->n_narrow = (int)units[3].size();
   out->n_bare = (int)units[4].size();
+  out->n_mid = (int)mid.size();
+  out->n_mid_wide = (int)mid_wide.size();
+  out->mid_all = few;
   return SPEC_OK;
 }
 
@@ -154,7 +188,8 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   if (b->rank < 0 || b->rank > kMaxRank) return fail(SPEC_ERR_UNSUPPORTED, "%s: rank %d (up to %d is built)", what, b->rank, kMaxRank);
   if (b->device < 0) return fail(SPEC_ERR_INVALID, "%s: device %d", what, b->device);
   if (plan->n_rows < 0 || plan->n_rows > kPlanRows || plan->n_wide < 0 || plan->n_narrow < 0 || plan->n_bare < 0 || plan->n_tall < 0 || plan->n_big < 0 ||
-      (int64_t)plan->n_tall + plan->n_big + plan->n_wide + plan->n_narrow + plan->n_bare > plan->n_rows)
+      plan->n_mid < 0 || plan->n_mid_wide < 0 || plan->n_mid_wide > plan->n_wide ||
+      (int64_t)plan->n_tall + plan->n_big + plan->n_wide + plan->n_narrow + plan->n_bare + plan->n_mid > plan->n_rows)
     return fail(SPEC_ERR_INVALID, "%s: not a plan", what);
   if (plan->n_adapters > b->n_adapters)
     return fail(SPEC_ERR_INVALID, "%s: a plan for %d adapters, the bank has %d", what, plan->n_adapters, b->n_adapters);
@@ -216,16 +251,27 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   cudaError_t e = multiprocessors(b->device, &sms);
   const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  p.units = units;
+  // Rows that units of 8 can take as well: do they?
+  const bool mid = plan->n_mid && (int64_t)b->rank * (b->k + b->n) * 2 <= (int64_t)kAgainMost * kNarrowRows *
+                                      (b->k * (x_f32 ? 4LL : 2LL) + 2 * b->n * (y_f32 ? 4LL : 2LL));
+  const bool rest = !(mid && plan->mid_all);  // there are others
   bool taken = false;
-  if (e == cudaSuccess && plan->n_tall && !x_f32)
+  p.units = units;
+  if (e == cudaSuccess && rest && plan->n_tall && !x_f32)
     e = launch_tall(p, status_of(plan), b->dtype, y_f32, plan->n_tall, cluster_for(plan->n_tall, 1, sms), s, &taken);
   p.units = units + plan->n_tall + (taken ? plan->n_big : 0);
-  const int wide = plan->n_wide + (taken ? 0 : plan->n_big);
+  const int wide = rest ? plan->n_wide - (mid ? plan->n_mid_wide : 0) + (taken ? 0 : plan->n_big) : 0;
   if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, cluster_for(wide, 2, sms), sms, s);
   p.units = units + plan->n_tall + plan->n_big + plan->n_wide;
-  const int n = plan->n_narrow + (in_place ? 0 : plan->n_bare);
-  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, cluster_for(n, 3, sms), s);
+  // Units of 8 rows, rows without an adapter and the units behind them: at once, but
+  // for rows in place, which have nothing to copy.
+  const int bare = plan->n_bare, again = mid ? plan->n_mid : 0;
+  const int n = in_place && bare ? plan->n_narrow : plan->n_narrow + bare + again;
+  if (e == cudaSuccess) e = launch_narrow(p, b->dtype, x_f32, y_f32, n, narrow_cluster(n, sms), s);
+  if (in_place && bare && again && e == cudaSuccess) {
+    p.units += plan->n_narrow + bare;
+    e = launch_narrow(p, b->dtype, x_f32, y_f32, again, narrow_cluster(again, sms), s);
+  }
   return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
 }
 

@@ -707,8 +707,9 @@ int spec_batch_verify_tree(const spec_batch_logits* l, int n_seqs, const int32_t
  * plan says which adapter each row of a step has (once per step, for all
  * projections and layers).  Sums and x A^T are f32 (the latter is split into
  * parts of 16 bits in all or more for the second product), each result is
- * rounded once.  Calls keep no state, wait for nothing, allocate nothing and can
- * be captured.  Pointers are device memory of `device` unless said otherwise. */
+ * rounded once.  One call's result does not depend on timing; a row's last bits
+ * may depend on the other rows of the plan.  Calls keep no state, wait for
+ * nothing, allocate nothing and can be captured.  Pointers are device memory of `device` unless said otherwise. */
 typedef struct spec_lora_bank {
   int device;
   int n_adapters;
@@ -729,7 +730,7 @@ typedef struct spec_lora_bank {
  * is a cudaMemcpy of some kind or done before a call is queued: a call looks at
  * its plan while the kernel queued before it still runs. */
 typedef struct spec_lora_plan {
-  int n_rows, n_adapters, n_wide, n_narrow, n_bare, n_tall, n_big, reserved;
+  int n_rows, n_adapters, n_wide, n_narrow, n_bare, n_tall, n_big, reserved, n_mid, n_mid_wide, mid_all;
   const void* device_copy;     /* 16-byte aligned */
 } spec_lora_plan;
 int64_t spec_lora_plan_bytes(int64_t n_rows);

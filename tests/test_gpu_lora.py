@@ -249,8 +249,8 @@ def test_far_strides(pkg):
     torch.cuda.empty_cache()
 
 
-def test_the_result_does_not_depend_on_other_adapters(pkg):
-    """Rows of an adapter give the same bits with and without other requests in the step."""
+def test_two_calls_give_the_same_bits(pkg):
+    """Units of two sizes in one call, twice."""
     import torch
     c = Case(pkg, [0] * 5 + [1] * 40, 2, 512, 384, 16, seed=9)
     both = torch.empty_like(c.y)
@@ -305,3 +305,17 @@ def test_refusals(pkg):
     c.bank.apply(pkg.LoraPlan([], 2), x[:0], y[:0])
     c.bank.apply(pkg.LoraPlan([-1] * 3, 2), x, y)
     assert torch.equal(y, keep)
+
+
+# Runs of rows that units of 8 and larger ones can take: by the bank's and the rows' bytes.
+@pytest.mark.parametrize("dtype,x,y", [("bf16", "same", "same"), ("bf16", "f32", "f32"), ("f16", "same", "f32")])
+@pytest.mark.parametrize("k,n,rank", [(2048, 96, 64), (64, 1000, 16), (520, 264, 128)])
+@pytest.mark.parametrize("runs,none", [((24, 40, 9, 64), 5), ((17, 300), 0), ((33,) * 40, 3), ((889,), 1), ((700, 100), 0)])
+def test_runs_that_two_kernels_take(pkg, runs, none, k, n, rank, dtype, x, y):
+    import torch
+    ids = np.repeat(np.arange(len(runs) + 1) - 1, (none,) + runs)
+    ids = np.random.default_rng(5).permutation(ids)
+    c = Case(pkg, ids, len(runs), k, n, rank, dtype, x=x, y=y, seed=7, pad=(8, 8, 8, 8))
+    out = torch.empty_like(c.y)
+    g = c.check(out)
+    assert (c.check() == g).all()  # in place, the rows without an adapter as they are

@@ -45,6 +45,33 @@ def test_every_row_is_in_one_unit_of_its_adapter(mod, n, adapters, seed):
     assert (buf[52 * n:] == 0).all()
 
 
+@pytest.mark.parametrize("runs", [(24, 20, 30), (256,), (64, 17, 3), (880,), (900,), (24,) * 60, (200,) + (40,) * 40, (17,) * 37,
+                                  (16,) * 30, (5, 70)])
+def test_rows_that_units_of_eight_can_take_too(mod, runs):
+    ids = np.random.default_rng(0).permutation(np.repeat(np.arange(len(runs)), runs))
+    rc, plan, buf = make(mod, ids, len(runs))
+    n = ids.size
+    order = buf[48 * n:52 * n].view(np.int32)
+    main = plan.n_tall + plan.n_big + plan.n_wide + plan.n_narrow + plan.n_bare
+    assert rc == 0 and main + plan.n_mid <= n and 0 <= plan.n_mid_wide <= plan.n_wide
+    units = buf[:48 * n].view(np.int32).reshape(-1, 12)
+
+    def rows_of(part, most):
+        out = []
+        for a, first, count, _, *near in part:
+            rows = order[first:first + count]
+            assert 0 < count <= most and a >= 0 and (ids[rows] == a).all() and near[:min(count, 8)] == rows[:8].tolist()
+            out += rows.tolist()
+        return sorted(out)
+
+    mid = rows_of(units[main:main + plan.n_mid], 8)
+    wide_end = plan.n_tall + plan.n_big + plan.n_wide
+    replaced = units[plan.n_tall:wide_end] if plan.mid_all else units[wide_end - plan.n_mid_wide:wide_end]
+    assert mid == rows_of(replaced, 64)
+    few = sum((r + 7) // 8 for r in runs) <= 111
+    assert bool(plan.mid_all) == few and (not few or len(mid) == sum(r for r in runs if r > 16))
+
+
 def test_empty_plans(mod):
     rc, plan, _ = make(mod, [], 3)
     assert rc == 0 and plan.n_wide == plan.n_narrow == plan.n_bare == 0
@@ -85,7 +112,7 @@ def test_bad_calls_are_refused(mod):
     for change in (dict(dtype=2), dict(dtype=-1), dict(rank=129), dict(rank=-1)):
         assert call(bank=change) == 3, change
     for change in (dict(n_rows=-1), dict(n_narrow=-1), dict(n_wide=-1), dict(n_bare=-1), dict(n_narrow=3), dict(n_wide=2), dict(n_tall=-1), dict(n_tall=2), dict(n_big=-1), dict(device_copy=None), dict(device_copy=P + 8),
-                   dict(n_rows=(1 << 20) + 1)):
+                   dict(n_rows=(1 << 20) + 1), dict(n_mid=-1), dict(n_mid=2), dict(n_mid_wide=-1), dict(n_mid_wide=1)):
         assert call(plan=change) == 1, change
     for which in ("x", "y", "out"):
         for change in (dict(ptr=None), dict(ptr=P + 1), dict(n_rows=2), dict(row_stride=-1), dict(row_stride=1 << 41)):
