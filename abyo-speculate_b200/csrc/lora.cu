@@ -18,6 +18,10 @@
 // for the second product it is split into bf16 numbers (three, 24 bits, for an
 // f32 result; two, 16 bits, for a bf16 one, which itself has 8), or two f16
 // numbers of t 2^-e, 2^e about the row's largest (22 bits).  All sums are f32.
+//
+// Bound by latency: 64 rows of 64 adapters of rank 32 and less, 3584 to 18944 in f16
+// with f32 results, 26 us of which 40 MB take 6 at the copy rate; 21 warps an SM read A, then B, in turn.
+// Stages of 32 columns and three blocks an SM (80 registers) took 30 to 26 us.
 #include "lora_mma.cuh"
 
 namespace specb200 {

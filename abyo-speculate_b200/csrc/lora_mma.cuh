@@ -1,4 +1,4 @@
-// What the two kernels of the low-rank adapters share: products on mma.sync from
+// What the kernels of the low-rank adapters share: products on mma.sync from
 // 16-byte pieces, parts that f32 numbers are split into, and clusters.
 //
 // A product's sum may run in any order, so a lane takes 8 consecutive elements of
