@@ -116,6 +116,18 @@ def test_sample_next_to_borders(pkg):
     check_sample(pkg, x.expand(len(u), v).contiguous(), np.repeat(host, len(u), 0), u, 1.0, want_probs=False)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v,spread,t", [(50001, 2.0, 0.7), (50001, 0.3, 1.0), (128256, 4.0, 1.0), (4096, 1.0, 0.3)])
+def test_sample_around_borders(pkg, v, spread, t, dtype):
+    """Uniforms from 2^-24 to 2^-16 off a cumulative weight, where f32 sums begin to decide."""
+    x, host = rows(1, v, dtype, seed=v % 11, spread=spread)
+    c = np.cumsum(ref.probs(host[0], t))
+    p = np.diff(c, prepend=0.0)
+    at = np.unique(np.concatenate([np.argsort(-p)[:6], np.searchsorted(c, [0.01, 0.1, 0.5, 0.9, 0.99])]))
+    u = np.concatenate([c[at] + s * 2.0 ** -e for s in (-1, 1) for e in range(16, 25)]).astype(np.float32)
+    check_sample(pkg, x.expand(len(u), v), np.broadcast_to(host, (len(u), v)), u, t, want_probs=False)
+
+
 def test_sample_flat_rows_and_odd_uniforms(pkg):
     """A flat distribution, where f32 sums decide little; uniforms at and outside the ends."""
     x, host = rows(12, 50001, "f32", seed=11, spread=0.05, hot=0)
@@ -230,6 +242,24 @@ def test_chain_at_the_border(pkg):
         u[r] = [near, np.nextafter(near, np.float32(0)), np.nextafter(near, np.float32(2))][r // 2 % 3]
         u[r + 1] = 0.37
     check_chain(pkg, x, host, t, q, drafts, u, start)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("noise", [0.05, 1.5])
+def test_chain_around_borders_of_the_rest(pkg, noise, dtype):
+    """Rejected drafts; the next uniform 2^-24 to 2^-12 off a cumulative weight of max(p - q, 0)."""
+    v, n = 20000, 128
+    x, host, t, q, drafts, start = chains([2] * (n // 2), v, dtype, seed=13, noise=noise)
+    u = np.ones(n, np.float32)
+    for i, r in enumerate(range(0, n, 2)):
+        p = ref.probs(host[r], t[r])
+        drafts[r] = int(np.argmax(q[r] - p))
+        rest = np.fmax(p - q[r].astype(np.float64), 0.0)
+        c = np.cumsum(rest) / rest.sum()
+        k = np.argsort(-rest)[i % 7] if i % 2 else np.searchsorted(c, (i + 0.5) / (n // 2))
+        u[r + 1] = np.clip(c[k] + (-1) ** (i // 2) * 2.0 ** -(12 + i % 13), 0, 1)
+    want = check_chain(pkg, x, host, t, q, drafts, u, start)
+    assert all(k == 0 for k, _ in want)
 
 
 def test_chain_draft_equal_to_the_target(pkg):
