@@ -319,3 +319,24 @@ def test_runs_that_two_kernels_take(pkg, runs, none, k, n, rank, dtype, x, y):
     out = torch.empty_like(c.y)
     g = c.check(out)
     assert (c.check() == g).all()  # in place, the rows without an adapter as they are
+
+
+def test_one_plan_on_two_streams_at_once(pkg):
+    """A plan and a bank used on two streams at a time, and dropped while their calls may still run."""
+    import torch
+    ids = mixed(200, 6, seed=11)
+    c = Case(pkg, ids, 6, 1024, 2048, 16, seed=12)
+    xs = [torch.randn_like(c.x) for _ in range(8)]
+    want = [c.bank.apply(c.plan, x, c.y, out=torch.empty_like(c.y)) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [torch.empty_like(c.y) for _ in xs]
+    plan, bank = c.plan, c.bank
+    del c.plan, c.bank
+    for i, (x, out) in enumerate(zip(xs, outs)):
+        with torch.cuda.stream(streams[i % 2]):
+            bank.apply(plan, x, c.y, out=out)
+    del plan, bank
+    junk = [torch.full((1 << 16,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want)) and junk
