@@ -21,13 +21,13 @@ constexpr int kPlanRows = 1 << 20;
 //   (a / b) in units of 32;
 // - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows 16.9 / 37 /
 //   38, 21.6 / 53 / 44 in units of 32; one of 256 8.9 / 21 / 21, 10.8 / 26 / 31.  For
-//   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are too
-//   many: 24 of 64 31 / 66 / 69, 33 / 90 / 82 in units of 64.  Not where A and B, read
+//   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are more
+//   than kHalvesMost: 24 of 64 31 / 66 / 69, 31 / 88 / 80 in units of 32.  Not where A and B, read
 //   again for every 8 rows, are more than kAgainMost times the rows (known when the
 //   plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
-// - units of 32 rows, not 64, for up to kHalvesMost of them: 4 of 64 11 / 26, 15 / 43; 24
-//   of 64 31 / 88, 33 / 90;
-// - units of 128, not 64, from kTallFrom of them on: 4 of them 21 / 28, 20.5 / 31 (8192
+//   (of 64 rows, which read A and B half as often, 16 of 128 took 42 / 130 / 96, 42 / 89
+//   / 88 of 32: half of the warps share K then, and half of the blocks are there);
+// - units of 128, not 32, of more than kTallMin rows, from kTallFrom of them on: 4 of them 21 / 28, 20.5 / 31 (8192
 //   to 2048 in bf16 for b), 8 of them 21 / 28, 31 / 49.
 constexpr int kNarrowMost = 16;
 constexpr int kFewUnits = 111;   // four blocks a cluster, three an SM
@@ -35,9 +35,12 @@ constexpr int kSomeUnits = 222;  // two
 constexpr int kAgainMost = 4;
 constexpr int kHalvesMost = 36;  // as many clusters of 8 blocks as a B200 holds, two an SM
 constexpr int kTallFrom = 5;
+constexpr int kTallMin = 64;
 
-// Layout of a plan: units (of adapters of very many rows by 128, the same by 64,
-// those of other adapters of many rows, those of few, rows without one), then the rows in their order, then the word of the device's waits.
+// Layout of a plan: units (of adapters of very many rows by 128, the same by 32,
+// those of other adapters of many rows, those of few, rows without one, rows of the
+// second and third kind by 8), then the rows in their order, then the word of the
+// device's waits.
 int64_t plan_bytes(int64_t n_rows) { return n_rows * (int64_t)(sizeof(Unit) + sizeof(int)) + 16; }
 
 struct Matrix {
@@ -97,14 +100,13 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
     runs.push_back(Run{adapters[order[i]], i, e});
     const int64_t n = adapters[order[i]] >= 0 ? (e - i + kNarrowRows - 1) / kNarrowRows : 0;
     eighths += n;
-    if (e - i <= kWideRows) near += n;
+    if (e - i <= kTallMin) near += n;
     if (adapters[order[i]] >= 0 && e - i > kNarrowMost) {
-      halves += (e - i + kWideRows / 2 - 1) / (kWideRows / 2);
-      if (e - i > kWideRows) tall += (e - i + kTallRows - 1) / kTallRows;
+      halves += (e - i + kWideRows - 1) / kWideRows;
+      if (e - i > kTallMin) tall += (e - i + kTallRows - 1) / kTallRows;
     }
     i = e;
   }
-  const int wide_rows = halves <= kHalvesMost ? kWideRows / 2 : kWideRows;
   const bool few = eighths <= kFewUnits, some = few || (halves > kHalvesMost && near <= kSomeUnits);
   std::vector<Unit> units[5], mid_wide, mid;
   auto cut = [&](std::vector<Unit>& to, const Run& r, int most) {
@@ -118,12 +120,12 @@ int make_plan(const char* what, const int32_t* adapters, int n_rows, int n_adapt
   };
   for (const Run& r : runs) {
     const int rows = r.end - r.begin;
-    const bool big = r.adapter >= 0 && rows > kWideRows && tall >= kTallFrom;
+    const bool big = r.adapter >= 0 && rows > kTallMin && tall >= kTallFrom;
     if (big) cut(units[0], r, kTallRows);
     if (r.adapter < 0) cut(units[4], r, 1);
     else if (rows <= kNarrowMost) cut(units[3], r, kNarrowRows);
-    else if (few || (some && rows <= kWideRows)) cut(big ? units[1] : mid_wide, r, wide_rows), cut(mid, r, kNarrowRows);
-    else cut(units[big ? 1 : 2], r, wide_rows);
+    else if (few || (some && rows <= kTallMin)) cut(big ? units[1] : mid_wide, r, kWideRows), cut(mid, r, kNarrowRows);
+    else cut(units[big ? 1 : 2], r, kWideRows);
   }
   units[2].insert(units[2].end(), mid_wide.begin(), mid_wide.end());
   uint8_t* b = static_cast<uint8_t*>(buf);

@@ -12,7 +12,7 @@ enum : int { T_BF16 = 0, T_F16 = 1, T_F32 = 2 };
 
 constexpr int kMaxRank = 128;
 constexpr int kNarrowRows = 8;  // rows of a unit of the kernel for few rows: one n-tile of the products
-constexpr int kWideRows = 64;   // of the one for many
+constexpr int kWideRows = 32;   // of the one for many
 constexpr int kTallRows = 128;  // and of the one for very many
 
 // Rows of one adapter (-1: none) that one cluster takes.

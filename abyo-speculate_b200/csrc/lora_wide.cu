@@ -1,13 +1,12 @@
 // Low-rank adapters, many rows of one adapter: out = y + s (x A^T) B^T for up to
-// 64 rows a cluster of blocks.
+// 32 rows a cluster of blocks.
 //
-// First product, T [64 x r] = X [64 x K] A^T: the blocks of a cluster share K, and
-// the warps of a block share its rows (32 each), the ranks (8 NT each) and its
-// columns, 128 bytes of a row at a time.  Every warp copies what it needs
+// First product, T [32 x r] = X [32 x K] A^T: the blocks of a cluster share K, and
+// the warps of a block share the ranks (8 NT each) and its columns, 128 bytes of a row at a time.  Every warp copies what it needs
 // asynchronously into a ring of its own and waits for nobody else; the warps add
 // up at the end.  The blocks' parts meet in distributed shared memory, each adding up
 // a slice of T and all of them collecting the slices.  Second product, Y += T
-// B^T: the blocks share N, the warps rows and columns, 32 of each; T's parts are the
+// B^T: the blocks share N, the warps columns, 32 at a time; T's parts are the
 // 16-row operand, from shared memory, B and y come straight to registers a tile
 // ahead, and B's columns are taken in an order that leaves a lane with 16 bytes of
 // its rows next to its neighbour's.  Up to 16 ranks a lane takes 4 of B, not 8 with
@@ -121,10 +120,10 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   const int r = p.ranks ? min(max(p.ranks[u.adapter], 0), p.rank) : p.rank;
   const T* A = static_cast<const T*>(p.a) + u.adapter * p.a_adapter;
   const T* B = static_cast<const T*>(p.b) + u.adapter * p.b_adapter;
-  // Warps: row groups of 32, rank blocks of 8 NT, and the rest takes columns in turn.
-  const int groups = (n_rows + 31) / 32, blocks = max((r + 8 * NT - 1) / (8 * NT), 1), turns = kWarps / (groups * blocks);
+  // Warps: rank blocks of 8 NT, and the rest takes columns in turn.
+  const int blocks = max((r + 8 * NT - 1) / (8 * NT), 1), turns = kWarps / blocks;
   const int W = blocks * 8 * NT;  // columns of T
-  const int mg = warp % groups, nb = warp / groups % blocks, kg = warp / (groups * blocks);
+  const int nb = warp % blocks, kg = warp / blocks;
 
   // ---- T ----
   float d[2][NT][4] = {};
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     __syncthreads();
     // Rows behind the last one are copies of it, T's columns behind the adapter's
     // rank whatever the memory holds: neither is used.
-    const TX* const* xp = reinterpret_cast<const TX* const*>(s_row) + mg * 32 + lane / 8;
+    const TX* const* xp = reinterpret_cast<const TX* const*>(s_row) + lane / 8;
     constexpr int AP = C / 8, AR = 32 / AP;  // 16-byte pieces of a rank's columns; ranks a pass
     const int ranks = min(r - nb * NT * 8, NT * 8);
     const T* ap = A + (nb * NT * 8 + lane / AP) * p.a_row + k0 + lane % AP * 8;
@@ -237,13 +236,13 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   // numbers that T is split into.
   float* part = reinterpret_cast<float*>(smem);
   float* all = reinterpret_cast<float*>(smem + kWideRows * RA * 6);
-  const int live = groups * 32 * W;
+  const int live = kWideRows * W;
   if (kg < turns) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float* o = part + kg * live + (mg * 32 + m * 16 + g) * W + nb * NT * 8 + n * 8 + 2 * t;
+        float* o = part + kg * live + (m * 16 + g) * W + nb * NT * 8 + n * 8 + 2 * t;
         *reinterpret_cast<float2*>(o) = make_float2(d[m][n][0], d[m][n][1]);
         *reinterpret_cast<float2*>(o + 8 * W) = make_float2(d[m][n][2], d[m][n][3]);
       }
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   }
   __syncthreads();
   const int steps = (r + 31) / 32, frag = kWideRows * 64;  // bytes of one part's 32 ranks
-  if (threadIdx.x < groups * 32 * 4) {                 // four threads a row
+  if (threadIdx.x < kWideRows * 4) {                 // four threads a row
     const int row = threadIdx.x / 4, c = threadIdx.x % 4;
     const float scale = p.scales ? p.scales[u.adapter] : 1.f;
     float top = 0.f;
@@ -320,7 +319,6 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   // ---- Y ----
   {
     constexpr int V = (int)sizeof(TY) / 2;  // 16-byte pieces of 8 columns
-    const int ways = kWarps / groups, ng = warp / groups, first = mg * 32 + g;
     const bool half = r <= 16, cut = r % (half ? 4 : 8) != 0, b_fast = p.b_wide && p.rank % 8 == 0;
     const int per = half ? 4 : 8;  // ranks a lane takes of a step
     const TY* yp[4];
@@ -328,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     float factor[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = first + i * 8, at = rows[min(row, n_rows - 1)];
+      const int row = g + i * 8, at = rows[min(row, n_rows - 1)];
       yp[i] = static_cast<const TY*>(p.y) + at * p.y_row + n0;
       op[i] = row < n_rows ? static_cast<TY*>(p.out) + at * p.out_row + n0 : nullptr;
       factor[i] = s_factor[row];
@@ -372,11 +370,11 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
         }
       }
     };
-    const int begin = ng < ways ? ng * 32 : width;
+    const int begin = warp * 32;
     load_b(begin, 0);
     load_y(begin);
 #pragma unroll 1
-    for (int n = begin; n < width; n += ways * 32) {
+    for (int n = begin; n < width; n += kWarps * 32) {
       float d2[2][4][4] = {};
 #pragma unroll 1
       for (int s = 0; s < steps; ++s) {
@@ -386,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
         }
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-          const uint8_t* f = smem + (q * steps + s) * frag + first * 64 + per * 2 * t;
+          const uint8_t* f = smem + (q * steps + s) * frag + g * 64 + per * 2 * t;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             if (half) {
@@ -403,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
           }
         }
         if (s + 1 < steps) load_b(n, s + 1);
-        else load_b(n + ways * 32, 0);
+        else load_b(n + kWarps * 32, 0);
       }
       const bool whole = p.out_wide && n + 32 <= width;
 #pragma unroll
@@ -440,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
           if (whole) *reinterpret_cast<uint4*>(op[i] + c) = y[i][h];
           else store_piece(op[i], c, width, y[i][h]);
         }
-      load_y(n + ways * 32);
+      load_y(n + kWarps * 32);
     }
   }
 }
@@ -450,10 +448,11 @@ cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s)
   constexpr int B = 8 * NT, kSlot = 2 * kArea + (sizeof(TX) == 4 ? 1 : 2) * area(B);
   WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0, 0};
   const int steps = (w.RA + 31) / 32;
-  // Two blocks an SM where there are that many.  At least: two slots a warp; the
+  // Two blocks an SM where there are many: alone on an SM, clusters of 8 leave part of
+  // a GPC's SMs empty (16 of them, one an SM: 20 us, two 11).  At least: two slots a warp; the
   // warps' parts of T, 32 rows and a block of ranks each; T whole behind the
   // numbers that it is split into.
-  int bytes = (long long)n_units * size > sms ? 112 * 1024 : 224 * 1024;
+  int bytes = (long long)n_units * size * 2 > sms ? 112 * 1024 : 224 * 1024;
   for (const int need : {kWarps * 2 * kSlot, kWarps * 32 * B * 4, kWideRows * w.RA * 10, 3 * steps * kWideRows * 64})
     if (bytes < need) bytes = need;
   w.ring = bytes / kWarps / 16 * 16;
