@@ -2,7 +2,7 @@
 // 32 rows a cluster of blocks.
 //
 // First product, T [32 x r] = X [32 x K] A^T: the blocks of a cluster share K, and
-// the warps of a block share the ranks (8 NT each) and its columns, 128 bytes of a row at a time.  Every warp copies what it needs
+// the warps of a block share the ranks (8 NT each) and its columns, 32 at a time.  Every warp copies what it needs
 // asynchronously into a ring of its own and waits for nobody else; the warps add
 // up at the end.  The blocks' parts meet in distributed shared memory, each adding up
 // a slice of T and all of them collecting the slices.  Second product, Y += T
@@ -128,15 +128,15 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
   // ---- T ----
   float d[2][NT][4] = {};
   {
-    constexpr int C = 128 / (int)sizeof(TX), S = C / 32;  // columns of a piece of work; slices of 32 in it
-    constexpr int kSlot = 2 * kArea + S * area(8 * NT);
+    constexpr int C = 32, XP = C * (int)sizeof(TX) / 16, XR = 32 / XP;  // columns of a piece of work; 16-byte pieces of a row; rows a pass
+    constexpr int XA = XP / 4 * kArea, kSlot = XA + area(8 * NT);
     const int k_per = (p.K + size * C - 1) / (size * C) * C, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K), length = k1 - k0;
     if (threadIdx.x < kWideRows)
       s_row[threadIdx.x] = static_cast<const TX*>(p.x) + rows[min((int)threadIdx.x, n_rows - 1)] * p.x_row + k0;
     __syncthreads();
     // Rows behind the last one are copies of it, T's columns behind the adapter's
     // rank whatever the memory holds: neither is used.
-    const TX* const* xp = reinterpret_cast<const TX* const*>(s_row) + lane / 8;
+    const TX* const* xp = reinterpret_cast<const TX* const*>(s_row) + lane / XP;
     constexpr int AP = C / 8, AR = 32 / AP;  // 16-byte pieces of a rank's columns; ranks a pass
     const int ranks = min(r - nb * NT * 8, NT * 8);
     const T* ap = A + (nb * NT * 8 + lane / AP) * p.a_row + k0 + lane % AP * 8;
@@ -146,19 +146,19 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     int next = kg < turns && r ? kg * C : length, at = 0;  // the next to fetch: its first column, its slot
     auto fetch = [&]() {
       if (next < length) {
-        uint8_t* to = ring + at + piece_at<TX>(lane % 8) + lane / 8 * 64;
-        const int xk = next + lane % 8 * (16 / (int)sizeof(TX));
-        uint8_t* ta = ring + at + 2 * kArea + lane % AP / 4 * area(8 * NT) + lane % 4 * 16 + lane / AP * 64;
+        uint8_t* to = ring + at + piece_at<TX>(lane % XP) + lane / XP * 64;
+        const int xk = next + lane % XP * (16 / (int)sizeof(TX));
+        uint8_t* ta = ring + at + XA + lane % AP * 16 + lane / AP * 64;
         const T* a = ap + next;
         if (fast && next + C <= length) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) cp_async16(to + i * 256, xp[i * 4] + xk);
+          for (int i = 0; i < XP; ++i) cp_async16(to + i * XR * 64, xp[i * XR] + xk);
 #pragma unroll
           for (int i = 0; i < NT * 8 / AR; ++i)
             if (lane / AP + i * AR < ranks) cp_async16(ta + i * AR * 64, a + i * AR * p.a_row);
         } else {
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) copy16(to + i * 256, xp[i * 4] + xk, length - xk, p.x_wide);
+          for (int i = 0; i < XP; ++i) copy16(to + i * XR * 64, xp[i * XR] + xk, length - xk, p.x_wide);
 #pragma unroll 1
           for (int i = 0; i < NT * 8 / AR; ++i)
             if (lane / AP + i * AR < ranks) copy16(ta + i * AR * 64, a + i * AR * p.a_row, length - next - lane % AP * 8, p.a_wide);
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
       cp_async_wait_for(slots - 2);
       __syncwarp();
       fetch();
-      const uint8_t *xb = st + g * 64 + t * 16, *ab = st + 2 * kArea + g * 64 + t * 16;
+      const uint8_t *xb = st + g * 64 + t * 16, *ab = st + XA + g * 64 + t * 16;
       if constexpr (kSplitX) {
 #pragma unroll
         for (int n0 = 0; n0 < NT; n0 += 4) {  // four rank tiles at a time
@@ -207,20 +207,16 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
           }
         }
       } else {
+        uint4 x[2][2];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          uint4 x[2][2];
+        for (int m = 0; m < 2; ++m) x[m][0] = lds128(xb + m * 1024), x[m][1] = lds128(xb + m * 1024 + 512);
 #pragma unroll
-          for (int m = 0; m < 2; ++m)
-            x[m][0] = lds128(xb + s * kArea + m * 1024), x[m][1] = lds128(xb + s * kArea + m * 1024 + 512);
+        for (int n = 0; n < NT; ++n) {
+          const uint4 a = lds128(ab + n * 512);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 a = lds128(ab + s * area(8 * NT) + n * 512);
+          for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
-          }
+          for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
         }
       }
       __syncwarp();
@@ -445,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 
 template <class T, class TX, class TY, int NT>
 cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s) {
-  constexpr int B = 8 * NT, kSlot = 2 * kArea + (sizeof(TX) == 4 ? 1 : 2) * area(B);
+  constexpr int B = 8 * NT, kSlot = (int)sizeof(TX) / 2 * kArea + area(B);
   WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0, 0};
   const int steps = (w.RA + 31) / 32;
   // Two blocks an SM where there are many: alone on an SM, clusters of 8 leave part of
