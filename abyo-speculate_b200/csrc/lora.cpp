@@ -22,7 +22,7 @@ constexpr int kPlanRows = 1 << 20;
 // - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows 16.9 / 37 /
 //   38, 21.6 / 53 / 44 in units of 32; one of 256 8.9 / 21 / 21, 10.8 / 26 / 31.  For
 //   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are more
-//   than kHalvesMost: 24 of 64 31 / 66 / 69, 31 / 88 / 80 in units of 32.  Not where A and B, read
+//   than kHalvesMost and x is f32: 24 of 48 30 / 65 / 67, 20 / 78 / 75 in units of 32.  Not where A and B, read
 //   again for every 8 rows, are more than kAgainMost times the rows (known when the
 //   plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
 //   (of 64 rows, which read A and B half as often, 16 of 128 took 42 / 130 / 96, 42 / 89
@@ -254,7 +254,7 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Rows that units of 8 can take as well: do they?
-  const bool mid = plan->n_mid && (int64_t)b->rank * (b->k + b->n) * 2 <= (int64_t)kAgainMost * kNarrowRows *
+  const bool mid = plan->n_mid && (plan->mid_all || x_f32) && (int64_t)b->rank * (b->k + b->n) * 2 <= (int64_t)kAgainMost * kNarrowRows *
                                       (b->k * (x_f32 ? 4LL : 2LL) + 2 * b->n * (y_f32 ? 4LL : 2LL));
   const bool rest = !(mid && plan->mid_all);  // there are others
   bool taken = false;

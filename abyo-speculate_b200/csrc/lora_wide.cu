@@ -317,14 +317,14 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
     constexpr int V = (int)sizeof(TY) / 2;  // 16-byte pieces of 8 columns
     const bool half = r <= 16, cut = r % (half ? 4 : 8) != 0, b_fast = p.b_wide && p.rank % 8 == 0;
     const int per = half ? 4 : 8;  // ranks a lane takes of a step
-    const TY* yp[4];
-    TY* op[4];
+    const TY* y0 = static_cast<const TY*>(p.y) + n0;
+    TY* out0 = static_cast<TY*>(p.out) + n0;
+    int at[4];  // the lane's rows, -1: none
     float factor[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = g + i * 8, at = rows[min(row, n_rows - 1)];
-      yp[i] = static_cast<const TY*>(p.y) + at * p.y_row + n0;
-      op[i] = row < n_rows ? static_cast<TY*>(p.out) + at * p.out_row + n0 : nullptr;
+      const int row = g + i * 8;
+      at[i] = row < n_rows ? rows[row] : -1;
       factor[i] = s_factor[row];
     }
     // Where a lane's 8 columns of a row lie: 8 t .. (16-bit), or 4 t .. and 16 + 4 t .. (f32);
@@ -340,14 +340,14 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            if (op[i]) y[i][v] = *reinterpret_cast<const uint4*>(yp[i] + n + (V == 2 ? 16 * v + 4 * t : 8 * t));
+            if (at[i] >= 0) y[i][v] = *reinterpret_cast<const uint4*>(y0 + at[i] * p.y_row + n + (V == 2 ? 16 * v + 4 * t : 8 * t));
         return;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          if (op[i]) y[i][v] = load_piece(yp[i], n + (V == 2 ? 16 * v + 4 * t : 8 * t), width);
+          if (at[i] >= 0) y[i][v] = load_piece(y0 + at[i] * p.y_row, n + (V == 2 ? 16 * v + 4 * t : 8 * t), width);
     };
     auto load_b = [&](int n, int s) {
       const int k = s * 32 + per * t;
@@ -430,9 +430,10 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 #pragma unroll
         for (int h = 0; h < V; ++h) {
           const int c = n + (V == 2 ? 16 * h + 4 * t : 8 * t);
-          if (!op[i]) continue;
-          if (whole) *reinterpret_cast<uint4*>(op[i] + c) = y[i][h];
-          else store_piece(op[i], c, width, y[i][h]);
+          if (at[i] < 0) continue;
+          TY* o = out0 + at[i] * p.out_row;
+          if (whole) *reinterpret_cast<uint4*>(o + c) = y[i][h];
+          else store_piece(o, c, width, y[i][h]);
         }
       load_y(n + kWarps * 32);
     }
