@@ -22,13 +22,13 @@ constexpr int kPlanRows = 1 << 20;
 // - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows 16.9 / 37 /
 //   38, 21.6 / 53 / 44 in units of 32; one of 256 8.9 / 21 / 21, 10.8 / 26 / 31.  For
 //   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are more
-//   than kHalvesMost and x is f32: 24 of 48 30 / 65 / 67, 20 / 78 / 75 in units of 32.  Not where A and B, read
-//   again for every 8 rows, are more than kAgainMost times the rows (known when the
-//   plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
+//   than kHalvesMost and x is f32: 24 of 48 30 / 65 / 67, 20 / 78 / 75 in units of 32.
+//   Not where A and B, read again for every 8 rows, are more than kAgainMost times
+//   the rows (known when the plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
 //   (of 64 rows, which read A and B half as often, 16 of 128 took 42 / 130 / 96, 42 / 89
 //   / 88 of 32: half of the warps share K then, and half of the blocks are there);
-// - units of 128, not 32, of more than kTallMin rows, from kTallFrom of them on: 4 of them 21 / 28, 20.5 / 31 (8192
-//   to 2048 in bf16 for b), 8 of them 21 / 28, 31 / 49.
+// - units of 128, not 32, of more than kTallMin rows, from kTallFrom of them on: 4 of
+//   them 21 / 28, 20.5 / 31 (8192 to 2048 in bf16 for b), 8 of them 21 / 28, 31 / 49.
 constexpr int kNarrowMost = 16;
 constexpr int kFewUnits = 111;   // four blocks a cluster, three an SM
 constexpr int kSomeUnits = 222;  // two

@@ -18,8 +18,8 @@
 // halves, 16-byte pieces in turn.
 //
 // Bound by latency: 24 requests of 5 to 60 f32 rows (870 in all), rank 16, 4096 to
-// 14336: 49 us, 18 at the copy rate.  x A^T takes 11, its join 4, the rest moves y
-// at 4.5 TB/s; 64 when y and B came through the warps' rings as well.
+// 14336: 48 to 56 us, 18 at the copy rate.  x A^T takes 11, its join 4, the rest moves
+// y at 4 TB/s; 64 when y and B came through the warps' rings as well.
 #include "lora_mma.cuh"
 
 namespace specb200 {
