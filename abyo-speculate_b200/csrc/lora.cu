@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
     const TX* x = static_cast<const TX*>(p.x) + (g < u.n_rows ? rows[g] : 0) * p.x_row;
     const int part = tiles ? warp / tiles : 0;
     for (int tile = tiles ? warp % tiles : 0; tile < tiles && part < kparts; tile += kWarps) {
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
       const int j0 = tile * 16 + g, j1 = j0 + 8;
       const T *a0 = A + j0 * p.a_row, *a1 = A + j1 * p.a_row;
 #pragma unroll 4
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
         const int at = k + 8 * t;
         const uint4 v0 = load8(a0, at, j0 < r ? k1 : 0, p.a_wide), v1 = load8(a1, at, j1 < r ? k1 : 0, p.a_wide);
         const int end = g < u.n_rows ? k1 : 0;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
         if constexpr (kSplitX) {
           float f0[8], f1[8], xv[8];
           widen(v0, f0, A);
@@ -160,20 +161,22 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
             const uint32_t l0 = tf32(rest(xv[i], h0)), l1 = tf32(rest(xv[i + 1], h1));
             const uint32_t w0 = __float_as_uint(f0[i]), w1 = __float_as_uint(f1[i]);
             const uint32_t w2 = __float_as_uint(f0[i + 1]), w3 = __float_as_uint(f1[i + 1]);
-            mma8(d, w0, w1, w2, w3, h0, h1);
             mma8(d, w0, w1, w2, w3, l0, l1);
+            mma8(d, w0, w1, w2, w3, h0, h1);
           }
         } else {
           const uint4 xv = load8(reinterpret_cast<const T*>(x), at, end, p.x_wide);
           mma16(d, v0.x, v1.x, v0.y, v1.y, xv.x, xv.y, A);
           mma16(d, v0.z, v1.z, v0.w, v1.w, xv.z, xv.w, A);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += d[i];
       }
       float* o = sm.part + (part * tiles + tile) * (kNarrowRows * 16);
-      o[2 * t * 16 + g] = d[0];
-      o[(2 * t + 1) * 16 + g] = d[1];
-      o[2 * t * 16 + g + 8] = d[2];
-      o[(2 * t + 1) * 16 + g + 8] = d[3];
+      o[2 * t * 16 + g] = sum[0];
+      o[(2 * t + 1) * 16 + g] = sum[1];
+      o[2 * t * 16 + g + 8] = sum[2];
+      o[(2 * t + 1) * 16 + g + 8] = sum[3];
     }
   }
   __syncthreads();
@@ -254,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
         for (int j = 0; j < 4; ++j) v[j] = first_of(v[j], r - s * 32 - 8 * t);
       }
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
+      for (int q = P - 1; q >= 0; --q) {
         const uint4 f = *reinterpret_cast<const uint4*>(&sm.frag[q][s][lane * 8]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) mma16(d[j], v[2 * j].x, v[2 * j + 1].x, v[2 * j].y, v[2 * j + 1].y, f.x, f.y, A);

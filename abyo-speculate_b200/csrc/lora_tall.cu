@@ -5,15 +5,18 @@
 // 16): the blocks of a cluster share K; stages of 128 columns of the rows and of A
 // are copied asynchronously into the K-major operand layout of 128-byte rows
 // whose 16-byte pieces are swizzled (piece c of row i lies at c ^ (i % 8)), so that
-// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products.  The blocks'
+// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products.
+// An accumulator adds up two stages, two accumulators in turn, and goes from there to
+// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 135 us;
+// one stage 2.5e-7 and 4 us longer; all of them 83e-7 and 6 us less).  The blocks'
 // parts join as in the kernel for fewer rows.  Second product: T's parts are the
 // 128-row operand, B's 64 columns a stage the other; while a stage's products
 // run, all threads add the stage before it to y, which came with B into rows 16
 // bytes further apart than they are long, and store it along the rows.
 //
-// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 128
-// us (55 at the copy rate), about 73 of them the first product, which brings 350 MB of x and
-// A at 4.8 TB/s, bound by the copies' 16-byte pieces in the load units; in the
+// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 135
+// us (55 at the copy rate), about 79 of them the first product, which brings 350 MB of x and
+// A at 4.4 TB/s, bound by the copies' 16-byte pieces in the load units; in the
 // second, 133 MB of y and out and the load units again.  On mma.sync 146 us.
 #include "lora_mma.cuh"
 
@@ -25,6 +28,7 @@ constexpr int kTallThreads = 512, kTallWarps = kTallThreads / 32;
 constexpr int kStep = 128;        // columns of a stage of the first product
 constexpr int kCols = 64;         // and of the second
 constexpr int kMaxStages = 6;
+constexpr int kChain = 2;         // stages that one accumulator adds up
 constexpr int kTmem = 256;        // columns: T, and two accumulators of the second product from 128 on
 
 struct TallParams {
@@ -62,6 +66,13 @@ SPEC_DEV void cp_async_wait_for(int n) {
     case 3: cp_async_wait<3>(); break;
     default: cp_async_wait<4>(); break;
   }
+}
+// 8 columns of tensor memory of this thread's row, there after tmem_wait_ld.
+SPEC_DEV void tmem_ld8(uint32_t at, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(at)
+               : "memory");
 }
 SPEC_DEV void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -173,6 +184,29 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       cp_async_commit();
     }
     const uint32_t id = idesc(N, A), base = smem_u32(smem);
+    // A warp adds up 32 rows, 8 columns in 32, of two accumulators in turn.
+    float sum[kMaxRank / 32][8] = {};
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16) + warp / 4 * 8;
+    auto add = [&](int chain) {
+      tc_fence_after();
+      const uint32_t from = lanes + chain % 2 * 128;
+#pragma unroll
+      for (int i = 0; i < kMaxRank / 32; i += 2) {
+        if (i * 32 >= N) break;
+        uint32_t v[2][8];
+        tmem_ld8(from + i * 32, v[0]);
+        tmem_ld8(from + i * 32 + 32, v[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            asm volatile("" : "+r"(v[h][k]));
+            sum[i + h][k] += __uint_as_float(v[h][k]);
+          }
+      }
+      tc_fence_before();
+    };
     int slot = 0, phase = 0;  // of this step; phase: of the slot before it
 #pragma unroll 1
     for (int step = 0; step < n_steps; ++step) {
@@ -185,41 +219,34 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
         const uint32_t xs = base + slot * sb, as = xs + kStep / 64 * xb;
 #pragma unroll 1
         for (int k = 0; k < kStep / 16; ++k)
-          umma_bf16(tmem, block_desc(xs + k / 4 * xb + k % 4 * 32), block_desc(as + k / 4 * ab + k % 4 * 32), id, step | k);
+          umma_bf16(tmem + step / kChain % 2 * 128, block_desc(xs + k / 4 * xb + k % 4 * 32), block_desc(as + k / 4 * ab + k % 4 * 32), id, step % kChain | k);
         umma_commit(&s_free[slot]);
       }
       // The slot before this one is filled again once its products are done.
       if (step > 0) {
         const int before = slot ? slot - 1 : stages - 1;
-        ok = mbar_wait_bounded(&s_free[before], phase, tp.err);
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_free[before], phase, tp.err));
         if (before == stages - 1) phase ^= 1;
       }
       if (step + stages - 1 < n_steps && ok) fetch();
       cp_async_commit();
+      if (step > 0 && step % kChain == 0) add(step / kChain - 1);
       slot = slot + 1 == stages ? 0 : slot + 1;
     }
     ok = __syncthreads_and(ok);
-    if (n_steps && ok) ok = mbar_wait_bounded(&s_free[slot ? slot - 1 : stages - 1], phase, tp.err);
+    if (n_steps && ok) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_free[slot ? slot - 1 : stages - 1], phase, tp.err));
+      add((n_steps - 1) / kChain);
+    }
     cp_async_wait<0>();
     ok = __syncthreads_and(ok);
-    tc_fence_after();
-    // A warp reads 32 rows, 8 columns in 32.
-    float* o = part + (warp % 4 * 32 + lane) * Wp;
-    for (int c = warp / 4 * 8; c < N; c += kTallWarps / 4 * 8) {
-      uint32_t v[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-      if (n_steps) {  // else this block has no part of K
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                     : "r"(tmem + ((uint32_t)(warp % 4 * 32) << 16) + c)
-                     : "memory");
-        tmem_wait_ld();
+    float* o = part + (warp % 4 * 32 + lane) * Wp + warp / 4 * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i])::"memory");
-      }
-      *reinterpret_cast<uint4*>(o + c) = make_uint4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<uint4*>(o + c + 4) = make_uint4(v[4], v[5], v[6], v[7]);
+    for (int i = 0; i < kMaxRank / 32; ++i) {
+      if (warp / 4 * 8 + i * 32 >= N) break;
+      *reinterpret_cast<float4*>(o + i * 32) = make_float4(sum[i][0], sum[i][1], sum[i][2], sum[i][3]);
+      *reinterpret_cast<float4*>(o + i * 32 + 4) = make_float4(sum[i][4], sum[i][5], sum[i][6], sum[i][7]);
     }
-    tc_fence_before();
     __syncthreads();
   }
 
@@ -351,11 +378,11 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
         tc_fence_after();
         const uint32_t bs = smem_u32(ring) + slot * sb + yb, to = tmem + 128 + step % 2 * kCols;
 #pragma unroll 1
-        for (int q = 0; q < P; ++q)
+        for (int q = P - 1; q >= 0; --q)
 #pragma unroll 1
           for (int k = 0; k < N / 16; ++k)
             umma_bf16(to, block_desc(frag + q * frag_bytes(1, N) + k / 4 * (kTallRows * 128) + k % 4 * 32),
-                      block_desc(bs + k / 4 * (kCols * 128) + k % 4 * 32), id, q | k);
+                      block_desc(bs + k / 4 * (kCols * 128) + k % 4 * 32), id, q < P - 1 || k);
         umma_commit(&s_done[step % 2]);
       }
       // The slot of two steps ago is free.
@@ -365,7 +392,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
         const int before = slot ? slot - 1 : stages - 1, n = (step - 1) * kCols;
         uint8_t* st = ring + before * sb;
         if (r) {
-          ok = mbar_wait_bounded(&s_done[(step - 1) % 2], (step - 1) / 2 % 2, tp.err);
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_done[(step - 1) % 2], (step - 1) / 2 % 2, tp.err));
           tc_fence_after();
           uint32_t v[16];
           tmem_ld16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + 128 + (step - 1) % 2 * kCols + warp / 4 * 16, v);

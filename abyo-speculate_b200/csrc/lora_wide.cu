@@ -99,7 +99,7 @@ SPEC_DEV void store_piece(E* p, int k, int n, const uint4& v) {
 }
 
 template <class T, class TX, class TY, int NT>
-__global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant__ WideParams wp) {
+__global__ void __launch_bounds__(kThreads, sizeof(TX) == 4 && NT == 8 ? 1 : 2) wide_kernel(const __grid_constant__ WideParams wp) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_factor[kWideRows];
   __shared__ const void* s_row[kWideRows];  // the rows of x, then of y, from this block's first column on
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             // Columns 8 t .. 8 t + 7 of two rows, as hi and lo.
+            float sum[4][4] = {};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint4 v = lds128(xb + h * kArea + m * 1024), w = lds128(xb + h * kArea + m * 1024 + 512);
@@ -199,11 +200,15 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
                 for (int n = 0; n < 4; ++n) {
                   const uint32_t pair = h ? (e ? a[n].w : a[n].z) : (e ? a[n].y : a[n].x);
                   const float2 f = widen2(pair, A);
-                  mma8(d[m][n0 + n], hi[0], hi[1], hi[2], hi[3], __float_as_uint(f.x), __float_as_uint(f.y));
-                  mma8(d[m][n0 + n], lo[0], lo[1], lo[2], lo[3], __float_as_uint(f.x), __float_as_uint(f.y));
+                  mma8(sum[n], lo[0], lo[1], lo[2], lo[3], __float_as_uint(f.x), __float_as_uint(f.y));
+                  mma8(sum[n], hi[0], hi[1], hi[2], hi[3], __float_as_uint(f.x), __float_as_uint(f.y));
                 }
               }
             }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) d[m][n0 + n][i] += sum[n][i];
           }
         }
       } else {
@@ -213,10 +218,15 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 a = lds128(ab + n * 512);
+          float sum[2][4] = {};
 #pragma unroll
-          for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
+          for (int m = 0; m < 2; ++m) mma16(sum[m], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a.x, a.y, A);
 #pragma unroll
-          for (int m = 0; m < 2; ++m) mma16(d[m][n], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
+          for (int m = 0; m < 2; ++m) mma16(sum[m], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a.z, a.w, A);
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[m][n][i] += sum[m][i];
         }
       }
       __syncwarp();
@@ -379,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 2) wide_kernel(const __grid_constant
           for (int j = 0; j < 4; ++j) b[j] = first_of(b[j], r - s * 32 - per * t);
         }
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
+        for (int q = P - 1; q >= 0; --q) {
           const uint8_t* f = smem + (q * steps + s) * frag + g * 64 + per * 2 * t;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {

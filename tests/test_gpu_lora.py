@@ -340,3 +340,27 @@ def test_one_plan_on_two_streams_at_once(pkg):
     junk = [torch.full((1 << 16,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want)) and junk
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,adapters,rank,x", [(8100, 3, 64, "same"), (2400, 40, 128, "f32"), (2400, 40, 128, "same"),
+                                                  (3000, 60, 16, "f32"), (300, 300, 128, "f32"), (300, 300, 128, "same"),
+                                                  (5, 5, 16, "f32")])
+def test_long_sums_are_no_less_than_f32(pkg, rows, adapters, rank, dtype, x):
+    """x A^T of 14336 positive terms: a sum that drops its last bits at every step ends too small.
+
+    B = 1 hands x A^T out in f32.  The tensor core adds up at most 16 instructions in a row, each of which may drop
+    2^-23 of the running sum on either side of it: (16 + 1) 2^-23 of positive terms.  Those sums meet in rounded
+    additions, at most 448 of them, random to first order: sqrt(448) 2^-24 in the norm.  Splits of x and of
+    x A^T: 2^-23 and 2^-22.  Together below 3.7e-6; 448 to 3584 instructions in a row end 1e-5 to 1e-4 too small."""
+    import torch
+    k, kind = 14336, kinds()[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(rank)
+    xs = 0.5 + 0.5 * torch.rand(rows, k, device="cuda", generator=gen)
+    xs = xs if x == "f32" else xs.to(kind)
+    a = ((0.5 + 0.5 * torch.rand(rank, k, device="cuda", generator=gen)) / 128).to(kind)
+    b = torch.eye(rank, device="cuda").to(kind)
+    bank = pkg.LoraBank(a.expand(adapters, rank, k), b.expand(adapters, rank, rank))
+    got = bank.apply(pkg.LoraPlan(np.arange(rows) % adapters, adapters), xs, torch.zeros(rows, rank, device="cuda"))
+    want = xs.double() @ a.double().T
+    assert float((got.double() - want).norm() / want.norm()) <= 17 * 2.0 ** -23 + 448 ** 0.5 * 2.0 ** -24 + 2.0 ** -23 + 2.0 ** -22
