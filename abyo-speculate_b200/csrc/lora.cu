@@ -15,8 +15,7 @@
 // x and A come by 16-byte loads from where they lie, without shared memory.
 //
 // f32 rows enter as two tf32 numbers, hi + lo, off by 2^-24.  t stays f32;
-// for the second product it is split into bf16 numbers (three, 24 bits, for an
-// f32 result; two, 16 bits, for a bf16 one, which itself has 8), or two f16
+// for the second product it is split into three bf16 numbers (24 bits), or two f16
 // numbers of t 2^-e, 2^e about the row's largest (22 bits).  All sums are f32.
 //
 // Bound by latency: 64 rows of 64 adapters of rank 32 and less, 3584 to 18944 in f16
@@ -80,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 3) narrow_kernel(const __grid_consta
   extern __shared__ __align__(128) uint8_t smem[];
   Smem& sm = *reinterpret_cast<Smem*>(smem);
   constexpr bool kSplitX = sizeof(TX) == 4;
-  constexpr int P = parts_of<TY>((const T*)nullptr);
+  constexpr int P = parts_of((const T*)nullptr);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = cluster_rank(), size = cluster_size();
   pdl_launch_dependents();

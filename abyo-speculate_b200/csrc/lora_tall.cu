@@ -7,14 +7,14 @@
 // whose 16-byte pieces are swizzled (piece c of row i lies at c ^ (i % 8)), so that
 // 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products.
 // An accumulator adds up two stages, two accumulators in turn, and goes from there to
-// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 135 us;
+// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 144 us;
 // one stage 2.5e-7 and 4 us longer; all of them 83e-7 and 6 us less).  The blocks'
 // parts join as in the kernel for fewer rows.  Second product: T's parts are the
 // 128-row operand, B's 64 columns a stage the other; while a stage's products
 // run, all threads add the stage before it to y, which came with B into rows 16
 // bytes further apart than they are long, and store it along the rows.
 //
-// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 135
+// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 144
 // us (55 at the copy rate), about 79 of them the first product, which brings 350 MB of x and
 // A at 4.4 TB/s, bound by the copies' 16-byte pieces in the load units; in the
 // second, 133 MB of y and out and the load units again.  On mma.sync 146 us.
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
   __shared__ uint32_t s_tmem;
   __shared__ const TY* s_row[kTallRows];
   const Params& p = tp.p;
-  constexpr int P = parts_of<TY>((const T*)nullptr);
+  constexpr int P = parts_of((const T*)nullptr);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = cluster_rank(), size = cluster_size(), N = tp.N;
   pdl_launch_dependents();
@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
 // Shared memory of the form for N columns of T, 0 where it does not fit.
 template <class T, class TY>
 int plan_memory(TallParams* t, int N) {
-  constexpr int P = parts_of<TY>((const T*)nullptr), kMost = 222 * 1024;
+  constexpr int P = parts_of((const T*)nullptr), kMost = 222 * 1024;
   const int whole = kTallRows * (N + 4) * 4, frag = frag_bytes(P, N);
   t->N = N;
   t->all_at = (whole > frag ? whole : frag) / 128 * 128 + 128;

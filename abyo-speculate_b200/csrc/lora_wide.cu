@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(TX) == 4 && NT == 8 ? 1 : 2) 
   __shared__ const void* s_row[kWideRows];  // the rows of x, then of y, from this block's first column on
   const Params& p = wp.p;
   constexpr bool kSplitX = sizeof(TX) == 4;
-  constexpr int P = parts_of<TY>((const T*)nullptr);
+  constexpr int P = parts_of((const T*)nullptr);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = cluster_rank(), size = cluster_size(), RA = wp.RA;
   pdl_launch_dependents();

@@ -705,9 +705,9 @@ int spec_batch_verify_tree(const spec_batch_logits* l, int n_seqs, const int32_t
  *   out = y + scale (x A^T) B^T,   A [rank x k], B [n x rank]
  * A bank holds the adapters of one projection in caller-owned device memory, a
  * plan says which adapter each row of a step has (once per step, for all
- * projections and layers).  Sums and x A^T are f32 (the latter is split into
- * parts of 16 bits in all or more for the second product), each result is
- * rounded once.  One call's result does not depend on timing; a row's last bits
+ * projections and layers).  Sums and x A^T are f32 (the latter is split
+ * into numbers of the adapters' type for the second product: 24 bits in bf16,
+ * 22 of the row's largest in f16), each result is rounded once.  One call's result does not depend on timing; a row's last bits
  * may depend on the other rows of the plan.  Calls keep no state, wait for
  * nothing, allocate nothing and can be captured.  Pointers are device memory of `device` unless said otherwise. */
 typedef struct spec_lora_bank {

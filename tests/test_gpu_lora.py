@@ -364,3 +364,27 @@ def test_long_sums_are_no_less_than_f32(pkg, rows, adapters, rank, dtype, x):
     got = bank.apply(pkg.LoraPlan(np.arange(rows) % adapters, adapters), xs, torch.zeros(rows, rank, device="cuda"))
     want = xs.double() @ a.double().T
     assert float((got.double() - want).norm() / want.norm()) <= 17 * 2.0 ** -23 + 448 ** 0.5 * 2.0 ** -24 + 2.0 ** -23 + 2.0 ** -22
+
+
+
+@pytest.mark.parametrize("dtype,x,y", TYPES)
+@pytest.mark.parametrize("rows", [3, 40, 1000])
+@pytest.mark.parametrize("rank", [2, 24, 72])
+def test_all_bits_of_the_first_product_count(pkg, rows, rank, dtype, x, y):
+    """x A^T holds 21-bit whole numbers t and -t + d: their sum d + y is small, so that it is exact in every type.
+
+    Every number that enters has at most 7 bits, every sum at most 21: f32 sums are exact, and t is, in parts of
+    21 bits in all or more."""
+    import torch
+    rng = np.random.default_rng(rows + rank)
+    k, n = 200, 96
+    digits = rng.integers(0, 128, (rows, 3))
+    at, pair = rng.permutation(k)[:3], rng.permutation(rank)[:2]
+    xs, a = np.zeros((rows, k)), np.zeros((1, rank, k))
+    xs[:, at] = digits
+    a[0, pair[0], at] = [1 << 14, 1 << 7, 1]
+    a[0, pair[1], at] = [-(1 << 14), -(1 << 7), 0]
+    ys = rng.integers(-64, 65, (rows, n))
+    bank = pkg.LoraBank(dev(a, dtype), dev(np.ones((1, n, rank)), dtype))
+    got = bank.apply(pkg.LoraPlan([0] * rows, 1), dev(xs, dtype if x == "same" else x), dev(ys, dtype if y == "same" else y))
+    assert np.array_equal(got.double().cpu().numpy(), (digits[:, 2:] + ys).astype(np.float64))
