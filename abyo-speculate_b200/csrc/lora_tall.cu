@@ -5,18 +5,19 @@
 // 16): the blocks of a cluster share K; stages of 128 columns of the rows and of A
 // are copied asynchronously into the K-major operand layout of 128-byte rows
 // whose 16-byte pieces are swizzled (piece c of row i lies at c ^ (i % 8)), so that
-// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products.
+// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products
+// (their descriptors are sums with constants: 144 us where each was put together anew).
 // An accumulator adds up two stages, two accumulators in turn, and goes from there to
-// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 144 us;
-// one stage 2.5e-7 and 4 us longer; all of them 83e-7 and 6 us less).  The blocks'
+// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 128.5 us;
+// one stage 2.5e-7, 131 us; all of them 81e-7, 126.5).  The blocks'
 // parts join as in the kernel for fewer rows.  Second product: T's parts are the
 // 128-row operand, B's 64 columns a stage the other; while a stage's products
 // run, all threads add the stage before it to y, which came with B into rows 16
 // bytes further apart than they are long, and store it along the rows.
 //
-// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 144
-// us (55 at the copy rate), about 79 of them the first product, which brings 350 MB of x and
-// A at 4.4 TB/s, bound by the copies' 16-byte pieces in the load units; in the
+// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 128.5
+// us (55 at the copy rate), about 73 of them the first product, which brings 350 MB of x and
+// A at 4.8 TB/s, bound by the copies' 16-byte pieces in the load units; in the
 // second, 133 MB of y and out and the load units again.  On mma.sync 146 us.
 #include "lora_mma.cuh"
 
@@ -216,10 +217,10 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       if (!ok) break;
       if (threadIdx.x == 0) {
         tc_fence_after();
-        const uint32_t xs = base + slot * sb, as = xs + kStep / 64 * xb;
-#pragma unroll 1
+        const uint64_t xs = block_desc(base + slot * sb), as = block_desc(base + slot * sb + kStep / 64 * xb);
+#pragma unroll
         for (int k = 0; k < kStep / 16; ++k)
-          umma_bf16(tmem + step / kChain % 2 * 128, block_desc(xs + k / 4 * xb + k % 4 * 32), block_desc(as + k / 4 * ab + k % 4 * 32), id, step % kChain | k);
+          umma_bf16(tmem + step / kChain % 2 * 128, xs + (k / 4 * xb + k % 4 * 32) / 16, as + (k / 4 * ab + k % 4 * 32) / 16, id, step % kChain | k);
         umma_commit(&s_free[slot]);
       }
       // The slot before this one is filled again once its products are done.
@@ -365,7 +366,8 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       if (s < n_steps) fetch();
       cp_async_commit();
     }
-    const uint32_t id = idesc(kCols, A), frag = smem_u32(smem);
+    const uint32_t id = idesc(kCols, A);
+    const uint64_t t = block_desc(smem_u32(smem));
     int slot = 0;
     // One step more than there are stages: the last one only finishes.
 #pragma unroll 1
@@ -376,13 +378,18 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       if (!ok) break;
       if (threadIdx.x == 0 && step < n_steps && r) {
         tc_fence_after();
-        const uint32_t bs = smem_u32(ring) + slot * sb + yb, to = tmem + 128 + step % 2 * kCols;
-#pragma unroll 1
+        const uint32_t to = tmem + 128 + step % 2 * kCols;
+        const uint64_t b = block_desc(smem_u32(ring) + slot * sb + yb);
+        uint32_t some = 0;  // whether the accumulator holds a sum
+#pragma unroll
         for (int q = P - 1; q >= 0; --q)
-#pragma unroll 1
-          for (int k = 0; k < N / 16; ++k)
-            umma_bf16(to, block_desc(frag + q * frag_bytes(1, N) + k / 4 * (kTallRows * 128) + k % 4 * 32),
-                      block_desc(bs + k / 4 * (kCols * 128) + k % 4 * 32), id, q < P - 1 || k);
+#pragma unroll
+          for (int k = 0; k < kMaxRank / 16; ++k)
+            if (k * 16 < N) {
+              umma_bf16(to, t + (q * frag_bytes(1, N) + k / 4 * (kTallRows * 128) + k % 4 * 32) / 16,
+                        b + (k / 4 * (kCols * 128) + k % 4 * 32) / 16, id, some);
+              some = 1;
+            }
         umma_commit(&s_done[step % 2]);
       }
       // The slot of two steps ago is free.
