@@ -73,13 +73,18 @@ Rows to_rows(const spec_batch_logits* l) {
 int verify(const char* what, const spec_batch_logits* l, VerifyParams& p, int32_t* path, bool trees, void* stream) {
   if (p.n_seqs < 0 || p.n_seqs > SPEC_BATCH_MAX_ROWS)
     return fail(SPEC_ERR_INVALID, "%s: %d sequences, 0 to %d are taken", what, p.n_seqs, SPEC_BATCH_MAX_ROWS);
-  if (p.n_seqs == 0) return SPEC_OK;
-  if (!p.row_start || !p.n_out || !p.next) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
+  const bool path_alone = p.n_seqs == 0 && trees && l->n_rows > 0;  // rows of no sequence: their path is -1
+  if (p.n_seqs == 0 && !path_alone) return SPEC_OK;
+  if (p.n_seqs > 0 && (!p.row_start || !p.n_out || !p.next)) return fail(SPEC_ERR_INVALID, "%s: null argument", what);
   for (const void* q : {(const void*)p.row_start, (const void*)p.tokens, (const void*)p.parents, (const void*)p.q,
                         (const void*)path, (const void*)p.n_out, (const void*)p.next})
     if (misaligned(q, 4)) return fail(SPEC_ERR_INVALID, "%s: a pointer is not aligned to 4 bytes", what);
   Current cur(l->device, what);
   if (cur.rc != SPEC_OK) return cur.rc;
+  if (path_alone) {
+    const cudaError_t e = cudaMemsetAsync(path, 0xff, (size_t)l->n_rows * sizeof(int32_t), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SPEC_OK : fail_cuda(e, what);
+  }
   p.r = to_rows(l);
   p.r.path = path;
   if (!trees) p.r.drafts = p.tokens, p.r.q = p.q, p.r.q_stride = p.q_stride;
@@ -149,7 +154,7 @@ int spec_batch_verify_tree(const spec_batch_logits* l, int n_seqs, const int32_t
   const char* what = "spec_batch_verify_tree";
   const int rc = check_logits(what, l);
   if (rc != SPEC_OK) return rc;
-  if (n_seqs > 0 && l->n_rows > 0 && (!tokens || !parents || !path))
+  if (l->n_rows > 0 && (!path || (n_seqs > 0 && (!tokens || !parents))))
     return fail(SPEC_ERR_INVALID, "%s: null tokens, parents or path", what);
   VerifyParams p{};
   p.row_start = row_start;

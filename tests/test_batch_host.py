@@ -88,3 +88,10 @@ def test_python_refuses_host_tensors(pkg):
         pkg.verify_drafts(x, u, x, u, u)
     with pytest.raises(pkg.SamplingError):
         pkg.verify_trees(x, u, u, u, u)
+
+
+def test_a_tree_call_without_sequences_needs_its_path(lib):
+    """Rows but no sequence: every row's path is to be -1, so that there has to be one."""
+    a, p = logits(), 1 << 20
+    assert lib.spec_batch_verify_tree(ctypes.byref(a), 0, None, None, None, None, None, None, None) == 1
+    assert lib.spec_batch_verify_tree(ctypes.byref(a), 0, None, None, None, p + 2, None, None, None) == 1

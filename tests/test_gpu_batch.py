@@ -462,3 +462,38 @@ def test_refusals(pkg):
     assert n.tolist() == [0, 0] and token.tolist() == [-1, -1]
     path, n, token = pkg.verify_trees(empty, none, none, u[:0], torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert path.numel() == 0 and n.tolist() == [0] and token.tolist() == [-1]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_without_sequences(pkg, dtype):
+    """Rows that belong to no sequence: their path is -1, nothing else is written."""
+    import torch
+    n, v = 300, 700
+    x, _ = rows(n, v, dtype, seed=3)
+    zeros, u = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n, device="cuda")
+    junk = [torch.full((n,), 5, dtype=torch.int32, device="cuda") for _ in range(4)]  # what a new tensor may hold
+    del junk
+    for start in ([0], [n], [-1]):
+        path, count, token = pkg.verify_trees(x, zeros, zeros, u, dev(start, np.int32))
+        assert path.tolist() == [-1] * n and count.numel() == token.numel() == 0
+    # The same through the C entry, into the middle of other memory.
+    lib = pkg.load()
+    from importlib import import_module
+    _lib = import_module("abyo-speculate_b200._lib")
+    kind = TYPES.index(dtype)
+    need = lib.spec_batch_workspace_bytes(n, v, kind)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a = _lib.BatchLogits(device=0, vocab=v, dtype=kind, temperature=1.0, logits=x.data_ptr(), row_stride=x.stride(0), n_rows=n,
+                         temperatures=None, uniforms=u.data_ptr(), workspace=work.data_ptr(), workspace_bytes=need)
+    wide = torch.full((n + 2,), 7, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.spec_batch_verify_tree(ctypes.byref(a), 0, None, None, None, wide[1:].data_ptr(), None, None, stream) == 0
+    assert wide.tolist() == [7] + [-1] * n + [7]
+    # And captured.
+    g = torch.cuda.CUDAGraph()
+    start = dev([0], np.int32)
+    with torch.cuda.graph(g):
+        path, _, _ = pkg.verify_trees(x, zeros, zeros, u, start)
+    path.fill_(3)
+    g.replay()
+    assert path.tolist() == [-1] * n
