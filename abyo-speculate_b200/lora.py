@@ -54,7 +54,7 @@ class LoraPlan:
             raise _invalid(f"a plan on {self.device}: a CUDA device is needed")
         self._desc.device_copy = self._copy.data_ptr()
         self._at = ctypes.addressof(self._desc)
-        self._made_on = torch.cuda.current_stream(self.device).cuda_stream
+        self._seen = set()  # streams that calls ran on
 
     def status(self) -> None:
         """Waits for the current stream's calls; raises if a device wait in a call with this plan gave up."""
@@ -97,7 +97,7 @@ class LoraBank:
                                       t.is_contiguous()):
                 raise _invalid(f"{what} is not a contiguous {dtype} tensor [{n}] on {self.device}")
         self._keep = (a, b, ranks, scales)
-        self._made_on = torch.cuda.current_stream(self.device).cuda_stream
+        self._seen = set()
         self._types = {a.dtype: types[a.dtype], torch.float32: 2}
         self._desc = _lib.LoraBankDesc(
             a.device.index, n, k, self.n, r, types[a.dtype], a.data_ptr(), b.data_ptr(), a.stride(0), a.stride(1),
@@ -135,10 +135,13 @@ class LoraBank:
         rc = lib.spec_lora_apply(self._at, plan._at, at, at + 32, at + 64, stream)
         if rc:
             _lib.check(rc)
-        # Memory of a plan or bank that is dropped is not handed out before this stream is done with it.
-        if stream != plan._made_on:
+        # Memory of a plan or bank that is dropped is not handed out before this stream is done with it.  Each stream
+        # counts, whichever was current when the bank was made: the caller's tensors may be of another one.
+        if stream not in plan._seen:
+            plan._seen.add(stream)
             plan._copy.record_stream(torch.cuda.current_stream(self.device))
-        if stream != self._made_on:
+        if stream not in self._seen:
+            self._seen.add(stream)
             for t in self._keep:
                 if t is not None:
                     t.record_stream(torch.cuda.current_stream(self.device))

@@ -388,3 +388,26 @@ def test_all_bits_of_the_first_product_count(pkg, rows, rank, dtype, x, y):
     bank = pkg.LoraBank(dev(a, dtype), dev(np.ones((1, n, rank)), dtype))
     got = bank.apply(pkg.LoraPlan([0] * rows, 1), dev(xs, dtype if x == "same" else x), dev(ys, dtype if y == "same" else y))
     assert np.array_equal(got.double().cpu().numpy(), (digits[:, 2:] + ys).astype(np.float64))
+
+
+def test_weights_of_another_stream_outlive_the_bank(pkg):
+    """Weights of one stream, bank and call on another, all dropped while the call waits: their memory is not handed out."""
+    import torch
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    shapes = ((3, 16, 1 << 17), (3, 1 << 17, 16))  # blocks of their own
+    kept = [torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in shapes]
+    ranks, scales = torch.full((3,), 16, dtype=torch.int32, device="cuda"), torch.ones(3, device="cuda")
+    x, y = (torch.zeros(3, 1 << 17, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    at = [t.data_ptr() for t in kept]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        bank = pkg.LoraBank(*kept, ranks=ranks, scales=scales)
+        plan = pkg.LoraPlan([0, 2, -1], 3)
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+        bank.apply(plan, x, y)
+    del kept, bank, plan
+    assert torch.cuda.current_stream() == main
+    again = [torch.empty(s, dtype=torch.bfloat16, device="cuda") for s in shapes * 2]
+    assert not side.query()  # the call has still to run
+    assert not {t.data_ptr() for t in again} & set(at)
+    side.synchronize()
