@@ -459,12 +459,15 @@ cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s)
   // a GPC's SMs empty (16 of them, one an SM: 20 us, two 11).  At least: two slots a warp; the
   // warps' parts of T, 32 rows and a block of ranks each; T whole behind the
   // numbers that it is split into.
-  int bytes = (long long)n_units * size * 2 > sms ? 112 * 1024 : 224 * 1024;
+  constexpr int kMost = 224 * 1024;
+  static_assert(kWarps * 2 * kSlot <= kMost && kWarps * 32 * B * 4 <= kMost && kWideRows * kMaxRank * 10 <= kMost, "");
+  int bytes = (long long)n_units * size * 2 > sms ? kMost / 2 : kMost;
   for (const int need : {kWarps * 2 * kSlot, kWarps * 32 * B * 4, kWideRows * w.RA * 10, 3 * steps * kWideRows * 64})
     if (bytes < need) bytes = need;
   w.ring = bytes / kWarps / 16 * 16;
   w.bytes = bytes;
-  const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T, TX, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  // The kernel's limit is the process's: one number, which no other thread's call lowers before the launch.
+  const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T, TX, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
   if (e != cudaSuccess) return e;
   return launch_clusters(wide_kernel<T, TX, TY, NT>, n_units, size, kThreads, bytes, s, w);
 }

@@ -411,3 +411,54 @@ def test_weights_of_another_stream_outlive_the_bank(pkg):
     assert not side.query()  # the call has still to run
     assert not {t.data_ptr() for t in again} & set(at)
     side.synchronize()
+
+
+CALLERS = r"""
+#include <atomic>
+#include <thread>
+#include "spec_b200.h"
+using Apply = int (*)(const spec_lora_bank*, const spec_lora_plan*, const spec_lora_rows*, const spec_lora_rows*, const spec_lora_rows*, void*);
+struct Call { void *bank, *plan, *rows, *stream; };
+extern "C" int run_callers(Apply apply, const Call* calls, int n, int turns) {
+  std::atomic<int> failed{0}, ready{0};
+  auto loop = [&](const Call& c) {
+    const spec_lora_rows* r = static_cast<const spec_lora_rows*>(c.rows);
+    for (++ready; ready < n;) {}
+    for (int i = 0; i < turns; ++i)
+      if (apply(static_cast<spec_lora_bank*>(c.bank), static_cast<spec_lora_plan*>(c.plan), r, r + 1, r + 2, c.stream)) ++failed;
+  };
+  std::thread other(loop, calls[1]);
+  loop(calls[0]);
+  other.join();
+  return failed;
+}
+"""
+
+
+def test_calls_of_two_host_threads(pkg, tmp_path):
+    """Few units, which take an SM's whole shared memory, beside many, which share it, from two native threads at once
+    (python's wait for each other's lock)."""
+    import ctypes
+    import os
+    import shutil
+    import subprocess
+    import torch
+    if not shutil.which("g++"):
+        pytest.skip("no C++ compiler")
+    src, lib = tmp_path / "callers.cpp", tmp_path / "libcallers.so"
+    src.write_text(CALLERS)
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-pthread", f"-I{include}", str(src), "-o", str(lib)], check=True)
+    cases = [Case(pkg, np.repeat(np.arange(n), 40), n, 128, 128, 64, seed=n) for n in (2, 40)]
+    outs, streams = [torch.zeros_like(c.y) for c in cases], [torch.cuda.Stream() for _ in cases]
+    want = [c.bank.apply(c.plan, c.x, c.y, out=torch.empty_like(c.y)) for c in cases]
+    torch.cuda.synchronize()
+    from importlib import import_module
+    rows = [import_module("abyo-speculate_b200.lora")._THREE_ROWS.pack(
+        *c.bank._rows(c.x, c.bank.k, "x"), *c.bank._rows(c.y, c.bank.n, "y"), *c.bank._rows(o, c.bank.n, "out")) for c, o in zip(cases, outs)]
+    calls = (ctypes.c_void_p * 8)(*[at for c, r, s in zip(cases, rows, streams) for at in (
+        c.bank._at, c.plan._at, ctypes.cast(ctypes.c_char_p(r), ctypes.c_void_p).value, s.cuda_stream)])
+    apply = ctypes.cast(pkg.load().spec_lora_apply, ctypes.c_void_p)
+    assert ctypes.CDLL(str(lib)).run_callers(apply, calls, 2, 5000) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
