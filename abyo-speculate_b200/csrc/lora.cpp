@@ -54,13 +54,6 @@ bool wide(const void* p, int64_t row, int64_t outer, int size) {
   return !misaligned(p, 16) && row * size % 16 == 0 && outer * size % 16 == 0;
 }
 
-// Blocks a cluster: 8, fewer where all clusters' blocks would not be resident at once.
-int cluster_for(int n, int per_sm, int sms) {
-  int size = 8;
-  while (size > 1 && (int64_t)n * size > (int64_t)sms * per_sm) size /= 2;
-  return size;
-}
-
 // Three blocks an SM at once; a single block a unit only for many: 256 units of 8
 // rows (c above) 141 us, 116 in clusters of two, a few of which start late.
 int narrow_cluster(int n, int sms) {
@@ -263,7 +256,7 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
     e = launch_tall(p, status_of(plan), b->dtype, y_f32, plan->n_tall, cluster_for(plan->n_tall, 1, sms), s, &taken);
   p.units = units + plan->n_tall + (taken ? plan->n_big : 0);
   const int wide = rest ? plan->n_wide - (mid ? plan->n_mid_wide : 0) + (taken ? 0 : plan->n_big) : 0;
-  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, cluster_for(wide, 2, sms), sms, s);
+  if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, sms, s);
   p.units = units + plan->n_tall + plan->n_big + plan->n_wide;
   // Units of 8 rows, rows without an adapter and the units behind them: at once, but
   // for rows in place, which have nothing to copy.

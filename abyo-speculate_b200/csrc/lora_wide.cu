@@ -29,6 +29,18 @@ namespace {
 constexpr int kArea = 32 * 64 + 64;  // 32 rows of 64 bytes
 __host__ __device__ constexpr int area(int rows) { return rows * 64 + 64; }
 
+// Shared memory of a block at most; bytes of a slot of a warp's ring; blocks that an SM
+// holds by that, two slots a warp at least (f32 rows of rank above 32: 131 KB, one).
+constexpr int kMost = 224 * 1024;
+template <class TX, int NT>
+__host__ __device__ constexpr int slot_bytes() {
+  return (int)sizeof(TX) / 2 * kArea + area(8 * NT);
+}
+template <class TX, int NT>
+__host__ __device__ constexpr int blocks_an_sm() {
+  return kWarps * 2 * slot_bytes<TX, NT>() <= kMost / 2 ? 2 : 1;
+}
+
 struct WideParams {
   Params p;
   int RA, ring, bytes;  // ranks' capacity (a multiple of 8 NT); bytes of a warp's ring in the first product, of shared memory
@@ -99,7 +111,7 @@ SPEC_DEV void store_piece(E* p, int k, int n, const uint4& v) {
 }
 
 template <class T, class TX, class TY, int NT>
-__global__ void __launch_bounds__(kThreads, sizeof(TX) == 4 && NT == 8 ? 1 : 2) wide_kernel(const __grid_constant__ WideParams wp) {
+__global__ void __launch_bounds__(kThreads, blocks_an_sm<TX, NT>()) wide_kernel(const __grid_constant__ WideParams wp) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_factor[kWideRows];
   __shared__ const void* s_row[kWideRows];  // the rows of x, then of y, from this block's first column on
@@ -129,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(TX) == 4 && NT == 8 ? 1 : 2) 
   float d[2][NT][4] = {};
   {
     constexpr int C = 32, XP = C * (int)sizeof(TX) / 16, XR = 32 / XP;  // columns of a piece of work; 16-byte pieces of a row; rows a pass
-    constexpr int XA = XP / 4 * kArea, kSlot = XA + area(8 * NT);
+    constexpr int XA = XP / 4 * kArea, kSlot = slot_bytes<TX, NT>();
     const int k_per = (p.K + size * C - 1) / (size * C) * C, k0 = min(rank * k_per, p.K), k1 = min(k0 + k_per, p.K), length = k1 - k0;
     if (threadIdx.x < kWideRows)
       s_row[threadIdx.x] = static_cast<const TX*>(p.x) + rows[min((int)threadIdx.x, n_rows - 1)] * p.x_row + k0;
@@ -451,19 +463,19 @@ __global__ void __launch_bounds__(kThreads, sizeof(TX) == 4 && NT == 8 ? 1 : 2) 
 }
 
 template <class T, class TX, class TY, int NT>
-cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s) {
-  constexpr int B = 8 * NT, kSlot = (int)sizeof(TX) / 2 * kArea + area(B);
+cudaError_t run(const Params& p, int n_units, int sms, cudaStream_t s) {
+  constexpr int B = 8 * NT, kFit = blocks_an_sm<TX, NT>();
   WideParams w{p, ((p.rank > 1 ? p.rank : 1) + B - 1) / B * B, 0, 0};
-  const int steps = (w.RA + 31) / 32;
-  // Two blocks an SM where there are many: alone on an SM, clusters of 8 leave part of
-  // a GPC's SMs empty (16 of them, one an SM: 20 us, two 11).  At least: two slots a warp; the
-  // warps' parts of T, 32 rows and a block of ranks each; T whole behind the
-  // numbers that it is split into.
-  constexpr int kMost = 224 * 1024;
-  static_assert(kWarps * 2 * kSlot <= kMost && kWarps * 32 * B * 4 <= kMost && kWideRows * kMaxRank * 10 <= kMost, "");
-  int bytes = (long long)n_units * size * 2 > sms ? kMost / 2 : kMost;
-  for (const int need : {kWarps * 2 * kSlot, kWarps * 32 * B * 4, kWideRows * w.RA * 10, 3 * steps * kWideRows * 64})
-    if (bytes < need) bytes = need;
+  // Two blocks an SM where they fit and there are many: alone on an SM, clusters of 8
+  // leave part of a GPC's SMs empty (16 of them, one an SM: 20 us, two 11).  Clusters for two
+  // where one fits run as two waves (f32 rows, 16 adapters of 128 rows of rank 64: 86 us,
+  // 78 so; 16 of 64 rows of rank 128: 117, 71).  Besides the rings a block holds
+  // the warps' parts of T, 32 rows and a block of ranks each; T whole behind the numbers
+  // that it is split into.
+  static_assert(kWarps * 2 * slot_bytes<TX, NT>() <= kMost && kWarps * 32 * B * 4 <= kMost / 2 &&
+                kWideRows * kMaxRank * 10 <= kMost / 2 && 3 * kWideRows * kMaxRank * 2 <= kMost / 2, "");
+  const int size = cluster_for(n_units, kFit, sms);
+  const int bytes = kFit == 2 && (long long)n_units * size * 2 > sms ? kMost / 2 : kMost;
   w.ring = bytes / kWarps / 16 * 16;
   w.bytes = bytes;
   // The kernel's limit is the process's: one number, which no other thread's call lowers before the launch.
@@ -472,21 +484,21 @@ cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s)
   return launch_clusters(wide_kernel<T, TX, TY, NT>, n_units, size, kThreads, bytes, s, w);
 }
 template <class T, class TX, class TY>
-cudaError_t run(const Params& p, int n_units, int size, int sms, cudaStream_t s) {
-  return p.rank <= 32 ? run<T, TX, TY, 4>(p, n_units, size, sms, s) : run<T, TX, TY, 8>(p, n_units, size, sms, s);
+cudaError_t run(const Params& p, int n_units, int sms, cudaStream_t s) {
+  return p.rank <= 32 ? run<T, TX, TY, 4>(p, n_units, sms, s) : run<T, TX, TY, 8>(p, n_units, sms, s);
 }
 template <class T>
-cudaError_t run(const Params& p, bool x_f32, bool y_f32, int n_units, int size, int sms, cudaStream_t s) {
-  if (x_f32) return y_f32 ? run<T, float, float>(p, n_units, size, sms, s) : run<T, float, T>(p, n_units, size, sms, s);
-  return y_f32 ? run<T, T, float>(p, n_units, size, sms, s) : run<T, T, T>(p, n_units, size, sms, s);
+cudaError_t run(const Params& p, bool x_f32, bool y_f32, int n_units, int sms, cudaStream_t s) {
+  if (x_f32) return y_f32 ? run<T, float, float>(p, n_units, sms, s) : run<T, float, T>(p, n_units, sms, s);
+  return y_f32 ? run<T, T, float>(p, n_units, sms, s) : run<T, T, T>(p, n_units, sms, s);
 }
 
 }  // namespace
 
-cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, int sms, cudaStream_t s) {
+cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int sms, cudaStream_t s) {
   if (n_units <= 0) return cudaSuccess;
-  return type == T_BF16 ? run<__nv_bfloat16>(p, x_f32, y_f32, n_units, size, sms, s)
-                        : run<__half>(p, x_f32, y_f32, n_units, size, sms, s);
+  return type == T_BF16 ? run<__nv_bfloat16>(p, x_f32, y_f32, n_units, sms, s)
+                        : run<__half>(p, x_f32, y_f32, n_units, sms, s);
 }
 
 }  // namespace lora
