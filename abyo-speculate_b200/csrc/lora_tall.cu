@@ -5,19 +5,21 @@
 // 16): the blocks of a cluster share K; stages of 128 columns of the rows and of A
 // are copied asynchronously into the K-major operand layout of 128-byte rows
 // whose 16-byte pieces are swizzled (piece c of row i lies at c ^ (i % 8)), so that
-// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products
-// (their descriptors are sums with constants: 144 us where each was put together anew).
+// 8 lanes copy 128 bytes of one row, and one thread issues the stage's 8 products;
+// their operands' addresses are sums with constants, as each step of arithmetic there delays
+// the whole block (put together anew: 16 us of the case below).
 // An accumulator adds up two stages, two accumulators in turn, and goes from there to
-// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share, 128.5 us;
-// one stage 2.5e-7, 131 us; all of them 81e-7, 126.5).  The blocks'
-// parts join as in the kernel for fewer rows.  Second product: T's parts are the
-// 128-row operand, B's 64 columns a stage the other; while a stage's products
+// f32 additions in registers (the case below: error 3.3e-7 of the adapters' share;
+// one stage 2.5e-7 and 2.5 us longer; all of them 81e-7 and 2 us less).  The blocks'
+// parts join as in the kernel for fewer rows.  Second product: T's numbers are the
+// 128-row operand, in tensor memory (in shared memory 126 us, not 120, and 237, not 206,
+// for 14336 output channels), B's 64 columns a stage the other; while a stage's products
 // run, all threads add the stage before it to y, which came with B into rows 16
 // bytes further apart than they are long, and store it along the rows.
 //
-// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 128.5
-// us (55 at the copy rate), about 73 of them the first product, which brings 350 MB of x and
-// A at 4.8 TB/s, bound by the copies' 16-byte pieces in the load units; in the
+// x has the adapters' type.  8100 rows of rank 64, 14336 to 4096 channels in bf16: 120
+// us (55 at the copy rate), about 75 of them the first product, which brings 350 MB of x and
+// A at 4.7 TB/s, bound by the copies' 16-byte pieces in the load units; in the
 // second, 133 MB of y and out and the load units again.  On mma.sync 146 us.
 #include "lora_mma.cuh"
 
@@ -30,7 +32,9 @@ constexpr int kStep = 128;        // columns of a stage of the first product
 constexpr int kCols = 64;         // and of the second
 constexpr int kMaxStages = 6;
 constexpr int kChain = 2;         // stages that one accumulator adds up
-constexpr int kTmem = 256;        // columns: T, and two accumulators of the second product from 128 on
+// Columns of tensor memory: two accumulators of the first product, in whose place two of
+// the second come, then the numbers that T is split into, two a column.
+constexpr int kTmem = 512, kParts = 256;
 
 struct TallParams {
   Params p;
@@ -54,7 +58,6 @@ __host__ __device__ constexpr int stage2(int N) {
   return (kTallRows * y_pitch<TY>() + 1023) / 1024 * 1024 + blocks_of(N) * kCols * 128;
 }
 __host__ __device__ constexpr int stage1(int N) { return kStep / 64 * (kTallRows * 128 + (N * 128 + 1023) / 1024 * 1024); }
-__host__ __device__ constexpr int frag_bytes(int P, int N) { return P * blocks_of(N) * kTallRows * 128; }
 
 SPEC_DEV uint32_t idesc(int N, const __nv_bfloat16*) { return umma_idesc_bf16(128, N); }
 SPEC_DEV uint32_t idesc(int N, const __half*) { return umma_idesc_bf16(128, N) & ~((7u << 7) | (7u << 10)); }  // formats 0: f16
@@ -74,6 +77,19 @@ SPEC_DEV void tmem_ld8(uint32_t at, uint32_t (&v)[8]) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                : "r"(at)
                : "memory");
+}
+SPEC_DEV void tmem_st4(uint32_t at, const uint32_t (&v)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+SPEC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D (+)= A B^T with A [128 x 16] in tensor memory, a row a lane, two numbers a column.
+SPEC_DEV void umma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 SPEC_DEV void publish_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -271,27 +287,29 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
     if (i / share != rank) *reinterpret_cast<float4*>(all + i) = remote_float4(all + i, i / share);
   cluster_arrive();  // nothing of the other blocks is read any more
   __syncthreads();
-  // In part's place: the numbers that T is split into, four threads a row.  A
-  // thread keeps the factor of the row that it finishes.
+  // The numbers that T is split into, four threads a row, to tensor memory.
   const int my_row = warp % 4 * 32 + lane;
   float factor;
   {
-    const int row = threadIdx.x / 4, h = threadIdx.x % 4;
+    const int h = warp / 4;
     const float scale = p.scales ? p.scales[u.adapter] : 1.f;
+    float* mine = all + my_row * Wp;
     float top = 0.f;
     for (int j = h * 8; j < r; j += 32)
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (j + k < r) top = fmaxf(top, fabsf(all[row * Wp + j + k] * scale));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (j + k < r) top = fmaxf(top, fabsf(mine[j + k] * scale));
+    mine[N + h] = top;  // the rows' pads: nothing else of them is read
+    __syncthreads();
+    top = fmaxf(fmaxf(mine[N], mine[N + 1]), fmaxf(mine[N + 2], mine[N + 3]));
     const int e = exponent(top, A);
     const float down = pow2i(-e);
+    factor = pow2i(e);
+    const uint32_t to = tmem + ((uint32_t)(warp % 4 * 32) << 16) + kParts;
     for (int j = h * 8; j < N; j += 32) {
-      uint8_t* to = smem + j / 64 * (kTallRows * 128) + swizzled(row, j / 8 % 8);
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = j + k < r ? all[row * Wp + j + k] * scale * down : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = j + k < r ? mine[j + k] * scale * down : 0.f;
 #pragma unroll
       for (int q = 0; q < P; ++q) {
         uint32_t w[4];
@@ -303,13 +321,11 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
           v[2 * k] = fabsf(v[2 * k]) < INFINITY ? v[2 * k] - to_float(hl[0]) : 0.f;
           v[2 * k + 1] = fabsf(v[2 * k + 1]) < INFINITY ? v[2 * k + 1] - to_float(hl[1]) : 0.f;
         }
-        *reinterpret_cast<uint4*>(to + q * frag_bytes(1, N)) = make_uint4(w[0], w[1], w[2], w[3]);
+        tmem_st4(to + (q * N + j) / 2, w);
       }
     }
-    // Row of thread 4 i is i: the factors change hands through the rows' pads.
-    if (h == 0) all[row * Wp + N] = pow2i(e);
-    __syncthreads();
-    factor = all[my_row * Wp + N];
+    tmem_wait_st();
+    tc_fence_before();
   }
   cluster_wait();  // nor anything of this one
   __syncthreads();
@@ -319,7 +335,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
     const int n_per = (p.N + size * kCols - 1) / (size * kCols) * kCols, n0 = min(rank * n_per, p.N), n1 = min(n0 + n_per, p.N);
     const int width = n1 - n0, n_steps = (width + kCols - 1) / kCols, stages = tp.stages2, sb = stage2<TY>(N);
     constexpr int YP = kCols * (int)sizeof(TY) / 16, YR = 32 / YP, YN = kTallRows / kTallWarps / YR, E = 16 / (int)sizeof(TY);
-    uint8_t* ring = smem + frag_bytes(P, N);  // `all` is not used any more
+    uint8_t* ring = smem;  // `all` is not used any more
     if (threadIdx.x < kTallRows) s_row[threadIdx.x] = static_cast<const TY*>(p.y) + rows[min((int)threadIdx.x, n_rows - 1)] * p.y_row + n0;
     __syncthreads();
     TY* out[YN];  // where this thread stores
@@ -361,13 +377,11 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       next += kCols;
       at = at + sb == stages * sb ? 0 : at + sb;
     };
-    publish_smem();  // T's parts
     for (int s = 0; s < stages - 2; ++s) {
       if (s < n_steps) fetch();
       cp_async_commit();
     }
     const uint32_t id = idesc(kCols, A);
-    const uint64_t t = block_desc(smem_u32(smem));
     int slot = 0;
     // One step more than there are stages: the last one only finishes.
 #pragma unroll 1
@@ -378,18 +392,19 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
       if (!ok) break;
       if (threadIdx.x == 0 && step < n_steps && r) {
         tc_fence_after();
-        const uint32_t to = tmem + 128 + step % 2 * kCols;
+        const uint32_t to = tmem + step % 2 * kCols;
         const uint64_t b = block_desc(smem_u32(ring) + slot * sb + yb);
-        uint32_t some = 0;  // whether the accumulator holds a sum
 #pragma unroll
-        for (int q = P - 1; q >= 0; --q)
+        for (int q = P - 1; q >= 0; --q) {  // the small parts first
+          const uint32_t from = tmem + kParts + q * N / 2;
+          int k = 0;
+#pragma unroll 1
+          for (; k + 64 <= N; k += 64)
 #pragma unroll
-          for (int k = 0; k < kMaxRank / 16; ++k)
-            if (k * 16 < N) {
-              umma_bf16(to, t + (q * frag_bytes(1, N) + k / 4 * (kTallRows * 128) + k % 4 * 32) / 16,
-                        b + (k / 4 * (kCols * 128) + k % 4 * 32) / 16, id, some);
-              some = 1;
-            }
+            for (int i = 0; i < 4; ++i) umma_from_tmem(to, from + k / 2 + i * 8, b + k * (kCols * 2) / 16 + i * 2, id, q < P - 1 || k + i);
+#pragma unroll 1
+          for (; k < N; k += 16) umma_from_tmem(to, from + k / 2, b + k / 64 * (kCols * 128 / 16) + k % 64 / 8, id, q < P - 1 || k);
+        }
         umma_commit(&s_done[step % 2]);
       }
       // The slot of two steps ago is free.
@@ -402,7 +417,7 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
           ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_done[(step - 1) % 2], (step - 1) / 2 % 2, tp.err));
           tc_fence_after();
           uint32_t v[16];
-          tmem_ld16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + 128 + (step - 1) % 2 * kCols + warp / 4 * 16, v);
+          tmem_ld16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + (step - 1) % 2 * kCols + warp / 4 * 16, v);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(v[i])::"memory");
@@ -445,13 +460,13 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
 // Shared memory of the form for N columns of T, 0 where it does not fit.
 template <class T, class TY>
 int plan_memory(TallParams* t, int N) {
-  constexpr int P = parts_of((const T*)nullptr), kMost = 222 * 1024;
-  const int whole = kTallRows * (N + 4) * 4, frag = frag_bytes(P, N);
+  constexpr int kMost = 222 * 1024;
+  const int whole = kTallRows * (N + 4) * 4;
   t->N = N;
-  t->all_at = (whole > frag ? whole : frag) / 128 * 128 + 128;
+  t->all_at = whole;
   t->stages = kMost / stage1(N) < kMaxStages ? kMost / stage1(N) : kMaxStages;
-  t->stages2 = (kMost - frag) / stage2<TY>(N) < kMaxStages ? (kMost - frag) / stage2<TY>(N) : kMaxStages;
-  return t->stages >= 2 && t->stages2 >= 3 && t->all_at + whole <= kMost ? kMost + 1024 : 0;
+  t->stages2 = kMost / stage2<TY>(N) < kMaxStages ? kMost / stage2<TY>(N) : kMaxStages;
+  return t->stages >= 2 && t->stages2 >= 3 && 2 * whole <= kMost ? kMost + 1024 : 0;
 }
 
 template <class T, class TY>
