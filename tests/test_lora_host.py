@@ -137,3 +137,20 @@ def test_python_refuses_host_tensors(pkg):
         pkg.LoraPlan([0, 2], 2, device="cpu")
     with pytest.raises(pkg.SamplingError):
         pkg.LoraPlan([0.5], 2, device="cpu")
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_units_fit_their_kernels(mod, seed):
+    """At most 128 rows for the kernel of very many, 32 for that of many, 8 for that of few, one without an adapter."""
+    rng = np.random.default_rng(seed)
+    runs = rng.integers(1, [10, 40, 70, 300, 3000][seed % 5], rng.integers(1, 60))
+    ids = rng.permutation(np.concatenate([np.repeat(np.arange(runs.size), runs), np.full(seed, -1)]))
+    rc, plan, buf = make(mod, ids, runs.size)
+    assert rc == 0
+    counts = [plan.n_tall, plan.n_big, plan.n_wide, plan.n_narrow, plan.n_bare, plan.n_mid]
+    units = buf[:48 * sum(counts)].view(np.int32).reshape(-1, 12)
+    most = np.repeat([128, 32, 32, 8, 1, 8], counts)
+    assert (units[:, 2] >= 1).all() and (units[:, 2] <= most).all()
+    assert ((units[:, 0] < 0) == (np.repeat(np.arange(6), counts) == 4)).all()
+    rows = units[:, 2].astype(np.int64)
+    assert sum(rows[sum(counts[:1]):sum(counts[:5])]) == ids.size
