@@ -15,26 +15,26 @@ using namespace specb200::lora;
 namespace {
 
 constexpr int kPlanRows = 1 << 20;
-// Which kernel takes an adapter's rows.  us for (a) rank 16, 4096 to 4096 channels in
-// bf16, (b) rank 64, 2048 to 8192, f32 rows, (c) rank 16, 4096 to 14336, f32 rows:
-// - up to kNarrowMost rows in units of 8: 24 adapters of 16 rows 9.4 / 24, 18.7 / 47
-//   (a / b) in units of 32;
-// - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows 16.9 / 37 /
-//   38, 21.6 / 53 / 44 in units of 32; one of 256 8.9 / 21 / 21, 10.8 / 26 / 31.  For
-//   up to kSomeUnits likewise those of at most 64 rows, where units of 32 are more
-//   than kHalvesMost and x is f32: 24 of 48 30 / 65 / 67, 20 / 78 / 75 in units of 32.
-//   Not where A and B, read again for every 8 rows, are more than kAgainMost times
-//   the rows (known when the plan is used): 24 of 32, rank 64, 14336 to 4096 in bf16 60, 46 in units of 32;
-//   (of 64 rows, which read A and B half as often, 16 of 128 took 42 / 130 / 96, 42 / 89
-//   / 88 of 32: half of the warps share K then, and half of the blocks are there);
-// - units of 128, not 32, of more than kTallMin rows, from kTallFrom of them on: 4 of
-//   them 21 / 28, 20.5 / 31 (8192 to 2048 in bf16 for b), 8 of them 21 / 28, 31 / 49.
+// Which kernel takes an adapter's rows.  us in units of 8 / of 32 for (a) rank 16, 4096 to
+// 4096 channels in bf16, (b) rank 64, 2048 to 8192, f32 rows, (c) rank 16, 4096 to 14336,
+// f32 rows:
+// - up to kNarrowMost rows in units of 8: 24 adapters of 16 rows 12 / 14, 24 / 41, 23 / 36;
+// - more, while all rows make kFewUnits units of 8, likewise: 24 of 32 rows b 37 / 45, c 38 / 45;
+//   one of 256 9 / 12, 22 / 26, 21 / 29.  16-bit rows only up to kFew16 (known when the plan is
+//   used, as what follows is): 6 of 64 rows a 10.5 / 14, 16 of 32 18 / 15.5.  f32 rows up to kSomeUnits
+//   as well those of at most 64 rows, where units of 32 are more than kHalvesMost:
+//   24 of 48 b 66 / 74, c 68 / 72.  Not where A and B, read again for every 8 rows, are more than kAgainMost times
+//   the rows: 24 of 32, rank 64, 14336 to 4096 in bf16 61 / 32.5.  Others are slower so:
+//   16 of 64 rows 30 / 20, 66 / 44, 68 / 60;
+// - of more than kTallMin rows, kTallFrom units of 128, where the device's SMs are used
+//   well by these (lora_tall.cu), which fewer of them do not.
 constexpr int kNarrowMost = 16;
 constexpr int kFewUnits = 111;   // four blocks a cluster, three an SM
+constexpr int kFew16 = 55;       // eight
 constexpr int kSomeUnits = 222;  // two
 constexpr int kAgainMost = 4;
 constexpr int kHalvesMost = 36;  // as many clusters of 8 blocks as a B200 holds, two an SM
-constexpr int kTallFrom = 5;
+constexpr int kTallFrom = 10;
 constexpr int kTallMin = 64;
 
 // Layout of a plan: units (of adapters of very many rows by 128, the same by 32,
@@ -54,10 +54,12 @@ bool wide(const void* p, int64_t row, int64_t outer, int size) {
   return !misaligned(p, 16) && row * size % 16 == 0 && outer * size % 16 == 0;
 }
 
+// Blocks a cluster of units of 8 rows: 8, fewer where three an SM are not enough.
 // Three blocks an SM at once; a single block a unit only for many: 256 units of 8
 // rows (c above) 141 us, 116 in clusters of two, a few of which start late.
 int narrow_cluster(int n, int sms) {
-  const int size = cluster_for(n, 3, sms);
+  int size = 8;
+  while (size > 1 && (int64_t)n * size > (int64_t)sms * 3) size /= 2;
   return size == 1 && (int64_t)n * 2 <= (int64_t)sms * 5 ? 2 : size;
 }
 
@@ -247,13 +249,14 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool x_f32 = x->dtype == T_F32, y_f32 = y->dtype == T_F32;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Rows that units of 8 can take as well: do they?
-  const bool mid = plan->n_mid && (plan->mid_all || x_f32) && (int64_t)b->rank * (b->k + b->n) * 2 <= (int64_t)kAgainMost * kNarrowRows *
+  const bool few = x_f32 || (plan->mid_all && (int64_t)plan->n_narrow + plan->n_mid <= kFew16);
+  const bool mid = plan->n_mid && few && (int64_t)b->rank * (b->k + b->n) * 2 <= (int64_t)kAgainMost * kNarrowRows *
                                       (b->k * (x_f32 ? 4LL : 2LL) + 2 * b->n * (y_f32 ? 4LL : 2LL));
   const bool rest = !(mid && plan->mid_all);  // there are others
   bool taken = false;
   p.units = units;
   if (e == cudaSuccess && rest && plan->n_tall && !x_f32)
-    e = launch_tall(p, status_of(plan), b->dtype, y_f32, plan->n_tall, cluster_for(plan->n_tall, 1, sms), s, &taken);
+    e = launch_tall(p, status_of(plan), b->dtype, y_f32, plan->n_tall, sms, s, &taken);
   p.units = units + plan->n_tall + (taken ? plan->n_big : 0);
   const int wide = rest ? plan->n_wide - (mid ? plan->n_mid_wide : 0) + (taken ? 0 : plan->n_big) : 0;
   if (e == cudaSuccess) e = launch_wide(p, b->dtype, x_f32, y_f32, wide, sms, s);

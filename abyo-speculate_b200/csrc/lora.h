@@ -36,19 +36,13 @@ struct Params {
   int a_wide, b_wide, x_wide, y_wide, out_wide;  // 8 consecutive elements from a multiple of 8 on are aligned 16-byte accesses
 };
 
-// Blocks a cluster: 8, fewer where all clusters' blocks would not be resident at once.
-inline int cluster_for(int n, int per_sm, int sms) {
-  int size = 8;
-  while (size > 1 && (long long)n * size > (long long)sms * per_sm) size /= 2;
-  return size;
-}
-
 // n_units units: of at most kNarrowRows rows (and those without an adapter) on
 // clusters of `size` blocks, or of at most kWideRows.
 cudaError_t launch_narrow(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int size, cudaStream_t s);
 cudaError_t launch_wide(const Params& p, int type, bool x_f32, bool y_f32, int n_units, int sms, cudaStream_t s);
-// The same of at most kTallRows rows, x of the adapters' type; *taken: the rank fits.  A device wait that gives up sets *err.
-cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int size, cudaStream_t s, bool* taken);
+// The same of at most kTallRows rows, x of the adapters' type; *taken: whether they were, or are left to units of
+// kWideRows.  A device wait that gives up sets *err.
+cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int sms, cudaStream_t s, bool* taken);
 
 }  // namespace lora
 }  // namespace specb200

@@ -221,6 +221,30 @@ cudaError_t launch_clusters(K* kernel, int n, int size, int threads, int smem, c
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+// Blocks a cluster of a kernel whose limit of shared memory is set: 8, fewer where n
+// clusters are not resident at once (a GPC's SMs hold whole clusters: of 8, with a block an SM, a B200
+// holds 15, not 18).
+template <class K>
+cudaError_t cluster_for(K* kernel, int n, int threads, int smem, int* size) {
+  for (*size = 8; *size > 1; *size /= 2) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = *size;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(*size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int resident = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&resident, kernel, &cfg);
+    if (e != cudaSuccess) return e;
+    if (n <= resident) break;
+  }
+  return cudaSuccess;
+}
+
 }  // namespace
 }  // namespace lora
 }  // namespace specb200

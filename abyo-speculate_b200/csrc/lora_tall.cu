@@ -457,35 +457,40 @@ __global__ void __launch_bounds__(kTallThreads, 1) tall_kernel(const __grid_cons
   if (warp == 0) tmem_dealloc(tmem, kTmem);
 }
 
-// Shared memory of the form for N columns of T, 0 where it does not fit.
-template <class T, class TY>
-int plan_memory(TallParams* t, int N) {
-  constexpr int kMost = 222 * 1024;
-  const int whole = kTallRows * (N + 4) * 4;
-  t->N = N;
-  t->all_at = whole;
-  t->stages = kMost / stage1(N) < kMaxStages ? kMost / stage1(N) : kMaxStages;
-  t->stages2 = kMost / stage2<TY>(N) < kMaxStages ? kMost / stage2<TY>(N) : kMaxStages;
-  return t->stages >= 2 && t->stages2 >= 3 && 2 * whole <= kMost ? kMost + 1024 : 0;
+// Shared memory for N columns of T, besides what aligns it to 1024 bytes.
+constexpr int kMost = 222 * 1024;
+__host__ __device__ constexpr int whole(int N) { return kTallRows * (N + 4) * 4; }
+template <class TY>
+TallParams plan_memory(const Params& p, unsigned* err, int N) {
+  static_assert(kMost >= 2 * stage1(kMaxRank) && kMost >= 3 * stage2<TY>(kMaxRank) && kMost >= 2 * whole(kMaxRank), "");
+  const int stages = kMost / stage1(N), stages2 = kMost / stage2<TY>(N);
+  return TallParams{p, err, N, stages < kMaxStages ? stages : kMaxStages, stages2 < kMaxStages ? stages2 : kMaxStages, whole(N)};
 }
 
+// Taken where the clusters, resident all at once, have at least half of the SMs; two waves
+// of them, or a few, are slower than units of 32 rows, two an SM.  us of units of 128 / of 32, for rank 64
+// 8192 to 2048 channels, the same 14336 to 4096, and rank 16 4096 to 4096, in bf16: 8 units of 128 25 /
+// 21, 38 / 30, 22 / 19; 10 25 / 31, 38 / 47, 22 / 22; 16 in clusters of 8 49 / 31, 74 / 47, 43 / 23; 20
+// in clusters of 4 39 / 50, 65 / 82, 36 / 35; 36 so 77 / 51, 127 / 85, 70 / 39; 50 69 / 86, 119 / 152, 65 / 66.
 template <class T, class TY>
-cudaError_t run(const Params& p, unsigned* err, int n_units, int size, cudaStream_t s, bool* taken) {
-  TallParams t{p, err, 0, 0, 0, 0};
-  const int bytes = plan_memory<T, TY>(&t, p.rank > 16 ? (p.rank + 15) / 16 * 16 : 16);
-  *taken = bytes > 0;
-  if (!bytes) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(tall_kernel<T, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+cudaError_t run(const Params& p, unsigned* err, int n_units, int sms, cudaStream_t s, bool* taken) {
+  const TallParams t = plan_memory<TY>(p, err, p.rank > 16 ? (p.rank + 15) / 16 * 16 : 16);
+  constexpr int bytes = kMost + 1024;
+  cudaError_t e = cudaFuncSetAttribute(tall_kernel<T, TY>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  int size = 1;
+  if (e == cudaSuccess) e = cluster_for(tall_kernel<T, TY>, n_units, kTallThreads, bytes, &size);
   if (e != cudaSuccess) return e;
+  *taken = (long long)n_units * size * 2 >= sms;
+  if (!*taken) return cudaSuccess;
   return launch_clusters(tall_kernel<T, TY>, n_units, size, kTallThreads, bytes, s, t);
 }
 
 }  // namespace
 
-cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int size, cudaStream_t s, bool* taken) {
+cudaError_t launch_tall(const Params& p, unsigned* err, int type, bool y_f32, int n_units, int sms, cudaStream_t s, bool* taken) {
   if (type == T_BF16)
-    return y_f32 ? run<__nv_bfloat16, float>(p, err, n_units, size, s, taken) : run<__nv_bfloat16, __nv_bfloat16>(p, err, n_units, size, s, taken);
-  return y_f32 ? run<__half, float>(p, err, n_units, size, s, taken) : run<__half, __half>(p, err, n_units, size, s, taken);
+    return y_f32 ? run<__nv_bfloat16, float>(p, err, n_units, sms, s, taken) : run<__nv_bfloat16, __nv_bfloat16>(p, err, n_units, sms, s, taken);
+  return y_f32 ? run<__half, float>(p, err, n_units, sms, s, taken) : run<__half, __half>(p, err, n_units, sms, s, taken);
 }
 
 }  // namespace lora

@@ -474,13 +474,14 @@ cudaError_t run(const Params& p, int n_units, int sms, cudaStream_t s) {
   // that it is split into.
   static_assert(kWarps * 2 * slot_bytes<TX, NT>() <= kMost && kWarps * 32 * B * 4 <= kMost / 2 &&
                 kWideRows * kMaxRank * 10 <= kMost / 2 && 3 * kWideRows * kMaxRank * 2 <= kMost / 2, "");
-  const int size = cluster_for(n_units, kFit, sms);
+  // The kernel's limit is the process's: one number, which no other thread's call lowers before the launch.
+  cudaError_t e = cudaFuncSetAttribute(wide_kernel<T, TX, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+  int size = 1;
+  if (e == cudaSuccess) e = cluster_for(wide_kernel<T, TX, TY, NT>, n_units, kThreads, kMost / kFit, &size);
+  if (e != cudaSuccess) return e;
   const int bytes = kFit == 2 && (long long)n_units * size * 2 > sms ? kMost / 2 : kMost;
   w.ring = bytes / kWarps / 16 * 16;
   w.bytes = bytes;
-  // The kernel's limit is the process's: one number, which no other thread's call lowers before the launch.
-  const cudaError_t e = cudaFuncSetAttribute(wide_kernel<T, TX, TY, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-  if (e != cudaSuccess) return e;
   return launch_clusters(wide_kernel<T, TX, TY, NT>, n_units, size, kThreads, bytes, s, w);
 }
 template <class T, class TX, class TY>

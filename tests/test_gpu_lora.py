@@ -462,3 +462,31 @@ def test_calls_of_two_host_threads(pkg, tmp_path):
     assert ctypes.CDLL(str(lib)).run_callers(apply, calls, 2, 5000) == 0
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype,x,y", [t for t in TYPES if t[1] == "same"])
+@pytest.mark.parametrize("counts,k,n,rank", [([1290, 9], 264, 200, 128), ([2500, 70, 40], 520, 333, 72), ([1900, 900], 4096, 64, 16),
+                                             ([4900], 136, 1025, 100), ([9600, 65], 72, 130, 24)])
+def test_units_of_128_rows_in_clusters_of_every_size(pkg, counts, k, n, rank, dtype, x, y):
+    """11, 21, 23, 39 and 76 units of 128 rows: clusters of 8, 4, 4, 2 blocks and single ones."""
+    import torch
+    ids = np.random.default_rng(3).permutation(np.repeat(np.arange(len(counts)), counts))
+    c = Case(pkg, ids, len(counts), k, n, rank, dtype, x, y, seed=rank)
+    c.check(out=torch.full_like(c.y, float("nan")))
+    c.check()
+    c.plan.status()
+
+
+@pytest.mark.parametrize("dtype,y", [("bf16", "same"), ("f16", "f32")])
+def test_very_many_rows_with_bad_rows_and_other_ranks(pkg, dtype, y):
+    """NaN and infinities reach their rows alone, and what lies behind an adapter's rank none."""
+    import torch
+    c = Case(pkg, np.arange(2700) % 3, 3, 264, 200, 80, dtype, "same", y, ranks=[80, 17, 0], seed=4)
+    good = c.bank.apply(c.plan, c.x, c.y, out=torch.empty_like(c.y))
+    c.x[300, 7], c.x[1501, 200] = float("nan"), float("inf")
+    got = c.bank.apply(c.plan, c.x, c.y, out=torch.empty_like(c.y))
+    same = torch.ones(2700, dtype=torch.bool, device="cuda")
+    same[300] = same[1501] = False
+    assert torch.equal(got[same], good[same]) and got[300].isnan().all()
+    c.x[300] = c.x[1501] = 0
+    c.check()
