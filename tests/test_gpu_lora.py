@@ -490,3 +490,22 @@ def test_very_many_rows_with_bad_rows_and_other_ranks(pkg, dtype, y):
     assert torch.equal(got[same], good[same]) and got[300].isnan().all()
     c.x[300] = c.x[1501] = 0
     c.check()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 200])
+def test_a_wait_that_gave_up_is_reported_once(pkg, rows):
+    """The plan's word of the device's waits, set as a wait that gives up sets it; calls leave it as it is."""
+    import torch
+    c = Case(pkg, [0] * rows, 1, 64, 48, 8)
+    c.check()
+    c.plan.status()
+    word = c.plan._copy[rows * 52:rows * 52 + 4]
+    assert c.plan._copy.numel() == rows * 52 + 16 and not word.any()
+    word[0] = 1
+    c.check()
+    with pytest.raises(pkg.DeviceError, match="gave up") as e:
+        c.plan.status()
+    assert e.value.code == 7
+    c.plan.status()
+    assert not word.any()
+    c.check()
