@@ -115,6 +115,9 @@ int spec_batch_sample(const spec_batch_logits* l, float* probs_out, int64_t prob
   if (probs_out && (probs_stride > kMaxStride || (l->n_rows > 1 && probs_stride < l->vocab)))
     return fail(SPEC_ERR_INVALID, "%s: probability rows %lld apart, the vocabulary is %d", what, (long long)probs_stride,
                 l->vocab);
+  const int64_t size = l->dtype == T_F32 ? 4 : 2;
+  if (probs_out && rows_meet(l->logits, l->row_stride * size, l->vocab * size, probs_out, probs_stride * 4, l->vocab * INT64_C(4), l->n_rows))
+    return fail(SPEC_ERR_INVALID, "%s: probabilities share memory with the logits", what);
   Current cur(l->device, what);
   if (cur.rc != SPEC_OK) return cur.rc;
   SampleParams p;

@@ -211,6 +211,10 @@ int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const s
   const bool in_place = y->ptr == out->ptr;
   if (in_place && plan->n_rows > 1 && y->row_stride != out->row_stride)
     return fail(SPEC_ERR_INVALID, "%s: y in place needs one row stride", what);
+  const int64_t xs = x->dtype == T_F32 ? 4 : 2, ys = y->dtype == T_F32 ? 4 : 2;
+  if (rows_meet(x->ptr, x->row_stride * xs, b->k * xs, out->ptr, out->row_stride * ys, b->n * ys, plan->n_rows) ||
+      (!in_place && rows_meet(y->ptr, y->row_stride * ys, b->n * ys, out->ptr, out->row_stride * ys, b->n * ys, plan->n_rows)))
+    return fail(SPEC_ERR_INVALID, "%s: out shares memory with x, or with other elements of y", what);
   if (plan->n_big || plan->n_wide || plan->n_narrow) {
     if ((b->rank > 0 && (!b->a || !b->b)) || misaligned(b->a, 2) || misaligned(b->b, 2) || misaligned(b->ranks, 4) || misaligned(b->scales, 4))
       return fail(SPEC_ERR_INVALID, "%s: a pointer of the bank is null or not aligned to its element size", what);

@@ -122,7 +122,7 @@ class LoraBank:
 
     def apply(self, plan: LoraPlan, x, y, out=None):
         """out = y + scale (x A^T) B^T, each row with its own adapter; x [rows, k],
-        y and out [rows, n] (out None: y itself).  Returns out."""
+        y and out [rows, n] (out None: y itself; otherwise memory of neither x nor y).  Returns out."""
         torch, lib, _, current = _setup()
         if plan.device != self.device:
             raise _invalid(f"the plan is on {plan.device}, the bank on {self.device}")

@@ -108,7 +108,7 @@ def sample_rows(logits, uniforms, temperature=1.0, probs_out=None, tokens_out=No
 
     uniforms: float32 [rows]; temperature: a number, or float32 [rows] (0: the
     first largest logit).  probs_out: float32 [rows, vocabulary] for the rows'
-    probabilities; tokens_out: contiguous int32 [rows]."""
+    probabilities, not in the logits' memory; tokens_out: contiguous int32 [rows]."""
     torch, lib, _, stream = _setup()
     a, work, index = _logits(logits, uniforms, temperature)
     n, v = logits.shape

@@ -646,8 +646,8 @@ int spec_kv4_status(spec_kv4_batch* b);
  * run at the same time (two graphs being replayed, say) can share.  They wait
  * for nothing, allocate nothing and can be captured.  `stream` is the
  * cudaStream_t (NULL = CUDA's default stream); all pointers are device memory
- * of `device`.  Inputs and outputs do not overlap.  Messages:
- * spec_last_error(NULL). */
+ * of `device`.  Inputs and outputs do not overlap (probabilities in the logits'
+ * memory are refused).  Messages: spec_last_error(NULL). */
 #define SPEC_BATCH_MAX_VOCAB (1 << 20)
 #define SPEC_BATCH_MAX_ROWS (1 << 20)
 typedef struct spec_batch_logits {
@@ -744,8 +744,8 @@ typedef struct spec_lora_rows {
   int dtype;
   int reserved;
 } spec_lora_rows;
-/* y and out have one type; out may be y itself (same row stride), or overlaps
- * neither x nor y.  Rows without an adapter are copied (in place: not touched),
+/* y and out have one type; out may be y itself (same row stride), or shares
+ * memory with neither x nor y (refused; rows beside each other in wider ones do not).  Rows without an adapter are copied (in place: not touched),
  * rows behind the plan's last one are left as they are. */
 int spec_lora_apply(const spec_lora_bank* b, const spec_lora_plan* plan, const spec_lora_rows* x, const spec_lora_rows* y,
                     const spec_lora_rows* out, void* stream);

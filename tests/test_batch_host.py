@@ -95,3 +95,10 @@ def test_a_tree_call_without_sequences_needs_its_path(lib):
     a, p = logits(), 1 << 20
     assert lib.spec_batch_verify_tree(ctypes.byref(a), 0, None, None, None, None, None, None, None) == 1
     assert lib.spec_batch_verify_tree(ctypes.byref(a), 0, None, None, None, p + 2, None, None, None) == 1
+
+
+@pytest.mark.parametrize("probs,stride", [(1 << 20, 1000), ((1 << 20) + 4 * 1000 * 3, 1000), ((1 << 20) - 4, 1000), ((1 << 20) - 4000 * 3, 1001)])
+def test_probabilities_on_the_logits_are_refused(lib, probs, stride):
+    a = logits(dtype=2, workspace_bytes=1 << 20)
+    assert lib.spec_batch_sample(ctypes.byref(a), probs, stride, 1 << 26, None) == 1
+    assert b"share memory" in lib.spec_last_error(None)

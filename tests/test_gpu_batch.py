@@ -497,3 +497,19 @@ def test_tree_without_sequences(pkg, dtype):
     path.fill_(3)
     g.replay()
     assert path.tolist() == [-1] * n
+
+
+def test_probabilities_beside_the_logits(pkg):
+    """Columns of one tensor, and rows in turn; not the logits' own memory."""
+    import torch
+    n, v = 6, 300
+    x, host = rows(n, v, "f32", seed=1)
+    _, u = uniforms(n, 4)
+    tokens, p = ref.sample(host, u, np.ones(n))
+    one = torch.cat([x, torch.zeros(n, v, device="cuda")], 1)
+    turns = torch.stack([x, torch.zeros(n, v, device="cuda")], 1).reshape(2 * n, v)
+    for logits, q in ((one[:, :v], one[:, v:]), (turns[0::2], turns[1::2])):
+        assert pkg.sample_rows(logits, dev(u, np.float32), probs_out=q).tolist() == tokens
+        assert (np.abs(q.cpu().numpy().astype(np.float64) - p) <= 2.0 ** -17 * p + 2.0 ** -120).all()
+        with pytest.raises(pkg.SamplingError):
+            pkg.sample_rows(logits, dev(u, np.float32), probs_out=logits)

@@ -509,3 +509,22 @@ def test_a_wait_that_gave_up_is_reported_once(pkg, rows):
     c.plan.status()
     assert not word.any()
     c.check()
+
+
+@pytest.mark.parametrize("rows", [1, 6, 300])
+def test_rows_beside_each_other(pkg, rows):
+    """x, y and the result as columns of one tensor, rows in turn, a row before or behind the others: none shares memory."""
+    import torch
+    c = Case(pkg, mixed(rows, 3, seed=rows, none=0) if rows > 1 else [0], 3, 64, 64, 16, seed=1)
+    want = c.bank.apply(c.plan, c.x, c.y, out=torch.empty_like(c.y))
+    one = torch.cat([c.x, c.y, torch.zeros_like(c.y)], 1)
+    got = c.bank.apply(c.plan, one[:, :64], one[:, 64:128], out=one[:, 128:])
+    assert torch.equal(got, want) and torch.equal(one[:, :64], c.x) and torch.equal(one[:, 64:128], c.y)
+    turns = torch.stack([c.x, c.y, torch.zeros_like(c.y)], 1).reshape(3 * rows, 64)
+    assert torch.equal(c.bank.apply(c.plan, turns[0::3], turns[1::3], out=turns[2::3]), want)
+    behind = torch.cat([c.x, c.y, torch.zeros_like(c.y)])
+    assert torch.equal(c.bank.apply(c.plan, behind[:rows], behind[rows:2 * rows], out=behind[2 * rows:]), want)
+    for bad in (lambda: c.bank.apply(c.plan, c.x, c.x), lambda: c.bank.apply(c.plan, c.x, c.y, out=c.x),
+                lambda: c.bank.apply(c.plan, one[:, :64], one[:, 64:128], out=one[:, 65:129])):
+        with pytest.raises(pkg.SamplingError):
+            bad()

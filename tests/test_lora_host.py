@@ -154,3 +154,24 @@ def test_units_fit_their_kernels(mod, seed):
     assert ((units[:, 0] < 0) == (np.repeat(np.arange(6), counts) == 4)).all()
     rows = units[:, 2].astype(np.int64)
     assert sum(rows[sum(counts[:1]):sum(counts[:5])]) == ids.size
+
+
+@pytest.mark.parametrize("x,y,out", [
+    ((P, 48), (P + 8192, 48), (P, 48)),                 # the result in x's place
+    ((P, 48), (P, 48), (P, 48)),                        # x, y and the result one
+    ((P, 48), (P + 8192, 48), (P + 8192 + 96, 48)),     # y a row further on
+    ((P, 48), (P + 8192, 48), (P + 8192 - 2, 48)),      # or an element
+    ((P, 0), (P + 8192, 0), (P + 8192 - 94, 48)),       # rows on one another, the result's first one meets them
+    ((P, 100), (P + 106, 100), (P + 106 - 10, 100)),    # columns of one wider row that meet
+    ((P + 4 * 96 + 40, 0), (P + 8192, 48), (P, 48)),    # x's only row under the result's fifth
+    ((P, 96), (P + 8192, 48), (P + 7 * 192 + 95, 50)),  # strides that differ: x's eighth row
+])
+def test_results_on_their_inputs_are_refused(mod, x, y, out):
+    lib = mod.load()
+    out = (out[0] & ~1, out[1])
+    bank = mod.LoraBankDesc(device=0, n_adapters=1, k=48, n=48, rank=8, dtype=0, a=P, b=P, a_adapter_stride=0, a_row_stride=48,
+                            b_adapter_stride=0, b_row_stride=8, ranks=None, scales=None)
+    plan = mod.LoraPlanDesc(n_rows=8, n_adapters=1, n_narrow=1, device_copy=P)
+    rows = [ctypes.byref(mod.LoraRows(ptr=p, row_stride=s, n_rows=8, dtype=0, reserved=0)) for p, s in (x, y, out)]
+    assert lib.spec_lora_apply(ctypes.byref(bank), ctypes.byref(plan), *rows, None) == 1
+    assert b"shares memory" in lib.spec_last_error(None)
