@@ -39,7 +39,8 @@
 // kernel is bound by memory (98 MB in 18 us, 5.4 TB/s), the second by its chain of
 // dependent reads and cluster barriers (5 to 20 us).  A row that needs 64 bits takes
 // 13 us more, a rejected draft's 30.  One launch for a single short chain, too, saves
-// the host 3 us and takes the device 7 longer.
+// the host 3 us and takes the device 7 longer.  Three blocks an SM of the chains' kernel leave 80
+// registers; with f32 rows 72 bytes a thread spill.
 #include "batch.h"
 #include "common.cuh"
 #include "kv4_rows.cuh"

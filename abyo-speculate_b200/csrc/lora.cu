@@ -14,7 +14,7 @@
 // its row for two instructions of 16 (its 2t, 2t + 1, 2t + 8, 2t + 9 of each):
 // x and A come by 16-byte loads from where they lie, without shared memory.
 //
-// f32 rows enter as two tf32 numbers, hi + lo, off by 2^-24.  t stays f32;
+// f32 rows enter as two tf32 numbers of 11 bits, hi + lo, off by at most 2^-23.  t stays f32;
 // for the second product it is split into three bf16 numbers (24 bits), or two f16
 // numbers of t 2^-e, 2^e about the row's largest (22 bits).  All sums are f32.
 //

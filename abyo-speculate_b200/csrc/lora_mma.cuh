@@ -115,14 +115,6 @@ SPEC_DEV uint4 first_of(const uint4& v, int n) {
   for (int i = 0; i < 4; ++i) o[i] = n >= 2 * i + 2 ? w[i] : n == 2 * i + 1 ? w[i] & 0xffffu : 0u;
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
-// 8 ranks from `k` on of a column's row of B: those at `r` and behind, which lie
-// in the row's memory up to `rank`, are zeros.
-template <class T>
-SPEC_DEV uint4 load_ranks(const T* p, int k, int r, int rank, bool wide) {
-  if (k >= r) return make_uint4(0u, 0u, 0u, 0u);
-  if (wide && k + 8 <= rank) return first_of(*reinterpret_cast<const uint4*>(p + k), r - k);
-  return load8(p, k, r, false);
-}
 SPEC_DEV void load8(const float* p, int k, int n, bool wide, float (&x)[8]) {
   if (wide && k + 8 <= n) {
     const float4 a = *reinterpret_cast<const float4*>(p + k), b = *reinterpret_cast<const float4*>(p + k + 4);
@@ -145,11 +137,6 @@ SPEC_DEV void widen(const uint4& v, float (&x)[8], const __half*) {
     x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
 }
-// 8 elements from column k on as f32, and each rounded once; those at `n` and behind are left out.
-template <class T>
-SPEC_DEV void load8(const T* p, int k, int n, bool wide, float (&x)[8]) {
-  widen(load8(p, k, n, wide), x, p);
-}
 SPEC_DEV uint32_t pack2(float lo, float hi, const __half*) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -157,28 +144,6 @@ SPEC_DEV uint32_t pack2(float lo, float hi, const __half*) {
 SPEC_DEV uint32_t pack2(float lo, float hi, const __nv_bfloat16*) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <class T>
-SPEC_DEV void store8(T* p, int k, int n, bool wide, const float (&x)[8]) {
-  const uint4 v = make_uint4(pack2(x[0], x[1], p), pack2(x[2], x[3], p), pack2(x[4], x[5], p), pack2(x[6], x[7], p));
-  if (wide && k + 8 <= n) {
-    *reinterpret_cast<uint4*>(p + k) = v;
-    return;
-  }
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (k + i < n) reinterpret_cast<uint16_t*>(p)[k + i] = (uint16_t)(w[i / 2] >> (i % 2 * 16));
-}
-SPEC_DEV void store8(float* p, int k, int n, bool wide, const float (&x)[8]) {
-  if (wide && k + 8 <= n) {
-    *reinterpret_cast<float4*>(p + k) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + k + 4) = make_float4(x[4], x[5], x[6], x[7]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (k + i < n) p[k + i] = x[i];
 }
 SPEC_DEV uint16_t bits(__half h) { return __half_as_ushort(h); }
 SPEC_DEV uint16_t bits(__nv_bfloat16 h) { return __bfloat16_as_ushort(h); }

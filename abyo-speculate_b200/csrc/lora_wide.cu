@@ -17,6 +17,9 @@
 // the operands' loads (16 bytes a lane) meet in a bank; f32 rows as two such
 // halves, 16-byte pieces in turn.
 //
+// Two blocks an SM leave 128 registers, of which 12 to 92 bytes a thread spill, and the one
+// block of f32 rows of rank above 32 255 (32 bytes).
+//
 // Bound by latency: 24 requests of 5 to 60 f32 rows (870 in all), rank 16, 4096 to
 // 14336: 48 to 56 us, 18 at the copy rate.  x A^T takes 11, its join 4, the rest moves
 // y at 4 TB/s; 64 when y and B came through the warps' rings as well.
@@ -114,7 +117,7 @@ template <class T, class TX, class TY, int NT>
 __global__ void __launch_bounds__(kThreads, blocks_an_sm<TX, NT>()) wide_kernel(const __grid_constant__ WideParams wp) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_factor[kWideRows];
-  __shared__ const void* s_row[kWideRows];  // the rows of x, then of y, from this block's first column on
+  __shared__ const void* s_row[kWideRows];  // the rows of x, from this block's first column on
   const Params& p = wp.p;
   constexpr bool kSplitX = sizeof(TX) == 4;
   constexpr int P = parts_of((const T*)nullptr);
