@@ -54,6 +54,17 @@ SPEC_DEV void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
+// Waits until at most n (up to 4) of this thread's groups of copies are under way.
+SPEC_DEV void cp_async_wait_for(int n) {
+  switch (n) {
+    case 0: cp_async_wait<0>(); break;
+    case 1: cp_async_wait<1>(); break;
+    case 2: cp_async_wait<2>(); break;
+    case 3: cp_async_wait<3>(); break;
+    default: cp_async_wait<4>(); break;
+  }
+}
+
 // Asks for `n` elements from `p` on to be brought to L2 (whole 16-byte pieces of
 // them, up to 64 KB).
 template <class E>

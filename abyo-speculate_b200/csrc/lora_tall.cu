@@ -62,15 +62,6 @@ __host__ __device__ constexpr int stage1(int N) { return kStep / 64 * (kTallRows
 SPEC_DEV uint32_t idesc(int N, const __nv_bfloat16*) { return umma_idesc_bf16(128, N); }
 SPEC_DEV uint32_t idesc(int N, const __half*) { return umma_idesc_bf16(128, N) & ~((7u << 7) | (7u << 10)); }  // formats 0: f16
 
-SPEC_DEV void cp_async_wait_for(int n) {
-  switch (n) {
-    case 0: cp_async_wait<0>(); break;
-    case 1: cp_async_wait<1>(); break;
-    case 2: cp_async_wait<2>(); break;
-    case 3: cp_async_wait<3>(); break;
-    default: cp_async_wait<4>(); break;
-  }
-}
 // 8 columns of tensor memory of this thread's row, there after tmem_wait_ld.
 SPEC_DEV void tmem_ld8(uint32_t at, uint32_t (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"

@@ -21,7 +21,7 @@
 // block of f32 rows of rank above 32 255 (32 bytes).
 //
 // Bound by latency: 24 requests of 5 to 60 f32 rows (870 in all), rank 16, 4096 to
-// 14336: 48 to 56 us, 18 at the copy rate.  x A^T takes 11, its join 4, the rest moves
+// 14336: 50 to 54 us, 18 at the copy rate.  x A^T takes about 11, its join 4, the rest moves
 // y at 4 TB/s; 64 when y and B came through the warps' rings as well.
 #include "lora_mma.cuh"
 
@@ -49,16 +49,6 @@ struct WideParams {
   int RA, ring, bytes;  // ranks' capacity (a multiple of 8 NT); bytes of a warp's ring in the first product, of shared memory
 };
 
-// Waits until at most n of this thread's groups of copies are under way.
-SPEC_DEV void cp_async_wait_for(int n) {
-  switch (n) {
-    case 0: cp_async_wait<0>(); break;
-    case 1: cp_async_wait<1>(); break;
-    case 2: cp_async_wait<2>(); break;
-    case 3: cp_async_wait<3>(); break;
-    default: cp_async_wait<4>(); break;
-  }
-}
 constexpr int kMaxSlots = 6;
 
 SPEC_DEV uint4 lds128(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
