@@ -50,6 +50,7 @@ inline bool misaligned(const void* p, size_t size) { return reinterpret_cast<uin
 inline bool rows_meet(const void* a, int64_t step_a, int64_t wide_a, const void* b, int64_t step_b, int64_t wide_b, int64_t n) {
   const int64_t pa = (int64_t)reinterpret_cast<intptr_t>(a), pb = (int64_t)reinterpret_cast<intptr_t>(b);
   if (n <= 0 || pa + (n - 1) * step_a + wide_a <= pb || pb + (n - 1) * step_b + wide_b <= pa) return false;
+  if (n == 1) return true;
   // A row of b that starts after `at - wide_b` and before `at + wide_a` meets a's row at `at`.
   auto meets = [&](int64_t at, int64_t first, int64_t last) {
     const int64_t lo = at - wide_b - pb, hi = at + wide_a - pb;  // lo < j step_b < hi

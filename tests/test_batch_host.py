@@ -102,3 +102,11 @@ def test_probabilities_on_the_logits_are_refused(lib, probs, stride):
     a = logits(dtype=2, workspace_bytes=1 << 20)
     assert lib.spec_batch_sample(ctypes.byref(a), probs, stride, 1 << 26, None) == 1
     assert b"share memory" in lib.spec_last_error(None)
+
+
+def test_one_row_of_probabilities_on_its_logits(lib):
+    """A single row's stride does not count, whatever it is."""
+    for stride in (-7, 0, 5):
+        a = logits(dtype=2, n_rows=1, workspace_bytes=1 << 20)
+        assert lib.spec_batch_sample(ctypes.byref(a), (1 << 20) + 3996, stride, 1 << 26, None) == 1
+        assert b"share memory" in lib.spec_last_error(None)
