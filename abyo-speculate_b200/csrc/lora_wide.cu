@@ -21,7 +21,7 @@
 // block of f32 rows of rank above 32 255 (32 bytes).
 //
 // Bound by latency: 24 requests of 5 to 60 f32 rows (870 in all), rank 16, 4096 to
-// 14336: 50 to 54 us, 18 at the copy rate.  x A^T takes about 11, its join 4, the rest moves
+// 14336: 50 to 55 us, 18 at the copy rate.  x A^T takes about 11, its join 4, the rest moves
 // y at 4 TB/s; 64 when y and B came through the warps' rings as well.
 #include "lora_mma.cuh"
 
