@@ -513,3 +513,59 @@ def test_probabilities_beside_the_logits(pkg):
         assert (np.abs(q.cpu().numpy().astype(np.float64) - p) <= 2.0 ** -17 * p + 2.0 ** -120).all()
         with pytest.raises(pkg.SamplingError):
             pkg.sample_rows(logits, dev(u, np.float32), probs_out=logits)
+
+
+@pytest.mark.parametrize("m", [512, 513, 700])
+def test_trees_of_very_many_nodes(pkg, m):
+    """Nodes behind the first 512: a path through all of them, one that ends behind them, and a bush whose child is its last."""
+    x, host, t, tokens, parents, start = trees([m, m, m], 900, "f16", seed=m, spread=0.3, hot=2)
+    _, u = uniforms(3 * m, 2)
+    t[:] = np.where(np.arange(3 * m) % 7 == 0, 1.0, 0.0)
+    drawn = [ref.token(ref.probs(host[i], t[i]), u[i]) for i in range(3 * m)]
+    for b, length in ((0, m), (1, m - 20)):
+        parents[b * m + 1:(b + 1) * m] = np.arange(m - 1)
+        tokens[b * m + 1:b * m + length] = drawn[b * m:b * m + length - 1]
+        tokens[b * m + length:(b + 1) * m] = -1
+    parents[2 * m:] = 0
+    tokens[2 * m:] = (drawn[2 * m] + 1) % 900
+    tokens[3 * m - 1] = drawn[2 * m]
+    assert check_tree(pkg, x, host, t, tokens, parents, u, start) == [m, m - 20, 2]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_largest_vocabulary(pkg, dtype):
+    import torch
+    v = 1 << 20
+    x, host = rows(6, v, dtype, seed=7, spread=1.0)
+    _, u = uniforms(6, 3)
+    u[1], u[2] = 1.0, 0.0
+    t = np.array([1.0, 1.0, 1.0, 0.0, 0.4, 2.0], np.float32)
+    check_sample(pkg, x, host, u, t)
+    with pytest.raises(pkg.SamplingError):
+        pkg.sample_rows(torch.zeros(1, v + 1, device="cuda"), dev(u[:1], np.float32))
+    q = np.stack([ref.probs(h, 1.0) for h in host * 0.9]).astype(np.float32)
+    drafts = np.array([int(np.argmax(h)) for h in host], np.int32)
+    check_chain(pkg, x, host, t, q, drafts, u, np.array([0, 3, 6], np.int32))
+    check_tree(pkg, x, host, t, np.array([0, drafts[0], 5, 0, drafts[3], 1], np.int32), np.array([0, 0, 0, 0, 0, 1], np.int32), u,
+               np.array([0, 3, 6], np.int32))
+
+
+def test_the_most_rows(pkg):
+    """2^20 rows, and as many sequences."""
+    import torch
+    n = 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    best = torch.randint(0, 3, (n,), device="cuda", generator=gen)
+    x = torch.zeros(n, 3, device="cuda").scatter_(1, best[:, None], 60.0)
+    u = torch.rand(n, device="cuda", generator=gen)
+    want = best.to(torch.int32)
+    q = torch.empty(n, 3, device="cuda")
+    assert torch.equal(pkg.sample_rows(x, u, probs_out=q), want) and (q.argmax(1) == best).all()
+    start = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    zeros = torch.zeros(n, dtype=torch.int32, device="cuda")
+    count, token = pkg.verify_drafts(x, zeros, q, u, start)
+    assert not count.any() and torch.equal(token, want)
+    path, count, token = pkg.verify_trees(x, zeros, zeros, u, start)
+    assert not path.any() and (count == 1).all() and torch.equal(token, want)
+    with pytest.raises(pkg.SamplingError):
+        pkg.sample_rows(torch.zeros(n + 1, 3, device="cuda"), torch.zeros(n + 1, device="cuda"))

@@ -528,3 +528,19 @@ def test_rows_beside_each_other(pkg, rows):
                 lambda: c.bank.apply(c.plan, one[:, :64], one[:, 64:128], out=one[:, 65:129])):
         with pytest.raises(pkg.SamplingError):
             bad()
+
+
+@pytest.mark.parametrize("x", ["same", "f32"])
+def test_the_most_rows(pkg, x):
+    """2^20 rows: of one adapter, and most without one."""
+    n = 1 << 20
+    Case(pkg, np.zeros(n, np.int32), 1, 24, 16, 5, "bf16", x, x, seed=1).check()
+    ids = np.full(n, -1)
+    ids[::4001], ids[-1] = 1, 0
+    Case(pkg, ids, 2, 24, 16, 5, "bf16", x, x, seed=2).check()
+    with pytest.raises(pkg.SamplingError):
+        pkg.LoraPlan(np.zeros(n + 1, np.int32), 1)
+
+
+def test_very_many_adapters(pkg):
+    Case(pkg, np.random.default_rng(0).permutation(20000), 20000, 40, 32, 8, seed=3).check()
